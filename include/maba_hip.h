@@ -67,6 +67,12 @@
  *                                   its input from RMSNorm, the gated residual +
  *                                   RMSNorm or SwiGLU (model.py:11-38, 92-128) in the
  *                                   same launch
+ *   maba_hip_gated_ffn              model.py:25-38 (SwiGLU's two projections, activation and
+ *                                   product; its gradients come from autograd there)
+ *   maba_hip_linear_epilogue        nn.Linear with what follows it: the bias, an activation,
+ *                                   the gated residual of model.py:92-128
+ *   maba_hip_checkpoint_pack        no counterpart: the input that those two keep for their
+ *                                   backward passes, in 8 bits
  */
 #ifndef MABA_HIP_H
 #define MABA_HIP_H
@@ -84,7 +90,9 @@ enum maba_dtype {
   MABA_BF16 = 2,
   MABA_F64 = 3,
   MABA_I64 = 4,
-  MABA_I32 = 5
+  MABA_I32 = 5,
+  MABA_E4M3 = 6,   /* 8-bit float codes of a packed activation (OCP e4m3fn) */
+  MABA_U8 = 7      /* their groups' scale bytes: exponent + 127 */
 };
 
 enum maba_status {
@@ -392,6 +400,58 @@ int maba_hip_decode_linear(const maba_tensor* a, const maba_tensor* rows, const 
  * column stride, 16-byte aligned rows, V a multiple of 8 (bf16) or 4 (f32)), as torch.argmax:
  * NaN counts as the maximum and -0 equals +0.  out int64 [M] or [M,1]. */
 int maba_hip_argmax_rows(const maba_tensor* x, maba_tensor* out, void* stream);
+
+/*
+ * The gated feed-forward block up to its down projection, h = silu(x Wg^T) * (x Wu^T), and its
+ * gradients.  x [M,C], w_gate, w_up [I,C], out [M,I]: one 16-bit dtype (f16 or bf16), unit column
+ * stride, any row stride and alignment; fp32 accumulation, one rounding.  Rows that are not 16-byte
+ * aligned chunks of eight elements are first copied into the workspace (except at M <= 32, the decode
+ * kernel); where every tensor is aligned the forward needs none (the query returns 0).
+ *
+ * Backward: dh [M,I]; x as above, or with x_scales its packed form (x: MABA_E4M3 codes [M,C], x_scales:
+ * MABA_U8 [M,ceil(C/32)]); any of dx [M,C], dw_gate, dw_up [I,C] may be NULL.  g and u are made again from
+ * x; [dg | du] is rounded to 16 bits once, as an operand of the next products.  Results are the same bits
+ * on every call.  The query depends on the current device's compute-unit count; with_dw says whether
+ * either weight gradient is wanted.
+ */
+size_t maba_hip_gated_ffn_workspace_size(const maba_tensor* x, const maba_tensor* w_gate, const maba_tensor* w_up);
+int maba_hip_gated_ffn(const maba_tensor* x, const maba_tensor* w_gate, const maba_tensor* w_up, maba_tensor* out,
+                       void* workspace, size_t workspace_bytes, void* stream);
+size_t maba_hip_gated_ffn_backward_workspace_size(const maba_tensor* x, const maba_tensor* x_scales,
+                                                  const maba_tensor* w_gate, const maba_tensor* w_up, int with_dw);
+int maba_hip_gated_ffn_backward(const maba_tensor* dh, const maba_tensor* x, const maba_tensor* x_scales,
+                                const maba_tensor* w_gate, const maba_tensor* w_up, maba_tensor* dx, maba_tensor* dw_gate,
+                                maba_tensor* dw_up, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * y = residual + gate * act(x W^T + bias) and its gradients.  x [M,K], weight [N,K], bias, gate [N],
+ * residual, out [M,N]: one 16-bit dtype, unit column stride; bias, gate and residual may be NULL; act 0
+ * none, 1 relu, 2 silu, 3 gelu (with the error function).  out may be residual itself.  Copies and the
+ * workspace as for maba_hip_gated_ffn.
+ *
+ * Backward: dy [M,N]; x as above or packed, with x_scales; any of dx [M,K], dw [N,K], dbias, dgate [N] may be
+ * NULL (the residual's gradient is dy).  needs: 1 dx, 2 dw, 4 dbias, 8 dgate.
+ */
+size_t maba_hip_linear_epilogue_workspace_size(const maba_tensor* x, const maba_tensor* weight);
+int maba_hip_linear_epilogue(const maba_tensor* x, const maba_tensor* weight, const maba_tensor* bias, int act,
+                             const maba_tensor* residual, const maba_tensor* gate, maba_tensor* out, void* workspace,
+                             size_t workspace_bytes, void* stream);
+size_t maba_hip_linear_epilogue_backward_workspace_size(const maba_tensor* dy, const maba_tensor* x,
+                                                        const maba_tensor* x_scales, const maba_tensor* weight, int act,
+                                                        int with_gate, int needs);
+int maba_hip_linear_epilogue_backward(const maba_tensor* dy, const maba_tensor* x, const maba_tensor* x_scales,
+                                      const maba_tensor* weight, const maba_tensor* bias, int act, const maba_tensor* gate,
+                                      maba_tensor* dx, maba_tensor* dw, maba_tensor* dbias, maba_tensor* dgate,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Activation checkpoints in 8 bits.  x, out [M,C] f32, f16 or bf16; codes [M,C] MABA_E4M3; scales
+ * [M,ceil(C/32)] MABA_U8.  Every 32 elements of a row share 2^e, the smallest power of two (e >= -127) with
+ * max|x| <= 448 * 2^e over the finite ones; scale = e + 127, code = x / 2^e rounded to nearest even.  NaN and
+ * infinities become e4m3's NaN.  Unpacked values are code * 2^e rounded to out's type.
+ */
+int maba_hip_checkpoint_pack(const maba_tensor* x, maba_tensor* codes, maba_tensor* scales, void* stream);
+int maba_hip_checkpoint_unpack(const maba_tensor* codes, const maba_tensor* scales, maba_tensor* out, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,147 @@
+// What the gated block and the linear layer share around the matrix-product core: launches with
+// their tile, operand copies where the core cannot read a tensor in place, and reductions.
+#pragma once
+
+#include "ffn_gemm.h"
+
+namespace maba {
+namespace ffn {
+
+// ---------------------------------------------------------------- copies and reductions (ffn_common.hip)
+
+// dst [rows, pad8(cols)] (contiguous) = src [rows, cols] with zeros behind each row, of 16-bit elements at any
+// alignment.  With scales: src holds the e4m3 codes of a packed activation, dst its values in `dtype`.
+int copy_rows(const maba_tensor* src, const maba_tensor* scales, int dtype, uint16_t* dst, hipStream_t s);
+
+// out = the sum of `splits` fp32 partials [splits][M][N] in split order, rounded to 16 bits; row m goes to
+// row m of out[0], or from `second` on to row m - second of out[1]; only `rows` rows of each are written, and
+// nothing to a null one.
+struct ReduceArgs {
+  const float* p;
+  int splits, M, N, second, rows, ncols;
+  Rows out[2];
+};
+int reduce_splits(const ReduceArgs& a, int dtype, hipStream_t s);
+
+// out[t][n] = the sum over r of p[r][t][n] (fp32 partials [R][2][N], t = 0, 1; a null out is skipped), 16 bits.
+int reduce_columns(const float* p, int64_t R, int N, void* out0, void* out1, int dtype, hipStream_t s);
+
+// p[r][0][n] = the sum of rows [128 r, 128 r + 128) of src [M, N] (16-bit), [ceil(M / 128)][2][N].
+int column_partials(const maba_tensor* src, float* p, hipStream_t s);
+
+// ---------------------------------------------------------------- launches
+
+constexpr int GEMM_BM = 128, GEMM_BN = 128, GEMM_BK = 64, GEMM_ST = 2;
+
+template <class T, int AMODE, int BMODE, class Epi>
+int gemm(GemmArgs g, const typename Epi::Args& e, int64_t M, int64_t N, int splits, hipStream_t s, const char* who) {
+  g.tiles_m = (int)ceil_div(M, GEMM_BM);
+  g.tiles_n = (int)ceil_div(N, GEMM_BN);
+  g.splits = splits;
+  g.k_split = ceil_div(ceil_div(g.K, splits), GEMM_BK) * GEMM_BK;
+  const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * splits;
+  if (grid > INT32_MAX) return fail(MABA_ERR_UNSUPPORTED, "%s: too many tiles", who);
+  hipLaunchKernelGGL((gemm_kernel<T, GEMM_BM, GEMM_BN, 2, 2, GEMM_BK, GEMM_ST, AMODE, BMODE, Epi>), dim3((unsigned)grid),
+                     dim3(256), 0, s, g, e);
+  return check_launch(who);
+}
+
+// Splits of a sum over K tokens whose output has M x N elements: enough workgroups for two per
+// compute unit, at least 512 tokens each, and none of them empty.
+inline int k_splits(int64_t M, int64_t N, int64_t K) {
+  const int64_t tiles = ceil_div(M, GEMM_BM) * ceil_div(N, GEMM_BN);
+  int64_t s = std::max<int64_t>(1, std::min<int64_t>(2 * device_cu_count() / std::max<int64_t>(tiles, 1), K / 512));
+  s = std::max<int64_t>(s, 1);
+  const int64_t each = ceil_div(ceil_div(std::max<int64_t>(K, 1), s), GEMM_BK) * GEMM_BK;
+  return (int)ceil_div(std::max<int64_t>(K, 1), each);
+}
+
+// ---------------------------------------------------------------- argument checks
+
+// A 2-D 16-bit tensor [rows, cols] (-1: any) with unit column stride.
+inline int check_rows(const maba_tensor* t, const char* who, const char* name, int dtype, int64_t rows, int64_t cols) {
+  if (!t) return fail(MABA_ERR_INVALID, "%s: %s is missing", who, name);
+  if (t->ndim != 2) return fail(MABA_ERR_INVALID, "%s: %s must be 2D, got %dD", who, name, t->ndim);
+  if ((rows >= 0 && t->shape[0] != rows) || (cols >= 0 && t->shape[1] != cols))
+    return fail(MABA_ERR_INVALID, "%s: %s is [%lld, %lld], expected [%lld, %lld]", who, name, (long long)t->shape[0],
+                (long long)t->shape[1], (long long)rows, (long long)cols);
+  if (t->dtype != dtype) return fail(MABA_ERR_DTYPE, "%s: %s has dtype code %d, expected %d", who, name, t->dtype, dtype);
+  if (t->shape[1] > 1 && t->stride[1] != 1) return fail(MABA_ERR_INVALID, "%s: %s needs unit column stride", who, name);
+  if (t->stride[0] < 0) return fail(MABA_ERR_INVALID, "%s: %s has a negative stride", who, name);
+  if (t->shape[0] > 0 && t->shape[1] > 0 && !t->data) return fail(MABA_ERR_INVALID, "%s: %s has no data", who, name);
+  return MABA_OK;
+}
+// An output: like check_rows, and its rows must not overlap one another.
+inline int check_out(const maba_tensor* t, const char* who, const char* name, int dtype, int64_t rows, int64_t cols) {
+  const int rc = check_rows(t, who, name, dtype, rows, cols);
+  if (rc) return rc;
+  if (t->shape[0] > 1 && t->stride[0] < t->shape[1]) return fail(MABA_ERR_INVALID, "%s: rows of %s overlap", who, name);
+  return MABA_OK;
+}
+inline int check_vec(const maba_tensor* t, const char* who, const char* name, int dtype, int64_t n) {
+  if (t->ndim != 1 || t->shape[0] != n) return fail(MABA_ERR_INVALID, "%s: %s must be [%lld]", who, name, (long long)n);
+  if (t->dtype != dtype) return fail(MABA_ERR_DTYPE, "%s: %s has dtype code %d, expected %d", who, name, t->dtype, dtype);
+  if (n > 1 && t->stride[0] != 1) return fail(MABA_ERR_INVALID, "%s: %s needs unit stride", who, name);
+  if (!t->data) return fail(MABA_ERR_INVALID, "%s: %s has no data", who, name);
+  return MABA_OK;
+}
+// Widths and row counts the kernels index with 32 bits.
+inline int check_sizes(const char* who, int64_t M, int64_t N, int64_t K) {
+  if (N < 1 || K < 1) return fail(MABA_ERR_INVALID, "%s: widths must be positive, got %lld and %lld", who, (long long)N, (long long)K);
+  if (M > (1 << 30) || N > (1 << 20) || K > (1 << 20)) return fail(MABA_ERR_UNSUPPORTED, "%s: sizes out of range", who);
+  return MABA_OK;
+}
+// The bytes that a tensor's elements span, as [first, last); and whether two spans meet.
+inline bool overlap(const maba_tensor* a, const maba_tensor* b) {
+  if (!a || !b) return false;
+  auto span = [](const maba_tensor* t, uintptr_t& lo, uintptr_t& hi) {
+    const int64_t size = t->dtype == MABA_F32 ? 4 : t->dtype == MABA_E4M3 || t->dtype == MABA_U8 ? 1 : 2;
+    int64_t last = 0;
+    for (int i = 0; i < t->ndim; ++i) {
+      if (t->shape[i] == 0) return false;
+      last += (t->shape[i] - 1) * t->stride[i];
+    }
+    lo = (uintptr_t)t->data;
+    hi = lo + (uintptr_t)((last + 1) * size);
+    return true;
+  };
+  uintptr_t al, ah, bl, bh;
+  return span(a, al, ah) && span(b, bl, bh) && al < bh && bl < ah;
+}
+
+// x of a backward pass: 16-bit rows, or the codes of a packed activation and their scales.
+inline int check_kept(const maba_tensor* x, const maba_tensor* scales, const char* who, int dtype, int64_t M, int64_t K) {
+  if (!scales) return check_rows(x, who, "x", dtype, M, K);
+  int rc = check_rows(x, who, "the codes of x", MABA_E4M3, M, K);
+  if (!rc) rc = check_rows(scales, who, "the scales of x", MABA_U8, M, ceil_div(K, 32));
+  return rc;
+}
+
+// A workspace handed out front to back in 256-byte steps.
+struct Carve {
+  char* p;
+  size_t used;
+  template <class U>
+  U* take(size_t n) {
+    U* r = (U*)(p ? p + used : nullptr);
+    used += up256(n * sizeof(U));
+    return r;
+  }
+};
+
+// p [rows][..] read along its rows; and the same [krows][cols] read along its columns.
+inline Operand rows_operand(const uint16_t* p, int64_t ld, int64_t rows) {
+  Operand o = {};
+  o.p[0] = o.p[1] = p;
+  o.ld[0] = o.ld[1] = ld;
+  o.rows = (int)rows;
+  return o;
+}
+inline Operand cols_operand(Operand o, int64_t cols) {
+  o.krows = o.rows;
+  o.rows = (int)cols;
+  return o;
+}
+
+}  // namespace ffn
+}  // namespace maba

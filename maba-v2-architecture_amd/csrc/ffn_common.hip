@@ -1,0 +1,140 @@
+// Copies and reductions of the feed-forward operators.
+#include <algorithm>
+
+#include "ffn_common.h"
+
+namespace maba {
+namespace ffn {
+
+// A thread makes eight elements of a padded row.  Elements are read one by one: this kernel serves the
+// tensors whose rows are not 16-byte aligned; it is bound by its launch or by HBM.
+__global__ __launch_bounds__(256) void copy_rows_kernel(const uint16_t* src, int64_t ld, int64_t rows, int cols, int chunks,
+                                                        uint16_t* dst) {
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < rows * chunks; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / chunks;
+    const int k = (int)(i % chunks) * 8;
+    const uint16_t* p = src + r * ld + k;
+    u32x4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t lo = k + 2 * j < cols ? p[2 * j] : 0, hi = k + 2 * j + 1 < cols ? p[2 * j + 1] : 0;
+      v[j] = lo | (hi << 16);
+    }
+    *(u32x4*)(dst + i * 8) = v;
+  }
+}
+
+// The same from e4m3 codes and their groups' exponents: code * 2^(scale - 127), exact in fp32, rounded once to
+// T (a bf16 holds it exactly unless it is subnormal there).
+template <class T>
+__global__ __launch_bounds__(256) void unpack_rows_kernel(const uint8_t* src, int64_t ld, const uint8_t* sc, int64_t lds_,
+                                                          int64_t rows, int cols, int chunks, int vec, uint16_t* dst) {
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < rows * chunks; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / chunks;
+    const int k = (int)(i % chunks) * 8;
+    const uint8_t* p = src + r * ld + k;
+    const int e = (int)sc[r * lds_ + (k >> 5)] - 127;
+    u32x2 w = {0, 0};
+    if (vec) w = *(const u32x2*)p;
+    else
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j >> 2] |= (k + j < cols ? (uint32_t)p[j] : 0u) << (8 * (j & 3));
+    u32x4 v;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], true);
+      v[2 * h] = T::down(__builtin_amdgcn_ldexpf(a[0], e)) | (T::down(__builtin_amdgcn_ldexpf(a[1], e)) << 16);
+      v[2 * h + 1] = T::down(__builtin_amdgcn_ldexpf(b[0], e)) | (T::down(__builtin_amdgcn_ldexpf(b[1], e)) << 16);
+    }
+    *(u32x4*)(dst + i * 8) = v;
+  }
+}
+
+int copy_rows(const maba_tensor* src, const maba_tensor* scales, int dtype, uint16_t* dst, hipStream_t s) {
+  const int64_t rows = src->shape[0], cols = src->shape[1], chunks = pad8(cols) / 8;
+  if (rows == 0) return MABA_OK;
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows * chunks, 256), 16384));
+  if (!scales) {
+    hipLaunchKernelGGL(copy_rows_kernel, grid, dim3(256), 0, s, (const uint16_t*)src->data, src->stride[0], rows, (int)cols,
+                       (int)chunks, dst);
+  } else {
+    const int vec = cols % 8 == 0 && src->stride[0] % 8 == 0 && (uintptr_t)src->data % 8 == 0;
+    auto k = dtype == MABA_BF16 ? unpack_rows_kernel<Bf16> : unpack_rows_kernel<Fp16>;
+    hipLaunchKernelGGL(k, grid, dim3(256), 0, s, (const uint8_t*)src->data, src->stride[0], (const uint8_t*)scales->data,
+                       scales->stride[0], rows, (int)cols, (int)chunks, vec, dst);
+  }
+  return check_launch("copy_rows");
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void reduce_splits_kernel(ReduceArgs a) {
+  const int quads = a.N / 4;
+  const int64_t total = (int64_t)a.M * quads, plane = (int64_t)a.M * a.N;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int m = (int)(i / quads), n = (int)(i % quads) * 4;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; ++s) v += *(const f32x4*)(a.p + s * plane + (int64_t)m * a.N + n);
+    const int t = m >= a.second, r = t ? m - a.second : m;
+    if (r < a.rows && a.out[t].p) store4<T>(a.out[t], r, n, a.ncols, v);
+  }
+}
+
+int reduce_splits(const ReduceArgs& a, int dtype, hipStream_t s) {
+  const int64_t total = (int64_t)a.M * (a.N / 4);
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(total, 256), 16384));
+  auto k = dtype == MABA_BF16 ? reduce_splits_kernel<Bf16> : reduce_splits_kernel<Fp16>;
+  hipLaunchKernelGGL(k, grid, dim3(256), 0, s, a);
+  return check_launch("reduce_splits");
+}
+
+// 32 columns of one output a workgroup, eight threads each, added through LDS in a fixed order.
+template <class T>
+__global__ __launch_bounds__(256) void reduce_columns_kernel(const float* p, int64_t R, int N, uint16_t* out0, uint16_t* out1) {
+  __shared__ float part[8][32];
+  uint16_t* out = blockIdx.y ? out1 : out0;
+  if (!out) return;
+  const int col = threadIdx.x & 31, lane = threadIdx.x >> 5, n = blockIdx.x * 32 + col;
+  float v = 0.f;
+  if (n < N)
+    for (int64_t r = lane; r < R; r += 8) v += p[(r * 2 + blockIdx.y) * N + n];
+  part[lane][col] = v;
+  __syncthreads();
+  if (lane == 0 && n < N) {
+    float w = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w += part[i][col];
+    out[n] = (uint16_t)T::down(w);
+  }
+}
+
+int reduce_columns(const float* p, int64_t R, int N, void* out0, void* out1, int dtype, hipStream_t s) {
+  auto k = dtype == MABA_BF16 ? reduce_columns_kernel<Bf16> : reduce_columns_kernel<Fp16>;
+  hipLaunchKernelGGL(k, dim3((unsigned)ceil_div(N, 32), 2), dim3(256), 0, s, p, R, N, (uint16_t*)out0, (uint16_t*)out1);
+  return check_launch("reduce_columns");
+}
+
+// A wave adds 64 columns of 32 rows, a workgroup of four its 128 rows through LDS.
+template <class T>
+__global__ __launch_bounds__(256) void column_partials_kernel(const uint16_t* src, int64_t ld, int64_t M, int N, float* p) {
+  __shared__ float part[4][64];
+  const int col = threadIdx.x & 63, w = threadIdx.x >> 6, n = blockIdx.y * 64 + col;
+  float v = 0.f;
+  if (n < N) {
+    const int64_t r0 = blockIdx.x * (int64_t)128 + w * 32, r1 = min(r0 + 32, M);
+    for (int64_t r = r0; r < r1; ++r) v += T::up(src[r * ld + n]);
+  }
+  part[w][col] = v;
+  __syncthreads();
+  if (w == 0 && n < N) p[blockIdx.x * (int64_t)2 * N + n] = part[0][col] + part[1][col] + part[2][col] + part[3][col];
+}
+
+int column_partials(const maba_tensor* src, float* p, hipStream_t s) {
+  const int64_t M = src->shape[0], N = src->shape[1];
+  auto k = src->dtype == MABA_BF16 ? column_partials_kernel<Bf16> : column_partials_kernel<Fp16>;
+  hipLaunchKernelGGL(k, dim3((unsigned)ceil_div(M, 128), (unsigned)ceil_div(N, 64)), dim3(256), 0, s,
+                     (const uint16_t*)src->data, src->stride[0], M, (int)N, p);
+  return check_launch("column_partials");
+}
+
+}  // namespace ffn
+}  // namespace maba

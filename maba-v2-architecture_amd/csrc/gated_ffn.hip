@@ -1,0 +1,261 @@
+// The gated feed-forward block up to its down projection, and its backward pass:
+//
+//   g = x Wg^T, u = x Wu^T, h = silu(g) u                               x [M, C], Wg, Wu [I, C], h [M, I]
+//   dg = dh u s (1 + g (1 - s)), du = dh g s, s = 1 / (1 + exp(-g))
+//   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x
+//
+// Forward: one product whose column tiles interleave 16 rows of Wg with 16 of Wu, so that a lane holds g and
+// u of the same elements and only h is written.
+//
+// Backward: the forward keeps nothing but x.  The first launch makes g and u again (4 M C I operations, which
+// cost about what writing and reading the two would at C <= 1000 or so) and its epilogue turns them with dh
+// into [dg | du], rounded once to 16 bits as an operand of the next products: kept in fp32 to here, so the
+// gradients carry that one rounding and their own.  The second launch is dx over k = [dg | du]'s columns with
+// both weights read along their columns, the third [dWg; dWu] = [dg | du]^T x, summed over token ranges into
+// fp32 partials that a last launch adds in order (the same bits every time).
+#include <algorithm>
+
+#include "ffn_common.h"
+#include "ffn_skinny.h"
+
+namespace maba {
+namespace ffn {
+
+struct EpiGated {
+  struct Args { Rows h; int M, I; };
+  template <class T>
+  static __device__ __forceinline__ void quad(const Args& e, int64_t m, int n, f32x4 g, f32x4 u) {
+    f32x4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = g[r] * sigmoid(g[r]) * u[r];
+    store4<T>(e.h, m, n, e.I, v);
+  }
+  template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
+  static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
+                                             int q, int wave, uint16_t* lds) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int m = m0 + 16 * i + c;
+#pragma unroll
+      for (int j = 0; j < NI; j += 2) {
+        const int n = n0 / 2 + 8 * j + 4 * q;
+        if (m < e.M && n < e.I) quad<T>(e, m, n, acc[i][j], acc[i][j + 1]);
+      }
+    }
+  }
+};
+
+// d [M, 2 Ip], Ip = I rounded up to 8: dg at column 0, du at column Ip, zeros behind each.
+struct EpiGatedBack {
+  struct Args { Rows dh, d; int M, I, Ip; };
+  template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
+  static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
+                                             int q, int wave, uint16_t* lds) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int m = m0 + 16 * i + c;
+#pragma unroll
+      for (int j = 0; j < NI; j += 2) {
+        const int n = n0 / 2 + 8 * j + 4 * q;
+        if (m >= e.M || n >= e.Ip) continue;
+        const f32x4 g = acc[i][j], u = acc[i][j + 1], dh = load4<T>(e.dh, m, n, e.I);
+        f32x4 dg, du;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float s = sigmoid(g[r]), a = dh[r] * s;
+          du[r] = a * g[r];
+          dg[r] = a * u[r] * (1.f + g[r] * (1.f - s));
+        }
+        store4<T>(e.d, m, n, e.Ip, dg);
+        store4<T>(e.d, m, e.Ip + n, 2 * e.Ip, du);
+      }
+    }
+  }
+};
+
+// Where everything of a call lies: operands in place or copied into the workspace.
+struct GatedPlan {
+  int64_t M, C, I, Cp, Ip;
+  bool copy_x, copy_w[2];
+  uint16_t *x, *w[2], *d;
+  float* part;
+  int splits;
+  size_t bytes;
+};
+
+static GatedPlan gated_plan(const maba_tensor* x, const maba_tensor* scales, const maba_tensor* wg, const maba_tensor* wu,
+                            bool back, bool dw, void* ws) {
+  GatedPlan p = {};
+  p.M = x->shape[0];
+  p.C = x->shape[1];
+  p.I = wg->shape[0];
+  p.Cp = pad8(p.C);
+  p.Ip = pad8(p.I);
+  const bool few = !back && p.M <= SKINNY_ROWS;       // that kernel reads any rows
+  p.copy_x = !few && (scales || !aligned_rows(x));
+  p.copy_w[0] = !few && !aligned_rows(wg);
+  p.copy_w[1] = !few && !aligned_rows(wu);
+  Carve c = {(char*)ws, 0};
+  if (p.copy_x) p.x = c.take<uint16_t>(p.M * p.Cp);
+  for (int i = 0; i < 2; ++i)
+    if (p.copy_w[i]) p.w[i] = c.take<uint16_t>(p.I * p.Cp);
+  if (back) {
+    p.d = c.take<uint16_t>(p.M * 2 * p.Ip);
+    if (dw) {
+      p.splits = k_splits(2 * p.Ip, p.Cp, p.M);
+      p.part = c.take<float>((int64_t)p.splits * 2 * p.Ip * p.Cp);
+    }
+  }
+  p.bytes = c.used;
+  return p;
+}
+
+// The operands of x W^T with both weights, after any copies.
+static int gated_operands(GatedPlan& p, const maba_tensor* x, const maba_tensor* scales, const maba_tensor* wg,
+                          const maba_tensor* wu, hipStream_t s, Operand& ox, Operand& ow) {
+  const maba_tensor* w[2] = {wg, wu};
+  if (p.copy_x)
+    if (int rc = copy_rows(x, scales, wg->dtype, p.x, s)) return rc;
+  ox = p.copy_x ? rows_operand(p.x, p.Cp, p.M) : rows_operand((const uint16_t*)x->data, x->stride[0], p.M);
+  ow = {};
+  ow.rows = (int)p.I;
+  for (int i = 0; i < 2; ++i) {
+    if (p.copy_w[i])
+      if (int rc = copy_rows(w[i], nullptr, wg->dtype, p.w[i], s)) return rc;
+    ow.p[i] = p.copy_w[i] ? p.w[i] : (const uint16_t*)w[i]->data;
+    ow.ld[i] = p.copy_w[i] ? p.Cp : w[i]->stride[0];
+  }
+  return MABA_OK;
+}
+
+template <class T>
+static int gated_forward(GatedPlan& p, const maba_tensor* x, const maba_tensor* wg, const maba_tensor* wu, maba_tensor* out,
+                         hipStream_t s, const char* who) {
+  const EpiGated::Args e = {rows_of(out), (int)p.M, (int)p.I};
+  if (p.M <= SKINNY_ROWS) {
+    SkinnyArgs a = {(const uint16_t*)x->data, x->stride[0], {(const uint16_t*)wg->data, (const uint16_t*)wu->data},
+                    {wg->stride[0], wu->stride[0]}, (int)p.M, (int)p.I, (int)p.C, aligned_rows(x),
+                    aligned_rows(wg) && aligned_rows(wu)};
+    return skinny<T, true, EpiGated>(a, e, s, who);
+  }
+  GemmArgs g = {};
+  if (int rc = gated_operands(p, x, nullptr, wg, wu, s, g.a, g.b)) return rc;
+  g.K = p.Cp;
+  return gemm<T, K_ROWS, K_ROWS_PAIR, EpiGated>(g, e, p.M, 2 * ceil_div(p.I, 16) * 16, 1, s, who);
+}
+
+template <class T>
+static int gated_backward(GatedPlan& p, const maba_tensor* dh, const maba_tensor* x, const maba_tensor* scales,
+                          const maba_tensor* wg, const maba_tensor* wu, maba_tensor* dx, maba_tensor* dwg, maba_tensor* dwu,
+                          hipStream_t s, const char* who) {
+  Operand ox, ow;
+  if (int rc = gated_operands(p, x, scales, wg, wu, s, ox, ow)) return rc;
+  const Operand d = rows_operand(p.d, 2 * p.Ip, p.M);
+  if (p.M > 0) {
+    GemmArgs g = {};
+    g.a = ox;
+    g.b = ow;
+    g.K = p.Cp;
+    const Rows rd = {p.d, 2 * p.Ip, 1};
+    const EpiGatedBack::Args e = {rows_of(dh), rd, (int)p.M, (int)p.I, (int)p.Ip};
+    if (int rc = gemm<T, K_ROWS, K_ROWS_PAIR, EpiGatedBack>(g, e, p.M, 2 * ceil_div(p.I, 16) * 16, 1, s, who)) return rc;
+  }
+  if (dx && p.M > 0) {
+    GemmArgs g = {};
+    g.a = d;
+    g.b = cols_operand(ow, p.Cp);
+    g.b.ksplit = (int)p.Ip;
+    g.K = 2 * p.Ip;
+    const EpiStore::Args e = {rows_of(dx), (int)p.M, (int)p.C};
+    if (int rc = gemm<T, K_ROWS, K_COLS_PAIR, EpiStore>(g, e, p.M, p.C, 1, s, who)) return rc;
+  }
+  if (dwg || dwu) {
+    if (p.M > 0) {
+      GemmArgs g = {};
+      g.a = cols_operand(d, 2 * p.Ip);
+      g.b = cols_operand(ox, p.Cp);
+      g.K = p.M;
+      const EpiPartial::Args e = {p.part, (int)(2 * p.Ip), (int)p.Cp};
+      if (int rc = gemm<T, K_COLS, K_COLS, EpiPartial>(g, e, 2 * p.Ip, p.Cp, p.splits, s, who)) return rc;
+    }
+    ReduceArgs r = {p.part, p.M > 0 ? p.splits : 0, (int)(2 * p.Ip), (int)p.Cp, (int)p.Ip, (int)p.I, (int)p.C, {}};
+    r.out[0] = rows_of(dwg);
+    r.out[1] = rows_of(dwu);
+    if (int rc = reduce_splits(r, wg->dtype, s)) return rc;
+  }
+  return MABA_OK;
+}
+
+static int gated_check(const maba_tensor* x, const maba_tensor* scales, const maba_tensor* wg, const maba_tensor* wu,
+                       const char* who) {
+  if (!x || !wg || !wu) return fail(MABA_ERR_INVALID, "%s: x, w_gate and w_up required", who);
+  if (wg->dtype != MABA_BF16 && wg->dtype != MABA_F16)
+    return fail(wg->dtype == MABA_F32 ? MABA_ERR_UNSUPPORTED : MABA_ERR_DTYPE, "%s: 16-bit weights only, got dtype code %d", who, wg->dtype);
+  if (x->ndim != 2 || wg->ndim != 2) return fail(MABA_ERR_INVALID, "%s: x and the weights must be 2D", who);
+  int rc = check_sizes(who, x->shape[0], wg->shape[0], x->shape[1]);
+  if (!rc) rc = check_kept(x, scales, who, wg->dtype, -1, x->shape[1]);
+  if (!rc) rc = check_rows(wg, who, "w_gate", wg->dtype, -1, x->shape[1]);
+  if (!rc) rc = check_rows(wu, who, "w_up", wg->dtype, wg->shape[0], x->shape[1]);
+  if (!rc && scales && scales->shape[0] != x->shape[0]) rc = fail(MABA_ERR_INVALID, "%s: scales do not match the codes", who);
+  return rc;
+}
+
+}  // namespace ffn
+}  // namespace maba
+
+using namespace maba;
+using namespace maba::ffn;
+
+extern "C" size_t maba_hip_gated_ffn_workspace_size(const maba_tensor* x, const maba_tensor* w_gate, const maba_tensor* w_up) {
+  if (gated_check(x, nullptr, w_gate, w_up, "gated_ffn")) return 0;
+  return gated_plan(x, nullptr, w_gate, w_up, false, false, nullptr).bytes;
+}
+
+extern "C" int maba_hip_gated_ffn(const maba_tensor* x, const maba_tensor* w_gate, const maba_tensor* w_up, maba_tensor* out,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "gated_ffn";
+  int rc = gated_check(x, nullptr, w_gate, w_up, who);
+  if (!rc) rc = check_out(out, who, "out", w_gate->dtype, x->shape[0], w_gate->shape[0]);
+  if (rc) return rc;
+  if (overlap(out, x) || overlap(out, w_gate) || overlap(out, w_up)) return fail(MABA_ERR_INVALID, "%s: out overlaps an input", who);
+  GatedPlan p = gated_plan(x, nullptr, w_gate, w_up, false, false, workspace);
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
+    return fail(MABA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, p.bytes);
+  if (p.M == 0) return MABA_OK;
+  return w_gate->dtype == MABA_BF16 ? gated_forward<Bf16>(p, x, w_gate, w_up, out, (hipStream_t)stream, who)
+                                    : gated_forward<Fp16>(p, x, w_gate, w_up, out, (hipStream_t)stream, who);
+}
+
+extern "C" size_t maba_hip_gated_ffn_backward_workspace_size(const maba_tensor* x, const maba_tensor* x_scales,
+                                                             const maba_tensor* w_gate, const maba_tensor* w_up, int with_dw) {
+  if (gated_check(x, x_scales, w_gate, w_up, "gated_ffn_backward")) return 0;
+  return gated_plan(x, x_scales, w_gate, w_up, true, with_dw != 0, nullptr).bytes;
+}
+
+extern "C" int maba_hip_gated_ffn_backward(const maba_tensor* dh, const maba_tensor* x, const maba_tensor* x_scales,
+                                           const maba_tensor* w_gate, const maba_tensor* w_up, maba_tensor* dx,
+                                           maba_tensor* dw_gate, maba_tensor* dw_up, void* workspace, size_t workspace_bytes,
+                                           void* stream) {
+  const char* who = "gated_ffn_backward";
+  int rc = gated_check(x, x_scales, w_gate, w_up, who);
+  if (rc) return rc;
+  const int dt = w_gate->dtype;
+  const int64_t M = x->shape[0], C = x->shape[1], I = w_gate->shape[0];
+  rc = check_rows(dh, who, "dh", dt, M, I);
+  if (!rc && dx) rc = check_out(dx, who, "dx", dt, M, C);
+  if (!rc && dw_gate) rc = check_out(dw_gate, who, "dw_gate", dt, I, C);
+  if (!rc && dw_up) rc = check_out(dw_up, who, "dw_up", dt, I, C);
+  if (rc) return rc;
+  const maba_tensor *outs[3] = {dx, dw_gate, dw_up}, *ins[5] = {dh, x, x_scales, w_gate, w_up};
+  for (int i = 0; i < 3; ++i) {
+    for (int j = 0; j < 5; ++j)
+      if (overlap(outs[i], ins[j])) return fail(MABA_ERR_INVALID, "%s: a gradient overlaps an input", who);
+    for (int j = 0; j < i; ++j)
+      if (overlap(outs[i], outs[j])) return fail(MABA_ERR_INVALID, "%s: two gradients overlap", who);
+  }
+  GatedPlan p = gated_plan(x, x_scales, w_gate, w_up, true, dw_gate || dw_up, workspace);
+  if (!workspace ? p.bytes > 0 : workspace_bytes < p.bytes)
+    return fail(MABA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, p.bytes);
+  return dt == MABA_BF16 ? gated_backward<Bf16>(p, dh, x, x_scales, w_gate, w_up, dx, dw_gate, dw_up, (hipStream_t)stream, who)
+                         : gated_backward<Fp16>(p, dh, x, x_scales, w_gate, w_up, dx, dw_gate, dw_up, (hipStream_t)stream, who);
+}

@@ -1,0 +1,358 @@
+// A linear layer with its epilogue, and its backward pass:
+//
+//   z = x W^T + b,  y = r + gate * act(z)           x [M, K], W [N, K], b, gate [N], r, y [M, N]
+//   dz = dy * gate * act'(z),  dx = dz W,  dW = dz^T x,  db = sum_m dz,  dgate = sum_m dy * act(z),  dr = dy
+//
+// act is none, relu, silu or gelu (with the error function); b, r and gate are each optional.  The epilogue works
+// on the fp32 accumulators and y is rounded once.
+//
+// Backward: where dz is not dy itself, one launch makes z again from x and its epilogue writes dz, rounded
+// once to 16 bits as the next products' operand, and the column sums of a tile's rows (fp32, before that
+// rounding) for db and dgate, which a later launch adds in order.  Then dx = dz W reads W along its columns, and
+// dW = dz^T x both operands, summed over token ranges into fp32 partials added in order.
+#include <algorithm>
+
+#include "ffn_common.h"
+#include "ffn_skinny.h"
+
+namespace maba {
+namespace ffn {
+
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
+
+template <int ACT>
+__device__ __forceinline__ float act_of(float z) {
+  if constexpr (ACT == ACT_RELU) return z > 0.f ? z : z != z ? z : 0.f;
+  else if constexpr (ACT == ACT_SILU) return z * sigmoid(z);
+  else if constexpr (ACT == ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678f));
+  else return z;
+}
+template <int ACT>
+__device__ __forceinline__ float dact_of(float z) {
+  if constexpr (ACT == ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  else if constexpr (ACT == ACT_SILU) {
+    const float s = sigmoid(z);
+    return s * (1.f + z * (1.f - s));
+  } else if constexpr (ACT == ACT_GELU) {
+    return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * fast_exp(-0.5f * z * z);
+  } else return 1.f;
+}
+
+template <int ACT>
+struct EpiLinear {
+  struct Args { Rows y, res; const uint16_t *bias, *gate; int M, N; };
+  template <class T>
+  static __device__ __forceinline__ void quad(const Args& e, int64_t m, int n, f32x4 z, f32x4) {
+    if (e.bias) z += vec4<T>(e.bias, n, e.N);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) z[r] = act_of<ACT>(z[r]);
+    if (e.gate) z *= vec4<T>(e.gate, n, e.N);
+    if (e.res.p) z += load4<T>(e.res, m, n, e.N);
+    store4<T>(e.y, m, n, e.N, z);
+  }
+  template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
+  static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
+                                             int q, int wave, uint16_t* lds) {
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int n = n0 + 16 * j + 4 * q;
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int m = m0 + 16 * i + c;
+        if (m < e.M && n < e.N) quad<T>(e, m, n, acc[i][j], acc[i][j]);
+      }
+    }
+  }
+};
+
+// dz [M, Np] (Np = N rounded up to 8, zeros behind N) and, with sums, the tile's column sums [tiles_m][2][N]: of dz
+// for the bias, of dy * act(z) for the gate.
+template <int ACT>
+struct EpiLinearBack {
+  struct Args { Rows dy, dz; const uint16_t *bias, *gate; float* sums; int M, N, Np; };
+  template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
+  static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
+                                             int q, int wave, uint16_t* lds) {
+    float* part = (float*)lds;                    // [WM][2][BN]
+    if (e.sums) __syncthreads();                  // the last stage has been read
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int n = n0 + 16 * j + 4 * q;
+      f32x4 gate = {1.f, 1.f, 1.f, 1.f}, bias = {0.f, 0.f, 0.f, 0.f}, sb = bias, sg = bias;
+      if (e.gate) gate = vec4<T>(e.gate, n, e.N);
+      if (e.bias) bias = vec4<T>(e.bias, n, e.N);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int m = m0 + 16 * i + c;
+        if (m >= e.M || n >= e.Np) continue;
+        const f32x4 dy = load4<T>(e.dy, m, n, e.N), z = acc[i][j] + bias;
+        f32x4 dz;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          dz[r] = dy[r] * gate[r] * dact_of<ACT>(z[r]);
+          sg[r] += dy[r] * act_of<ACT>(z[r]);
+        }
+        sb += dz;
+        store4<T>(e.dz, m, n, e.Np, dz);
+      }
+      if (e.sums) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {             // over the 16 rows that the lanes of a quarter hold
+#pragma unroll
+          for (int s = 1; s < 16; s <<= 1) {
+            sb[r] += __shfl_xor(sb[r], s);
+            sg[r] += __shfl_xor(sg[r], s);
+          }
+        }
+        if (c == 0) {
+          const int col = (wave % WN) * (BN / WN) + 16 * j + 4 * q;
+          *(f32x4*)(part + ((wave / WN) * 2 + 0) * BN + col) = sb;
+          *(f32x4*)(part + ((wave / WN) * 2 + 1) * BN + col) = sg;
+        }
+      }
+    }
+    if (e.sums) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < 2 * BN; i += 64 * WM * WN) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < WM; ++w) v += part[(w * 2 + i / BN) * BN + i % BN];
+        const int n = t.n * BN + i % BN;
+        if (n < e.N) e.sums[((int64_t)t.m * 2 + i / BN) * e.N + n] = v;
+      }
+    }
+  }
+};
+
+struct LinearPlan {
+  int64_t M, N, K, Kp, Np, sum_rows;
+  bool copy_x, copy_w, copy_dy, z;      // z: dz is made from z, otherwise it is dy
+  uint16_t *x, *w, *dz;
+  float *part, *sums;
+  int splits;
+  size_t bytes;
+};
+
+struct LinearNeeds { bool dx, dw, dbias, dgate; };
+
+static LinearPlan linear_plan(const maba_tensor* x, const maba_tensor* scales, const maba_tensor* w, int act, bool gate,
+                              const maba_tensor* dy, const LinearNeeds* need, void* ws) {
+  LinearPlan p = {};
+  p.M = x->shape[0];
+  p.K = x->shape[1];
+  p.N = w->shape[0];
+  p.Kp = pad8(p.K);
+  p.Np = pad8(p.N);
+  const bool few = !need && p.M <= SKINNY_ROWS;
+  p.z = need && (act != ACT_NONE || gate);
+  // which products read x and W: forward both; backward x for z and dW, W for z and dx
+  const bool use_x = !need || p.z || need->dw, use_w = !need || p.z || need->dx;
+  p.copy_x = !few && use_x && (scales || !aligned_rows(x));
+  p.copy_w = !few && use_w && !aligned_rows(w);
+  p.copy_dy = need && !p.z && (need->dx || need->dw) && !aligned_rows(dy);
+  Carve c = {(char*)ws, 0};
+  if (p.copy_x) p.x = c.take<uint16_t>(p.M * p.Kp);
+  if (p.copy_w) p.w = c.take<uint16_t>(p.N * p.Kp);
+  if (need) {
+    if (p.z || p.copy_dy) p.dz = c.take<uint16_t>(p.M * p.Np);
+    if (need->dbias || need->dgate) {
+      p.sum_rows = ceil_div(p.M, 128);
+      p.sums = c.take<float>(p.sum_rows * 2 * p.N);
+    }
+    if (need->dw) {
+      p.splits = k_splits(p.Np, p.Kp, p.M);
+      p.part = c.take<float>((int64_t)p.splits * p.Np * p.Kp);
+    }
+  }
+  p.bytes = c.used;
+  return p;
+}
+static_assert(GEMM_BM == 128, "column sums are kept for 128 rows at a time");
+
+static int linear_operands(LinearPlan& p, const maba_tensor* x, const maba_tensor* scales, const maba_tensor* w, hipStream_t s,
+                           Operand& ox, Operand& ow) {
+  if (p.copy_x)
+    if (int rc = copy_rows(x, scales, w->dtype, p.x, s)) return rc;
+  if (p.copy_w)
+    if (int rc = copy_rows(w, nullptr, w->dtype, p.w, s)) return rc;
+  ox = p.copy_x ? rows_operand(p.x, p.Kp, p.M) : rows_operand((const uint16_t*)x->data, x->stride[0], p.M);
+  ow = p.copy_w ? rows_operand(p.w, p.Kp, p.N) : rows_operand((const uint16_t*)w->data, w->stride[0], p.N);
+  return MABA_OK;
+}
+
+static const uint16_t* vec_of(const maba_tensor* t) { return t ? (const uint16_t*)t->data : nullptr; }
+
+template <class T, int ACT>
+static int linear_forward(LinearPlan& p, const maba_tensor* x, const maba_tensor* w, const maba_tensor* bias,
+                          const maba_tensor* res, const maba_tensor* gate, maba_tensor* y, hipStream_t s, const char* who) {
+  typedef EpiLinear<ACT> E;
+  const typename E::Args e = {rows_of(y), rows_of(res), vec_of(bias), vec_of(gate), (int)p.M, (int)p.N};
+  if (p.M <= SKINNY_ROWS) {
+    const uint16_t* wp = (const uint16_t*)w->data;
+    SkinnyArgs a = {(const uint16_t*)x->data, x->stride[0], {wp, wp}, {w->stride[0], w->stride[0]}, (int)p.M, (int)p.N,
+                    (int)p.K, aligned_rows(x), aligned_rows(w)};
+    return skinny<T, false, E>(a, e, s, who);
+  }
+  GemmArgs g = {};
+  if (int rc = linear_operands(p, x, nullptr, w, s, g.a, g.b)) return rc;
+  g.K = p.Kp;
+  return gemm<T, K_ROWS, K_ROWS, E>(g, e, p.M, p.N, 1, s, who);
+}
+
+template <class T, int ACT>
+static int make_dz(const LinearPlan& p, const Operand& ox, const Operand& ow, const maba_tensor* dy, const maba_tensor* bias,
+                   const maba_tensor* gate, hipStream_t s, const char* who) {
+  typedef EpiLinearBack<ACT> E;
+  GemmArgs g = {};
+  g.a = ox;
+  g.b = ow;
+  g.K = p.Kp;
+  const Rows dz = {p.dz, p.Np, 1};
+  const typename E::Args e = {rows_of(dy), dz, vec_of(bias), vec_of(gate), p.sums, (int)p.M, (int)p.N, (int)p.Np};
+  return gemm<T, K_ROWS, K_ROWS, E>(g, e, p.M, p.Np, 1, s, who);
+}
+
+template <class T>
+static int linear_backward(LinearPlan& p, const maba_tensor* dy, const maba_tensor* x, const maba_tensor* scales,
+                           const maba_tensor* w, const maba_tensor* bias, int act, const maba_tensor* gate, maba_tensor* dx,
+                           maba_tensor* dw, maba_tensor* dbias, maba_tensor* dgate, hipStream_t s, const char* who) {
+  Operand ox, ow;
+  if (int rc = linear_operands(p, x, scales, w, s, ox, ow)) return rc;
+  Operand dz = rows_operand((const uint16_t*)dy->data, dy->stride[0], p.M);
+  if (p.z || p.copy_dy) dz = rows_operand(p.dz, p.Np, p.M);
+  if (p.M > 0) {
+    int rc = MABA_OK;
+    if (p.z)
+      rc = act == ACT_RELU   ? make_dz<T, ACT_RELU>(p, ox, ow, dy, bias, gate, s, who)
+           : act == ACT_SILU ? make_dz<T, ACT_SILU>(p, ox, ow, dy, bias, gate, s, who)
+           : act == ACT_GELU ? make_dz<T, ACT_GELU>(p, ox, ow, dy, bias, gate, s, who)
+                             : make_dz<T, ACT_NONE>(p, ox, ow, dy, bias, gate, s, who);
+    else if (p.copy_dy) rc = copy_rows(dy, nullptr, w->dtype, p.dz, s);
+    if (!rc && !p.z && dbias) rc = column_partials(dy, p.sums, s);
+    if (rc) return rc;
+  }
+  if (dbias || dgate)
+    if (int rc = reduce_columns(p.sums, p.sum_rows, (int)p.N, dbias ? dbias->data : nullptr, dgate ? dgate->data : nullptr,
+                                w->dtype, s))
+      return rc;
+  if (dx && p.M > 0) {
+    GemmArgs g = {};
+    g.a = dz;
+    g.b = cols_operand(ow, p.Kp);
+    g.K = p.Np;                 // dz is N wide where N is a whole number of chunks, padded with zeros otherwise
+    const EpiStore::Args e = {rows_of(dx), (int)p.M, (int)p.K};
+    if (int rc = gemm<T, K_ROWS, K_COLS, EpiStore>(g, e, p.M, p.K, 1, s, who)) return rc;
+  }
+  if (dw) {
+    if (p.M > 0) {
+      GemmArgs g = {};
+      g.a = cols_operand(dz, p.Np);
+      g.b = cols_operand(ox, p.Kp);
+      g.K = p.M;
+      const EpiPartial::Args e = {p.part, (int)p.Np, (int)p.Kp};
+      if (int rc = gemm<T, K_COLS, K_COLS, EpiPartial>(g, e, p.Np, p.Kp, p.splits, s, who)) return rc;
+    }
+    ReduceArgs r = {p.part, p.M > 0 ? p.splits : 0, (int)p.Np, (int)p.Kp, (int)p.Np, (int)p.N, (int)p.K, {}};
+    r.out[0] = rows_of(dw);
+    if (int rc = reduce_splits(r, w->dtype, s)) return rc;
+  }
+  return MABA_OK;
+}
+
+static int linear_check(const maba_tensor* x, const maba_tensor* scales, const maba_tensor* w, const maba_tensor* bias, int act,
+                        const maba_tensor* gate, const char* who) {
+  if (!x || !w) return fail(MABA_ERR_INVALID, "%s: x and weight required", who);
+  if (w->dtype != MABA_BF16 && w->dtype != MABA_F16)
+    return fail(w->dtype == MABA_F32 ? MABA_ERR_UNSUPPORTED : MABA_ERR_DTYPE, "%s: 16-bit weights only, got dtype code %d", who, w->dtype);
+  if (x->ndim != 2 || w->ndim != 2) return fail(MABA_ERR_INVALID, "%s: x and weight must be 2D", who);
+  if (act < ACT_NONE || act > ACT_GELU) return fail(MABA_ERR_INVALID, "%s: activation code %d is not in [0, 3]", who, act);
+  int rc = check_sizes(who, x->shape[0], w->shape[0], x->shape[1]);
+  if (!rc) rc = check_kept(x, scales, who, w->dtype, -1, x->shape[1]);
+  if (!rc && scales && scales->shape[0] != x->shape[0]) rc = fail(MABA_ERR_INVALID, "%s: scales do not match the codes", who);
+  if (!rc) rc = check_rows(w, who, "weight", w->dtype, -1, x->shape[1]);
+  if (!rc && bias) rc = check_vec(bias, who, "bias", w->dtype, w->shape[0]);
+  if (!rc && gate) rc = check_vec(gate, who, "gate", w->dtype, w->shape[0]);
+  return rc;
+}
+
+}  // namespace ffn
+}  // namespace maba
+
+using namespace maba;
+using namespace maba::ffn;
+
+extern "C" size_t maba_hip_linear_epilogue_workspace_size(const maba_tensor* x, const maba_tensor* weight) {
+  if (linear_check(x, nullptr, weight, nullptr, 0, nullptr, "linear_epilogue")) return 0;
+  return linear_plan(x, nullptr, weight, 0, false, nullptr, nullptr, nullptr).bytes;
+}
+
+extern "C" int maba_hip_linear_epilogue(const maba_tensor* x, const maba_tensor* weight, const maba_tensor* bias, int act,
+                                        const maba_tensor* residual, const maba_tensor* gate, maba_tensor* out, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  const char* who = "linear_epilogue";
+  int rc = linear_check(x, nullptr, weight, bias, act, gate, who);
+  if (rc) return rc;
+  const int dt = weight->dtype;
+  const int64_t M = x->shape[0], N = weight->shape[0];
+  if (residual) rc = check_rows(residual, who, "residual", dt, M, N);
+  if (!rc) rc = check_out(out, who, "out", dt, M, N);
+  if (rc) return rc;
+  if (overlap(out, x) || overlap(out, weight) || overlap(out, bias) || overlap(out, gate))
+    return fail(MABA_ERR_INVALID, "%s: out overlaps an input", who);
+  // each element of the residual is read by the lane that then writes its sum: the very same rows may be out
+  if (residual && overlap(out, residual) && (out->data != residual->data || out->stride[0] != residual->stride[0]))
+    return fail(MABA_ERR_INVALID, "%s: out overlaps the residual at another place", who);
+  LinearPlan p = linear_plan(x, nullptr, weight, act, gate != nullptr, nullptr, nullptr, workspace);
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
+    return fail(MABA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, p.bytes);
+  if (p.M == 0) return MABA_OK;
+  const hipStream_t s = (hipStream_t)stream;
+#define LINEAR_FORWARD(T)                                                                                  \
+  (act == ACT_RELU   ? linear_forward<T, ACT_RELU>(p, x, weight, bias, residual, gate, out, s, who)        \
+   : act == ACT_SILU ? linear_forward<T, ACT_SILU>(p, x, weight, bias, residual, gate, out, s, who)        \
+   : act == ACT_GELU ? linear_forward<T, ACT_GELU>(p, x, weight, bias, residual, gate, out, s, who)        \
+                     : linear_forward<T, ACT_NONE>(p, x, weight, bias, residual, gate, out, s, who))
+  return dt == MABA_BF16 ? LINEAR_FORWARD(Bf16) : LINEAR_FORWARD(Fp16);
+#undef LINEAR_FORWARD
+}
+
+extern "C" size_t maba_hip_linear_epilogue_backward_workspace_size(const maba_tensor* dy, const maba_tensor* x,
+                                                                   const maba_tensor* x_scales, const maba_tensor* weight, int act,
+                                                                   int with_gate, int needs) {
+  if (linear_check(x, x_scales, weight, nullptr, act, nullptr, "linear_epilogue_backward")) return 0;
+  if (check_rows(dy, "linear_epilogue_backward", "dy", weight->dtype, x->shape[0], weight->shape[0])) return 0;
+  const LinearNeeds n = {(needs & 1) != 0, (needs & 2) != 0, (needs & 4) != 0, (needs & 8) != 0};
+  return linear_plan(x, x_scales, weight, act, with_gate != 0, dy, &n, nullptr).bytes;
+}
+
+extern "C" int maba_hip_linear_epilogue_backward(const maba_tensor* dy, const maba_tensor* x, const maba_tensor* x_scales,
+                                                 const maba_tensor* weight, const maba_tensor* bias, int act,
+                                                 const maba_tensor* gate, maba_tensor* dx, maba_tensor* dw, maba_tensor* dbias,
+                                                 maba_tensor* dgate, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "linear_epilogue_backward";
+  int rc = linear_check(x, x_scales, weight, bias, act, gate, who);
+  if (rc) return rc;
+  const int dt = weight->dtype;
+  const int64_t M = x->shape[0], K = x->shape[1], N = weight->shape[0];
+  rc = check_rows(dy, who, "dy", dt, M, N);
+  if (!rc && dx) rc = check_out(dx, who, "dx", dt, M, K);
+  if (!rc && dw) rc = check_out(dw, who, "dw", dt, N, K);
+  if (!rc && dbias) rc = check_vec(dbias, who, "dbias", dt, N);
+  if (!rc && dgate) rc = check_vec(dgate, who, "dgate", dt, N);
+  if (!rc && dgate && !gate) rc = fail(MABA_ERR_INVALID, "%s: dgate without a gate", who);
+  if (rc) return rc;
+  const maba_tensor *outs[4] = {dx, dw, dbias, dgate}, *ins[6] = {dy, x, x_scales, weight, bias, gate};
+  for (int i = 0; i < 4; ++i) {
+    for (int j = 0; j < 6; ++j)
+      if (overlap(outs[i], ins[j])) return fail(MABA_ERR_INVALID, "%s: a gradient overlaps an input", who);
+    for (int j = 0; j < i; ++j)
+      if (overlap(outs[i], outs[j])) return fail(MABA_ERR_INVALID, "%s: two gradients overlap", who);
+  }
+  const LinearNeeds need = {dx != nullptr, dw != nullptr, dbias != nullptr, dgate != nullptr};
+  LinearPlan p = linear_plan(x, x_scales, weight, act, gate != nullptr, dy, &need, workspace);
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
+    return fail(MABA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, p.bytes);
+  return dt == MABA_BF16
+             ? linear_backward<Bf16>(p, dy, x, x_scales, weight, bias, act, gate, dx, dw, dbias, dgate, (hipStream_t)stream, who)
+             : linear_backward<Fp16>(p, dy, x, x_scales, weight, bias, act, gate, dx, dw, dbias, dgate, (hipStream_t)stream, who);
+}

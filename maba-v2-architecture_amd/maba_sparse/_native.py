@@ -7,6 +7,7 @@ when a HIP op is called, so a GPU run can never silently take another path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import struct
@@ -19,7 +20,7 @@ LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib")
 # MABA_HIP_LIBRARY names another build of the same library (a missing file still raises)
 LIB_PATH = os.environ.get("MABA_HIP_LIBRARY") or os.path.join(LIB_DIR, "libmaba_hip.so")
 
-MABA_F32, MABA_F16, MABA_BF16, MABA_F64, MABA_I64, MABA_I32 = 0, 1, 2, 3, 4, 5
+MABA_F32, MABA_F16, MABA_BF16, MABA_F64, MABA_I64, MABA_I32, MABA_E4M3, MABA_U8 = 0, 1, 2, 3, 4, 5, 6, 7
 _DTYPE_CODES = {
     torch.float32: MABA_F32,
     torch.float16: MABA_F16,
@@ -27,6 +28,8 @@ _DTYPE_CODES = {
     torch.float64: MABA_F64,
     torch.int64: MABA_I64,
     torch.int32: MABA_I32,
+    torch.float8_e4m3fn: MABA_E4M3,
+    torch.uint8: MABA_U8,
 }
 
 MABA_OK, MABA_ERR_INVALID, MABA_ERR_DTYPE, MABA_ERR_UNSUPPORTED, MABA_ERR_HIP, MABA_ERR_WORKSPACE = range(6)
@@ -64,6 +67,16 @@ EXPORTED_SYMBOLS = (
     "maba_hip_argmax_rows",
     "maba_hip_cache_append_heads",
     "maba_hip_maba_sa_decode_dev_heads",
+    "maba_hip_gated_ffn_workspace_size",
+    "maba_hip_gated_ffn",
+    "maba_hip_gated_ffn_backward_workspace_size",
+    "maba_hip_gated_ffn_backward",
+    "maba_hip_linear_epilogue_workspace_size",
+    "maba_hip_linear_epilogue",
+    "maba_hip_linear_epilogue_backward_workspace_size",
+    "maba_hip_linear_epilogue_backward",
+    "maba_hip_checkpoint_pack",
+    "maba_hip_checkpoint_unpack",
 )
 
 
@@ -122,6 +135,16 @@ def _declare(lib) -> None:
         "maba_hip_argmax_rows": ([T, T, vp], i),
         "maba_hip_cache_append_heads": ([T, T, vp, T, T, T, T, i, i, T, T, T, T, T, T, vp], i),
         "maba_hip_maba_sa_decode_dev_heads": ([T, T, T, T, T, vp, i64, f, i, i, i, i, T, T, T, vp, sz, vp], i),
+        "maba_hip_gated_ffn_workspace_size": ([T, T, T], sz),
+        "maba_hip_gated_ffn": ([T, T, T, T, vp, sz, vp], i),
+        "maba_hip_gated_ffn_backward_workspace_size": ([T, T, T, T, i], sz),
+        "maba_hip_gated_ffn_backward": ([T, T, T, T, T, T, T, T, vp, sz, vp], i),
+        "maba_hip_linear_epilogue_workspace_size": ([T, T], sz),
+        "maba_hip_linear_epilogue": ([T, T, T, i, T, T, T, vp, sz, vp], i),
+        "maba_hip_linear_epilogue_backward_workspace_size": ([T, T, T, T, i, i, i], sz),
+        "maba_hip_linear_epilogue_backward": ([T, T, T, T, T, i, T, T, T, T, T, vp, sz, vp], i),
+        "maba_hip_checkpoint_pack": ([T, T, T, vp], i),
+        "maba_hip_checkpoint_unpack": ([T, T, T, vp], i),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -188,6 +211,11 @@ def desc_array(tensors: Sequence[Optional[torch.Tensor]]):
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is current (kernel launches and workspace queries go by it)."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def check(rc: int, what: str) -> None:

@@ -437,3 +437,112 @@ reference_stream_superposition = ref_stream_superposition
 ref_centroids = ref_compute_centroids
 ref_topk = ref_index_topk
 ref_superposition = ref_stream_superposition
+
+
+# ----------------------------------------------------------------------------- feed-forward operators
+
+PACK_GROUP = 32            # elements of a row that share one power of two in a packed activation
+ACTIVATIONS = ("none", "relu", "silu", "gelu")
+
+
+def _pow2(e):
+    """``2^e`` in fp64 for integers ``-1022 <= e <= 1023``, from its bits (exact on every device)."""
+    return ((e.to(torch.int64) + 1023) << 52).view(torch.float64)
+
+
+def ref_checkpoint_pack(x, **kwargs: Any):
+    """``x [..., C]`` as ``(codes, scales)``: float8_e4m3fn codes of x's shape and uint8 scales
+    ``[..., ceil(C / 32)]``.  Every 32 elements of a row share ``2^e``, the smallest power of two
+    (e >= -127) with ``max|x| <= 448 * 2^e`` over the finite ones; ``scale = e + 127`` and
+    ``code = x / 2^e`` rounded to nearest even.  NaN and infinities become e4m3's NaN."""
+    C = x.shape[-1]
+    groups = -(-C // PACK_GROUP)
+    xg = torch.nn.functional.pad(x.float(), (0, groups * PACK_GROUP - C)).unflatten(-1, (groups, PACK_GROUP))
+    fin = torch.where(torch.isfinite(xg), xg.abs(), torch.zeros((), device=x.device))
+    mant, exp = torch.frexp(fin.amax(dim=-1, keepdim=True))           # mant in [0.5, 1), 0 for 0
+    e = torch.where(mant > 0, exp - 9 + (mant > 448 / 512).to(exp.dtype), -127).clamp(min=-127)
+    v = torch.where(torch.isfinite(xg), (xg.double() * _pow2(-e)).float(), torch.full((), float("nan"), device=x.device))
+    codes = v.to(torch.float8_e4m3fn).flatten(-2)[..., :C].contiguous()
+    return codes, (e + 127).to(torch.uint8).squeeze(-1)
+
+
+def ref_checkpoint_unpack(codes, scales, dtype: torch.dtype = torch.bfloat16, **kwargs: Any):
+    """The values that a packed activation stands for, ``code * 2^(scale - 127)`` rounded to ``dtype``."""
+    C = codes.shape[-1]
+    e = (scales.to(torch.int32) - 127).repeat_interleave(PACK_GROUP, dim=-1)[..., :C]
+    # 2^-127 is subnormal in fp32: the product is formed in fp64 (exact) and rounded once
+    return (codes.float().double() * _pow2(e)).to(dtype)
+
+
+def _kept(x, x_scales, ct):
+    return ref_checkpoint_unpack(x, x_scales, dtype=ct) if x_scales is not None else x.to(ct)
+
+
+def ref_gated_ffn(x, w_gate, w_up, **kwargs: Any):
+    """``silu(x Wg^T) * (x Wu^T)`` (reference model.py:25-38 up to the down projection), in fp32 (fp64
+    for fp64 inputs) and rounded once."""
+    ct = torch.promote_types(x.dtype, torch.float32)
+    g, u = x.to(ct) @ w_gate.to(ct).t(), x.to(ct) @ w_up.to(ct).t()
+    return (g * torch.sigmoid(g) * u).to(x.dtype)
+
+
+def ref_gated_ffn_backward(dh, x, w_gate, w_up, x_scales=None, needs=(True, True, True), **kwargs: Any):
+    """``(dx, dw_gate, dw_up)`` of ``ref_gated_ffn`` (None where ``needs`` says so); ``x`` may be the
+    codes of a packed activation, with ``x_scales``."""
+    dt, C = w_gate.dtype, x.shape[-1]
+    ct = torch.promote_types(dt, torch.float32)
+    xf, d = _kept(x, x_scales, ct).reshape(-1, C), dh.to(ct).reshape(-1, dh.shape[-1])
+    wg, wu = w_gate.to(ct), w_up.to(ct)
+    g, u = xf @ wg.t(), xf @ wu.t()
+    s = torch.sigmoid(g)
+    dg, du = d * u * s * (1 + g * (1 - s)), d * g * s
+    dx = (dg @ wg + du @ wu).to(dt).reshape(x.shape) if needs[0] else None
+    return dx, (dg.t() @ xf).to(dt) if needs[1] else None, (du.t() @ xf).to(dt) if needs[2] else None
+
+
+def _act(z, activation):
+    """``act(z)`` and its derivative."""
+    if activation == "relu":
+        return torch.relu(z), (z > 0).to(z.dtype)
+    if activation == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s * (1 + z * (1 - s))
+    if activation == "gelu":
+        cdf = 0.5 * (1 + torch.erf(z * math.sqrt(0.5)))
+        return z * cdf, cdf + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    return z, torch.ones_like(z)
+
+
+def ref_linear_epilogue(x, weight, bias=None, activation: str = "none", residual=None, gate=None, **kwargs: Any):
+    """``residual + gate * act(x W^T + bias)`` (nn.Linear and the gated residual of reference
+    model.py:92-128), in fp32 (fp64 for fp64 inputs) and rounded once."""
+    ct = torch.promote_types(x.dtype, torch.float32)
+    z = x.to(ct) @ weight.to(ct).t()
+    if bias is not None:
+        z = z + bias.to(ct)
+    y = _act(z, activation)[0]
+    if gate is not None:
+        y = y * gate.to(ct)
+    if residual is not None:
+        y = y + residual.to(ct)
+    return y.to(x.dtype)
+
+
+def ref_linear_epilogue_backward(dy, x, weight, bias=None, activation: str = "none", gate=None, x_scales=None,
+                                 needs=(True, True, True, True), **kwargs: Any):
+    """``(dx, dw, dbias, dgate)`` of ``ref_linear_epilogue`` (None where ``needs`` says so, or where there
+    is no bias or gate); the residual's gradient is ``dy``."""
+    dt, K = weight.dtype, x.shape[-1]
+    ct = torch.promote_types(dt, torch.float32)
+    d, w = dy.to(ct).reshape(-1, dy.shape[-1]), weight.to(ct)
+    xf = _kept(x, x_scales, ct).reshape(-1, K)
+    z = xf @ w.t()
+    if bias is not None:
+        z = z + bias.to(ct)
+    a, da = _act(z, activation)
+    dz = d * da if gate is None else d * gate.to(ct) * da
+    dx = (dz @ w).to(dt).reshape(x.shape) if needs[0] else None
+    dw = (dz.t() @ xf).to(dt) if needs[1] else None
+    dbias = dz.sum(0).to(dt) if needs[2] and bias is not None else None
+    dgate = (d * a).sum(0).to(dt) if needs[3] and gate is not None else None
+    return dx, dw, dbias, dgate

@@ -22,6 +22,9 @@ Differences, all deliberate:
   prefill streams and their gate, layers/sparse_attention.py:95-219,275) and
   ``dgda_prologue`` (the DGDA layer's conv, gates and key normalisation,
   layers/dgda.py:103-121,186-207).
+* The feed-forward operators ``gated_ffn`` and ``linear_epilogue`` (model.py:25-38, 92-128, where
+  the reference composes torch modules) carry their own gradients on every backend, through their
+  ``*_backward`` ops; ``checkpoint_pack`` and ``checkpoint_unpack`` hold activations in 8 bits.
 * ``allow_mixed_dtypes=True`` (keyword) lets ``dgda_prefill``/``dgda_step``
   accept bf16 q/k/v with fp32 gates and state; without it the reference's
   "dtypes must match" ``TypeError`` is kept.
@@ -38,6 +41,7 @@ import torch
 from maba_sparse._native import HipLibraryMissing
 from maba_sparse.kernels import common as _c
 from maba_sparse.kernels import cpu_dgda as _cpu
+from maba_sparse.kernels import feed_forward as _ff
 
 logger = logging.getLogger(__name__)
 
@@ -53,6 +57,12 @@ _KERNEL_REGISTRY: Dict[str, Dict[str, Callable]] = {
         "maba_sa_decode": _c.ref_maba_sa_decode,
         "dgda_prologue": _c.ref_dgda_prologue,
         "maba_sa_prefill": _c.ref_maba_sa_prefill,
+        "gated_ffn": _c.ref_gated_ffn,
+        "gated_ffn_backward": _c.ref_gated_ffn_backward,
+        "linear_epilogue": _c.ref_linear_epilogue,
+        "linear_epilogue_backward": _c.ref_linear_epilogue_backward,
+        "checkpoint_pack": _c.ref_checkpoint_pack,
+        "checkpoint_unpack": _c.ref_checkpoint_unpack,
     },
     # host cores: the chunked DGDA of the reference's CPU backend (cpu_dgda.py), the rest as
     # the reference ops in torch
@@ -67,6 +77,12 @@ _KERNEL_REGISTRY: Dict[str, Dict[str, Callable]] = {
         "maba_sa_decode": _c.ref_maba_sa_decode,
         "dgda_prologue": _c.ref_dgda_prologue,
         "maba_sa_prefill": _c.ref_maba_sa_prefill,
+        "gated_ffn": _c.ref_gated_ffn,
+        "gated_ffn_backward": _c.ref_gated_ffn_backward,
+        "linear_epilogue": _c.ref_linear_epilogue,
+        "linear_epilogue_backward": _c.ref_linear_epilogue_backward,
+        "checkpoint_pack": _c.ref_checkpoint_pack,
+        "checkpoint_unpack": _c.ref_checkpoint_unpack,
     },
     "hip": {},
     "xla": {},
@@ -348,6 +364,192 @@ def dispatch_maba_sa_prefill(q, k, v, kh, vh, early, idx, gate_logits, scale: fl
                                              block_size=block_size, pool=pool, **kwargs))
 
 
+# ----------------------------------------------------------------------------- feed-forward operators
+
+
+def _ffn_same(x, named) -> None:
+    """One floating dtype and one device for all tensors."""
+    if x.dtype not in (torch.float32, torch.float16, torch.bfloat16, torch.float64):
+        raise TypeError(f"Unsupported dtype {x.dtype}. Supported: "
+                        f"{(torch.float32, torch.float16, torch.bfloat16, torch.float64)}")
+    for name, t in named:
+        if t is None:
+            continue
+        if t.device != x.device:
+            raise RuntimeError(
+                f"Expected all tensors to be on the same device, but got {x.device} and {t.device} for {name}")
+        if t.dtype != x.dtype:
+            raise TypeError(f"Tensor dtypes must match, but got {x.dtype} and {t.dtype} for {name}")
+
+
+def _ffn_shape(name, t, shape) -> None:
+    if t is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+
+
+def _ffn_weight(name, w, width) -> None:
+    if w.dim() != 2 or w.shape[1] != width or w.shape[0] == 0 or width == 0:
+        raise ValueError(f"{name} must be [width, {width}] with positive widths, got {list(w.shape)}")
+
+
+def _ffn_input(x) -> None:
+    if x.dim() < 1:
+        raise ValueError("x must have a channel dimension")
+
+
+def _ffn_checkpoint(checkpoint) -> None:
+    if checkpoint not in (None, "e4m3"):
+        raise ValueError(f"checkpoint must be None or 'e4m3', got {checkpoint!r}")
+
+
+def _ffn_activation(activation) -> None:
+    if activation not in _c.ACTIVATIONS:
+        raise ValueError(f"activation must be one of {_c.ACTIVATIONS}, got {activation!r}")
+
+
+def _ffn_kept(x, x_scales) -> None:
+    """The kept input of a backward op: a tensor, or codes with their scales."""
+    if x_scales is None:
+        return
+    if x.dtype != torch.float8_e4m3fn or x_scales.dtype != torch.uint8:
+        raise TypeError(f"a packed input is float8_e4m3fn codes and uint8 scales, got {x.dtype} and {x_scales.dtype}")
+    _ffn_shape("x_scales", x_scales, (*x.shape[:-1], -(-x.shape[-1] // _c.PACK_GROUP)))
+    if x.device != x_scales.device:
+        raise RuntimeError(
+            f"Expected all tensors to be on the same device, but got {x.device} and {x_scales.device} for x_scales")
+
+
+class _FFNOps:
+    """The ops that the autograd functions call, through the backend of their tensors' device."""
+
+    @staticmethod
+    def pack(x):
+        return _run("checkpoint_pack", x.device, dict(x=x))
+
+    @staticmethod
+    def gated_ffn(x, w_gate, w_up):
+        return _run("gated_ffn", x.device, dict(x=x, w_gate=w_gate, w_up=w_up))
+
+    @staticmethod
+    def gated_ffn_backward(dh, x, w_gate, w_up, x_scales, needs):
+        return _run("gated_ffn_backward", dh.device, dict(dh=dh, x=x, w_gate=w_gate, w_up=w_up, x_scales=x_scales,
+                                                          needs=tuple(needs)))
+
+    @staticmethod
+    def linear_epilogue(x, weight, bias, activation, residual, gate):
+        return _run("linear_epilogue", x.device, dict(x=x, weight=weight, bias=bias, activation=activation,
+                                                      residual=residual, gate=gate))
+
+    @staticmethod
+    def linear_epilogue_backward(dy, x, weight, bias, activation, gate, x_scales, needs):
+        return _run("linear_epilogue_backward", dy.device, dict(dy=dy, x=x, weight=weight, bias=bias, gate=gate,
+                                                                activation=activation, x_scales=x_scales,
+                                                                needs=tuple(needs)))
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def dispatch_gated_ffn(x, w_gate, w_up, checkpoint: Optional[str] = None) -> torch.Tensor:
+    """``silu(x Wg^T) * (x Wu^T)``: the gated feed-forward block up to its down projection.
+
+    x ``[..., C]``, w_gate and w_up ``[I, C]`` of one dtype and device; returns ``[..., I]``, computed in
+    fp32 and rounded once.  Differentiable on every backend.  What the backward pass keeps is ``x``; with
+    ``checkpoint="e4m3"`` its packed form, half the bytes, and the gradients are those at the unpacked input."""
+    _ffn_input(x)
+    _ffn_same(x, (("w_gate", w_gate), ("w_up", w_up)))
+    _ffn_weight("w_gate", w_gate, x.shape[-1])
+    _ffn_shape("w_up", w_up, w_gate.shape)
+    _ffn_checkpoint(checkpoint)
+    if _wants_grad(x, w_gate, w_up):
+        return _ff.guard_capture(_ff.GatedFFN.apply(_FFNOps, checkpoint, x, w_gate, w_up))
+    return _FFNOps.gated_ffn(x, w_gate, w_up)
+
+
+def dispatch_gated_ffn_backward(dh, x, w_gate, w_up, x_scales=None, needs=(True, True, True)):
+    """``(dx, dw_gate, dw_up)`` of ``gated_ffn`` for its output's gradient ``dh [..., I]``, None where ``needs``
+    is false.  ``x`` is the forward's input, or with ``x_scales`` its packed codes.  No autograd takes part."""
+    _ffn_input(x)
+    _ffn_kept(x, x_scales)
+    _ffn_same(dh, (("x", x if x_scales is None else None), ("w_gate", w_gate), ("w_up", w_up)))
+    _ffn_weight("w_gate", w_gate, x.shape[-1])
+    _ffn_shape("w_up", w_up, w_gate.shape)
+    _ffn_shape("dh", dh, (*x.shape[:-1], w_gate.shape[0]))
+    if len(needs) != 3:
+        raise ValueError(f"needs takes three flags (dx, dw_gate, dw_up), got {needs!r}")
+    with torch.no_grad():
+        return _FFNOps.gated_ffn_backward(dh, x, w_gate, w_up, x_scales, needs)
+
+
+def dispatch_linear_epilogue(x, weight, bias=None, activation: str = "none", residual=None, gate=None,
+                             checkpoint: Optional[str] = None) -> torch.Tensor:
+    """``residual + gate * act(x W^T + bias)``: a linear layer with what follows it in its epilogue.
+
+    x ``[..., K]``, weight ``[N, K]``, bias and gate ``[N]``, residual ``[..., N]`` of one dtype and device; bias,
+    gate and residual are optional; activation none, relu, silu or gelu (with the error function).  Computed
+    in fp32 and rounded once.  Differentiable on every backend; ``checkpoint`` as for ``gated_ffn``."""
+    _ffn_input(x)
+    _ffn_same(x, (("weight", weight), ("bias", bias), ("residual", residual), ("gate", gate)))
+    _ffn_weight("weight", weight, x.shape[-1])
+    n = weight.shape[0]
+    _ffn_shape("bias", bias, (n,))
+    _ffn_shape("gate", gate, (n,))
+    _ffn_shape("residual", residual, (*x.shape[:-1], n))
+    _ffn_activation(activation)
+    _ffn_checkpoint(checkpoint)
+    if _wants_grad(x, weight, bias, residual, gate):
+        return _ff.guard_capture(_ff.LinearEpilogue.apply(_FFNOps, checkpoint, activation, x, weight, bias, residual, gate))
+    return _FFNOps.linear_epilogue(x, weight, bias, activation, residual, gate)
+
+
+def dispatch_linear_epilogue_backward(dy, x, weight, bias=None, activation: str = "none", gate=None, x_scales=None,
+                                      needs=(True, True, True, True)):
+    """``(dx, dw, dbias, dgate)`` of ``linear_epilogue`` for its output's gradient ``dy [..., N]``, None where
+    ``needs`` is false or there is no bias or gate; the residual's gradient is ``dy``.  ``x`` as for
+    ``gated_ffn_backward``.  No autograd takes part."""
+    _ffn_input(x)
+    _ffn_kept(x, x_scales)
+    _ffn_same(dy, (("x", x if x_scales is None else None), ("weight", weight), ("bias", bias), ("gate", gate)))
+    _ffn_weight("weight", weight, x.shape[-1])
+    n = weight.shape[0]
+    _ffn_shape("bias", bias, (n,))
+    _ffn_shape("gate", gate, (n,))
+    _ffn_shape("dy", dy, (*x.shape[:-1], n))
+    _ffn_activation(activation)
+    if len(needs) != 4:
+        raise ValueError(f"needs takes four flags (dx, dw, dbias, dgate), got {needs!r}")
+    with torch.no_grad():
+        return _FFNOps.linear_epilogue_backward(dy, x, weight, bias, activation, gate, x_scales, needs)
+
+
+def dispatch_checkpoint_pack(x) -> Tuple[torch.Tensor, torch.Tensor]:
+    """An activation ``x [..., C]`` in 8 bits: ``(codes, scales)`` (see ``common.ref_checkpoint_pack``), not
+    differentiable."""
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"x must have a positive channel dimension, got {list(x.shape)}")
+    if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f"Unsupported dtype {x.dtype}. Supported: {(torch.float32, torch.float16, torch.bfloat16)}")
+    with torch.no_grad():
+        return _FFNOps.pack(x)
+
+
+def dispatch_checkpoint_unpack(codes, scales, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values that ``(codes, scales)`` stand for, in ``dtype``."""
+    if codes.dim() < 1 or codes.shape[-1] == 0:
+        raise ValueError(f"codes must have a positive channel dimension, got {list(codes.shape)}")
+    _ffn_kept(codes, scales)
+    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f"Unsupported dtype {dtype}. Supported: {(torch.float32, torch.float16, torch.bfloat16)}")
+    return _run("checkpoint_unpack", codes.device, dict(codes=codes, scales=scales, dtype=dtype))
+
+
+gated_ffn = dispatch_gated_ffn
+gated_ffn_backward = dispatch_gated_ffn_backward
+linear_epilogue = dispatch_linear_epilogue
+linear_epilogue_backward = dispatch_linear_epilogue_backward
+checkpoint_pack = dispatch_checkpoint_pack
+checkpoint_unpack = dispatch_checkpoint_unpack
 dgda_prefill = dispatch_dgda_prefill
 dgda_step = dispatch_dgda_step
 compute_centroids = dispatch_compute_centroids

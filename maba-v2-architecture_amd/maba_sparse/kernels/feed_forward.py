@@ -1,0 +1,78 @@
+"""Gradients of the feed-forward operators: autograd functions over the dispatcher's forward and
+backward ops, the same on every backend.
+
+The forward pass keeps its input (or, with ``checkpoint="e4m3"``, the input's packed form) and the
+parameters; the backward op makes the pre-activations again from it.  With a checkpoint the gradients
+are those at the unpacked input: the forward result is unaffected.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+
+class GatedFFN(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ops, checkpoint, x, w_gate, w_up):
+        ctx.ops = ops
+        if any(ctx.needs_input_grad):
+            kept = ops.pack(x) if checkpoint else (x,)
+            ctx.save_for_backward(w_gate, w_up, *kept)
+        return ops.gated_ffn(x, w_gate, w_up)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        w_gate, w_up, x, *scales = ctx.saved_tensors
+        grads = ctx.ops.gated_ffn_backward(dh, x, w_gate, w_up, scales[0] if scales else None, ctx.needs_input_grad[2:5])
+        return (None, None, *grads)
+
+
+class LinearEpilogue(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ops, checkpoint, activation, x, weight, bias, residual, gate):
+        ctx.ops, ctx.activation = ops, activation
+        dx, dw, dbias, _, dgate = ctx.needs_input_grad[3:8]
+        ctx.has = (bias is not None, gate is not None)
+        # x is read by dW and, where dz is not dy itself, to make z again
+        ctx.keeps_x = dw or dgate or ((dx or dbias) and (activation != "none" or gate is not None))
+        kept = (ops.pack(x) if checkpoint else (x,)) if ctx.keeps_x else ()
+        ctx.x_like = x.shape
+        if dx or dw or dbias or dgate:
+            ctx.save_for_backward(weight, *(t for t in (bias, gate) if t is not None), *kept)
+        return ops.linear_epilogue(x, weight, bias, activation, residual, gate)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        dx, dw, dbias, dres, dgate = ctx.needs_input_grad[3:8]
+        grads = (None, None, None, None)
+        if dx or dw or dbias or dgate:
+            weight, *rest = ctx.saved_tensors
+            bias = rest.pop(0) if ctx.has[0] else None
+            gate = rest.pop(0) if ctx.has[1] else None
+            # where x is not read, a view of its shape over one weight row takes its place
+            x = rest[0] if ctx.keeps_x else weight[0].expand(ctx.x_like)
+            scales = rest[1] if len(rest) > 1 else None
+            grads = ctx.ops.linear_epilogue_backward(dy, x, weight, bias, ctx.activation, gate, scales, (dx, dw, dbias, dgate))
+        return (None, None, None, grads[0], grads[1], grads[2], dy if dres else None, grads[3])
+
+
+def guard_capture(out: torch.Tensor) -> torch.Tensor:
+    """Refuses to record a backward pass whose gradients would reach a leaf through an autograd node
+    of another stream.  Such a node lives as long as any eager graph of that leaf does; the engine
+    would then make the node's stream wait inside the capture, which ends the process.  The node keeps
+    the stream that it was first seen on, so a capture beside a live eager graph of these operators
+    raises here instead."""
+    if out.is_cuda and out.grad_fn is not None:
+        stream = torch.cuda.current_stream(out.device).cuda_stream
+        capturing = torch.cuda.is_current_stream_capturing()
+        for node, _ in out.grad_fn.next_functions:
+            if node is None or not hasattr(node, "variable"):
+                continue
+            first = node.metadata.setdefault("maba_stream", stream)
+            if capturing and first != stream:
+                raise RuntimeError(
+                    "a leaf of this captured call still belongs to an eager autograd graph on another stream: drop "
+                    "that graph's outputs first, or capture the *_backward ops, which need no autograd")
+    return out

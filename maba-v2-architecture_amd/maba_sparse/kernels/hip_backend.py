@@ -299,6 +299,128 @@ def hip_maba_sa_prefill(q, k, v, kh, vh, early, idx, gate_logits, scale: float, 
     return out
 
 
+# ----------------------------------------------------------------------------- feed-forward operators
+# 16-bit tensors; fp32 and fp64 ones raise NotImplementedError (the dispatcher's reference computes them).
+
+_ACT_CODES = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t [..., C]`` as ``[rows, C]`` with unit column stride: a view where the strides allow it."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _row(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+@register_kernel("hip", "gated_ffn")
+def hip_gated_ffn(x, w_gate, w_up, **kwargs: Any) -> torch.Tensor:
+    """``silu(x Wg^T) * (x Wu^T)`` in one launch (contract: ``dispatcher.dispatch_gated_ffn``)."""
+    _no_grad_needed("gated_ffn", x, w_gate, w_up)
+    dev = N.require_device([x, w_gate, w_up], "gated_ffn")
+    with N.on_device(dev):
+        lib = N.load()
+        x2 = _rows(x)
+        out = torch.empty(x2.shape[0], w_gate.shape[0], dtype=x.dtype, device=dev)
+        dx, dg, du = N.desc(x2), N.desc(_rows(w_gate)), N.desc(_rows(w_up))
+        nbytes = lib.maba_hip_gated_ffn_workspace_size(dx, dg, du)
+        ws = _workspace(nbytes, dev) if nbytes else None
+        rc = lib.maba_hip_gated_ffn(dx, dg, du, N.desc(out), ws.data_ptr() if nbytes else None, nbytes, N.stream_ptr(dev))
+        N.check(rc, "gated_ffn")
+    return out.view(*x.shape[:-1], w_gate.shape[0])
+
+
+@register_kernel("hip", "gated_ffn_backward")
+def hip_gated_ffn_backward(dh, x, w_gate, w_up, x_scales=None, needs=(True, True, True), **kwargs: Any):
+    """``(dx, dw_gate, dw_up)`` (contract: ``dispatcher.dispatch_gated_ffn_backward``)."""
+    _no_grad_needed("gated_ffn_backward", dh, x, w_gate, w_up)
+    dev = N.require_device([dh, x, w_gate, w_up, x_scales], "gated_ffn_backward")
+    with N.on_device(dev):
+        lib = N.load()
+        x2, sc = _rows(x), None if x_scales is None else _rows(x_scales)
+        dt = w_gate.dtype
+        dx = torch.empty(x2.shape, dtype=dt, device=dev) if needs[0] else None
+        dws = [torch.empty(w_gate.shape, dtype=dt, device=dev) if n else None for n in needs[1:3]]
+        ddx, dsc, dg, du = N.desc(x2), N.desc(sc), N.desc(_rows(w_gate)), N.desc(_rows(w_up))
+        ws = _workspace(lib.maba_hip_gated_ffn_backward_workspace_size(ddx, dsc, dg, du, int(any(needs[1:3]))), dev)
+        rc = lib.maba_hip_gated_ffn_backward(N.desc(_rows(dh)), ddx, dsc, dg, du, N.desc(dx), N.desc(dws[0]),
+                                             N.desc(dws[1]), ws.data_ptr(), ws.numel(), N.stream_ptr(dev))
+        N.check(rc, "gated_ffn_backward")
+    return (dx.view(x.shape) if needs[0] else None, *dws)
+
+
+@register_kernel("hip", "linear_epilogue")
+def hip_linear_epilogue(x, weight, bias=None, activation: str = "none", residual=None, gate=None,
+                        **kwargs: Any) -> torch.Tensor:
+    """``residual + gate * act(x W^T + bias)`` in one launch (contract: ``dispatcher.dispatch_linear_epilogue``)."""
+    _no_grad_needed("linear_epilogue", x, weight, bias, residual, gate)
+    dev = N.require_device([x, weight, bias, residual, gate], "linear_epilogue")
+    with N.on_device(dev):
+        lib = N.load()
+        x2 = _rows(x)
+        out = torch.empty(x2.shape[0], weight.shape[0], dtype=x.dtype, device=dev)
+        dx, dw = N.desc(x2), N.desc(_rows(weight))
+        nbytes = lib.maba_hip_linear_epilogue_workspace_size(dx, dw)
+        ws = _workspace(nbytes, dev) if nbytes else None
+        rc = lib.maba_hip_linear_epilogue(dx, dw, N.desc(_row(bias)), _ACT_CODES[activation],
+                                          N.desc(None if residual is None else _rows(residual)), N.desc(_row(gate)),
+                                          N.desc(out), ws.data_ptr() if nbytes else None, nbytes, N.stream_ptr(dev))
+        N.check(rc, "linear_epilogue")
+    return out.view(*x.shape[:-1], weight.shape[0])
+
+
+@register_kernel("hip", "linear_epilogue_backward")
+def hip_linear_epilogue_backward(dy, x, weight, bias=None, activation: str = "none", gate=None, x_scales=None,
+                                 needs=(True, True, True, True), **kwargs: Any):
+    """``(dx, dw, dbias, dgate)`` (contract: ``dispatcher.dispatch_linear_epilogue_backward``)."""
+    _no_grad_needed("linear_epilogue_backward", dy, x, weight, bias, gate)
+    dev = N.require_device([dy, x, weight, bias, gate, x_scales], "linear_epilogue_backward")
+    with N.on_device(dev):
+        lib = N.load()
+        x2, sc = _rows(x), None if x_scales is None else _rows(x_scales)
+        dt, n_out = weight.dtype, weight.shape[0]
+        needs = (needs[0], needs[1], needs[2] and bias is not None, needs[3] and gate is not None)
+        shapes = (x2.shape, weight.shape, (n_out,), (n_out,))
+        outs = [torch.empty(s, dtype=dt, device=dev) if n else None for s, n in zip(shapes, needs)]
+        ddy, ddx, dsc, dw = N.desc(_rows(dy)), N.desc(x2), N.desc(sc), N.desc(_rows(weight))
+        act = _ACT_CODES[activation]
+        ws = _workspace(lib.maba_hip_linear_epilogue_backward_workspace_size(
+            ddy, ddx, dsc, dw, act, int(gate is not None), sum(1 << i for i, n in enumerate(needs) if n)), dev)
+        rc = lib.maba_hip_linear_epilogue_backward(ddy, ddx, dsc, dw, N.desc(_row(bias)), act, N.desc(_row(gate)),
+                                                   *(N.desc(o) for o in outs), ws.data_ptr(), ws.numel(), N.stream_ptr(dev))
+        N.check(rc, "linear_epilogue_backward")
+    return (outs[0].view(x.shape) if needs[0] else None, *outs[1:])
+
+
+@register_kernel("hip", "checkpoint_pack")
+def hip_checkpoint_pack(x, **kwargs: Any) -> Tuple[torch.Tensor, torch.Tensor]:
+    """e4m3 codes and scales of ``x`` (contract: ``common.ref_checkpoint_pack``)."""
+    dev = N.require_device([x], "checkpoint_pack")
+    with N.on_device(dev):
+        x2 = _rows(x)
+        rows, C = x2.shape
+        groups = (C + 31) // 32
+        codes = torch.empty(rows, C, dtype=torch.float8_e4m3fn, device=dev)
+        scales = torch.empty(rows, groups, dtype=torch.uint8, device=dev)
+        N.check(N.load().maba_hip_checkpoint_pack(N.desc(x2), N.desc(codes), N.desc(scales), N.stream_ptr(dev)),
+                "checkpoint_pack")
+    return codes.view(x.shape), scales.view(*x.shape[:-1], groups)
+
+
+@register_kernel("hip", "checkpoint_unpack")
+def hip_checkpoint_unpack(codes, scales, dtype: torch.dtype = torch.bfloat16, **kwargs: Any) -> torch.Tensor:
+    """The values of a packed activation (contract: ``common.ref_checkpoint_unpack``)."""
+    dev = N.require_device([codes, scales], "checkpoint_unpack")
+    with N.on_device(dev):
+        c2 = _rows(codes)
+        out = torch.empty(c2.shape, dtype=dtype, device=dev)
+        N.check(N.load().maba_hip_checkpoint_unpack(N.desc(c2), N.desc(_rows(scales)), N.desc(out), N.stream_ptr(dev)),
+                "checkpoint_unpack")
+    return out.view(codes.shape)
+
+
 # ----------------------------------------------------------------------------- serving path
 # Entry points for a decode step whose per-step scalars (the cache position) live in device
 # memory, so that one captured HIP graph serves every position.  Not dispatcher ops: the
