@@ -38,6 +38,7 @@ int gemm(GemmArgs g, const typename Epi::Args& e, int64_t M, int64_t N, int spli
   g.tiles_m = (int)ceil_div(M, GEMM_BM);
   g.tiles_n = (int)ceil_div(N, GEMM_BN);
   g.splits = splits;
+  if (!g.segments) g.segments = 1;
   g.k_split = ceil_div(ceil_div(g.K, splits), GEMM_BK) * GEMM_BK;
   const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * splits;
   if (grid > INT32_MAX) return fail(MABA_ERR_UNSUPPORTED, "%s: too many tiles", who);

@@ -6,7 +6,7 @@
 //   columns of k  A[k * lda + m]: the same tensors where the sum runs over their rows (dx = dz W
 //                 reads W that way, dW = dz^T x reads both)
 // so that no operand is transposed in memory beforehand.  A tile of either kind goes from HBM to LDS by
-// direct loads (16 bytes a lane, no registers), ST stages deep.  Rows of k are read back as 16-byte
+// direct loads (16 bytes a lane, no registers).  Rows of k are read back as 16-byte
 // fragments, columns of k with the transposing LDS read.  Both layouts XOR the 16-byte chunk index
 // with bits of the row, on the global address side since a direct load fills LDS in lane order, so
 // that the 16 lanes of a fragment read meet distinct banks.
@@ -45,37 +45,42 @@ struct Fp16 {
   static __device__ __forceinline__ uint32_t down(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }
 };
 
-// Rows [M, N] of 16-bit elements in global memory that an epilogue reads or writes four columns at a
-// time.  vec: every row start is 8-byte aligned, so that whole quads move at once.
+// Rows [M, N] of 16-bit elements in global memory that an epilogue reads or writes four columns at a time, at
+// any alignment of an element (global memory takes unaligned vector accesses).
 struct Rows {
   uint16_t* p;
   int64_t ld;
-  int vec;
 };
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
 template <class T>
-__device__ __forceinline__ f32x4 load4(const Rows& r, int64_t m, int n, int nend) {
+__device__ __forceinline__ f32x4 up4(u32x2 u) {
+  return f32x4{T::up(u[0] & 0xffffu), T::up(u[0] >> 16), T::up(u[1] & 0xffffu), T::up(u[1] >> 16)};
+}
+template <class T>
+__device__ __forceinline__ u32x2 down4(f32x4 v) {
+  return u32x2{T::down(v[0]) | (T::down(v[1]) << 16), T::down(v[2]) | (T::down(v[3]) << 16)};
+}
+// The raw quad at (m, n); rows from mend and columns from nend on are zeros and are not read.
+__device__ __forceinline__ u32x2 load4(const Rows& r, int64_t m, int n, int mend, int nend) {
   const uint16_t* p = r.p + m * r.ld + n;
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  if (r.vec && n + 4 <= nend) {
-    const u32x2 u = *(const u32x2*)p;
-    v[0] = T::up(u[0] & 0xffffu); v[1] = T::up(u[0] >> 16); v[2] = T::up(u[1] & 0xffffu); v[3] = T::up(u[1] >> 16);
-  } else {
+  if (m >= mend) return u32x2{0, 0};
+  if (n + 4 <= nend) return *(const u32x2_any*)p;
+  u32x2 u = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < nend) v[i] = T::up(p[i]);
-  }
-  return v;
+  for (int i = 0; i < 3; ++i)
+    if (n + i < nend) u[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+  return u;
 }
 template <class T>
 __device__ __forceinline__ void store4(const Rows& r, int64_t m, int n, int nend, f32x4 v) {
   uint16_t* p = r.p + m * r.ld + n;
-  if (r.vec && n + 4 <= nend) {
-    const u32x2 u = {T::down(v[0]) | (T::down(v[1]) << 16), T::down(v[2]) | (T::down(v[3]) << 16)};
-    *(u32x2*)p = u;
+  const u32x2 u = down4<T>(v);
+  if (n + 4 <= nend) {
+    *(u32x2_any*)p = u;
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < nend) p[i] = (uint16_t)T::down(v[i]);
+    for (int i = 0; i < 3; ++i)
+      if (n + i < nend) p[i] = (uint16_t)(u[i >> 1] >> (16 * (i & 1)));
   }
 }
 // Four consecutive elements of a vector [N].
@@ -88,69 +93,80 @@ __device__ __forceinline__ f32x4 vec4(const uint16_t* p, int n, int nend) {
   return v;
 }
 
-enum { K_ROWS = 0, K_ROWS_PAIR = 1, K_COLS = 2, K_COLS_PAIR = 3 };
+enum { K_ROWS = 0, K_ROWS_PAIR = 1, K_COLS = 2 };
 
 // One operand.  K_ROWS: p[0] is [rows][K], ld[0] apart.  K_ROWS_PAIR: two such tensors of `rows` rows
 // each, whose rows alternate in runs of 16 along the tile (a gate run, then its up run).  K_COLS:
-// p[0] is [krows][rows]; k from krows to K (fewer than eight) count as zeros.  K_COLS_PAIR: k < ksplit reads
-// p[0], later k row k - ksplit of p[1]; both have krows rows, and rows from there to ksplit count as zeros.
+// p[0] is [krows][rows]; k from krows to K (fewer than eight) count as zeros.  A sum of two segments of K each
+// (dx = dg Wg + du Wu) goes on with column K of p[0] in K_ROWS, with p[1] in K_COLS.
 struct Operand {
   const uint16_t* p[2];
   int64_t ld[2];
-  int rows;
-  int ksplit, krows;
+  int rows, krows;
 };
 
 struct GemmArgs {
   Operand a, b;
-  int64_t K;
+  int64_t K;            // of a segment
+  int segments;         // 1 or 2
   int tiles_m, tiles_n, splits;
-  int64_t k_split;      // k of one split, a multiple of the stage depth
+  int64_t k_split;      // k of one split, a multiple of the stage depth (one segment only)
 };
 
 constexpr uint32_t OUT_OF_RANGE = 0x80000000u;   // a lane offset past every descriptor's end
 
+// The same in every lane; said so to the compiler, which otherwise loops over the lanes' descriptors.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, uint32_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)bytes, 0x00027000);
+  const uint64_t a = (uint64_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a), hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc((void*)((uint64_t)hi << 32 | lo), 0, (int)__builtin_amdgcn_readfirstlane(bytes),
+                                           0x00027000);
 }
 __device__ __forceinline__ void lds_load16(__amdgpu_buffer_rsrc_t r, uint16_t* lds, uint32_t voff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, (int)voff, 0, 0, 0);
 }
 
+// Swizzles.  Rows of k: LDS row r (BK elements) keeps 16-byte chunk c at c ^ key_rows(r), so that 16 consecutive
+// rows' chunks c lie in the 64 banks once each.  Columns of k: LDS row k (R elements) keeps the pair of chunks p at
+// p ^ key_cols(k); a fragment read takes rows 4 j .. 4 j + 3 of two j that differ by 2, whose own offsets (R / 2 banks a
+// row) leave log2(128 / gcd(R, 128)) of the three bits that tell the eight rows apart to the row number.
+template <int BK>
+__device__ __forceinline__ constexpr int key_rows(int r) {
+  return (r / (16 / (BK / 8))) & (BK / 8 - 1);
+}
+template <int R>
+__device__ __forceinline__ constexpr int key_cols(int k) {
+  return R % 128 == 0 ? (k & 3) | (k >> 3 & 1) << 2 : R % 64 == 0 ? (k >> 1 & 1) | (k >> 3 & 1) << 1 : k >> 3 & 1;
+}
+
 // Stages R rows (or columns) x BK of an operand.
 template <int R, int BK, int NW, int MODE>
 struct Stager {
-  static constexpr bool COLS = MODE == K_COLS || MODE == K_COLS_PAIR;
+  static constexpr bool COLS = MODE == K_COLS;
   static constexpr int CPR = (COLS ? R : BK) / 8;                  // 16-byte chunks of an LDS row
-  static constexpr int RPI = 64 / CPR;                             // LDS rows of one wave instruction
   static constexpr int LOADS = R * BK / (512 * NW);
-  static_assert(R * BK % (512 * NW) == 0 && CPR <= 64, "whole instructions");
-  static constexpr int PAIRMASK = CPR >= 16 ? 7 : CPR / 2 - 1;
+  static_assert(R * BK % (512 * NW) == 0 && R % 32 == 0, "whole instructions");
 
-  uint32_t voff[LOADS];        // lane offsets from the tile's base (K_COLS_PAIR: without the row's part)
-  uint32_t rowoff[2];          // K_COLS_PAIR: the row's part, with either tensor's stride
+  uint32_t voff[LOADS];        // lane offsets from the tile's base
   int chunk;                   // rows of k: the lane's chunk of its row, the same for every load
   const char* base[2];         // of the tile, at the first k
   uint32_t span;               // rows of k: bytes from base to the operand's end (rows of this tile)
   int64_t ldb[2];
   int wave, cols;
 
-  // Swizzles: LDS row r keeps chunk c at c ^ key(r).
-  static __device__ __forceinline__ int key_rows(int r) { return (r / (16 / CPR)) & (CPR - 1); }
-  static __device__ __forceinline__ int key_cols(int k) { return 2 * (((k & 3) | ((k >> 3) & 1) << 2) & PAIRMASK); }
-
-  __device__ __forceinline__ void init(const Operand& o, int64_t K, int64_t kbeg, int r0, int wave_, int lane) {
+  __device__ __forceinline__ void init(const Operand& o, const GemmArgs& g, int64_t kbeg, int r0, int wave_, int lane) {
     wave = wave_;
     ldb[0] = o.ld[0] * 2;
     ldb[1] = o.ld[1] * 2;
     if constexpr (!COLS) {
+      constexpr int RPI = 64 / CPR;                                // LDS rows of one wave instruction
       static_assert(MODE == K_ROWS || NW * RPI % 32 == 0, "a wave's loads belong to one of the paired tensors");
-      chunk = (lane % CPR) ^ key_rows(wave * RPI + lane / CPR);
+      chunk = (lane % CPR) ^ key_rows<BK>(wave * RPI + lane / CPR);
       const int t = MODE == K_ROWS_PAIR ? (wave * RPI >> 4) & 1 : 0;
       const int first = MODE == K_ROWS_PAIR ? r0 / 2 : r0, most = MODE == K_ROWS_PAIR ? R / 2 : R;
       const int rows = min(o.rows - first, most);
       base[0] = (const char*)(t ? o.p[1] : o.p[0]) + (int64_t)first * ldb[t] + 2 * kbeg;
-      span = rows > 0 ? (uint32_t)((rows - 1) * ldb[t] + 2 * (K - kbeg)) : 0u;
+      span = rows > 0 ? (uint32_t)((rows - 1) * ldb[t] + 2 * (g.segments * g.K - kbeg)) : 0u;
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         int r = (i * NW + wave) * RPI + lane / CPR;
@@ -161,42 +177,33 @@ struct Stager {
       cols = 2 * min(o.rows - r0, R);
       base[0] = (const char*)o.p[0] + 2 * (int64_t)r0;
       base[1] = (const char*)o.p[1] + 2 * (int64_t)r0;
-      rowoff[0] = (uint32_t)((lane / CPR) * ldb[0]);
-      rowoff[1] = (uint32_t)((lane / CPR) * ldb[1]);
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int k = (i * NW + wave) * RPI + lane / CPR;
-        voff[i] = 16 * ((lane % CPR) ^ key_cols(k)) + (MODE == K_COLS ? (uint32_t)(k * ldb[0]) : 0u);
+        const int l = (i * NW + wave) * 64 + lane, k = l / CPR, x = l % CPR;
+        // both segments' tensors have the same stride
+        voff[i] = (uint32_t)(k * ldb[0]) + 16 * ((((x >> 1) ^ key_cols<R>(k)) << 1) | (x & 1));
       }
     }
   }
 
-  // k0: the stage's first k; kend: the end of this workgroup's k range.
-  __device__ __forceinline__ void issue(const Operand& o, uint16_t* lds, int64_t k0, int64_t kbeg, int64_t kend) {
+  // k0: the stage's first k of segment seg; kend: the end of this workgroup's k range in it.
+  __device__ __forceinline__ void issue(const Operand& o, const GemmArgs& g, uint16_t* lds, int seg, int64_t k0, int64_t kbeg,
+                                        int64_t kend) {
+    const char* p;
+    uint32_t bytes, dead = 0;
     if constexpr (!COLS) {
-      const uint32_t adv = 2 * (uint32_t)(k0 - kbeg);
-      const uint32_t dead = k0 + 8 * chunk >= kend ? OUT_OF_RANGE : 0u;
-      const auto r = rsrc(base[0] + adv, span > adv ? span - adv : 0u);
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) lds_load16(r, lds + (i * NW + wave) * 512, voff[i] | dead);
-    } else if constexpr (MODE == K_COLS) {
-      const uint32_t bytes = (uint32_t)((min(min(kend, (int64_t)o.krows) - k0, (int64_t)BK) - 1) * ldb[0] + cols);
-      const auto r = rsrc(base[0] + k0 * ldb[0], bytes);
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) lds_load16(r, lds + (i * NW + wave) * 512, voff[i]);
+      const uint32_t adv = 2 * (uint32_t)(seg * g.K + k0 - kbeg);
+      p = base[0] + adv;
+      bytes = span > adv ? span - adv : 0u;
+      dead = k0 + 8 * chunk >= kend ? OUT_OF_RANGE : 0u;
     } else {
-      // ksplit is a multiple of 8, so an instruction's rows lie on one side of it; each side has its own
-      // stride, and its own end
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int64_t k = k0 + (i * NW + wave) * RPI;
-        const int t = k >= o.ksplit;
-        const int64_t row = k - (t ? o.ksplit : 0), left = o.krows - row, ld = t ? ldb[1] : ldb[0];
-        const uint32_t bytes = left > 0 ? (uint32_t)((min(left, (int64_t)RPI) - 1) * ld + cols) : 0u;
-        lds_load16(rsrc((t ? base[1] : base[0]) + row * ld, bytes), lds + (i * NW + wave) * 512,
-                   voff[i] + (t ? rowoff[1] : rowoff[0]));
-      }
+      const int64_t rows = min(min(kend, (int64_t)o.krows) - k0, (int64_t)BK);
+      p = base[seg] + k0 * ldb[0];
+      bytes = (uint32_t)((rows - 1) * ldb[0] + cols);
     }
+    const auto r = rsrc(p, bytes);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) lds_load16(r, lds + (i * NW + wave) * 512, voff[i] | dead);
   }
 };
 
@@ -204,15 +211,10 @@ struct Stager {
 // row r0 + c.
 template <int R, int BK, int MODE>
 __device__ __forceinline__ u32x4 fragment(const uint16_t* lds, int r0, int kk, int c, int q) {
-  if constexpr (MODE == K_ROWS || MODE == K_ROWS_PAIR) {
-    constexpr int CPR = BK / 8;
-    const int key = (c / (16 / CPR)) & (CPR - 1);                  // r0 is a multiple of 16
-    return *(const u32x4*)(lds + (r0 + c) * BK + 8 * ((kk * 4 + q) ^ key));
+  if constexpr (MODE != K_COLS) {
+    return *(const u32x4*)(lds + (r0 + c) * BK + 8 * ((kk * 4 + q) ^ key_rows<BK>(c)));   // r0 is a multiple of 16
   } else {
-    constexpr int CPR = R / 8;
-    constexpr int MASK = CPR >= 16 ? 7 : CPR / 2 - 1;
-    const int key = ((c >> 2) | (q & 1) << 2) & MASK;
-    const uint16_t* p = lds + (kk * 32 + q * 8 + (c >> 2)) * R + 16 * ((r0 >> 4) ^ key) + 4 * (c & 3);
+    const uint16_t* p = lds + (kk * 32 + q * 8 + (c >> 2)) * R + 16 * ((r0 >> 4) ^ key_cols<R>(q * 8 + (c >> 2))) + 4 * (c & 3);
     typedef __attribute__((address_space(3))) i16x4 lds4;
     const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p));
     const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * R)));
@@ -241,66 +243,112 @@ __device__ __forceinline__ TileId tile_of(const GemmArgs& g) {
   return r;
 }
 
+// The main loop keeps two stages of 64 k in LDS and the fragments of two steps of 32 k in registers.  While the
+// products of one step run, the fragments of the next are read; the one barrier of a stage stands between its two
+// steps, where every wave has the stage's last fragments in registers (its buffer is free for the loads of the stage
+// after next) and the next stage has landed (its first fragments can be read).  So neither LDS reads nor
+// loads are waited for between products, except by the first.
 template <class T, int BM, int BN, int WM, int WN, int BK, int ST, int AMODE, int BMODE, class Epi>
-__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g, typename Epi::Args e) {
+__global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) void gemm_kernel(GemmArgs g, typename Epi::Args e) {
   constexpr int NW = WM * WN, MI = BM / WM / 16, NI = BN / WN / 16;
-  constexpr int A_EL = BM * BK, B_EL = BN * BK;
+  constexpr int A_EL = BM * BK, STAGE = (BM + BN) * BK;
   typedef Stager<BM, BK, NW, AMODE> SA;
   typedef Stager<BN, BK, NW, BMODE> SB;
-  constexpr int LOADS = SA::LOADS + SB::LOADS;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[ST * (A_EL + B_EL)];
+  __shared__ __attribute__((aligned(16))) uint16_t lds[ST * STAGE];
 
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
   const int c = lane & 15, q = lane >> 4;
   const TileId t = tile_of(g);
   const int m0 = t.m * BM, n0 = t.n * BN;
   const int64_t kbeg = t.split * g.k_split, kend = min(g.K, kbeg + g.k_split);
-  const int nk = (int)((kend - kbeg + BK - 1) / BK);
+  const int nk1 = (int)((kend - kbeg + BK - 1) / BK), nk = nk1 * g.segments;     // stages of a segment, of all
+  const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
 
   SA sa;
   SB sb;
-  sa.init(g.a, g.K, kbeg, m0, wave, lane);
-  sb.init(g.b, g.K, kbeg, n0, wave, lane);
-  auto issue = [&](int it) {
-    uint16_t* p = lds + (it % ST) * (A_EL + B_EL);
-    const int64_t k0 = kbeg + (int64_t)it * BK;
-    sa.issue(g.a, p, k0, kbeg, kend);
-    sb.issue(g.b, p + A_EL, k0, kbeg, kend);
+  sa.init(g.a, g, kbeg, m0, wave, lane);
+  sb.init(g.b, g, kbeg, n0, wave, lane);
+  auto issue = [&](int s) {
+    uint16_t* p = lds + (s % ST) * STAGE;
+    const int seg = s >= nk1;
+    const int64_t k0 = kbeg + (int64_t)(s - seg * nk1) * BK;
+    sa.issue(g.a, g, p, seg, k0, kbeg, kend);
+    sb.issue(g.b, g, p + A_EL, seg, k0, kbeg, kend);
   };
-
+  struct Frags { u32x4 a[MI], b[NI]; };
+  auto read = [&](Frags& f, int s, int kk) {
+    const uint16_t* p = lds + (s % ST) * STAGE;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) f.b[j] = fragment<BN, BK, BMODE>(p + A_EL, wn + 16 * j, kk, c, q);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) f.a[i] = fragment<BM, BK, AMODE>(p, wm + 16 * i, kk, c, q);
+  };
   f32x4 acc[MI][NI];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
+  auto products = [&](const Frags& f) {
 #pragma unroll
-  for (int s = 0; s < ST - 1; ++s)
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] = T::mma(f.b[j], f.a[i], acc[i][j]);
+  };
+  // one LDS read with every other product or so
+  auto interleave = [] {
+    constexpr int READS = MI * (SA::COLS ? 2 : 1) + NI * (SB::COLS ? 2 : 1), PER = MI * NI / READS > 1 ? MI * NI / READS : 1;
+#pragma unroll
+    for (int i = 0; i < READS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // LDS read
+      __builtin_amdgcn_sched_group_barrier(0x008, PER, 0); // MFMA
+    }
+  };
+
+  constexpr int LOADS = SA::LOADS + SB::LOADS;
+  Frags f0, f1;
+#pragma unroll
+  for (int s = 0; s < ST; ++s)
     if (s < nk) issue(s);
-  const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
-  for (int it = 0; it < nk; ++it) {
-    // this wave's loads of the stage have landed, then everyone's; the stage read last is free
-    if (ST > 2 && it + ST - 2 < nk) wait_vm<(ST - 2) * LOADS>();
+  if (nk >= ST) wait_vm<(ST - 1) * LOADS>();
+  else wait_vm<0>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  read(f0, 0, 0);
+  // between two steps: the next stage has landed, and every wave holds the fragments of stage s
+  auto turn = [&](int s) {
+    if (ST > 2 && s + ST - 1 < nk) wait_vm<(ST - 2) * LOADS>();
     else wait_vm<0>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (it + ST - 1 < nk) issue(it + ST - 1);
-    const uint16_t* pa = lds + (it % ST) * (A_EL + B_EL);
-    const uint16_t* pb = pa + A_EL;
-#pragma unroll
-    for (int kk = 0; kk < BK / 32; ++kk) {
-      u32x4 fa[MI], fb[NI];
-#pragma unroll
-      for (int j = 0; j < NI; ++j) fb[j] = fragment<BN, BK, BMODE>(pb, wn + 16 * j, kk, c, q);
-#pragma unroll
-      for (int i = 0; i < MI; ++i) fa[i] = fragment<BM, BK, AMODE>(pa, wm + 16 * i, kk, c, q);
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = T::mma(fb[j], fa[i], acc[i][j]);
+    if (s + ST < nk) issue(s + ST);
+  };
+  if constexpr (BK == 64) {
+    for (int s = 0; s < nk; ++s) {
+      read(f1, s, 1);
+      products(f0);
+      interleave();
+      turn(s);
+      // past the last stage these are stale values that nothing uses
+      read(f0, s + 1, 0);
+      products(f1);
+      interleave();
     }
+  } else {
+    int s = 0;
+    for (; s + 1 < nk; s += 2) {
+      turn(s);
+      read(f1, s + 1, 0);
+      products(f0);
+      interleave();
+      turn(s + 1);
+      read(f0, s + 2, 0);
+      products(f1);
+      interleave();
+    }
+    if (s < nk) products(f0);
   }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   Epi::template run<T, BM, BN, WM, WN, MI, NI>(e, acc, t, m0 + wm, n0 + wn, c, q, wave, lds);
 }
 
@@ -350,7 +398,6 @@ inline Rows rows_of(const maba_tensor* t) {
   Rows r;
   r.p = t ? (uint16_t*)t->data : nullptr;
   r.ld = t ? t->stride[0] : 0;
-  r.vec = t && t->stride[0] % 4 == 0 && (uintptr_t)t->data % 8 == 0;
   return r;
 }
 

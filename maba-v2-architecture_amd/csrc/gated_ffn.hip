@@ -51,18 +51,23 @@ struct EpiGatedBack {
   template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
   static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
                                              int q, int wave, uint16_t* lds) {
+    u32x2 dh[MI][NI / 2];        // all of dh first: the loads are in flight together
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI / 2; ++j) dh[i][j] = load4(e.dh, m0 + 16 * i + c, n0 / 2 + 16 * j + 4 * q, e.M, e.I);
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const int m = m0 + 16 * i + c;
 #pragma unroll
-      for (int j = 0; j < NI; j += 2) {
-        const int n = n0 / 2 + 8 * j + 4 * q;
+      for (int j = 0; j < NI / 2; ++j) {
+        const int n = n0 / 2 + 16 * j + 4 * q;
         if (m >= e.M || n >= e.Ip) continue;
-        const f32x4 g = acc[i][j], u = acc[i][j + 1], dh = load4<T>(e.dh, m, n, e.I);
+        const f32x4 g = acc[i][2 * j], u = acc[i][2 * j + 1], d = up4<T>(dh[i][j]);
         f32x4 dg, du;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float s = sigmoid(g[r]), a = dh[r] * s;
+          const float s = sigmoid(g[r]), a = d[r] * s;
           du[r] = a * g[r];
           dg[r] = a * u[r] * (1.f + g[r] * (1.f - s));
         }
@@ -93,8 +98,10 @@ static GatedPlan gated_plan(const maba_tensor* x, const maba_tensor* scales, con
   p.Ip = pad8(p.I);
   const bool few = !back && p.M <= SKINNY_ROWS;       // that kernel reads any rows
   p.copy_x = !few && (scales || !aligned_rows(x));
-  p.copy_w[0] = !few && !aligned_rows(wg);
-  p.copy_w[1] = !few && !aligned_rows(wu);
+  // dx reads both weights with one stride
+  const bool apart = back && wg->stride[0] != wu->stride[0];
+  p.copy_w[0] = !few && (!aligned_rows(wg) || apart);
+  p.copy_w[1] = !few && (!aligned_rows(wu) || apart);
   Carve c = {(char*)ws, 0};
   if (p.copy_x) p.x = c.take<uint16_t>(p.M * p.Cp);
   for (int i = 0; i < 2; ++i)
@@ -156,7 +163,7 @@ static int gated_backward(GatedPlan& p, const maba_tensor* dh, const maba_tensor
     g.a = ox;
     g.b = ow;
     g.K = p.Cp;
-    const Rows rd = {p.d, 2 * p.Ip, 1};
+    const Rows rd = {p.d, 2 * p.Ip};
     const EpiGatedBack::Args e = {rows_of(dh), rd, (int)p.M, (int)p.I, (int)p.Ip};
     if (int rc = gemm<T, K_ROWS, K_ROWS_PAIR, EpiGatedBack>(g, e, p.M, 2 * ceil_div(p.I, 16) * 16, 1, s, who)) return rc;
   }
@@ -164,10 +171,10 @@ static int gated_backward(GatedPlan& p, const maba_tensor* dh, const maba_tensor
     GemmArgs g = {};
     g.a = d;
     g.b = cols_operand(ow, p.Cp);
-    g.b.ksplit = (int)p.Ip;
-    g.K = 2 * p.Ip;
+    g.K = p.Ip;
+    g.segments = 2;
     const EpiStore::Args e = {rows_of(dx), (int)p.M, (int)p.C};
-    if (int rc = gemm<T, K_ROWS, K_COLS_PAIR, EpiStore>(g, e, p.M, p.C, 1, s, who)) return rc;
+    if (int rc = gemm<T, K_ROWS, K_COLS, EpiStore>(g, e, p.M, p.C, 1, s, who)) return rc;
   }
   if (dwg || dwu) {
     if (p.M > 0) {

@@ -41,25 +41,45 @@ __device__ __forceinline__ float dact_of(float z) {
 template <int ACT>
 struct EpiLinear {
   struct Args { Rows y, res; const uint16_t *bias, *gate; int M, N; };
+  // bias and gate: the quads of their vectors
   template <class T>
-  static __device__ __forceinline__ void quad(const Args& e, int64_t m, int n, f32x4 z, f32x4) {
-    if (e.bias) z += vec4<T>(e.bias, n, e.N);
+  static __device__ __forceinline__ void store(const Args& e, int64_t m, int n, f32x4 z, f32x4 bias, f32x4 gate, u32x2 res) {
+    z += bias;
 #pragma unroll
     for (int r = 0; r < 4; ++r) z[r] = act_of<ACT>(z[r]);
-    if (e.gate) z *= vec4<T>(e.gate, n, e.N);
-    if (e.res.p) z += load4<T>(e.res, m, n, e.N);
-    store4<T>(e.y, m, n, e.N, z);
+    store4<T>(e.y, m, n, e.N, z * gate + up4<T>(res));
+  }
+  template <class T>
+  static __device__ __forceinline__ void vectors(const Args& e, int n, f32x4& bias, f32x4& gate) {
+    bias = f32x4{0.f, 0.f, 0.f, 0.f};
+    gate = f32x4{1.f, 1.f, 1.f, 1.f};
+    if (e.bias) bias = vec4<T>(e.bias, n, e.N);
+    if (e.gate) gate = vec4<T>(e.gate, n, e.N);
+  }
+  template <class T>
+  static __device__ __forceinline__ void quad(const Args& e, int64_t m, int n, f32x4 z, f32x4) {
+    f32x4 bias, gate;
+    vectors<T>(e, n, bias, gate);
+    store<T>(e, m, n, z, bias, gate, e.res.p ? load4(e.res, m, n, e.M, e.N) : u32x2{0, 0});
   }
   template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
   static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
                                              int q, int wave, uint16_t* lds) {
+    u32x2 res[MI][NI];           // all of the residual first: the loads are in flight together
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        res[i][j] = e.res.p ? load4(e.res, m0 + 16 * i + c, n0 + 16 * j + 4 * q, e.M, e.N) : u32x2{0, 0};
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const int n = n0 + 16 * j + 4 * q;
+      f32x4 bias, gate;
+      vectors<T>(e, n, bias, gate);
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const int m = m0 + 16 * i + c;
-        if (m < e.M && n < e.N) quad<T>(e, m, n, acc[i][j], acc[i][j]);
+        if (m < e.M && n < e.N) store<T>(e, m, n, acc[i][j], bias, gate, res[i][j]);
       }
     }
   }
@@ -75,6 +95,11 @@ struct EpiLinearBack {
                                              int q, int wave, uint16_t* lds) {
     float* part = (float*)lds;                    // [WM][2][BN]
     if (e.sums) __syncthreads();                  // the last stage has been read
+    u32x2 dys[MI][NI];                            // all of dy first: the loads are in flight together
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) dys[i][j] = load4(e.dy, m0 + 16 * i + c, n0 + 16 * j + 4 * q, e.M, e.N);
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const int n = n0 + 16 * j + 4 * q;
@@ -85,7 +110,7 @@ struct EpiLinearBack {
       for (int i = 0; i < MI; ++i) {
         const int m = m0 + 16 * i + c;
         if (m >= e.M || n >= e.Np) continue;
-        const f32x4 dy = load4<T>(e.dy, m, n, e.N), z = acc[i][j] + bias;
+        const f32x4 dy = up4<T>(dys[i][j]), z = acc[i][j] + bias;
         f32x4 dz;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -207,7 +232,7 @@ static int make_dz(const LinearPlan& p, const Operand& ox, const Operand& ow, co
   g.a = ox;
   g.b = ow;
   g.K = p.Kp;
-  const Rows dz = {p.dz, p.Np, 1};
+  const Rows dz = {p.dz, p.Np};
   const typename E::Args e = {rows_of(dy), dz, vec_of(bias), vec_of(gate), p.sums, (int)p.M, (int)p.N, (int)p.Np};
   return gemm<T, K_ROWS, K_ROWS, E>(g, e, p.M, p.Np, 1, s, who);
 }
