@@ -411,14 +411,14 @@ int maba_hip_argmax_rows(const maba_tensor* x, maba_tensor* out, void* stream);
  * Backward: dh [M,I]; x as above, or with x_scales its packed form (x: MABA_E4M3 codes [M,C], x_scales:
  * MABA_U8 [M,ceil(C/32)]); any of dx [M,C], dw_gate, dw_up [I,C] may be NULL.  g and u are made again from
  * x; [dg | du] is rounded to 16 bits once, as an operand of the next products.  Results are the same bits
- * on every call.  The query depends on the current device's compute-unit count; with_dw says whether
- * either weight gradient is wanted.
+ * on every call.  The query depends on the current device's compute-unit count; needs: 1 dx, 2 either
+ * weight gradient.
  */
 size_t maba_hip_gated_ffn_workspace_size(const maba_tensor* x, const maba_tensor* w_gate, const maba_tensor* w_up);
 int maba_hip_gated_ffn(const maba_tensor* x, const maba_tensor* w_gate, const maba_tensor* w_up, maba_tensor* out,
                        void* workspace, size_t workspace_bytes, void* stream);
 size_t maba_hip_gated_ffn_backward_workspace_size(const maba_tensor* x, const maba_tensor* x_scales,
-                                                  const maba_tensor* w_gate, const maba_tensor* w_up, int with_dw);
+                                                  const maba_tensor* w_gate, const maba_tensor* w_up, int needs);
 int maba_hip_gated_ffn_backward(const maba_tensor* dh, const maba_tensor* x, const maba_tensor* x_scales,
                                 const maba_tensor* w_gate, const maba_tensor* w_up, maba_tensor* dx, maba_tensor* dw_gate,
                                 maba_tensor* dw_up, void* workspace, size_t workspace_bytes, void* stream);

@@ -2,6 +2,8 @@
 // their tile, operand copies where the core cannot read a tensor in place, and reductions.
 #pragma once
 
+#include <algorithm>
+
 #include "ffn_gemm.h"
 
 namespace maba {
@@ -31,30 +33,59 @@ int column_partials(const maba_tensor* src, float* p, hipStream_t s);
 
 // ---------------------------------------------------------------- launches
 
-constexpr int GEMM_BM = 128, GEMM_BN = 128, GEMM_BK = 64, GEMM_ST = 2;
+// The tiles: BM, BN, waves along m and n, stages in LDS (three and four measured no faster, also where a compute
+// unit has one small tile).
+struct Tile256 { static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, ST = 2; };
+struct Tile192 { static constexpr int BM = 192, BN = 128, WM = 2, WN = 2, ST = 2; };
+struct Tile128 { static constexpr int BM = 128, BN = 128, WM = 2, WN = 2, ST = 2; };
+struct Tile64 { static constexpr int BM = 64, BN = 64, WM = 2, WN = 2, ST = 2; };
+constexpr int GEMM_BK = 64;
 
-template <class T, int AMODE, int BMODE, class Epi>
-int gemm(GemmArgs g, const typename Epi::Args& e, int64_t M, int64_t N, int splits, hipStream_t s, const char* who) {
-  g.tiles_m = (int)ceil_div(M, GEMM_BM);
-  g.tiles_n = (int)ceil_div(N, GEMM_BN);
-  g.splits = splits;
-  if (!g.segments) g.segments = 1;
-  g.k_split = ceil_div(ceil_div(g.K, splits), GEMM_BK) * GEMM_BK;
+// How a product runs: which tile, and into how many runs of stages its sum is split (more than one writes fp32
+// partials that reduce_splits adds).
+struct GemmPlan {
+  int tile, splits, split_stages, tiles_m;
+};
+GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, bool may_split);
+
+template <class T, class Tile, int AMODE, int BMODE, class Epi>
+int gemm_tile(GemmArgs& g, const typename Epi::Args& e, int64_t M, int64_t N, int splits, hipStream_t s, const char* who) {
+  g.tiles_m = (int)ceil_div(M, Tile::BM);
+  g.tiles_n = (int)ceil_div(N, Tile::BN);
   const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * splits;
   if (grid > INT32_MAX) return fail(MABA_ERR_UNSUPPORTED, "%s: too many tiles", who);
-  hipLaunchKernelGGL((gemm_kernel<T, GEMM_BM, GEMM_BN, 2, 2, GEMM_BK, GEMM_ST, AMODE, BMODE, Epi>), dim3((unsigned)grid),
-                     dim3(256), 0, s, g, e);
+  hipLaunchKernelGGL((gemm_kernel<T, Tile::BM, Tile::BN, Tile::WM, Tile::WN, GEMM_BK, Tile::ST, AMODE, BMODE, Epi>),
+                     dim3((unsigned)grid), dim3(64 * Tile::WM * Tile::WN), 0, s, g, e);
   return check_launch(who);
 }
 
-// Splits of a sum over K tokens whose output has M x N elements: enough workgroups for two per
-// compute unit, at least 512 tokens each, and none of them empty.
-inline int k_splits(int64_t M, int64_t N, int64_t K) {
-  const int64_t tiles = ceil_div(M, GEMM_BM) * ceil_div(N, GEMM_BN);
-  int64_t s = std::max<int64_t>(1, std::min<int64_t>(2 * device_cu_count() / std::max<int64_t>(tiles, 1), K / 512));
-  s = std::max<int64_t>(s, 1);
-  const int64_t each = ceil_div(ceil_div(std::max<int64_t>(K, 1), s), GEMM_BK) * GEMM_BK;
-  return (int)ceil_div(std::max<int64_t>(K, 1), each);
+inline int64_t gemm_stages(int64_t K, int segments) { return ceil_div(K, GEMM_BK) * segments; }
+
+template <class T, int AMODE, int BMODE, class Epi>
+int gemm(GemmArgs g, const typename Epi::Args& e, int64_t M, int64_t N, const GemmPlan& p, hipStream_t s, const char* who) {
+  g.segments = g.segments ? g.segments : 1;
+  g.split_stages = p.split_stages;
+  switch (p.tile) {
+    case 0: return gemm_tile<T, Tile256, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
+    case 1: return gemm_tile<T, Tile192, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
+    case 2: return gemm_tile<T, Tile128, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
+    default: return gemm_tile<T, Tile64, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
+  }
+}
+
+// out [M, N] (16 bits) = a product, Np >= N wide with zeros behind N, through fp32 partials where its plan splits it.
+template <class T, int AMODE, int BMODE>
+int product_to(const GemmArgs& g, const maba_tensor* out, int64_t M, int64_t N, int64_t Np, const GemmPlan& p, float* part,
+               hipStream_t s, const char* who) {
+  if (p.splits == 1) {
+    const EpiStore::Args e = {rows_of(out), (int)M, (int)N};
+    return gemm<T, AMODE, BMODE, EpiStore>(g, e, M, Np, p, s, who);
+  }
+  const EpiPartial::Args e = {part, (int)M, (int)Np};
+  if (int rc = gemm<T, AMODE, BMODE, EpiPartial>(g, e, M, Np, p, s, who)) return rc;
+  ReduceArgs r = {part, p.splits, (int)M, (int)Np, (int)M, (int)M, (int)N, {}};
+  r.out[0] = rows_of(out);
+  return reduce_splits(r, T::CODE, s);
 }
 
 // ---------------------------------------------------------------- argument checks

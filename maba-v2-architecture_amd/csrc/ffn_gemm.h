@@ -109,8 +109,8 @@ struct GemmArgs {
   Operand a, b;
   int64_t K;            // of a segment
   int segments;         // 1 or 2
-  int tiles_m, tiles_n, splits;
-  int64_t k_split;      // k of one split, a multiple of the stage depth (one segment only)
+  int tiles_m, tiles_n;
+  int split_stages;     // stages of a split's run of the sum (the last split may have fewer)
 };
 
 constexpr uint32_t OUT_OF_RANGE = 0x80000000u;   // a lane offset past every descriptor's end
@@ -154,7 +154,7 @@ struct Stager {
   int64_t ldb[2];
   int wave, cols;
 
-  __device__ __forceinline__ void init(const Operand& o, const GemmArgs& g, int64_t kbeg, int r0, int wave_, int lane) {
+  __device__ __forceinline__ void init(const Operand& o, const GemmArgs& g, int r0, int wave_, int lane) {
     wave = wave_;
     ldb[0] = o.ld[0] * 2;
     ldb[1] = o.ld[1] * 2;
@@ -165,8 +165,8 @@ struct Stager {
       const int t = MODE == K_ROWS_PAIR ? (wave * RPI >> 4) & 1 : 0;
       const int first = MODE == K_ROWS_PAIR ? r0 / 2 : r0, most = MODE == K_ROWS_PAIR ? R / 2 : R;
       const int rows = min(o.rows - first, most);
-      base[0] = (const char*)(t ? o.p[1] : o.p[0]) + (int64_t)first * ldb[t] + 2 * kbeg;
-      span = rows > 0 ? (uint32_t)((rows - 1) * ldb[t] + 2 * (g.segments * g.K - kbeg)) : 0u;
+      base[0] = (const char*)(t ? o.p[1] : o.p[0]) + (int64_t)first * ldb[t];
+      span = rows > 0 ? (uint32_t)((rows - 1) * ldb[t] + 2 * g.segments * g.K) : 0u;
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         int r = (i * NW + wave) * RPI + lane / CPR;
@@ -186,18 +186,17 @@ struct Stager {
     }
   }
 
-  // k0: the stage's first k of segment seg; kend: the end of this workgroup's k range in it.
-  __device__ __forceinline__ void issue(const Operand& o, const GemmArgs& g, uint16_t* lds, int seg, int64_t k0, int64_t kbeg,
-                                        int64_t kend) {
+  // k0: the stage's first k of segment seg.
+  __device__ __forceinline__ void issue(const Operand& o, const GemmArgs& g, uint16_t* lds, int seg, int64_t k0) {
     const char* p;
     uint32_t bytes, dead = 0;
     if constexpr (!COLS) {
-      const uint32_t adv = 2 * (uint32_t)(seg * g.K + k0 - kbeg);
+      const uint32_t adv = 2 * (uint32_t)(seg * g.K + k0);
       p = base[0] + adv;
       bytes = span > adv ? span - adv : 0u;
-      dead = k0 + 8 * chunk >= kend ? OUT_OF_RANGE : 0u;
+      dead = k0 + 8 * chunk >= g.K ? OUT_OF_RANGE : 0u;
     } else {
-      const int64_t rows = min(min(kend, (int64_t)o.krows) - k0, (int64_t)BK);
+      const int64_t rows = min(min(g.K, (int64_t)o.krows) - k0, (int64_t)BK);
       p = base[seg] + k0 * ldb[0];
       bytes = (uint32_t)((rows - 1) * ldb[0] + cols);
     }
@@ -260,20 +259,20 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) 
   const int c = lane & 15, q = lane >> 4;
   const TileId t = tile_of(g);
   const int m0 = t.m * BM, n0 = t.n * BN;
-  const int64_t kbeg = t.split * g.k_split, kend = min(g.K, kbeg + g.k_split);
-  const int nk1 = (int)((kend - kbeg + BK - 1) / BK), nk = nk1 * g.segments;     // stages of a segment, of all
+  const int nk1 = (int)((g.K + BK - 1) / BK);                                    // stages of a segment
+  const int s0 = t.split * g.split_stages, nk = min(nk1 * g.segments - s0, g.split_stages);
   const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
 
   SA sa;
   SB sb;
-  sa.init(g.a, g, kbeg, m0, wave, lane);
-  sb.init(g.b, g, kbeg, n0, wave, lane);
+  sa.init(g.a, g, m0, wave, lane);
+  sb.init(g.b, g, n0, wave, lane);
   auto issue = [&](int s) {
     uint16_t* p = lds + (s % ST) * STAGE;
-    const int seg = s >= nk1;
-    const int64_t k0 = kbeg + (int64_t)(s - seg * nk1) * BK;
-    sa.issue(g.a, g, p, seg, k0, kbeg, kend);
-    sb.issue(g.b, g, p + A_EL, seg, k0, kbeg, kend);
+    const int seg = s0 + s >= nk1;
+    const int64_t k0 = (int64_t)(s0 + s - seg * nk1) * BK;
+    sa.issue(g.a, g, p, seg, k0);
+    sb.issue(g.b, g, p + A_EL, seg, k0);
   };
   struct Frags { u32x4 a[MI], b[NI]; };
   auto read = [&](Frags& f, int s, int kk) {

@@ -83,13 +83,13 @@ struct GatedPlan {
   int64_t M, C, I, Cp, Ip;
   bool copy_x, copy_w[2];
   uint16_t *x, *w[2], *d;
-  float* part;
-  int splits;
+  float* part;             // fp32 partials, of dx and then of the weights
+  GemmPlan gu, dx, dw;     // the products with both weights, for dx and for the weights' gradients
   size_t bytes;
 };
 
 static GatedPlan gated_plan(const maba_tensor* x, const maba_tensor* scales, const maba_tensor* wg, const maba_tensor* wu,
-                            bool back, bool dw, void* ws) {
+                            bool back, bool dx, bool dw, void* ws) {
   GatedPlan p = {};
   p.M = x->shape[0];
   p.C = x->shape[1];
@@ -108,11 +108,18 @@ static GatedPlan gated_plan(const maba_tensor* x, const maba_tensor* scales, con
     if (p.copy_w[i]) p.w[i] = c.take<uint16_t>(p.I * p.Cp);
   if (back) {
     p.d = c.take<uint16_t>(p.M * 2 * p.Ip);
-    if (dw) {
-      p.splits = k_splits(2 * p.Ip, p.Cp, p.M);
-      p.part = c.take<float>((int64_t)p.splits * 2 * p.Ip * p.Cp);
+    int64_t part = 0;
+    if (dx) {
+      p.dx = gemm_plan(p.M, p.Cp, gemm_stages(p.Ip, 2), true);
+      if (p.dx.splits > 1) part = (int64_t)p.dx.splits * p.M * p.Cp;
     }
+    if (dw) {
+      p.dw = gemm_plan(2 * p.Ip, p.Cp, gemm_stages(p.M, 1), true);
+      part = std::max(part, (int64_t)p.dw.splits * 2 * p.Ip * p.Cp);
+    }
+    p.part = c.take<float>(part);
   }
+  p.gu = gemm_plan(p.M, 2 * ceil_div(p.I, 16) * 16, gemm_stages(p.Cp, 1), false);
   p.bytes = c.used;
   return p;
 }
@@ -148,7 +155,7 @@ static int gated_forward(GatedPlan& p, const maba_tensor* x, const maba_tensor* 
   GemmArgs g = {};
   if (int rc = gated_operands(p, x, nullptr, wg, wu, s, g.a, g.b)) return rc;
   g.K = p.Cp;
-  return gemm<T, K_ROWS, K_ROWS_PAIR, EpiGated>(g, e, p.M, 2 * ceil_div(p.I, 16) * 16, 1, s, who);
+  return gemm<T, K_ROWS, K_ROWS_PAIR, EpiGated>(g, e, p.M, 2 * ceil_div(p.I, 16) * 16, p.gu, s, who);
 }
 
 template <class T>
@@ -165,7 +172,7 @@ static int gated_backward(GatedPlan& p, const maba_tensor* dh, const maba_tensor
     g.K = p.Cp;
     const Rows rd = {p.d, 2 * p.Ip};
     const EpiGatedBack::Args e = {rows_of(dh), rd, (int)p.M, (int)p.I, (int)p.Ip};
-    if (int rc = gemm<T, K_ROWS, K_ROWS_PAIR, EpiGatedBack>(g, e, p.M, 2 * ceil_div(p.I, 16) * 16, 1, s, who)) return rc;
+    if (int rc = gemm<T, K_ROWS, K_ROWS_PAIR, EpiGatedBack>(g, e, p.M, 2 * ceil_div(p.I, 16) * 16, p.gu, s, who)) return rc;
   }
   if (dx && p.M > 0) {
     GemmArgs g = {};
@@ -173,8 +180,7 @@ static int gated_backward(GatedPlan& p, const maba_tensor* dh, const maba_tensor
     g.b = cols_operand(ow, p.Cp);
     g.K = p.Ip;
     g.segments = 2;
-    const EpiStore::Args e = {rows_of(dx), (int)p.M, (int)p.C};
-    if (int rc = gemm<T, K_ROWS, K_COLS, EpiStore>(g, e, p.M, p.C, 1, s, who)) return rc;
+    if (int rc = product_to<T, K_ROWS, K_COLS>(g, dx, p.M, p.C, p.Cp, p.dx, p.part, s, who)) return rc;
   }
   if (dwg || dwu) {
     if (p.M > 0) {
@@ -183,9 +189,9 @@ static int gated_backward(GatedPlan& p, const maba_tensor* dh, const maba_tensor
       g.b = cols_operand(ox, p.Cp);
       g.K = p.M;
       const EpiPartial::Args e = {p.part, (int)(2 * p.Ip), (int)p.Cp};
-      if (int rc = gemm<T, K_COLS, K_COLS, EpiPartial>(g, e, 2 * p.Ip, p.Cp, p.splits, s, who)) return rc;
+      if (int rc = gemm<T, K_COLS, K_COLS, EpiPartial>(g, e, 2 * p.Ip, p.Cp, p.dw, s, who)) return rc;
     }
-    ReduceArgs r = {p.part, p.M > 0 ? p.splits : 0, (int)(2 * p.Ip), (int)p.Cp, (int)p.Ip, (int)p.I, (int)p.C, {}};
+    ReduceArgs r = {p.part, p.M > 0 ? p.dw.splits : 0, (int)(2 * p.Ip), (int)p.Cp, (int)p.Ip, (int)p.I, (int)p.C, {}};
     r.out[0] = rows_of(dwg);
     r.out[1] = rows_of(dwu);
     if (int rc = reduce_splits(r, wg->dtype, s)) return rc;
@@ -215,7 +221,7 @@ using namespace maba::ffn;
 
 extern "C" size_t maba_hip_gated_ffn_workspace_size(const maba_tensor* x, const maba_tensor* w_gate, const maba_tensor* w_up) {
   if (gated_check(x, nullptr, w_gate, w_up, "gated_ffn")) return 0;
-  return gated_plan(x, nullptr, w_gate, w_up, false, false, nullptr).bytes;
+  return gated_plan(x, nullptr, w_gate, w_up, false, false, false, nullptr).bytes;
 }
 
 extern "C" int maba_hip_gated_ffn(const maba_tensor* x, const maba_tensor* w_gate, const maba_tensor* w_up, maba_tensor* out,
@@ -225,7 +231,7 @@ extern "C" int maba_hip_gated_ffn(const maba_tensor* x, const maba_tensor* w_gat
   if (!rc) rc = check_out(out, who, "out", w_gate->dtype, x->shape[0], w_gate->shape[0]);
   if (rc) return rc;
   if (overlap(out, x) || overlap(out, w_gate) || overlap(out, w_up)) return fail(MABA_ERR_INVALID, "%s: out overlaps an input", who);
-  GatedPlan p = gated_plan(x, nullptr, w_gate, w_up, false, false, workspace);
+  GatedPlan p = gated_plan(x, nullptr, w_gate, w_up, false, false, false, workspace);
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
     return fail(MABA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, p.bytes);
   if (p.M == 0) return MABA_OK;
@@ -234,9 +240,9 @@ extern "C" int maba_hip_gated_ffn(const maba_tensor* x, const maba_tensor* w_gat
 }
 
 extern "C" size_t maba_hip_gated_ffn_backward_workspace_size(const maba_tensor* x, const maba_tensor* x_scales,
-                                                             const maba_tensor* w_gate, const maba_tensor* w_up, int with_dw) {
+                                                             const maba_tensor* w_gate, const maba_tensor* w_up, int needs) {
   if (gated_check(x, x_scales, w_gate, w_up, "gated_ffn_backward")) return 0;
-  return gated_plan(x, x_scales, w_gate, w_up, true, with_dw != 0, nullptr).bytes;
+  return gated_plan(x, x_scales, w_gate, w_up, true, needs & 1, needs & 2, nullptr).bytes;
 }
 
 extern "C" int maba_hip_gated_ffn_backward(const maba_tensor* dh, const maba_tensor* x, const maba_tensor* x_scales,
@@ -260,7 +266,7 @@ extern "C" int maba_hip_gated_ffn_backward(const maba_tensor* dh, const maba_ten
     for (int j = 0; j < i; ++j)
       if (overlap(outs[i], outs[j])) return fail(MABA_ERR_INVALID, "%s: two gradients overlap", who);
   }
-  GatedPlan p = gated_plan(x, x_scales, w_gate, w_up, true, dw_gate || dw_up, workspace);
+  GatedPlan p = gated_plan(x, x_scales, w_gate, w_up, true, dx != nullptr, dw_gate || dw_up, workspace);
   if (!workspace ? p.bytes > 0 : workspace_bytes < p.bytes)
     return fail(MABA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, p.bytes);
   return dt == MABA_BF16 ? gated_backward<Bf16>(p, dh, x, x_scales, w_gate, w_up, dx, dw_gate, dw_up, (hipStream_t)stream, who)

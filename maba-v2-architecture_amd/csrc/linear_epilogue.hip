@@ -154,7 +154,7 @@ struct LinearPlan {
   bool copy_x, copy_w, copy_dy, z;      // z: dz is made from z, otherwise it is dy
   uint16_t *x, *w, *dz;
   float *part, *sums;
-  int splits;
+  GemmPlan xw, dx, dw;                  // the products x W^T, dz W and dz^T x
   size_t bytes;
 };
 
@@ -180,19 +180,25 @@ static LinearPlan linear_plan(const maba_tensor* x, const maba_tensor* scales, c
   if (p.copy_w) p.w = c.take<uint16_t>(p.N * p.Kp);
   if (need) {
     if (p.z || p.copy_dy) p.dz = c.take<uint16_t>(p.M * p.Np);
-    if (need->dbias || need->dgate) {
-      p.sum_rows = ceil_div(p.M, 128);
-      p.sums = c.take<float>(p.sum_rows * 2 * p.N);
+    int64_t part = 0;
+    if (need->dx) {
+      p.dx = gemm_plan(p.M, p.Kp, gemm_stages(p.Np, 1), true);
+      if (p.dx.splits > 1) part = (int64_t)p.dx.splits * p.M * p.Kp;
     }
     if (need->dw) {
-      p.splits = k_splits(p.Np, p.Kp, p.M);
-      p.part = c.take<float>((int64_t)p.splits * p.Np * p.Kp);
+      p.dw = gemm_plan(p.Np, p.Kp, gemm_stages(p.M, 1), true);
+      part = std::max(part, (int64_t)p.dw.splits * p.Np * p.Kp);
     }
+    p.part = c.take<float>(part);
+  }
+  p.xw = gemm_plan(p.M, p.Np, gemm_stages(p.Kp, 1), false);
+  if (need && (need->dbias || need->dgate)) {
+    p.sum_rows = p.z ? p.xw.tiles_m : ceil_div(p.M, 128);     // a tile's rows, or those of column_partials
+    p.sums = c.take<float>(p.sum_rows * 2 * p.N);
   }
   p.bytes = c.used;
   return p;
 }
-static_assert(GEMM_BM == 128, "column sums are kept for 128 rows at a time");
 
 static int linear_operands(LinearPlan& p, const maba_tensor* x, const maba_tensor* scales, const maba_tensor* w, hipStream_t s,
                            Operand& ox, Operand& ow) {
@@ -221,7 +227,7 @@ static int linear_forward(LinearPlan& p, const maba_tensor* x, const maba_tensor
   GemmArgs g = {};
   if (int rc = linear_operands(p, x, nullptr, w, s, g.a, g.b)) return rc;
   g.K = p.Kp;
-  return gemm<T, K_ROWS, K_ROWS, E>(g, e, p.M, p.N, 1, s, who);
+  return gemm<T, K_ROWS, K_ROWS, E>(g, e, p.M, p.Np, p.xw, s, who);
 }
 
 template <class T, int ACT>
@@ -234,7 +240,7 @@ static int make_dz(const LinearPlan& p, const Operand& ox, const Operand& ow, co
   g.K = p.Kp;
   const Rows dz = {p.dz, p.Np};
   const typename E::Args e = {rows_of(dy), dz, vec_of(bias), vec_of(gate), p.sums, (int)p.M, (int)p.N, (int)p.Np};
-  return gemm<T, K_ROWS, K_ROWS, E>(g, e, p.M, p.Np, 1, s, who);
+  return gemm<T, K_ROWS, K_ROWS, E>(g, e, p.M, p.Np, p.xw, s, who);
 }
 
 template <class T>
@@ -265,8 +271,7 @@ static int linear_backward(LinearPlan& p, const maba_tensor* dy, const maba_tens
     g.a = dz;
     g.b = cols_operand(ow, p.Kp);
     g.K = p.Np;                 // dz is N wide where N is a whole number of chunks, padded with zeros otherwise
-    const EpiStore::Args e = {rows_of(dx), (int)p.M, (int)p.K};
-    if (int rc = gemm<T, K_ROWS, K_COLS, EpiStore>(g, e, p.M, p.K, 1, s, who)) return rc;
+    if (int rc = product_to<T, K_ROWS, K_COLS>(g, dx, p.M, p.K, p.Kp, p.dx, p.part, s, who)) return rc;
   }
   if (dw) {
     if (p.M > 0) {
@@ -275,9 +280,9 @@ static int linear_backward(LinearPlan& p, const maba_tensor* dy, const maba_tens
       g.b = cols_operand(ox, p.Kp);
       g.K = p.M;
       const EpiPartial::Args e = {p.part, (int)p.Np, (int)p.Kp};
-      if (int rc = gemm<T, K_COLS, K_COLS, EpiPartial>(g, e, p.Np, p.Kp, p.splits, s, who)) return rc;
+      if (int rc = gemm<T, K_COLS, K_COLS, EpiPartial>(g, e, p.Np, p.Kp, p.dw, s, who)) return rc;
     }
-    ReduceArgs r = {p.part, p.M > 0 ? p.splits : 0, (int)p.Np, (int)p.Kp, (int)p.Np, (int)p.N, (int)p.K, {}};
+    ReduceArgs r = {p.part, p.M > 0 ? p.dw.splits : 0, (int)p.Np, (int)p.Kp, (int)p.Np, (int)p.N, (int)p.K, {}};
     r.out[0] = rows_of(dw);
     if (int rc = reduce_splits(r, w->dtype, s)) return rc;
   }

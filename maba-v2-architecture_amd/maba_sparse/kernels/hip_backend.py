@@ -344,7 +344,7 @@ def hip_gated_ffn_backward(dh, x, w_gate, w_up, x_scales=None, needs=(True, True
         dx = torch.empty(x2.shape, dtype=dt, device=dev) if needs[0] else None
         dws = [torch.empty(w_gate.shape, dtype=dt, device=dev) if n else None for n in needs[1:3]]
         ddx, dsc, dg, du = N.desc(x2), N.desc(sc), N.desc(_rows(w_gate)), N.desc(_rows(w_up))
-        ws = _workspace(lib.maba_hip_gated_ffn_backward_workspace_size(ddx, dsc, dg, du, int(any(needs[1:3]))), dev)
+        ws = _workspace(lib.maba_hip_gated_ffn_backward_workspace_size(ddx, dsc, dg, du, bool(needs[0]) + 2 * any(needs[1:3])), dev)
         rc = lib.maba_hip_gated_ffn_backward(N.desc(_rows(dh)), ddx, dsc, dg, du, N.desc(dx), N.desc(dws[0]),
                                              N.desc(dws[1]), ws.data_ptr(), ws.numel(), N.stream_ptr(dev))
         N.check(rc, "gated_ffn_backward")
