@@ -46,7 +46,8 @@ constexpr int GEMM_BK = 64;
 struct GemmPlan {
   int tile, splits, split_stages, tiles_m;
 };
-GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, bool may_split);
+// columns: an operand is read along its columns.
+GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, bool columns, bool may_split);
 
 template <class T, class Tile, int AMODE, int BMODE, class Epi>
 int gemm_tile(GemmArgs& g, const typename Epi::Args& e, int64_t M, int64_t N, int splits, hipStream_t s, const char* who) {

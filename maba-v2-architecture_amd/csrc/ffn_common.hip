@@ -6,19 +6,24 @@
 namespace maba {
 namespace ffn {
 
-// The plan is the least of a sum's estimated times over the tiles and splits.  A compute unit that holds `slots` tiles at
-// once takes, for a stage of each, the longer of one tile's latency (`lone`) and of all their work (`full` each), and
-// `ends` a tile for its first loads and its epilogue.  Measured on MI355X, us:
-//              256 x 256   192 x 128   128 x 128   64 x 64
-//   full         1.5          0.68        0.56       0.25     (per element 23, 28, 34 and 61 ps: larger tiles move less
-//   lone         1.5          0.9         0.72       0.42      through LDS, smaller ones fill the chip sooner)
-// (4,096 x 11,008 x 2,048: 167, 189, 223 us with the first three; 16,384 x 640 x 2,496: 85, 61, 89; 2,048 x 2,496 x 640:
-// 20, 14.3, 14.3 and 16.7; 64 x 640 x 2,496 with the last, in 1, 4 and 8 splits: 19.9, 7.2 and 5.2.)
-struct TileCost { int bm, bn, slots; float full, lone, ends; };
-static const TileCost TILES[4] = {{256, 256, 1, 1.5f, 1.5f, 7.f}, {192, 128, 2, 0.68f, 0.9f, 2.f}, {128, 128, 2, 0.56f, 0.72f, 1.5f},
-                                  {64, 64, 4, 0.25f, 0.42f, 0.8f}};
+// The plan is the least of a sum's estimated times over the tiles and splits.  A compute unit with n tiles takes for
+// each its stages at `full` and `ends` for its first loads and its epilogue; with fewer than `slots`, which is what it
+// holds at once, a stage's latency (`lone`) bounds it.  Measured on MI355X, us, with an operand read along its columns
+// in brackets:
+//              256 x 256      192 x 128      128 x 128      64 x 64
+//   full       1.36 (1.72)    0.55 (0.66)    0.41 (0.53)    0.20 (0.25)
+//   lone       1.36 (1.72)    0.80 (1.00)    0.60 (0.74)    0.36 (0.47)
+//   ends       7.6            4              3              0.75
+// (4,096 x 11,008 x 2,048, rows: 154, 172, 178 us with the first three; 16,384 x 640 x 2,496, columns: 83, 62, 88;
+// 2,048 x 2,496 x 640, rows: 20, 14.3, 14.3 and 16.7; 64 x 640 x 2,496 with the last, in 1, 4 and 8 splits: 19.9,
+// 7.2 and 5.2.)
+struct TileCost { int bm, bn, slots; float full[2], lone[2], ends; };
+static const TileCost TILES[4] = {{256, 256, 1, {1.36f, 1.72f}, {1.36f, 1.72f}, 7.6f},
+                                  {192, 128, 2, {0.55f, 0.66f}, {0.80f, 1.00f}, 4.f},
+                                  {128, 128, 2, {0.41f, 0.53f}, {0.60f, 0.74f}, 3.f},
+                                  {64, 64, 5, {0.20f, 0.25f}, {0.36f, 0.47f}, 0.75f}};
 
-GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, bool may_split) {
+GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, bool columns, bool may_split) {
   const int64_t cus = device_cu_count();
   GemmPlan best = {3, 1, (int)stages, 0};
   float least = 0.f;
@@ -29,9 +34,9 @@ GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, bool may_split) {
     for (int want = 1; want <= most; ++want) {
       const int64_t per = ceil_div(stages, want), splits = ceil_div(stages, per);
       if (splits != want) continue;
-      const int64_t n = ceil_div(tiles * splits, cus), rounds = n / t.slots, rest = n % t.slots;
-      float us = rounds * (per * std::max(t.lone, t.slots * t.full) + t.ends);
-      if (rest) us += per * std::max(t.lone, rest * t.full) + t.ends;
+      const int64_t n = ceil_div(tiles * splits, cus);
+      float us = n * (per * t.full[columns] + t.ends);
+      if (n < t.slots) us = std::max(us, per * t.lone[columns] + t.ends);
       if (splits > 1) us += 2.5f + (float)(M * N) * (4.f * splits + 2.f) / 5e6f;     // reduce_splits, at 5 TB/s
       if (least == 0.f || us < least) {
         least = us;

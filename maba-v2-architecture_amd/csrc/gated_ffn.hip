@@ -21,14 +21,18 @@
 namespace maba {
 namespace ffn {
 
+// A wave's 32 columns of a tile are 16 of g and the same 16 of u; the epilogues take four such blocks at once.
 struct EpiGated {
   struct Args { Rows h; int M, I; };
-  template <class T>
-  static __device__ __forceinline__ void quad(const Args& e, int64_t m, int n, f32x4 g, f32x4 u) {
+  static __device__ __forceinline__ f32x4 gated(f32x4 g, f32x4 u) {
     f32x4 v;
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = g[r] * sigmoid(g[r]) * u[r];
-    store4<T>(e.h, m, n, e.I, v);
+    return v;
+  }
+  template <class T>
+  static __device__ __forceinline__ void quad(const Args& e, int64_t m, int n, f32x4 g, f32x4 u) {
+    store4<T>(e.h, m, n, e.I, gated(g, u));
   }
   template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
   static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
@@ -36,10 +40,17 @@ struct EpiGated {
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const int m = m0 + 16 * i + c;
+      if constexpr (NI % 4 == 0) {
 #pragma unroll
-      for (int j = 0; j < NI; j += 2) {
-        const int n = n0 / 2 + 8 * j + 4 * q;
-        if (m < e.M && n < e.I) quad<T>(e, m, n, acc[i][j], acc[i][j + 1]);
+        for (int j = 0; j < NI; j += 4)
+          store8(e.h, m, n0 / 2 + 8 * j + 8 * q, e.M, e.I,
+                 eight_of({down4<T>(gated(acc[i][j], acc[i][j + 1])), down4<T>(gated(acc[i][j + 2], acc[i][j + 3]))}));
+      } else {
+#pragma unroll
+        for (int j = 0; j < NI; j += 2) {
+          const int n = n0 / 2 + 8 * j + 4 * q;
+          if (m < e.M && n < e.I) quad<T>(e, m, n, acc[i][j], acc[i][j + 1]);
+        }
       }
     }
   }
@@ -48,31 +59,52 @@ struct EpiGated {
 // d [M, 2 Ip], Ip = I rounded up to 8: dg at column 0, du at column Ip, zeros behind each.
 struct EpiGatedBack {
   struct Args { Rows dh, d; int M, I, Ip; };
+  static __device__ __forceinline__ void grads(f32x4 g, f32x4 u, f32x4 dh, f32x4& dg, f32x4& du) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float s = sigmoid(g[r]), a = dh[r] * s;
+      du[r] = a * g[r];
+      dg[r] = a * u[r] * (1.f + g[r] * (1.f - s));
+    }
+  }
   template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
   static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
                                              int q, int wave, uint16_t* lds) {
-    u32x2 dh[MI][NI / 2];        // all of dh first: the loads are in flight together
+    if constexpr (NI % 4 == 0) {
+      u32x4 dh[MI][NI / 4];      // all of dh first: the loads are in flight together
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+      for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int j = 0; j < NI / 2; ++j) dh[i][j] = load4(e.dh, m0 + 16 * i + c, n0 / 2 + 16 * j + 4 * q, e.M, e.I);
+        for (int j = 0; j < NI / 4; ++j) dh[i][j] = load8(e.dh, m0 + 16 * i + c, n0 / 2 + 32 * j + 8 * q, e.M, e.I);
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int m = m0 + 16 * i + c;
+      for (int i = 0; i < MI; ++i) {
+        const int m = m0 + 16 * i + c;
 #pragma unroll
-      for (int j = 0; j < NI / 2; ++j) {
-        const int n = n0 / 2 + 16 * j + 4 * q;
-        if (m >= e.M || n >= e.Ip) continue;
-        const f32x4 g = acc[i][2 * j], u = acc[i][2 * j + 1], d = up4<T>(dh[i][j]);
-        f32x4 dg, du;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float s = sigmoid(g[r]), a = d[r] * s;
-          du[r] = a * g[r];
-          dg[r] = a * u[r] * (1.f + g[r] * (1.f - s));
+        for (int j = 0; j < NI / 4; ++j) {
+          const int n = n0 / 2 + 32 * j + 8 * q;
+          const Quads d = quads_of(dh[i][j]);
+          f32x4 dg[2], du[2];
+          grads(acc[i][4 * j], acc[i][4 * j + 1], up4<T>(d.a), dg[0], du[0]);
+          grads(acc[i][4 * j + 2], acc[i][4 * j + 3], up4<T>(d.b), dg[1], du[1]);
+          store8(e.d, m, n, e.M, e.Ip, eight_of({down4<T>(dg[0]), down4<T>(dg[1])}));
+          // columns behind Ip would be du's neighbours: none is stored there
+          const u32x4 u = eight_of({down4<T>(du[0]), down4<T>(du[1])});
+          if (n < e.Ip) store8(e.d, m, e.Ip + n, e.M, 2 * e.Ip, u);
         }
-        store4<T>(e.d, m, n, e.Ip, dg);
-        store4<T>(e.d, m, e.Ip + n, 2 * e.Ip, du);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int m = m0 + 16 * i + c;
+#pragma unroll
+        for (int j = 0; j < NI; j += 2) {
+          const int n = n0 / 2 + 8 * j + 4 * q;
+          if (m >= e.M || n >= e.Ip) continue;
+          f32x4 dg, du;
+          grads(acc[i][j], acc[i][j + 1], up4<T>(load4(e.dh, m, n, e.I)), dg, du);
+          store4<T>(e.d, m, n, e.Ip, dg);
+          store4<T>(e.d, m, e.Ip + n, 2 * e.Ip, du);
+        }
       }
     }
   }
@@ -110,16 +142,16 @@ static GatedPlan gated_plan(const maba_tensor* x, const maba_tensor* scales, con
     p.d = c.take<uint16_t>(p.M * 2 * p.Ip);
     int64_t part = 0;
     if (dx) {
-      p.dx = gemm_plan(p.M, p.Cp, gemm_stages(p.Ip, 2), true);
+      p.dx = gemm_plan(p.M, p.Cp, gemm_stages(p.Ip, 2), true, true);
       if (p.dx.splits > 1) part = (int64_t)p.dx.splits * p.M * p.Cp;
     }
     if (dw) {
-      p.dw = gemm_plan(2 * p.Ip, p.Cp, gemm_stages(p.M, 1), true);
+      p.dw = gemm_plan(2 * p.Ip, p.Cp, gemm_stages(p.M, 1), true, true);
       part = std::max(part, (int64_t)p.dw.splits * 2 * p.Ip * p.Cp);
     }
     p.part = c.take<float>(part);
   }
-  p.gu = gemm_plan(p.M, 2 * ceil_div(p.I, 16) * 16, gemm_stages(p.Cp, 1), false);
+  p.gu = gemm_plan(p.M, 2 * ceil_div(p.I, 16) * 16, gemm_stages(p.Cp, 1), false, false);
   p.bytes = c.used;
   return p;
 }

@@ -38,48 +38,49 @@ __device__ __forceinline__ float dact_of(float z) {
   } else return 1.f;
 }
 
+// The quads of the bias (zeros without one) and the gate (ones).
+template <class T>
+__device__ __forceinline__ f32x4 bias4(const uint16_t* p, int n, int nend) {
+  return p ? vec4<T>(p, n, nend) : f32x4{0.f, 0.f, 0.f, 0.f};
+}
+template <class T>
+__device__ __forceinline__ f32x4 gate4(const uint16_t* p, int n, int nend) {
+  return p ? vec4<T>(p, n, nend) : f32x4{1.f, 1.f, 1.f, 1.f};
+}
+
 template <int ACT>
 struct EpiLinear {
   struct Args { Rows y, res; const uint16_t *bias, *gate; int M, N; };
-  // bias and gate: the quads of their vectors
-  template <class T>
-  static __device__ __forceinline__ void store(const Args& e, int64_t m, int n, f32x4 z, f32x4 bias, f32x4 gate, u32x2 res) {
+  static __device__ __forceinline__ f32x4 value(f32x4 z, f32x4 bias, f32x4 gate, f32x4 res) {
     z += bias;
 #pragma unroll
     for (int r = 0; r < 4; ++r) z[r] = act_of<ACT>(z[r]);
-    store4<T>(e.y, m, n, e.N, z * gate + up4<T>(res));
-  }
-  template <class T>
-  static __device__ __forceinline__ void vectors(const Args& e, int n, f32x4& bias, f32x4& gate) {
-    bias = f32x4{0.f, 0.f, 0.f, 0.f};
-    gate = f32x4{1.f, 1.f, 1.f, 1.f};
-    if (e.bias) bias = vec4<T>(e.bias, n, e.N);
-    if (e.gate) gate = vec4<T>(e.gate, n, e.N);
+    return z * gate + res;
   }
   template <class T>
   static __device__ __forceinline__ void quad(const Args& e, int64_t m, int n, f32x4 z, f32x4) {
-    f32x4 bias, gate;
-    vectors<T>(e, n, bias, gate);
-    store<T>(e, m, n, z, bias, gate, e.res.p ? load4(e.res, m, n, e.M, e.N) : u32x2{0, 0});
+    const u32x2 res = e.res.p ? load4(e.res, m, n, e.N) : u32x2{0, 0};
+    store4<T>(e.y, m, n, e.N, value(z, bias4<T>(e.bias, n, e.N), gate4<T>(e.gate, n, e.N), up4<T>(res)));
   }
   template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
   static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
                                              int q, int wave, uint16_t* lds) {
-    u32x2 res[MI][NI];           // all of the residual first: the loads are in flight together
+    u32x4 res[MI][NI / 2];       // all of the residual first: the loads are in flight together
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int j = 0; j < NI; ++j)
-        res[i][j] = e.res.p ? load4(e.res, m0 + 16 * i + c, n0 + 16 * j + 4 * q, e.M, e.N) : u32x2{0, 0};
+      for (int j = 0; j < NI / 2; ++j)
+        res[i][j] = e.res.p ? load8(e.res, m0 + 16 * i + c, n0 + 32 * j + 8 * q, e.M, e.N) : u32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int n = n0 + 16 * j + 4 * q;
-      f32x4 bias, gate;
-      vectors<T>(e, n, bias, gate);
+    for (int j = 0; j < NI / 2; ++j) {
+      const int n = n0 + 32 * j;
+      const f32x4 ba = bias4<T>(e.bias, n + 4 * q, e.N), bb = bias4<T>(e.bias, n + 16 + 4 * q, e.N);
+      const f32x4 ga = gate4<T>(e.gate, n + 4 * q, e.N), gb = gate4<T>(e.gate, n + 16 + 4 * q, e.N);
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
-        const int m = m0 + 16 * i + c;
-        if (m < e.M && n < e.N) store<T>(e, m, n, acc[i][j], bias, gate, res[i][j]);
+        const Quads r = quads_of(res[i][j]);
+        const f32x4 a = value(acc[i][2 * j], ba, ga, up4<T>(r.a)), b = value(acc[i][2 * j + 1], bb, gb, up4<T>(r.b));
+        store8(e.y, m0 + 16 * i + c, n + 8 * q, e.M, e.N, eight_of({down4<T>(a), down4<T>(b)}));
       }
     }
   }
@@ -90,49 +91,62 @@ struct EpiLinear {
 template <int ACT>
 struct EpiLinearBack {
   struct Args { Rows dy, dz; const uint16_t *bias, *gate; float* sums; int M, N, Np; };
+  // dz, and its terms and those of dy * act(z) added to the column sums.  dy is zero behind the last row.
+  static __device__ __forceinline__ f32x4 value(f32x4 z, f32x4 dy, f32x4 bias, f32x4 gate, f32x4& sb, f32x4& sg, bool in) {
+    f32x4 dz;
+    z += bias;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      dz[r] = dy[r] * gate[r] * dact_of<ACT>(z[r]);
+      sg[r] += in ? dy[r] * act_of<ACT>(z[r]) : 0.f;
+      sb[r] += in ? dz[r] : 0.f;
+    }
+    return dz;
+  }
   template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
   static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
                                              int q, int wave, uint16_t* lds) {
     float* part = (float*)lds;                    // [WM][2][BN]
     if (e.sums) __syncthreads();                  // the last stage has been read
-    u32x2 dys[MI][NI];                            // all of dy first: the loads are in flight together
+    u32x4 dys[MI][NI / 2];                        // all of dy first: the loads are in flight together
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int j = 0; j < NI; ++j) dys[i][j] = load4(e.dy, m0 + 16 * i + c, n0 + 16 * j + 4 * q, e.M, e.N);
+      for (int j = 0; j < NI / 2; ++j) dys[i][j] = load8(e.dy, m0 + 16 * i + c, n0 + 32 * j + 8 * q, e.M, e.N);
 #pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int n = n0 + 16 * j + 4 * q;
-      f32x4 gate = {1.f, 1.f, 1.f, 1.f}, bias = {0.f, 0.f, 0.f, 0.f}, sb = bias, sg = bias;
-      if (e.gate) gate = vec4<T>(e.gate, n, e.N);
-      if (e.bias) bias = vec4<T>(e.bias, n, e.N);
+    for (int j = 0; j < NI / 2; ++j) {
+      f32x4 bias[2], gate[2], sb[2], sg[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int n = n0 + 32 * j + 16 * h + 4 * q;
+        bias[h] = bias4<T>(e.bias, n, e.N);
+        gate[h] = gate4<T>(e.gate, n, e.N);
+        sb[h] = sg[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const int m = m0 + 16 * i + c;
-        if (m >= e.M || n >= e.Np) continue;
-        const f32x4 dy = up4<T>(dys[i][j]), z = acc[i][j] + bias;
-        f32x4 dz;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          dz[r] = dy[r] * gate[r] * dact_of<ACT>(z[r]);
-          sg[r] += dy[r] * act_of<ACT>(z[r]);
-        }
-        sb += dz;
-        store4<T>(e.dz, m, n, e.Np, dz);
+        const Quads d = quads_of(dys[i][j]);
+        const f32x4 a = value(acc[i][2 * j], up4<T>(d.a), bias[0], gate[0], sb[0], sg[0], m < e.M);
+        const f32x4 b = value(acc[i][2 * j + 1], up4<T>(d.b), bias[1], gate[1], sb[1], sg[1], m < e.M);
+        store8(e.dz, m, n0 + 32 * j + 8 * q, e.M, e.Np, eight_of({down4<T>(a), down4<T>(b)}));
       }
       if (e.sums) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {             // over the 16 rows that the lanes of a quarter hold
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int s = 1; s < 16; s <<= 1) {
-            sb[r] += __shfl_xor(sb[r], s);
-            sg[r] += __shfl_xor(sg[r], s);
+          for (int r = 0; r < 4; ++r) {           // over the 16 rows that the lanes of a quarter hold
+#pragma unroll
+            for (int s = 1; s < 16; s <<= 1) {
+              sb[h][r] += __shfl_xor(sb[h][r], s);
+              sg[h][r] += __shfl_xor(sg[h][r], s);
+            }
           }
-        }
-        if (c == 0) {
-          const int col = (wave % WN) * (BN / WN) + 16 * j + 4 * q;
-          *(f32x4*)(part + ((wave / WN) * 2 + 0) * BN + col) = sb;
-          *(f32x4*)(part + ((wave / WN) * 2 + 1) * BN + col) = sg;
+          if (c == 0) {
+            const int col = (wave % WN) * (BN / WN) + 32 * j + 16 * h + 4 * q;
+            *(f32x4*)(part + ((wave / WN) * 2 + 0) * BN + col) = sb[h];
+            *(f32x4*)(part + ((wave / WN) * 2 + 1) * BN + col) = sg[h];
+          }
         }
       }
     }
@@ -182,16 +196,16 @@ static LinearPlan linear_plan(const maba_tensor* x, const maba_tensor* scales, c
     if (p.z || p.copy_dy) p.dz = c.take<uint16_t>(p.M * p.Np);
     int64_t part = 0;
     if (need->dx) {
-      p.dx = gemm_plan(p.M, p.Kp, gemm_stages(p.Np, 1), true);
+      p.dx = gemm_plan(p.M, p.Kp, gemm_stages(p.Np, 1), true, true);
       if (p.dx.splits > 1) part = (int64_t)p.dx.splits * p.M * p.Kp;
     }
     if (need->dw) {
-      p.dw = gemm_plan(p.Np, p.Kp, gemm_stages(p.M, 1), true);
+      p.dw = gemm_plan(p.Np, p.Kp, gemm_stages(p.M, 1), true, true);
       part = std::max(part, (int64_t)p.dw.splits * p.Np * p.Kp);
     }
     p.part = c.take<float>(part);
   }
-  p.xw = gemm_plan(p.M, p.Np, gemm_stages(p.Kp, 1), false);
+  p.xw = gemm_plan(p.M, p.Np, gemm_stages(p.Kp, 1), false, false);
   if (need && (need->dbias || need->dgate)) {
     p.sum_rows = p.z ? p.xw.tiles_m : ceil_div(p.M, 128);     // a tile's rows, or those of column_partials
     p.sums = c.take<float>(p.sum_rows * 2 * p.N);

@@ -39,10 +39,12 @@ def _linear(M, K, N, dt, seed=0):
 
 GATED = [(1, 8, 8), (1, 640, 1248), (3, 7, 5), (15, 33, 24), (16, 64, 16), (17, 72, 17), (32, 96, 40), (33, 96, 40), (64, 1, 1),
          (100, 40, 1), (127, 136, 63), (128, 64, 64), (129, 200, 65), (257, 130, 100), (700, 64, 200), (1100, 256, 136)]
+# One size for each tile and a few for its edges; sums that are split and that are not.
+LARGE = [(2048, 640, 1248), (3001, 200, 776), (5000, 512, 3000), (8192, 128, 1096), (4100, 1000, 264), (16390, 72, 136)]
 
 
 @pytest.mark.parametrize("dt", [BF, HF])
-@pytest.mark.parametrize("M,Cw,I", GATED)
+@pytest.mark.parametrize("M,Cw,I", GATED + LARGE)
 def test_gated_forward_and_gradients(M, Cw, I, dt):
     x, wg, wu, dh = _gated(M, Cw, I, dt)
     want = B.gated(x, wg, wu, dh)
@@ -52,7 +54,7 @@ def test_gated_forward_and_gradients(M, Cw, I, dt):
 
 
 @pytest.mark.parametrize("dt", [BF, HF])
-@pytest.mark.parametrize("M,K,N", GATED)
+@pytest.mark.parametrize("M,K,N", GATED + LARGE)
 @pytest.mark.parametrize("act,bias,residual,gate", [("none", 0, 0, 0), ("none", 0, 1, 1), ("relu", 1, 0, 0), ("silu", 0, 1, 1),
                                                     ("gelu", 1, 1, 0), ("none", 1, 0, 0)])
 def test_linear_forward_and_gradients(M, K, N, dt, act, bias, residual, gate):
