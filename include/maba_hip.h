@@ -438,7 +438,7 @@ int maba_hip_linear_epilogue(const maba_tensor* x, const maba_tensor* weight, co
                              size_t workspace_bytes, void* stream);
 size_t maba_hip_linear_epilogue_backward_workspace_size(const maba_tensor* dy, const maba_tensor* x,
                                                         const maba_tensor* x_scales, const maba_tensor* weight, int act,
-                                                        int with_gate, int needs);
+                                                        int with_bias, int with_gate, int needs);
 int maba_hip_linear_epilogue_backward(const maba_tensor* dy, const maba_tensor* x, const maba_tensor* x_scales,
                                       const maba_tensor* weight, const maba_tensor* bias, int act, const maba_tensor* gate,
                                       maba_tensor* dx, maba_tensor* dw, maba_tensor* dbias, maba_tensor* dgate,

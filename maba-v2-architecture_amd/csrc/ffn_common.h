@@ -11,9 +11,29 @@ namespace ffn {
 
 // ---------------------------------------------------------------- copies and reductions (ffn_common.hip)
 
-// dst [rows, pad8(cols)] (contiguous) = src [rows, cols] with zeros behind each row, of 16-bit elements at any
-// alignment.  With scales: src holds the e4m3 codes of a packed activation, dst its values in `dtype`.
-int copy_rows(const maba_tensor* src, const maba_tensor* scales, int dtype, uint16_t* dst, hipStream_t s);
+// dst [rows, chunks * 8] (contiguous) = src [rows, cols] with zeros behind each row, of 16-bit elements at any
+// alignment, scaled by gate[row] where there is one; with scales: src holds the e4m3 codes of a packed activation,
+// dst its values.
+struct CopyJob {
+  const void* src; int64_t ld;
+  const uint8_t* scales; int64_t scale_ld;
+  const uint16_t* gate;
+  int64_t rows;
+  int cols, chunks;
+  uint16_t* dst;
+};
+constexpr int MAX_COPIES = 3;
+// A call's copies, made by one launch.
+struct Copies {
+  CopyJob job[MAX_COPIES];
+  int count = 0;
+  void add(const maba_tensor* src, const maba_tensor* scales, uint16_t* dst, const maba_tensor* gate = nullptr) {
+    job[count++] = {src->data, src->stride[0], scales ? (const uint8_t*)scales->data : nullptr, scales ? scales->stride[0] : 0,
+                    gate ? (const uint16_t*)gate->data : nullptr, src->shape[0], (int)src->shape[1],
+                    (int)((src->shape[1] + 7) / 8), dst};
+  }
+  int launch(int dtype, hipStream_t s) const;
+};
 
 // out = the sum of `splits` fp32 partials [splits][M][N] in split order, rounded to 16 bits; row m goes to
 // row m of out[0], or from `second` on to row m - second of out[1]; only `rows` rows of each are written, and
@@ -25,8 +45,21 @@ struct ReduceArgs {
 };
 int reduce_splits(const ReduceArgs& a, int dtype, hipStream_t s);
 
-// out[t][n] = the sum over r of p[r][t][n] (fp32 partials [R][2][N], t = 0, 1; a null out is skipped), 16 bits.
-int reduce_columns(const float* p, int64_t R, int N, void* out0, void* out1, int dtype, hipStream_t s);
+// out[t][n] = the sum over r of p[r][t][n] (fp32 partials [R][2][N], t = 0, 1; a null out is skipped), 16 bits; with a
+// gate out[0] is multiplied by it; sum[n] is t = 0's in fp32.
+int reduce_columns(const float* p, int64_t R, int N, void* out0, void* out1, const void* gate, float* sum, int dtype, hipStream_t s);
+
+// For G = the sum of `splits` partials [splits][M][N]: dw = gate * G, dgate[m] = <w[m], G[m]> + bias[m] colsum[m]; a null
+// dw or dgate is skipped.
+struct GatedReduceArgs {
+  const float* p;
+  int splits, M, N, ncols;
+  Rows dw, w;
+  const uint16_t *gate, *bias;
+  const float* colsum;
+  uint16_t* dgate;
+};
+int reduce_gated(const GatedReduceArgs& a, int rows, int dtype, hipStream_t s);
 
 // p[r][0][n] = the sum of rows [128 r, 128 r + 128) of src [M, N] (16-bit), [ceil(M / 128)][2][N].
 int column_partials(const maba_tensor* src, float* p, hipStream_t s);

@@ -47,63 +47,73 @@ GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, bool columns, bool may_
   return best;
 }
 
-// A thread makes eight elements of a padded row.  Elements are read one by one: this kernel serves the
-// tensors whose rows are not 16-byte aligned; it is bound by its launch or by HBM.
-__global__ __launch_bounds__(256) void copy_rows_kernel(const uint16_t* src, int64_t ld, int64_t rows, int cols, int chunks,
-                                                        uint16_t* dst) {
-  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < rows * chunks; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / chunks;
-    const int k = (int)(i % chunks) * 8;
-    const uint16_t* p = src + r * ld + k;
-    u32x4 v;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t lo = k + 2 * j < cols ? p[2 * j] : 0, hi = k + 2 * j + 1 < cols ? p[2 * j + 1] : 0;
-      v[j] = lo | (hi << 16);
-    }
-    *(u32x4*)(dst + i * 8) = v;
-  }
-}
+// A thread makes eight elements of a padded row of one of the launch's copies.  Bound by the launch or by HBM.
+struct CopyArgs {
+  CopyJob job[MAX_COPIES];
+  int64_t end[MAX_COPIES];     // chunks of the copies up to and with each
+};
 
-// The same from e4m3 codes and their groups' exponents: code * 2^(scale - 127), exact in fp32, rounded once to
-// T (a bf16 holds it exactly unless it is subnormal there).
+// The values of e4m3 codes: code * 2^(scale - 127), exact in fp32, rounded once to T (a bf16 holds it exactly unless
+// it is subnormal there).
 template <class T>
-__global__ __launch_bounds__(256) void unpack_rows_kernel(const uint8_t* src, int64_t ld, const uint8_t* sc, int64_t lds_,
-                                                          int64_t rows, int cols, int chunks, int vec, uint16_t* dst) {
-  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < rows * chunks; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / chunks;
-    const int k = (int)(i % chunks) * 8;
-    const uint8_t* p = src + r * ld + k;
-    const int e = (int)sc[r * lds_ + (k >> 5)] - 127;
-    u32x2 w = {0, 0};
-    if (vec) w = *(const u32x2*)p;
-    else
+__device__ __forceinline__ u32x4 unpack8(u32x2 w, int e) {
+  u32x4 v;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j >> 2] |= (k + j < cols ? (uint32_t)p[j] : 0u) << (8 * (j & 3));
-    u32x4 v;
+  for (int h = 0; h < 2; ++h) {
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], true);
+    v[2 * h] = T::down(__builtin_amdgcn_ldexpf(a[0], e)) | (T::down(__builtin_amdgcn_ldexpf(a[1], e)) << 16);
+    v[2 * h + 1] = T::down(__builtin_amdgcn_ldexpf(b[0], e)) | (T::down(__builtin_amdgcn_ldexpf(b[1], e)) << 16);
+  }
+  return v;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void copy_rows_kernel(CopyArgs a) {
+  typedef u32x2 u32x2_byte __attribute__((aligned(1)));
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < a.end[MAX_COPIES - 1]; i += (int64_t)gridDim.x * 256) {
+    const int t = i < a.end[0] ? 0 : i < a.end[1] ? 1 : 2;
+    const CopyJob& c = a.job[t];
+    const int64_t at = i - (t ? a.end[t - 1] : 0), r = at / c.chunks;
+    const int k = (int)(at % c.chunks) * 8, n = c.cols - k;
+    u32x4 v = {0, 0, 0, 0};
+    if (c.scales) {
+      const uint8_t* p = (const uint8_t*)c.src + r * c.ld + k;
+      u32x2 w = {0, 0};
+      if (n >= 8) w = *(const u32x2_byte*)p;
+      else
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], true);
-      v[2 * h] = T::down(__builtin_amdgcn_ldexpf(a[0], e)) | (T::down(__builtin_amdgcn_ldexpf(a[1], e)) << 16);
-      v[2 * h + 1] = T::down(__builtin_amdgcn_ldexpf(b[0], e)) | (T::down(__builtin_amdgcn_ldexpf(b[1], e)) << 16);
+        for (int j = 0; j < 7; ++j) w[j >> 2] |= (j < n ? (uint32_t)p[j] : 0u) << (8 * (j & 3));
+      v = unpack8<T>(w, (int)c.scales[r * c.scale_ld + (k >> 5)] - 127);
+    } else {
+      const uint16_t* p = (const uint16_t*)c.src + r * c.ld + k;
+      if (n >= 8) v = *(const u32x4_any*)p;
+      else
+#pragma unroll
+        for (int j = 0; j < 7; ++j) v[j >> 1] |= (j < n ? (uint32_t)p[j] : 0u) << (16 * (j & 1));
+      if (c.gate) {
+        const float g = T::up(c.gate[r]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = T::down(T::up(v[j] & 0xffffu) * g) | (T::down(T::up(v[j] >> 16) * g) << 16);
+      }
     }
-    *(u32x4*)(dst + i * 8) = v;
+    *(u32x4*)(c.dst + at * 8) = v;
   }
 }
 
-int copy_rows(const maba_tensor* src, const maba_tensor* scales, int dtype, uint16_t* dst, hipStream_t s) {
-  const int64_t rows = src->shape[0], cols = src->shape[1], chunks = pad8(cols) / 8;
-  if (rows == 0) return MABA_OK;
-  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows * chunks, 256), 16384));
-  if (!scales) {
-    hipLaunchKernelGGL(copy_rows_kernel, grid, dim3(256), 0, s, (const uint16_t*)src->data, src->stride[0], rows, (int)cols,
-                       (int)chunks, dst);
-  } else {
-    const int vec = cols % 8 == 0 && src->stride[0] % 8 == 0 && (uintptr_t)src->data % 8 == 0;
-    auto k = dtype == MABA_BF16 ? unpack_rows_kernel<Bf16> : unpack_rows_kernel<Fp16>;
-    hipLaunchKernelGGL(k, grid, dim3(256), 0, s, (const uint8_t*)src->data, src->stride[0], (const uint8_t*)scales->data,
-                       scales->stride[0], rows, (int)cols, (int)chunks, vec, dst);
+int Copies::launch(int dtype, hipStream_t s) const {
+  CopyArgs a = {};
+  int64_t total = 0;
+  for (int i = 0; i < MAX_COPIES; ++i) {
+    if (i < count) {
+      a.job[i] = job[i];
+      total += job[i].rows * job[i].chunks;
+    }
+    a.end[i] = total;
   }
+  if (total == 0) return MABA_OK;
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(total, 256), 16384));
+  auto k = dtype == MABA_BF16 ? copy_rows_kernel<Bf16> : copy_rows_kernel<Fp16>;
+  hipLaunchKernelGGL(k, grid, dim3(256), 0, s, a);
   return check_launch("copy_rows");
 }
 
@@ -128,12 +138,50 @@ int reduce_splits(const ReduceArgs& a, int dtype, hipStream_t s) {
   return check_launch("reduce_splits");
 }
 
+// A workgroup a row of G = sum of the partials: dw = gate * G, and dgate = <w, G> (+ bias * colsum, added by the caller's
+// term), the lanes' parts added in a fixed order.
+template <class T>
+__global__ __launch_bounds__(256) void reduce_gated_kernel(GatedReduceArgs a) {
+  __shared__ float part[4];
+  const int m = blockIdx.x, wave = threadIdx.x >> 6;
+  const int64_t plane = (int64_t)a.M * a.N;
+  const float gate = T::up(a.gate[m]);
+  float dot = 0.f;
+  for (int n = threadIdx.x * 4; n < a.ncols; n += 1024) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; ++s) v += *(const f32x4*)(a.p + s * plane + (int64_t)m * a.N + n);
+    if (a.dgate) {
+      const f32x4 w = up4<T>(load4(a.w, m, n, a.ncols));
+      dot += v[0] * w[0] + v[1] * w[1] + v[2] * w[2] + v[3] * w[3];
+    }
+    if (a.dw.p) store4<T>(a.dw, m, n, a.ncols, v * gate);
+  }
+  if (a.dgate) {
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) dot += __shfl_xor(dot, s);
+    if ((threadIdx.x & 63) == 0) part[wave] = dot;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      float v = part[0] + part[1] + part[2] + part[3];
+      if (a.bias) v += T::up(a.bias[m]) * a.colsum[m];
+      a.dgate[m] = (uint16_t)T::down(v);
+    }
+  }
+}
+
+int reduce_gated(const GatedReduceArgs& a, int rows, int dtype, hipStream_t s) {
+  auto k = dtype == MABA_BF16 ? reduce_gated_kernel<Bf16> : reduce_gated_kernel<Fp16>;
+  hipLaunchKernelGGL(k, dim3((unsigned)rows), dim3(256), 0, s, a);
+  return check_launch("reduce_gated");
+}
+
 // 32 columns of one output a workgroup, eight threads each, added through LDS in a fixed order.
 template <class T>
-__global__ __launch_bounds__(256) void reduce_columns_kernel(const float* p, int64_t R, int N, uint16_t* out0, uint16_t* out1) {
+__global__ __launch_bounds__(256) void reduce_columns_kernel(const float* p, int64_t R, int N, uint16_t* out0, uint16_t* out1,
+                                                             const uint16_t* gate, float* sum) {
   __shared__ float part[8][32];
   uint16_t* out = blockIdx.y ? out1 : out0;
-  if (!out) return;
+  if (!out && !sum) return;
   const int col = threadIdx.x & 31, lane = threadIdx.x >> 5, n = blockIdx.x * 32 + col;
   float v = 0.f;
   if (n < N)
@@ -144,13 +192,15 @@ __global__ __launch_bounds__(256) void reduce_columns_kernel(const float* p, int
     float w = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) w += part[i][col];
-    out[n] = (uint16_t)T::down(w);
+    if (sum) sum[n] = w;
+    if (out) out[n] = (uint16_t)T::down(gate ? w * T::up(gate[n]) : w);
   }
 }
 
-int reduce_columns(const float* p, int64_t R, int N, void* out0, void* out1, int dtype, hipStream_t s) {
+int reduce_columns(const float* p, int64_t R, int N, void* out0, void* out1, const void* gate, float* sum, int dtype, hipStream_t s) {
   auto k = dtype == MABA_BF16 ? reduce_columns_kernel<Bf16> : reduce_columns_kernel<Fp16>;
-  hipLaunchKernelGGL(k, dim3((unsigned)ceil_div(N, 32), 2), dim3(256), 0, s, p, R, N, (uint16_t*)out0, (uint16_t*)out1);
+  hipLaunchKernelGGL(k, dim3((unsigned)ceil_div(N, 32), out1 ? 2 : 1), dim3(256), 0, s, p, R, N, (uint16_t*)out0, (uint16_t*)out1,
+                     (const uint16_t*)gate, sum);
   return check_launch("reduce_columns");
 }
 

@@ -160,18 +160,17 @@ static GatedPlan gated_plan(const maba_tensor* x, const maba_tensor* scales, con
 static int gated_operands(GatedPlan& p, const maba_tensor* x, const maba_tensor* scales, const maba_tensor* wg,
                           const maba_tensor* wu, hipStream_t s, Operand& ox, Operand& ow) {
   const maba_tensor* w[2] = {wg, wu};
-  if (p.copy_x)
-    if (int rc = copy_rows(x, scales, wg->dtype, p.x, s)) return rc;
+  Copies copies;
+  if (p.copy_x) copies.add(x, scales, p.x);
   ox = p.copy_x ? rows_operand(p.x, p.Cp, p.M) : rows_operand((const uint16_t*)x->data, x->stride[0], p.M);
   ow = {};
   ow.rows = (int)p.I;
   for (int i = 0; i < 2; ++i) {
-    if (p.copy_w[i])
-      if (int rc = copy_rows(w[i], nullptr, wg->dtype, p.w[i], s)) return rc;
+    if (p.copy_w[i]) copies.add(w[i], nullptr, p.w[i]);
     ow.p[i] = p.copy_w[i] ? p.w[i] : (const uint16_t*)w[i]->data;
     ow.ld[i] = p.copy_w[i] ? p.Cp : w[i]->stride[0];
   }
-  return MABA_OK;
+  return copies.launch(wg->dtype, s);
 }
 
 template <class T>

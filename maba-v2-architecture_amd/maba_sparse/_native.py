@@ -141,7 +141,7 @@ def _declare(lib) -> None:
         "maba_hip_gated_ffn_backward": ([T, T, T, T, T, T, T, T, vp, sz, vp], i),
         "maba_hip_linear_epilogue_workspace_size": ([T, T], sz),
         "maba_hip_linear_epilogue": ([T, T, T, i, T, T, T, vp, sz, vp], i),
-        "maba_hip_linear_epilogue_backward_workspace_size": ([T, T, T, T, i, i, i], sz),
+        "maba_hip_linear_epilogue_backward_workspace_size": ([T, T, T, T, i, i, i, i], sz),
         "maba_hip_linear_epilogue_backward": ([T, T, T, T, T, i, T, T, T, T, T, vp, sz, vp], i),
         "maba_hip_checkpoint_pack": ([T, T, T, vp], i),
         "maba_hip_checkpoint_unpack": ([T, T, T, vp], i),
@@ -210,7 +210,7 @@ def desc_array(tensors: Sequence[Optional[torch.Tensor]]):
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None else torch.cuda.current_device())
 
 
 def on_device(device: torch.device):

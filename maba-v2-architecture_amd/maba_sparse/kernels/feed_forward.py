@@ -34,8 +34,8 @@ class LinearEpilogue(torch.autograd.Function):
         ctx.ops, ctx.activation = ops, activation
         dx, dw, dbias, _, dgate = ctx.needs_input_grad[3:8]
         ctx.has = (bias is not None, gate is not None)
-        # x is read by dW and, where dz is not dy itself, to make z again
-        ctx.keeps_x = dw or dgate or ((dx or dbias) and (activation != "none" or gate is not None))
+        # x is read by dW and dgate and, with an activation, to make z again
+        ctx.keeps_x = dw or dgate or ((dx or dbias) and activation != "none")
         kept = (ops.pack(x) if checkpoint else (x,)) if ctx.keeps_x else ()
         ctx.x_like = x.shape
         if dx or dw or dbias or dgate:

@@ -307,7 +307,8 @@ _ACT_CODES = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t [..., C]`` as ``[rows, C]`` with unit column stride: a view where the strides allow it."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
@@ -387,7 +388,7 @@ def hip_linear_epilogue_backward(dy, x, weight, bias=None, activation: str = "no
         ddy, ddx, dsc, dw = N.desc(_rows(dy)), N.desc(x2), N.desc(sc), N.desc(_rows(weight))
         act = _ACT_CODES[activation]
         ws = _workspace(lib.maba_hip_linear_epilogue_backward_workspace_size(
-            ddy, ddx, dsc, dw, act, int(gate is not None), sum(1 << i for i, n in enumerate(needs) if n)), dev)
+            ddy, ddx, dsc, dw, act, int(bias is not None), int(gate is not None), sum(1 << i for i, n in enumerate(needs) if n)), dev)
         rc = lib.maba_hip_linear_epilogue_backward(ddy, ddx, dsc, dw, N.desc(_row(bias)), act, N.desc(_row(gate)),
                                                    *(N.desc(o) for o in outs), ws.data_ptr(), ws.numel(), N.stream_ptr(dev))
         N.check(rc, "linear_epilogue_backward")

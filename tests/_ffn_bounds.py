@@ -116,7 +116,10 @@ def linear(x, w, bias=None, act="none", residual=None, gate=None, dy=None, kept=
     E = e32 if act == "none" and gate is None else _round(dz, e32, dt)
     M = x.shape[0]
     dx = dz @ w
-    out["dx"] = (dx, _round(dx, (E + (w.shape[0] + 16) * U * dz.abs()) @ w.abs(), dt))
+    ex = (E + (w.shape[0] + 16) * U * dz.abs()) @ w.abs()
+    if act == "none" and gate is not None:      # the gate may be on the weight: gate * w rounded, subnormal or not
+        ex = ex + d.abs().sum(1, keepdim=True) * torch.finfo(dt).tiny * half_step(dt)
+    out["dx"] = (dx, _round(dx, ex, dt))
     dw = dz.t() @ x
     out["dw"] = (dw, _round(dw, (E + (M + 64) * U * dz.abs()).t() @ x.abs(), dt))
     if bias is not None:
@@ -124,7 +127,10 @@ def linear(x, w, bias=None, act="none", residual=None, gate=None, dy=None, kept=
         out["dbias"] = (db, _round(db, (e32 + (M + 64) * U * dz.abs()).sum(0), dt))
     if gate is not None:
         dgt = (d * a).sum(0)
-        out["dgate"] = (dgt, _round(dgt, (d.abs() * (slope * ez + near * z.abs()) + (M + 64) * U * (d * a).abs()).sum(0), dt))
+        eg = (d.abs() * (slope * ez + near * z.abs()) + (M + 64) * U * (d * a).abs()).sum(0)
+        if act == "none":                       # or <w, dy^T x> + bias * sum(dy): sums of M and of K products
+            eg = eg + (M + x.shape[1] + 72) * U * (d.abs() * (x.abs() @ w.abs().t() + abs(b))).sum(0)
+        out["dgate"] = (dgt, _round(dgt, eg, dt))
     return out
 
 

@@ -56,7 +56,7 @@ def test_gated_forward_and_gradients(M, Cw, I, dt):
 @pytest.mark.parametrize("dt", [BF, HF])
 @pytest.mark.parametrize("M,K,N", GATED + LARGE)
 @pytest.mark.parametrize("act,bias,residual,gate", [("none", 0, 0, 0), ("none", 0, 1, 1), ("relu", 1, 0, 0), ("silu", 0, 1, 1),
-                                                    ("gelu", 1, 1, 0), ("none", 1, 0, 0)])
+                                                    ("gelu", 1, 1, 0), ("none", 1, 0, 0), ("none", 1, 1, 1)])
 def test_linear_forward_and_gradients(M, K, N, dt, act, bias, residual, gate):
     t = _linear(M, K, N, dt)
     b, r, g = (t[k] if on else None for k, on in (("bias", bias), ("residual", residual), ("gate", gate)))
