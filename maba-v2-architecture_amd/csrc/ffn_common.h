@@ -66,13 +66,11 @@ int column_partials(const maba_tensor* src, float* p, hipStream_t s);
 
 // ---------------------------------------------------------------- launches
 
-// The tiles: BM, BN, waves along m and n, stages in LDS (three and four measured no faster, also where a compute
-// unit has one small tile).
-struct Tile256 { static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, ST = 2; };
-struct Tile192 { static constexpr int BM = 192, BN = 128, WM = 2, WN = 2, ST = 2; };
-struct Tile128 { static constexpr int BM = 128, BN = 128, WM = 2, WN = 2, ST = 2; };
-struct Tile64 { static constexpr int BM = 64, BN = 64, WM = 2, WN = 2, ST = 2; };
-constexpr int GEMM_BK = 64;
+// The tiles: BM, BN, waves along m and n.
+struct Tile256 { static constexpr int BM = 256, BN = 256, WM = 2, WN = 4; };
+struct Tile192 { static constexpr int BM = 192, BN = 128, WM = 2, WN = 2; };
+struct Tile128 { static constexpr int BM = 128, BN = 128, WM = 2, WN = 2; };
+struct Tile64 { static constexpr int BM = 64, BN = 64, WM = 2, WN = 2; };
 
 // How a product runs: which tile, and into how many runs of stages its sum is split (more than one writes fp32
 // partials that reduce_splits adds).
@@ -88,7 +86,7 @@ int gemm_tile(GemmArgs& g, const typename Epi::Args& e, int64_t M, int64_t N, in
   g.tiles_n = (int)ceil_div(N, Tile::BN);
   const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * splits;
   if (grid > INT32_MAX) return fail(MABA_ERR_UNSUPPORTED, "%s: too many tiles", who);
-  hipLaunchKernelGGL((gemm_kernel<T, Tile::BM, Tile::BN, Tile::WM, Tile::WN, GEMM_BK, Tile::ST, AMODE, BMODE, Epi>),
+  hipLaunchKernelGGL((gemm_kernel<T, Tile::BM, Tile::BN, Tile::WM, Tile::WN, AMODE, BMODE, Epi>),
                      dim3((unsigned)grid), dim3(64 * Tile::WM * Tile::WN), 0, s, g, e);
   return check_launch(who);
 }

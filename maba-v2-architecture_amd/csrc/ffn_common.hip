@@ -11,16 +11,16 @@ namespace ffn {
 // holds at once, a stage's latency (`lone`) bounds it.  Measured on MI355X, us, with an operand read along its columns
 // in brackets:
 //              256 x 256      192 x 128      128 x 128      64 x 64
-//   full       1.36 (1.72)    0.55 (0.66)    0.41 (0.53)    0.20 (0.25)
-//   lone       1.36 (1.72)    0.80 (1.00)    0.60 (0.74)    0.36 (0.47)
+//   full       1.36 (1.38)    0.55 (0.63)    0.41 (0.48)    0.20 (0.25)
+//   lone       1.36 (1.38)    0.80 (1.00)    0.60 (0.74)    0.36 (0.47)
 //   ends       7.6            4              3              0.75
-// (4,096 x 11,008 x 2,048, rows: 154, 172, 178 us with the first three; 16,384 x 640 x 2,496, columns: 83, 62, 88;
+// (4,096 x 11,008 x 2,048, rows: 152, 172, 178 us with the first three; 16,384 x 640 x 2,496, columns: 69, 62, 82;
 // 2,048 x 2,496 x 640, rows: 20, 14.3, 14.3 and 16.7; 64 x 640 x 2,496 with the last, in 1, 4 and 8 splits: 19.9,
 // 7.2 and 5.2.)
 struct TileCost { int bm, bn, slots; float full[2], lone[2], ends; };
-static const TileCost TILES[4] = {{256, 256, 1, {1.36f, 1.72f}, {1.36f, 1.72f}, 7.6f},
-                                  {192, 128, 2, {0.55f, 0.66f}, {0.80f, 1.00f}, 4.f},
-                                  {128, 128, 2, {0.41f, 0.53f}, {0.60f, 0.74f}, 3.f},
+static const TileCost TILES[4] = {{256, 256, 1, {1.36f, 1.38f}, {1.36f, 1.38f}, 7.6f},
+                                  {192, 128, 2, {0.55f, 0.63f}, {0.80f, 1.00f}, 4.f},
+                                  {128, 128, 2, {0.41f, 0.48f}, {0.60f, 0.74f}, 3.f},
                                   {64, 64, 5, {0.20f, 0.25f}, {0.36f, 0.47f}, 0.75f}};
 
 GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, bool columns, bool may_split) {

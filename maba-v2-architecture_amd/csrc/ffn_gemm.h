@@ -168,6 +168,7 @@ struct GemmArgs {
   int split_stages;     // stages of a split's run of the sum (the last split may have fewer)
 };
 
+constexpr int GEMM_BK = 64;      // k of a stage: two steps
 constexpr uint32_t OUT_OF_RANGE = 0x80000000u;   // a lane offset past every descriptor's end
 
 // The same in every lane; said so to the compiler, which otherwise loops over the lanes' descriptors.
@@ -308,9 +309,9 @@ __device__ __forceinline__ TileId tile_of(const GemmArgs& g) {
 // steps, where every wave has the stage's last fragments in registers (its buffer is free for the loads of the stage
 // after next) and the next stage has landed (its first fragments can be read).  So neither LDS reads nor
 // loads are waited for between products, except by the first.
-template <class T, int BM, int BN, int WM, int WN, int BK, int ST, int AMODE, int BMODE, class Epi>
+template <class T, int BM, int BN, int WM, int WN, int AMODE, int BMODE, class Epi>
 __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) void gemm_kernel(GemmArgs g, typename Epi::Args e) {
-  constexpr int NW = WM * WN, MI = BM / WM / 16, NI = BN / WN / 16;
+  constexpr int NW = WM * WN, MI = BM / WM / 16, NI = BN / WN / 16, BK = GEMM_BK, ST = 2;
   constexpr int A_EL = BM * BK, STAGE = (BM + BN) * BK;
   typedef Stager<BM, BK, NW, AMODE> SA;
   typedef Stager<BN, BK, NW, BMODE> SB;
@@ -354,9 +355,10 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) 
 #pragma unroll
       for (int j = 0; j < NI; ++j) acc[i][j] = T::mma(f.b[j], f.a[i], acc[i][j]);
   };
-  // one LDS read with every other product or so
+  // LDS reads between the products: one with each at eight waves, spread over all of them at four (256 x 256 rows on
+  // 4,096 x 11,008 x 2,048: 152 us against 155; the smaller tiles the same either way)
   auto interleave = [] {
-    constexpr int READS = MI * (SA::COLS ? 2 : 1) + NI * (SB::COLS ? 2 : 1), PER = MI * NI / READS > 1 ? MI * NI / READS : 1;
+    constexpr int READS = MI * (SA::COLS ? 2 : 1) + NI * (SB::COLS ? 2 : 1), PER = NW == 8 || MI * NI < READS ? 1 : MI * NI / READS;
 #pragma unroll
     for (int i = 0; i < READS; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // LDS read
@@ -374,39 +376,30 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) 
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   read(f0, 0, 0);
+  // The loads of the stage after next, which write LDS, are issued before the reads of the next fragments or behind
+  // them.  Behind them measured faster where those are transposing reads or eight waves' (256 x 256 tiles: dx of
+  // 4,096 x 2,048 x 11,008 233 us against 297, dW of 11,008 x 2,048 x 4,096 191 against 220), before them for four
+  // waves' row reads (192 x 128 on 32,768 x 640 x 1,248: 59 us against 61).
+  constexpr bool LATE = SA::COLS || SB::COLS || NW == 8;
   // between two steps: the next stage has landed, and every wave holds the fragments of stage s
   auto turn = [&](int s) {
-    if (ST > 2 && s + ST - 1 < nk) wait_vm<(ST - 2) * LOADS>();
-    else wait_vm<0>();
+    wait_vm<0>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (s + ST < nk) issue(s + ST);
+    if (!LATE && s + ST < nk) issue(s + ST);
   };
-  if constexpr (BK == 64) {
-    for (int s = 0; s < nk; ++s) {
-      read(f1, s, 1);
-      products(f0);
-      interleave();
-      turn(s);
-      // past the last stage these are stale values that nothing uses
-      read(f0, s + 1, 0);
-      products(f1);
-      interleave();
-    }
-  } else {
-    int s = 0;
-    for (; s + 1 < nk; s += 2) {
-      turn(s);
-      read(f1, s + 1, 0);
-      products(f0);
-      interleave();
-      turn(s + 1);
-      read(f0, s + 2, 0);
-      products(f1);
-      interleave();
-    }
-    if (s < nk) products(f0);
+
+  for (int s = 0; s < nk; ++s) {
+    read(f1, s, 1);
+    products(f0);
+    interleave();
+    turn(s);
+    // past the last stage these are stale values that nothing uses
+    read(f0, s + 1, 0);
+    if (LATE && s + ST < nk) issue(s + ST);
+    products(f1);
+    interleave();
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   Epi::template run<T, BM, BN, WM, WN, MI, NI>(e, acc, t, m0 + wm, n0 + wn, c, q, wave, lds);
