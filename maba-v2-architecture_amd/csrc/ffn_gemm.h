@@ -138,16 +138,6 @@ __device__ __forceinline__ void store4(const Rows& r, int64_t m, int n, int nend
       if (n + i < nend) p[i] = (uint16_t)(u[i >> 1] >> (16 * (i & 1)));
   }
 }
-// Four consecutive elements of a vector [N].
-template <class T>
-__device__ __forceinline__ f32x4 vec4(const uint16_t* p, int n, int nend) {
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (n + i < nend) v[i] = T::up(p[n + i]);
-  return v;
-}
-
 enum { K_ROWS = 0, K_ROWS_PAIR = 1, K_COLS = 2 };
 
 // One operand.  K_ROWS: p[0] is [rows][K], ld[0] apart.  K_ROWS_PAIR: two such tensors of `rows` rows

@@ -43,14 +43,11 @@ __device__ __forceinline__ float dact_of(float z) {
   } else return 1.f;
 }
 
-// The quads of the bias (zeros without one) and the gate (ones).
+// The quads at n of a vector [N], or of a constant in its place.
 template <class T>
-__device__ __forceinline__ f32x4 bias4(const uint16_t* p, int n, int nend) {
-  return p ? vec4<T>(p, n, nend) : f32x4{0.f, 0.f, 0.f, 0.f};
-}
-template <class T>
-__device__ __forceinline__ f32x4 gate4(const uint16_t* p, int n, int nend) {
-  return p ? vec4<T>(p, n, nend) : f32x4{1.f, 1.f, 1.f, 1.f};
+__device__ __forceinline__ f32x4 vec4(const uint16_t* p, float other, int n, int nend) {
+  if (!p) return f32x4{other, other, other, other};
+  return up4<T>(load4(Rows{(uint16_t*)p, 0}, 0, n, nend));
 }
 
 template <int ACT>
@@ -65,12 +62,18 @@ struct EpiLinear {
   template <class T>
   static __device__ __forceinline__ void quad(const Args& e, int64_t m, int n, f32x4 z, f32x4) {
     const u32x2 res = e.res.p ? load4(e.res, m, n, e.N) : u32x2{0, 0};
-    store4<T>(e.y, m, n, e.N, value(z, bias4<T>(e.bias, n, e.N), gate4<T>(e.gate, n, e.N), up4<T>(res)));
+    store4<T>(e.y, m, n, e.N, value(z, vec4<T>(e.bias, 0.f, n, e.N), vec4<T>(e.gate, 1.f, n, e.N), up4<T>(res)));
   }
   template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
   static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
                                              int q, int wave, uint16_t* lds) {
-    u32x4 res[MI][NI / 2];       // all of the residual first: the loads are in flight together
+    f32x4 bias[NI], gate[NI];    // all that is read first: the loads are in flight together
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      bias[j] = vec4<T>(e.bias, 0.f, n0 + 16 * j + 4 * q, e.N);
+      gate[j] = vec4<T>(e.gate, 1.f, n0 + 16 * j + 4 * q, e.N);
+    }
+    u32x4 res[MI][NI / 2];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -79,12 +82,11 @@ struct EpiLinear {
 #pragma unroll
     for (int j = 0; j < NI / 2; ++j) {
       const int n = n0 + 32 * j;
-      const f32x4 ba = bias4<T>(e.bias, n + 4 * q, e.N), bb = bias4<T>(e.bias, n + 16 + 4 * q, e.N);
-      const f32x4 ga = gate4<T>(e.gate, n + 4 * q, e.N), gb = gate4<T>(e.gate, n + 16 + 4 * q, e.N);
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const Quads r = quads_of(res[i][j]);
-        const f32x4 a = value(acc[i][2 * j], ba, ga, up4<T>(r.a)), b = value(acc[i][2 * j + 1], bb, gb, up4<T>(r.b));
+        const f32x4 a = value(acc[i][2 * j], bias[2 * j], gate[2 * j], up4<T>(r.a));
+        const f32x4 b = value(acc[i][2 * j + 1], bias[2 * j + 1], gate[2 * j + 1], up4<T>(r.b));
         store8(e.y, m0 + 16 * i + c, n + 8 * q, e.M, e.N, eight_of({down4<T>(a), down4<T>(b)}));
       }
     }
@@ -113,27 +115,27 @@ struct EpiLinearBack {
                                              int q, int wave, uint16_t* lds) {
     float* part = (float*)lds;                    // [WM][2][BN]
     if (e.sums) __syncthreads();                  // the last stage has been read
-    u32x4 dys[MI][NI / 2];                        // all of dy first: the loads are in flight together
+    f32x4 bias[NI], gate[NI];                     // all that is read first: the loads are in flight together
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      bias[j] = vec4<T>(e.bias, 0.f, n0 + 16 * j + 4 * q, e.N);
+      gate[j] = vec4<T>(e.gate, 1.f, n0 + 16 * j + 4 * q, e.N);
+    }
+    u32x4 dys[MI][NI / 2];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NI / 2; ++j) dys[i][j] = load8(e.dy, m0 + 16 * i + c, n0 + 32 * j + 8 * q, e.M, e.N);
 #pragma unroll
     for (int j = 0; j < NI / 2; ++j) {
-      f32x4 bias[2], gate[2], sb[2], sg[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int n = n0 + 32 * j + 16 * h + 4 * q;
-        bias[h] = bias4<T>(e.bias, n, e.N);
-        gate[h] = gate4<T>(e.gate, n, e.N);
-        sb[h] = sg[h] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
+      f32x4 sb[2], sg[2];
+      sb[0] = sb[1] = sg[0] = sg[1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const int m = m0 + 16 * i + c;
         const Quads d = quads_of(dys[i][j]);
-        const f32x4 a = value(acc[i][2 * j], up4<T>(d.a), bias[0], gate[0], sb[0], sg[0], m < e.M);
-        const f32x4 b = value(acc[i][2 * j + 1], up4<T>(d.b), bias[1], gate[1], sb[1], sg[1], m < e.M);
+        const f32x4 a = value(acc[i][2 * j], up4<T>(d.a), bias[2 * j], gate[2 * j], sb[0], sg[0], m < e.M);
+        const f32x4 b = value(acc[i][2 * j + 1], up4<T>(d.b), bias[2 * j + 1], gate[2 * j + 1], sb[1], sg[1], m < e.M);
         store8(e.dz, m, n0 + 32 * j + 8 * q, e.M, e.Np, eight_of({down4<T>(a), down4<T>(b)}));
       }
       if (e.sums) {
