@@ -448,7 +448,8 @@ int maba_hip_linear_epilogue_backward(const maba_tensor* dy, const maba_tensor* 
  * Activation checkpoints in 8 bits.  x, out [M,C] f32, f16 or bf16; codes [M,C] MABA_E4M3; scales
  * [M,ceil(C/32)] MABA_U8.  Every 32 elements of a row share 2^e, the smallest power of two (e >= -127) with
  * max|x| <= 448 * 2^e over the finite ones; scale = e + 127, code = x / 2^e rounded to nearest even.  NaN and
- * infinities become e4m3's NaN.  Unpacked values are code * 2^e rounded to out's type.
+ * infinities become e4m3's NaN.  Unpacked values are code * 2^e rounded to out's type, or its largest
+ * finite value where they are past it.
  */
 int maba_hip_checkpoint_pack(const maba_tensor* x, maba_tensor* codes, maba_tensor* scales, void* stream);
 int maba_hip_checkpoint_unpack(const maba_tensor* codes, const maba_tensor* scales, maba_tensor* out, void* stream);

@@ -12,8 +12,6 @@
 namespace maba {
 namespace ffn {
 
-__device__ __forceinline__ float elem(const void* p, int64_t i, int dt) { return load_elem(p, dt, i); }
-
 template <int DT>
 __device__ __forceinline__ void load8(const void* base, int64_t i, int n, bool vec, float (&v)[8]) {
   if (vec) {
@@ -113,14 +111,15 @@ __global__ __launch_bounds__(256) void unpack_kernel(UnpackArgs a) {
     else
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j >> 2] |= (j < n ? (uint32_t)p[j] : 0u) << (8 * (j & 3));
+    constexpr float most = DT == MABA_F32 ? 3.40282347e38f : DT == MABA_BF16 ? Bf16::MOST : Fp16::MOST;
     float v[8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], true);
-      v[4 * h] = __builtin_amdgcn_ldexpf(lo[0], e);
-      v[4 * h + 1] = __builtin_amdgcn_ldexpf(lo[1], e);
-      v[4 * h + 2] = __builtin_amdgcn_ldexpf(hi[0], e);
-      v[4 * h + 3] = __builtin_amdgcn_ldexpf(hi[1], e);
+      v[4 * h] = scaled(lo[0], e, most);
+      v[4 * h + 1] = scaled(lo[1], e, most);
+      v[4 * h + 2] = scaled(hi[0], e, most);
+      v[4 * h + 3] = scaled(hi[1], e, most);
     }
     const int64_t o = r * a.ys + k;
     if (a.vec) {

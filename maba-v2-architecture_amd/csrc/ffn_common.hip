@@ -25,6 +25,7 @@ static const TileCost TILES[4] = {{256, 256, 1, {1.36f, 1.38f}, {1.36f, 1.38f}, 
 
 GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, bool columns, bool may_split) {
   const int64_t cus = device_cu_count();
+  stages = std::max<int64_t>(stages, 1);      // no rows: nothing is launched
   GemmPlan best = {3, 1, (int)stages, 0};
   float least = 0.f;
   for (int i = 0; i < 4; ++i) {
@@ -53,16 +54,16 @@ struct CopyArgs {
   int64_t end[MAX_COPIES];     // chunks of the copies up to and with each
 };
 
-// The values of e4m3 codes: code * 2^(scale - 127), exact in fp32, rounded once to T (a bf16 holds it exactly unless
-// it is subnormal there).
+// The values of e4m3 codes: code * 2^e, exact in fp32, rounded once to T (a bf16 holds it exactly unless it is
+// subnormal there).
 template <class T>
 __device__ __forceinline__ u32x4 unpack8(u32x2 w, int e) {
   u32x4 v;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], true);
-    v[2 * h] = T::down(__builtin_amdgcn_ldexpf(a[0], e)) | (T::down(__builtin_amdgcn_ldexpf(a[1], e)) << 16);
-    v[2 * h + 1] = T::down(__builtin_amdgcn_ldexpf(b[0], e)) | (T::down(__builtin_amdgcn_ldexpf(b[1], e)) << 16);
+    v[2 * h] = T::down(scaled(a[0], e, T::MOST)) | (T::down(scaled(a[1], e, T::MOST)) << 16);
+    v[2 * h + 1] = T::down(scaled(b[0], e, T::MOST)) | (T::down(scaled(b[1], e, T::MOST)) << 16);
   }
   return v;
 }

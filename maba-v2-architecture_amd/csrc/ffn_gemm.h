@@ -30,6 +30,7 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 // The two 16-bit types: products, and conversions that round to nearest even.
 struct Bf16 {
   static constexpr int CODE = MABA_BF16;
+  static constexpr float MOST = 3.38953139e38f;     // the largest finite value
   static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -38,6 +39,7 @@ struct Bf16 {
 };
 struct Fp16 {
   static constexpr int CODE = MABA_F16;
+  static constexpr float MOST = 65504.f;
   static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
@@ -427,6 +429,13 @@ struct EpiPartial {
     }
   }
 };
+
+// An unpacked element: code * 2^e, at most `most` in magnitude (a finite value may have rounded up past its type's
+// range); NaN stays NaN.
+__device__ __forceinline__ float scaled(float code, int e, float most) {
+  const float v = __builtin_amdgcn_ldexpf(code, e);
+  return v > most ? most : v < -most ? -most : v;
+}
 
 __device__ __forceinline__ float sigmoid(float x) { return fast_rcp(1.f + fast_exp(-x)); }
 

@@ -467,11 +467,13 @@ def ref_checkpoint_pack(x, **kwargs: Any):
 
 
 def ref_checkpoint_unpack(codes, scales, dtype: torch.dtype = torch.bfloat16, **kwargs: Any):
-    """The values that a packed activation stands for, ``code * 2^(scale - 127)`` rounded to ``dtype``."""
+    """The values that a packed activation stands for, ``code * 2^(scale - 127)`` rounded to ``dtype``; one
+    past its range (a finite value may have rounded up past it) becomes its largest finite one."""
     C = codes.shape[-1]
     e = (scales.to(torch.int32) - 127).repeat_interleave(PACK_GROUP, dim=-1)[..., :C]
     # 2^-127 is subnormal in fp32: the product is formed in fp64 (exact) and rounded once
-    return (codes.float().double() * _pow2(e)).to(dtype)
+    most = torch.finfo(dtype).max
+    return (codes.float().double() * _pow2(e)).clamp(-most, most).to(dtype)
 
 
 def _kept(x, x_scales, ct):

@@ -8,7 +8,8 @@ prefill, then single-token steps in which the DGDA blocks carry their recurrent 
 states and the MABA-SA blocks decode over a preallocated ``LatentCache`` (incremental
 latent rows, HCA means and indexer centroids) instead of the reference's per-step
 ``torch.cat`` of the whole cache (``model.py:280-313`` with ``sparse_attention.py:241-261``).
-The multi-token-prediction head and the loss are training-side and are not built here.
+The multi-token-prediction head and the loss are training-side and are not built here; the
+feed-forward half of a block trains on the GPU with ``MabaConfig.fused_ffn``.
 """
 from __future__ import annotations
 
@@ -20,7 +21,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from maba_sparse.layers._wcache import WeightCacheMixin, cached
-from maba_sparse.kernels.dispatcher import get_backend
+from maba_sparse.kernels.dispatcher import gated_ffn, get_backend, linear_epilogue
 from maba_sparse.layers.dgda import DGDALayer
 from maba_sparse.layers.sparse_attention import DeviceCache, LatentCache, MabaSparseAttention
 
@@ -47,6 +48,11 @@ class MabaConfig:
     intermediate_size: int = 1248
     rms_norm_eps: float = 1e-6
     residual_gate_bias: float = 2.0
+    # The feed-forward half of a block through the dispatcher's fused operators (gated_ffn and
+    # linear_epilogue), forward and backward; off, it composes torch modules as the reference does.
+    fused_ffn: bool = False
+    # With fused_ffn: what those operators keep for the backward pass, None (16 bits) or "e4m3" (8 bits).
+    ffn_checkpoint: Optional[str] = None
 
 
 def get_101m_config(**overrides: Any) -> MabaConfig:
@@ -73,20 +79,35 @@ def _frozen(module: nn.Module, key: str, fn, *params: torch.Tensor) -> torch.Ten
 
 
 class SwiGLUFFN(WeightCacheMixin, nn.Module):
-    def __init__(self, dim: int, intermediate_size: int) -> None:
+    def __init__(self, dim: int, intermediate_size: int, fused: bool = False, checkpoint: Optional[str] = None) -> None:
         super().__init__()
+        self.fused = fused
+        self.checkpoint = checkpoint
         self.w_gate = nn.Linear(dim, intermediate_size, bias=False)
         self.w_up = nn.Linear(dim, intermediate_size, bias=False)
         self.w_down = nn.Linear(intermediate_size, dim, bias=False)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.fused:
+            return self.forward_fused(x)
         # gate and up projections as one GEMM over the stacked weights
         w = _frozen(self, "gate_up", lambda a, b: torch.cat([a, b], dim=0), self.w_gate.weight, self.w_up.weight)
         g, u = F.linear(x, w).chunk(2, dim=-1)
         return self.w_down(F.silu(g) * u)
 
+    def forward_fused(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None,
+                      gate: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``residual + gate * forward(x)`` (both optional) as the dispatcher's two feed-forward
+        operators: the activation stays in the first one's epilogue, the gated residual in the
+        second's, and their backward passes keep only x and the product (in 8 bits where
+        ``checkpoint`` says so)."""
+        h = gated_ffn(x, self.w_gate.weight, self.w_up.weight, checkpoint=self.checkpoint)
+        return linear_epilogue(h, self.w_down.weight, residual=residual, gate=gate, checkpoint=self.checkpoint)
+
     def forward_hip(self, x: torch.Tensor) -> torch.Tensor:
         """``forward`` with the activation ``silu(g) * u`` as one HIP kernel."""
+        if self.fused:
+            return self.forward_fused(x)
         from maba_sparse.kernels import hip_backend as hb
         w = _frozen(self, "gate_up", lambda a, b: torch.cat([a, b], dim=0), self.w_gate.weight, self.w_up.weight)
         return self.w_down(hb.hip_swiglu(F.linear(x, w)))
@@ -110,7 +131,7 @@ class MabaBlock(WeightCacheMixin, nn.Module):
         self.norm1 = RMSNorm(config.dim, eps=config.rms_norm_eps)
         self.mixer = MabaSparseAttention(config) if self.is_attention else DGDALayer(config)
         self.norm2 = RMSNorm(config.dim, eps=config.rms_norm_eps)
-        self.ffn = SwiGLUFFN(config.dim, config.intermediate_size)
+        self.ffn = SwiGLUFFN(config.dim, config.intermediate_size, config.fused_ffn, config.ffn_checkpoint)
         self.res_gate1 = nn.Parameter(torch.full((config.dim,), config.residual_gate_bias))
         self.res_gate2 = nn.Parameter(torch.full((config.dim,), config.residual_gate_bias))
 
@@ -118,6 +139,8 @@ class MabaBlock(WeightCacheMixin, nn.Module):
         g1 = _frozen(self, "g1", torch.sigmoid, self.res_gate1)
         g2 = _frozen(self, "g2", torch.sigmoid, self.res_gate2)
         x = torch.addcmul(x, g1, mo)
+        if self.ffn.fused:
+            return self.ffn.forward_fused(self.norm2(x), residual=x, gate=g2)
         return torch.addcmul(x, g2, self.ffn(self.norm2(x)))
 
     def forward(self, x, state=None, conv_state=None, past_c_kv=None):

@@ -68,3 +68,378 @@ def test_linear_forward_and_gradients(M, K, N, dt, act, bias, residual, gate):
             assert name not in want
         else:
             B.check(v, want[name], name)
+
+
+# ----------------------------------------------------------------------------- packed activations
+
+
+@pytest.mark.parametrize("dt", [torch.float32, HF, BF])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 31), (5, 32), (2, 3, 33), (64, 640), (7, 1248), (1000, 77), (333, 641)])
+def test_pack_bits_equal_the_reference(shape, dt):
+    r = _gen(sum(shape))
+    x = (r(*shape) * torch.exp2(4 * r(*shape[:-1], 1))).to(dt)
+    x.view(-1)[:: 97] = float("nan")
+    x.view(-1)[3:: 89] = float("inf")
+    x[-1] = 0
+    codes, scales = D.checkpoint_pack(x)
+    rc, rs = C.ref_checkpoint_pack(x.cpu())
+    assert torch.equal(scales.cpu(), rs)
+    nan = torch.isnan(rc.float())
+    got = codes.cpu()
+    assert torch.equal(torch.isnan(got.float()), nan)
+    assert torch.equal(got.view(torch.uint8)[~nan], rc.view(torch.uint8)[~nan])
+    for out in (torch.float32, HF, BF):
+        torch.testing.assert_close(D.checkpoint_unpack(codes, scales, out).cpu(), C.ref_checkpoint_unpack(rc, rs, out), rtol=0,
+                                   atol=0, equal_nan=True)
+
+
+def test_pack_extremes():
+    x = torch.zeros(6, 32, device=DEV)
+    x[0, 3], x[1, 3], x[3, 0] = 3.4e38, 1e-40, 2.0 ** -149
+    x[2, :2] = torch.tensor([448.0, 464.0])
+    x[4] = float("nan")
+    x[5] = torch.arange(32, device=DEV) / 512 - 0.03       # e4m3's subnormals
+    x[5, 0] = 448
+    codes, scales = D.checkpoint_pack(x)
+    rc, rs = C.ref_checkpoint_pack(x.cpu())
+    assert torch.equal(scales.cpu(), rs)
+    for out in (torch.float32, HF, BF):
+        torch.testing.assert_close(D.checkpoint_unpack(codes, scales, out).cpu(), C.ref_checkpoint_unpack(rc, rs, out), rtol=0,
+                                   atol=0, equal_nan=True)
+
+
+def test_pack_reads_and_writes_strided_rows():
+    r = _gen(5)
+    big = r(40, 200).to(BF)
+    for cut in (big[:, 8:72], big[:, 3:80], big[::3, 1:34], big.t()[:, :40], big[:, :1]):
+        codes, scales = D.checkpoint_pack(cut)
+        rc, rs = C.ref_checkpoint_pack(cut.cpu().contiguous())
+        assert torch.equal(codes.cpu().view(torch.uint8), rc.view(torch.uint8)) and torch.equal(scales.cpu(), rs)
+        assert torch.equal(D.checkpoint_unpack(codes, scales, BF).cpu(), C.ref_checkpoint_unpack(rc, rs, BF))
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("M,Cw,I", [(1, 8, 8), (33, 96, 40), (129, 200, 65), (257, 130, 100), (1500, 640, 256), (5000, 512, 1500)])
+def test_gradients_at_a_packed_input(M, Cw, I, dt):
+    x, wg, wu, dh = _gated(M, Cw, I, dt, seed=3)
+    codes, scales = D.checkpoint_pack(x)
+    kept = B.unpack64(codes, scales)
+    want = B.gated(x, wg, wu, dh, kept=kept)
+    for name, got in zip(("dx", "dw_gate", "dw_up"), D.gated_ffn_backward(dh, codes, wg, wu, x_scales=scales)):
+        B.check(got, want[name], name)
+    for act, gate in (("none", True), ("none", False), ("silu", True)):
+        t = _linear(M, Cw, I, dt, seed=4)
+        codes, scales = D.checkpoint_pack(t["x"])
+        g = t["gate"] if gate else None
+        want = B.linear(t["x"], t["w"], t["bias"], act, None, g, t["dy"], kept=B.unpack64(codes, scales))
+        got = D.linear_epilogue_backward(t["dy"], codes, t["w"], t["bias"], act, g, x_scales=scales)
+        for name, v in zip(("dx", "dw", "dbias", "dgate"), got):
+            if v is not None:
+                B.check(v, want[name], (act, name))
+
+
+# ----------------------------------------------------------------------------- layouts
+
+
+def _inside(t, left, right, rows=0, fill=float("nan")):
+    """``t`` as a view of a larger tensor that holds ``fill`` around it."""
+    big = torch.full((t.shape[0] + 2 * rows, left + t.shape[1] + right), fill, dtype=t.dtype, device=t.device)
+    view = big[rows:rows + t.shape[0], left:left + t.shape[1]]
+    view.copy_(t)
+    return view
+
+
+@pytest.mark.parametrize("left,right", [(0, 8), (8, 16), (3, 2), (1, 0), (4, 4), (0, 24)])
+@pytest.mark.parametrize("M,Cw,I", [(5, 40, 24), (70, 72, 40), (300, 136, 72), (64, 21, 19)])
+def test_what_lies_around_the_tensors_does_not_count(M, Cw, I, left, right):
+    x, wg, wu, dh = _gated(M, Cw, I, BF, seed=7)
+    want = B.gated(x, wg, wu, dh)
+    args = [_inside(t, left, right, rows=2) for t in (x, wg, wu)]
+    B.check(D.gated_ffn(*args), want["h"], "h")
+    for name, got in zip(("dx", "dw_gate", "dw_up"), D.gated_ffn_backward(_inside(dh, left, right, rows=2), *args)):
+        B.check(got, want[name], name)
+    # the two weights with strides of their own
+    args[2] = _inside(wu, left + 8, right, rows=1)
+    B.check(D.gated_ffn_backward(dh, *args)[0], want["dx"], "dx")
+    t = _linear(M, Cw, I, BF, seed=8)
+    v = {k: _inside(t[k], left, right, rows=1) for k in ("x", "w", "residual", "dy")}
+    want = B.linear(t["x"], t["w"], t["bias"], "silu", t["residual"], t["gate"], t["dy"])
+    B.check(D.linear_epilogue(v["x"], v["w"], t["bias"], "silu", v["residual"], t["gate"]), want["y"], "y")
+    for act in ("silu", "none"):
+        want = B.linear(t["x"], t["w"], t["bias"], act, t["residual"], t["gate"], t["dy"])
+        for name, got in zip(("dx", "dw", "dbias", "dgate"),
+                             D.linear_epilogue_backward(v["dy"], v["x"], v["w"], t["bias"], act, t["gate"])):
+            B.check(got, want[name], (act, name))
+
+
+def test_outer_shapes_transposed_and_broadcast_inputs():
+    r = _gen(11)
+    x = r(3, 40, 64).to(BF)
+    wg, wu = (r(64, 24) / 8).to(BF).t(), (r(24, 64) / 8).to(BF)              # a transposed weight
+    want = B.gated(x.view(-1, 64), wg, wu)
+    got = D.gated_ffn(x, wg, wu)
+    assert got.shape == (3, 40, 24)
+    B.check(got.view(-1, 24), want["h"], "h")
+    xt = x.transpose(0, 1)                                                    # tokens first
+    B.check(D.gated_ffn(xt, wg, wu).transpose(0, 1).reshape(-1, 24), want["h"], "h")
+    one = r(24).to(BF).requires_grad_()                                       # a broadcast residual, and its gradient
+    w = wu.detach().clone().requires_grad_()
+    y = D.linear_epilogue(x, w, residual=one.expand(3, 40, 24))
+    y.sum().backward()                                                        # a broadcast output gradient
+    assert torch.equal(one.grad.float(), torch.full((24,), 120.0, device=DEV))
+    want = B.linear(x.view(-1, 64), wu, dy=torch.ones(120, 24, device=DEV, dtype=BF))
+    B.check(w.grad, want["dw"], "dw")
+
+
+def test_offsets_past_32_bits():
+    """Rows more than 2^32 bytes into x, dh and the outputs' operands."""
+    M, Cw, I, ld = 70000, 32, 16, 32768
+    big = torch.zeros(M, ld, dtype=BF, device=DEV)                            # 4.6 GB
+    x, wg, wu, dh = _gated(M, Cw, I, BF, seed=13)
+    view = big[:, 64:64 + Cw]
+    view.copy_(x)
+    last = slice(M - 300, M)
+    want = B.gated(x[last], wg, wu, dh[last])
+    B.check(D.gated_ffn(view, wg, wu)[last], want["h"], "h")
+    dx, dwg, _ = D.gated_ffn_backward(dh, view, wg, wu)
+    B.check(dx[last], want["dx"], "dx")
+    B.check(dwg, B.gated(x, wg, wu, dh)["dw_gate"], "dw_gate")
+    big[:, 128:128 + I].copy_(dh)
+    B.check(D.linear_epilogue(view, wg, residual=big[:, 128:128 + I])[last],
+            B.linear(x[last], wg, residual=dh[last])["y"], "y")
+    codes, scales = D.checkpoint_pack(big[:, 61:61 + Cw])                     # unaligned rows
+    rc, rs = C.ref_checkpoint_pack(big[last, 61:61 + Cw].cpu())
+    assert torch.equal(codes[last].cpu().view(torch.uint8), rc.view(torch.uint8)) and torch.equal(scales[last].cpu(), rs)
+
+
+def test_no_rows():
+    x, wg, wu, dh = _gated(4, 40, 24, BF)
+    e = x[:0]
+    assert D.gated_ffn(e, wg, wu).shape == (0, 24)
+    dx, a, b = D.gated_ffn_backward(dh[:0], e, wg, wu)
+    assert dx.shape == (0, 40) and not a.any() and not b.any()
+    for act in ("none", "gelu"):
+        for gate in (None, x.new_ones(24)):
+            assert D.linear_epilogue(e, wg, wg[:, 0].contiguous(), act, dh[:0], gate).shape == (0, 24)
+            got = D.linear_epilogue_backward(dh[:0], e, wg, x.new_ones(24), act, gate)
+            assert got[0].shape == (0, 40) and not any(t.any() for t in got[1:] if t is not None)
+    codes, scales = D.checkpoint_pack(e)
+    assert codes.shape == (0, 40) and scales.shape == (0, 2) and D.checkpoint_unpack(codes, scales).shape == (0, 40)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), 3e38])
+@pytest.mark.parametrize("M", [6, 90])
+def test_a_bad_row_stays_in_its_row(M, bad):
+    x, wg, wu, dh = _gated(M, 48, 40, BF, seed=17)
+    t = _linear(M, 48, 40, BF, seed=18)
+    rows = torch.arange(M, device=DEV) != 3
+    for v in (x, t["x"]):
+        v[3, 5] = bad
+    want = B.gated(x[rows], wg, wu, dh[rows])
+    h = D.gated_ffn(x, wg, wu)
+    B.check(h[rows], want["h"], "h")
+    assert not torch.isfinite(h[3]).all()
+    dx, dwg, _ = D.gated_ffn_backward(dh, x, wg, wu)
+    B.check(dx[rows], want["dx"], "dx")
+    assert not torch.isfinite(dwg).all()
+    want = B.linear(t["x"][rows], t["w"], t["bias"], "gelu", t["residual"][rows], None, t["dy"][rows])
+    B.check(D.linear_epilogue(t["x"], t["w"], t["bias"], "gelu", t["residual"])[rows], want["y"], "y")
+    B.check(D.linear_epilogue_backward(t["dy"], t["x"], t["w"], t["bias"], "gelu")[0][rows], want["dx"], "dx")
+
+
+# ----------------------------------------------------------------------------- calls
+
+
+@pytest.mark.parametrize("needs", [(1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (0, 1, 1), (0, 0, 0)])
+def test_gated_gradients_of_some_inputs(needs):
+    x, wg, wu, dh = _gated(200, 72, 48, BF, seed=19)
+    want = D.gated_ffn_backward(dh, x, wg, wu)
+    got = D.gated_ffn_backward(dh, x, wg, wu, needs=tuple(map(bool, needs)))
+    for n, g, w in zip(needs, got, want):
+        assert torch.equal(g, w) if n else g is None
+
+
+@pytest.mark.parametrize("act", ["none", "silu"])
+@pytest.mark.parametrize("needs", [(1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (0, 0, 1, 1), (1, 0, 0, 1), (0, 0, 0, 0)])
+def test_linear_gradients_of_some_inputs(act, needs):
+    t = _linear(200, 72, 48, BF, seed=20)
+    args = (t["dy"], t["x"], t["w"], t["bias"], act, t["gate"])
+    want = D.linear_epilogue_backward(*args)
+    got = D.linear_epilogue_backward(*args, needs=tuple(map(bool, needs)))
+    for n, g, w in zip(needs, got, want):
+        assert torch.equal(g, w) if n else g is None
+
+
+def test_the_same_bits_every_time_and_on_two_streams():
+    x, wg, wu, dh = _gated(3000, 640, 1248, BF, seed=21)
+    t = _linear(3000, 1248, 640, BF, seed=22)
+
+    def all_of():
+        return [D.gated_ffn(x, wg, wu), *D.gated_ffn_backward(dh, x, wg, wu),
+                *D.linear_epilogue_backward(t["dy"], t["x"], t["w"], t["bias"], "silu", t["gate"]),
+                *D.linear_epilogue_backward(t["dy"], t["x"], t["w"], t["bias"], "none", t["gate"])]
+
+    want = all_of()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(all_of())
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want))
+
+
+def test_out_may_be_the_residual():
+    """The C entry's documented in-place form: out = the residual's own rows."""
+    from maba_sparse import _native as N
+    t = _linear(333, 72, 48, BF, seed=23)
+    want = D.linear_epilogue(t["x"], t["w"], None, "none", t["residual"], t["gate"])
+    y = t["residual"].clone()
+    rc = N.load().maba_hip_linear_epilogue(N.desc(t["x"]), N.desc(t["w"]), None, 0, N.desc(y), N.desc(t["gate"]), N.desc(y), None, 0,
+                                           N.stream_ptr(y.device))
+    N.check(rc, "linear_epilogue")
+    assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("ckpt", [None, "e4m3"])
+@pytest.mark.parametrize("M,Cw,I", [(1, 64, 96), (50, 64, 96), (1000, 200, 136)])
+def test_a_block_trained_through_autograd(M, Cw, I, ckpt):
+    """Both operators in a row, as the model's feed-forward half runs them: each one's gradients against its
+    formulas at the values that it saw."""
+    r = _gen(M)
+    x, res = r(M, Cw).to(BF).requires_grad_(), r(M, Cw).to(BF).requires_grad_()
+    wg, wu, wd = ((r(a, b) / b ** 0.5).to(BF).requires_grad_() for a, b in ((I, Cw), (I, Cw), (Cw, I)))
+    gate = torch.sigmoid(r(Cw)).to(BF).requires_grad_()
+    h = D.gated_ffn(x, wg, wu, checkpoint=ckpt)
+    h.retain_grad()
+    y = D.linear_epilogue(h, wd, residual=res, gate=gate, checkpoint=ckpt)
+    dy = r(M, Cw).to(BF)
+    y.backward(dy)
+
+    def kept(t):
+        return B.unpack64(*D.checkpoint_pack(t.detach())) if ckpt else None
+
+    with torch.no_grad():
+        want = B.linear(h, wd, None, "none", res, gate, dy, kept=kept(h))
+        for got, name in ((y, "y"), (h.grad, "dx"), (wd.grad, "dw"), (gate.grad, "dgate")):
+            B.check(got, want[name], name)
+        assert torch.equal(res.grad, dy)
+        want = B.gated(x, wg, wu, h.grad, kept=kept(x))
+        for got, name in ((h, "h"), (x.grad, "dx"), (wg.grad, "dw_gate"), (wu.grad, "dw_up")):
+            B.check(got, want[name], name)
+
+
+def test_fp32_takes_the_reference_path(monkeypatch):
+    x, wg, wu, dh = _gated(20, 24, 16, torch.float32)
+    with pytest.raises(RuntimeError):                        # strict: a fallback is an error
+        D.gated_ffn(x, wg, wu)
+    monkeypatch.setenv("MABA_STRICT_BACKEND", "0")
+    with pytest.warns(RuntimeWarning):
+        D.clear_fallback_warnings()
+        got = D.gated_ffn(x, wg, wu)
+    torch.testing.assert_close(got, C.ref_gated_ffn(x, wg, wu))
+
+
+def test_model_block_fused_feed_forward():
+    from maba_sparse.model import SwiGLUFFN
+    torch.manual_seed(3)
+    ffn = SwiGLUFFN(640, 1248, fused=True, checkpoint="e4m3").to(DEV, BF)
+    x = torch.randn(2, 300, 640, device=DEV).to(BF)
+    res, gate = torch.randn_like(x), torch.rand(640, device=DEV).to(BF)
+    y = ffn.forward_fused(x, residual=res, gate=gate)
+    y.float().square().mean().backward()
+    assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in ffn.parameters())
+    with torch.no_grad():
+        h = D.gated_ffn(x, ffn.w_gate.weight, ffn.w_up.weight)
+        assert torch.equal(y, D.linear_epilogue(h, ffn.w_down.weight, residual=res, gate=gate))
+        assert torch.equal(ffn(x), ffn.forward_hip(x))
+
+
+# ----------------------------------------------------------------------------- graphs
+
+
+def test_captured_step_replays_with_new_inputs():
+    """Forward and backward ops recorded once, replayed on new data between eager calls of the same ops."""
+    M, Cw, I = 2050, 128, 264
+    x, wg, wu, dh = _gated(M, Cw, I, BF, seed=31)
+    t = _linear(M, I, Cw, BF, seed=32)
+
+    def step():
+        h = D.gated_ffn(x, wg, wu)
+        y = D.linear_epilogue(h, t["w"], t["bias"], "silu", t["residual"], t["gate"])
+        codes, scales = D.checkpoint_pack(h)
+        down = D.linear_epilogue_backward(t["dy"], codes, t["w"], t["bias"], "silu", t["gate"], x_scales=scales)
+        plain = D.linear_epilogue_backward(t["dy"], h, t["w"], t["bias"], "none", t["gate"])
+        up = D.gated_ffn_backward(down[0], x, wg, wu)
+        return [h, y, *down, *plain, *up, D.checkpoint_unpack(codes, scales, BF)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    r = _gen(33)
+    for _ in range(4):
+        for v in (x, dh, t["dy"], t["residual"]):
+            v.copy_(r(*v.shape).to(BF))
+        g.replay()
+        torch.cuda.synchronize()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        torch.cuda.synchronize()
+
+
+def test_captured_autograd_step():
+    """A whole training step recorded through autograd once no eager graph of its leaves lives."""
+    x, wg, wu, dh = _gated(130, 64, 72, BF, seed=35)
+    leaves = [v.requires_grad_() for v in (x, wg, wu)]
+
+    def step():
+        return torch.autograd.grad(D.gated_ffn(*leaves, checkpoint="e4m3"), leaves, dh)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    r = _gen(36)
+    for _ in range(3):
+        with torch.no_grad():
+            x.copy_(r(*x.shape).to(BF))
+        g.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+def test_capture_beside_a_live_eager_graph_is_refused():
+    """The forward of such a capture raises before any backward could reach the eager graph's nodes; the
+    backward ops themselves can be captured beside it."""
+    x, wg, wu, dh = _gated(70, 64, 40, BF, seed=37)
+    w = wg.requires_grad_()
+    eager = D.gated_ffn(x, w, wu)                            # keeps the leaf's node on the current stream
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager autograd graph"):
+        with torch.cuda.graph(g):
+            D.gated_ffn(x, w, wu)
+    torch.cuda.synchronize()
+    g2 = torch.cuda.CUDAGraph()
+    wd = w.detach()
+    with torch.cuda.graph(g2):
+        out = D.gated_ffn_backward(dh, x, wd, wu)
+    g2.replay()
+    torch.cuda.synchronize()
+    (want,) = torch.autograd.grad(eager, (w,), dh)
+    assert torch.equal(out[1], want)
+    del eager
+    gc.collect()
