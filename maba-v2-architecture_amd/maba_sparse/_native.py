@@ -135,16 +135,17 @@ def _declare(lib) -> None:
         "maba_hip_argmax_rows": ([T, T, vp], i),
         "maba_hip_cache_append_heads": ([T, T, vp, T, T, T, T, i, i, T, T, T, T, T, T, vp], i),
         "maba_hip_maba_sa_decode_dev_heads": ([T, T, T, T, T, vp, i64, f, i, i, i, i, T, T, T, vp, sz, vp], i),
-        "maba_hip_gated_ffn_workspace_size": ([T, T, T], sz),
-        "maba_hip_gated_ffn": ([T, T, T, T, vp, sz, vp], i),
-        "maba_hip_gated_ffn_backward_workspace_size": ([T, T, T, T, i], sz),
-        "maba_hip_gated_ffn_backward": ([T, T, T, T, T, T, T, T, vp, sz, vp], i),
-        "maba_hip_linear_epilogue_workspace_size": ([T, T], sz),
-        "maba_hip_linear_epilogue": ([T, T, T, i, T, T, T, vp, sz, vp], i),
-        "maba_hip_linear_epilogue_backward_workspace_size": ([T, T, T, T, i, i, i, i], sz),
-        "maba_hip_linear_epilogue_backward": ([T, T, T, T, T, i, T, T, T, T, T, vp, sz, vp], i),
-        "maba_hip_checkpoint_pack": ([T, T, T, vp], i),
-        "maba_hip_checkpoint_unpack": ([T, T, T, vp], i),
+        # feed-forward operators: descriptors as packed bytes (``rows_desc``) or pointers
+        "maba_hip_gated_ffn_workspace_size": ([vp, vp, vp], sz),
+        "maba_hip_gated_ffn": ([vp, vp, vp, vp, vp, sz, vp], i),
+        "maba_hip_gated_ffn_backward_workspace_size": ([vp, vp, vp, vp, i], sz),
+        "maba_hip_gated_ffn_backward": ([vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp], i),
+        "maba_hip_linear_epilogue_workspace_size": ([vp, vp], sz),
+        "maba_hip_linear_epilogue": ([vp, vp, vp, i, vp, vp, vp, vp, sz, vp], i),
+        "maba_hip_linear_epilogue_backward_workspace_size": ([vp, vp, vp, vp, i, i, i, i], sz),
+        "maba_hip_linear_epilogue_backward": ([vp, vp, vp, vp, vp, i, vp, vp, vp, vp, vp, vp, sz, vp], i),
+        "maba_hip_checkpoint_pack": ([vp, vp, vp, vp], i),
+        "maba_hip_checkpoint_unpack": ([vp, vp, vp, vp], i),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -201,6 +202,20 @@ def desc(t: Optional[torch.Tensor]):
     if t is None:
         return None
     return ctypes.byref(_struct(t))
+
+
+def rows_desc(t: Optional[torch.Tensor]) -> Optional[bytes]:
+    """The ``maba_tensor`` of a 1-D or 2-D tensor as bytes, which a void-pointer argument takes as they are: no
+    ctypes object per tensor (0.5 us against 0.9, of an op call's 15)."""
+    if t is None:
+        return None
+    code = _DTYPE_CODES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"unsupported dtype {t.dtype}")
+    n, st = t.shape, t.stride()
+    if len(n) == 2:
+        return _PACK.pack(t.data_ptr(), code, 2, n[0], n[1], 1, 1, st[0], st[1], 0, 0)
+    return _PACK.pack(t.data_ptr(), code, 1, n[0], 1, 1, 1, st[0], 0, 0, 0)
 
 
 def desc_array(tensors: Sequence[Optional[torch.Tensor]]):

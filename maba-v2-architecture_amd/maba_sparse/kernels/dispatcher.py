@@ -367,23 +367,26 @@ def dispatch_maba_sa_prefill(q, k, v, kh, vh, early, idx, gate_logits, scale: fl
 # ----------------------------------------------------------------------------- feed-forward operators
 
 
-def _ffn_same(x, named) -> None:
+_FFN_DTYPES = frozenset((torch.float32, torch.float16, torch.bfloat16, torch.float64))
+
+
+def _ffn_same(first, /, **named) -> None:
     """One floating dtype and one device for all tensors."""
-    if x.dtype not in (torch.float32, torch.float16, torch.bfloat16, torch.float64):
-        raise TypeError(f"Unsupported dtype {x.dtype}. Supported: "
+    dtype, device = first.dtype, first.device
+    if dtype not in _FFN_DTYPES:
+        raise TypeError(f"Unsupported dtype {dtype}. Supported: "
                         f"{(torch.float32, torch.float16, torch.bfloat16, torch.float64)}")
-    for name, t in named:
+    for name, t in named.items():
         if t is None:
             continue
-        if t.device != x.device:
-            raise RuntimeError(
-                f"Expected all tensors to be on the same device, but got {x.device} and {t.device} for {name}")
-        if t.dtype != x.dtype:
-            raise TypeError(f"Tensor dtypes must match, but got {x.dtype} and {t.dtype} for {name}")
+        if t.device != device:
+            raise RuntimeError(f"Expected all tensors to be on the same device, but got {device} and {t.device} for {name}")
+        if t.dtype != dtype:
+            raise TypeError(f"Tensor dtypes must match, but got {dtype} and {t.dtype} for {name}")
 
 
 def _ffn_shape(name, t, shape) -> None:
-    if t is not None and tuple(t.shape) != tuple(shape):
+    if t is not None and t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
 
 
@@ -458,7 +461,7 @@ def dispatch_gated_ffn(x, w_gate, w_up, checkpoint: Optional[str] = None) -> tor
     fp32 and rounded once.  Differentiable on every backend.  What the backward pass keeps is ``x``; with
     ``checkpoint="e4m3"`` its packed form, half the bytes, and the gradients are those at the unpacked input."""
     _ffn_input(x)
-    _ffn_same(x, (("w_gate", w_gate), ("w_up", w_up)))
+    _ffn_same(x, w_gate=w_gate, w_up=w_up)
     _ffn_weight("w_gate", w_gate, x.shape[-1])
     _ffn_shape("w_up", w_up, w_gate.shape)
     _ffn_checkpoint(checkpoint)
@@ -472,7 +475,7 @@ def dispatch_gated_ffn_backward(dh, x, w_gate, w_up, x_scales=None, needs=(True,
     is false.  ``x`` is the forward's input, or with ``x_scales`` its packed codes.  No autograd takes part."""
     _ffn_input(x)
     _ffn_kept(x, x_scales)
-    _ffn_same(dh, (("x", x if x_scales is None else None), ("w_gate", w_gate), ("w_up", w_up)))
+    _ffn_same(dh, x=x if x_scales is None else None, w_gate=w_gate, w_up=w_up)
     _ffn_weight("w_gate", w_gate, x.shape[-1])
     _ffn_shape("w_up", w_up, w_gate.shape)
     _ffn_shape("dh", dh, (*x.shape[:-1], w_gate.shape[0]))
@@ -490,7 +493,7 @@ def dispatch_linear_epilogue(x, weight, bias=None, activation: str = "none", res
     gate and residual are optional; activation none, relu, silu or gelu (with the error function).  Computed
     in fp32 and rounded once.  Differentiable on every backend; ``checkpoint`` as for ``gated_ffn``."""
     _ffn_input(x)
-    _ffn_same(x, (("weight", weight), ("bias", bias), ("residual", residual), ("gate", gate)))
+    _ffn_same(x, weight=weight, bias=bias, residual=residual, gate=gate)
     _ffn_weight("weight", weight, x.shape[-1])
     n = weight.shape[0]
     _ffn_shape("bias", bias, (n,))
@@ -510,7 +513,7 @@ def dispatch_linear_epilogue_backward(dy, x, weight, bias=None, activation: str 
     ``gated_ffn_backward``.  No autograd takes part."""
     _ffn_input(x)
     _ffn_kept(x, x_scales)
-    _ffn_same(dy, (("x", x if x_scales is None else None), ("weight", weight), ("bias", bias), ("gate", gate)))
+    _ffn_same(dy, x=x if x_scales is None else None, weight=weight, bias=bias, gate=gate)
     _ffn_weight("weight", weight, x.shape[-1])
     n = weight.shape[0]
     _ffn_shape("bias", bias, (n,))

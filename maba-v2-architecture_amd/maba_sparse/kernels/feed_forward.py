@@ -10,6 +10,8 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
+from maba_sparse._native import stream_ptr
+
 
 class GatedFFN(torch.autograd.Function):
     @staticmethod
@@ -65,7 +67,7 @@ def guard_capture(out: torch.Tensor) -> torch.Tensor:
     the stream that it was first seen on, so a capture beside a live eager graph of these operators
     raises here instead."""
     if out.is_cuda and out.grad_fn is not None:
-        stream = torch.cuda.current_stream(out.device).cuda_stream
+        stream = stream_ptr(out.device)
         capturing = torch.cuda.is_current_stream_capturing()
         for node, _ in out.grad_fn.next_functions:
             if node is None or not hasattr(node, "variable"):

@@ -312,42 +312,49 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _row(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+def _vec(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _forward(fn, args, size, size_args, dev: torch.device, what: str) -> None:
+    """``fn`` with no workspace, which is what it needs with every operand aligned, or with one."""
+    rc = fn(*args, None, 0, N.stream_ptr(dev))
+    if rc == N.MABA_ERR_WORKSPACE:
+        ws = _workspace(size(*size_args), dev)
+        rc = fn(*args, ws.data_ptr(), ws.numel(), N.stream_ptr(dev))
+    N.check(rc, what)
 
 
 @register_kernel("hip", "gated_ffn")
 def hip_gated_ffn(x, w_gate, w_up, **kwargs: Any) -> torch.Tensor:
     """``silu(x Wg^T) * (x Wu^T)`` in one launch (contract: ``dispatcher.dispatch_gated_ffn``)."""
     _no_grad_needed("gated_ffn", x, w_gate, w_up)
-    dev = N.require_device([x, w_gate, w_up], "gated_ffn")
+    dev = N.require_device((x, w_gate, w_up), "gated_ffn")
     with N.on_device(dev):
         lib = N.load()
-        x2 = _rows(x)
-        out = torch.empty(x2.shape[0], w_gate.shape[0], dtype=x.dtype, device=dev)
-        dx, dg, du = N.desc(x2), N.desc(_rows(w_gate)), N.desc(_rows(w_up))
-        nbytes = lib.maba_hip_gated_ffn_workspace_size(dx, dg, du)
-        ws = _workspace(nbytes, dev) if nbytes else None
-        rc = lib.maba_hip_gated_ffn(dx, dg, du, N.desc(out), ws.data_ptr() if nbytes else None, nbytes, N.stream_ptr(dev))
-        N.check(rc, "gated_ffn")
-    return out.view(*x.shape[:-1], w_gate.shape[0])
+        x2, wg, wu = _rows(x), _rows(w_gate), _rows(w_up)
+        out = torch.empty(x2.shape[0], wg.shape[0], dtype=x.dtype, device=dev)
+        ins = (N.rows_desc(x2), N.rows_desc(wg), N.rows_desc(wu))
+        _forward(lib.maba_hip_gated_ffn, (*ins, N.rows_desc(out)), lib.maba_hip_gated_ffn_workspace_size, ins, dev, "gated_ffn")
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], wg.shape[0])
 
 
 @register_kernel("hip", "gated_ffn_backward")
 def hip_gated_ffn_backward(dh, x, w_gate, w_up, x_scales=None, needs=(True, True, True), **kwargs: Any):
     """``(dx, dw_gate, dw_up)`` (contract: ``dispatcher.dispatch_gated_ffn_backward``)."""
     _no_grad_needed("gated_ffn_backward", dh, x, w_gate, w_up)
-    dev = N.require_device([dh, x, w_gate, w_up, x_scales], "gated_ffn_backward")
+    dev = N.require_device((dh, x, w_gate, w_up, x_scales), "gated_ffn_backward")
     with N.on_device(dev):
         lib = N.load()
-        x2, sc = _rows(x), None if x_scales is None else _rows(x_scales)
+        dh2, x2, wg, wu = _rows(dh), _rows(x), _rows(w_gate), _rows(w_up)
+        sc = None if x_scales is None else _rows(x_scales)
         dt = w_gate.dtype
         dx = torch.empty(x2.shape, dtype=dt, device=dev) if needs[0] else None
         dws = [torch.empty(w_gate.shape, dtype=dt, device=dev) if n else None for n in needs[1:3]]
-        ddx, dsc, dg, du = N.desc(x2), N.desc(sc), N.desc(_rows(w_gate)), N.desc(_rows(w_up))
-        ws = _workspace(lib.maba_hip_gated_ffn_backward_workspace_size(ddx, dsc, dg, du, bool(needs[0]) + 2 * any(needs[1:3])), dev)
-        rc = lib.maba_hip_gated_ffn_backward(N.desc(_rows(dh)), ddx, dsc, dg, du, N.desc(dx), N.desc(dws[0]),
-                                             N.desc(dws[1]), ws.data_ptr(), ws.numel(), N.stream_ptr(dev))
+        ins = (N.rows_desc(x2), N.rows_desc(sc), N.rows_desc(wg), N.rows_desc(wu))
+        ws = _workspace(lib.maba_hip_gated_ffn_backward_workspace_size(*ins, bool(needs[0]) + 2 * any(needs[1:3])), dev)
+        rc = lib.maba_hip_gated_ffn_backward(N.rows_desc(dh2), *ins, N.rows_desc(dx), N.rows_desc(dws[0]), N.rows_desc(dws[1]),
+                                             ws.data_ptr(), ws.numel(), N.stream_ptr(dev))
         N.check(rc, "gated_ffn_backward")
     return (dx.view(x.shape) if needs[0] else None, *dws)
 
@@ -357,19 +364,17 @@ def hip_linear_epilogue(x, weight, bias=None, activation: str = "none", residual
                         **kwargs: Any) -> torch.Tensor:
     """``residual + gate * act(x W^T + bias)`` in one launch (contract: ``dispatcher.dispatch_linear_epilogue``)."""
     _no_grad_needed("linear_epilogue", x, weight, bias, residual, gate)
-    dev = N.require_device([x, weight, bias, residual, gate], "linear_epilogue")
+    dev = N.require_device((x, weight, bias, residual, gate), "linear_epilogue")
     with N.on_device(dev):
         lib = N.load()
-        x2 = _rows(x)
-        out = torch.empty(x2.shape[0], weight.shape[0], dtype=x.dtype, device=dev)
-        dx, dw = N.desc(x2), N.desc(_rows(weight))
-        nbytes = lib.maba_hip_linear_epilogue_workspace_size(dx, dw)
-        ws = _workspace(nbytes, dev) if nbytes else None
-        rc = lib.maba_hip_linear_epilogue(dx, dw, N.desc(_row(bias)), _ACT_CODES[activation],
-                                          N.desc(None if residual is None else _rows(residual)), N.desc(_row(gate)),
-                                          N.desc(out), ws.data_ptr() if nbytes else None, nbytes, N.stream_ptr(dev))
-        N.check(rc, "linear_epilogue")
-    return out.view(*x.shape[:-1], weight.shape[0])
+        x2, w = _rows(x), _rows(weight)
+        res, bias, gate = None if residual is None else _rows(residual), _vec(bias), _vec(gate)
+        out = torch.empty(x2.shape[0], w.shape[0], dtype=x.dtype, device=dev)
+        ins = (N.rows_desc(x2), N.rows_desc(w))
+        _forward(lib.maba_hip_linear_epilogue, (*ins, N.rows_desc(bias), _ACT_CODES[activation], N.rows_desc(res),
+                                                N.rows_desc(gate), N.rows_desc(out)),
+                 lib.maba_hip_linear_epilogue_workspace_size, ins, dev, "linear_epilogue")
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], w.shape[0])
 
 
 @register_kernel("hip", "linear_epilogue_backward")
@@ -377,20 +382,21 @@ def hip_linear_epilogue_backward(dy, x, weight, bias=None, activation: str = "no
                                  needs=(True, True, True, True), **kwargs: Any):
     """``(dx, dw, dbias, dgate)`` (contract: ``dispatcher.dispatch_linear_epilogue_backward``)."""
     _no_grad_needed("linear_epilogue_backward", dy, x, weight, bias, gate)
-    dev = N.require_device([dy, x, weight, bias, gate, x_scales], "linear_epilogue_backward")
+    dev = N.require_device((dy, x, weight, bias, gate, x_scales), "linear_epilogue_backward")
     with N.on_device(dev):
         lib = N.load()
-        x2, sc = _rows(x), None if x_scales is None else _rows(x_scales)
+        dy2, x2, w = _rows(dy), _rows(x), _rows(weight)
+        sc, bias, gate = None if x_scales is None else _rows(x_scales), _vec(bias), _vec(gate)
         dt, n_out = weight.dtype, weight.shape[0]
         needs = (needs[0], needs[1], needs[2] and bias is not None, needs[3] and gate is not None)
         shapes = (x2.shape, weight.shape, (n_out,), (n_out,))
         outs = [torch.empty(s, dtype=dt, device=dev) if n else None for s, n in zip(shapes, needs)]
-        ddy, ddx, dsc, dw = N.desc(_rows(dy)), N.desc(x2), N.desc(sc), N.desc(_rows(weight))
         act = _ACT_CODES[activation]
+        ins = (N.rows_desc(dy2), N.rows_desc(x2), N.rows_desc(sc), N.rows_desc(w))
         ws = _workspace(lib.maba_hip_linear_epilogue_backward_workspace_size(
-            ddy, ddx, dsc, dw, act, int(bias is not None), int(gate is not None), sum(1 << i for i, n in enumerate(needs) if n)), dev)
-        rc = lib.maba_hip_linear_epilogue_backward(ddy, ddx, dsc, dw, N.desc(_row(bias)), act, N.desc(_row(gate)),
-                                                   *(N.desc(o) for o in outs), ws.data_ptr(), ws.numel(), N.stream_ptr(dev))
+            *ins, act, bias is not None, gate is not None, sum(1 << i for i, n in enumerate(needs) if n)), dev)
+        rc = lib.maba_hip_linear_epilogue_backward(*ins, N.rows_desc(bias), act, N.rows_desc(gate), *map(N.rows_desc, outs),
+                                                   ws.data_ptr(), ws.numel(), N.stream_ptr(dev))
         N.check(rc, "linear_epilogue_backward")
     return (outs[0].view(x.shape) if needs[0] else None, *outs[1:])
 
@@ -398,28 +404,28 @@ def hip_linear_epilogue_backward(dy, x, weight, bias=None, activation: str = "no
 @register_kernel("hip", "checkpoint_pack")
 def hip_checkpoint_pack(x, **kwargs: Any) -> Tuple[torch.Tensor, torch.Tensor]:
     """e4m3 codes and scales of ``x`` (contract: ``common.ref_checkpoint_pack``)."""
-    dev = N.require_device([x], "checkpoint_pack")
+    dev = N.require_device((x,), "checkpoint_pack")
     with N.on_device(dev):
         x2 = _rows(x)
         rows, C = x2.shape
         groups = (C + 31) // 32
         codes = torch.empty(rows, C, dtype=torch.float8_e4m3fn, device=dev)
         scales = torch.empty(rows, groups, dtype=torch.uint8, device=dev)
-        N.check(N.load().maba_hip_checkpoint_pack(N.desc(x2), N.desc(codes), N.desc(scales), N.stream_ptr(dev)),
+        N.check(N.load().maba_hip_checkpoint_pack(N.rows_desc(x2), N.rows_desc(codes), N.rows_desc(scales), N.stream_ptr(dev)),
                 "checkpoint_pack")
-    return codes.view(x.shape), scales.view(*x.shape[:-1], groups)
+    return (codes, scales) if x.dim() == 2 else (codes.view(x.shape), scales.view(*x.shape[:-1], groups))
 
 
 @register_kernel("hip", "checkpoint_unpack")
 def hip_checkpoint_unpack(codes, scales, dtype: torch.dtype = torch.bfloat16, **kwargs: Any) -> torch.Tensor:
     """The values of a packed activation (contract: ``common.ref_checkpoint_unpack``)."""
-    dev = N.require_device([codes, scales], "checkpoint_unpack")
+    dev = N.require_device((codes, scales), "checkpoint_unpack")
     with N.on_device(dev):
-        c2 = _rows(codes)
+        c2, s2 = _rows(codes), _rows(scales)
         out = torch.empty(c2.shape, dtype=dtype, device=dev)
-        N.check(N.load().maba_hip_checkpoint_unpack(N.desc(c2), N.desc(_rows(scales)), N.desc(out), N.stream_ptr(dev)),
+        N.check(N.load().maba_hip_checkpoint_unpack(N.rows_desc(c2), N.rows_desc(s2), N.rows_desc(out), N.stream_ptr(dev)),
                 "checkpoint_unpack")
-    return out.view(codes.shape)
+    return out if codes.dim() == 2 else out.view(codes.shape)
 
 
 # ----------------------------------------------------------------------------- serving path
