@@ -105,18 +105,28 @@ int gemm(GemmArgs g, const typename Epi::Args& e, int64_t M, int64_t N, const Ge
   }
 }
 
-// out [M, N] (16 bits) = a product, Np >= N wide with zeros behind N, through fp32 partials where its plan splits it.
+// A product of M x Np in 16-bit outputs of N columns, through fp32 partials where its plan splits it: rows from
+// `second` on (a multiple of 16, or M and more: none) are the second output's; either may be null, and has `rows` rows.
+struct Outputs {
+  Rows out[2];
+  int second, rows, N;
+};
 template <class T, int AMODE, int BMODE>
-int product_to(const GemmArgs& g, const maba_tensor* out, int64_t M, int64_t N, int64_t Np, const GemmPlan& p, float* part,
-               hipStream_t s, const char* who) {
+int product_to(const GemmArgs& g, const Outputs& o, int64_t M, int64_t Np, const GemmPlan& p, float* part, hipStream_t s,
+               const char* who) {
   if (p.splits == 1) {
-    const EpiStore::Args e = {rows_of(out), (int)M, (int)N};
+    const EpiStore::Args e = {{o.out[0], o.out[1]}, o.second, o.rows, o.N};
     return gemm<T, AMODE, BMODE, EpiStore>(g, e, M, Np, p, s, who);
   }
   const EpiPartial::Args e = {part, (int)M, (int)Np};
   if (int rc = gemm<T, AMODE, BMODE, EpiPartial>(g, e, M, Np, p, s, who)) return rc;
-  ReduceArgs r = {part, p.splits, (int)M, (int)Np, (int)M, (int)M, (int)N, {}};
-  r.out[0] = rows_of(out);
+  const ReduceArgs r = {part, p.splits, (int)M, (int)Np, o.second, o.rows, o.N, {o.out[0], o.out[1]}};
+  return reduce_splits(r, T::CODE, s);
+}
+// Zeros in the outputs, for a sum over no rows.
+template <class T>
+int zeros_to(const Outputs& o, int64_t M, int64_t Np, hipStream_t s) {
+  const ReduceArgs r = {nullptr, 0, (int)M, (int)Np, o.second, o.rows, o.N, {o.out[0], o.out[1]}};
   return reduce_splits(r, T::CODE, s);
 }
 

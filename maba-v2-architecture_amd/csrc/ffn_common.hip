@@ -38,7 +38,7 @@ GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, bool columns, bool may_
       const int64_t n = ceil_div(tiles * splits, cus);
       float us = n * (per * t.full[columns] + t.ends);
       if (n < t.slots) us = std::max(us, per * t.lone[columns] + t.ends);
-      if (splits > 1) us += 2.5f + (float)(M * N) * (4.f * splits + 2.f) / 5e6f;     // reduce_splits, at 5 TB/s
+      if (splits > 1) us += 2.5f + (float)(M * N) * (8.f * splits + 2.f) / 5e6f;     // the partials, at 5 TB/s
       if (least == 0.f || us < least) {
         least = us;
         best = {i, (int)splits, (int)per, (int)ceil_div(M, t.bm)};

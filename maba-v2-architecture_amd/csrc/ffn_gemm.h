@@ -397,17 +397,22 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) 
   Epi::template run<T, BM, BN, WM, WN, MI, NI>(e, acc, t, m0 + wm, n0 + wn, c, q, wave, lds);
 }
 
-// Epilogue: C as it is, rounded once to 16 bits.
+// Epilogue: C as it is, rounded once to 16 bits; from row `second` on it goes to the second tensor's rows (`second`
+// is a multiple of 16).  M: rows of each.
 struct EpiStore {
-  struct Args { Rows c; int M, N; };
+  struct Args { Rows c[2]; int second, M, N; };
   template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
   static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
                                              int q, int wave, uint16_t* lds) {
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+    for (int i = 0; i < MI; ++i) {
+      const int at = m0 + 16 * i >= e.second, m = m0 + 16 * i - (at ? e.second : 0) + c;
+      const Rows r = at ? e.c[1] : e.c[0];
+      if (!r.p) continue;
 #pragma unroll
       for (int j = 0; j < NI; j += 2)
-        store8(e.c, m0 + 16 * i + c, n0 + 16 * j + 8 * q, e.M, e.N, eight_of({down4<T>(acc[i][j]), down4<T>(acc[i][j + 1])}));
+        store8(r, m, n0 + 16 * j + 8 * q, e.M, e.N, eight_of({down4<T>(acc[i][j]), down4<T>(acc[i][j + 1])}));
+    }
   }
 };
 

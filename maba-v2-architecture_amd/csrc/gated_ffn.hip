@@ -56,9 +56,9 @@ struct EpiGated {
   }
 };
 
-// d [M, 2 Ip], Ip = I rounded up to 8: dg at column 0, du at column Ip, zeros behind each.
+// d [M, 2 Iw], Iw = I rounded up to 16: dg at column 0, du at column Iw, zeros behind each.
 struct EpiGatedBack {
-  struct Args { Rows dh, d; int M, I, Ip; };
+  struct Args { Rows dh, d; int M, I, Iw; };
   static __device__ __forceinline__ void grads(f32x4 g, f32x4 u, f32x4 dh, f32x4& dg, f32x4& du) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -86,10 +86,10 @@ struct EpiGatedBack {
           f32x4 dg[2], du[2];
           grads(acc[i][4 * j], acc[i][4 * j + 1], up4<T>(d.a), dg[0], du[0]);
           grads(acc[i][4 * j + 2], acc[i][4 * j + 3], up4<T>(d.b), dg[1], du[1]);
-          store8(e.d, m, n, e.M, e.Ip, eight_of({down4<T>(dg[0]), down4<T>(dg[1])}));
-          // columns behind Ip would be du's neighbours: none is stored there
+          store8(e.d, m, n, e.M, e.Iw, eight_of({down4<T>(dg[0]), down4<T>(dg[1])}));
+          // columns behind Iw would be du's neighbours: none is stored there
           const u32x4 u = eight_of({down4<T>(du[0]), down4<T>(du[1])});
-          if (n < e.Ip) store8(e.d, m, e.Ip + n, e.M, 2 * e.Ip, u);
+          if (n < e.Iw) store8(e.d, m, e.Iw + n, e.M, 2 * e.Iw, u);
         }
       }
     } else {
@@ -99,11 +99,11 @@ struct EpiGatedBack {
 #pragma unroll
         for (int j = 0; j < NI; j += 2) {
           const int n = n0 / 2 + 8 * j + 4 * q;
-          if (m >= e.M || n >= e.Ip) continue;
+          if (m >= e.M || n >= e.Iw) continue;
           f32x4 dg, du;
           grads(acc[i][j], acc[i][j + 1], up4<T>(load4(e.dh, m, n, e.I)), dg, du);
-          store4<T>(e.d, m, n, e.Ip, dg);
-          store4<T>(e.d, m, e.Ip + n, 2 * e.Ip, du);
+          store4<T>(e.d, m, n, e.Iw, dg);
+          store4<T>(e.d, m, e.Iw + n, 2 * e.Iw, du);
         }
       }
     }
@@ -112,7 +112,7 @@ struct EpiGatedBack {
 
 // Where everything of a call lies: operands in place or copied into the workspace.
 struct GatedPlan {
-  int64_t M, C, I, Cp, Ip;
+  int64_t M, C, I, Cp, Iw;       // widths padded to 8 (C) and to 16 (I, a half of [dg | du])
   bool copy_x, copy_w[2];
   uint16_t *x, *w[2], *d;
   float* part;             // fp32 partials, of dx and then of the weights
@@ -127,7 +127,7 @@ static GatedPlan gated_plan(const maba_tensor* x, const maba_tensor* scales, con
   p.C = x->shape[1];
   p.I = wg->shape[0];
   p.Cp = pad8(p.C);
-  p.Ip = pad8(p.I);
+  p.Iw = ceil_div(p.I, 16) * 16;
   const bool few = !back && p.M <= SKINNY_ROWS;       // that kernel reads any rows
   p.copy_x = !few && (scales || !aligned_rows(x));
   // dx reads both weights with one stride
@@ -139,19 +139,19 @@ static GatedPlan gated_plan(const maba_tensor* x, const maba_tensor* scales, con
   for (int i = 0; i < 2; ++i)
     if (p.copy_w[i]) p.w[i] = c.take<uint16_t>(p.I * p.Cp);
   if (back) {
-    p.d = c.take<uint16_t>(p.M * 2 * p.Ip);
+    p.d = c.take<uint16_t>(p.M * 2 * p.Iw);
     int64_t part = 0;
     if (dx) {
-      p.dx = gemm_plan(p.M, p.Cp, gemm_stages(p.Ip, 2), true, true);
+      p.dx = gemm_plan(p.M, p.Cp, gemm_stages(p.Iw, 2), true, true);
       if (p.dx.splits > 1) part = (int64_t)p.dx.splits * p.M * p.Cp;
     }
     if (dw) {
-      p.dw = gemm_plan(2 * p.Ip, p.Cp, gemm_stages(p.M, 1), true, true);
-      part = std::max(part, (int64_t)p.dw.splits * 2 * p.Ip * p.Cp);
+      p.dw = gemm_plan(2 * p.Iw, p.Cp, gemm_stages(p.M, 1), true, true);
+      part = std::max(part, (int64_t)p.dw.splits * 2 * p.Iw * p.Cp);
     }
     p.part = c.take<float>(part);
   }
-  p.gu = gemm_plan(p.M, 2 * ceil_div(p.I, 16) * 16, gemm_stages(p.Cp, 1), false, false);
+  p.gu = gemm_plan(p.M, 2 * p.Iw, gemm_stages(p.Cp, 1), false, false);
   p.bytes = c.used;
   return p;
 }
@@ -186,7 +186,7 @@ static int gated_forward(GatedPlan& p, const maba_tensor* x, const maba_tensor* 
   GemmArgs g = {};
   if (int rc = gated_operands(p, x, nullptr, wg, wu, s, g.a, g.b)) return rc;
   g.K = p.Cp;
-  return gemm<T, K_ROWS, K_ROWS_PAIR, EpiGated>(g, e, p.M, 2 * ceil_div(p.I, 16) * 16, p.gu, s, who);
+  return gemm<T, K_ROWS, K_ROWS_PAIR, EpiGated>(g, e, p.M, 2 * p.Iw, p.gu, s, who);
 }
 
 template <class T>
@@ -195,37 +195,33 @@ static int gated_backward(GatedPlan& p, const maba_tensor* dh, const maba_tensor
                           hipStream_t s, const char* who) {
   Operand ox, ow;
   if (int rc = gated_operands(p, x, scales, wg, wu, s, ox, ow)) return rc;
-  const Operand d = rows_operand(p.d, 2 * p.Ip, p.M);
+  const Operand d = rows_operand(p.d, 2 * p.Iw, p.M);
   if (p.M > 0) {
     GemmArgs g = {};
     g.a = ox;
     g.b = ow;
     g.K = p.Cp;
-    const Rows rd = {p.d, 2 * p.Ip};
-    const EpiGatedBack::Args e = {rows_of(dh), rd, (int)p.M, (int)p.I, (int)p.Ip};
-    if (int rc = gemm<T, K_ROWS, K_ROWS_PAIR, EpiGatedBack>(g, e, p.M, 2 * ceil_div(p.I, 16) * 16, p.gu, s, who)) return rc;
+    const Rows rd = {p.d, 2 * p.Iw};
+    const EpiGatedBack::Args e = {rows_of(dh), rd, (int)p.M, (int)p.I, (int)p.Iw};
+    if (int rc = gemm<T, K_ROWS, K_ROWS_PAIR, EpiGatedBack>(g, e, p.M, 2 * p.Iw, p.gu, s, who)) return rc;
   }
   if (dx && p.M > 0) {
     GemmArgs g = {};
     g.a = d;
     g.b = cols_operand(ow, p.Cp);
-    g.K = p.Ip;
+    g.K = p.Iw;
     g.segments = 2;
-    if (int rc = product_to<T, K_ROWS, K_COLS>(g, dx, p.M, p.C, p.Cp, p.dx, p.part, s, who)) return rc;
+    const Outputs o = {{rows_of(dx), rows_of(nullptr)}, INT32_MAX, (int)p.M, (int)p.C};
+    if (int rc = product_to<T, K_ROWS, K_COLS>(g, o, p.M, p.Cp, p.dx, p.part, s, who)) return rc;
   }
   if (dwg || dwu) {
-    if (p.M > 0) {
-      GemmArgs g = {};
-      g.a = cols_operand(d, 2 * p.Ip);
-      g.b = cols_operand(ox, p.Cp);
-      g.K = p.M;
-      const EpiPartial::Args e = {p.part, (int)(2 * p.Ip), (int)p.Cp};
-      if (int rc = gemm<T, K_COLS, K_COLS, EpiPartial>(g, e, 2 * p.Ip, p.Cp, p.dw, s, who)) return rc;
-    }
-    ReduceArgs r = {p.part, p.M > 0 ? p.dw.splits : 0, (int)(2 * p.Ip), (int)p.Cp, (int)p.Ip, (int)p.I, (int)p.C, {}};
-    r.out[0] = rows_of(dwg);
-    r.out[1] = rows_of(dwu);
-    if (int rc = reduce_splits(r, wg->dtype, s)) return rc;
+    const Outputs o = {{rows_of(dwg), rows_of(dwu)}, (int)p.Iw, (int)p.I, (int)p.C};
+    if (p.M == 0) return zeros_to<T>(o, 2 * p.Iw, p.Cp, s);
+    GemmArgs g = {};
+    g.a = cols_operand(d, 2 * p.Iw);
+    g.b = cols_operand(ox, p.Cp);
+    g.K = p.M;
+    if (int rc = product_to<T, K_COLS, K_COLS>(g, o, 2 * p.Iw, p.Cp, p.dw, p.part, s, who)) return rc;
   }
   return MABA_OK;
 }

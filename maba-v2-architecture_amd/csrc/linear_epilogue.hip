@@ -297,25 +297,26 @@ static int linear_backward(LinearPlan& p, const maba_tensor* dy, const maba_tens
     g.a = dz;
     g.b = cols_operand(ow, p.Kp);
     g.K = p.Np;                 // dz is N wide where N is a whole number of chunks, padded with zeros otherwise
-    if (int rc = product_to<T, K_ROWS, K_COLS>(g, dx, p.M, p.K, p.Kp, p.dx, p.part, s, who)) return rc;
+    const Outputs o = {{rows_of(dx), rows_of(nullptr)}, INT32_MAX, (int)p.M, (int)p.K};
+    if (int rc = product_to<T, K_ROWS, K_COLS>(g, o, p.M, p.Kp, p.dx, p.part, s, who)) return rc;
   }
   if (p.g) {
-    if (p.M > 0) {
-      GemmArgs g = {};
-      g.a = cols_operand(dz, p.Np);
-      g.b = cols_operand(ox, p.Kp);
-      g.K = p.M;
-      const EpiPartial::Args e = {p.part, (int)p.Np, (int)p.Kp};
-      if (int rc = gemm<T, K_COLS, K_COLS, EpiPartial>(g, e, p.Np, p.Kp, p.dw, s, who)) return rc;
-    }
-    ReduceArgs r = {p.part, p.M > 0 ? p.dw.splits : 0, (int)p.Np, (int)p.Kp, (int)p.Np, (int)p.N, (int)p.K, {}};
-    r.out[0] = rows_of(dw);
+    GemmArgs g = {};
+    g.a = cols_operand(dz, p.Np);
+    g.b = cols_operand(ox, p.Kp);
+    g.K = p.M;
     if (!p.z && gate) {
-      const GatedReduceArgs a = {p.part, r.splits, (int)p.Np, (int)p.Kp, (int)p.K, rows_of(dw), rows_of(w), vec_of(gate),
-                                 vec_of(bias), p.colsum, dgate ? (uint16_t*)dgate->data : nullptr};
+      if (p.M > 0) {
+        const EpiPartial::Args e = {p.part, (int)p.Np, (int)p.Kp};
+        if (int rc = gemm<T, K_COLS, K_COLS, EpiPartial>(g, e, p.Np, p.Kp, p.dw, s, who)) return rc;
+      }
+      const GatedReduceArgs a = {p.part, p.M > 0 ? p.dw.splits : 0, (int)p.Np, (int)p.Kp, (int)p.K, rows_of(dw), rows_of(w),
+                                 vec_of(gate), vec_of(bias), p.colsum, dgate ? (uint16_t*)dgate->data : nullptr};
       return reduce_gated(a, (int)p.N, w->dtype, s);
     }
-    if (int rc = reduce_splits(r, w->dtype, s)) return rc;
+    const Outputs o = {{rows_of(dw), rows_of(nullptr)}, INT32_MAX, (int)p.N, (int)p.K};
+    if (p.M == 0) return zeros_to<T>(o, p.Np, p.Kp, s);
+    if (int rc = product_to<T, K_COLS, K_COLS>(g, o, p.Np, p.Kp, p.dw, p.part, s, who)) return rc;
   }
   return MABA_OK;
 }
