@@ -69,6 +69,7 @@ int column_partials(const maba_tensor* src, float* p, hipStream_t s);
 // The tiles: BM, BN, waves along m and n.
 struct Tile256 { static constexpr int BM = 256, BN = 256, WM = 2, WN = 4; };
 struct Tile192 { static constexpr int BM = 192, BN = 128, WM = 2, WN = 2; };
+struct Tile160 { static constexpr int BM = 128, BN = 160, WM = 4, WN = 1; };
 struct Tile128 { static constexpr int BM = 128, BN = 128, WM = 2, WN = 2; };
 struct Tile64 { static constexpr int BM = 64, BN = 64, WM = 2, WN = 2; };
 
@@ -77,8 +78,9 @@ struct Tile64 { static constexpr int BM = 64, BN = 64, WM = 2, WN = 2; };
 struct GemmPlan {
   int tile, splits, split_stages, tiles_m;
 };
-// columns: an operand is read along its columns.
-GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, bool columns, bool may_split);
+enum { PLAN_COLUMNS = 1, PLAN_SPLIT = 2, PLAN_PAIRS = 4 };     // an operand is read along its columns; the sum may be
+                                                               // split; the columns are a gate's and an up's by turns
+GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, int what);
 
 template <class T, class Tile, int AMODE, int BMODE, class Epi>
 int gemm_tile(GemmArgs& g, const typename Epi::Args& e, int64_t M, int64_t N, int splits, hipStream_t s, const char* who) {
@@ -100,7 +102,10 @@ int gemm(GemmArgs g, const typename Epi::Args& e, int64_t M, int64_t N, const Ge
   switch (p.tile) {
     case 0: return gemm_tile<T, Tile256, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
     case 1: return gemm_tile<T, Tile192, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
-    case 2: return gemm_tile<T, Tile128, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
+    case 2:
+      if constexpr (BMODE != K_ROWS_PAIR) return gemm_tile<T, Tile160, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
+      else return fail(MABA_ERR_INVALID, "%s: no such tile", who);
+    case 3: return gemm_tile<T, Tile128, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
     default: return gemm_tile<T, Tile64, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
   }
 }

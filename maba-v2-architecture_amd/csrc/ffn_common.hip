@@ -10,26 +10,30 @@ namespace ffn {
 // each its stages at `full` and `ends` for its first loads and its epilogue; with fewer than `slots`, which is what it
 // holds at once, a stage's latency (`lone`) bounds it.  Measured on MI355X, us, with an operand read along its columns
 // in brackets:
-//              256 x 256      192 x 128      128 x 128      64 x 64
-//   full       1.36 (1.38)    0.55 (0.63)    0.41 (0.48)    0.20 (0.25)
-//   lone       1.36 (1.38)    0.80 (1.00)    0.60 (0.74)    0.36 (0.47)
-//   ends       7.6            4              3              0.75
-// (4,096 x 11,008 x 2,048, rows: 152, 172, 178 us with the first three; 16,384 x 640 x 2,496, columns: 69, 62, 82;
-// 2,048 x 2,496 x 640, rows: 20, 14.3, 14.3 and 16.7; 64 x 640 x 2,496 with the last, in 1, 4 and 8 splits: 19.9,
-// 7.2 and 5.2.)
+//              256 x 256      192 x 128      128 x 160      128 x 128      64 x 64
+//   full       1.36 (1.38)    0.55 (0.63)    0.57 (0.64)    0.46 (0.48)    0.20 (0.25)
+//   lone       1.36 (1.38)    0.80 (1.00)    0.75 (0.95)    0.60 (0.74)    0.36 (0.47)
+//   ends       7.6            4              3              3              0.75
+// (4,096 x 11,008 x 2,048, rows: 152, 172, 221, 178 us with the first four; 16,384 x 640 x 2,496, columns: 70, 63, 58,
+// 81, and 32,768 x 640 x 1,248, rows: 70, 62, 59, 66, where 160 columns leave no part of a tile over; 2,048 x 2,496 x 640,
+// rows: 20, 14.3, -, 14.3 and 16.7; 64 x 640 x 2,496 with the last, in 1, 4 and 8 splits: 19.9, 7.2 and 5.2.)
 struct TileCost { int bm, bn, slots; float full[2], lone[2], ends; };
-static const TileCost TILES[4] = {{256, 256, 1, {1.36f, 1.38f}, {1.36f, 1.38f}, 7.6f},
-                                  {192, 128, 2, {0.55f, 0.63f}, {0.80f, 1.00f}, 4.f},
-                                  {128, 128, 2, {0.41f, 0.48f}, {0.60f, 0.74f}, 3.f},
-                                  {64, 64, 5, {0.20f, 0.25f}, {0.36f, 0.47f}, 0.75f}};
+constexpr int TILE_COUNT = 5;
+static const TileCost TILES[TILE_COUNT] = {{256, 256, 1, {1.36f, 1.38f}, {1.36f, 1.38f}, 7.6f},
+                                           {192, 128, 2, {0.55f, 0.63f}, {0.80f, 1.00f}, 4.f},
+                                           {128, 160, 2, {0.57f, 0.64f}, {0.75f, 0.95f}, 3.f},
+                                           {128, 128, 2, {0.46f, 0.48f}, {0.60f, 0.74f}, 3.f},
+                                           {64, 64, 5, {0.20f, 0.25f}, {0.36f, 0.47f}, 0.75f}};
 
-GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, bool columns, bool may_split) {
+GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, int what) {
+  const bool columns = what & PLAN_COLUMNS, may_split = what & PLAN_SPLIT;
   const int64_t cus = device_cu_count();
   stages = std::max<int64_t>(stages, 1);      // no rows: nothing is launched
-  GemmPlan best = {3, 1, (int)stages, 0};
+  GemmPlan best = {TILE_COUNT - 1, 1, (int)stages, 0};
   float least = 0.f;
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < TILE_COUNT; ++i) {
     const TileCost& t = TILES[i];
+    if (t.bn % 64 && (what & PLAN_PAIRS)) continue;      // whose epilogue takes 64 columns at a time
     const int64_t tiles = ceil_div(M, t.bm) * ceil_div(N, t.bn);
     const int most = may_split ? (int)std::max<int64_t>(1, std::min<int64_t>({32, stages / 2, 8 * cus / std::max<int64_t>(tiles, 1)})) : 1;
     for (int want = 1; want <= most; ++want) {

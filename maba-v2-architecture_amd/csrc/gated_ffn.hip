@@ -142,16 +142,16 @@ static GatedPlan gated_plan(const maba_tensor* x, const maba_tensor* scales, con
     p.d = c.take<uint16_t>(p.M * 2 * p.Iw);
     int64_t part = 0;
     if (dx) {
-      p.dx = gemm_plan(p.M, p.Cp, gemm_stages(p.Iw, 2), true, true);
+      p.dx = gemm_plan(p.M, p.Cp, gemm_stages(p.Iw, 2), PLAN_COLUMNS | PLAN_SPLIT);
       if (p.dx.splits > 1) part = (int64_t)p.dx.splits * p.M * p.Cp;
     }
     if (dw) {
-      p.dw = gemm_plan(2 * p.Iw, p.Cp, gemm_stages(p.M, 1), true, true);
+      p.dw = gemm_plan(2 * p.Iw, p.Cp, gemm_stages(p.M, 1), PLAN_COLUMNS | PLAN_SPLIT);
       part = std::max(part, (int64_t)p.dw.splits * 2 * p.Iw * p.Cp);
     }
     p.part = c.take<float>(part);
   }
-  p.gu = gemm_plan(p.M, 2 * p.Iw, gemm_stages(p.Cp, 1), false, false);
+  p.gu = gemm_plan(p.M, 2 * p.Iw, gemm_stages(p.Cp, 1), PLAN_PAIRS);
   p.bytes = c.used;
   return p;
 }

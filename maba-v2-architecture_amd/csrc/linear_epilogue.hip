@@ -206,16 +206,16 @@ static LinearPlan linear_plan(const maba_tensor* x, const maba_tensor* scales, c
     if (p.z || p.copy_dy) p.dz = c.take<uint16_t>(p.M * p.Np);
     int64_t part = 0;
     if (need->dx) {
-      p.dx = gemm_plan(p.M, p.Kp, gemm_stages(p.Np, 1), true, true);
+      p.dx = gemm_plan(p.M, p.Kp, gemm_stages(p.Np, 1), PLAN_COLUMNS | PLAN_SPLIT);
       if (p.dx.splits > 1) part = (int64_t)p.dx.splits * p.M * p.Kp;
     }
     if (p.g) {
-      p.dw = gemm_plan(p.Np, p.Kp, gemm_stages(p.M, 1), true, true);
+      p.dw = gemm_plan(p.Np, p.Kp, gemm_stages(p.M, 1), PLAN_COLUMNS | PLAN_SPLIT);
       part = std::max(part, (int64_t)p.dw.splits * p.Np * p.Kp);
     }
     p.part = c.take<float>(part);
   }
-  p.xw = gemm_plan(p.M, p.Np, gemm_stages(p.Kp, 1), false, false);
+  p.xw = gemm_plan(p.M, p.Np, gemm_stages(p.Kp, 1), 0);
   p.cols = need && (need->dbias || (need->dgate && (p.z || bias)));
   if (p.cols) {
     p.colsum = c.take<float>(p.N);
