@@ -91,7 +91,9 @@ int skinny(const SkinnyArgs& a, const typename Epi::Args& e, hipStream_t s, cons
   hipLaunchKernelGGL(k, grid, dim3(64 * SKINNY_NW), 0, s, a, e);
   return check_launch(who);
 }
-constexpr int SKINNY_ROWS = 32;
+// Whether M rows of K go this way.  Every workgroup reads all of x, so that more than 16 rows of a long k are better
+// off in tiles with their sum split.
+inline bool few_rows(int64_t M, int64_t K) { return M <= 16 || (M <= 32 && K <= 2048); }
 
 }  // namespace ffn
 }  // namespace maba

@@ -110,6 +110,24 @@ struct EpiGatedBack {
   }
 };
 
+// The forward's sum split over few rows' long k: h from the partial products' sums [splits][M][2 Iw], in split order.
+template <class T>
+__global__ __launch_bounds__(256) void reduce_gated_forward(const float* p, int splits, int64_t plane, int Iw, EpiGated::Args e) {
+  const int quads = Iw / 4;
+  const int64_t total = (int64_t)e.M * quads;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int m = (int)(i / quads), n = (int)(i % quads) * 4;
+    if (n >= e.I) continue;
+    const float* at = p + (int64_t)m * 2 * Iw + 2 * (n & ~15) + (n & 15);
+    f32x4 g = {0.f, 0.f, 0.f, 0.f}, u = g;
+    for (int s = 0; s < splits; ++s) {
+      g += *(const f32x4*)(at + s * plane);
+      u += *(const f32x4*)(at + s * plane + 16);
+    }
+    EpiGated::quad<T>(e, m, n, g, u);
+  }
+}
+
 // Where everything of a call lies: operands in place or copied into the workspace.
 struct GatedPlan {
   int64_t M, C, I, Cp, Iw;       // widths padded to 8 (C) and to 16 (I, a half of [dg | du])
@@ -128,7 +146,7 @@ static GatedPlan gated_plan(const maba_tensor* x, const maba_tensor* scales, con
   p.I = wg->shape[0];
   p.Cp = pad8(p.C);
   p.Iw = ceil_div(p.I, 16) * 16;
-  const bool few = !back && p.M <= SKINNY_ROWS;       // that kernel reads any rows
+  const bool few = !back && few_rows(p.M, p.C);       // that kernel reads any rows
   p.copy_x = !few && (scales || !aligned_rows(x));
   // dx reads both weights with one stride
   const bool apart = back && wg->stride[0] != wu->stride[0];
@@ -151,7 +169,8 @@ static GatedPlan gated_plan(const maba_tensor* x, const maba_tensor* scales, con
     }
     p.part = c.take<float>(part);
   }
-  p.gu = gemm_plan(p.M, 2 * p.Iw, gemm_stages(p.Cp, 1), PLAN_PAIRS);
+  p.gu = gemm_plan(p.M, 2 * p.Iw, gemm_stages(p.Cp, 1), PLAN_PAIRS | (back || few ? 0 : PLAN_SPLIT));
+  if (p.gu.splits > 1) p.part = c.take<float>((int64_t)p.gu.splits * p.M * 2 * p.Iw);
   p.bytes = c.used;
   return p;
 }
@@ -177,7 +196,7 @@ template <class T>
 static int gated_forward(GatedPlan& p, const maba_tensor* x, const maba_tensor* wg, const maba_tensor* wu, maba_tensor* out,
                          hipStream_t s, const char* who) {
   const EpiGated::Args e = {rows_of(out), (int)p.M, (int)p.I};
-  if (p.M <= SKINNY_ROWS) {
+  if (few_rows(p.M, p.C)) {
     SkinnyArgs a = {(const uint16_t*)x->data, x->stride[0], {(const uint16_t*)wg->data, (const uint16_t*)wu->data},
                     {wg->stride[0], wu->stride[0]}, (int)p.M, (int)p.I, (int)p.C, aligned_rows(x),
                     aligned_rows(wg) && aligned_rows(wu)};
@@ -186,7 +205,12 @@ static int gated_forward(GatedPlan& p, const maba_tensor* x, const maba_tensor* 
   GemmArgs g = {};
   if (int rc = gated_operands(p, x, nullptr, wg, wu, s, g.a, g.b)) return rc;
   g.K = p.Cp;
-  return gemm<T, K_ROWS, K_ROWS_PAIR, EpiGated>(g, e, p.M, 2 * p.Iw, p.gu, s, who);
+  if (p.gu.splits == 1) return gemm<T, K_ROWS, K_ROWS_PAIR, EpiGated>(g, e, p.M, 2 * p.Iw, p.gu, s, who);
+  const EpiPartial::Args ep = {p.part, (int)p.M, (int)(2 * p.Iw)};
+  if (int rc = gemm<T, K_ROWS, K_ROWS_PAIR, EpiPartial>(g, ep, p.M, 2 * p.Iw, p.gu, s, who)) return rc;
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(p.M * (p.Iw / 4), 256), 16384));
+  hipLaunchKernelGGL(reduce_gated_forward<T>, grid, dim3(256), 0, s, p.part, p.gu.splits, p.M * 2 * p.Iw, (int)p.Iw, e);
+  return check_launch(who);
 }
 
 template <class T>

@@ -170,6 +170,21 @@ struct EpiLinearBack {
   }
 };
 
+// The forward's sum split over few rows' long k: y from the partial products' sums [splits][M][Np], in split order.
+template <class T, int ACT>
+__global__ __launch_bounds__(256) void reduce_linear_forward(const float* p, int splits, int64_t plane, int Np,
+                                                             typename EpiLinear<ACT>::Args e) {
+  const int quads = Np / 4;
+  const int64_t total = (int64_t)e.M * quads;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int m = (int)(i / quads), n = (int)(i % quads) * 4;
+    if (n >= e.N) continue;
+    f32x4 z = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s) z += *(const f32x4*)(p + s * plane + (int64_t)m * Np + n);
+    EpiLinear<ACT>::template quad<T>(e, m, n, z, z);
+  }
+}
+
 struct LinearPlan {
   int64_t M, N, K, Kp, Np, sum_rows;
   bool copy_x, copy_w, copy_dy, z;      // z: dz is made from z, otherwise the products take dy
@@ -190,7 +205,7 @@ static LinearPlan linear_plan(const maba_tensor* x, const maba_tensor* scales, c
   p.N = w->shape[0];
   p.Kp = pad8(p.K);
   p.Np = pad8(p.N);
-  const bool few = !need && p.M <= SKINNY_ROWS;
+  const bool few = !need && few_rows(p.M, p.K);
   p.z = need && act != ACT_NONE;
   // the sum over tokens that dW and, without z, dgate come from
   p.g = need && (need->dw || (!p.z && need->dgate));
@@ -215,7 +230,8 @@ static LinearPlan linear_plan(const maba_tensor* x, const maba_tensor* scales, c
     }
     p.part = c.take<float>(part);
   }
-  p.xw = gemm_plan(p.M, p.Np, gemm_stages(p.Kp, 1), 0);
+  p.xw = gemm_plan(p.M, p.Np, gemm_stages(p.Kp, 1), need || few ? 0 : PLAN_SPLIT);
+  if (p.xw.splits > 1) p.part = c.take<float>((int64_t)p.xw.splits * p.M * p.Np);
   p.cols = need && (need->dbias || (need->dgate && (p.z || bias)));
   if (p.cols) {
     p.colsum = c.take<float>(p.N);
@@ -245,7 +261,7 @@ static int linear_forward(LinearPlan& p, const maba_tensor* x, const maba_tensor
                           const maba_tensor* res, const maba_tensor* gate, maba_tensor* y, hipStream_t s, const char* who) {
   typedef EpiLinear<ACT> E;
   const typename E::Args e = {rows_of(y), rows_of(res), vec_of(bias), vec_of(gate), (int)p.M, (int)p.N};
-  if (p.M <= SKINNY_ROWS) {
+  if (few_rows(p.M, p.K)) {
     const uint16_t* wp = (const uint16_t*)w->data;
     SkinnyArgs a = {(const uint16_t*)x->data, x->stride[0], {wp, wp}, {w->stride[0], w->stride[0]}, (int)p.M, (int)p.N,
                     (int)p.K, aligned_rows(x), aligned_rows(w)};
@@ -254,7 +270,12 @@ static int linear_forward(LinearPlan& p, const maba_tensor* x, const maba_tensor
   GemmArgs g = {};
   if (int rc = linear_operands(p, x, nullptr, w, nullptr, nullptr, s, g.a, g.b)) return rc;
   g.K = p.Kp;
-  return gemm<T, K_ROWS, K_ROWS, E>(g, e, p.M, p.Np, p.xw, s, who);
+  if (p.xw.splits == 1) return gemm<T, K_ROWS, K_ROWS, E>(g, e, p.M, p.Np, p.xw, s, who);
+  const EpiPartial::Args ep = {p.part, (int)p.M, (int)p.Np};
+  if (int rc = gemm<T, K_ROWS, K_ROWS, EpiPartial>(g, ep, p.M, p.Np, p.xw, s, who)) return rc;
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(p.M * (p.Np / 4), 256), 16384));
+  hipLaunchKernelGGL((reduce_linear_forward<T, ACT>), grid, dim3(256), 0, s, p.part, p.xw.splits, p.M * p.Np, (int)p.Np, e);
+  return check_launch(who);
 }
 
 template <class T, int ACT>
