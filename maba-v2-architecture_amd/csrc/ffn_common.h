@@ -66,20 +66,23 @@ int column_partials(const maba_tensor* src, float* p, hipStream_t s);
 
 // ---------------------------------------------------------------- launches
 
-// The tiles: BM, BN, waves along m and n.
-struct Tile256 { static constexpr int BM = 256, BN = 256, WM = 2, WN = 4; };
-struct Tile192 { static constexpr int BM = 192, BN = 128, WM = 2, WN = 2; };
-struct Tile160 { static constexpr int BM = 128, BN = 160, WM = 4, WN = 1; };
-struct Tile128 { static constexpr int BM = 128, BN = 128, WM = 2, WN = 2; };
-struct Tile64 { static constexpr int BM = 64, BN = 64, WM = 2, WN = 2; };
+// The tiles: BM, BN, waves along m and n, stages in LDS.  Tile64's third stage is for weights that come from HBM and few
+// tiles (64 rows, 2,048 to 2 x 5,504: 27 us with two, 16.7, 14.3 with four); a product whose operands are in the caches
+// would rather have the LDS (1,003 rows, 640 to 2 x 1,248: 9.6, 9.8, 11.1).
+struct Tile256 { static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, ST = 2; };
+struct Tile192 { static constexpr int BM = 192, BN = 128, WM = 2, WN = 2, ST = 2; };
+struct Tile160 { static constexpr int BM = 128, BN = 160, WM = 4, WN = 1, ST = 2; };
+struct Tile128 { static constexpr int BM = 128, BN = 128, WM = 2, WN = 2, ST = 2; };
+struct Tile64 { static constexpr int BM = 64, BN = 64, WM = 2, WN = 2, ST = 3; };
 
 // How a product runs: which tile, and into how many runs of stages its sum is split (more than one writes fp32
 // partials that reduce_splits adds).
 struct GemmPlan {
   int tile, splits, split_stages, tiles_m;
 };
-enum { PLAN_COLUMNS = 1, PLAN_SPLIT = 2, PLAN_PAIRS = 4 };     // an operand is read along its columns; the sum may be
-                                                               // split; the columns are a gate's and an up's by turns
+// An operand is read along its columns; the sum may be split; the columns are a gate's and an up's by turns; the
+// epilogue takes long and many registers, and no tile that has a compute unit to itself is taken.
+enum { PLAN_COLUMNS = 1, PLAN_SPLIT = 2, PLAN_PAIRS = 4, PLAN_LONG = 8 };
 GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, int what);
 
 template <class T, class Tile, int AMODE, int BMODE, class Epi>
@@ -88,7 +91,7 @@ int gemm_tile(GemmArgs& g, const typename Epi::Args& e, int64_t M, int64_t N, in
   g.tiles_n = (int)ceil_div(N, Tile::BN);
   const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * splits;
   if (grid > INT32_MAX) return fail(MABA_ERR_UNSUPPORTED, "%s: too many tiles", who);
-  hipLaunchKernelGGL((gemm_kernel<T, Tile::BM, Tile::BN, Tile::WM, Tile::WN, AMODE, BMODE, Epi>),
+  hipLaunchKernelGGL((gemm_kernel<T, Tile::BM, Tile::BN, Tile::WM, Tile::WN, Tile::ST, AMODE, BMODE, Epi>),
                      dim3((unsigned)grid), dim3(64 * Tile::WM * Tile::WN), 0, s, g, e);
   return check_launch(who);
 }
@@ -100,7 +103,9 @@ int gemm(GemmArgs g, const typename Epi::Args& e, int64_t M, int64_t N, const Ge
   g.segments = g.segments ? g.segments : 1;
   g.split_stages = p.split_stages;
   switch (p.tile) {
-    case 0: return gemm_tile<T, Tile256, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
+    case 0:
+      if constexpr (!Epi::LONG) return gemm_tile<T, Tile256, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
+      else return fail(MABA_ERR_INVALID, "%s: no such tile", who);
     case 1: return gemm_tile<T, Tile192, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
     case 2:
       if constexpr (BMODE != K_ROWS_PAIR) return gemm_tile<T, Tile160, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);

@@ -34,6 +34,7 @@ GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, int what) {
   for (int i = 0; i < TILE_COUNT; ++i) {
     const TileCost& t = TILES[i];
     if (t.bn % 64 && (what & PLAN_PAIRS)) continue;      // whose epilogue takes 64 columns at a time
+    if (t.slots == 1 && (what & PLAN_LONG)) continue;
     const int64_t tiles = ceil_div(M, t.bm) * ceil_div(N, t.bn);
     const int most = may_split ? (int)std::max<int64_t>(1, std::min<int64_t>({32, stages / 2, 8 * cus / std::max<int64_t>(tiles, 1)})) : 1;
     for (int want = 1; want <= most; ++want) {

@@ -199,13 +199,11 @@ struct Stager {
   int chunk;                   // rows of k: the lane's chunk of its row, the same for every load
   const char* base[2];         // of the tile, at the first k
   uint32_t span;               // rows of k: bytes from base to the operand's end (rows of this tile)
-  int64_t ldb[2];
+  int64_t ldb;                 // bytes from row to row (both tensors of a K_COLS operand have the same stride)
   int wave, cols;
 
   __device__ __forceinline__ void init(const Operand& o, const GemmArgs& g, int r0, int wave_, int lane) {
     wave = wave_;
-    ldb[0] = o.ld[0] * 2;
-    ldb[1] = o.ld[1] * 2;
     if constexpr (!COLS) {
       constexpr int RPI = 64 / CPR;                                // LDS rows of one wave instruction
       static_assert(MODE == K_ROWS || NW * RPI % 32 == 0, "a wave's loads belong to one of the paired tensors");
@@ -213,23 +211,25 @@ struct Stager {
       const int t = MODE == K_ROWS_PAIR ? (wave * RPI >> 4) & 1 : 0;
       const int first = MODE == K_ROWS_PAIR ? r0 / 2 : r0, most = MODE == K_ROWS_PAIR ? R / 2 : R;
       const int rows = min(o.rows - first, most);
-      base[0] = (const char*)(t ? o.p[1] : o.p[0]) + (int64_t)first * ldb[t];
-      span = rows > 0 ? (uint32_t)((rows - 1) * ldb[t] + 2 * g.segments * g.K) : 0u;
+      ldb = (t ? o.ld[1] : o.ld[0]) * 2;
+      base[0] = (const char*)(t ? o.p[1] : o.p[0]) + (int64_t)first * ldb;
+      base[1] = base[0];
+      span = rows > 0 ? (uint32_t)((rows - 1) * ldb + 2 * g.segments * g.K) : 0u;
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         int r = (i * NW + wave) * RPI + lane / CPR;
         if constexpr (MODE == K_ROWS_PAIR) r = ((r >> 5) << 4) | (r & 15);
-        voff[i] = (uint32_t)(r * ldb[t]) + 16 * chunk;
+        voff[i] = (uint32_t)(r * ldb) + 16 * chunk;
       }
     } else {
+      ldb = o.ld[0] * 2;
       cols = 2 * min(o.rows - r0, R);
       base[0] = (const char*)o.p[0] + 2 * (int64_t)r0;
       base[1] = (const char*)o.p[1] + 2 * (int64_t)r0;
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const int l = (i * NW + wave) * 64 + lane, k = l / CPR, x = l % CPR;
-        // both segments' tensors have the same stride
-        voff[i] = (uint32_t)(k * ldb[0]) + 16 * ((((x >> 1) ^ key_cols<R>(k)) << 1) | (x & 1));
+        voff[i] = (uint32_t)(k * ldb) + 16 * ((((x >> 1) ^ key_cols<R>(k)) << 1) | (x & 1));
       }
     }
   }
@@ -245,8 +245,8 @@ struct Stager {
       dead = k0 + 8 * chunk >= g.K ? OUT_OF_RANGE : 0u;
     } else {
       const int64_t rows = min(min(g.K, (int64_t)o.krows) - k0, (int64_t)BK);
-      p = base[seg] + k0 * ldb[0];
-      bytes = (uint32_t)((rows - 1) * ldb[0] + cols);
+      p = (seg ? base[1] : base[0]) + k0 * ldb;
+      bytes = (uint32_t)((rows - 1) * ldb + cols);
     }
     const auto r = rsrc(p, bytes);
 #pragma unroll
@@ -296,14 +296,14 @@ __device__ __forceinline__ TileId tile_of(const GemmArgs& g) {
   return r;
 }
 
-// The main loop keeps two stages of 64 k in LDS and the fragments of two steps of 32 k in registers.  While the
+// The main loop keeps ST stages of 64 k in LDS and the fragments of two steps of 32 k in registers.  While the
 // products of one step run, the fragments of the next are read; the one barrier of a stage stands between its two
 // steps, where every wave has the stage's last fragments in registers (its buffer is free for the loads of the stage
-// after next) and the next stage has landed (its first fragments can be read).  So neither LDS reads nor
+// ST ahead) and the next stage has landed (its first fragments can be read).  So neither LDS reads nor
 // loads are waited for between products, except by the first.
-template <class T, int BM, int BN, int WM, int WN, int AMODE, int BMODE, class Epi>
+template <class T, int BM, int BN, int WM, int WN, int ST, int AMODE, int BMODE, class Epi>
 __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) void gemm_kernel(GemmArgs g, typename Epi::Args e) {
-  constexpr int NW = WM * WN, MI = BM / WM / 16, NI = BN / WN / 16, BK = GEMM_BK, ST = 2;
+  constexpr int NW = WM * WN, MI = BM / WM / 16, NI = BN / WN / 16, BK = GEMM_BK;
   constexpr int A_EL = BM * BK, STAGE = (BM + BN) * BK;
   typedef Stager<BM, BK, NW, AMODE> SA;
   typedef Stager<BN, BK, NW, BMODE> SB;
@@ -368,14 +368,15 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) 
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   read(f0, 0, 0);
-  // The loads of the stage after next, which write LDS, are issued before the reads of the next fragments or behind
+  // The loads of the stage ST ahead, which write LDS, are issued before the reads of the next fragments or behind
   // them.  Behind them measured faster where those are transposing reads or eight waves' (256 x 256 tiles: dx of
   // 4,096 x 2,048 x 11,008 233 us against 297, dW of 11,008 x 2,048 x 4,096 191 against 220), before them for four
   // waves' row reads (192 x 128 on 32,768 x 640 x 1,248: 59 us against 61).
   constexpr bool LATE = SA::COLS || SB::COLS || NW == 8;
   // between two steps: the next stage has landed, and every wave holds the fragments of stage s
   auto turn = [&](int s) {
-    wait_vm<0>();
+    if (ST > 2 && s + ST - 1 < nk) wait_vm<(ST - 2) * LOADS>();
+    else wait_vm<0>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -400,6 +401,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) 
 // Epilogue: C as it is, rounded once to 16 bits; from row `second` on it goes to the second tensor's rows (`second`
 // is a multiple of 16).  M: rows of each.
 struct EpiStore {
+  static constexpr bool LONG = false;
   struct Args { Rows c[2]; int second, M, N; };
   template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
   static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
@@ -418,6 +420,7 @@ struct EpiStore {
 
 // Epilogue: fp32 partial products of one k split, [splits][M][N] (N padded to a multiple of 4).
 struct EpiPartial {
+  static constexpr bool LONG = false;
   struct Args { float* p; int M, N; };
   template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
   static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,

@@ -23,6 +23,7 @@ namespace ffn {
 
 // A wave's 32 columns of a tile are 16 of g and the same 16 of u; the epilogues take four such blocks at once.
 struct EpiGated {
+  static constexpr bool LONG = false;
   struct Args { Rows h; int M, I; };
   static __device__ __forceinline__ f32x4 gated(f32x4 g, f32x4 u) {
     f32x4 v;
@@ -58,6 +59,7 @@ struct EpiGated {
 
 // d [M, 2 Iw], Iw = I rounded up to 16: dg at column 0, du at column Iw, zeros behind each.
 struct EpiGatedBack {
+  static constexpr bool LONG = false;
   struct Args { Rows dh, d; int M, I, Iw; };
   static __device__ __forceinline__ void grads(f32x4 g, f32x4 u, f32x4 dh, f32x4& dg, f32x4& du) {
 #pragma unroll
