@@ -66,14 +66,16 @@ int column_partials(const maba_tensor* src, float* p, hipStream_t s);
 
 // ---------------------------------------------------------------- launches
 
-// The tiles: BM, BN, waves along m and n, stages in LDS.  Tile64's third stage is for weights that come from HBM and few
-// tiles (64 rows, 2,048 to 2 x 5,504: 27 us with two, 16.7, 14.3 with four); a product whose operands are in the caches
-// would rather have the LDS (1,003 rows, 640 to 2 x 1,248: 9.6, 9.8, 11.1).
+// The tiles: BM, BN, waves along m and n, stages in LDS.  Two stages leave room for other workgroups on the compute
+// unit, which hide the loads better than more stages do; Tile64Deep is for rows whose few tiles are all resident at once
+// and whose weights come from HBM (64 rows, 2,048 to 2 x 5,504: 26.1 us with two stages, 16.7 with three, 14.3 with
+// four; of operands in the caches, 4,096 rows, 1,248 to 640, 640 tiles: 15.4, 18.1, 19.2).
 struct Tile256 { static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, ST = 2; };
 struct Tile192 { static constexpr int BM = 192, BN = 128, WM = 2, WN = 2, ST = 2; };
 struct Tile160 { static constexpr int BM = 128, BN = 160, WM = 4, WN = 1, ST = 2; };
 struct Tile128 { static constexpr int BM = 128, BN = 128, WM = 2, WN = 2, ST = 2; };
-struct Tile64 { static constexpr int BM = 64, BN = 64, WM = 2, WN = 2, ST = 3; };
+struct Tile64 { static constexpr int BM = 64, BN = 64, WM = 2, WN = 2, ST = 2; };
+struct Tile64Deep { static constexpr int BM = 64, BN = 64, WM = 2, WN = 2, ST = 4; };
 
 // How a product runs: which tile, and into how many runs of stages its sum is split (more than one writes fp32
 // partials that reduce_splits adds).
@@ -111,7 +113,11 @@ int gemm(GemmArgs g, const typename Epi::Args& e, int64_t M, int64_t N, const Ge
       if constexpr (BMODE != K_ROWS_PAIR) return gemm_tile<T, Tile160, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
       else return fail(MABA_ERR_INVALID, "%s: no such tile", who);
     case 3: return gemm_tile<T, Tile128, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
-    default: return gemm_tile<T, Tile64, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
+    default:
+      if constexpr (AMODE == K_ROWS && BMODE != K_COLS)
+        if (ceil_div(M, 64) * ceil_div(N, 64) * p.splits <= 2 * device_cu_count())
+          return gemm_tile<T, Tile64Deep, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
+      return gemm_tile<T, Tile64, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
   }
 }
 

@@ -11,18 +11,20 @@ namespace ffn {
 // holds at once, a stage's latency (`lone`) bounds it.  Measured on MI355X, us, with an operand read along its columns
 // in brackets:
 //              256 x 256      192 x 128      128 x 160      128 x 128      64 x 64
-//   full       1.36 (1.38)    0.55 (0.63)    0.57 (0.64)    0.46 (0.48)    0.20 (0.25)
+//   full       1.36 (1.38)    0.55 (0.63)    0.57 (0.64)    0.46 (0.50)    0.20 (0.25)
 //   lone       1.36 (1.38)    0.80 (1.00)    0.75 (0.95)    0.60 (0.74)    0.36 (0.47)
-//   ends       7.6            4              3              3              0.75
-// (4,096 x 11,008 x 2,048, rows: 152, 172, 221, 178 us with the first four; 16,384 x 640 x 2,496, columns: 70, 63, 58,
-// 81, and 32,768 x 640 x 1,248, rows: 70, 62, 59, 66, where 160 columns leave no part of a tile over; 2,048 x 2,496 x 640,
-// rows: 20, 14.3, -, 14.3 and 16.7; 64 x 640 x 2,496 with the last, in 1, 4 and 8 splits: 19.9, 7.2 and 5.2.)
+//   ends       9              4              3              3              0.75
+// Over 43 products of rows and columns, in up to twelve splits, each timed with every tile, the plan takes 1.5 % more
+// than the best of them on average, 9 % at most.  (4,096 x 11,008 x 2,048, rows: 150, 169, -, 175 us with the first
+// four; 16,384 x 640 x 2,496, columns: 70, 58, 56, 79, and 32,768 x 640 x 1,248, rows: 70, 64, 58, 63, where 160 columns
+// leave no part of a tile over; 16,384 x 2,496 x 640, rows: 60, 54, -, 57, the smallest 81; 64 x 640 x 2,496 with the last, in 1, 4 and
+// 8 splits: 19.9, 7.2 and 5.2.)
 struct TileCost { int bm, bn, slots; float full[2], lone[2], ends; };
 constexpr int TILE_COUNT = 5;
-static const TileCost TILES[TILE_COUNT] = {{256, 256, 1, {1.36f, 1.38f}, {1.36f, 1.38f}, 7.6f},
+static const TileCost TILES[TILE_COUNT] = {{256, 256, 1, {1.36f, 1.38f}, {1.36f, 1.38f}, 9.f},
                                            {192, 128, 2, {0.55f, 0.63f}, {0.80f, 1.00f}, 4.f},
                                            {128, 160, 2, {0.57f, 0.64f}, {0.75f, 0.95f}, 3.f},
-                                           {128, 128, 2, {0.46f, 0.48f}, {0.60f, 0.74f}, 3.f},
+                                           {128, 128, 2, {0.46f, 0.50f}, {0.60f, 0.74f}, 3.f},
                                            {64, 64, 5, {0.20f, 0.25f}, {0.36f, 0.47f}, 0.75f}};
 
 GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, int what) {

@@ -18,6 +18,8 @@
 // n of one m.
 #pragma once
 
+#include <type_traits>
+
 #include "maba_common.h"
 
 namespace maba {
@@ -349,16 +351,17 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) 
   };
   // LDS reads between the products: one with each at eight waves, spread over all of them at four (256 x 256 rows on
   // 4,096 x 11,008 x 2,048: 152 us against 155; the smaller tiles the same either way)
-  auto interleave = [] {
+  constexpr int LOADS = SA::LOADS + SB::LOADS;
+  auto interleave = [](auto loads) {
     constexpr int READS = MI * (SA::COLS ? 2 : 1) + NI * (SB::COLS ? 2 : 1), PER = NW == 8 || MI * NI < READS ? 1 : MI * NI / READS;
 #pragma unroll
     for (int i = 0; i < READS; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // LDS read
+      if (decltype(loads)::value && i < LOADS) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x008, PER, 0); // MFMA
     }
   };
 
-  constexpr int LOADS = SA::LOADS + SB::LOADS;
   Frags f0, f1;
 #pragma unroll
   for (int s = 0; s < ST; ++s)
@@ -373,27 +376,26 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) 
   // 4,096 x 2,048 x 11,008 233 us against 297, dW of 11,008 x 2,048 x 4,096 191 against 220), before them for four
   // waves' row reads (192 x 128 on 32,768 x 640 x 1,248: 59 us against 61).
   constexpr bool LATE = SA::COLS || SB::COLS || NW == 8;
-  // between two steps: the next stage has landed, and every wave holds the fragments of stage s
-  auto turn = [&](int s) {
-    if (ST > 2 && s + ST - 1 < nk) wait_vm<(ST - 2) * LOADS>();
-    else wait_vm<0>();
+  // the steps of stage s; between them the next stage has landed, and every wave holds the fragments of stage s
+  auto stage = [&](int s, auto more) {
+    constexpr bool MORE = decltype(more)::value;          // there is a stage ST ahead
+    read(f1, s, 1);
+    products(f0);
+    interleave(std::false_type{});
+    wait_vm<MORE ? (ST - 2) * LOADS : 0>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (!LATE && s + ST < nk) issue(s + ST);
-  };
-
-  for (int s = 0; s < nk; ++s) {
-    read(f1, s, 1);
-    products(f0);
-    interleave();
-    turn(s);
+    if (MORE && !LATE) issue(s + ST);
     // past the last stage these are stale values that nothing uses
     read(f0, s + 1, 0);
-    if (LATE && s + ST < nk) issue(s + ST);
+    if (MORE && LATE) issue(s + ST);
     products(f1);
-    interleave();
-  }
+    interleave(more);
+  };
+  int s = 0;
+  for (; s + ST < nk; ++s) stage(s, std::true_type{});
+  for (; s < nk; ++s) stage(s, std::false_type{});
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   Epi::template run<T, BM, BN, WM, WN, MI, NI>(e, acc, t, m0 + wm, n0 + wn, c, q, wave, lds);
 }
