@@ -407,7 +407,7 @@ int maba_hip_argmax_rows(const maba_tensor* x, maba_tensor* out, void* stream);
  * stride, any row stride and alignment; fp32 accumulation, one rounding.  Rows that are not 16-byte
  * aligned chunks of eight elements are first copied into the workspace (except where the decode kernel
  * takes them, M <= 16 and up to 32), and a few rows' sum over a long C is split through it; the query returns 0
- * where the forward needs none.
+ * where the forward needs none.  A workspace is 16-byte aligned and belongs to one call at a time.
  *
  * Backward: dh [M,I]; x as above, or with x_scales its packed form (x: MABA_E4M3 codes [M,C], x_scales:
  * MABA_U8 [M,ceil(C/32)]); any of dx [M,C], dw_gate, dw_up [I,C] may be NULL.  g and u are made again from

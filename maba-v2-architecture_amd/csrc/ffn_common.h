@@ -207,6 +207,14 @@ inline int check_kept(const maba_tensor* x, const maba_tensor* scales, const cha
   return rc;
 }
 
+// What a call needs of its workspace: the bytes, at an address that 16-byte accesses can take.
+inline int check_workspace(const char* who, const void* p, size_t bytes, size_t need) {
+  if (need == 0) return MABA_OK;
+  if (!p || bytes < need) return fail(MABA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, p ? bytes : 0, need);
+  if ((uintptr_t)p % 16) return fail(MABA_ERR_INVALID, "%s: the workspace must be 16-byte aligned", who);
+  return MABA_OK;
+}
+
 // A workspace handed out front to back in 256-byte steps.
 struct Carve {
   char* p;

@@ -285,8 +285,7 @@ extern "C" int maba_hip_gated_ffn(const maba_tensor* x, const maba_tensor* w_gat
   if (rc) return rc;
   if (overlap(out, x) || overlap(out, w_gate) || overlap(out, w_up)) return fail(MABA_ERR_INVALID, "%s: out overlaps an input", who);
   GatedPlan p = gated_plan(x, nullptr, w_gate, w_up, false, false, false, workspace);
-  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
-    return fail(MABA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, p.bytes);
+  if ((rc = check_workspace(who, workspace, workspace_bytes, p.bytes))) return rc;
   if (p.M == 0) return MABA_OK;
   return w_gate->dtype == MABA_BF16 ? gated_forward<Bf16>(p, x, w_gate, w_up, out, (hipStream_t)stream, who)
                                     : gated_forward<Fp16>(p, x, w_gate, w_up, out, (hipStream_t)stream, who);
@@ -320,8 +319,7 @@ extern "C" int maba_hip_gated_ffn_backward(const maba_tensor* dh, const maba_ten
       if (overlap(outs[i], outs[j])) return fail(MABA_ERR_INVALID, "%s: two gradients overlap", who);
   }
   GatedPlan p = gated_plan(x, x_scales, w_gate, w_up, true, dx != nullptr, dw_gate || dw_up, workspace);
-  if (!workspace ? p.bytes > 0 : workspace_bytes < p.bytes)
-    return fail(MABA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, p.bytes);
+  if ((rc = check_workspace(who, workspace, workspace_bytes, p.bytes))) return rc;
   return dt == MABA_BF16 ? gated_backward<Bf16>(p, dh, x, x_scales, w_gate, w_up, dx, dw_gate, dw_up, (hipStream_t)stream, who)
                          : gated_backward<Fp16>(p, dh, x, x_scales, w_gate, w_up, dx, dw_gate, dw_up, (hipStream_t)stream, who);
 }

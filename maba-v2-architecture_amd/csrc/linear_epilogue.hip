@@ -437,8 +437,7 @@ extern "C" int maba_hip_linear_epilogue(const maba_tensor* x, const maba_tensor*
   if (residual && overlap(out, residual) && (out->data != residual->data || out->stride[0] != residual->stride[0]))
     return fail(MABA_ERR_INVALID, "%s: out overlaps the residual at another place", who);
   LinearPlan p = linear_plan(x, nullptr, weight, act, gate != nullptr, bias != nullptr, nullptr, nullptr, workspace);
-  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
-    return fail(MABA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, p.bytes);
+  if ((rc = check_workspace(who, workspace, workspace_bytes, p.bytes))) return rc;
   if (p.M == 0) return MABA_OK;
   const hipStream_t s = (hipStream_t)stream;
 #define LINEAR_FORWARD(T)                                                                                  \
@@ -484,8 +483,7 @@ extern "C" int maba_hip_linear_epilogue_backward(const maba_tensor* dy, const ma
   }
   const LinearNeeds need = {dx != nullptr, dw != nullptr, dbias != nullptr, dgate != nullptr};
   LinearPlan p = linear_plan(x, x_scales, weight, act, gate != nullptr, bias != nullptr, dy, &need, workspace);
-  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
-    return fail(MABA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, p.bytes);
+  if ((rc = check_workspace(who, workspace, workspace_bytes, p.bytes))) return rc;
   return dt == MABA_BF16
              ? linear_backward<Bf16>(p, dy, x, x_scales, weight, bias, act, gate, dx, dw, dbias, dgate, (hipStream_t)stream, who)
              : linear_backward<Fp16>(p, dy, x, x_scales, weight, bias, act, gate, dx, dw, dbias, dgate, (hipStream_t)stream, who);

@@ -339,6 +339,18 @@ def test_c_workspace_sizes(lib):
     assert some >= 2 * 64 * 96 and b(_t([64, 32]), None, _t([48, 32]), _t([48, 32]), 3) >= some
 
 
+def test_c_workspace_must_be_aligned(lib):
+    x, wg, wu, dh = _t([64, 31], data=X), _t([48, 31], data=W), _t([48, 31], data=W + 0x10000), _t([64, 48], data=H)
+    far = 0x900000
+    assert lib.maba_hip_gated_ffn(x, wg, wu, dh, far + 8, 1 << 20, None) == 1
+    assert b"16-byte aligned" in lib.maba_hip_last_error()
+    assert lib.maba_hip_gated_ffn_backward(dh, x, None, wg, wu, _t([64, 31], data=far), None, None, 2 * far + 2, 1 << 20, None) == 1
+    assert lib.maba_hip_linear_epilogue(x, wg, None, 0, None, None, dh, far + 4, 1 << 20, None) == 1
+    assert lib.maba_hip_linear_epilogue_backward(dh, x, None, wg, None, 0, None, _t([64, 31], data=far), None, None, None, 2 * far + 8,
+                                                 1 << 20, None) == 1
+    assert lib.maba_hip_gated_ffn(x, wg, wu, dh, far, 64, None) == 5
+
+
 def test_c_backward_refusals(lib):
     x, wg, wu, dh = _t([64, 32], data=X), _t([48, 32], data=W), _t([48, 32], data=W + 0x10000), _t([64, 48], data=H)
     dx, far = _t([64, 32], data=H + 0x100000), 0x900000

@@ -305,6 +305,58 @@ def test_out_may_be_the_residual():
     assert torch.equal(y, want)
 
 
+@pytest.mark.parametrize("M,K,N", [(7, 640, 96), (40, 2816, 104), (64, 5504, 130), (300, 70, 47), (2100, 640, 640), (4096, 128, 2504),
+                                   (5000, 72, 1100)])
+def test_the_residual_is_updated_in_place_by_every_kernel(M, K, N):
+    from maba_sparse import _native as N_
+    t = _linear(M, K, N, BF, seed=24)
+    want = D.linear_epilogue(t["x"], t["w"], t["bias"], "silu", t["residual"], t["gate"])
+    y = t["residual"].clone()
+    lib = N_.load()
+    need = lib.maba_hip_linear_epilogue_workspace_size(N_.rows_desc(t["x"]), N_.rows_desc(t["w"]))
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=DEV)
+    N_.check(lib.maba_hip_linear_epilogue(*map(N_.rows_desc, (t["x"], t["w"], t["bias"])), 2, *map(N_.rows_desc, (y, t["gate"], y)),
+                                          ws.data_ptr(), ws.numel(), N_.stream_ptr(y.device)), "linear_epilogue")
+    assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("K", [1, 8, 63, 64, 65, 128, 129, 192, 250, 256, 257, 320, 328, 640, 1000])
+@pytest.mark.parametrize("M", [33, 70, 128])
+def test_a_few_tiles_of_every_length(M, K):
+    """Fewer stages than the small tile holds, as many, and more."""
+    x, wg, wu, dh = _gated(M, K, 72, BF, seed=41)
+    B.check(D.gated_ffn(x, wg, wu), B.gated(x, wg, wu)["h"], "h")
+    t = _linear(M, K, 72, HF, seed=42)
+    want = B.linear(t["x"], t["w"], t["bias"], "silu", t["residual"], t["gate"], t["dy"])
+    B.check(D.linear_epilogue(t["x"], t["w"], t["bias"], "silu", t["residual"], t["gate"]), want["y"], "y")
+    got = D.linear_epilogue_backward(t["dy"], t["x"], t["w"], t["bias"], "silu", t["gate"])
+    for name, v in zip(("dx", "dw", "dbias", "dgate"), got):
+        B.check(v, want[name], name)
+
+
+@pytest.mark.parametrize("K", [1528, 1536, 1537, 1544, 2048, 2056])
+@pytest.mark.parametrize("M", [16, 17, 32, 33])
+def test_where_few_rows_change_kernels(M, K):
+    x, wg, wu, _ = _gated(M, K, 40, BF, seed=43)
+    B.check(D.gated_ffn(x, wg, wu), B.gated(x, wg, wu)["h"], "h")
+    t = _linear(M, K, 40, BF, seed=44)
+    B.check(D.linear_epilogue(t["x"], t["w"], None, "gelu", t["residual"]),
+            B.linear(t["x"], t["w"], None, "gelu", t["residual"])["y"], "y")
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu"])
+def test_activations_over_their_whole_range(act, dt):
+    """z and dz themselves, through a unit weight: from where the activation vanishes to where it is z."""
+    z = torch.cat([torch.linspace(-16, 16, 8 * 900), torch.linspace(-90, 90, 8 * 99), 2.0 ** torch.arange(-20.0, 12.0),
+                   -2.0 ** torch.arange(-20.0, 12.0)])
+    x = z.reshape(-1, 8).to(dt).to(DEV)
+    w, dy = torch.eye(8, device=DEV, dtype=dt), torch.ones(x.shape, device=DEV, dtype=dt)
+    want = B.linear(x, w, None, act, None, None, dy)
+    B.check(D.linear_epilogue(x, w, None, act), want["y"], "y")
+    B.check(D.linear_epilogue_backward(dy, x, w, None, act)[0], want["dx"], "dx")
+
+
 @pytest.mark.parametrize("ckpt", [None, "e4m3"])
 @pytest.mark.parametrize("M,Cw,I", [(1, 64, 96), (50, 64, 96), (1000, 200, 136)])
 def test_a_block_trained_through_autograd(M, Cw, I, ckpt):
@@ -394,6 +446,33 @@ def test_captured_step_replays_with_new_inputs():
         want = step()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
         torch.cuda.synchronize()
+
+
+def test_two_graphs_of_one_pool_replayed_by_turns():
+    """Their workspaces share memory: each replay must make all that it reads."""
+    sets = [(_gated(600 + 90 * i, 72, 104, BF, seed=50 + i), _linear(40 + 30 * i, 2816, 72, BF, seed=60 + i)) for i in range(2)]
+
+    def step(s):
+        (x, wg, wu, dh), t = s
+        return [*D.gated_ffn_backward(dh, x, wg, wu), D.linear_epilogue(t["x"], t["w"], t["bias"], "relu", t["residual"]),
+                *D.linear_epilogue_backward(t["dy"], t["x"], t["w"], t["bias"], "gelu", t["gate"])]
+
+    want = [step(s) for s in sets]
+    torch.cuda.synchronize()
+    graphs, outs, pool = [], [], None
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(step(s))
+        pool = g.pool()
+        graphs.append(g)
+    for turn in (0, 1, 1, 0, 1, 0, 0):
+        for v in outs[turn]:
+            v.zero_()
+        graphs[turn].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs[turn], want[turn]))
+        assert all(torch.equal(a, b) for a, b in zip(step(sets[turn]), want[turn]))
 
 
 def test_captured_autograd_step():
