@@ -349,16 +349,16 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) 
 #pragma unroll
       for (int j = 0; j < NI; ++j) acc[i][j] = T::mma(f.b[j], f.a[i], acc[i][j]);
   };
-  // LDS reads between the products: one with each at eight waves, spread over all of them at four (256 x 256 rows on
-  // 4,096 x 11,008 x 2,048: 152 us against 155; the smaller tiles the same either way)
   constexpr int LOADS = SA::LOADS + SB::LOADS;
+  // An LDS read and, where the step has any, a load before each of the first products.  With all the loads in one place
+  // a compute unit with few waves waits for their issue (dx of 8,191 x 640 x 2,496: 45 us against 50).
   auto interleave = [](auto loads) {
-    constexpr int READS = MI * (SA::COLS ? 2 : 1) + NI * (SB::COLS ? 2 : 1), PER = NW == 8 || MI * NI < READS ? 1 : MI * NI / READS;
+    constexpr int READS = MI * (SA::COLS ? 2 : 1) + NI * (SB::COLS ? 2 : 1);
 #pragma unroll
     for (int i = 0; i < READS; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // LDS read
       if (decltype(loads)::value && i < LOADS) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, PER, 0); // MFMA
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // MFMA
     }
   };
 
@@ -371,11 +371,6 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) 
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   read(f0, 0, 0);
-  // The loads of the stage ST ahead, which write LDS, are issued before the reads of the next fragments or behind
-  // them.  Behind them measured faster where those are transposing reads or eight waves' (256 x 256 tiles: dx of
-  // 4,096 x 2,048 x 11,008 233 us against 297, dW of 11,008 x 2,048 x 4,096 191 against 220), before them for four
-  // waves' row reads (192 x 128 on 32,768 x 640 x 1,248: 59 us against 61).
-  constexpr bool LATE = SA::COLS || SB::COLS || NW == 8;
   // the steps of stage s; between them the next stage has landed, and every wave holds the fragments of stage s
   auto stage = [&](int s, auto more) {
     constexpr bool MORE = decltype(more)::value;          // there is a stage ST ahead
@@ -386,10 +381,11 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) 
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (MORE && !LATE) issue(s + ST);
     // past the last stage these are stale values that nothing uses
     read(f0, s + 1, 0);
-    if (MORE && LATE) issue(s + ST);
+    // behind the reads: before them, dx of 4,096 x 2,048 x 11,008 takes 151 us against 141, dW of 11,008 x 2,048 x 4,096 in
+    // 256 x 256 tiles 206 against 189, the smaller tiles' products the same
+    if (MORE) issue(s + ST);
     products(f1);
     interleave(more);
   };

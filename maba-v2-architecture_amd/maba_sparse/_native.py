@@ -218,6 +218,22 @@ def rows_desc(t: Optional[torch.Tensor]) -> Optional[bytes]:
     return _PACK.pack(t.data_ptr(), code, 1, n[0], 1, 1, 1, st[0], 0, 0, 0)
 
 
+def rows_of(t: Optional[torch.Tensor]):
+    """``t [..., C]`` as ``[rows, C]`` with unit column stride, a view where the strides allow it, and its descriptor."""
+    if t is None:
+        return None, None
+    n, st = t.shape, t.stride()
+    if len(n) != 2 or (st[1] != 1 and n[1] != 1):
+        t = t.reshape(-1, n[-1])
+        if t.stride(1) != 1 and n[-1] != 1:
+            t = t.contiguous()
+        return t, rows_desc(t)
+    code = _DTYPE_CODES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"unsupported dtype {t.dtype}")
+    return t, _PACK.pack(t.data_ptr(), code, 2, n[0], n[1], 1, 1, st[0], st[1], 0, 0)
+
+
 def desc_array(tensors: Sequence[Optional[torch.Tensor]]):
     """A C array of descriptor pointers (``const maba_tensor* const*``); None entries are NULL."""
     T = ctypes.POINTER(MabaTensor)
@@ -228,9 +244,12 @@ def stream_ptr(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None else torch.cuda.current_device())
 
 
+_NOTHING = contextlib.nullcontext()
+
+
 def on_device(device: torch.device):
     """A context in which ``device`` is current (kernel launches and workspace queries go by it)."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _NOTHING if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def check(rc: int, what: str) -> None:

@@ -201,8 +201,9 @@ def _log_fallback_warning(op_name: str, backend: str, exc: Optional[Exception] =
         logger.debug(msg)
 
 
-def _run(op_name: str, device, kwargs: Dict[str, Any]):
-    backend = get_backend(device)
+def _run(op_name: str, device, kwargs: Dict[str, Any], backend: Optional[str] = None):
+    if backend is None:
+        backend = get_backend(device)
     fn = get_kernel(backend, op_name)
     if fn is not None and backend != "reference":
         try:
@@ -423,31 +424,32 @@ def _ffn_kept(x, x_scales) -> None:
 
 
 class _FFNOps:
-    """The ops that the autograd functions call, through the backend of their tensors' device."""
+    """The ops that the autograd functions call, through the backend of the tensors' device: a backward pass runs
+    where its forward did."""
 
-    @staticmethod
-    def pack(x):
-        return _run("checkpoint_pack", x.device, dict(x=x))
+    __slots__ = ("backend",)
 
-    @staticmethod
-    def gated_ffn(x, w_gate, w_up):
-        return _run("gated_ffn", x.device, dict(x=x, w_gate=w_gate, w_up=w_up))
+    def __init__(self, device):
+        self.backend = get_backend(device)
 
-    @staticmethod
-    def gated_ffn_backward(dh, x, w_gate, w_up, x_scales, needs):
-        return _run("gated_ffn_backward", dh.device, dict(dh=dh, x=x, w_gate=w_gate, w_up=w_up, x_scales=x_scales,
-                                                          needs=tuple(needs)))
+    def pack(self, x):
+        return _run("checkpoint_pack", None, dict(x=x), self.backend)
 
-    @staticmethod
-    def linear_epilogue(x, weight, bias, activation, residual, gate):
-        return _run("linear_epilogue", x.device, dict(x=x, weight=weight, bias=bias, activation=activation,
-                                                      residual=residual, gate=gate))
+    def gated_ffn(self, x, w_gate, w_up):
+        return _run("gated_ffn", None, dict(x=x, w_gate=w_gate, w_up=w_up), self.backend)
 
-    @staticmethod
-    def linear_epilogue_backward(dy, x, weight, bias, activation, gate, x_scales, needs):
-        return _run("linear_epilogue_backward", dy.device, dict(dy=dy, x=x, weight=weight, bias=bias, gate=gate,
-                                                                activation=activation, x_scales=x_scales,
-                                                                needs=tuple(needs)))
+    def gated_ffn_backward(self, dh, x, w_gate, w_up, x_scales, needs):
+        return _run("gated_ffn_backward", None,
+                    dict(dh=dh, x=x, w_gate=w_gate, w_up=w_up, x_scales=x_scales, needs=tuple(needs)), self.backend)
+
+    def linear_epilogue(self, x, weight, bias, activation, residual, gate):
+        return _run("linear_epilogue", None, dict(x=x, weight=weight, bias=bias, activation=activation, residual=residual,
+                                                  gate=gate), self.backend)
+
+    def linear_epilogue_backward(self, dy, x, weight, bias, activation, gate, x_scales, needs):
+        return _run("linear_epilogue_backward", None,
+                    dict(dy=dy, x=x, weight=weight, bias=bias, gate=gate, activation=activation, x_scales=x_scales,
+                         needs=tuple(needs)), self.backend)
 
 
 def _wants_grad(*tensors) -> bool:
@@ -466,8 +468,8 @@ def dispatch_gated_ffn(x, w_gate, w_up, checkpoint: Optional[str] = None) -> tor
     _ffn_shape("w_up", w_up, w_gate.shape)
     _ffn_checkpoint(checkpoint)
     if _wants_grad(x, w_gate, w_up):
-        return _ff.guard_capture(_ff.GatedFFN.apply(_FFNOps, checkpoint, x, w_gate, w_up))
-    return _FFNOps.gated_ffn(x, w_gate, w_up)
+        return _ff.guard_capture(_ff.GatedFFN.apply(_FFNOps(x.device), checkpoint, x, w_gate, w_up))
+    return _FFNOps(x.device).gated_ffn(x, w_gate, w_up)
 
 
 def dispatch_gated_ffn_backward(dh, x, w_gate, w_up, x_scales=None, needs=(True, True, True)):
@@ -482,7 +484,7 @@ def dispatch_gated_ffn_backward(dh, x, w_gate, w_up, x_scales=None, needs=(True,
     if len(needs) != 3:
         raise ValueError(f"needs takes three flags (dx, dw_gate, dw_up), got {needs!r}")
     with torch.no_grad():
-        return _FFNOps.gated_ffn_backward(dh, x, w_gate, w_up, x_scales, needs)
+        return _FFNOps(dh.device).gated_ffn_backward(dh, x, w_gate, w_up, x_scales, needs)
 
 
 def dispatch_linear_epilogue(x, weight, bias=None, activation: str = "none", residual=None, gate=None,
@@ -502,8 +504,8 @@ def dispatch_linear_epilogue(x, weight, bias=None, activation: str = "none", res
     _ffn_activation(activation)
     _ffn_checkpoint(checkpoint)
     if _wants_grad(x, weight, bias, residual, gate):
-        return _ff.guard_capture(_ff.LinearEpilogue.apply(_FFNOps, checkpoint, activation, x, weight, bias, residual, gate))
-    return _FFNOps.linear_epilogue(x, weight, bias, activation, residual, gate)
+        return _ff.guard_capture(_ff.LinearEpilogue.apply(_FFNOps(x.device), checkpoint, activation, x, weight, bias, residual, gate))
+    return _FFNOps(x.device).linear_epilogue(x, weight, bias, activation, residual, gate)
 
 
 def dispatch_linear_epilogue_backward(dy, x, weight, bias=None, activation: str = "none", gate=None, x_scales=None,
@@ -523,7 +525,7 @@ def dispatch_linear_epilogue_backward(dy, x, weight, bias=None, activation: str 
     if len(needs) != 4:
         raise ValueError(f"needs takes four flags (dx, dw, dbias, dgate), got {needs!r}")
     with torch.no_grad():
-        return _FFNOps.linear_epilogue_backward(dy, x, weight, bias, activation, gate, x_scales, needs)
+        return _FFNOps(dy.device).linear_epilogue_backward(dy, x, weight, bias, activation, gate, x_scales, needs)
 
 
 def dispatch_checkpoint_pack(x) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -533,8 +535,7 @@ def dispatch_checkpoint_pack(x) -> Tuple[torch.Tensor, torch.Tensor]:
         raise ValueError(f"x must have a positive channel dimension, got {list(x.shape)}")
     if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise TypeError(f"Unsupported dtype {x.dtype}. Supported: {(torch.float32, torch.float16, torch.bfloat16)}")
-    with torch.no_grad():
-        return _FFNOps.pack(x)
+    return _FFNOps(x.device).pack(x.detach() if x.requires_grad else x)
 
 
 def dispatch_checkpoint_unpack(codes, scales, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:

@@ -305,13 +305,6 @@ def hip_maba_sa_prefill(q, k, v, kh, vh, early, idx, gate_logits, scale: float, 
 _ACT_CODES = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t [..., C]`` as ``[rows, C]`` with unit column stride: a view where the strides allow it."""
-    if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
-
-
 def _vec(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t if t is None or t.is_contiguous() else t.contiguous()
 
@@ -332,9 +325,9 @@ def hip_gated_ffn(x, w_gate, w_up, **kwargs: Any) -> torch.Tensor:
     dev = N.require_device((x, w_gate, w_up), "gated_ffn")
     with N.on_device(dev):
         lib = N.load()
-        x2, wg, wu = _rows(x), _rows(w_gate), _rows(w_up)
+        (x2, dx2), (wg, dwg), (wu, dwu) = N.rows_of(x), N.rows_of(w_gate), N.rows_of(w_up)
         out = torch.empty(x2.shape[0], wg.shape[0], dtype=x.dtype, device=dev)
-        ins = (N.rows_desc(x2), N.rows_desc(wg), N.rows_desc(wu))
+        ins = (dx2, dwg, dwu)
         _forward(lib.maba_hip_gated_ffn, (*ins, N.rows_desc(out)), lib.maba_hip_gated_ffn_workspace_size, ins, dev, "gated_ffn")
     return out if x.dim() == 2 else out.view(*x.shape[:-1], wg.shape[0])
 
@@ -346,17 +339,16 @@ def hip_gated_ffn_backward(dh, x, w_gate, w_up, x_scales=None, needs=(True, True
     dev = N.require_device((dh, x, w_gate, w_up, x_scales), "gated_ffn_backward")
     with N.on_device(dev):
         lib = N.load()
-        dh2, x2, wg, wu = _rows(dh), _rows(x), _rows(w_gate), _rows(w_up)
-        sc = None if x_scales is None else _rows(x_scales)
+        (dh2, ddh), (x2, dx2), (wg, dwg), (wu, dwu), (sc, dsc) = map(N.rows_of, (dh, x, w_gate, w_up, x_scales))
         dt = w_gate.dtype
         dx = torch.empty(x2.shape, dtype=dt, device=dev) if needs[0] else None
         dws = [torch.empty(w_gate.shape, dtype=dt, device=dev) if n else None for n in needs[1:3]]
-        ins = (N.rows_desc(x2), N.rows_desc(sc), N.rows_desc(wg), N.rows_desc(wu))
+        ins = (dx2, dsc, dwg, dwu)
         ws = _workspace(lib.maba_hip_gated_ffn_backward_workspace_size(*ins, bool(needs[0]) + 2 * any(needs[1:3])), dev)
-        rc = lib.maba_hip_gated_ffn_backward(N.rows_desc(dh2), *ins, N.rows_desc(dx), N.rows_desc(dws[0]), N.rows_desc(dws[1]),
+        rc = lib.maba_hip_gated_ffn_backward(ddh, *ins, N.rows_desc(dx), N.rows_desc(dws[0]), N.rows_desc(dws[1]),
                                              ws.data_ptr(), ws.numel(), N.stream_ptr(dev))
         N.check(rc, "gated_ffn_backward")
-    return (dx.view(x.shape) if needs[0] else None, *dws)
+    return (dx if dx is None or x.dim() == 2 else dx.view(x.shape), *dws)
 
 
 @register_kernel("hip", "linear_epilogue")
@@ -367,11 +359,11 @@ def hip_linear_epilogue(x, weight, bias=None, activation: str = "none", residual
     dev = N.require_device((x, weight, bias, residual, gate), "linear_epilogue")
     with N.on_device(dev):
         lib = N.load()
-        x2, w = _rows(x), _rows(weight)
-        res, bias, gate = None if residual is None else _rows(residual), _vec(bias), _vec(gate)
+        (x2, dx2), (w, dw2), (res, dres) = N.rows_of(x), N.rows_of(weight), N.rows_of(residual)
+        bias, gate = _vec(bias), _vec(gate)
         out = torch.empty(x2.shape[0], w.shape[0], dtype=x.dtype, device=dev)
-        ins = (N.rows_desc(x2), N.rows_desc(w))
-        _forward(lib.maba_hip_linear_epilogue, (*ins, N.rows_desc(bias), _ACT_CODES[activation], N.rows_desc(res),
+        ins = (dx2, dw2)
+        _forward(lib.maba_hip_linear_epilogue, (*ins, N.rows_desc(bias), _ACT_CODES[activation], dres,
                                                 N.rows_desc(gate), N.rows_desc(out)),
                  lib.maba_hip_linear_epilogue_workspace_size, ins, dev, "linear_epilogue")
     return out if x.dim() == 2 else out.view(*x.shape[:-1], w.shape[0])
@@ -385,20 +377,21 @@ def hip_linear_epilogue_backward(dy, x, weight, bias=None, activation: str = "no
     dev = N.require_device((dy, x, weight, bias, gate, x_scales), "linear_epilogue_backward")
     with N.on_device(dev):
         lib = N.load()
-        dy2, x2, w = _rows(dy), _rows(x), _rows(weight)
-        sc, bias, gate = None if x_scales is None else _rows(x_scales), _vec(bias), _vec(gate)
+        (dy2, ddy), (x2, dx2), (w, dw2), (sc, dsc) = map(N.rows_of, (dy, x, weight, x_scales))
+        bias, gate = _vec(bias), _vec(gate)
         dt, n_out = weight.dtype, weight.shape[0]
         needs = (needs[0], needs[1], needs[2] and bias is not None, needs[3] and gate is not None)
         shapes = (x2.shape, weight.shape, (n_out,), (n_out,))
         outs = [torch.empty(s, dtype=dt, device=dev) if n else None for s, n in zip(shapes, needs)]
         act = _ACT_CODES[activation]
-        ins = (N.rows_desc(dy2), N.rows_desc(x2), N.rows_desc(sc), N.rows_desc(w))
+        ins = (ddy, dx2, dsc, dw2)
         ws = _workspace(lib.maba_hip_linear_epilogue_backward_workspace_size(
             *ins, act, bias is not None, gate is not None, sum(1 << i for i, n in enumerate(needs) if n)), dev)
         rc = lib.maba_hip_linear_epilogue_backward(*ins, N.rows_desc(bias), act, N.rows_desc(gate), *map(N.rows_desc, outs),
                                                    ws.data_ptr(), ws.numel(), N.stream_ptr(dev))
         N.check(rc, "linear_epilogue_backward")
-    return (outs[0].view(x.shape) if needs[0] else None, *outs[1:])
+    dx = outs[0]
+    return (dx if dx is None or x.dim() == 2 else dx.view(x.shape), *outs[1:])
 
 
 @register_kernel("hip", "checkpoint_pack")
@@ -406,12 +399,12 @@ def hip_checkpoint_pack(x, **kwargs: Any) -> Tuple[torch.Tensor, torch.Tensor]:
     """e4m3 codes and scales of ``x`` (contract: ``common.ref_checkpoint_pack``)."""
     dev = N.require_device((x,), "checkpoint_pack")
     with N.on_device(dev):
-        x2 = _rows(x)
+        x2, dx2 = N.rows_of(x)
         rows, C = x2.shape
         groups = (C + 31) // 32
         codes = torch.empty(rows, C, dtype=torch.float8_e4m3fn, device=dev)
         scales = torch.empty(rows, groups, dtype=torch.uint8, device=dev)
-        N.check(N.load().maba_hip_checkpoint_pack(N.rows_desc(x2), N.rows_desc(codes), N.rows_desc(scales), N.stream_ptr(dev)),
+        N.check(N.load().maba_hip_checkpoint_pack(dx2, N.rows_desc(codes), N.rows_desc(scales), N.stream_ptr(dev)),
                 "checkpoint_pack")
     return (codes, scales) if x.dim() == 2 else (codes.view(x.shape), scales.view(*x.shape[:-1], groups))
 
@@ -421,10 +414,9 @@ def hip_checkpoint_unpack(codes, scales, dtype: torch.dtype = torch.bfloat16, **
     """The values of a packed activation (contract: ``common.ref_checkpoint_unpack``)."""
     dev = N.require_device((codes, scales), "checkpoint_unpack")
     with N.on_device(dev):
-        c2, s2 = _rows(codes), _rows(scales)
+        (c2, dc), (s2, ds) = N.rows_of(codes), N.rows_of(scales)
         out = torch.empty(c2.shape, dtype=dtype, device=dev)
-        N.check(N.load().maba_hip_checkpoint_unpack(N.rows_desc(c2), N.rows_desc(s2), N.rows_desc(out), N.stream_ptr(dev)),
-                "checkpoint_unpack")
+        N.check(N.load().maba_hip_checkpoint_unpack(dc, ds, N.rows_desc(out), N.stream_ptr(dev)), "checkpoint_unpack")
     return out if codes.dim() == 2 else out.view(codes.shape)
 
 
