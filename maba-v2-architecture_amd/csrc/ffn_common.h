@@ -66,16 +66,20 @@ int column_partials(const maba_tensor* src, float* p, hipStream_t s);
 
 // ---------------------------------------------------------------- launches
 
-// The tiles: BM, BN, waves along m and n, stages in LDS.  Two stages leave room for other workgroups on the compute
-// unit, which hide the loads better than more stages do; Tile64Deep is for rows whose few tiles are all resident at once
-// and whose weights come from HBM (64 rows, 2,048 to 2 x 5,504: 26.1 us with two stages, 16.7 with three, 14.3 with
-// four; of operands in the caches, 4,096 rows, 1,248 to 640, 640 tiles: 15.4, 18.1, 19.2).
-struct Tile256 { static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, ST = 2; };
-struct Tile192 { static constexpr int BM = 192, BN = 128, WM = 2, WN = 2, ST = 2; };
-struct Tile160 { static constexpr int BM = 128, BN = 160, WM = 4, WN = 1, ST = 2; };
-struct Tile128 { static constexpr int BM = 128, BN = 128, WM = 2, WN = 2, ST = 2; };
-struct Tile64 { static constexpr int BM = 64, BN = 64, WM = 2, WN = 2, ST = 2; };
-struct Tile64Deep { static constexpr int BM = 64, BN = 64, WM = 2, WN = 2, ST = 4; };
+// The tiles: BM, BN, waves along m and n, stages in LDS, groups of waves.  Two stages leave room for other workgroups on
+// the compute unit, which hide the loads better than more stages do; Tile64Deep is for rows whose few tiles are all
+// resident at once (64 rows, 2,048 to 2 x 5,504, weights from HBM: 26.1 us with two stages, 16.7 with three, 14.3 with
+// four; 2,048 rows, 1,248 to 640 with a residual, 320 tiles: 14.6 with two, 13.2 with four; 4,096 rows, 640 tiles: 15.4
+// with two, 19.2 with four).
+struct Tile256 { static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, ST = 2, KG = 1; };
+struct Tile192 { static constexpr int BM = 192, BN = 128, WM = 2, WN = 2, ST = 2, KG = 1; };
+struct Tile160 { static constexpr int BM = 128, BN = 160, WM = 4, WN = 1, ST = 2, KG = 1; };
+struct Tile128 { static constexpr int BM = 128, BN = 128, WM = 2, WN = 2, ST = 2, KG = 1; };
+struct Tile64 { static constexpr int BM = 64, BN = 64, WM = 2, WN = 2, ST = 2, KG = 1; };
+struct Tile160Two { static constexpr int BM = 128, BN = 160, WM = 4, WN = 1, ST = 2, KG = 2; };
+struct Tile128Two { static constexpr int BM = 128, BN = 128, WM = 2, WN = 2, ST = 2, KG = 2; };
+struct Tile64Two { static constexpr int BM = 64, BN = 64, WM = 2, WN = 2, ST = 2, KG = 2; };
+struct Tile64Deep { static constexpr int BM = 64, BN = 64, WM = 2, WN = 2, ST = 4, KG = 1; };
 
 // How a product runs: which tile, and into how many runs of stages its sum is split (more than one writes fp32
 // partials that reduce_splits adds).
@@ -83,8 +87,9 @@ struct GemmPlan {
   int tile, splits, split_stages, tiles_m;
 };
 // An operand is read along its columns; the sum may be split; the columns are a gate's and an up's by turns; the
-// epilogue takes long and many registers, and no tile that has a compute unit to itself is taken.
-enum { PLAN_COLUMNS = 1, PLAN_SPLIT = 2, PLAN_PAIRS = 4, PLAN_LONG = 8 };
+// epilogue takes long and many registers, and no tile that has a compute unit to itself is taken; the epilogue can do with
+// half of a tile's rows, so that two groups of waves may share a tile (KG = 2).
+enum { PLAN_COLUMNS = 1, PLAN_SPLIT = 2, PLAN_PAIRS = 4, PLAN_LONG = 8, PLAN_GROUPS = 16 };
 GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, int what);
 
 template <class T, class Tile, int AMODE, int BMODE, class Epi>
@@ -93,8 +98,8 @@ int gemm_tile(GemmArgs& g, const typename Epi::Args& e, int64_t M, int64_t N, in
   g.tiles_n = (int)ceil_div(N, Tile::BN);
   const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * splits;
   if (grid > INT32_MAX) return fail(MABA_ERR_UNSUPPORTED, "%s: too many tiles", who);
-  hipLaunchKernelGGL((gemm_kernel<T, Tile::BM, Tile::BN, Tile::WM, Tile::WN, Tile::ST, AMODE, BMODE, Epi>),
-                     dim3((unsigned)grid), dim3(64 * Tile::WM * Tile::WN), 0, s, g, e);
+  hipLaunchKernelGGL((gemm_kernel<T, Tile::BM, Tile::BN, Tile::WM, Tile::WN, Tile::ST, AMODE, BMODE, Epi, Tile::KG>),
+                     dim3((unsigned)grid), dim3(64 * Tile::WM * Tile::WN * Tile::KG), 0, s, g, e);
   return check_launch(who);
 }
 
@@ -113,6 +118,14 @@ int gemm(GemmArgs g, const typename Epi::Args& e, int64_t M, int64_t N, const Ge
       if constexpr (BMODE != K_ROWS_PAIR) return gemm_tile<T, Tile160, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
       else return fail(MABA_ERR_INVALID, "%s: no such tile", who);
     case 3: return gemm_tile<T, Tile128, AMODE, BMODE, Epi>(g, e, M, N, p.splits, s, who);
+    case 5:
+    case 6:
+    case 7:
+      if constexpr (Epi::GROUPS && AMODE == K_ROWS)
+        return p.tile == 5   ? gemm_tile<T, Tile160Two, AMODE, BMODE, Epi>(g, e, M, N, 1, s, who)
+               : p.tile == 6 ? gemm_tile<T, Tile128Two, AMODE, BMODE, Epi>(g, e, M, N, 1, s, who)
+                             : gemm_tile<T, Tile64Two, AMODE, BMODE, Epi>(g, e, M, N, 1, s, who);
+      else return fail(MABA_ERR_INVALID, "%s: no such tile", who);
     default:
       if constexpr (AMODE == K_ROWS && BMODE != K_COLS)
         if (ceil_div(M, 64) * ceil_div(N, 64) * p.splits <= 2 * device_cu_count())

@@ -19,32 +19,47 @@ namespace ffn {
 // four; 16,384 x 640 x 2,496, columns: 70, 58, 56, 79, and 32,768 x 640 x 1,248, rows: 70, 64, 58, 63, where 160 columns
 // leave no part of a tile over; 16,384 x 2,496 x 640, rows: 60, 54, -, 57, the smallest 81; 64 x 640 x 2,496 with the last, in 1, 4 and
 // 8 splits: 19.9, 7.2 and 5.2.)
-struct TileCost { int bm, bn, slots; float full[2], lone[2], ends; };
-constexpr int TILE_COUNT = 5;
-static const TileCost TILES[TILE_COUNT] = {{256, 256, 1, {1.36f, 1.38f}, {1.36f, 1.38f}, 9.f},
-                                           {192, 128, 2, {0.55f, 0.63f}, {0.80f, 1.00f}, 4.f},
-                                           {128, 160, 2, {0.57f, 0.64f}, {0.75f, 0.95f}, 3.f},
-                                           {128, 128, 2, {0.46f, 0.50f}, {0.60f, 0.74f}, 3.f},
-                                           {64, 64, 5, {0.20f, 0.25f}, {0.36f, 0.47f}, 0.75f}};
+//
+// Two groups of waves on a tile (`groups`; a stage is then two) serve tiles too few to share a compute unit.  Its one
+// group of four waves keeps the matrix units 26 % busy; a second workgroup's would do the same as a second group.
+// 640 columns, k = 2 x 1,248, of 8,191, 6,000 and 2,048 rows: 41 us -> 35 (128 x 160), 36 -> 31 (128 x 128), 26 -> 20.5
+// (64 x 64).  With more tiles than that they cost more (8,191 rows in 128 x 128: 58) and are not taken.
+//              128 x 160      128 x 128      64 x 64
+//   full       1.20 (1.45)    0.95 (1.27)    0.47 (0.46)
+//   lone       1.20 (1.45)    0.95 (1.27)    0.60 (0.60)
+//   ends       5              5              0.9
+struct TileCost { int bm, bn, slots, groups; float full[2], lone[2], ends; };
+constexpr int TILE_COUNT = 8;
+static const TileCost TILES[TILE_COUNT] = {{256, 256, 1, 1, {1.36f, 1.38f}, {1.36f, 1.38f}, 9.f},
+                                           {192, 128, 2, 1, {0.55f, 0.63f}, {0.80f, 1.00f}, 4.f},
+                                           {128, 160, 2, 1, {0.57f, 0.64f}, {0.75f, 0.95f}, 3.f},
+                                           {128, 128, 2, 1, {0.46f, 0.50f}, {0.60f, 0.74f}, 3.f},
+                                           {64, 64, 5, 1, {0.20f, 0.25f}, {0.36f, 0.47f}, 0.75f},
+                                           {128, 160, 1, 2, {1.20f, 1.45f}, {1.20f, 1.45f}, 5.f},
+                                           {128, 128, 1, 2, {0.95f, 1.27f}, {0.95f, 1.27f}, 5.f},
+                                           {64, 64, 2, 2, {0.47f, 0.46f}, {0.60f, 0.60f}, 0.9f}};
 
 GemmPlan gemm_plan(int64_t M, int64_t N, int64_t stages, int what) {
   const bool columns = what & PLAN_COLUMNS, may_split = what & PLAN_SPLIT;
   const int64_t cus = device_cu_count();
   stages = std::max<int64_t>(stages, 1);      // no rows: nothing is launched
-  GemmPlan best = {TILE_COUNT - 1, 1, (int)stages, 0};
+  GemmPlan best = {};
   float least = 0.f;
   for (int i = 0; i < TILE_COUNT; ++i) {
     const TileCost& t = TILES[i];
     if (t.bn % 64 && (what & PLAN_PAIRS)) continue;      // whose epilogue takes 64 columns at a time
     if (t.slots == 1 && (what & PLAN_LONG)) continue;
+    if (t.groups > 1 && !(what & PLAN_GROUPS)) continue;
     const int64_t tiles = ceil_div(M, t.bm) * ceil_div(N, t.bn);
-    const int most = may_split ? (int)std::max<int64_t>(1, std::min<int64_t>({32, stages / 2, 8 * cus / std::max<int64_t>(tiles, 1)})) : 1;
+    const int most = may_split && t.groups == 1 ? (int)std::max<int64_t>(1, std::min<int64_t>({32, stages / 2, 8 * cus / std::max<int64_t>(tiles, 1)})) : 1;
     for (int want = 1; want <= most; ++want) {
       const int64_t per = ceil_div(stages, want), splits = ceil_div(stages, per);
       if (splits != want) continue;
       const int64_t n = ceil_div(tiles * splits, cus);
-      float us = n * (per * t.full[columns] + t.ends);
-      if (n < t.slots) us = std::max(us, per * t.lone[columns] + t.ends);
+      if (t.groups > 1 && n > t.slots) continue;
+      const int64_t turns = ceil_div(per, t.groups);
+      float us = n * (turns * t.full[columns] + t.ends);
+      if (n < t.slots) us = std::max(us, turns * t.lone[columns] + t.ends);
       if (splits > 1) us += 2.5f + (float)(M * N) * (8.f * splits + 2.f) / 5e6f;     // the partials, at 5 TB/s
       if (least == 0.f || us < least) {
         least = us;

@@ -248,7 +248,7 @@ struct Stager {
     } else {
       const int64_t rows = min(min(g.K, (int64_t)o.krows) - k0, (int64_t)BK);
       p = (seg ? base[1] : base[0]) + k0 * ldb;
-      bytes = (uint32_t)((rows - 1) * ldb + cols);
+      bytes = rows > 0 ? (uint32_t)((rows - 1) * ldb + cols) : 0u;
     }
     const auto r = rsrc(p, bytes);
 #pragma unroll
@@ -303,20 +303,25 @@ __device__ __forceinline__ TileId tile_of(const GemmArgs& g) {
 // steps, where every wave has the stage's last fragments in registers (its buffer is free for the loads of the stage
 // ST ahead) and the next stage has landed (its first fragments can be read).  So neither LDS reads nor
 // loads are waited for between products, except by the first.
-template <class T, int BM, int BN, int WM, int WN, int ST, int AMODE, int BMODE, class Epi>
-__global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) void gemm_kernel(GemmArgs g, typename Epi::Args e) {
+//
+// With KG = 2 two groups of WM x WN waves each make the whole tile from every other stage, their own in LDS, and add up
+// at the end, half of the rows each.
+template <class T, int BM, int BN, int WM, int WN, int ST, int AMODE, int BMODE, class Epi, int KG = 1>
+__global__ __launch_bounds__(64 * WM * WN * KG, KG == 2 || BM * BN / (WM * WN) <= 12288 ? 2 : 1) void gemm_kernel(GemmArgs g, typename Epi::Args e) {
   constexpr int NW = WM * WN, MI = BM / WM / 16, NI = BN / WN / 16, BK = GEMM_BK;
   constexpr int A_EL = BM * BK, STAGE = (BM + BN) * BK;
   typedef Stager<BM, BK, NW, AMODE> SA;
   typedef Stager<BN, BK, NW, BMODE> SB;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[ST * STAGE];
+  __shared__ __attribute__((aligned(16))) uint16_t lds_all[KG * ST * STAGE];
 
-  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+  const int wave_all = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+  const int kg = KG == 1 ? 0 : wave_all / NW, wave = wave_all - kg * NW;       // the wave's group, and its number there
+  uint16_t* lds = lds_all + kg * ST * STAGE;
   const int c = lane & 15, q = lane >> 4;
   const TileId t = tile_of(g);
   const int m0 = t.m * BM, n0 = t.n * BN;
   const int nk1 = (int)((g.K + BK - 1) / BK);                                    // stages of a segment
-  const int s0 = t.split * g.split_stages, nk = min(nk1 * g.segments - s0, g.split_stages);
+  const int s0 = t.split * g.split_stages, nk = (min(nk1 * g.segments - s0, g.split_stages) + KG - 1) / KG;
   const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
 
   SA sa;
@@ -325,8 +330,8 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) 
   sb.init(g.b, g, n0, wave, lane);
   auto issue = [&](int s) {
     uint16_t* p = lds + (s % ST) * STAGE;
-    const int seg = s0 + s >= nk1;
-    const int64_t k0 = (int64_t)(s0 + s - seg * nk1) * BK;
+    const int at = s0 + KG * s + kg, seg = at >= nk1 && g.segments > 1;         // of an odd number of stages one group's last is past the end: zeros
+    const int64_t k0 = (int64_t)(at - seg * nk1) * BK;
     sa.issue(g.a, g, p, seg, k0);
     sb.issue(g.b, g, p + A_EL, seg, k0);
   };
@@ -393,13 +398,35 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 12288 ? 1 : 2) 
   for (; s + ST < nk; ++s) stage(s, std::true_type{});
   for (; s < nk; ++s) stage(s, std::false_type{});
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  Epi::template run<T, BM, BN, WM, WN, MI, NI>(e, acc, t, m0 + wm, n0 + wn, c, q, wave, lds);
+  if constexpr (KG == 1) {
+    Epi::template run<T, BM, BN, WM, WN, MI, NI>(e, acc, t, m0 + wm, n0 + wn, c, q, wave, lds);
+  } else {
+    static_assert(MI % 2 == 0 && BM * BN * 2 <= KG * ST * STAGE, "halves, through the stages' LDS");
+    constexpr int HI = MI / 2;
+    f32x4* part = (f32x4*)lds_all + (size_t)wave * HI * NI * 64 + lane;       // [2][NW][HI][NI][64]
+    constexpr int OTHER = NW * HI * NI * 64;
+    __syncthreads();                               // the last stages have been read
+    f32x4 sum[HI][NI];
+#pragma unroll
+    for (int i = 0; i < HI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        sum[i][j] = kg ? acc[HI + i][j] : acc[i][j];
+        part[kg * OTHER + (i * NI + j) * 64] = kg ? acc[i][j] : acc[HI + i][j];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < HI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) sum[i][j] += part[(1 - kg) * OTHER + (i * NI + j) * 64];
+    Epi::template run<T, BM, BN, WM, WN, HI, NI>(e, sum, t, m0 + wm + 16 * HI * kg, n0 + wn, c, q, wave, lds);
+  }
 }
 
 // Epilogue: C as it is, rounded once to 16 bits; from row `second` on it goes to the second tensor's rows (`second`
 // is a multiple of 16).  M: rows of each.
 struct EpiStore {
-  static constexpr bool LONG = false;
+  static constexpr bool LONG = false, GROUPS = true;
   struct Args { Rows c[2]; int second, M, N; };
   template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
   static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
@@ -418,7 +445,7 @@ struct EpiStore {
 
 // Epilogue: fp32 partial products of one k split, [splits][M][N] (N padded to a multiple of 4).
 struct EpiPartial {
-  static constexpr bool LONG = false;
+  static constexpr bool LONG = false, GROUPS = false;
   struct Args { float* p; int M, N; };
   template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
   static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,

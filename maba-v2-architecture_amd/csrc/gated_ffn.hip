@@ -23,7 +23,7 @@ namespace ffn {
 
 // A wave's 32 columns of a tile are 16 of g and the same 16 of u; the epilogues take four such blocks at once.
 struct EpiGated {
-  static constexpr bool LONG = false;
+  static constexpr bool LONG = false, GROUPS = false;
   struct Args { Rows h; int M, I; };
   static __device__ __forceinline__ f32x4 gated(f32x4 g, f32x4 u) {
     f32x4 v;
@@ -59,7 +59,7 @@ struct EpiGated {
 
 // d [M, 2 Iw], Iw = I rounded up to 16: dg at column 0, du at column Iw, zeros behind each.
 struct EpiGatedBack {
-  static constexpr bool LONG = false;
+  static constexpr bool LONG = false, GROUPS = false;
   struct Args { Rows dh, d; int M, I, Iw; };
   static __device__ __forceinline__ void grads(f32x4 g, f32x4 u, f32x4 dh, f32x4& dg, f32x4& du) {
 #pragma unroll
@@ -162,7 +162,7 @@ static GatedPlan gated_plan(const maba_tensor* x, const maba_tensor* scales, con
     p.d = c.take<uint16_t>(p.M * 2 * p.Iw);
     int64_t part = 0;
     if (dx) {
-      p.dx = gemm_plan(p.M, p.Cp, gemm_stages(p.Iw, 2), PLAN_COLUMNS | PLAN_SPLIT);
+      p.dx = gemm_plan(p.M, p.Cp, gemm_stages(p.Iw, 2), PLAN_COLUMNS | PLAN_SPLIT | PLAN_GROUPS);
       if (p.dx.splits > 1) part = (int64_t)p.dx.splits * p.M * p.Cp;
     }
     if (dw) {

@@ -102,7 +102,7 @@ struct Reads {
 
 template <int ACT>
 struct EpiLinear {
-  static constexpr bool LONG = false;
+  static constexpr bool LONG = false, GROUPS = true;
   struct Args { Rows y, res; const uint16_t *bias, *gate; int M, N; };
   static __device__ __forceinline__ f32x4 value(f32x4 z, f32x4 bias, f32x4 gate, f32x4 res) {
     z += bias;
@@ -153,7 +153,7 @@ template <int ACT>
 struct EpiLinearBack {
   // beside a 256 x 256 tile's sums its values do not fit into the registers (16,384 x 640 to 2,496: relu 150 us and gelu
   // 202, with 192 x 128 92 and 121)
-  static constexpr bool LONG = true;
+  static constexpr bool LONG = true, GROUPS = false;
   struct Args { Rows dy, dz; const uint16_t *bias, *gate; float* sums; int M, N, Np; };
   // dz, and its terms and those of dy * act(z) added to the column sums.  dy is zero behind the last row.
   static __device__ __forceinline__ f32x4 value(f32x4 z, f32x4 dy, f32x4 bias, f32x4 gate, f32x4& sb, f32x4& sg, bool in) {
@@ -272,7 +272,7 @@ static LinearPlan linear_plan(const maba_tensor* x, const maba_tensor* scales, c
     if (p.z || p.copy_dy) p.dz = c.take<uint16_t>(p.M * p.Np);
     int64_t part = 0;
     if (need->dx) {
-      p.dx = gemm_plan(p.M, p.Kp, gemm_stages(p.Np, 1), PLAN_COLUMNS | PLAN_SPLIT);
+      p.dx = gemm_plan(p.M, p.Kp, gemm_stages(p.Np, 1), PLAN_COLUMNS | PLAN_SPLIT | PLAN_GROUPS);
       if (p.dx.splits > 1) part = (int64_t)p.dx.splits * p.M * p.Kp;
     }
     if (p.g) {
@@ -281,7 +281,7 @@ static LinearPlan linear_plan(const maba_tensor* x, const maba_tensor* scales, c
     }
     p.part = c.take<float>(part);
   }
-  p.xw = gemm_plan(p.M, p.Np, gemm_stages(p.Kp, 1), need ? PLAN_LONG : few ? 0 : PLAN_SPLIT);
+  p.xw = gemm_plan(p.M, p.Np, gemm_stages(p.Kp, 1), need ? PLAN_LONG : few ? 0 : PLAN_SPLIT | PLAN_GROUPS);
   if (p.xw.splits > 1) p.part = c.take<float>((int64_t)p.xw.splits * p.M * p.Np);
   p.cols = need && (need->dbias || (need->dgate && (p.z || bias)));
   if (p.cols) {

@@ -334,6 +334,22 @@ def test_a_few_tiles_of_every_length(M, K):
         B.check(v, want[name], name)
 
 
+@pytest.mark.parametrize("K", [320, 328, 449, 576, 1000, 1160, 1250])
+@pytest.mark.parametrize("M,N", [(600, 640), (2048, 640), (4000, 640), (6100, 640), (8190, 636), (1777, 1000)])
+def test_two_groups_of_waves_on_a_tile(M, N, K):
+    """Tiles fewer than compute units; odd and even numbers of stages, each group's half."""
+    t = _linear(M, K, N, BF, seed=45)
+    want = B.linear(t["x"], t["w"], t["bias"], "relu", t["residual"], t["gate"])
+    B.check(D.linear_epilogue(t["x"], t["w"], t["bias"], "relu", t["residual"], t["gate"]), want["y"], "y")
+    # dx of a layer of K outputs: the sum runs over K
+    dy, w = t["x"], t["w"].t().contiguous()
+    want = B.linear(t["residual"], w, None, "none", None, None, dy)
+    B.check(D.linear_epilogue_backward(dy, t["residual"], w, needs=(True, False, False, False))[0], want["dx"], "dx")
+    if M < 3000:
+        x, wg, wu, dh = _gated(M, N, K // 2 + 5, HF, seed=46)
+        B.check(D.gated_ffn_backward(dh, x, wg, wu, needs=(True, False, False))[0], B.gated(x, wg, wu, dh)["dx"], "dx")
+
+
 @pytest.mark.parametrize("K", [1528, 1536, 1537, 1544, 2048, 2056])
 @pytest.mark.parametrize("M", [16, 17, 32, 33])
 def test_where_few_rows_change_kernels(M, K):
