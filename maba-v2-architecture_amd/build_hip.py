@@ -74,6 +74,26 @@ def build_library() -> str:
     return LIB
 
 
+def build_torch_binding() -> str:
+    """``csrc/torch_binding.cpp`` (host code over torch's C++ API) as a Python module beside the library."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    out = os.path.join(os.path.dirname(LIB), "maba_torch.so")
+    os.makedirs(os.path.dirname(out), exist_ok=True)
+    tmp = out + ".tmp"
+    includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include")]
+    _run([HIPCC, "-x", "c++", "-O2", "-fPIC", "-std=c++17", "-shared", "-Wall", "-Wno-unused-function", "-DUSE_ROCM=1",
+          "-D__HIP_PLATFORM_AMD__=1", "-DTORCH_EXTENSION_NAME=maba_torch",
+          *(f for d in includes for f in ("-isystem", d)),
+          os.path.join(CSRC, "torch_binding.cpp"), "-o", tmp, "-L" + os.path.join(root, "lib"),
+          "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python"])
+    os.replace(tmp, out)
+    return out
+
+
 def build_test_probes() -> str:
     src = os.path.join(REPO, "tests", "hip", "mfma_probe.hip")
     out_dir = os.path.join(REPO, "tests", "hip", "_build")
@@ -88,5 +108,8 @@ def clean() -> None:
 
 
 if __name__ == "__main__":
-    print(build_library())
+    with cf.ThreadPoolExecutor(max_workers=2) as ex:
+        binding = ex.submit(build_torch_binding)
+        print(build_library())
+        print(binding.result())
     print(build_test_probes())

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import importlib.util
 import os
 import struct
 import threading
@@ -250,6 +251,30 @@ _NOTHING = contextlib.nullcontext()
 def on_device(device: torch.device):
     """A context in which ``device`` is current (kernel launches and workspace queries go by it)."""
     return _NOTHING if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+_binding = None
+_BOUND = ("gated_ffn_workspace_size", "gated_ffn", "gated_ffn_backward_workspace_size", "gated_ffn_backward",
+          "linear_epilogue_workspace_size", "linear_epilogue", "linear_epilogue_backward_workspace_size",
+          "linear_epilogue_backward", "checkpoint_pack", "checkpoint_unpack", "last_error")
+
+
+def binding():
+    """The native torch binding (``csrc/torch_binding.cpp``) over the loaded library; raises ``HipLibraryMissing``."""
+    global _binding
+    if _binding is None:
+        lib = load()
+        with _lock:
+            if _binding is None:
+                path = os.path.join(LIB_DIR, "maba_torch.so")
+                if not os.path.exists(path):
+                    raise HipLibraryMissing(f"{path} not found; run __graft_entry__.build() first")
+                spec = importlib.util.spec_from_file_location("maba_torch", path)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                module.bind({n: ctypes.cast(getattr(lib, "maba_hip_" + n), ctypes.c_void_p).value for n in _BOUND})
+                _binding = module
+    return _binding
 
 
 def check(rc: int, what: str) -> None:

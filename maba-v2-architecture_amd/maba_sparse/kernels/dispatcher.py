@@ -38,6 +38,7 @@ from typing import Any, Callable, Dict, Optional, Set, Tuple, Union
 
 import torch
 
+from maba_sparse import _native
 from maba_sparse._native import HipLibraryMissing
 from maba_sparse.kernels import common as _c
 from maba_sparse.kernels import cpu_dgda as _cpu
@@ -452,6 +453,36 @@ class _FFNOps:
                          needs=tuple(needs)), self.backend)
 
 
+# op -> the native binding's form of it, and the kernels of this package that it stands for
+_NATIVE: Dict[str, Tuple[Callable, Tuple[Tuple[str, Callable], ...]]] = {}
+
+
+def _load_native() -> None:
+    _ensure_hip_registered()
+    import maba_sparse.kernels.hip_backend as hb
+    binding, ops = _native.binding(), {}
+    for op, names in (("gated_ffn", ("gated_ffn", "gated_ffn_backward")), ("checkpoint_pack", ("checkpoint_pack",)),
+                      ("linear_epilogue", ("linear_epilogue", "linear_epilogue_backward")),
+                      ("checkpoint_unpack", ("checkpoint_unpack",))):
+        ops[op] = (getattr(binding, op), tuple((n, getattr(hb, "hip_" + n)) for n in names))
+    _NATIVE.update(ops)
+
+
+def _bound(op: str, x) -> Optional[Callable]:
+    """The native binding's form of ``op`` where ``x`` goes to this package's own HIP kernels, else None.  It returns None
+    for a call that is not plain, which then takes the path with the checks, the fallbacks and the errors."""
+    if not x.is_cuda or get_backend(x.device) != "hip":
+        return None
+    if not _NATIVE:
+        _load_native()
+    fn, own = _NATIVE[op]
+    registered = _KERNEL_REGISTRY["hip"]
+    for name, kernel in own:
+        if registered.get(name) is not kernel:
+            return None
+    return fn
+
+
 def _wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -462,11 +493,16 @@ def dispatch_gated_ffn(x, w_gate, w_up, checkpoint: Optional[str] = None) -> tor
     x ``[..., C]``, w_gate and w_up ``[I, C]`` of one dtype and device; returns ``[..., I]``, computed in
     fp32 and rounded once.  Differentiable on every backend.  What the backward pass keeps is ``x``; with
     ``checkpoint="e4m3"`` its packed form, half the bytes, and the gradients are those at the unpacked input."""
+    _ffn_checkpoint(checkpoint)
+    native = _bound("gated_ffn", x)
+    if native is not None:
+        out = native(x, w_gate, w_up, checkpoint is not None)
+        if out is not None:
+            return _ff.guard_capture(out)
     _ffn_input(x)
     _ffn_same(x, w_gate=w_gate, w_up=w_up)
     _ffn_weight("w_gate", w_gate, x.shape[-1])
     _ffn_shape("w_up", w_up, w_gate.shape)
-    _ffn_checkpoint(checkpoint)
     if _wants_grad(x, w_gate, w_up):
         return _ff.guard_capture(_ff.GatedFFN.apply(_FFNOps(x.device), checkpoint, x, w_gate, w_up))
     return _FFNOps(x.device).gated_ffn(x, w_gate, w_up)
@@ -494,6 +530,13 @@ def dispatch_linear_epilogue(x, weight, bias=None, activation: str = "none", res
     x ``[..., K]``, weight ``[N, K]``, bias and gate ``[N]``, residual ``[..., N]`` of one dtype and device; bias,
     gate and residual are optional; activation none, relu, silu or gelu (with the error function).  Computed
     in fp32 and rounded once.  Differentiable on every backend; ``checkpoint`` as for ``gated_ffn``."""
+    _ffn_activation(activation)
+    _ffn_checkpoint(checkpoint)
+    native = _bound("linear_epilogue", x)
+    if native is not None:
+        out = native(x, weight, bias, _c.ACTIVATIONS.index(activation), residual, gate, checkpoint is not None)
+        if out is not None:
+            return _ff.guard_capture(out)
     _ffn_input(x)
     _ffn_same(x, weight=weight, bias=bias, residual=residual, gate=gate)
     _ffn_weight("weight", weight, x.shape[-1])
@@ -501,8 +544,6 @@ def dispatch_linear_epilogue(x, weight, bias=None, activation: str = "none", res
     _ffn_shape("bias", bias, (n,))
     _ffn_shape("gate", gate, (n,))
     _ffn_shape("residual", residual, (*x.shape[:-1], n))
-    _ffn_activation(activation)
-    _ffn_checkpoint(checkpoint)
     if _wants_grad(x, weight, bias, residual, gate):
         return _ff.guard_capture(_ff.LinearEpilogue.apply(_FFNOps(x.device), checkpoint, activation, x, weight, bias, residual, gate))
     return _FFNOps(x.device).linear_epilogue(x, weight, bias, activation, residual, gate)
@@ -535,6 +576,11 @@ def dispatch_checkpoint_pack(x) -> Tuple[torch.Tensor, torch.Tensor]:
         raise ValueError(f"x must have a positive channel dimension, got {list(x.shape)}")
     if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise TypeError(f"Unsupported dtype {x.dtype}. Supported: {(torch.float32, torch.float16, torch.bfloat16)}")
+    native = _bound("checkpoint_pack", x)
+    if native is not None:
+        out = native(x)
+        if out is not None:
+            return out
     return _FFNOps(x.device).pack(x.detach() if x.requires_grad else x)
 
 
@@ -545,6 +591,11 @@ def dispatch_checkpoint_unpack(codes, scales, dtype: torch.dtype = torch.bfloat1
     _ffn_kept(codes, scales)
     if dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise TypeError(f"Unsupported dtype {dtype}. Supported: {(torch.float32, torch.float16, torch.bfloat16)}")
+    native = _bound("checkpoint_unpack", codes)
+    if native is not None:
+        out = native(codes, scales, dtype)
+        if out is not None:
+            return out
     return _run("checkpoint_unpack", codes.device, dict(codes=codes, scales=scales, dtype=dtype))
 
 

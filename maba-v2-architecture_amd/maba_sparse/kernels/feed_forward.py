@@ -4,6 +4,9 @@ backward ops, the same on every backend.
 The forward pass keeps its input (or, with ``checkpoint="e4m3"``, the input's packed form) and the
 parameters; the backward op makes the pre-activations again from it.  With a checkpoint the gradients
 are those at the unpacked input: the forward result is unaffected.
+
+Calls that go to this package's own HIP kernels take the same functions natively (``csrc/torch_binding.cpp``); these
+here serve the other backends, kernels registered in their place and calls that the binding declines.
 """
 from __future__ import annotations
 

@@ -427,6 +427,123 @@ def test_model_block_fused_feed_forward():
         assert torch.equal(ffn(x), ffn.forward_hip(x))
 
 
+# ----------------------------------------------------------------------------- the native binding and the Python path
+
+
+def _both_ways(monkeypatch, call):
+    """``call`` through the native binding and, with wrapped kernels registered, through Python."""
+    native = call()
+    hip = D._KERNEL_REGISTRY["hip"]
+    used = []
+    for name in ("gated_ffn", "gated_ffn_backward", "linear_epilogue", "linear_epilogue_backward", "checkpoint_pack",
+                 "checkpoint_unpack"):
+        def wrapped(_f=hip[name], _n=name, **kw):
+            used.append(_n)
+            return _f(**kw)
+        monkeypatch.setitem(hip, name, wrapped)
+    return native, call(), used
+
+
+@pytest.mark.parametrize("ckpt", [None, "e4m3"])
+@pytest.mark.parametrize("shape", [(5, 64), (3, 50, 72), (200, 33), (64,)])
+def test_native_and_python_paths_give_the_same_bits(monkeypatch, shape, ckpt):
+    r = _gen(71)
+    Cw = shape[-1]
+    x, wg, wu, w = (r(*s).to(BF).requires_grad_() for s in (shape, (40, Cw), (40, Cw), (24, 40)))
+    b, g, res = (r(*s).to(BF).requires_grad_() for s in ((24,), (24,), (*shape[:-1], 24)))
+    dy = r(*shape[:-1], 24).to(BF)
+
+    def call():
+        h = D.gated_ffn(x, wg, wu, checkpoint=ckpt)
+        y = D.linear_epilogue(h, w, b, "gelu", res, g, checkpoint=ckpt)
+        with torch.no_grad():
+            plain = D.linear_epilogue(D.gated_ffn(x, wg, wu), w, b, "gelu", res, g)
+        codes, scales = D.checkpoint_pack(x)
+        grads = torch.autograd.grad(y, (x, wg, wu, w, b, res, g), dy)
+        some = torch.autograd.grad(D.linear_epilogue(x.detach(), wg, None, "none", None, None), (wg,), torch.ones_like(h))
+        return [y, plain, codes.view(torch.uint8), scales, D.checkpoint_unpack(codes, scales, HF), *grads, *some]
+
+    native, python, used = _both_ways(monkeypatch, call)
+    assert set(used) >= {"gated_ffn", "gated_ffn_backward", "linear_epilogue", "linear_epilogue_backward", "checkpoint_pack"}
+    assert all(a.shape == b.shape and a.dtype == b.dtype and torch.equal(a, b) for a, b in zip(native, python))
+
+
+def test_double_backward_is_refused_and_first_is_not():
+    x, wg, wu, dh = _gated(20, 64, 24, BF, seed=72)
+    x.requires_grad_()
+    w = wg.detach().clone().requires_grad_()
+    for call in (lambda: D.gated_ffn(x, w, wu), lambda: D.linear_epilogue(x, w, None, "silu")):
+        plain = torch.autograd.grad(call(), (x, w), dh)
+        grads = torch.autograd.grad(call(), (x, w), dh, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(plain, grads))
+        with pytest.raises(RuntimeError, match="twice"):
+            (grads[0].float().sum() + grads[1].float().sum()).backward()
+
+
+def test_calls_that_the_binding_declines_raise_as_before():
+    x, wg, wu, _ = _gated(20, 64, 24, BF, seed=73)
+    with pytest.raises(RuntimeError, match="same device"):
+        D.gated_ffn(x, wg.cpu(), wu)
+    with pytest.raises(TypeError, match="dtypes must match"):
+        D.gated_ffn(x, wg.half(), wu)
+    with pytest.raises(ValueError, match="w_gate"):
+        D.gated_ffn(x[:, :32], wg, wu)
+    with pytest.raises(ValueError, match="w_up"):
+        D.gated_ffn(x, wg, wu[:-1])
+    with pytest.raises(ValueError, match="checkpoint"):
+        D.gated_ffn(x, wg, wu, checkpoint="int4")
+    with pytest.raises(ValueError, match="residual"):
+        D.linear_epilogue(x, wg, None, "none", x)
+    with pytest.raises(ValueError, match="gate"):
+        D.linear_epilogue(x, wg, gate=wg[0])
+    with pytest.raises(ValueError, match="activation"):
+        D.linear_epilogue(x, wg, None, "tanh")
+    codes, scales = D.checkpoint_pack(x)
+    with pytest.raises(ValueError, match="x_scales"):
+        D.checkpoint_unpack(codes, scales[:, :1])
+    with pytest.raises(TypeError):
+        D.checkpoint_unpack(codes, scales, torch.float64)
+
+
+def test_saved_tensors_follow_their_hooks_and_versions():
+    x, wg, wu, dh = _gated(20, 64, 24, BF, seed=74)
+    x.requires_grad_()
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t.shape) or t.cpu(), lambda t: t.to(DEV)):
+        y = D.gated_ffn(x, wg, wu)
+    assert len(seen) == 3
+    assert torch.equal(torch.autograd.grad(y, x, dh)[0], torch.autograd.grad(D.gated_ffn(x, wg, wu), x, dh)[0])
+    w = wg.clone()
+    y = D.gated_ffn(x, w, wu)
+    w.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, x, dh)
+
+
+def test_two_threads_call_at_once():
+    import threading
+    sets = [_gated(300 + 40 * i, 136, 72, BF, seed=80 + i) for i in range(2)]
+    want = [torch.autograd.grad(D.gated_ffn(x.requires_grad_(), wg, wu), x, dh)[0] for x, wg, wu, dh in sets]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        x, wg, wu, dh = sets[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = torch.autograd.grad(D.gated_ffn(x, wg, wu, checkpoint=None), x, dh)[0]
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(got, want[i]):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 # ----------------------------------------------------------------------------- graphs
 
 
