@@ -339,6 +339,16 @@ def test_c_workspace_sizes(lib):
     assert some >= 2 * 64 * 96 and b(_t([64, 32]), None, _t([48, 32]), _t([48, 32]), 3) >= some
 
 
+def test_native_binding_declines_what_is_not_on_a_gpu(lib):
+    m = N.binding()
+    x, w = torch.randn(3, 8).bfloat16(), torch.randn(5, 8).bfloat16()
+    assert m.gated_ffn(x, w, w, False) is None
+    assert m.linear_epilogue(x, w, None, 0, None, None, True) is None
+    assert m.checkpoint_pack(x) is None
+    codes, scales = D.checkpoint_pack(x)
+    assert m.checkpoint_unpack(codes, scales, torch.float16) is None
+
+
 def test_c_workspace_must_be_aligned(lib):
     x, wg, wu, dh = _t([64, 31], data=X), _t([48, 31], data=W), _t([48, 31], data=W + 0x10000), _t([64, 48], data=H)
     far = 0x900000

@@ -468,6 +468,23 @@ def test_native_and_python_paths_give_the_same_bits(monkeypatch, shape, ckpt):
     assert all(a.shape == b.shape and a.dtype == b.dtype and torch.equal(a, b) for a, b in zip(native, python))
 
 
+@pytest.mark.parametrize("which", [(0,), (1,), (2,), (3,), (4,), (0, 2), (2, 3), (1, 4)])
+@pytest.mark.parametrize("act,ckpt", [("none", None), ("none", "e4m3"), ("silu", None), ("silu", "e4m3")])
+def test_autograd_of_some_inputs(act, ckpt, which):
+    """Frozen inputs change nothing for the others, also where x need not be kept."""
+    t = _linear(70, 48, 40, BF, seed=75)
+    names = ("x", "w", "bias", "residual", "gate")
+
+    def grads(live):
+        a = [t[n].detach().clone().requires_grad_(i in live) for i, n in enumerate(names)]
+        y = D.linear_epilogue(a[0], a[1], a[2], act, a[3], a[4], checkpoint=ckpt)
+        return dict(zip(live, torch.autograd.grad(y, [a[i] for i in live], t["dy"])))
+
+    every = grads(range(5))
+    for i, g in grads(which).items():
+        assert torch.equal(g, every[i]), names[i]
+
+
 def test_double_backward_is_refused_and_first_is_not():
     x, wg, wu, dh = _gated(20, 64, 24, BF, seed=72)
     x.requires_grad_()
