@@ -10,6 +10,9 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <cstdlib>
+#include <strings.h>
+
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -275,8 +278,18 @@ struct LinearEpilogue : public torch::autograd::Function<LinearEpilogue> {
 
 // ---------------------------------------------------------------- the module's functions
 
+// Whether the dispatcher's backend for GPU tensors is this library: MABA_BACKEND as its get_backend reads it, without the
+// 1.3 us that takes in Python.  Any other value is declined, and the Python path routes or refuses it.
+bool routed_here() {
+  const char* e = std::getenv("MABA_BACKEND");
+  if (!e || !*e) return true;
+  for (const char* name : {"auto", "hip", "triton", "cuda", "gpu"})
+    if (!strcasecmp(e, name)) return true;
+  return false;
+}
+
 Maybe gated_ffn(const Tensor& x, const Tensor& wg, const Tensor& wu, bool packed) {
-  if (!alike(x, {&wg, &wu}) || x.dim() < 1 || wg.dim() != 2 || wg.size(0) == 0 || x.size(-1) == 0 || wg.size(1) != x.size(-1) ||
+  if (!routed_here() || !alike(x, {&wg, &wu}) || x.dim() < 1 || wg.dim() != 2 || wg.size(0) == 0 || x.size(-1) == 0 || wg.size(1) != x.size(-1) ||
       wu.sizes() != wg.sizes())
     return std::nullopt;
   try {
@@ -290,7 +303,7 @@ Maybe gated_ffn(const Tensor& x, const Tensor& wg, const Tensor& wu, bool packed
 Maybe linear_epilogue(const Tensor& x, const Tensor& w, const Maybe& bias_, int64_t act, const Maybe& res_, const Maybe& gate_,
                       bool packed) {
   const Tensor bias = bias_.value_or(Tensor()), res = res_.value_or(Tensor()), gate = gate_.value_or(Tensor());
-  if (!alike(x, {&w, &bias, &res, &gate}) || x.dim() < 1 || w.dim() != 2 || w.size(0) == 0 || x.size(-1) == 0 ||
+  if (!routed_here() || !alike(x, {&w, &bias, &res, &gate}) || x.dim() < 1 || w.dim() != 2 || w.size(0) == 0 || x.size(-1) == 0 ||
       w.size(1) != x.size(-1))
     return std::nullopt;
   for (const Tensor* v : {&bias, &gate})
@@ -305,7 +318,7 @@ Maybe linear_epilogue(const Tensor& x, const Tensor& w, const Maybe& bias_, int6
 }
 
 std::optional<std::pair<Tensor, Tensor>> checkpoint_pack(const Tensor& x) {
-  if (!plain(x) || x.dim() < 1 || x.size(-1) == 0) return std::nullopt;
+  if (!routed_here() || !plain(x) || x.dim() < 1 || x.size(-1) == 0) return std::nullopt;
   try {
     return pack_call(x.requires_grad() ? x.detach() : x);
   } catch (const Declined&) {
@@ -314,7 +327,7 @@ std::optional<std::pair<Tensor, Tensor>> checkpoint_pack(const Tensor& x) {
 }
 
 Maybe checkpoint_unpack(const Tensor& codes, const Tensor& scales, at::ScalarType dtype) {
-  if (!plain(codes) || !plain(scales) || codes.device() != scales.device() || codes.dim() < 1 || codes.size(-1) == 0 ||
+  if (!routed_here() || !plain(codes) || !plain(scales) || codes.device() != scales.device() || codes.dim() < 1 || codes.size(-1) == 0 ||
       codes.scalar_type() != at::kFloat8_e4m3fn || scales.scalar_type() != at::kByte ||
       scales.sizes() != at::IntArrayRef(outer(codes, (codes.size(-1) + 31) / 32)))
     return std::nullopt;

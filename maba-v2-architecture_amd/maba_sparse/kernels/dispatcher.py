@@ -469,9 +469,10 @@ def _load_native() -> None:
 
 
 def _bound(op: str, x) -> Optional[Callable]:
-    """The native binding's form of ``op`` where ``x`` goes to this package's own HIP kernels, else None.  It returns None
-    for a call that is not plain, which then takes the path with the checks, the fallbacks and the errors."""
-    if not x.is_cuda or get_backend(x.device) != "hip":
+    """The native binding's form of ``op`` for a GPU tensor ``x``, unless another kernel is registered in place of this
+    package's own.  It returns None for a call that is not plain or goes to another backend, which then takes the path
+    with the checks, the fallbacks and the errors."""
+    if not x.is_cuda or torch.version.hip is None:
         return None
     if not _NATIVE:
         _load_native()

@@ -672,3 +672,21 @@ def test_capture_beside_a_live_eager_graph_is_refused():
     assert torch.equal(out[1], want)
     del eager
     gc.collect()
+
+
+@pytest.mark.parametrize("env,reference", [("reference", True), ("HIP", False), ("auto", False), ("", False)])
+def test_the_backend_that_is_asked_for(monkeypatch, env, reference):
+    x, wg, wu, _ = _gated(20, 64, 24, BF, seed=76)
+    used = []
+
+    def ref(_f=D._KERNEL_REGISTRY["reference"]["gated_ffn"], **kw):
+        used.append("reference")
+        return _f(**kw)
+
+    monkeypatch.setitem(D._KERNEL_REGISTRY["reference"], "gated_ffn", ref)
+    monkeypatch.setenv("MABA_BACKEND", env)
+    B.check(D.gated_ffn(x, wg, wu), B.gated(x, wg, wu)["h"], "h")
+    assert bool(used) == reference
+    monkeypatch.setenv("MABA_BACKEND", "rocm")
+    with pytest.raises(ValueError):
+        D.gated_ffn(x, wg, wu)
