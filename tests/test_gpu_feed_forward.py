@@ -690,3 +690,23 @@ def test_the_backend_that_is_asked_for(monkeypatch, env, reference):
     monkeypatch.setenv("MABA_BACKEND", "rocm")
     with pytest.raises(ValueError):
         D.gated_ffn(x, wg, wu)
+
+
+def test_outputs_are_ordinary_autograd_tensors():
+    """In-place changes of an output are recorded, and refused once a later op has kept it."""
+    x, wg, wu, dh = _gated(20, 64, 24, BF, seed=77)
+    w = _linear(20, 24, 16, BF, seed=78)["w"]
+    x.requires_grad_()
+    h = D.gated_ffn(x, wg, wu)
+    assert not h.is_leaf and not h.is_inference()
+    h.mul_(2)
+    want = torch.autograd.grad(D.gated_ffn(x, wg, wu), x, 2 * dh)[0]
+    assert torch.equal(torch.autograd.grad(h, x, dh)[0], want)
+    h = D.gated_ffn(x, wg, wu)
+    w.requires_grad_()
+    y = D.linear_epilogue(h, w)
+    h.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():
+        assert D.gated_ffn(x, wg, wu).is_inference()
