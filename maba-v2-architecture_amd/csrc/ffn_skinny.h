@@ -93,7 +93,7 @@ int skinny(const SkinnyArgs& a, const typename Epi::Args& e, hipStream_t s, cons
 }
 // Whether M rows of K go this way.  Every workgroup reads all of x, so that more than 16 rows of a long k are better
 // off in tiles: 32 rows, 2,048 to 2 x 5,504: 19.8 us here and 15.5 there (16 rows: 16.9 here), 1,024 to 2 x 2,816: 7.1 and
-// 7.7, and 1,248 to 640, where the tiles need their sum split: 5.0 and 8.3.
+// 7.7, and 1,248 to 640, where the tiles need their sum split: 5.0 and 6.9.
 inline bool few_rows(int64_t M, int64_t K) { return M <= 16 || (M <= 32 && K <= 1536); }
 
 }  // namespace ffn

@@ -122,6 +122,7 @@ __global__ __launch_bounds__(256) void reduce_gated_forward(const float* p, int 
     if (n >= e.I) continue;
     const float* at = p + (int64_t)m * 2 * Iw + 2 * (n & ~15) + (n & 15);
     f32x4 g = {0.f, 0.f, 0.f, 0.f}, u = g;
+#pragma unroll 8
     for (int s = 0; s < splits; ++s) {
       g += *(const f32x4*)(at + s * plane);
       u += *(const f32x4*)(at + s * plane + 16);

@@ -231,6 +231,7 @@ __global__ __launch_bounds__(256) void reduce_linear_forward(const float* p, int
     const int m = (int)(i / quads), n = (int)(i % quads) * 4;
     if (n >= e.N) continue;
     f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
     for (int s = 0; s < splits; ++s) z += *(const f32x4*)(p + s * plane + (int64_t)m * Np + n);
     EpiLinear<ACT>::template quad<T>(e, m, n, z, z);
   }
