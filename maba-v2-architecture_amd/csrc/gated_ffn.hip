@@ -151,10 +151,10 @@ static GatedPlan gated_plan(const maba_tensor* x, const maba_tensor* scales, con
   p.Iw = ceil_div(p.I, 16) * 16;
   const bool few = !back && few_rows(p.M, p.C);       // that kernel reads any rows
   p.copy_x = !few && (scales || !aligned_rows(x));
-  // dx reads both weights with one stride
-  const bool apart = back && wg->stride[0] != wu->stride[0];
-  p.copy_w[0] = !few && (!aligned_rows(wg) || apart);
-  p.copy_w[1] = !few && (!aligned_rows(wu) || apart);
+  p.copy_w[0] = !few && !aligned_rows(wg);
+  p.copy_w[1] = !few && !aligned_rows(wu);
+  // dx reads both weights with one stride: each in place at the same stride, or both copied
+  if (back && (p.copy_w[0] || p.copy_w[1] || wg->stride[0] != wu->stride[0])) p.copy_w[0] = p.copy_w[1] = true;
   Carve c = {(char*)ws, 0};
   if (p.copy_x) p.x = c.take<uint16_t>(p.M * p.Cp);
   for (int i = 0; i < 2; ++i)

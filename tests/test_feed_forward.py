@@ -395,3 +395,16 @@ def test_c_pack_refusals(lib):
     assert call(x, _t([4, 40], dtype=N.MABA_U8, data=H), scales, None) == 2
     assert call(_t([4, 40], dtype=N.MABA_F64, data=X), codes, scales, None) == 2
     assert call(x, codes, _t([4, 2], dtype=N.MABA_U8, data=H + 8), None) == 1                   # scales over codes
+
+
+def test_c_backward_copies_both_weights_or_neither(lib):
+    """dx reads the two weights with one row stride: where one of them has to be copied, so is the other."""
+    size = lib.maba_hip_gated_ffn_backward_workspace_size
+    x, ld = _t([64, 72], data=X), [160, 1]
+    aligned, shifted = _t([48, 72], strides=ld, data=W), _t([48, 72], strides=ld, data=W + 152)
+    narrow = _t([48, 72], data=W)
+    for needs in (1, 2, 3):
+        both = size(x, None, shifted, shifted, needs)
+        assert size(x, None, aligned, shifted, needs) == size(x, None, shifted, aligned, needs) == both
+        assert size(x, None, aligned, narrow, needs) == size(x, None, narrow, aligned, needs) == both     # strides of their own
+        assert size(x, None, aligned, aligned, needs) == size(x, None, narrow, narrow, needs) < both

@@ -710,3 +710,24 @@ def test_outputs_are_ordinary_autograd_tensors():
         y.sum().backward()
     with torch.inference_mode():
         assert D.gated_ffn(x, wg, wu).is_inference()
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("M,Cw,I", [(5, 72, 48), (70, 72, 48), (300, 136, 264)])
+@pytest.mark.parametrize("up_first", [False, True])
+def test_weights_cut_from_one_tensor_at_unlike_alignments(M, Cw, I, up_first, dt):
+    """Two column ranges of one tensor, only one of which starts on a 16-byte boundary: one row stride, one weight read
+    in place and one copied by the forward."""
+    x, wg, wu, dh = _gated(M, Cw, I, dt, seed=90)
+    want = B.gated(x, wg, wu, dh)
+    big = torch.full((I, 2 * Cw + 24), float("nan"), dtype=dt, device=DEV)
+    a, b = big[:, :Cw], big[:, Cw + 4:2 * Cw + 4]
+    vg, vu = (b, a) if up_first else (a, b)
+    vg.copy_(wg)
+    vu.copy_(wu)
+    B.check(D.gated_ffn(x, vg, vu), want["h"], "h")
+    for name, got in zip(("dx", "dw_gate", "dw_up"), D.gated_ffn_backward(dh, x, vg, vu)):
+        B.check(got, want[name], name)
+    codes, scales = D.checkpoint_pack(x)
+    want = B.gated(x, wg, wu, dh, kept=B.unpack64(codes, scales))
+    B.check(D.gated_ffn_backward(dh, codes, vg, vu, x_scales=scales)[0], want["dx"], "dx")
