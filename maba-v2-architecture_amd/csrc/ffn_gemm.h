@@ -487,6 +487,9 @@ inline Rows rows_of(const maba_tensor* t) {
 inline bool aligned_rows(const maba_tensor* t) {
   return t->stride[0] % 8 == 0 && t->shape[1] % 8 == 0 && (uintptr_t)t->data % 16 == 0 && t->stride[0] <= (1 << 21);
 }
+// The same for reading it along its columns: rows past the last one are zeros by the descriptor's end, which takes rows
+// that lie apart (broadcast or overlapping ones would be read again in their place).
+inline bool aligned_columns(const maba_tensor* t) { return aligned_rows(t) && t->stride[0] >= t->shape[1]; }
 inline int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 inline size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 

@@ -150,9 +150,10 @@ static GatedPlan gated_plan(const maba_tensor* x, const maba_tensor* scales, con
   p.Cp = pad8(p.C);
   p.Iw = ceil_div(p.I, 16) * 16;
   const bool few = !back && few_rows(p.M, p.C);       // that kernel reads any rows
-  p.copy_x = !few && (scales || !aligned_rows(x));
-  p.copy_w[0] = !few && !aligned_rows(wg);
-  p.copy_w[1] = !few && !aligned_rows(wu);
+  const auto in_place = back ? aligned_columns : aligned_rows;
+  p.copy_x = !few && (scales || !in_place(x));
+  p.copy_w[0] = !few && !in_place(wg);
+  p.copy_w[1] = !few && !in_place(wu);
   // dx reads both weights with one stride: each in place at the same stride, or both copied
   if (back && (p.copy_w[0] || p.copy_w[1] || wg->stride[0] != wu->stride[0])) p.copy_w[0] = p.copy_w[1] = true;
   Carve c = {(char*)ws, 0};

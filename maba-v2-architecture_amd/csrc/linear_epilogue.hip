@@ -263,9 +263,10 @@ static LinearPlan linear_plan(const maba_tensor* x, const maba_tensor* scales, c
   p.g = need && (need->dw || (!p.z && need->dgate));
   // which products read x and W: forward both; backward x for z and G, W for z and dx
   const bool use_x = !need || p.z || p.g, use_w = !need || p.z || need->dx;
-  p.copy_x = !few && use_x && (scales || !aligned_rows(x));
-  p.copy_w = !few && use_w && (!aligned_rows(w) || (need && !p.z && gate));      // gate * W
-  p.copy_dy = need && !p.z && (need->dx || p.g) && !aligned_rows(dy);
+  const auto in_place = need ? aligned_columns : aligned_rows;
+  p.copy_x = !few && use_x && (scales || !in_place(x));
+  p.copy_w = !few && use_w && (!in_place(w) || (need && !p.z && gate));          // gate * W
+  p.copy_dy = need && !p.z && (need->dx || p.g) && !in_place(dy);
   Carve c = {(char*)ws, 0};
   if (p.copy_x) p.x = c.take<uint16_t>(p.M * p.Kp);
   if (p.copy_w) p.w = c.take<uint16_t>(p.N * p.Kp);

@@ -408,3 +408,17 @@ def test_c_backward_copies_both_weights_or_neither(lib):
         assert size(x, None, aligned, shifted, needs) == size(x, None, shifted, aligned, needs) == both
         assert size(x, None, aligned, narrow, needs) == size(x, None, narrow, aligned, needs) == both     # strides of their own
         assert size(x, None, aligned, aligned, needs) == size(x, None, narrow, narrow, needs) < both
+
+
+def test_c_backward_copies_rows_that_overlap(lib):
+    """What is read along its columns ends at its last row only if rows lie apart: broadcast and overlapping rows are
+    copied, rows that are apart are not."""
+    lin, gated = lib.maba_hip_linear_epilogue_backward_workspace_size, lib.maba_hip_gated_ffn_backward_workspace_size
+    for rows in (1, 100):
+        dense, broadcast, windows = (_t([rows, 64], strides=[s, 1], data=X) for s in (64, 0, 8))
+        x_copy, w = rows * 64 * 2, _t([64, 64], data=W)
+        for cut in (broadcast, windows):
+            assert lin(dense, cut, None, w, 0, 0, 0, 2) >= lin(dense, dense, None, w, 0, 0, 0, 2) + x_copy
+            assert lin(cut, dense, None, w, 0, 0, 0, 2) >= lin(dense, dense, None, w, 0, 0, 0, 2) + x_copy
+            assert gated(cut, None, w, w, 3) >= gated(dense, None, w, w, 3) + x_copy
+            assert lib.maba_hip_linear_epilogue_workspace_size(cut, w) == 0                  # along rows they are read in place

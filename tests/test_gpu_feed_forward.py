@@ -731,3 +731,44 @@ def test_weights_cut_from_one_tensor_at_unlike_alignments(M, Cw, I, up_first, dt
     codes, scales = D.checkpoint_pack(x)
     want = B.gated(x, wg, wu, dh, kept=B.unpack64(codes, scales))
     B.check(D.gated_ffn_backward(dh, codes, vg, vu, x_scales=scales)[0], want["dx"], "dx")
+
+
+@pytest.mark.parametrize("M", [1, 5, 64, 100, 1000])
+@pytest.mark.parametrize("act,gate", [("none", False), ("none", True), ("silu", True)])
+def test_rows_that_are_broadcast_or_overlap(M, act, gate):
+    """x, the output's gradient or both as one row repeated (strides (0, 1)) or as windows of a signal (strides (8, 1)):
+    no row past the last one counts."""
+    t = _linear(M, 64, 72, BF, seed=91)
+    r = _gen(92)
+
+    def forms(width):
+        yield r(1, width).to(BF).expand(M, width)
+        yield r(8 * M + width).to(BF).as_strided((M, width), (8, 1))
+
+    g = t["gate"] if gate else None
+    for x in (*forms(64), t["x"]):
+        for dy in (*forms(72), t["dy"]):
+            want = B.linear(x, t["w"], t["bias"], act, None, g, dy)
+            for name, got in zip(("dx", "dw", "dbias", "dgate"), D.linear_epilogue_backward(dy, x, t["w"], t["bias"], act, g)):
+                if got is not None:
+                    B.check(got, want[name], (act, name))
+    w = t["w"].clone().requires_grad_()
+    x = r(1, 64).to(BF).expand(M, 64)
+    D.linear_epilogue(x, w).sum(0).float().sum().backward()              # autograd hands back one row for all
+    B.check(w.grad, B.linear(x, w.detach(), dy=torch.ones(M, 72, dtype=BF, device=DEV))["dw"], "dw")
+
+
+def test_gated_rows_that_are_broadcast_or_overlap():
+    r = _gen(93)
+    for M in (1, 100, 1000):
+        _, wg, wu, dh = _gated(M, 64, 72, BF, seed=94)
+        for x in (r(1, 64).to(BF).expand(M, 64), r(8 * M + 64).to(BF).as_strided((M, 64), (8, 1))):
+            for d in (dh, dh[:1].expand(M, 72)):
+                want = B.gated(x, wg, wu, d)
+                B.check(D.gated_ffn(x, wg, wu), want["h"], "h")
+                for name, got in zip(("dx", "dw_gate", "dw_up"), D.gated_ffn_backward(d, x, wg, wu)):
+                    B.check(got, want[name], name)
+        one = wg[:1].expand(72, 64)                                       # and weights whose rows are one
+        want = B.gated(t := r(M, 64).to(BF), one, one, dh)
+        for name, got in zip(("dx", "dw_gate", "dw_up"), D.gated_ffn_backward(dh, t, one, one)):
+            B.check(got, want[name], name)
