@@ -4,8 +4,8 @@
 // Bound by the host: a training step of 1,777 x 555 to 1,001, whose kernels take 65 us, takes 95 us here and took 177 by the
 // Python path (an empty autograd function in Python: 78); a forward call 9 and 19.
 //
-// A call that is not plain (other dtypes or devices, shapes that do not fit, tensor subclasses, sizes that the library
-// refuses) is declined: the function returns None and the caller takes the Python path, which checks, raises or falls
+// A call that is not plain (other dtypes or devices, shapes that do not fit, tensor subclasses, tangents of forward-mode
+// derivatives, sizes that the library refuses) is declined: the function returns None and the caller takes the Python path, which checks, raises or falls
 // back.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -97,9 +97,9 @@ struct Scope {
   explicit Scope(const Tensor& t) : device(t.device()) {}
 };
 
-// Plain tensors of one 16-bit dtype on one GPU.
+// Plain tensors of one 16-bit dtype on one GPU, without a tangent.
 bool plain(const Tensor& t) {
-  return t.defined() && t.is_cuda() && t.layout() == at::kStrided &&
+  return t.defined() && t.is_cuda() && t.layout() == at::kStrided && !t._fw_grad(0).defined() &&
          !t.unsafeGetTensorImpl()->key_set().has_any(
              c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
                                   c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize}));

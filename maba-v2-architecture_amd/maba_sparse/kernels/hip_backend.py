@@ -19,6 +19,7 @@ import math
 from typing import Any, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from maba_sparse import _native as N
 from maba_sparse.kernels.common import (
@@ -33,6 +34,8 @@ from maba_sparse.kernels.dispatcher import register_kernel
 def _no_grad_needed(op: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise NotImplementedError(f"{op}: HIP kernels are forward-only; autograd uses the reference path")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{op}: HIP kernels carry no tangents; forward-mode derivatives use the reference path")
 
 
 def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:

@@ -422,3 +422,19 @@ def test_c_backward_copies_rows_that_overlap(lib):
             assert lin(cut, dense, None, w, 0, 0, 0, 2) >= lin(dense, dense, None, w, 0, 0, 0, 2) + x_copy
             assert gated(cut, None, w, w, 3) >= gated(dense, None, w, w, 3) + x_copy
             assert lib.maba_hip_linear_epilogue_workspace_size(cut, w) == 0                  # along rows they are read in place
+
+
+def test_tangents_are_not_dropped():
+    """Forward-mode derivatives: the host ops carry them, the HIP wrappers decline what would lose them."""
+    from torch.autograd import forward_ad
+
+    from maba_sparse.kernels import hip_backend as hb
+    x, w, t = _rand(3, 8, grad=False), _rand(5, 8, grad=False), _rand(3, 8, grad=False, seed=9)
+    hb._no_grad_needed("op", x, None)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, t)
+        torch.testing.assert_close(forward_ad.unpack_dual(D.linear_epilogue(dual, w)).tangent, t @ w.t())
+        assert forward_ad.unpack_dual(D.gated_ffn(dual, w, w)).tangent is not None
+        hb._no_grad_needed("op", x, None)
+        with pytest.raises(NotImplementedError, match="tangents"):
+            hb._no_grad_needed("op", w, None, dual)

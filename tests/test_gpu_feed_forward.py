@@ -772,3 +772,26 @@ def test_gated_rows_that_are_broadcast_or_overlap():
         want = B.gated(t := r(M, 64).to(BF), one, one, dh)
         for name, got in zip(("dx", "dw_gate", "dw_up"), D.gated_ffn_backward(dh, t, one, one)):
             B.check(got, want[name], name)
+
+
+def test_tangents_take_the_reference_path(monkeypatch):
+    """Forward-mode derivatives of 16-bit calls: the reference ops' with one warning, an error where fallbacks are errors."""
+    from torch.autograd import forward_ad
+    x, wg, wu, dh = _gated(20, 64, 24, BF, seed=95)
+    t = _gen(96)(20, 64).to(BF)
+    calls = [(lambda f, x, g: f(x, wg, wu), D.gated_ffn, C.ref_gated_ffn),
+             (lambda f, x, g: f(x, wg, None, "silu", None, wu[:, 0]), D.linear_epilogue, C.ref_linear_epilogue),
+             (lambda f, x, g: f(g, x, wg, wu)[0], D.gated_ffn_backward, C.ref_gated_ffn_backward)]
+    for call, op, ref in calls:
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(x, t)
+            with pytest.raises(RuntimeError):
+                call(op, dual, dh)
+            monkeypatch.setenv("MABA_STRICT_BACKEND", "0")
+            D.clear_fallback_warnings()
+            with pytest.warns(RuntimeWarning, match="tangents"):
+                got = forward_ad.unpack_dual(call(op, dual, dh))
+            monkeypatch.setenv("MABA_STRICT_BACKEND", "1")
+            want = forward_ad.unpack_dual(call(ref, dual, dh))
+        assert got.tangent is not None
+        assert torch.equal(got.tangent, want.tangent) and torch.equal(got.primal, want.primal)
