@@ -475,6 +475,8 @@ def _bound(op: str, x) -> Optional[Callable]:
     if not x.is_cuda or torch.version.hip is None:
         return None
     if not _NATIVE:
+        if get_backend(x.device) != "hip":         # later the binding reads the choice by itself
+            return None
         _load_native()
     fn, own = _NATIVE[op]
     registered = _KERNEL_REGISTRY["hip"]

@@ -438,3 +438,27 @@ def test_tangents_are_not_dropped():
         hb._no_grad_needed("op", x, None)
         with pytest.raises(NotImplementedError, match="tangents"):
             hb._no_grad_needed("op", w, None, dual)
+
+
+@pytest.mark.parametrize("env,loads", [("reference", False), ("cpu", False), ("hip", True), ("", True)])
+def test_another_backend_needs_no_built_module(monkeypatch, env, loads):
+    """A GPU tensor's call that goes to another backend does not ask for the native binding."""
+    class Gpu:
+        is_cuda, device = True, torch.device("cuda", 0)
+
+    def missing():
+        raise N.HipLibraryMissing("not built")
+
+    monkeypatch.setattr(D, "_NATIVE", {})
+    monkeypatch.setattr(D, "_load_native", missing)
+    monkeypatch.setattr(torch.version, "hip", "7.0")
+    monkeypatch.setenv("MABA_BACKEND", env)
+    for op in ("gated_ffn", "linear_epilogue", "checkpoint_pack", "checkpoint_unpack"):
+        if loads:
+            with pytest.raises(N.HipLibraryMissing):
+                D._bound(op, Gpu)
+        else:
+            assert D._bound(op, Gpu) is None
+    monkeypatch.setenv("MABA_BACKEND", "rocm")
+    with pytest.raises(ValueError, match="MABA_BACKEND"):
+        D._bound("gated_ffn", Gpu)
