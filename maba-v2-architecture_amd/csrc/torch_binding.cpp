@@ -279,7 +279,8 @@ struct LinearEpilogue : public torch::autograd::Function<LinearEpilogue> {
 // ---------------------------------------------------------------- the module's functions
 
 // Whether the dispatcher's backend for GPU tensors is this library: MABA_BACKEND as its get_backend reads it, without the
-// 1.3 us that takes in Python.  Any other value is declined, and the Python path routes or refuses it.
+// 1.3 us that takes in Python.  Any other value is declined, and the Python path routes or refuses it.  Called with the
+// interpreter's lock held: a write to os.environ in another thread holds it too.
 bool routed_here() {
   const char* e = std::getenv("MABA_BACKEND");
   if (!e || !*e) return true;
@@ -289,7 +290,7 @@ bool routed_here() {
 }
 
 Maybe gated_ffn(const Tensor& x, const Tensor& wg, const Tensor& wu, bool packed) {
-  if (!routed_here() || !alike(x, {&wg, &wu}) || x.dim() < 1 || wg.dim() != 2 || wg.size(0) == 0 || x.size(-1) == 0 || wg.size(1) != x.size(-1) ||
+  if (!alike(x, {&wg, &wu}) || x.dim() < 1 || wg.dim() != 2 || wg.size(0) == 0 || x.size(-1) == 0 || wg.size(1) != x.size(-1) ||
       wu.sizes() != wg.sizes())
     return std::nullopt;
   try {
@@ -303,7 +304,7 @@ Maybe gated_ffn(const Tensor& x, const Tensor& wg, const Tensor& wu, bool packed
 Maybe linear_epilogue(const Tensor& x, const Tensor& w, const Maybe& bias_, int64_t act, const Maybe& res_, const Maybe& gate_,
                       bool packed) {
   const Tensor bias = bias_.value_or(Tensor()), res = res_.value_or(Tensor()), gate = gate_.value_or(Tensor());
-  if (!routed_here() || !alike(x, {&w, &bias, &res, &gate}) || x.dim() < 1 || w.dim() != 2 || w.size(0) == 0 || x.size(-1) == 0 ||
+  if (!alike(x, {&w, &bias, &res, &gate}) || x.dim() < 1 || w.dim() != 2 || w.size(0) == 0 || x.size(-1) == 0 ||
       w.size(1) != x.size(-1))
     return std::nullopt;
   for (const Tensor* v : {&bias, &gate})
@@ -318,7 +319,7 @@ Maybe linear_epilogue(const Tensor& x, const Tensor& w, const Maybe& bias_, int6
 }
 
 std::optional<std::pair<Tensor, Tensor>> checkpoint_pack(const Tensor& x) {
-  if (!routed_here() || !plain(x) || x.dim() < 1 || x.size(-1) == 0) return std::nullopt;
+  if (!plain(x) || x.dim() < 1 || x.size(-1) == 0) return std::nullopt;
   try {
     return pack_call(x.requires_grad() ? x.detach() : x);
   } catch (const Declined&) {
@@ -327,7 +328,7 @@ std::optional<std::pair<Tensor, Tensor>> checkpoint_pack(const Tensor& x) {
 }
 
 Maybe checkpoint_unpack(const Tensor& codes, const Tensor& scales, at::ScalarType dtype) {
-  if (!routed_here() || !plain(codes) || !plain(scales) || codes.device() != scales.device() || codes.dim() < 1 || codes.size(-1) == 0 ||
+  if (!plain(codes) || !plain(scales) || codes.device() != scales.device() || codes.dim() < 1 || codes.size(-1) == 0 ||
       codes.scalar_type() != at::kFloat8_e4m3fn || scales.scalar_type() != at::kByte ||
       scales.sizes() != at::IntArrayRef(outer(codes, (codes.size(-1) + 31) / 32)))
     return std::nullopt;
@@ -342,13 +343,22 @@ Maybe checkpoint_unpack(const Tensor& codes, const Tensor& scales, at::ScalarTyp
   }
 }
 
+// `f` without the interpreter's lock, where the backend is this library.
+template <class R, class... A>
+auto unlocked(R (*f)(A...)) {
+  return [f](A... a) -> R {
+    if (!routed_here()) return std::nullopt;
+    py::gil_scoped_release free;
+    return f(a...);
+  };
+}
+
 }  // namespace
 
 PYBIND11_MODULE(maba_torch, m) {
-  typedef py::call_guard<py::gil_scoped_release> free;
   m.def("bind", &bind);
-  m.def("gated_ffn", &gated_ffn, free());
-  m.def("linear_epilogue", &linear_epilogue, free());
-  m.def("checkpoint_pack", &checkpoint_pack, free());
-  m.def("checkpoint_unpack", &checkpoint_unpack, free());
+  m.def("gated_ffn", unlocked(&gated_ffn));
+  m.def("linear_epilogue", unlocked(&linear_epilogue));
+  m.def("checkpoint_pack", unlocked(&checkpoint_pack));
+  m.def("checkpoint_unpack", unlocked(&checkpoint_unpack));
 }

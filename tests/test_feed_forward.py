@@ -462,3 +462,29 @@ def test_another_backend_needs_no_built_module(monkeypatch, env, loads):
     monkeypatch.setenv("MABA_BACKEND", "rocm")
     with pytest.raises(ValueError, match="MABA_BACKEND"):
         D._bound("gated_ffn", Gpu)
+
+
+def test_the_environment_may_change_while_the_binding_is_called(lib):
+    """The binding reads MABA_BACKEND under the interpreter's lock, as os.environ is written."""
+    import sys
+    import threading
+    m, x, stop = N.binding(), torch.randn(3, 8).bfloat16(), threading.Event()
+
+    def churn():
+        n = 0
+        while not stop.is_set():
+            os.environ[f"MABA_TEST_{n % 500}"] = "x" * (n % 97)
+            n += 1
+
+    t, interval = threading.Thread(target=churn), sys.getswitchinterval()
+    sys.setswitchinterval(1e-5)
+    t.start()
+    try:
+        for _ in range(5000):
+            assert m.checkpoint_pack(x) is None
+    finally:
+        sys.setswitchinterval(interval)
+        stop.set()
+        t.join()
+        for i in range(500):
+            os.environ.pop(f"MABA_TEST_{i}", None)
