@@ -424,33 +424,52 @@ def _ffn_kept(x, x_scales) -> None:
             f"Expected all tensors to be on the same device, but got {x.device} and {x_scales.device} for x_scales")
 
 
+_AUTOCAST_DTYPES = frozenset((torch.float32, torch.float16, torch.bfloat16))      # fp64 stays as it is, as in torch
+
+
+def _autocast_dtype(x) -> Optional[torch.dtype]:
+    """The type that autocast asks for on ``x``'s device, or None."""
+    kind = "cuda" if x.is_cuda else x.device.type
+    if kind not in ("cuda", "cpu") or not torch.is_autocast_enabled(kind):
+        return None
+    return torch.get_autocast_dtype(kind)
+
+
+def _autocast_to(dtype, *tensors):
+    return (t if t is None or t.dtype not in _AUTOCAST_DTYPES else t.to(dtype) for t in tensors)
+
+
 class _FFNOps:
     """The ops that the autograd functions call, through the backend of the tensors' device: a backward pass runs
-    where its forward did."""
+    where its forward did, and both in their tensors' types whatever autocast says."""
 
-    __slots__ = ("backend",)
+    __slots__ = ("backend", "kind")
 
     def __init__(self, device):
         self.backend = get_backend(device)
+        self.kind = device.type if device.type in ("cuda", "cpu") else None
+
+    def _run(self, op, **kwargs):
+        if self.kind is not None and torch.is_autocast_enabled(self.kind):
+            with torch.autocast(self.kind, enabled=False):
+                return _run(op, None, kwargs, self.backend)
+        return _run(op, None, kwargs, self.backend)
 
     def pack(self, x):
-        return _run("checkpoint_pack", None, dict(x=x), self.backend)
+        return self._run("checkpoint_pack", x=x)
 
     def gated_ffn(self, x, w_gate, w_up):
-        return _run("gated_ffn", None, dict(x=x, w_gate=w_gate, w_up=w_up), self.backend)
+        return self._run("gated_ffn", x=x, w_gate=w_gate, w_up=w_up)
 
     def gated_ffn_backward(self, dh, x, w_gate, w_up, x_scales, needs):
-        return _run("gated_ffn_backward", None,
-                    dict(dh=dh, x=x, w_gate=w_gate, w_up=w_up, x_scales=x_scales, needs=tuple(needs)), self.backend)
+        return self._run("gated_ffn_backward", dh=dh, x=x, w_gate=w_gate, w_up=w_up, x_scales=x_scales, needs=tuple(needs))
 
     def linear_epilogue(self, x, weight, bias, activation, residual, gate):
-        return _run("linear_epilogue", None, dict(x=x, weight=weight, bias=bias, activation=activation, residual=residual,
-                                                  gate=gate), self.backend)
+        return self._run("linear_epilogue", x=x, weight=weight, bias=bias, activation=activation, residual=residual, gate=gate)
 
     def linear_epilogue_backward(self, dy, x, weight, bias, activation, gate, x_scales, needs):
-        return _run("linear_epilogue_backward", None,
-                    dict(dy=dy, x=x, weight=weight, bias=bias, gate=gate, activation=activation, x_scales=x_scales,
-                         needs=tuple(needs)), self.backend)
+        return self._run("linear_epilogue_backward", dy=dy, x=x, weight=weight, bias=bias, gate=gate, activation=activation,
+                         x_scales=x_scales, needs=tuple(needs))
 
 
 # op -> the native binding's form of it, and the kernels of this package that it stands for
@@ -495,8 +514,12 @@ def dispatch_gated_ffn(x, w_gate, w_up, checkpoint: Optional[str] = None) -> tor
 
     x ``[..., C]``, w_gate and w_up ``[I, C]`` of one dtype and device; returns ``[..., I]``, computed in
     fp32 and rounded once.  Differentiable on every backend.  What the backward pass keeps is ``x``; with
-    ``checkpoint="e4m3"`` its packed form, half the bytes, and the gradients are those at the unpacked input."""
+    ``checkpoint="e4m3"`` its packed form, half the bytes, and the gradients are those at the unpacked input.  Under
+    autocast the tensors are cast to its type first, and gradients come back in each tensor's own."""
     _ffn_checkpoint(checkpoint)
+    dtype = _autocast_dtype(x)
+    if dtype is not None:
+        x, w_gate, w_up = _autocast_to(dtype, x, w_gate, w_up)
     native = _bound("gated_ffn", x)
     if native is not None:
         out = native(x, w_gate, w_up, checkpoint is not None)
@@ -526,15 +549,37 @@ def dispatch_gated_ffn_backward(dh, x, w_gate, w_up, x_scales=None, needs=(True,
         return _FFNOps(dh.device).gated_ffn_backward(dh, x, w_gate, w_up, x_scales, needs)
 
 
+def _gated_residual(y, gate, residual):
+    """``residual + gate * y`` (both optional) in the widest of their types."""
+    _ffn_shape("gate", gate, y.shape[-1:])
+    _ffn_shape("residual", residual, y.shape)
+    wide = y.dtype
+    for t in (gate, residual):
+        if t is not None:
+            wide = torch.promote_types(wide, t.dtype)
+    y = y.to(wide)
+    if residual is None:
+        return y * gate.to(wide)
+    return residual.to(wide) + y if gate is None else torch.addcmul(residual.to(wide), gate.to(wide), y)
+
+
 def dispatch_linear_epilogue(x, weight, bias=None, activation: str = "none", residual=None, gate=None,
                              checkpoint: Optional[str] = None) -> torch.Tensor:
     """``residual + gate * act(x W^T + bias)``: a linear layer with what follows it in its epilogue.
 
     x ``[..., K]``, weight ``[N, K]``, bias and gate ``[N]``, residual ``[..., N]`` of one dtype and device; bias,
     gate and residual are optional; activation none, relu, silu or gelu (with the error function).  Computed
-    in fp32 and rounded once.  Differentiable on every backend; ``checkpoint`` as for ``gated_ffn``."""
+    in fp32 and rounded once.  Differentiable on every backend; ``checkpoint`` as for ``gated_ffn``.  Under autocast x,
+    weight and bias are cast to its type; a gate or residual of another type is then applied by itself, in the widest of
+    them, and the result has that type (torch's addcmul does the same under autocast)."""
     _ffn_activation(activation)
     _ffn_checkpoint(checkpoint)
+    dtype = _autocast_dtype(x)
+    if dtype is not None:
+        x, weight, bias = _autocast_to(dtype, x, weight, bias)
+        apart = [t.dtype for t in (gate, residual) if t is not None and t.dtype != x.dtype]
+        if apart and _AUTOCAST_DTYPES.issuperset((*apart, x.dtype)):
+            return _gated_residual(linear_epilogue(x, weight, bias, activation, checkpoint=checkpoint), gate, residual)
     native = _bound("linear_epilogue", x)
     if native is not None:
         out = native(x, weight, bias, _c.ACTIVATIONS.index(activation), residual, gate, checkpoint is not None)

@@ -488,3 +488,87 @@ def test_the_environment_may_change_while_the_binding_is_called(lib):
         t.join()
         for i in range(500):
             os.environ.pop(f"MABA_TEST_{i}", None)
+
+
+# ----------------------------------------------------------------------------- autocast
+
+
+def _cast(dtype):
+    return lambda t: t if t is None else t.to(dtype)
+
+
+@pytest.mark.parametrize("xt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+def test_autocast_computes_in_its_type(xt, checkpoint):
+    """fp32 parameters under autocast: the products' type is autocast's whatever x is, gradients have each leaf's own type, and
+    both are those of a call on cast tensors."""
+    x, wg, wu = _rand(6, 40, dtype=xt), _rand(24, 40, dtype=torch.float32, seed=1), _rand(24, 40, dtype=torch.float32, seed=2)
+    w, b = _rand(10, 24, dtype=torch.float32, seed=3), _rand(10, dtype=torch.float32, seed=4)
+    to = _cast(torch.bfloat16)
+    with torch.autocast("cpu", torch.bfloat16):
+        h = D.gated_ffn(x, wg, wu, checkpoint=checkpoint)
+        y = D.linear_epilogue(h, w, b, "gelu", checkpoint=checkpoint)
+        torch.manual_seed(0)
+        dy = torch.randn(6, 10).bfloat16()
+        got = torch.autograd.grad(y, (x, wg, wu, w, b), dy, retain_graph=True)          # inside the region
+    outside = torch.autograd.grad(y, (x, wg, wu, w, b), dy)
+    want_y = D.linear_epilogue(D.gated_ffn(to(x), to(wg), to(wu), checkpoint=checkpoint), to(w), to(b), "gelu", checkpoint=checkpoint)
+    assert y.dtype == torch.bfloat16 and torch.equal(y, want_y)
+    want = torch.autograd.grad(want_y, (x, wg, wu, w, b), dy)
+    for a, o, c, leaf in zip(got, outside, want, (x, wg, wu, w, b)):
+        assert a.dtype == leaf.dtype and torch.equal(a, c) and torch.equal(o, c)
+
+
+@pytest.mark.parametrize("rt,gt", [(torch.float32, torch.float32), (torch.float32, None), (None, torch.float32),
+                                   (torch.bfloat16, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float32, torch.bfloat16)])
+def test_autocast_keeps_a_wide_residual(rt, gt):
+    """The gated residual of a type wider than autocast's stays in it, as torch's own addcmul does under autocast."""
+    x, w = _rand(6, 40, dtype=torch.float32), _rand(10, 40, dtype=torch.float32, seed=1)
+    res = None if rt is None else _rand(6, 10, dtype=rt, seed=2)
+    gate = None if gt is None else _rand(10, dtype=gt, seed=3)
+    live = [t for t in (x, w, res, gate) if t is not None]
+    with torch.autocast("cpu", torch.bfloat16):
+        got = D.linear_epilogue(x, w, None, "silu", res, gate)
+    to = _cast(torch.bfloat16)
+    wide = [t.dtype for t in (res, gate) if t is not None]
+    if all(t == torch.bfloat16 for t in wide):
+        want = D.linear_epilogue(to(x), to(w), None, "silu", res, gate)
+    else:
+        y = D.linear_epilogue(to(x), to(w), None, "silu").float()
+        y = y if gate is None else y * gate
+        want = y if res is None else torch.addcmul(res.float(), gate.float(), D.linear_epilogue(to(x), to(w), None, "silu").float()) \
+            if gate is not None else res + y
+    assert got.dtype == want.dtype and torch.equal(got, want)
+    dy = torch.ones_like(got)
+    for a, b in zip(torch.autograd.grad(got, live, dy), torch.autograd.grad(want, live, dy)):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("xt", [torch.float32, torch.bfloat16])
+def test_autocast_of_the_model_feed_forward(xt):
+    """What fused=True returns under autocast has the type of what fused=False does, and a block keeps its residual's."""
+    torch.manual_seed(0)
+    plain, fused = SwiGLUFFN(64, 96), SwiGLUFFN(64, 96, fused=True)
+    fused.load_state_dict(plain.state_dict())
+    x = torch.randn(3, 64).to(xt)
+    with torch.autocast("cpu", torch.bfloat16):
+        ys = [plain(x), fused(x)]
+    assert ys[0].dtype == ys[1].dtype == torch.bfloat16
+    for m, y in zip((plain, fused), ys):
+        y.float().square().sum().backward()
+    assert all(p.grad.dtype == torch.float32 for p in fused.parameters())
+    cfg = dict(dim=64, n_heads=1, intermediate_size=40, n_layers=1)
+    blocks = [MabaBlock(MabaConfig(**cfg, fused_ffn=f), 0) for f in (False, True)]
+    res, mo = torch.randn(3, 5, 64), torch.randn(3, 5, 64)
+    with torch.autocast("cpu", torch.bfloat16):
+        outs = [b._residual(res, mo) for b in blocks]
+    assert outs[0].dtype == outs[1].dtype == torch.float32
+
+
+def test_autocast_leaves_64_bits_alone():
+    x, w = _rand(6, 40), _rand(10, 40, seed=1)
+    with torch.autocast("cpu", torch.bfloat16):
+        y = D.linear_epilogue(x, w)
+        with pytest.raises(TypeError, match="dtypes must match"):
+            D.linear_epilogue(x, w.float())
+    assert y.dtype == F64 and torch.equal(y, D.linear_epilogue(x, w))

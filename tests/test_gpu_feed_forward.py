@@ -795,3 +795,46 @@ def test_tangents_take_the_reference_path(monkeypatch):
             want = forward_ad.unpack_dual(call(ref, dual, dh))
         assert got.tangent is not None
         assert torch.equal(got.tangent, want.tangent) and torch.equal(got.primal, want.primal)
+
+
+@pytest.mark.parametrize("ckpt", [None, "e4m3"])
+@pytest.mark.parametrize("at", [BF, HF])
+@pytest.mark.parametrize("xt", [torch.float32, BF, HF])
+def test_fp32_parameters_under_autocast_reach_the_kernels(xt, at, ckpt):
+    """The usual mixed-precision recipe: the values and gradients of a call on cast tensors, the gradients in each leaf's
+    type.  A fallback would raise (``strict``)."""
+    r = _gen(97)
+    x, res = r(70, 64).to(xt).requires_grad_(), r(70, 40).requires_grad_()
+    wg, wu, w, b, g = (r(*s).requires_grad_() for s in ((72, 64), (72, 64), (40, 72), (40,), (40,)))
+    dy = r(70, 40)
+    leaves = (x, wg, wu, w, b, res, g)
+
+    def cast(*ts):
+        return (t.to(at) for t in ts)
+
+    with torch.autocast("cuda", at):
+        h = D.gated_ffn(x, wg, wu, checkpoint=ckpt)
+        y = D.linear_epilogue(h, w, b, "silu", res, g, checkpoint=ckpt)
+        narrow = D.linear_epilogue(h, w, b, "silu", *cast(res, g), checkpoint=ckpt)
+    assert h.dtype == narrow.dtype == at and y.dtype == torch.float32
+    h2 = D.gated_ffn(*cast(x, wg, wu), checkpoint=ckpt)
+    want = torch.addcmul(res, g, D.linear_epilogue(h2, *cast(w, b), "silu", checkpoint=ckpt).float())
+    want_narrow = D.linear_epilogue(h2, *cast(w, b), "silu", *cast(res, g), checkpoint=ckpt)
+    assert torch.equal(y, want) and torch.equal(narrow, want_narrow)
+    for a, c, d in ((y, want, dy), (narrow, want_narrow, dy.to(at))):
+        for got, ref, leaf in zip(torch.autograd.grad(a, leaves, d, retain_graph=True),
+                                  torch.autograd.grad(c, leaves, d, retain_graph=True), leaves):
+            assert got.dtype == leaf.dtype and torch.equal(got, ref)
+
+
+def test_the_model_feed_forward_under_autocast():
+    from maba_sparse.model import SwiGLUFFN
+    torch.manual_seed(4)
+    plain, fused = SwiGLUFFN(64, 96).to(DEV), SwiGLUFFN(64, 96, fused=True).to(DEV)
+    fused.load_state_dict(plain.state_dict())
+    for x in (torch.randn(90, 64, device=DEV), torch.randn(90, 64, device=DEV).to(BF)):
+        with torch.autocast("cuda", BF):
+            a, b = plain(x), fused(x)
+            b.float().square().mean().backward()                       # inside the region
+        assert a.dtype == b.dtype == BF
+        assert all(p.grad.dtype == torch.float32 and bool(torch.isfinite(p.grad).all()) for p in fused.parameters())
