@@ -8,6 +8,7 @@
 // derivatives, sizes that the library refuses) is declined: the function returns None and the caller takes the Python path, which checks, raises or falls
 // back.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <cstdlib>
@@ -343,6 +344,22 @@ Maybe checkpoint_unpack(const Tensor& codes, const Tensor& scales, at::ScalarTyp
   }
 }
 
+// Whether a leaf that `out` was made from, by itself or cast to another type, keeps its autograd node from another stream
+// than the current one: the stream that was current when the eager graph it belongs to was made, by whatever op.
+bool leaf_of_another_stream(const Tensor& out) {
+  const auto fn = out.grad_fn();
+  if (!fn) return false;
+  const auto now = c10::hip::getCurrentHIPStream(out.device().index());
+  for (const auto& edge : fn->next_edges()) {
+    torch::autograd::Node* node = edge.function.get();
+    while (node && node->num_outputs() > 0 && node->name() == "ToCopyBackward0") node = node->next_edge(0).function.get();
+    if (!dynamic_cast<torch::autograd::AccumulateGrad*>(node)) continue;
+    const auto made = node->stream();
+    if (made && (made->id() != now.id() || made->device_index() != now.device_index())) return true;
+  }
+  return false;
+}
+
 // `f` without the interpreter's lock, where the backend is this library.
 template <class R, class... A>
 auto unlocked(R (*f)(A...)) {
@@ -357,6 +374,7 @@ auto unlocked(R (*f)(A...)) {
 
 PYBIND11_MODULE(maba_torch, m) {
   m.def("bind", &bind);
+  m.def("leaf_of_another_stream", &leaf_of_another_stream);
   m.def("gated_ffn", unlocked(&gated_ffn));
   m.def("linear_epilogue", unlocked(&linear_epilogue));
   m.def("checkpoint_pack", unlocked(&checkpoint_pack));

@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
-from maba_sparse._native import stream_ptr
+from maba_sparse import _native
 
 
 def _once(backward):
@@ -75,19 +75,15 @@ class LinearEpilogue(torch.autograd.Function):
 
 def guard_capture(out: torch.Tensor) -> torch.Tensor:
     """Refuses to record a backward pass whose gradients would reach a leaf through an autograd node
-    of another stream.  Such a node lives as long as any eager graph of that leaf does; the engine
-    would then make the node's stream wait inside the capture, which ends the process.  The node keeps
-    the stream that it was first seen on, so a capture beside a live eager graph of these operators
-    raises here instead."""
-    if out.is_cuda and out.grad_fn is not None:
-        stream = stream_ptr(out.device)
-        capturing = torch.cuda.is_current_stream_capturing()
-        for node, _ in out.grad_fn.next_functions:
-            if node is None or not hasattr(node, "variable"):
-                continue
-            first = node.metadata.setdefault("maba_stream", stream)
-            if capturing and first != stream:
-                raise RuntimeError(
-                    "a leaf of this captured call still belongs to an eager autograd graph on another stream: drop "
-                    "that graph's outputs first, or capture the *_backward ops, which need no autograd")
+    of another stream.  Such a node lives as long as any eager graph of that leaf does, whichever op made
+    it; the engine would then make the node's stream wait inside the capture, which ends the process."""
+    if out.is_cuda and out.grad_fn is not None and torch.cuda.is_current_stream_capturing():
+        try:
+            binding = _native.binding()
+        except _native.HipLibraryMissing:                  # another backend's call, where nothing is built
+            return out
+        if binding.leaf_of_another_stream(out):
+            raise RuntimeError(
+                "a leaf of this captured call still belongs to an eager autograd graph on another stream: drop "
+                "that graph's outputs first, or capture the *_backward ops, which need no autograd")
     return out

@@ -838,3 +838,35 @@ def test_the_model_feed_forward_under_autocast():
             b.float().square().mean().backward()                       # inside the region
         assert a.dtype == b.dtype == BF
         assert all(p.grad.dtype == torch.float32 and bool(torch.isfinite(p.grad).all()) for p in fused.parameters())
+
+
+@pytest.mark.parametrize("kind", ["another op", "under autocast", "python path"])
+def test_capture_beside_an_eager_graph_of_any_op_is_refused(monkeypatch, kind):
+    """The leaf's node is known by the stream that it was made on, whichever op made it and whatever cast lies between.
+    Only forwards are recorded here; once the eager graph is gone the same call is taken."""
+    x, wg, wu, dh = _gated(70, 64, 40, BF, seed=98)
+    if kind == "under autocast":
+        x, wg = x.float(), wg.float()
+    w = wg.requires_grad_()
+    if kind == "python path":
+        hip = D._KERNEL_REGISTRY["hip"]
+        monkeypatch.setitem(hip, "gated_ffn", lambda _f=hip["gated_ffn"], **kw: _f(**kw))
+
+    def call():
+        with torch.autocast("cuda", BF, enabled=kind == "under autocast"):
+            return D.gated_ffn(x, w, wu)
+
+    call()
+    eager = torch.nn.functional.linear(x, w)                 # another op's graph, on the current stream
+    with pytest.raises(RuntimeError, match="eager autograd graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            call()
+    torch.cuda.synchronize()
+    del eager
+    gc.collect()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, call())
