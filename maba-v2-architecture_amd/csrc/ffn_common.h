@@ -12,12 +12,13 @@ namespace ffn {
 // ---------------------------------------------------------------- copies and reductions (ffn_common.hip)
 
 // dst [rows, chunks * 8] (contiguous) = src [rows, cols] with zeros behind each row, of 16-bit elements at any
-// alignment, scaled by gate[row] where there is one; with scales: src holds the e4m3 codes of a packed activation,
+// alignment, times gate[row] and 2^*exponent where there are any; with scales: src holds the e4m3 codes of a packed activation,
 // dst its values.
 struct CopyJob {
   const void* src; int64_t ld;
   const uint8_t* scales; int64_t scale_ld;
   const uint16_t* gate;
+  const int* exponent;
   int64_t rows;
   int cols, chunks;
   uint16_t* dst;
@@ -27,21 +28,23 @@ constexpr int MAX_COPIES = 3;
 struct Copies {
   CopyJob job[MAX_COPIES];
   int count = 0;
-  void add(const maba_tensor* src, const maba_tensor* scales, uint16_t* dst, const maba_tensor* gate = nullptr) {
+  void add(const maba_tensor* src, const maba_tensor* scales, uint16_t* dst, const maba_tensor* gate = nullptr,
+           const int* exponent = nullptr) {
     job[count++] = {src->data, src->stride[0], scales ? (const uint8_t*)scales->data : nullptr, scales ? scales->stride[0] : 0,
-                    gate ? (const uint16_t*)gate->data : nullptr, src->shape[0], (int)src->shape[1],
+                    gate ? (const uint16_t*)gate->data : nullptr, exponent, src->shape[0], (int)src->shape[1],
                     (int)((src->shape[1] + 7) / 8), dst};
   }
   int launch(int dtype, hipStream_t s) const;
 };
 
-// out = the sum of `splits` fp32 partials [splits][M][N] in split order, rounded to 16 bits; row m goes to
-// row m of out[0], or from `second` on to row m - second of out[1]; only `rows` rows of each are written, and
-// nothing to a null one.
+// out = the sum of `splits` fp32 partials [splits][M][N] in split order, times 2^-*exponent where there is one, rounded
+// to 16 bits; row m goes to row m of out[0], or from `second` on to row m - second of out[1]; only `rows` rows of each
+// are written, and nothing to a null one.
 struct ReduceArgs {
   const float* p;
   int splits, M, N, second, rows, ncols;
   Rows out[2];
+  const int* exponent;
 };
 int reduce_splits(const ReduceArgs& a, int dtype, hipStream_t s);
 
@@ -63,6 +66,36 @@ int reduce_gated(const GatedReduceArgs& a, int rows, int dtype, hipStream_t s);
 
 // p[r][0][n] = the sum of rows [128 r, 128 r + 128) of src [M, N] (16-bit), [ceil(M / 128)][2][N].
 int column_partials(const maba_tensor* src, float* p, hipStream_t s);
+
+// What a backward pass makes as a 16-bit operand of its next products ([dg | du], dz, gate * W) is held in fp16 as its
+// value times 2^e, and the products' results are multiplied by 2^-e: fp16's own range loses small gradients and gates
+// below its smallest step and turns large ones into infinities, which fp32 does not.  e is the largest with
+// bound * 2^e <= 2^15 for a bound of the operand's magnitudes made before it, as a product of up to three factors: each
+// is the largest element of some tensors, or the largest norm of their rows.  So every operand is below 2^16, and
+// one of 2^-28 of the bound still has all of fp16's bits.  bf16 has fp32's range and takes none of this.
+//
+// (Elements that are not finite do not count: their rows' results are not finite either.)
+constexpr int MAX_FACTORS = 3, MAX_MAGNITUDES = 4, MAGNITUDE_GROUPS = 2048;
+struct Magnitude {
+  const uint16_t* p; int64_t ld, cols, segments;      // of a row, SEGMENT elements each
+  int64_t units;                                       // segments of all rows
+  int factor, norm;
+};
+struct Magnitudes {
+  static constexpr int SEGMENT = 1024;
+  Magnitude job[MAX_MAGNITUDES];
+  int count = 0;
+  void add(int factor, const void* p, int64_t ld, int64_t rows, int64_t cols, bool norm) {
+    if (!norm && ld == cols) {                         // elements one after another
+      cols *= rows;
+      rows = 1;
+    }
+    const int64_t segments = ceil_div(cols, SEGMENT);
+    job[count++] = {(const uint16_t*)p, ld, cols, segments, rows * segments, factor, norm};
+  }
+  // *exponent = e; partial: MAX_FACTORS * MAGNITUDE_GROUPS floats of workspace.
+  int launch(float slope, float* partial, int* exponent, hipStream_t s) const;
+};
 
 // ---------------------------------------------------------------- launches
 
@@ -139,23 +172,24 @@ int gemm(GemmArgs g, const typename Epi::Args& e, int64_t M, int64_t N, const Ge
 struct Outputs {
   Rows out[2];
   int second, rows, N;
+  const int* exponent;       // the operands' power of two, taken out of the result
 };
 template <class T, int AMODE, int BMODE>
 int product_to(const GemmArgs& g, const Outputs& o, int64_t M, int64_t Np, const GemmPlan& p, float* part, hipStream_t s,
                const char* who) {
   if (p.splits == 1) {
-    const EpiStore::Args e = {{o.out[0], o.out[1]}, o.second, o.rows, o.N};
+    const EpiStore::Args e = {{o.out[0], o.out[1]}, o.second, o.rows, o.N, o.exponent};
     return gemm<T, AMODE, BMODE, EpiStore>(g, e, M, Np, p, s, who);
   }
   const EpiPartial::Args e = {part, (int)M, (int)Np};
   if (int rc = gemm<T, AMODE, BMODE, EpiPartial>(g, e, M, Np, p, s, who)) return rc;
-  const ReduceArgs r = {part, p.splits, (int)M, (int)Np, o.second, o.rows, o.N, {o.out[0], o.out[1]}};
+  const ReduceArgs r = {part, p.splits, (int)M, (int)Np, o.second, o.rows, o.N, {o.out[0], o.out[1]}, o.exponent};
   return reduce_splits(r, T::CODE, s);
 }
 // Zeros in the outputs, for a sum over no rows.
 template <class T>
 int zeros_to(const Outputs& o, int64_t M, int64_t Np, hipStream_t s) {
-  const ReduceArgs r = {nullptr, 0, (int)M, (int)Np, o.second, o.rows, o.N, {o.out[0], o.out[1]}};
+  const ReduceArgs r = {nullptr, 0, (int)M, (int)Np, o.second, o.rows, o.N, {o.out[0], o.out[1]}, nullptr};
   return reduce_splits(r, T::CODE, s);
 }
 

@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(CopyArgs a) {
 #pragma unroll
         for (int j = 0; j < 7; ++j) v[j >> 1] |= (j < n ? (uint32_t)p[j] : 0u) << (16 * (j & 1));
       if (c.gate) {
-        const float g = T::up(c.gate[r]);
+        const float g = T::up(c.gate[r]) * power_of<T>(c.exponent, 1);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = T::down(T::up(v[j] & 0xffffu) * g) | (T::down(T::up(v[j] >> 16) * g) << 16);
       }
@@ -151,13 +151,14 @@ template <class T>
 __global__ __launch_bounds__(256) void reduce_splits_kernel(ReduceArgs a) {
   const int quads = a.N / 4;
   const int64_t total = (int64_t)a.M * quads, plane = (int64_t)a.M * a.N;
+  const float scale = power_of<T>(a.exponent, -1);
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int m = (int)(i / quads), n = (int)(i % quads) * 4;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
     for (int s = 0; s < a.splits; ++s) v += *(const f32x4*)(a.p + s * plane + (int64_t)m * a.N + n);
     const int t = m >= a.second, r = t ? m - a.second : m;
-    if (r < a.rows && a.out[t].p) store4<T>(a.out[t], r, n, a.ncols, v);
+    if (r < a.rows && a.out[t].p) store4<T>(a.out[t], r, n, a.ncols, v * scale);
   }
 }
 
@@ -167,6 +168,113 @@ int reduce_splits(const ReduceArgs& a, int dtype, hipStream_t s) {
   auto k = dtype == MABA_BF16 ? reduce_splits_kernel<Bf16> : reduce_splits_kernel<Fp16>;
   hipLaunchKernelGGL(k, grid, dim3(256), 0, s, a);
   return check_launch("reduce_splits");
+}
+
+// Sixteen lanes take a segment of a row, 64 elements a lane loaded together, a wave four of one tensor.
+// partial[f][b]: workgroup b's largest of factor f.  A norm is bounded by its largest segment's times the root of their
+// number.  Bound by HBM: 34 MB (dh of 8,191 x 1,248, x of 8,191 x 640 and two weights) take 7.7 us, and 16 with a wave per
+// row, where a wave waits for several rows one by one.
+struct MagnitudeArgs {
+  Magnitude job[MAX_MAGNITUDES];
+  int64_t end[MAX_MAGNITUDES];      // fours of segments up to and with each job's
+  float* partial;
+};
+// The finite ones of two fp16 numbers' magnitudes, zero for the others.
+__device__ __forceinline__ uint32_t finite2(uint32_t v) {
+  typedef __attribute__((ext_vector_type(2))) int16_t i16x2;
+  const uint32_t m = v & 0x7fff7fffu;
+  const i16x2 bad = __builtin_bit_cast(i16x2, m + 0x04000400u) >> 15;       // from 0x7c00 on
+  return m & ~__builtin_bit_cast(uint32_t, bad);
+}
+__global__ __launch_bounds__(256) void magnitudes_kernel(MagnitudeArgs a) {
+  constexpr int SEG = Magnitudes::SEGMENT, LOADS = SEG / 128;
+  typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
+  __shared__ uint32_t part[MAX_FACTORS];             // bits: they order as the magnitudes do
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+  if (threadIdx.x < MAX_FACTORS) part[threadIdx.x] = 0;
+  __syncthreads();
+  for (int64_t u = blockIdx.x * (int64_t)4 + wave; u < a.end[MAX_MAGNITUDES - 1]; u += (int64_t)gridDim.x * 4) {
+    int t = 0;
+#pragma unroll
+    for (int i = 0; i < MAX_MAGNITUDES - 1; ++i) t += u >= a.end[i];
+    const Magnitude& j = a.job[t];
+    const int64_t at = (u - (t ? a.end[t - 1] : 0)) * 4 + (lane >> 4);
+    const bool in = at < j.units;
+    int64_t row = 0, seg = 0;                        // both 0 past the end, where nothing is read
+    if (j.segments == 1) row = at;
+    else if (j.segments == j.units) seg = at;
+    else row = at / j.segments, seg = at - row * j.segments;
+    const Rows r = {(uint16_t*)j.p + (in ? row * j.ld + seg * SEG : 0), 0};
+    const int n = in ? (int)min(j.cols - seg * SEG, (int64_t)SEG) : 0;
+    u32x4 v[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) v[i] = load8(r, 0, 8 * (lane & 15) + 128 * i, n ? 1 : 0, n);
+    float x = 0.f;
+    if (j.norm) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const float lo = Fp16::up(v[i][h] & 0xffffu), hi = Fp16::up(v[i][h] >> 16);
+          x = fmaf(hi, hi, fmaf(lo, lo, x));
+        }
+      x = x < 3e38f ? x : 0.f;                       // not finite: nor are the products of this row
+      x = sqrtf(sum16(x) * (float)j.segments);
+    } else {
+      u16x2 m = {0, 0};
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+        for (int h = 0; h < 4; ++h) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, finite2(v[i][h])));
+      x = Fp16::up(max((uint32_t)m[0], (uint32_t)m[1]));
+      x = max16(x);
+    }
+    if ((lane & 15) == 0) atomicMax(&part[j.factor], __float_as_uint(x));
+  }
+  __syncthreads();
+  if (threadIdx.x < MAX_FACTORS) a.partial[threadIdx.x * MAGNITUDE_GROUPS + blockIdx.x] = __uint_as_float(part[threadIdx.x]);
+}
+
+// 2 us, most of it the launch.  bound = 1.25 slope * the factors' product (the quarter covers the rounding of the sums that the operand is made of and
+// of these); a wave reads a factor's partials.
+__global__ __launch_bounds__(64 * MAX_FACTORS) void exponent_kernel(const float* partial, int groups, int factors, float slope, int* exponent) {
+  __shared__ float part[MAX_FACTORS];
+  const int f = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  float x = 0.f;
+#pragma unroll 8
+  for (int i = lane; i < groups; i += 64) x = fmaxf(x, partial[f * MAGNITUDE_GROUPS + i]);
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) x = fmaxf(x, __shfl_xor(x, s));
+  if (lane == 0) part[f] = f < factors ? x : 1.f;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float bound = 1.25f * slope;
+#pragma unroll
+    for (int i = 0; i < MAX_FACTORS; ++i) bound *= part[i];
+    // bound < 2^(E + 1)
+    const int e = 14 - ((int)(__float_as_uint(bound) >> 23) - 127);
+    *exponent = bound > 0.f ? min(e, 100) : 0;
+  }
+}
+
+int Magnitudes::launch(float slope, float* partial, int* exponent, hipStream_t s) const {
+  MagnitudeArgs a = {};
+  int64_t total = 0;
+  int factors = 0;
+  for (int i = 0; i < MAX_MAGNITUDES; ++i) {
+    if (i < count) {
+      a.job[i] = job[i];
+      total += ceil_div(job[i].units, 4);
+      factors = std::max(factors, job[i].factor + 1);
+    }
+    a.end[i] = total;
+  }
+  a.partial = partial;
+  const int groups = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(total, 4), MAGNITUDE_GROUPS));
+  hipLaunchKernelGGL(magnitudes_kernel, dim3(groups), dim3(256), 0, s, a);
+  if (int rc = check_launch("magnitudes")) return rc;
+  hipLaunchKernelGGL(exponent_kernel, dim3(1), dim3(64 * MAX_FACTORS), 0, s, partial, groups, factors, slope, exponent);
+  return check_launch("exponent");
 }
 
 // A workgroup a row of G = sum of the partials: dw = gate * G, and dgate = <w, G> (+ bias * colsum, added by the caller's

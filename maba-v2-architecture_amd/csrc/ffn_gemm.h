@@ -32,6 +32,7 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 // The two 16-bit types: products, and conversions that round to nearest even.
 struct Bf16 {
   static constexpr int CODE = MABA_BF16;
+  static constexpr bool SCALED = false;             // operands made on the way are held as they are
   static constexpr float MOST = 3.38953139e38f;     // the largest finite value
   static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -41,6 +42,7 @@ struct Bf16 {
 };
 struct Fp16 {
   static constexpr int CODE = MABA_F16;
+  static constexpr bool SCALED = true;              // times a power of two (Magnitudes)
   static constexpr float MOST = 65504.f;
   static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -423,14 +425,22 @@ __global__ __launch_bounds__(64 * WM * WN * KG, KG == 2 || BM * BN / (WM * WN) <
   }
 }
 
-// Epilogue: C as it is, rounded once to 16 bits; from row `second` on it goes to the second tensor's rows (`second`
+// 2^e of a scaled operand's exponent, and 2^-e; 1 without one.
+template <class T>
+__device__ __forceinline__ float power_of(const int* exponent, int sign) {
+  if constexpr (T::SCALED) return exponent ? __builtin_amdgcn_ldexpf(1.f, sign * *exponent) : 1.f;
+  else return 1.f;
+}
+
+// Epilogue: C, times 2^-*exponent where there is one, rounded once to 16 bits; from row `second` on it goes to the second tensor's rows (`second`
 // is a multiple of 16).  M: rows of each.
 struct EpiStore {
   static constexpr bool LONG = false, GROUPS = true;
-  struct Args { Rows c[2]; int second, M, N; };
+  struct Args { Rows c[2]; int second, M, N; const int* exponent; };
   template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
   static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
                                              int q, int wave, uint16_t* lds) {
+    const float scale = power_of<T>(e.exponent, -1);
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const int at = m0 + 16 * i >= e.second, m = m0 + 16 * i - (at ? e.second : 0) + c;
@@ -438,7 +448,7 @@ struct EpiStore {
       if (!r.p) continue;
 #pragma unroll
       for (int j = 0; j < NI; j += 2)
-        store8(r, m, n0 + 16 * j + 8 * q, e.M, e.N, eight_of({down4<T>(acc[i][j]), down4<T>(acc[i][j + 1])}));
+        store8(r, m, n0 + 16 * j + 8 * q, e.M, e.N, eight_of({down4<T>(acc[i][j] * scale), down4<T>(acc[i][j + 1] * scale)}));
     }
   }
 };
@@ -471,6 +481,18 @@ __device__ __forceinline__ float scaled(float code, int e, float most) {
 }
 
 __device__ __forceinline__ float sigmoid(float x) { return fast_rcp(1.f + fast_exp(-x)); }
+
+// Over the 16 lanes of a quarter of the wave, in each of them: neighbours, pairs, quads and eights.
+template <class F>
+__device__ __forceinline__ float over16(float v, F f) {
+  v = f(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xb1, 0xf, 0xf, true)));     // lanes 1 0 3 2
+  v = f(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4e, 0xf, 0xf, true)));     // lanes 2 3 0 1
+  v = f(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xf, 0xf, true)));    // a half mirrored
+  v = f(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xf, 0xf, true)));    // mirrored
+  return v;
+}
+__device__ __forceinline__ float sum16(float v) { return over16(v, [](float a, float b) { return a + b; }); }
+__device__ __forceinline__ float max16(float v) { return over16(v, [](float a, float b) { return fmaxf(a, b); }); }
 
 // ---------------------------------------------------------------- host side
 

@@ -10,7 +10,8 @@
 // Backward: the forward keeps nothing but x.  The first launch makes g and u again (4 M C I operations, which
 // cost about what writing and reading the two would at C <= 1000 or so) and its epilogue turns them with dh
 // into [dg | du], rounded once to 16 bits as an operand of the next products: kept in fp32 to here, so the
-// gradients carry that one rounding and their own.  The second launch is dx over k = [dg | du]'s columns with
+// gradients carry that one rounding and their own.  In fp16 [dg | du] is held times a power of two, from the bounds
+// |dg|, |du| <= 1.1 |dh| max(|g|, |u|) and |g|, |u| <= |x| |w|, norms of rows (two launches; Magnitudes).  The second launch is dx over k = [dg | du]'s columns with
 // both weights read along their columns, the third [dWg; dWu] = [dg | du]^T x, summed over token ranges into
 // fp32 partials that a last launch adds in order (the same bits every time).
 #include <algorithm>
@@ -60,7 +61,7 @@ struct EpiGated {
 // d [M, 2 Iw], Iw = I rounded up to 16: dg at column 0, du at column Iw, zeros behind each.
 struct EpiGatedBack {
   static constexpr bool LONG = false, GROUPS = false;
-  struct Args { Rows dh, d; int M, I, Iw; };
+  struct Args { Rows dh, d; int M, I, Iw; const int* exponent; };
   static __device__ __forceinline__ void grads(f32x4 g, f32x4 u, f32x4 dh, f32x4& dg, f32x4& du) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -72,6 +73,7 @@ struct EpiGatedBack {
   template <class T, int BM, int BN, int WM, int WN, int MI, int NI>
   static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
                                              int q, int wave, uint16_t* lds) {
+    const float scale = power_of<T>(e.exponent, 1);
     if constexpr (NI % 4 == 0) {
       u32x4 dh[MI][NI / 4];      // all of dh first: the loads are in flight together
 #pragma unroll
@@ -86,8 +88,8 @@ struct EpiGatedBack {
           const int n = n0 / 2 + 32 * j + 8 * q;
           const Quads d = quads_of(dh[i][j]);
           f32x4 dg[2], du[2];
-          grads(acc[i][4 * j], acc[i][4 * j + 1], up4<T>(d.a), dg[0], du[0]);
-          grads(acc[i][4 * j + 2], acc[i][4 * j + 3], up4<T>(d.b), dg[1], du[1]);
+          grads(acc[i][4 * j], acc[i][4 * j + 1], up4<T>(d.a) * scale, dg[0], du[0]);
+          grads(acc[i][4 * j + 2], acc[i][4 * j + 3], up4<T>(d.b) * scale, dg[1], du[1]);
           store8(e.d, m, n, e.M, e.Iw, eight_of({down4<T>(dg[0]), down4<T>(dg[1])}));
           // columns behind Iw would be du's neighbours: none is stored there
           const u32x4 u = eight_of({down4<T>(du[0]), down4<T>(du[1])});
@@ -103,7 +105,7 @@ struct EpiGatedBack {
           const int n = n0 / 2 + 8 * j + 4 * q;
           if (m >= e.M || n >= e.Iw) continue;
           f32x4 dg, du;
-          grads(acc[i][j], acc[i][j + 1], up4<T>(load4(e.dh, m, n, e.I)), dg, du);
+          grads(acc[i][j], acc[i][j + 1], up4<T>(load4(e.dh, m, n, e.I)) * scale, dg, du);
           store4<T>(e.d, m, n, e.Iw, dg);
           store4<T>(e.d, m, e.Iw + n, 2 * e.Iw, du);
         }
@@ -137,6 +139,8 @@ struct GatedPlan {
   bool copy_x, copy_w[2];
   uint16_t *x, *w[2], *d;
   float* part;             // fp32 partials, of dx and then of the weights
+  float* magnitudes;       // and the power of two of d, in fp16
+  int* exponent;
   GemmPlan gu, dx, dw;     // the products with both weights, for dx and for the weights' gradients
   size_t bytes;
 };
@@ -172,6 +176,10 @@ static GatedPlan gated_plan(const maba_tensor* x, const maba_tensor* scales, con
       part = std::max(part, (int64_t)p.dw.splits * 2 * p.Iw * p.Cp);
     }
     p.part = c.take<float>(part);
+    if (wg->dtype == MABA_F16) {
+      p.magnitudes = c.take<float>(MAX_FACTORS * MAGNITUDE_GROUPS);
+      p.exponent = c.take<int>(1);
+    }
   }
   p.gu = gemm_plan(p.M, 2 * p.Iw, gemm_stages(p.Cp, 1), PLAN_PAIRS | (back || few ? 0 : PLAN_SPLIT));
   if (p.gu.splits > 1) p.part = c.take<float>((int64_t)p.gu.splits * p.M * 2 * p.Iw);
@@ -225,12 +233,19 @@ static int gated_backward(GatedPlan& p, const maba_tensor* dh, const maba_tensor
   if (int rc = gated_operands(p, x, scales, wg, wu, s, ox, ow)) return rc;
   const Operand d = rows_operand(p.d, 2 * p.Iw, p.M);
   if (p.M > 0) {
+    if (T::SCALED) {
+      Magnitudes m;
+      m.add(0, dh->data, dh->stride[0], p.M, p.I, false);
+      m.add(1, ox.p[0], ox.ld[0], p.M, p.C, true);
+      for (int i = 0; i < 2; ++i) m.add(2, ow.p[i], ow.ld[i], p.I, p.C, true);
+      if (int rc = m.launch(1.1f, p.magnitudes, p.exponent, s)) return rc;
+    }
     GemmArgs g = {};
     g.a = ox;
     g.b = ow;
     g.K = p.Cp;
     const Rows rd = {p.d, 2 * p.Iw};
-    const EpiGatedBack::Args e = {rows_of(dh), rd, (int)p.M, (int)p.I, (int)p.Iw};
+    const EpiGatedBack::Args e = {rows_of(dh), rd, (int)p.M, (int)p.I, (int)p.Iw, p.exponent};
     if (int rc = gemm<T, K_ROWS, K_ROWS_PAIR, EpiGatedBack>(g, e, p.M, 2 * p.Iw, p.gu, s, who)) return rc;
   }
   if (dx && p.M > 0) {
@@ -239,11 +254,11 @@ static int gated_backward(GatedPlan& p, const maba_tensor* dh, const maba_tensor
     g.b = cols_operand(ow, p.Cp);
     g.K = p.Iw;
     g.segments = 2;
-    const Outputs o = {{rows_of(dx), rows_of(nullptr)}, INT32_MAX, (int)p.M, (int)p.C};
+    const Outputs o = {{rows_of(dx), rows_of(nullptr)}, INT32_MAX, (int)p.M, (int)p.C, p.exponent};
     if (int rc = product_to<T, K_ROWS, K_COLS>(g, o, p.M, p.Cp, p.dx, p.part, s, who)) return rc;
   }
   if (dwg || dwu) {
-    const Outputs o = {{rows_of(dwg), rows_of(dwu)}, (int)p.Iw, (int)p.I, (int)p.C};
+    const Outputs o = {{rows_of(dwg), rows_of(dwu)}, (int)p.Iw, (int)p.I, (int)p.C, p.exponent};
     if (p.M == 0) return zeros_to<T>(o, 2 * p.Iw, p.Cp, s);
     GemmArgs g = {};
     g.a = cols_operand(d, 2 * p.Iw);

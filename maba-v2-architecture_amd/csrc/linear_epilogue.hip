@@ -15,6 +15,9 @@
 //   dx = dy (diag(gate) W),  dW = diag(gate) G,  dgate = rowdot(W, G) + b * colsum(dy),  db = gate * colsum(dy):
 // the gate goes onto the N x K weight (one rounding, as dz would have) and into the reduction, not onto the M x N
 // gradient (the down projection of 16,384 tokens: 48 us of 205).
+//
+// In fp16 dz and gate * W are held times a power of two, from the bounds |dz| <= 1.13 |dy| |gate| and |gate| |W| (two
+// launches; Magnitudes).
 #include <algorithm>
 
 #include "ffn_common.h"
@@ -138,15 +141,6 @@ struct EpiLinear {
   }
 };
 
-// The sum over the 16 lanes of a quarter of the wave, in each of them: neighbours, pairs, quads and eights.
-__device__ __forceinline__ float sum16(float v) {
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xb1, 0xf, 0xf, true));     // lanes 1 0 3 2
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4e, 0xf, 0xf, true));     // lanes 2 3 0 1
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xf, 0xf, true));    // a half mirrored
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xf, 0xf, true));    // mirrored
-  return v;
-}
-
 // dz [M, Np] (Np = N rounded up to 8, zeros behind N) and, with sums, the tile's column sums [tiles_m][2][N]: of dz
 // for the bias, of dy * act(z) for the gate.
 template <int ACT>
@@ -154,7 +148,7 @@ struct EpiLinearBack {
   // beside a 256 x 256 tile's sums its values do not fit into the registers (16,384 x 640 to 2,496: relu 150 us and gelu
   // 202, with 192 x 128 92 and 121)
   static constexpr bool LONG = true, GROUPS = false;
-  struct Args { Rows dy, dz; const uint16_t *bias, *gate; float* sums; int M, N, Np; };
+  struct Args { Rows dy, dz; const uint16_t *bias, *gate; float* sums; int M, N, Np; const int* exponent; };
   // dz, and its terms and those of dy * act(z) added to the column sums.  dy is zero behind the last row.
   static __device__ __forceinline__ f32x4 value(f32x4 z, f32x4 dy, f32x4 bias, f32x4 gate, f32x4& sb, f32x4& sg, bool in) {
     f32x4 dz;
@@ -171,6 +165,7 @@ struct EpiLinearBack {
   static __device__ __forceinline__ void run(const Args& e, f32x4 (&acc)[MI][NI], const TileId& t, int m0, int n0, int c,
                                              int q, int wave, uint16_t* lds) {
     float* part = (float*)lds;                    // [WM][2][BN]
+    const float scale = power_of<T>(e.exponent, 1);
     if (e.sums) __syncthreads();                  // the last stage has been read
     // 32 columns at a time, what the next ones read in flight meanwhile where that fits into the registers too
     constexpr bool AHEAD = MI < 6;
@@ -188,7 +183,7 @@ struct EpiLinearBack {
         const Quads d = quads_of(cur.rows[i]);
         const f32x4 a = value(acc[i][2 * j], up4<T>(d.a), bias[0], gate[0], sb[0], sg[0], m < e.M);
         const f32x4 b = value(acc[i][2 * j + 1], up4<T>(d.b), bias[1], gate[1], sb[1], sg[1], m < e.M);
-        store8(e.dz, m, n0 + 32 * j + 8 * q, e.M, e.Np, eight_of({down4<T>(a), down4<T>(b)}));
+        store8(e.dz, m, n0 + 32 * j + 8 * q, e.M, e.Np, eight_of({down4<T>(a * scale), down4<T>(b * scale)}));
       }
       if (e.sums) {
 #pragma unroll
@@ -242,7 +237,8 @@ struct LinearPlan {
   bool copy_x, copy_w, copy_dy, z;      // z: dz is made from z, otherwise the products take dy
   bool g, cols;                         // G is made; column sums are
   uint16_t *x, *w, *dz;
-  float *part, *sums, *colsum;
+  float *part, *sums, *colsum, *magnitudes;
+  int* exponent;                        // of dz, or of gate * W, in fp16
   GemmPlan xw, dx, dw;                  // the products x W^T, dz W and dz^T x
   size_t bytes;
 };
@@ -282,6 +278,10 @@ static LinearPlan linear_plan(const maba_tensor* x, const maba_tensor* scales, c
       part = std::max(part, (int64_t)p.dw.splits * p.Np * p.Kp);
     }
     p.part = c.take<float>(part);
+    if (w->dtype == MABA_F16 && (p.z || (gate && need->dx))) {
+      p.magnitudes = c.take<float>(MAX_FACTORS * MAGNITUDE_GROUPS);
+      p.exponent = c.take<int>(1);
+    }
   }
   p.xw = gemm_plan(p.M, p.Np, gemm_stages(p.Kp, 1), need ? PLAN_LONG : few ? 0 : PLAN_SPLIT | PLAN_GROUPS);
   if (p.xw.splits > 1) p.part = c.take<float>((int64_t)p.xw.splits * p.M * p.Np);
@@ -299,7 +299,7 @@ static int linear_operands(LinearPlan& p, const maba_tensor* x, const maba_tenso
                            const maba_tensor* gate, const maba_tensor* dy, hipStream_t s, Operand& ox, Operand& ow) {
   Copies copies;
   if (p.copy_x) copies.add(x, scales, p.x);
-  if (p.copy_w) copies.add(w, nullptr, p.w, p.z ? nullptr : gate);
+  if (p.copy_w) copies.add(w, nullptr, p.w, p.z ? nullptr : gate, p.exponent);
   if (p.copy_dy) copies.add(dy, nullptr, p.dz);
   if (int rc = copies.launch(w->dtype, s)) return rc;
   ox = p.copy_x ? rows_operand(p.x, p.Kp, p.M) : rows_operand((const uint16_t*)x->data, x->stride[0], p.M);
@@ -340,7 +340,7 @@ static int make_dz(const LinearPlan& p, const Operand& ox, const Operand& ow, co
   g.b = ow;
   g.K = p.Kp;
   const Rows dz = {p.dz, p.Np};
-  const typename E::Args e = {rows_of(dy), dz, vec_of(bias), vec_of(gate), p.sums, (int)p.M, (int)p.N, (int)p.Np};
+  const typename E::Args e = {rows_of(dy), dz, vec_of(bias), vec_of(gate), p.sums, (int)p.M, (int)p.N, (int)p.Np, p.exponent};
   return gemm<T, K_ROWS, K_ROWS, E>(g, e, p.M, p.Np, p.xw, s, who);
 }
 
@@ -349,6 +349,13 @@ static int linear_backward(LinearPlan& p, const maba_tensor* dy, const maba_tens
                            const maba_tensor* w, const maba_tensor* bias, int act, const maba_tensor* gate, maba_tensor* dx,
                            maba_tensor* dw, maba_tensor* dbias, maba_tensor* dgate, hipStream_t s, const char* who) {
   Operand ox, ow;
+  if (p.exponent && p.M > 0) {
+    Magnitudes m;
+    if (p.z) m.add(0, dy->data, dy->stride[0], p.M, p.N, false);
+    else m.add(0, w->data, w->stride[0], p.N, p.K, false);
+    if (gate) m.add(1, gate->data, 0, 1, p.N, false);
+    if (int rc = m.launch(p.z ? 1.13f : 1.f, p.magnitudes, p.exponent, s)) return rc;
+  }
   if (int rc = linear_operands(p, x, scales, w, gate, dy, s, ox, ow)) return rc;
   Operand dz = rows_operand((const uint16_t*)dy->data, dy->stride[0], p.M);
   if (p.z || p.copy_dy) dz = rows_operand(p.dz, p.Np, p.M);
@@ -371,7 +378,7 @@ static int linear_backward(LinearPlan& p, const maba_tensor* dy, const maba_tens
     g.a = dz;
     g.b = cols_operand(ow, p.Kp);
     g.K = p.Np;                 // dz is N wide where N is a whole number of chunks, padded with zeros otherwise
-    const Outputs o = {{rows_of(dx), rows_of(nullptr)}, INT32_MAX, (int)p.M, (int)p.K};
+    const Outputs o = {{rows_of(dx), rows_of(nullptr)}, INT32_MAX, (int)p.M, (int)p.K, p.exponent};
     if (int rc = product_to<T, K_ROWS, K_COLS>(g, o, p.M, p.Kp, p.dx, p.part, s, who)) return rc;
   }
   if (p.g) {
@@ -388,7 +395,7 @@ static int linear_backward(LinearPlan& p, const maba_tensor* dy, const maba_tens
                                  vec_of(gate), vec_of(bias), p.colsum, dgate ? (uint16_t*)dgate->data : nullptr};
       return reduce_gated(a, (int)p.N, w->dtype, s);
     }
-    const Outputs o = {{rows_of(dw), rows_of(nullptr)}, INT32_MAX, (int)p.N, (int)p.K};
+    const Outputs o = {{rows_of(dw), rows_of(nullptr)}, INT32_MAX, (int)p.N, (int)p.K, p.z ? p.exponent : nullptr};
     if (p.M == 0) return zeros_to<T>(o, p.Np, p.Kp, s);
     if (int rc = product_to<T, K_COLS, K_COLS>(g, o, p.Np, p.Kp, p.dw, p.part, s, who)) return rc;
   }
