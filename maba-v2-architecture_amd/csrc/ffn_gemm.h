@@ -281,9 +281,7 @@ __device__ __forceinline__ void wait_vm() {
 // Tile of this workgroup.  Consecutive ids go to the eight XCDs in turn, each with its own L2: every XCD gets a
 // contiguous run of tiles, in groups of GROUP_M rows of tiles taken column by column, so that the 32 to 64 workgroups
 // it runs at once share about as many panels of A as of B.
-#ifndef GROUP_M
-#define GROUP_M 4
-#endif
+constexpr uint32_t GROUP_M = 4;
 struct TileId { int m, n, split; };
 __device__ __forceinline__ TileId tile_of(const GemmArgs& g) {
   const uint32_t total = gridDim.x, id = blockIdx.x;
