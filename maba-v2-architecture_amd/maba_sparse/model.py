@@ -79,6 +79,8 @@ def _frozen(module: nn.Module, key: str, fn, *params: torch.Tensor) -> torch.Ten
 
 
 class SwiGLUFFN(WeightCacheMixin, nn.Module):
+    fused, checkpoint = False, None            # of a module that was saved without them
+
     def __init__(self, dim: int, intermediate_size: int, fused: bool = False, checkpoint: Optional[str] = None) -> None:
         super().__init__()
         self.fused = fused
@@ -131,7 +133,8 @@ class MabaBlock(WeightCacheMixin, nn.Module):
         self.norm1 = RMSNorm(config.dim, eps=config.rms_norm_eps)
         self.mixer = MabaSparseAttention(config) if self.is_attention else DGDALayer(config)
         self.norm2 = RMSNorm(config.dim, eps=config.rms_norm_eps)
-        self.ffn = SwiGLUFFN(config.dim, config.intermediate_size, config.fused_ffn, config.ffn_checkpoint)
+        self.ffn = SwiGLUFFN(config.dim, config.intermediate_size, getattr(config, "fused_ffn", False),
+                             getattr(config, "ffn_checkpoint", None))
         self.res_gate1 = nn.Parameter(torch.full((config.dim,), config.residual_gate_bias))
         self.res_gate2 = nn.Parameter(torch.full((config.dim,), config.residual_gate_bias))
 

@@ -572,3 +572,16 @@ def test_autocast_leaves_64_bits_alone():
         with pytest.raises(TypeError, match="dtypes must match"):
             D.linear_epilogue(x, w.float())
     assert y.dtype == F64 and torch.equal(y, D.linear_epilogue(x, w))
+
+
+def test_blocks_of_configs_and_modules_from_before_the_switch():
+    """A config without the fused fields and a module saved without them run as they did."""
+    from types import SimpleNamespace
+    cfg = MabaConfig(dim=64, n_heads=1, intermediate_size=40, n_layers=1)
+    old = SimpleNamespace(**{k: v for k, v in vars(cfg).items() if k not in ("fused_ffn", "ffn_checkpoint")})
+    blk = MabaBlock(old, 0)
+    x = torch.randn(2, 6, 64)
+    want = blk(x)[0]
+    for name in ("fused", "checkpoint"):
+        del blk.ffn.__dict__[name]
+    assert torch.equal(blk(x)[0], want)
