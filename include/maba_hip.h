@@ -411,8 +411,10 @@ int maba_hip_argmax_rows(const maba_tensor* x, maba_tensor* out, void* stream);
  *
  * Backward: dh [M,I]; x as above, or with x_scales its packed form (x: MABA_E4M3 codes [M,C], x_scales:
  * MABA_U8 [M,ceil(C/32)]); any of dx [M,C], dw_gate, dw_up [I,C] may be NULL.  g and u are made again from
- * x; [dg | du] is rounded to 16 bits once, as an operand of the next products.  Results are the same bits
- * on every call.  The query depends on the current device's compute-unit count; needs: 1 dx, 2 either
+ * x; [dg | du] is rounded to 16 bits once, as an operand of the next products, in fp16 times a power of two
+ * that keeps what fp32 keeps of it.  Results are the same bits on every call.  An x, dh or weight whose rows
+ * are broadcast or overlap (row stride below the width), and both weights where one of them is not aligned
+ * or their row strides differ, are copied too.  The query depends on the current device's compute-unit count; needs: 1 dx, 2 either
  * weight gradient.
  */
 size_t maba_hip_gated_ffn_workspace_size(const maba_tensor* x, const maba_tensor* w_gate, const maba_tensor* w_up);
@@ -430,7 +432,8 @@ int maba_hip_gated_ffn_backward(const maba_tensor* dh, const maba_tensor* x, con
  * none, 1 relu, 2 silu, 3 gelu (with the error function).  out may be residual itself.  Copies and the
  * workspace as for maba_hip_gated_ffn.
  *
- * Backward: dy [M,N]; x as above or packed, with x_scales; any of dx [M,K], dw [N,K], dbias, dgate [N] may be
+ * Backward: dy [M,N] (copies and roundings as above; the operands rounded on the way are dz, or gate * weight
+ * without an activation); x as above or packed, with x_scales; any of dx [M,K], dw [N,K], dbias, dgate [N] may be
  * NULL (the residual's gradient is dy).  needs: 1 dx, 2 dw, 4 dbias, 8 dgate.
  */
 size_t maba_hip_linear_epilogue_workspace_size(const maba_tensor* x, const maba_tensor* weight);

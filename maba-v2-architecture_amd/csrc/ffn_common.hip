@@ -14,11 +14,12 @@ namespace ffn {
 //   full       1.36 (1.38)    0.55 (0.63)    0.57 (0.64)    0.46 (0.50)    0.20 (0.25)
 //   lone       1.36 (1.38)    0.80 (1.00)    0.75 (0.95)    0.60 (0.74)    0.36 (0.47)
 //   ends       9              4              3              3              0.75
-// Over 31 products of rows and columns, in up to twelve splits, each timed with every tile, the plan takes 1.5 % more
-// than the best of them on average, 9 % at most.  (4,096 x 11,008 x 2,048, rows: 150, 169, -, 175 us with the first
-// four; 16,384 x 640 x 2,496, columns: 70, 58, 56, 79, and 32,768 x 640 x 1,248, rows: 70, 64, 58, 63, where 160 columns
-// leave no part of a tile over; 16,384 x 2,496 x 640, rows: 60, 54, -, 57, the smallest 81; 64 x 640 x 2,496 with the last, in 1, 4 and
-// 8 splits: 19.9, 7.2 and 5.2.)
+// Over 31 products of rows and columns, in up to twelve splits, each timed with every tile of one group
+// (profiles/feed_forward_tiles.txt), the plan's choice of the timed ones takes 1.6 % more than the best of them on average, 20 % at most and but for
+// that one 9 %.  (4,096 x 11,008 x 2,048, rows: 150, 169, -, 175 us with the first four; 16,384 x 640 x 2,496, columns: 70, 58,
+// 56, 79, and 32,768 x 640 x 1,248, rows: 70, 64, 58, 63, where 160 columns leave no part of a tile over; 16,384 x 2,496 x 640,
+// rows: 60, 54, -, 57, the smallest 81; 64 x 640 x 2,496 with the last, in 1, 4 and 8 splits: 19.9, 7.2 and 5.2.)  The smallest
+// tile is priced with two stages; rows whose few tiles are all resident then run it with four (Tile64Deep).
 //
 // Two groups of waves on a tile (`groups`; a stage is then two) serve tiles too few to share a compute unit.  Its one
 // group of four waves keeps the matrix units 26 % busy; a second workgroup's would do the same as a second group.

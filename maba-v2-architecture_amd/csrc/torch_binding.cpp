@@ -1,7 +1,7 @@
 // The feed-forward operators as native autograd functions for torch: what the Python path does (maba_sparse/kernels/
 // feed_forward.py over hip_backend.py), without Python in the call or in the autograd engine's thread.
 //
-// Bound by the host: a training step of 1,777 x 555 to 1,001, whose kernels take 65 us, takes 95 us here and took 177 by the
+// Bound by the host: a training step of 1,777 x 555 to 1,001, whose kernels take 74 us, takes 95 us here and took 177 by the
 // Python path (an empty autograd function in Python: 78); a forward call 9 and 19.
 //
 // A call that is not plain (other dtypes or devices, shapes that do not fit, tensor subclasses, tangents of forward-mode

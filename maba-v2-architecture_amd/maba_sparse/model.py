@@ -50,6 +50,7 @@ class MabaConfig:
     residual_gate_bias: float = 2.0
     # The feed-forward half of a block through the dispatcher's fused operators (gated_ffn and
     # linear_epilogue), forward and backward; off, it composes torch modules as the reference does.
+    # A decode step's projections are decode_linear's either way.
     fused_ffn: bool = False
     # With fused_ffn: what those operators keep for the backward pass, None (16 bits) or "e4m3" (8 bits).
     ffn_checkpoint: Optional[str] = None
