@@ -100,3 +100,60 @@ def test_linear_gradients_at_every_size_of_gate_weight_and_output_gradient(M, K,
         assert bool(inside.any())
         over = (v.double() - value).abs() / bound
         assert float(over[inside].max()) <= 1.0, (name, float(over[inside].max()))
+
+
+def test_a_replayed_graph_scales_by_what_it_finds():
+    """The powers of two belong to the values of each replay, in two graphs that share their workspaces' memory."""
+    r = _gen(7)
+    sets = []
+    for M, Cw, I in ((300, 136, 72), (70, 64, 200)):
+        sets.append(dict(x=r(M, Cw).to(HF), wg=(r(I, Cw) / Cw ** 0.5).to(HF), wu=(r(I, Cw) / Cw ** 0.5).to(HF), dh=r(M, I).to(HF),
+                         gate=torch.rand(I, device=DEV).to(HF)))
+
+    def step(t):
+        return [*D.gated_ffn_backward(t["dh"], t["x"], t["wg"], t["wu"]),
+                *D.linear_epilogue_backward(t["dh"], t["x"], t["wg"], t["gate"], "silu", t["gate"]),
+                *D.linear_epilogue_backward(t["dh"], t["x"], t["wg"], None, "none", t["gate"])[:2]]
+
+    for t in sets:
+        step(t)
+    torch.cuda.synchronize()
+    graphs, outs, pool = [], [], None
+    for t in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(step(t))
+        pool = g.pool()
+        graphs.append(g)
+    for turn, power in ((0, 0), (1, -12), (1, 6), (0, -14), (1, 0), (0, 3), (0, -8)):
+        t = sets[turn]
+        t["dh"].copy_(r(*t["dh"].shape) * 2.0 ** power)
+        t["gate"].copy_(torch.rand(t["gate"].shape, device=DEV) * 2.0 ** (power / 2))
+        graphs[turn].replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs[turn]]
+        assert all(torch.equal(a, b) for a, b in zip(got, step(t))), (turn, power)
+        want = B.gated(t["x"], t["wg"], t["wu"], t["dh"].double() * 2.0 ** 16)
+        for name, v in zip(("dx", "dw_gate", "dw_up"), got):
+            B.check(v, _at(want[name], 16), name)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_bad_element_spoils_only_what_is_made_of_it(bad):
+    """Elements that are not finite take no part in the bound: the rest keeps its bits, and small gradients theirs."""
+    M, Cw, I = 90, 48, 40
+    r = _gen(8)
+    x, wg, wu, dh = r(M, Cw).to(HF), (r(I, Cw) / 7).to(HF), (r(I, Cw) / 7).to(HF), (r(M, I) * 2.0 ** -12).to(HF)
+    rows = torch.arange(M, device=DEV) != 3
+    for where in ("x", "dh"):
+        args = dict(x=x.clone(), dh=dh.clone())
+        args[where][3, 5] = bad
+        want = B.gated(x[rows], wg, wu, dh[rows].double() * 2.0 ** 16)
+        dx, dwg, _ = D.gated_ffn_backward(args["dh"], args["x"], wg, wu)
+        B.check(dx[rows], _at(want["dx"], 16), where)
+        assert not torch.isfinite(dx[3]).any() and not torch.isfinite(dwg).all()
+        for act in ("silu", "none"):
+            b, g = wu[:, 0].contiguous(), wu[:, 1].abs().contiguous()
+            want = B.linear(x[rows], wg, b, act, None, g, dh[rows].double() * 2.0 ** 16)
+            dx = D.linear_epilogue_backward(args["dh"], args["x"], wg, b, act, g)[0]
+            B.check(dx[rows], _at(want["dx"], 16), (where, act))
