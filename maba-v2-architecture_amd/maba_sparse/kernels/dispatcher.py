@@ -536,7 +536,8 @@ def dispatch_gated_ffn(x, w_gate, w_up, checkpoint: Optional[str] = None) -> tor
 
 def dispatch_gated_ffn_backward(dh, x, w_gate, w_up, x_scales=None, needs=(True, True, True)):
     """``(dx, dw_gate, dw_up)`` of ``gated_ffn`` for its output's gradient ``dh [..., I]``, None where ``needs``
-    is false.  ``x`` is the forward's input, or with ``x_scales`` its packed codes.  No autograd takes part."""
+    is false.  ``x`` is the forward's input, or with ``x_scales`` its packed codes.  No autograd takes part.  On the HIP
+    backend the gradients of the two pre-activations are rounded to 16 bits once, as operands of the products."""
     _ffn_input(x)
     _ffn_kept(x, x_scales)
     _ffn_same(dh, x=x if x_scales is None else None, w_gate=w_gate, w_up=w_up)
@@ -601,7 +602,8 @@ def dispatch_linear_epilogue_backward(dy, x, weight, bias=None, activation: str 
                                       needs=(True, True, True, True)):
     """``(dx, dw, dbias, dgate)`` of ``linear_epilogue`` for its output's gradient ``dy [..., N]``, None where
     ``needs`` is false or there is no bias or gate; the residual's gradient is ``dy``.  ``x`` as for
-    ``gated_ffn_backward``.  No autograd takes part."""
+    ``gated_ffn_backward``.  No autograd takes part.  On the HIP backend the pre-activation's gradient (without an
+    activation, gate times weight) is rounded to 16 bits once, as an operand of the products."""
     _ffn_input(x)
     _ffn_kept(x, x_scales)
     _ffn_same(dy, x=x if x_scales is None else None, weight=weight, bias=bias, gate=gate)
