@@ -15,8 +15,8 @@ namespace ffn {
 //   lone       1.36 (1.38)    0.80 (1.00)    0.75 (0.95)    0.60 (0.74)    0.36 (0.47)
 //   ends       9              4              3              3              0.75
 // Over 31 products of rows and columns, in up to twelve splits, each timed with every tile of one group
-// (profiles/feed_forward_tiles.txt), the plan's choice of the timed ones takes 1.6 % more than the best of them on average, 20 % at most and but for
-// that one 9 %.  (4,096 x 11,008 x 2,048, rows: 150, 169, -, 175 us with the first four; 16,384 x 640 x 2,496, columns: 70, 58,
+// (profiles/feed_forward_tiles.txt), the plan's choice of the timed ones takes 1.6 % more than the best of them on
+// average, 20 % at most and but for that one 9 %.  (4,096 x 11,008 x 2,048, rows: 150, 169, -, 175 us with the first four; 16,384 x 640 x 2,496, columns: 70, 58,
 // 56, 79, and 32,768 x 640 x 1,248, rows: 70, 64, 58, 63, where 160 columns leave no part of a tile over; 16,384 x 2,496 x 640,
 // rows: 60, 54, -, 57, the smallest 81; 64 x 640 x 2,496 with the last, in 1, 4 and 8 splits: 19.9, 7.2 and 5.2.)  The smallest
 // tile is priced with two stages; rows whose few tiles are all resident then run it with four (Tile64Deep).
@@ -236,9 +236,10 @@ __global__ __launch_bounds__(256) void magnitudes_kernel(MagnitudeArgs a) {
   if (threadIdx.x < MAX_FACTORS) a.partial[threadIdx.x * MAGNITUDE_GROUPS + blockIdx.x] = __uint_as_float(part[threadIdx.x]);
 }
 
-// 2 us, most of it the launch.  bound = 1.25 slope * the factors' product (the quarter covers the rounding of the sums that the operand is made of and
-// of these); a wave reads a factor's partials.
-__global__ __launch_bounds__(64 * MAX_FACTORS) void exponent_kernel(const float* partial, int groups, int factors, float slope, int* exponent) {
+// bound = 1.25 slope * the factors' product (the quarter covers the rounding of the sums that the operand is made of
+// and of these); a wave reads a factor's partials.  2 us, most of it the launch.
+__global__ __launch_bounds__(64 * MAX_FACTORS) void exponent_kernel(const float* partial, int groups, int factors, float slope,
+                                                                    int* exponent) {
   __shared__ float part[MAX_FACTORS];
   const int f = threadIdx.x >> 6, lane = threadIdx.x & 63;
   float x = 0.f;

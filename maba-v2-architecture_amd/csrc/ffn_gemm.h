@@ -430,8 +430,8 @@ __device__ __forceinline__ float power_of(const int* exponent, int sign) {
   else return 1.f;
 }
 
-// Epilogue: C, times 2^-*exponent where there is one, rounded once to 16 bits; from row `second` on it goes to the second tensor's rows (`second`
-// is a multiple of 16).  M: rows of each.
+// Epilogue: C, times 2^-*exponent where there is one, rounded once to 16 bits; from row `second` on it goes to the
+// second tensor's rows (`second` is a multiple of 16).  M: rows of each.
 struct EpiStore {
   static constexpr bool LONG = false, GROUPS = true;
   struct Args { Rows c[2]; int second, M, N; const int* exponent; };

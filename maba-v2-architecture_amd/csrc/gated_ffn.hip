@@ -10,10 +10,12 @@
 // Backward: the forward keeps nothing but x.  The first launch makes g and u again (4 M C I operations, which
 // cost about what writing and reading the two would at C <= 1000 or so) and its epilogue turns them with dh
 // into [dg | du], rounded once to 16 bits as an operand of the next products: kept in fp32 to here, so the
-// gradients carry that one rounding and their own.  In fp16 [dg | du] is held times a power of two, from the bounds
-// |dg|, |du| <= 1.1 |dh| max(|g|, |u|) and |g|, |u| <= |x| |w|, norms of rows (two launches; Magnitudes).  The second launch is dx over k = [dg | du]'s columns with
+// gradients carry that one rounding and their own.  The second launch is dx over k = [dg | du]'s columns with
 // both weights read along their columns, the third [dWg; dWu] = [dg | du]^T x, summed over token ranges into
 // fp32 partials that a last launch adds in order (the same bits every time).
+//
+// In fp16 [dg | du] is held times a power of two, from the bounds |dg|, |du| <= 1.1 |dh| max(|g|, |u|) and
+// |g|, |u| <= |x| |w|, norms of rows: two launches before the first (Magnitudes).
 #include <algorithm>
 
 #include "ffn_common.h"

@@ -5,8 +5,8 @@
 // Python path (an empty autograd function in Python: 78); a forward call 9 and 19.
 //
 // A call that is not plain (other dtypes or devices, shapes that do not fit, tensor subclasses, tangents of forward-mode
-// derivatives, sizes that the library refuses) is declined: the function returns None and the caller takes the Python path, which checks, raises or falls
-// back.
+// derivatives, sizes that the library refuses) is declined: the function returns None and the caller takes the Python
+// path, which checks, raises or falls back.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
