@@ -71,6 +71,10 @@
  *                                   product; its gradients come from autograd there)
  *   maba_hip_linear_epilogue        nn.Linear with what follows it: the bias, an activation,
  *                                   the gated residual of model.py:92-128
+ *   maba_hip_residual_norm          model.py:11-22, 92-128 (the gated residual between a norm after a
+ *                                   sub-layer and the norm before the next, with dropout), and its
+ *                                   gradients, which come from autograd there
+ *   maba_hip_dropout                no counterpart: dropout whose mask is made from a counter
  *   maba_hip_checkpoint_pack        no counterpart: the input that those two keep for their
  *                                   backward passes, in 8 bits
  */
@@ -457,6 +461,42 @@ int maba_hip_linear_epilogue_backward(const maba_tensor* dy, const maba_tensor* 
  */
 int maba_hip_checkpoint_pack(const maba_tensor* x, maba_tensor* codes, maba_tensor* scales, void* stream);
 int maba_hip_checkpoint_unpack(const maba_tensor* codes, const maba_tensor* scales, maba_tensor* out, void* stream);
+
+/*
+ * Dropout.  x, out [M,C] f32, f16 or bf16, one type, unit column stride, any row stride and alignment; out may be x
+ * itself.  out = x / (1 - p) where the element is kept and 0, whatever x is, where it is dropped; computed in fp32
+ * and rounded once.  Element (m, c) is kept iff its word is at least round(p 2^32): word c % 4 of Philox4x32 with
+ * seven rounds (Salmon et al., 2011), counter (c / 4, m mod 2^32, m / 2^32, stream_id), key *seed (low word first).
+ * seed is one uint64 in device memory, read when the kernel runs (so a replayed graph follows it), and not read for
+ * p = 0 or 1.  The gradient is the same call on the output's gradient.
+ */
+int maba_hip_dropout(const maba_tensor* x, double p, const int64_t* seed, uint32_t stream_id, maba_tensor* out,
+                     void* stream);
+
+/*
+ * The boundary between two sub-layers: x_out = x + scale * gate * dropout(z), z = y / sqrt(mean(y^2) + eps) *
+ * post_weight (y itself without post_weight), and h = x_out / sqrt(mean(x_out^2) + eps) * weight.  x, y, x_out, h
+ * [M,C] f32, f16 or bf16, weight, post_weight, gate [C], one type; C <= 8192, unit column stride, any row stride and
+ * alignment; y (then h is x's norm), weight with h, post_weight, gate and x_out may be NULL, and x_out may be x.
+ * fp32 arithmetic; x_out is rounded once, and h once from the unrounded x_out.  Dropout as in maba_hip_dropout.
+ *
+ * Backward: dx_out, dh [M,C], either of which may be NULL (zeros); x_out as the forward returned it, read only with dh;
+ * y is read only with post_weight or for dgate; any of dx, dy [M,C], dweight, dpost_weight, dgate [C] may be NULL.
+ * Parameters' gradients are summed in fp32 through the workspace (16-byte aligned, of one call at a time; the query
+ * depends on the current device's compute-unit count; grads: 1 dweight, 2 dgate, 4 dpost_weight), in a fixed order:
+ * results are the same bits on every call.
+ */
+int maba_hip_residual_norm(const maba_tensor* x, const maba_tensor* y, const maba_tensor* weight,
+                           const maba_tensor* post_weight, const maba_tensor* gate, float scale, double p,
+                           const int64_t* seed, uint32_t stream_id, float eps, maba_tensor* x_out, maba_tensor* h,
+                           void* stream);
+size_t maba_hip_residual_norm_backward_workspace_size(const maba_tensor* x_out, int grads);
+int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const maba_tensor* dh, const maba_tensor* x_out,
+                                    const maba_tensor* y, const maba_tensor* weight, const maba_tensor* post_weight,
+                                    const maba_tensor* gate, float scale, double p, const int64_t* seed,
+                                    uint32_t stream_id, float eps, maba_tensor* dx, maba_tensor* dy,
+                                    maba_tensor* dweight, maba_tensor* dpost_weight, maba_tensor* dgate,
+                                    void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,559 @@
+// The boundary between two sub-layers and dropout by itself, forward and backward:
+//   z  = RMSNorm(y) * w_post  (or y)             the norm after the sub-layer that made y
+//   x' = x + scale * gate * dropout(z)           the residual stream
+//   h  = RMSNorm(x') * w                         the norm before the next sub-layer
+// (reference model.py:11-22, 92-128 has the gated residual and the norm before, composed of torch modules.)
+//
+// Backward, for the gradients d' of x' and dh of h, with x^ = x' r, y^ = y rp the normalised rows:
+//   dX = d' + r (dh w - x^ mean(dh w x^))        the gradient of x, and of x' behind its norm
+//   dz = scale gate dropout(dX)                  the same mask, made again
+//   dy = rp (dz w_post - y^ mean(dz w_post y^))
+//   dw = sum dh x^,  dgate = sum scale dX dropout(z),  dw_post = sum dz y^     over the rows
+// r and rp are made again from the rows that are read anyway; nothing but x' and y is kept from the forward pass.
+//
+// Bound: HBM.  Forward reads x and y and writes x' and h; backward reads d', dh, x', y and writes dx and dy, once each.
+#include "row_vec.h"
+
+namespace maba {
+namespace rowvec {
+
+struct BoundaryArgs {
+  const void *x, *y, *w, *wp, *g;
+  void *xo, *h;
+  int64_t xs, ys, xos, hs, R;
+  int C, lg;
+  float scale, eps;
+  Drop d;
+};
+
+template <class T, int NCH>
+__global__ __launch_bounds__(1 << MAX_LG) void boundary_kernel(BoundaryArgs a) {
+  constexpr int V = Traits<T>::VEC;
+  __shared__ float red[2 * (1 << MAX_LG) / 64];
+  int turn = 0;
+  const int lg = a.lg, l = threadIdx.x & ((1 << lg) - 1), slots = blockDim.x >> lg;
+  // the wave's first row of the workgroup's, and which of the wave's this lane is in
+  const int first = __builtin_amdgcn_readfirstlane(threadIdx.x >> lg), sub = lg < 6 ? (threadIdx.x & 63) >> lg : 0;
+  const Walk<T> wx(a.x, a.xs, l, sub), wy(a.y, a.ys, l, sub), wxo(a.xo, a.xos, l, sub), wh(a.h, a.hs, l, sub);
+  const Walk<T> vw(a.w, 0, l, 0), vp(a.wp, 0, l, 0), vg(a.g, 0, l, 0);
+  const uint64_t key = a.d.mode == 1 ? *a.d.seed : 0;
+  const float inv_c = 1.f / (float)a.C;
+  u32x4 w[NCH] = {}, wp[NCH] = {}, g[NCH] = {};
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int at = (l + (i << lg)) * V;
+    if (a.w) w[i] = load_chunk<T>(vw.at(0, i << lg), vw.off, a.C - at);
+    if (a.wp) wp[i] = load_chunk<T>(vp.at(0, i << lg), vp.off, a.C - at);
+    if (a.g) g[i] = load_chunk<T>(vg.at(0, i << lg), vg.off, a.C - at);
+  }
+  for (int64_t r0 = (int64_t)blockIdx.x * slots; r0 < a.R; r0 += (int64_t)gridDim.x * slots) {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) asm volatile("" : "+v"(w[i]), "+v"(wp[i]), "+v"(g[i]));     // held packed, not unpacked ahead of the loop
+    const int64_t ru = r0 + first, r = ru + sub;
+    const int C = r < a.R ? a.C : 0;               // a row past the last one has no elements
+    u32x4 x[NCH], y[NCH];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int at = (l + (i << lg)) * V;
+      x[i] = load_chunk<T>(wx.at(ru, i << lg), wx.off, C - at);
+      if (a.y) y[i] = load_chunk<T>(wy.at(ru, i << lg), wy.off, C - at);
+    }
+    float rp = 1.f;
+    if (a.wp) {
+      float s[1] = {0.f};
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        float v[V];
+        unpack<T>(y[i], v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[0] = fmaf(v[e], v[e], s[0]);
+      }
+      row_sums<1>(s, lg, red, turn);
+      rp = rsqrtf(s[0] * inv_c + a.eps);
+    }
+    float xn[NCH][V], ss[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int at = (l + (i << lg)) * V;
+      unpack<T>(x[i], xn[i]);
+      if (a.y) {
+        float z[V], p[V];
+        unpack<T>(y[i], z);
+        if (a.wp) {
+          unpack<T>(wp[i], p);
+#pragma unroll
+          for (int e = 0; e < V; ++e) z[e] *= rp * p[e];
+        }
+        drop_chunk<V>(z, a.d, key, r, at);
+        if (a.g) {
+          unpack<T>(g[i], p);
+#pragma unroll
+          for (int e = 0; e < V; ++e) z[e] *= p[e];
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) xn[i][e] = fmaf(a.scale, z[e], xn[i][e]);
+        if (a.xo) store_chunk<T>(wxo.at(ru, i << lg), wxo.off, C - at, pack<T>(xn[i]));
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) ss[0] = fmaf(xn[i][e], xn[i][e], ss[0]);
+      __builtin_amdgcn_sched_barrier(0);           // chunk after chunk: side by side their masks cost 50 registers more
+    }
+    if (a.w) {
+      row_sums<1>(ss, lg, red, turn);
+      const float rx = rsqrtf(ss[0] * inv_c + a.eps);
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        const int at = (l + (i << lg)) * V;
+        float p[V];
+        unpack<T>(w[i], p);
+#pragma unroll
+        for (int e = 0; e < V; ++e) p[e] *= xn[i][e] * rx;
+        store_chunk<T>(wh.at(ru, i << lg), wh.off, C - at, pack<T>(p));
+      }
+    }
+  }
+}
+
+// The parameters' gradients: a lane sums its columns over its rows in registers, a workgroup its rows' lanes in LDS, and
+// columns_kernel the workgroups' partials [groups][n][C] in their order.
+enum { GRAD_W = 1, GRAD_GATE = 2, GRAD_POST = 4 };
+struct BoundaryBackArgs {
+  const void *dxo, *dh, *xo, *y, *w, *wp, *g;
+  void *dx, *dy;
+  float* partial;
+  int64_t dxos, dhs, xos, ys, dxs, dys, R;
+  int C, lg, grads;
+  float scale, eps;
+  Drop d;
+};
+
+template <class T, int NCH, bool POST>
+__global__ __launch_bounds__(1 << MAX_LG) void boundary_back_kernel(BoundaryBackArgs a) {
+  constexpr int V = Traits<T>::VEC, NG = POST ? 3 : 2;
+  __shared__ float red[2 * 3 * (1 << MAX_LG) / 64];
+  extern __shared__ float sums[];                  // [NG][threads * V]
+  const int threads = blockDim.x;
+  int turn = 0;
+  const int lg = a.lg, l = threadIdx.x & ((1 << lg) - 1), slots = threads >> lg;
+  const int first = __builtin_amdgcn_readfirstlane(threadIdx.x >> lg), sub = lg < 6 ? (threadIdx.x & 63) >> lg : 0;
+  const Walk<T> wd(a.dxo, a.dxos, l, sub), wh(a.dh, a.dhs, l, sub), wx(a.xo, a.xos, l, sub), wy(a.y, a.ys, l, sub);
+  const Walk<T> wdx(a.dx, a.dxs, l, sub), wdy(a.dy, a.dys, l, sub);
+  const Walk<T> vw(a.w, 0, l, 0), vp(a.wp, 0, l, 0), vg(a.g, 0, l, 0);
+  const uint64_t key = a.d.mode == 1 ? *a.d.seed : 0;
+  const float inv_c = 1.f / (float)a.C;
+  float acc[NG][NCH][V] = {};
+  for (int64_t r0 = (int64_t)blockIdx.x * slots; r0 < a.R; r0 += (int64_t)gridDim.x * slots) {
+    const int64_t ru = r0 + first, r = ru + sub;
+    const int C = r < a.R ? a.C : 0;
+    u32x4 ud[NCH], uh[NCH], ux[NCH], uy[NCH];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int at = (l + (i << lg)) * V;
+      if (a.dh) {
+        uh[i] = load_chunk<T>(wh.at(ru, i << lg), wh.off, C - at);
+        ux[i] = load_chunk<T>(wx.at(ru, i << lg), wx.off, C - at);
+      }
+      if (a.dxo) ud[i] = load_chunk<T>(wd.at(ru, i << lg), wd.off, C - at);
+      if (a.y) uy[i] = load_chunk<T>(wy.at(ru, i << lg), wy.off, C - at);
+    }
+    float s[3] = {0.f, 0.f, 0.f};            // of dh w x', x'^2, y^2
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int at = (l + (i << lg)) * V;
+      if (a.dh) {
+        float h[V], x[V], p[V];
+        unpack<T>(uh[i], h);
+        unpack<T>(ux[i], x);
+        unpack<T>(load_chunk<T>(vw.at(0, i << lg), vw.off, C - at), p);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          s[0] = fmaf(h[e] * p[e], x[e], s[0]);
+          s[1] = fmaf(x[e], x[e], s[1]);
+        }
+      }
+      if constexpr (POST) {
+        float y[V];
+        unpack<T>(uy[i], y);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[2] = fmaf(y[e], y[e], s[2]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (a.dh || POST) row_sums<3>(s, lg, red, turn);
+    const float rx = rsqrtf(s[1] * inv_c + a.eps), mean = s[0] * rx * inv_c;
+    const float rp = POST ? rsqrtf(s[2] * inv_c + a.eps) : 1.f;
+    float dz[NCH][V], t[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int at = (l + (i << lg)) * V;
+      float d[V] = {};
+      if (a.dxo) unpack<T>(ud[i], d);
+      if (a.dh) {
+        float h[V], x[V], p[V];
+        unpack<T>(uh[i], h);
+        unpack<T>(ux[i], x);
+        unpack<T>(load_chunk<T>(vw.at(0, i << lg), vw.off, C - at), p);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float xh = x[e] * rx;
+          d[e] = fmaf(rx, fmaf(h[e], p[e], -xh * mean), d[e]);
+          acc[0][i][e] = fmaf(h[e], xh, acc[0][i][e]);
+        }
+      }
+      if (a.dx) store_chunk<T>(wdx.at(ru, i << lg), wdx.off, C - at, pack<T>(d));
+      if (!a.dy && !(a.grads & (GRAD_GATE | GRAD_POST))) continue;
+      // dropout(z) = m z with m in {0, 1 / (1 - p)}: both products with m follow from m dX
+      drop_chunk<V>(d, a.d, key, r, at);
+      float p[V], y[V];
+      if (a.y) unpack<T>(uy[i], y);
+      if constexpr (POST) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[e] *= rp;
+        unpack<T>(load_chunk<T>(vp.at(0, i << lg), vp.off, C - at), p);
+      }
+      if (a.grads & GRAD_GATE)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[1][i][e] = fmaf(d[e], POST ? y[e] * p[e] : y[e], acc[1][i][e]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) dz[i][e] = a.scale * d[e];
+      if (a.g) {
+        float q[V];
+        unpack<T>(load_chunk<T>(vg.at(0, i << lg), vg.off, C - at), q);
+#pragma unroll
+        for (int e = 0; e < V; ++e) dz[i][e] *= q[e];
+      }
+      if constexpr (POST) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          acc[NG - 1][i][e] = fmaf(dz[i][e], y[e], acc[NG - 1][i][e]);
+          dz[i][e] *= p[e];
+          t[0] = fmaf(dz[i][e], y[e], t[0]);
+        }
+      } else if (a.dy) {
+        store_chunk<T>(wdy.at(ru, i << lg), wdy.off, C - at, pack<T>(dz[i]));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (POST) {
+      if (a.dy) {
+        row_sums<1>(t, lg, red, turn);
+        const float m = t[0] * inv_c * rp;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+          const int at = (l + (i << lg)) * V;
+          float y[V];
+          unpack<T>(uy[i], y);
+#pragma unroll
+          for (int e = 0; e < V; ++e) dz[i][e] = rp * fmaf(-y[e], m, dz[i][e]);
+          store_chunk<T>(wdy.at(ru, i << lg), wdy.off, C - at, pack<T>(dz[i]));
+        }
+      }
+    }
+  }
+  if (!a.grads) return;
+  // rows that share a wave first, then those of the workgroup's waves
+  const int lanes = 1 << lg, wave = threadIdx.x >> 6;
+  const int units = lg < 6 ? threads / 64 : slots;
+  const int mine = lg < 6 ? wave * lanes + (threadIdx.x & 63) : threadIdx.x;
+  const bool writes = lg >= 6 || (int)(threadIdx.x & 63) < lanes;
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float v = acc[n][i][e];
+        if (lg < 5) v += __shfl_xor(v, 16);
+        if (lg < 6) v += __shfl_xor(v, 32);
+        if (writes) sums[(n * threads + mine) * V + e] = v;
+      }
+    __syncthreads();
+    int k = 0;
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      if (!(a.grads >> n & 1)) continue;
+      float* out = a.partial + ((int64_t)blockIdx.x * __builtin_popcount(a.grads) + k++) * a.C;
+      for (int c = threadIdx.x; c < lanes * V; c += threads) {
+        const int col = (i << lg) * V + c;
+        if (col >= a.C) continue;
+        float v = 0.f;
+        for (int u = 0; u < units; ++u) v += sums[(n * threads + u * lanes) * V + c];
+        out[col] = v;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// out[c] = factor * the sum over g of p[g][n][c], in the order of g within each of sixteen runs and of the runs.
+struct ColumnsArgs {
+  const float* p;
+  void* out[3];
+  float factor[3];
+  int groups, n, C;
+};
+template <class T>
+__global__ __launch_bounds__(1024) void columns_kernel(ColumnsArgs a) {
+  __shared__ float part[16][64];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), run = threadIdx.x >> 6, n = blockIdx.y;
+  float s = 0.f;
+  if (c < a.C) {
+    const float* p = a.p + (int64_t)n * a.C + c;
+#pragma unroll 8
+    for (int g = run; g < a.groups; g += 16) s += p[(int64_t)g * a.n * a.C];
+  }
+  part[run][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (run == 0 && c < a.C) {
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v += part[i][threadIdx.x];
+    v *= a.factor[n];
+    if constexpr (T::CODE == MABA_F32) ((float*)a.out[n])[c] = v;
+    else ((uint16_t*)a.out[n])[c] = (uint16_t)T::down(v);
+  }
+}
+
+// ---------------------------------------------------------------- dropout
+
+struct DropArgs {
+  const void* x; void* y;
+  int64_t xs, ys, R;
+  int C, lg;
+  Drop d;
+};
+// 2^lg lanes a row, four chunks a lane in flight.
+template <class T>
+__global__ __launch_bounds__(256) void dropout_kernel(DropArgs a) {
+  constexpr int V = Traits<T>::VEC, N = 4;
+  const int l = threadIdx.x & ((1 << a.lg) - 1), slots = 256 >> a.lg;
+  const uint64_t key = a.d.mode == 1 ? *a.d.seed : 0;
+  const int chunks = (a.C + V - 1) / V;
+  for (int64_t r = (int64_t)blockIdx.x * slots + (threadIdx.x >> a.lg); r < a.R; r += (int64_t)gridDim.x * slots)
+    for (int c0 = l; c0 < chunks; c0 += N << a.lg) {
+      u32x4 u[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int64_t at = ((int64_t)c0 + (i << a.lg)) * V;
+        u[i] = load_chunk<T>((const typename Traits<T>::elem*)a.x + r * a.xs + at, 0, at < a.C ? (int)(a.C - at) : 0);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int64_t at = ((int64_t)c0 + (i << a.lg)) * V;
+        if (at >= a.C) continue;
+        float v[V];
+        unpack<T>(u[i], v);
+        drop_chunk<V>(v, a.d, key, r, (int)at);
+        store_chunk<T>((typename Traits<T>::elem*)a.y + r * a.ys + at, 0, (int)(a.C - at), pack<T>(v));
+      }
+    }
+}
+
+// ---------------------------------------------------------------- arguments
+
+static int check_float_rows(const maba_tensor* t, const char* who) {
+  if (!t) return fail(MABA_ERR_INVALID, "%s: x is missing", who);
+  if (!is_float_dt(t->dtype)) return fail(MABA_ERR_DTYPE, "%s: f32, f16 or bf16 only, got dtype code %d", who, t->dtype);
+  if (t->ndim != 2) return fail(MABA_ERR_INVALID, "%s: x must be 2D, got %dD", who, t->ndim);
+  if (t->shape[1] < 1) return fail(MABA_ERR_INVALID, "%s: the width must be positive", who);
+  if (t->shape[1] > (1 << 30) || t->shape[0] > (int64_t)1 << 40) return fail(MABA_ERR_UNSUPPORTED, "%s: sizes out of range", who);
+  return MABA_OK;
+}
+static int check_drop(const char* who, double p, const int64_t* seed) {
+  if (!(p >= 0.0 && p <= 1.0)) return fail(MABA_ERR_INVALID, "%s: p=%g must be in [0, 1]", who, p);
+  if (p > 0.0 && p < 1.0 && (!seed || (uintptr_t)seed % 8)) return fail(MABA_ERR_INVALID, "%s: dropout needs a seed", who);
+  return MABA_OK;
+}
+static int chunk_elems(int dtype) { return dtype == MABA_F32 ? 4 : 8; }
+static bool same_place(const maba_tensor* a, const maba_tensor* b) {
+  return a->data == b->data && (a->shape[0] <= 1 || a->stride[0] == b->stride[0]);
+}
+
+// Whether four rows of one of the tensors are further apart than 32 bits of bytes tell.
+static bool far_rows(std::initializer_list<const maba_tensor*> all) {
+  for (const maba_tensor* t : all)
+    if (t && t->shape[0] > 1 && t->stride[0] > (int64_t)1 << 27) return true;
+  return false;
+}
+// Elements of a row a lane has: what is kept of them fits the registers of two waves a SIMD.
+constexpr int FORWARD_ELEMS = 24;
+static constexpr int back_elems(bool post) { return post ? 16 : 24; }
+static int row_threads(int lg) { return std::max(256, 1 << lg); }
+// The workgroups of a backward pass: two waves a SIMD, which its registers allow.
+static int back_groups(int64_t R, int lg) {
+  const int threads = row_threads(lg);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(R, threads >> lg), (int64_t)device_cu_count() * (512 / threads)));
+}
+template <int N>
+struct Num { static constexpr int value = N; };
+// f(Num<nch>()), nch chunks of T being at most MOST elements.
+template <class T, int MOST, int N = 1, class F>
+static void with_chunks(int nch, F f) {
+  if constexpr ((N + 1) * Traits<T>::VEC <= MOST) {
+    if (nch > N) return with_chunks<T, MOST, N + 1>(nch, f);
+  }
+  f(Num<N>());
+}
+template <class F>
+static void with_type(int dtype, F f) {
+  if (dtype == MABA_F32) return f(F32());
+  if (dtype == MABA_BF16) return f(Bf16());
+  return f(Fp16());
+}
+
+}  // namespace rowvec
+}  // namespace maba
+
+using namespace maba;
+using namespace maba::rowvec;
+using ffn::check_out;
+using ffn::check_rows;
+using ffn::check_vec;
+using ffn::overlap;
+
+extern "C" int maba_hip_dropout(const maba_tensor* x, double p, const int64_t* seed, uint32_t stream_id, maba_tensor* out,
+                                void* stream) {
+  const char* who = "dropout";
+  int rc = check_float_rows(x, who);
+  if (!rc) rc = check_drop(who, p, seed);
+  if (!rc) rc = check_rows(x, who, "x", x->dtype, -1, -1);
+  if (!rc) rc = check_out(out, who, "out", x->dtype, x->shape[0], x->shape[1]);
+  if (rc) return rc;
+  if (overlap(x, out) && !same_place(x, out)) return fail(MABA_ERR_INVALID, "%s: x and out overlap", who);
+  DropArgs a = {x->data, out->data, x->stride[0], out->stride[0], x->shape[0], (int)x->shape[1], 0, make_drop(p, seed, stream_id)};
+  if (a.R == 0) return MABA_OK;
+  const int64_t chunks = ceil_div(a.C, chunk_elems(x->dtype));
+  while (a.lg < 8 && chunks > (int64_t)4 << a.lg) ++a.lg;
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(a.R, 256 >> a.lg), 65536));
+  auto k = x->dtype == MABA_F32 ? dropout_kernel<F32> : x->dtype == MABA_BF16 ? dropout_kernel<Bf16> : dropout_kernel<Fp16>;
+  hipLaunchKernelGGL(k, grid, dim3(256), 0, (hipStream_t)stream, a);
+  return check_launch(who);
+}
+
+extern "C" int maba_hip_residual_norm(const maba_tensor* x, const maba_tensor* y, const maba_tensor* weight,
+                                      const maba_tensor* post_weight, const maba_tensor* gate, float scale, double p,
+                                      const int64_t* seed, uint32_t stream_id, float eps, maba_tensor* x_out, maba_tensor* h,
+                                      void* stream) {
+  const char* who = "residual_norm";
+  int rc = check_float_rows(x, who);
+  if (!rc) rc = check_drop(who, p, seed);
+  if (!rc) rc = check_rows(x, who, "x", x->dtype, -1, -1);
+  if (rc) return rc;
+  const int64_t R = x->shape[0], C = x->shape[1];
+  const int dt = x->dtype;
+  if (!y && (post_weight || gate || x_out)) return fail(MABA_ERR_INVALID, "%s: post_weight, gate and x_out go with y", who);
+  if (!weight != !h) return fail(MABA_ERR_INVALID, "%s: weight and h go together", who);
+  if (!h && !x_out) return fail(MABA_ERR_INVALID, "%s: nothing to compute", who);
+  if (y) rc = check_rows(y, who, "y", dt, R, C);
+  if (!rc && weight) rc = check_vec(weight, who, "weight", dt, C);
+  if (!rc && post_weight) rc = check_vec(post_weight, who, "post_weight", dt, C);
+  if (!rc && gate) rc = check_vec(gate, who, "gate", dt, C);
+  if (!rc && x_out) rc = check_out(x_out, who, "x_out", dt, R, C);
+  if (!rc && h) rc = check_out(h, who, "h", dt, R, C);
+  if (rc) return rc;
+  // x_out may be x itself: a lane reads all it needs of a row before it writes
+  if (overlap(h, x) || overlap(h, y) || overlap(h, x_out) || overlap(x_out, y) || (overlap(x_out, x) && !same_place(x_out, x)))
+    return fail(MABA_ERR_INVALID, "%s: tensors overlap", who);
+  if (C > MAX_WIDTH) return fail(MABA_ERR_UNSUPPORTED, "%s: at most %d channels", who, MAX_WIDTH);
+  const Geometry geo = row_geometry(C, chunk_elems(dt), FORWARD_ELEMS, far_rows({x, y, x_out, h}));
+  BoundaryArgs a = {x->data, y ? y->data : nullptr, weight ? weight->data : nullptr, post_weight ? post_weight->data : nullptr,
+                    gate ? gate->data : nullptr, x_out ? x_out->data : nullptr, h ? h->data : nullptr,
+                    x->stride[0], y ? y->stride[0] : 0, x_out ? x_out->stride[0] : 0, h ? h->stride[0] : 0, R, (int)C, geo.lg,
+                    scale, eps, make_drop(p, seed, stream_id)};
+  if (R == 0) return MABA_OK;
+  const int threads = row_threads(geo.lg);
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(R, threads >> geo.lg), (int64_t)device_cu_count() * 8));
+  with_type(dt, [&](auto type) {
+    typedef decltype(type) T;
+    with_chunks<T, FORWARD_ELEMS>(geo.nch, [&](auto n) {
+      hipLaunchKernelGGL((boundary_kernel<T, decltype(n)::value>), grid, dim3(threads), 0, (hipStream_t)stream, a);
+    });
+  });
+  return check_launch(who);
+}
+
+extern "C" size_t maba_hip_residual_norm_backward_workspace_size(const maba_tensor* x_out, int grads) {
+  if (!x_out || x_out->ndim != 2 || x_out->shape[1] < 1 || !is_float_dt(x_out->dtype) || !(grads & 7)) return 0;
+  if (x_out->shape[1] > MAX_WIDTH) return 0;
+  int groups = 0;                                  // the most that any call on these rows has
+  for (bool post : {false, true})
+    groups = std::max(groups, back_groups(x_out->shape[0],
+                                          row_geometry(x_out->shape[1], chunk_elems(x_out->dtype), back_elems(post), true).lg));
+  return (size_t)groups * __builtin_popcount(grads & 7) * x_out->shape[1] * sizeof(float);
+}
+
+extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const maba_tensor* dh, const maba_tensor* x_out,
+                                               const maba_tensor* y, const maba_tensor* weight, const maba_tensor* post_weight,
+                                               const maba_tensor* gate, float scale, double p, const int64_t* seed,
+                                               uint32_t stream_id, float eps, maba_tensor* dx, maba_tensor* dy,
+                                               maba_tensor* dweight, maba_tensor* dpost_weight, maba_tensor* dgate,
+                                               void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "residual_norm_backward";
+  int rc = check_float_rows(x_out, who);
+  if (!rc) rc = check_drop(who, p, seed);
+  if (!rc) rc = check_rows(x_out, who, "x_out", x_out->dtype, -1, -1);
+  if (rc) return rc;
+  const int64_t R = x_out->shape[0], C = x_out->shape[1];
+  const int dt = x_out->dtype;
+  if (!dx_out && !dh) return fail(MABA_ERR_INVALID, "%s: dx_out or dh is required", who);
+  if (dh && !weight) return fail(MABA_ERR_INVALID, "%s: dh goes with weight", who);
+  if (!y && (post_weight || dpost_weight || dgate)) return fail(MABA_ERR_INVALID, "%s: post_weight and its and gate's gradients go with y", who);
+  if ((dpost_weight && !post_weight) || (dgate && !gate) || (dweight && !weight))
+    return fail(MABA_ERR_INVALID, "%s: a gradient of a missing parameter", who);
+  for (const auto& t : {std::make_pair(dx_out, "dx_out"), std::make_pair(dh, "dh"), std::make_pair(y, "y")})
+    if (!rc && t.first) rc = check_rows(t.first, who, t.second, dt, R, C);
+  for (const auto& t : {std::make_pair(weight, "weight"), std::make_pair(post_weight, "post_weight"), std::make_pair(gate, "gate"),
+                        std::make_pair((const maba_tensor*)dweight, "dweight"),
+                        std::make_pair((const maba_tensor*)dpost_weight, "dpost_weight"),
+                        std::make_pair((const maba_tensor*)dgate, "dgate")})
+    if (!rc && t.first) rc = check_vec(t.first, who, t.second, dt, C);
+  if (!rc && dx) rc = check_out(dx, who, "dx", dt, R, C);
+  if (!rc && dy) rc = check_out(dy, who, "dy", dt, R, C);
+  if (rc) return rc;
+  maba_tensor* outs[] = {dx, dy, dweight, dpost_weight, dgate};
+  for (int i = 0; i < 5; ++i) {
+    for (const maba_tensor* in : {dx_out, dh, x_out, y, weight, post_weight, gate})
+      if (overlap(outs[i], in)) return fail(MABA_ERR_INVALID, "%s: an output overlaps an input", who);
+    for (int j = 0; j < i; ++j)
+      if (overlap(outs[i], outs[j])) return fail(MABA_ERR_INVALID, "%s: outputs overlap", who);
+  }
+  if (C > MAX_WIDTH) return fail(MABA_ERR_UNSUPPORTED, "%s: at most %d channels", who, MAX_WIDTH);
+  const Geometry geo = row_geometry(C, chunk_elems(dt), back_elems(post_weight), far_rows({dx_out, dh, x_out, y, dx, dy}));
+  const int grads = (dweight ? GRAD_W : 0) | (dgate ? GRAD_GATE : 0) | (dpost_weight ? GRAD_POST : 0);
+  if (!grads && !dx && !dy) return MABA_OK;
+  const int groups = back_groups(R, geo.lg), n = __builtin_popcount(grads);
+  rc = ffn::check_workspace(who, workspace, workspace_bytes, (size_t)groups * n * C * sizeof(float));
+  if (rc) return rc;
+  const bool need_y = post_weight || dgate;
+  BoundaryBackArgs a = {dx_out ? dx_out->data : nullptr, dh ? dh->data : nullptr, x_out->data, need_y ? y->data : nullptr,
+                        weight ? weight->data : nullptr, post_weight ? post_weight->data : nullptr, gate ? gate->data : nullptr,
+                        dx ? dx->data : nullptr, dy ? dy->data : nullptr, (float*)workspace,
+                        dx_out ? dx_out->stride[0] : 0, dh ? dh->stride[0] : 0, x_out->stride[0], y ? y->stride[0] : 0,
+                        dx ? dx->stride[0] : 0, dy ? dy->stride[0] : 0, R, (int)C, geo.lg, grads, scale, eps,
+                        make_drop(p, seed, stream_id)};
+  if (R > 0) {
+    const int threads = row_threads(geo.lg);
+    const size_t lds = grads ? (size_t)(post_weight ? 3 : 2) * threads * chunk_elems(dt) * sizeof(float) : 0;
+    with_type(dt, [&](auto type) {
+      typedef decltype(type) T;
+      auto run = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(groups), dim3(threads), lds, (hipStream_t)stream, a);
+      };
+      if (post_weight) with_chunks<T, back_elems(true)>(geo.nch, [&](auto n) { run(boundary_back_kernel<T, decltype(n)::value, true>); });
+      else with_chunks<T, back_elems(false)>(geo.nch, [&](auto n) { run(boundary_back_kernel<T, decltype(n)::value, false>); });
+    });
+    rc = check_launch(who);
+    if (rc) return rc;
+  }
+  if (grads) {
+    ColumnsArgs c = {(const float*)workspace, {}, {}, R > 0 ? groups : 0, n, (int)C};
+    int k = 0;
+    if (dweight) { c.out[k] = dweight->data; c.factor[k++] = 1.f; }
+    if (dgate) { c.out[k] = dgate->data; c.factor[k++] = scale; }
+    if (dpost_weight) { c.out[k] = dpost_weight->data; c.factor[k++] = 1.f; }
+    auto f = dt == MABA_F32 ? columns_kernel<F32> : dt == MABA_BF16 ? columns_kernel<Bf16> : columns_kernel<Fp16>;
+    hipLaunchKernelGGL(f, dim3((unsigned)ceil_div(C, 64), n), dim3(1024), 0, (hipStream_t)stream, c);
+    return check_launch(who);
+  }
+  return MABA_OK;
+}

@@ -1,0 +1,197 @@
+// Rows of bf16, fp16 or fp32 elements in 16-byte chunks at any alignment of an element (global memory takes unaligned
+// vector accesses), sums over the lanes that share a row, and the generator behind dropout.
+#pragma once
+
+#include "ffn_common.h"
+
+namespace maba {
+namespace rowvec {
+
+using ffn::u32x4;
+using ffn::u32x4_any;
+using ffn::Bf16;
+using ffn::Fp16;
+typedef u32x4 u32x4_any4 __attribute__((aligned(4)));
+
+struct F32 { static constexpr int CODE = MABA_F32; };
+template <class T> struct Traits { typedef uint16_t elem; static constexpr int VEC = 8; };
+template <> struct Traits<F32> { typedef float elem; static constexpr int VEC = 4; };
+
+// The elements of a chunk in fp32, and back with one rounding to nearest even.
+template <class T>
+__device__ __forceinline__ void unpack(u32x4 u, float (&v)[Traits<T>::VEC]) {
+  if constexpr (T::CODE == MABA_F32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(u[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = T::up(u[i] & 0xffffu);
+      v[2 * i + 1] = T::CODE == MABA_BF16 ? __uint_as_float(u[i] & 0xffff0000u) : T::up(u[i] >> 16);
+    }
+  }
+}
+template <class T>
+__device__ __forceinline__ u32x4 pack(const float (&v)[Traits<T>::VEC]) {
+  u32x4 u;
+  if constexpr (T::CODE == MABA_F32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = T::down(v[2 * i]) | (T::down(v[2 * i + 1]) << 16);
+  }
+  return u;
+}
+
+// The chunk `off` bytes behind `base`, of which `left` elements belong to the row; the rest are zeros that are not read, or
+// not written.  `base` is the same in all lanes of a wave: it stays in scalar registers, and an address costs a lane one.
+template <class T>
+__device__ __forceinline__ u32x4 load_chunk(const void* base, uint32_t off, int left) {
+  constexpr int V = Traits<T>::VEC;
+  const auto* q = (const typename Traits<T>::elem*)((const char*)base + off);
+  u32x4 u = {0, 0, 0, 0};
+  if (left >= V) {
+    if constexpr (V == 4) u = *(const u32x4_any4*)q;
+    else u = *(const u32x4_any*)q;
+  } else if (left > 0) {
+#pragma unroll
+    for (int i = 0; i < V - 1; ++i) {
+      if (i >= left) continue;
+      if constexpr (V == 4) u[i] = __float_as_uint(q[i]);
+      else u[i >> 1] |= (uint32_t)q[i] << (16 * (i & 1));
+    }
+  }
+  return u;
+}
+template <class T>
+__device__ __forceinline__ void store_chunk(void* base, uint32_t off, int left, u32x4 u) {
+  constexpr int V = Traits<T>::VEC;
+  auto* q = (typename Traits<T>::elem*)((char*)base + off);
+  if (left >= V) {
+    if constexpr (V == 4) *(u32x4_any4*)q = u;
+    else *(u32x4_any*)q = u;
+  } else if (left > 0) {
+#pragma unroll
+    for (int i = 0; i < V - 1; ++i) {
+      if (i >= left) continue;
+      if constexpr (V == 4) q[i] = __uint_as_float(u[i]);
+      else q[i] = (uint16_t)(u[i >> 1] >> (16 * (i & 1)));
+    }
+  }
+}
+
+// Rows of a tensor as a wave goes through them: `at` is where chunk 0 of the wave's first row is, `off` how far behind it
+// this lane's is.
+template <class T>
+struct Walk {
+  char* p;
+  int64_t stride;          // bytes
+  uint32_t off;
+  __device__ __forceinline__ Walk(const void* q, int64_t ld, int l, int sub)
+      : p((char*)q), stride(ld * (int64_t)sizeof(typename Traits<T>::elem)), off((uint32_t)(sub * stride) + 16 * l) {}
+  __device__ __forceinline__ char* at(int64_t row, int chunk) const { return p + row * stride + 16 * (int64_t)chunk; }
+};
+
+// A row's lanes: 2^lg of them, lane l of which holds the chunks l, l + 2^lg, ...  Rows narrower than a wave share it.
+// `most` is how many elements a lane may have; far: the rows that share a wave would be further apart than 32 bits of bytes tell.
+constexpr int MAX_LG = 9, MAX_WIDTH = 16 << MAX_LG;
+struct Geometry {
+  int lg, nch;
+};
+inline Geometry row_geometry(int64_t C, int vec, int most, bool far) {      // C <= MAX_WIDTH, most >= 16
+  const int64_t chunks = ceil_div(C, vec);
+  int lg = far ? 6 : 4;
+  while (chunks > (int64_t)(most / vec) << lg) ++lg;
+  return {lg, (int)ceil_div(chunks, (int64_t)1 << lg)};
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+  return v + __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+// The sums of v over the 2^lg lanes of a row (lg >= 4), the same bits in each of them.  Rows of more than one wave meet in
+// `red` [2][N][waves]; every thread of the workgroup takes part, and the two halves take turns, so that one barrier a
+// sum is enough.
+template <int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], int lg, float* red, int& turn) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    v[n] = dpp_add<0xb1>(v[n]);       // lane ^ 1
+    v[n] = dpp_add<0x4e>(v[n]);       // lane ^ 2
+    v[n] = dpp_add<0x141>(v[n]);      // the other four of eight
+    v[n] = dpp_add<0x140>(v[n]);      // the other eight of sixteen
+  }
+  if (lg > 4)
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] += __shfl_xor(v[n], 16);
+  if (lg > 5)
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] += __shfl_xor(v[n], 32);
+  if (lg > 6) {
+    const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, per = 1 << (lg - 6);
+    float* r = red + turn * N * waves;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int n = 0; n < N; ++n) r[n * waves + wave] = v[n];
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const float* q = r + n * waves + (wave & ~(per - 1));
+      float s = 0.f;
+      for (int i = 0; i < per; ++i) s += q[i];
+      v[n] = s;
+    }
+    turn ^= 1;
+  }
+}
+
+// ---------------------------------------------------------------- dropout
+
+// Element (row, column) is dropped where its random word is below p * 2^32.  The words are those of Philox4x32 (Salmon,
+// Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011): a block cipher of the counter
+// (column / 4, row, stream) under the seed, whose four output words serve four neighbouring columns.  So any part of the
+// mask can be made anywhere, in any order, and it is never stored.  Seven rounds, the fewest that pass the statistical
+// tests in that paper: ten cost half as much again of what bounds a pass over 16-bit elements next to its traffic.
+struct Drop {
+  const uint64_t* seed;
+  uint32_t below, stream;
+  float keep;              // 1 / (1 - p)
+  int mode;                // 0 nothing is dropped, 1 as above, 2 everything is (p = 1)
+};
+inline Drop make_drop(double p, const void* seed, uint32_t stream) {
+  const double t = __builtin_nearbyint(p * 4294967296.0);       // p is at least 0 and at most 1
+  if (t <= 0) return {nullptr, 0, 0, 1.f, 0};
+  if (p >= 1.0) return {nullptr, 0, 0, 0.f, 2};
+  return {(const uint64_t*)seed, (uint32_t)(t < 4294967295.0 ? t : 4294967295.0), stream, (float)(1.0 / (1.0 - p)), 1};
+}
+
+__device__ __forceinline__ u32x4 philox(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1) {
+#pragma unroll
+  for (int i = 0; i < 7; ++i) {
+    const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c1 = (uint32_t)b;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c3 = (uint32_t)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return u32x4{c0, c1, c2, c3};
+}
+// v where it is kept, times 1 / (1 - p); zero, whatever v is, where it is dropped.  `at` is a multiple of four.
+template <int V>
+__device__ __forceinline__ void drop_chunk(float (&v)[V], const Drop& d, uint64_t key, int64_t row, int at) {
+  if (d.mode == 0) return;
+#pragma unroll
+  for (int q = 0; q < V / 4; ++q) {
+    u32x4 w = {0, 0, 0, 0};
+    if (d.mode == 1)
+      w = philox((uint32_t)(at / 4 + q), (uint32_t)row, (uint32_t)(row >> 32), d.stream, (uint32_t)key, (uint32_t)(key >> 32));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[4 * q + e] = d.mode == 1 && w[e] >= d.below ? v[4 * q + e] * d.keep : 0.f;
+  }
+}
+
+}  // namespace rowvec
+}  // namespace maba

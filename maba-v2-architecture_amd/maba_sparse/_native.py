@@ -78,6 +78,10 @@ EXPORTED_SYMBOLS = (
     "maba_hip_linear_epilogue_backward",
     "maba_hip_checkpoint_pack",
     "maba_hip_checkpoint_unpack",
+    "maba_hip_dropout",
+    "maba_hip_residual_norm",
+    "maba_hip_residual_norm_backward_workspace_size",
+    "maba_hip_residual_norm_backward",
 )
 
 
@@ -104,6 +108,7 @@ def _declare(lib) -> None:
     T = ctypes.POINTER(MabaTensor)
     TA = ctypes.POINTER(T)   # array of descriptor pointers
     vp, i, f, i64, sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64, ctypes.c_size_t
+    d, u32 = ctypes.c_double, ctypes.c_uint32
     sig = {
         "maba_hip_last_error": ([], ctypes.c_char_p),
         "maba_hip_abi_version": ([], i),
@@ -147,6 +152,11 @@ def _declare(lib) -> None:
         "maba_hip_linear_epilogue_backward": ([vp, vp, vp, vp, vp, i, vp, vp, vp, vp, vp, vp, sz, vp], i),
         "maba_hip_checkpoint_pack": ([vp, vp, vp, vp], i),
         "maba_hip_checkpoint_unpack": ([vp, vp, vp, vp], i),
+        # the block boundary and dropout
+        "maba_hip_dropout": ([vp, d, vp, u32, vp, vp], i),
+        "maba_hip_residual_norm": ([vp, vp, vp, vp, vp, f, d, vp, u32, f, vp, vp, vp], i),
+        "maba_hip_residual_norm_backward_workspace_size": ([vp, i], sz),
+        "maba_hip_residual_norm_backward": ([vp] * 7 + [f, d, vp, u32, f] + [vp] * 6 + [sz, vp], i),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)

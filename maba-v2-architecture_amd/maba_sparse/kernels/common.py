@@ -548,3 +548,96 @@ def ref_linear_epilogue_backward(dy, x, weight, bias=None, activation: str = "no
     dbias = dz.sum(0).to(dt) if needs[2] and bias is not None else None
     dgate = (d * a).sum(0).to(dt) if needs[3] and gate is not None else None
     return dx, dw, dbias, dgate
+
+
+# ----------------------------------------------------------------------------- the block boundary and dropout
+
+
+def philox_words(rows: int, cols: int, seed, stream: int = 0) -> torch.Tensor:
+    """The random words of dropout, int64 ``[rows, cols]`` in ``[0, 2^32)``: word ``c % 4`` of Philox4x32 with seven rounds
+    (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011), counter ``(c // 4, r mod 2^32,
+    r // 2^32, stream)``, key ``seed`` (low word first)."""
+    low, dev = 0xFFFFFFFF, seed.device
+    seed = seed.reshape(())
+    r = torch.arange(rows, device=dev).unsqueeze(1)
+    c = [torch.arange(-(-cols // 4), device=dev).unsqueeze(0), r & low, r >> 32, torch.full((1, 1), stream, device=dev)]
+    k0, k1 = seed & low, (seed >> 32) & low
+    for _ in range(7):
+        a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57          # modulo 2^64: the shift's sign bits are masked off
+        c = [((b >> 32) & low) ^ c[1] ^ k0, b & low, ((a >> 32) & low) ^ c[3] ^ k1, a & low]
+        k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
+    return torch.stack(torch.broadcast_tensors(*c), dim=-1).reshape(rows, -1)[:, :cols]
+
+
+def _dropped(v, p, seed, stream):
+    """``v [rows, cols]`` with dropout applied: a dropped element is 0 whatever it was."""
+    below = round(p * 2 ** 32)
+    if below == 0:
+        return v
+    zero = torch.zeros((), dtype=v.dtype, device=v.device)
+    if p >= 1:
+        return torch.where(torch.zeros((), dtype=torch.bool, device=v.device), v, zero)
+    return torch.where(philox_words(*v.shape, seed, stream) >= min(below, 2 ** 32 - 1), v * (1 / (1 - p)), zero)
+
+
+def ref_dropout(x, p, seed=None, stream: int = 0, **kwargs: Any):
+    """Elements of ``x [..., C]`` zeroed with probability ``p``, the others times ``1 / (1 - p)``, in fp32 (fp64 for fp64
+    inputs) and rounded once.  Rows are counted over the leading dimensions."""
+    ct = torch.promote_types(x.dtype, torch.float32)
+    return _dropped(x.to(ct).reshape(-1, x.shape[-1]), p, seed, stream).to(x.dtype).reshape(x.shape)
+
+
+def _rows32(t):
+    return None if t is None else t.to(torch.promote_types(t.dtype, torch.float32)).reshape(-1, t.shape[-1])
+
+
+def _one(t, like):
+    return torch.ones((), dtype=like.dtype, device=like.device) if t is None else t.to(like.dtype)
+
+
+def ref_residual_norm(x, y=None, weight=None, post_weight=None, gate=None, scale: float = 1.0, p: float = 0.0, seed=None,
+                      stream: int = 0, eps: float = 1e-6, **kwargs: Any):
+    """``(x_out, h)``: ``x_out = x + scale * gate * dropout(z)`` with ``z = RMSNorm(y) * post_weight`` (``y`` without
+    post_weight; ``x_out`` is ``x`` without ``y``) and ``h = RMSNorm(x_out) * weight`` (None without weight); reference
+    model.py:11-22, 92-128.  In fp32 (fp64 for fp64 inputs), each result rounded once."""
+    xf, yf, out = _rows32(x), _rows32(y), x
+    if y is not None:
+        z = yf
+        if post_weight is not None:
+            z = yf * torch.rsqrt((yf * yf).mean(-1, keepdim=True) + eps) * post_weight.to(yf.dtype)
+        xf = xf + scale * (_one(gate, yf) * _dropped(z, p, seed, stream))
+        out = xf.to(x.dtype).reshape(x.shape)
+    if weight is None:
+        return out, None
+    h = xf * torch.rsqrt((xf * xf).mean(-1, keepdim=True) + eps) * weight.to(xf.dtype)
+    return out, h.to(x.dtype).reshape(x.shape)
+
+
+def ref_residual_norm_backward(dx_out, dh, x_out, y=None, weight=None, post_weight=None, gate=None, scale: float = 1.0,
+                               p: float = 0.0, seed=None, stream: int = 0, eps: float = 1e-6,
+                               needs=(True, True, True, True, True), **kwargs: Any):
+    """``(dx, dy, dweight, dpost_weight, dgate)`` of ``ref_residual_norm`` (None where ``needs`` says so, or where there is
+    no such input) for the gradients of ``x_out`` and ``h``, either of which may be None."""
+    dt, shape = x_out.dtype, x_out.shape
+    d = _rows32(dx_out) if dx_out is not None else torch.zeros_like(_rows32(x_out))
+    yf, one = _rows32(y), _one(None, d)
+    dw = dpw = dg = None
+    if dh is not None:
+        g, xf = _rows32(dh), _rows32(x_out)
+        r = torch.rsqrt((xf * xf).mean(-1, keepdim=True) + eps)
+        xh, gw = xf * r, g * weight.to(g.dtype)
+        dw = (g * xh).sum(0)
+        d = d + r * (gw - xh * (gw * xh).mean(-1, keepdim=True))
+    elif weight is not None:
+        dw = torch.zeros(shape[-1], dtype=d.dtype, device=d.device)
+    m = _dropped(d, p, seed, stream)                          # the product of the mask and either side
+    rp = torch.rsqrt((yf * yf).mean(-1, keepdim=True) + eps) if post_weight is not None else one
+    if gate is not None and needs[4]:
+        dg = scale * (m * (yf * rp * _one(post_weight, d))).sum(0)
+    dz = scale * (_one(gate, d) * m)
+    if post_weight is not None:
+        yh, wp = yf * rp, post_weight.to(d.dtype)
+        dpw = (dz * yh).sum(0)
+        dz = rp * (dz * wp - yh * (dz * wp * yh).mean(-1, keepdim=True))
+    grads = (d.reshape(shape), dz.reshape(shape), dw, dpw, dg)
+    return tuple(g.to(dt) if n and g is not None else None for g, n in zip(grads, needs))

@@ -40,6 +40,7 @@ import torch
 
 from maba_sparse import _native
 from maba_sparse._native import HipLibraryMissing
+from maba_sparse.kernels import block_ends as _be
 from maba_sparse.kernels import common as _c
 from maba_sparse.kernels import cpu_dgda as _cpu
 from maba_sparse.kernels import feed_forward as _ff
@@ -64,6 +65,9 @@ _KERNEL_REGISTRY: Dict[str, Dict[str, Callable]] = {
         "linear_epilogue_backward": _c.ref_linear_epilogue_backward,
         "checkpoint_pack": _c.ref_checkpoint_pack,
         "checkpoint_unpack": _c.ref_checkpoint_unpack,
+        "dropout": _c.ref_dropout,
+        "residual_norm": _c.ref_residual_norm,
+        "residual_norm_backward": _c.ref_residual_norm_backward,
     },
     # host cores: the chunked DGDA of the reference's CPU backend (cpu_dgda.py), the rest as
     # the reference ops in torch
@@ -84,6 +88,9 @@ _KERNEL_REGISTRY: Dict[str, Dict[str, Callable]] = {
         "linear_epilogue_backward": _c.ref_linear_epilogue_backward,
         "checkpoint_pack": _c.ref_checkpoint_pack,
         "checkpoint_unpack": _c.ref_checkpoint_unpack,
+        "dropout": _c.ref_dropout,
+        "residual_norm": _c.ref_residual_norm,
+        "residual_norm_backward": _c.ref_residual_norm_backward,
     },
     "hip": {},
     "xla": {},
@@ -455,6 +462,8 @@ class _FFNOps:
                 return _run(op, None, kwargs, self.backend)
         return _run(op, None, kwargs, self.backend)
 
+    run = _run
+
     def pack(self, x):
         return self._run("checkpoint_pack", x=x)
 
@@ -649,6 +658,127 @@ def dispatch_checkpoint_unpack(codes, scales, dtype: torch.dtype = torch.bfloat1
     return _run("checkpoint_unpack", codes.device, dict(codes=codes, scales=scales, dtype=dtype))
 
 
+# ----------------------------------------------------------------------------- the block boundary and dropout
+
+
+def _drop_args(x, p, seed, stream) -> None:
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"p must be in [0, 1], got {p}")
+    if not 0 <= stream < 2 ** 32:
+        raise ValueError(f"stream must be in [0, 2^32), got {stream}")
+    if 0.0 < p < 1.0:
+        if seed is None:
+            raise ValueError("dropout needs a seed: an int64 tensor of one element")
+        if seed.dtype != torch.int64:
+            raise TypeError(f"the seed must be int64, got {seed.dtype}")
+        if seed.numel() != 1:
+            raise ValueError(f"the seed must have one element, got {list(seed.shape)}")
+        if seed.device != x.device:
+            raise RuntimeError(f"Expected all tensors to be on the same device, but got {x.device} and {seed.device} for seed")
+
+
+def _channels(x, name: str = "x") -> None:
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"{name} must have a positive channel dimension, got {list(x.shape)}")
+
+
+def dispatch_dropout(x, p: float, seed=None, stream: int = 0) -> torch.Tensor:
+    """Elements of ``x [..., C]`` zeroed with probability ``p``, the others times ``1 / (1 - p)``.
+
+    The mask is never stored: it is a function of ``seed`` (an int64 tensor of one element on x's device, read when the
+    kernel runs), ``stream`` (an int in ``[0, 2^32)``: one for each place that drops under the same seed), the row
+    (counted over the leading dimensions) and the column; see ``common.philox_words``.  A dropped element is 0 whatever it
+    was.  A seed that is advanced in place after the backward pass, also inside a captured graph, gives every step
+    masks of its own.  Differentiable on every backend."""
+    _channels(x)
+    _ffn_same(x)
+    _drop_args(x, p, seed, stream)
+    if _wants_grad(x):
+        return _ff.guard_capture(_be.Dropout.apply(_FFNOps(x.device), p, stream, x, seed))
+    return _FFNOps(x.device).run("dropout", x=x, p=p, seed=seed, stream=stream)
+
+
+def _widest(*tensors):
+    """The tensors in the widest of their floating types."""
+    wide = None
+    for t in tensors:
+        if t is not None:
+            wide = t.dtype if wide is None else torch.promote_types(wide, t.dtype)
+    return tuple(t if t is None or t.dtype == wide else t.to(wide) for t in tensors)
+
+
+def _boundary_check(x, y, weight, post_weight, gate) -> None:
+    _channels(x)
+    _ffn_same(x, y=y, weight=weight, post_weight=post_weight, gate=gate)
+    _ffn_shape("y", y, x.shape)
+    for name, t in (("weight", weight), ("post_weight", post_weight), ("gate", gate)):
+        _ffn_shape(name, t, x.shape[-1:])
+
+
+def dispatch_residual_norm(x, y=None, weight=None, post_weight=None, gate=None, scale: float = 1.0, p: float = 0.0, seed=None,
+                           stream: int = 0, eps: float = 1e-6) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """The boundary between two sub-layers: ``(x_out, h)`` with
+
+    ``x_out = x + scale * gate * dropout(z)``, ``z = RMSNorm(y) * post_weight`` (``y`` itself without post_weight), and
+    ``h = RMSNorm(x_out) * weight`` (None without weight).
+
+    x and y ``[..., C]``, weight, post_weight and gate ``[C]`` of one dtype and device; all but x are optional, and without
+    y x_out is x itself.  ``p``, ``seed`` and ``stream`` as for ``dropout``.  Computed in fp32 and each result rounded once
+    (h from the unrounded x_out).  Differentiable on every backend, with x_out and (for post_weight or the gate's gradient)
+    y kept for it.  Under autocast the tensors are first cast to the widest of their types.  The HIP backend takes up to
+    8,192 channels."""
+    dtype = _autocast_dtype(x)
+    if dtype is not None:
+        x, y, weight, post_weight, gate = _widest(x, y, weight, post_weight, gate)
+    _boundary_check(x, y, weight, post_weight, gate)
+    _drop_args(x, p, seed, stream)
+    if y is None:
+        if post_weight is not None or gate is not None:
+            raise ValueError("post_weight and gate go with y")
+        if weight is None:
+            return x, None
+        p, seed, scale = 0.0, None, 1.0
+    ops = _FFNOps(x.device)
+    if _wants_grad(x, y, weight, post_weight, gate):
+        out = _be.ResidualNorm.apply(ops, scale, p, stream, eps, x, y, weight, post_weight, gate, seed)
+        if y is None:
+            return x, _ff.guard_capture(out)
+        return (_ff.guard_capture(out[0]), out[1]) if weight is not None else (_ff.guard_capture(out), None)
+    out = ops.run("residual_norm", x=x, y=y, weight=weight, post_weight=post_weight, gate=gate, scale=scale, p=p, seed=seed,
+                  stream=stream, eps=eps)
+    return (x, out[1]) if y is None else out
+
+
+def dispatch_residual_norm_backward(dx_out, dh, x_out, y=None, weight=None, post_weight=None, gate=None, scale: float = 1.0,
+                                    p: float = 0.0, seed=None, stream: int = 0, eps: float = 1e-6,
+                                    needs=(True, True, True, True, True)):
+    """``(dx, dy, dweight, dpost_weight, dgate)`` of ``residual_norm`` for the gradients of its results, either of which
+    may be None, each None where ``needs`` is false or there is no such input.  ``x_out`` is the forward's result (only its
+    shape and type count without ``dh``), ``y`` its input (not read without post_weight and without the gate's gradient).
+    No autograd takes part."""
+    first = dx_out if dx_out is not None else dh
+    if first is None:
+        raise ValueError("dx_out or dh is required")
+    _boundary_check(x_out, y, weight, post_weight, gate)
+    _ffn_same(x_out, dx_out=dx_out, dh=dh)
+    _ffn_shape("dx_out", dx_out, x_out.shape)
+    _ffn_shape("dh", dh, x_out.shape)
+    _drop_args(x_out, p, seed, stream)
+    if dh is not None and weight is None:
+        raise ValueError("dh goes with weight")
+    if len(needs) != 5:
+        raise ValueError(f"needs takes five flags (dx, dy, dweight, dpost_weight, dgate), got {needs!r}")
+    if y is None and (post_weight is not None or (gate is not None and needs[4])):
+        raise ValueError("post_weight and the gate's gradient need y")
+    with torch.no_grad():
+        return _FFNOps(x_out.device).run("residual_norm_backward", dx_out=dx_out, dh=dh, x_out=x_out, y=y, weight=weight,
+                                         post_weight=post_weight, gate=gate, scale=scale, p=p, seed=seed, stream=stream, eps=eps,
+                                         needs=tuple(needs))
+
+
+dropout = dispatch_dropout
+residual_norm = dispatch_residual_norm
+residual_norm_backward = dispatch_residual_norm_backward
 gated_ffn = dispatch_gated_ffn
 gated_ffn_backward = dispatch_gated_ffn_backward
 linear_epilogue = dispatch_linear_epilogue

@@ -423,6 +423,81 @@ def hip_checkpoint_unpack(codes, scales, dtype: torch.dtype = torch.bfloat16, **
     return out if codes.dim() == 2 else out.view(codes.shape)
 
 
+# ----------------------------------------------------------------------------- the block boundary and dropout
+
+
+def _seed_ptr(p: float, seed: Optional[torch.Tensor]) -> Optional[int]:
+    return seed.data_ptr() if 0 < p < 1 else None
+
+
+@register_kernel("hip", "dropout")
+def hip_dropout(x, p, seed=None, stream: int = 0, **kwargs: Any) -> torch.Tensor:
+    """Dropout with a mask from a counter (contract: ``common.ref_dropout``)."""
+    _no_grad_needed("dropout", x)
+    dev = N.require_device((x, seed), "dropout")
+    with N.on_device(dev):
+        x2, dx = N.rows_of(x)
+        out = torch.empty(x2.shape, dtype=x.dtype, device=dev)
+        N.check(N.load().maba_hip_dropout(dx, float(p), _seed_ptr(p, seed), stream, N.rows_desc(out), N.stream_ptr(dev)), "dropout")
+    return out if x.dim() == 2 else out.view(x.shape)
+
+
+@register_kernel("hip", "residual_norm")
+def hip_residual_norm(x, y=None, weight=None, post_weight=None, gate=None, scale: float = 1.0, p: float = 0.0, seed=None,
+                      stream: int = 0, eps: float = 1e-6, x_out=None, **kwargs: Any):
+    """``(x_out, h)`` in one launch (contract: ``common.ref_residual_norm``); ``x_out`` may be a buffer of x's shape whose
+    rows can be written in place, ``x`` itself among them."""
+    _no_grad_needed("residual_norm", x, y, weight, post_weight, gate)
+    dev = N.require_device((x, y, weight, post_weight, gate, seed, x_out), "residual_norm")
+    with N.on_device(dev):
+        (x2, dx), (_y, dy) = N.rows_of(x), N.rows_of(y)
+        weight, post_weight, gate = _vec(weight), _vec(post_weight), _vec(gate)
+        made = x_out
+        if y is not None and made is None:
+            made = torch.empty(x2.shape, dtype=x.dtype, device=dev)
+        m2, dm = N.rows_of(made) if y is not None else (None, None)
+        if m2 is not None and m2.data_ptr() != made.data_ptr():
+            raise ValueError("residual_norm: x_out's rows cannot be written in place")
+        h = torch.empty(x2.shape, dtype=x.dtype, device=dev) if weight is not None else None
+        if dm is not None or h is not None:
+            rc = N.load().maba_hip_residual_norm(dx, dy, N.rows_desc(weight), N.rows_desc(post_weight), N.rows_desc(gate), float(scale),
+                                                 float(p), _seed_ptr(p, seed), stream, float(eps), dm, N.rows_desc(h), N.stream_ptr(dev))
+            N.check(rc, "residual_norm")
+    if y is None:
+        made = x
+    if x.dim() == 2:
+        return made, h
+    return made.view(x.shape) if made is not x else x, h if h is None else h.view(x.shape)
+
+
+@register_kernel("hip", "residual_norm_backward")
+def hip_residual_norm_backward(dx_out, dh, x_out, y=None, weight=None, post_weight=None, gate=None, scale: float = 1.0,
+                               p: float = 0.0, seed=None, stream: int = 0, eps: float = 1e-6,
+                               needs=(True, True, True, True, True), **kwargs: Any):
+    """``(dx, dy, dweight, dpost_weight, dgate)`` (contract: ``dispatcher.dispatch_residual_norm_backward``)."""
+    _no_grad_needed("residual_norm_backward", dx_out, dh, x_out, y, weight, post_weight, gate)
+    dev = N.require_device((dx_out, dh, x_out, y, weight, post_weight, gate, seed), "residual_norm_backward")
+    with N.on_device(dev):
+        lib = N.load()
+        (_d, dd), (_h, ddh), (xo, dxo), (_y, dy_) = map(N.rows_of, (dx_out, dh, x_out, y))
+        weight, post_weight, gate = _vec(weight), _vec(post_weight), _vec(gate)
+        there = (True, True, weight is not None, post_weight is not None, gate is not None)
+        needs = tuple(bool(n) and t for n, t in zip(needs, there))
+        C = x_out.shape[-1]
+        outs = [torch.empty(s, dtype=x_out.dtype, device=dev) if n else None
+                for n, s in zip(needs, (xo.shape, xo.shape, (C,), (C,), (C,)))]
+        grads = needs[2] + 2 * needs[4] + 4 * needs[3]
+        ws = _workspace(lib.maba_hip_residual_norm_backward_workspace_size(dxo, grads), dev) if grads else None
+        rc = lib.maba_hip_residual_norm_backward(dd, ddh, dxo, dy_, N.rows_desc(weight), N.rows_desc(post_weight), N.rows_desc(gate),
+                                                 float(scale), float(p), _seed_ptr(p, seed), stream, float(eps),
+                                                 *map(N.rows_desc, outs), ws.data_ptr() if grads else None,
+                                                 ws.numel() if grads else 0, N.stream_ptr(dev))
+        N.check(rc, "residual_norm_backward")
+    if x_out.dim() != 2:
+        outs[:2] = [o if o is None else o.view(x_out.shape) for o in outs[:2]]
+    return tuple(outs)
+
+
 # ----------------------------------------------------------------------------- serving path
 # Entry points for a decode step whose per-step scalars (the cache position) live in device
 # memory, so that one captured HIP graph serves every position.  Not dispatcher ops: the
