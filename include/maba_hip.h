@@ -75,6 +75,8 @@
  *                                   sub-layer and the norm before the next, with dropout), and its
  *                                   gradients, which come from autograd there
  *   maba_hip_dropout                no counterpart: dropout whose mask is made from a counter
+ *   maba_hip_token_logprobs         no counterpart: log probabilities of given tokens, entropy and the
+ *                                   likeliest alternatives, and their gradient
  *   maba_hip_checkpoint_pack        no counterpart: the input that those two keep for their
  *                                   backward passes, in 8 bits
  */
@@ -497,6 +499,25 @@ int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const maba_tensor
                                     uint32_t stream_id, float eps, maba_tensor* dx, maba_tensor* dy,
                                     maba_tensor* dweight, maba_tensor* dpost_weight, maba_tensor* dgate,
                                     void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Log probabilities.  logits [M,V] or [B,L,V] (M = B L) f32, f16 or bf16, unit column stride, any other strides and
+ * alignment, V <= 2^28; targets int64 [M]; logp, entropy, lse f32 [M]; top_logp f32 and top_ids int64 [M,k], 1 <= k <=
+ * min(64, V), or both NULL.  With u = logits / temperature: lse = log sum exp(u), logp = u[target] - lse (0 where the
+ * target is negative, NaN where it is V or more), entropy of exp(u - lse), and the k largest with their log
+ * probabilities: by logit (NaN above all, -0 as +0), then the lower index.  A row of nothing but -inf has lse and log
+ * probabilities -inf and entropy 0; a row with NaN or +inf has NaN.  fp32 arithmetic.
+ *
+ * Backward: dlogp, dentropy, dlse f32 [M], any of which may be NULL (zeros); lse and entropy as the forward returned
+ * them; dlogits like logits (it may be logits itself).  A row of nothing but -inf has no gradient, and dlogp counts only
+ * where there is a target.
+ */
+int maba_hip_token_logprobs(const maba_tensor* logits, const maba_tensor* targets, double temperature,
+                            maba_tensor* logp, maba_tensor* entropy, maba_tensor* lse, maba_tensor* top_logp,
+                            maba_tensor* top_ids, void* stream);
+int maba_hip_token_logprobs_backward(const maba_tensor* dlogp, const maba_tensor* dentropy, const maba_tensor* dlse,
+                                     const maba_tensor* logits, const maba_tensor* targets, const maba_tensor* lse,
+                                     const maba_tensor* entropy, double temperature, maba_tensor* dlogits, void* stream);
 
 #ifdef __cplusplus
 }

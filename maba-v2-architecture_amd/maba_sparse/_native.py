@@ -82,6 +82,8 @@ EXPORTED_SYMBOLS = (
     "maba_hip_residual_norm",
     "maba_hip_residual_norm_backward_workspace_size",
     "maba_hip_residual_norm_backward",
+    "maba_hip_token_logprobs",
+    "maba_hip_token_logprobs_backward",
 )
 
 
@@ -152,7 +154,9 @@ def _declare(lib) -> None:
         "maba_hip_linear_epilogue_backward": ([vp, vp, vp, vp, vp, i, vp, vp, vp, vp, vp, vp, sz, vp], i),
         "maba_hip_checkpoint_pack": ([vp, vp, vp, vp], i),
         "maba_hip_checkpoint_unpack": ([vp, vp, vp, vp], i),
-        # the block boundary and dropout
+        # dropout, the block boundary and token log probabilities
+        "maba_hip_token_logprobs": ([vp, vp, d] + [vp] * 6, i),
+        "maba_hip_token_logprobs_backward": ([vp] * 7 + [d, vp, vp], i),
         "maba_hip_dropout": ([vp, d, vp, u32, vp, vp], i),
         "maba_hip_residual_norm": ([vp, vp, vp, vp, vp, f, d, vp, u32, f, vp, vp, vp], i),
         "maba_hip_residual_norm_backward_workspace_size": ([vp, i], sz),

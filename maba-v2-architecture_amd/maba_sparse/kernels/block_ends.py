@@ -64,3 +64,25 @@ class ResidualNorm(torch.autograd.Function):
                           weight=weight, post_weight=post_weight, gate=gate, seed=seed, needs=tuple(ctx.needs_input_grad[5:10]),
                           **ctx.args)
         return (None,) * 5 + tuple(out) + (None,)
+
+
+class TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ops, temperature, top, logits, targets):
+        ctx.ops, ctx.temperature = ops, temperature
+        ctx.set_materialize_grads(False)
+        logp, entropy, lse, top_logp, top_ids = ops.run("token_logprobs", logits=logits, targets=targets, temperature=temperature, top=top)
+        ctx.save_for_backward(logits, targets, lse, entropy)
+        if top:
+            ctx.mark_non_differentiable(top_logp, top_ids)
+        return logp, entropy, lse, top_logp, top_ids
+
+    @staticmethod
+    @_once
+    def backward(ctx, dlogp, dentropy, dlse, *_):
+        if dlogp is None and dentropy is None and dlse is None:
+            return (None,) * 5
+        logits, targets, lse, entropy = ctx.saved_tensors
+        d = ctx.ops.run("token_logprobs_backward", dlogp=dlogp, dentropy=dentropy, dlse=dlse, logits=logits, targets=targets, lse=lse,
+                        entropy=entropy, temperature=ctx.temperature)
+        return None, None, None, d, None

@@ -641,3 +641,46 @@ def ref_residual_norm_backward(dx_out, dh, x_out, y=None, weight=None, post_weig
         dz = rp * (dz * wp - yh * (dz * wp * yh).mean(-1, keepdim=True))
     grads = (d.reshape(shape), dz.reshape(shape), dw, dpw, dg)
     return tuple(g.to(dt) if n and g is not None else None for g, n in zip(grads, needs))
+
+
+# ----------------------------------------------------------------------------- token log probabilities
+
+
+def ref_token_logprobs(logits, targets, temperature: float = 1.0, top: int = 0, **kwargs: Any):
+    """``(logp, entropy, lse, top_logp, top_ids)`` of ``logits [..., V] / temperature`` (the last two None for ``top=0``), in
+    fp32 (fp64 for fp64 logits).  ``logp`` is 0 where the target is negative and NaN where it is V or more; a row of nothing
+    but -inf has lse and log probabilities -inf and entropy 0.  Ties among the ``top`` go to the lower index."""
+    x = logits.to(torch.promote_types(logits.dtype, torch.float32))
+    V, inv = x.shape[-1], 1 / temperature
+    zero, ninf = (torch.full((), c, dtype=x.dtype, device=x.device) for c in (0.0, -math.inf))
+    m = x.amax(-1, keepdim=True)
+    none = m == -math.inf
+    d = x - torch.where(none, zero, m)
+    e = torch.exp(d * inv)
+    log_s = torch.log(e.sum(-1, keepdim=True))
+    lp = torch.where(none, ninf, d * inv - log_s)
+    mean = (torch.where(e == 0, zero, d) * e).sum(-1, keepdim=True) / e.sum(-1, keepdim=True)
+    entropy = torch.where(none, zero, log_s - inv * mean)
+    lse = torch.where(none, ninf, m * inv + log_s)
+    t = targets.unsqueeze(-1)
+    logp = torch.where(t < 0, zero, torch.where(t >= V, zero / zero, lp.gather(-1, t.clamp(0, V - 1))))
+    top_logp = top_ids = None
+    if top:
+        top_ids = torch.sort(logits, dim=-1, descending=True, stable=True).indices[..., :top].contiguous()
+        top_logp = lp.gather(-1, top_ids)
+    return logp.squeeze(-1), entropy.squeeze(-1), lse.squeeze(-1), top_logp, top_ids
+
+
+def ref_token_logprobs_backward(dlogp, dentropy, dlse, logits, targets, lse, entropy, temperature: float = 1.0, **kwargs: Any):
+    """The logits' gradient of ``ref_token_logprobs`` for the gradients of logp, entropy and lse, any of which may be None."""
+    x = logits.to(torch.promote_types(logits.dtype, torch.float32))
+    inv, zero = 1 / temperature, torch.zeros((), dtype=x.dtype, device=x.device)
+    none, t = (lse == -math.inf).unsqueeze(-1), targets.unsqueeze(-1)
+    gl, gh, gz = (zero if g is None else g.to(x.dtype).unsqueeze(-1) for g in (dlogp, dentropy, dlse))
+    gl = torch.where((t < 0) | none, zero, torch.where(t >= x.shape[-1], zero / zero, gl))
+    lp = torch.where(none, torch.full((), -math.inf, dtype=x.dtype, device=x.device), x * inv - lse.unsqueeze(-1))
+    p = torch.exp(lp)
+    plogp = torch.where(p == 0, p, p * lp)
+    d = (gz - gl) * p - gh * (plogp + p * entropy.unsqueeze(-1))
+    d = d + torch.where(torch.arange(x.shape[-1], device=x.device) == t, gl, zero)
+    return (inv * d).to(logits.dtype)

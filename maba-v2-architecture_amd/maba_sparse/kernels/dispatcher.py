@@ -68,6 +68,8 @@ _KERNEL_REGISTRY: Dict[str, Dict[str, Callable]] = {
         "dropout": _c.ref_dropout,
         "residual_norm": _c.ref_residual_norm,
         "residual_norm_backward": _c.ref_residual_norm_backward,
+        "token_logprobs": _c.ref_token_logprobs,
+        "token_logprobs_backward": _c.ref_token_logprobs_backward,
     },
     # host cores: the chunked DGDA of the reference's CPU backend (cpu_dgda.py), the rest as
     # the reference ops in torch
@@ -91,6 +93,8 @@ _KERNEL_REGISTRY: Dict[str, Dict[str, Callable]] = {
         "dropout": _c.ref_dropout,
         "residual_norm": _c.ref_residual_norm,
         "residual_norm_backward": _c.ref_residual_norm_backward,
+        "token_logprobs": _c.ref_token_logprobs,
+        "token_logprobs_backward": _c.ref_token_logprobs_backward,
     },
     "hip": {},
     "xla": {},
@@ -776,6 +780,63 @@ def dispatch_residual_norm_backward(dx_out, dh, x_out, y=None, weight=None, post
                                          needs=tuple(needs))
 
 
+# ----------------------------------------------------------------------------- token log probabilities
+
+
+def _logprobs_check(logits, targets, temperature) -> None:
+    _channels(logits, "logits")
+    _ffn_same(logits)
+    if targets.dtype != torch.int64:
+        raise TypeError(f"targets must be int64, got {targets.dtype}")
+    if targets.device != logits.device:
+        raise RuntimeError(f"Expected all tensors to be on the same device, but got {logits.device} and {targets.device} for targets")
+    _ffn_shape("targets", targets, logits.shape[:-1])
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"temperature must be positive, got {temperature}")
+
+
+def dispatch_token_logprobs(logits, targets, temperature: float = 1.0, top: int = 0):
+    """``(logp, entropy, lse, top_logp, top_ids)`` of the distributions ``softmax(logits / temperature)``.
+
+    logits ``[..., V]``, targets int64 ``[...]``; logp (of the target), entropy and lse (the normaliser ``log sum exp``)
+    ``[...]``, and the ``top`` likeliest tokens with their log probabilities ``[..., top]``, likeliest first, ties by the
+    lower index (None for ``top=0``; the HIP backend takes up to 64).  fp32, for fp64 logits fp64.  A negative target
+    stands for none: its logp is 0 and has no gradient; one of V or more gives NaN, since a GPU call cannot refuse it.  Logits
+    of -inf have probability zero; a row of nothing else has lse and log probabilities -inf, entropy 0 and no gradient.
+    logp, entropy and lse are differentiable on every backend (the logits are kept for it), the alternatives are not."""
+    _logprobs_check(logits, targets, temperature)
+    if not 0 <= top <= logits.shape[-1]:
+        raise ValueError(f"top must be in [0, {logits.shape[-1]}], got {top}")
+    ops = _FFNOps(logits.device)
+    if _wants_grad(logits):
+        out = _be.TokenLogprobs.apply(ops, temperature, top, logits, targets)
+        _ff.guard_capture(out[0])
+        return out
+    return ops.run("token_logprobs", logits=logits, targets=targets, temperature=temperature, top=top)
+
+
+def dispatch_token_logprobs_backward(dlogp, dentropy, dlse, logits, targets, lse, entropy, temperature: float = 1.0):
+    """The logits' gradient of ``token_logprobs`` for the gradients of logp, entropy and lse ``[...]``, any of which may be
+    None; lse and entropy as the forward returned them.  No autograd takes part."""
+    _logprobs_check(logits, targets, temperature)
+    wide = torch.promote_types(logits.dtype, torch.float32)
+    for name, t in (("dlogp", dlogp), ("dentropy", dentropy), ("dlse", dlse), ("lse", lse), ("entropy", entropy)):
+        if t is None:
+            continue
+        _ffn_shape(name, t, logits.shape[:-1])
+        if t.dtype != wide:
+            raise TypeError(f"{name} must be {wide}, got {t.dtype}")
+        if t.device != logits.device:
+            raise RuntimeError(f"Expected all tensors to be on the same device, but got {logits.device} and {t.device} for {name}")
+    if dlogp is None and dentropy is None and dlse is None:
+        raise ValueError("one of dlogp, dentropy and dlse is required")
+    with torch.no_grad():
+        return _FFNOps(logits.device).run("token_logprobs_backward", dlogp=dlogp, dentropy=dentropy, dlse=dlse, logits=logits,
+                                          targets=targets, lse=lse, entropy=entropy, temperature=temperature)
+
+
+token_logprobs = dispatch_token_logprobs
+token_logprobs_backward = dispatch_token_logprobs_backward
 dropout = dispatch_dropout
 residual_norm = dispatch_residual_norm
 residual_norm_backward = dispatch_residual_norm_backward

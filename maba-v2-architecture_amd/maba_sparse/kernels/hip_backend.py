@@ -498,6 +498,52 @@ def hip_residual_norm_backward(dx_out, dh, x_out, y=None, weight=None, post_weig
     return tuple(outs)
 
 
+# ----------------------------------------------------------------------------- token log probabilities
+
+
+def _logit_rows(t):
+    """``t [..., V]`` as [M, V] or [B, L, V] with unit column stride, a view where the strides allow it."""
+    if t.dim() not in (2, 3):
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+@register_kernel("hip", "token_logprobs")
+def hip_token_logprobs(logits, targets, temperature: float = 1.0, top: int = 0, **kwargs: Any):
+    """``(logp, entropy, lse, top_logp, top_ids)`` in one launch (contract: ``common.ref_token_logprobs``)."""
+    _no_grad_needed("token_logprobs", logits)
+    dev = N.require_device((logits, targets), "token_logprobs")
+    with N.on_device(dev):
+        x, t = _logit_rows(logits), targets.reshape(-1).contiguous()
+        M = t.numel()
+        out = torch.empty(3, M, dtype=torch.float32, device=dev)
+        logp, entropy, lse = out.unbind(0)
+        top_logp = torch.empty(M, top, dtype=torch.float32, device=dev) if top else None
+        top_ids = torch.empty(M, top, dtype=torch.long, device=dev) if top else None
+        rc = N.load().maba_hip_token_logprobs(N.desc(x), N.rows_desc(t), float(temperature),
+                                              *map(N.rows_desc, (logp, entropy, lse, top_logp, top_ids)), N.stream_ptr(dev))
+        N.check(rc, "token_logprobs")
+    lead = logits.shape[:-1]
+    if top:
+        top_logp, top_ids = top_logp.view(*lead, top), top_ids.view(*lead, top)
+    return logp.view(lead), entropy.view(lead), lse.view(lead), top_logp, top_ids
+
+
+@register_kernel("hip", "token_logprobs_backward")
+def hip_token_logprobs_backward(dlogp, dentropy, dlse, logits, targets, lse, entropy, temperature: float = 1.0, **kwargs: Any):
+    """The logits' gradient (contract: ``common.ref_token_logprobs_backward``)."""
+    _no_grad_needed("token_logprobs_backward", dlogp, dentropy, dlse, logits)
+    dev = N.require_device((dlogp, dentropy, dlse, logits, targets, lse, entropy), "token_logprobs_backward")
+    with N.on_device(dev):
+        x = _logit_rows(logits)
+        rows = [None if t is None else t.reshape(-1).contiguous() for t in (dlogp, dentropy, dlse, targets, lse, entropy)]
+        d = [N.rows_desc(t) for t in rows]
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        rc = N.load().maba_hip_token_logprobs_backward(*d[:3], N.desc(x), *d[3:], float(temperature), N.desc(dx), N.stream_ptr(dev))
+        N.check(rc, "token_logprobs_backward")
+    return dx.view(logits.shape)
+
+
 # ----------------------------------------------------------------------------- serving path
 # Entry points for a decode step whose per-step scalars (the cache position) live in device
 # memory, so that one captured HIP graph serves every position.  Not dispatcher ops: the
