@@ -127,44 +127,88 @@ struct BoundaryBackArgs {
   Drop d;
 };
 
-template <class T, int NCH, bool POST>
+// WHOLE: rows of whole 16-byte chunks (WholeWalk).  The next rows' chunks are loaded ahead of the present ones' arithmetic.
+template <class T, int NCH, bool POST, bool WHOLE>
 __global__ __launch_bounds__(1 << MAX_LG) void boundary_back_kernel(BoundaryBackArgs a) {
   constexpr int V = Traits<T>::VEC, NG = POST ? 3 : 2;
   __shared__ float red[2 * 3 * (1 << MAX_LG) / 64];
-  extern __shared__ float sums[];                  // [NG][threads * V]
+  extern __shared__ float sums[];                  // [NG][threads * V]; before that, the parameters' chunks
   const int threads = blockDim.x;
   int turn = 0;
   const int lg = a.lg, l = threadIdx.x & ((1 << lg) - 1), slots = threads >> lg;
   const int first = __builtin_amdgcn_readfirstlane(threadIdx.x >> lg), sub = lg < 6 ? (threadIdx.x & 63) >> lg : 0;
-  const Walk<T> wd(a.dxo, a.dxos, l, sub), wh(a.dh, a.dhs, l, sub), wx(a.xo, a.xos, l, sub), wy(a.y, a.ys, l, sub);
-  const Walk<T> wdx(a.dx, a.dxs, l, sub), wdy(a.dy, a.dys, l, sub);
-  const Walk<T> vw(a.w, 0, l, 0), vp(a.wp, 0, l, 0), vg(a.g, 0, l, 0);
+  typedef std::conditional_t<WHOLE, WholeWalk<T>, Walk<T>> Rows;
+  const Rows wd(a.dxo, a.dxos, l, sub), wh(a.dh, a.dhs, l, sub), wx(a.xo, a.xos, l, sub), wy(a.y, a.ys, l, sub);
+  const Rows wdx(a.dx, a.dxs, l, sub), wdy(a.dy, a.dys, l, sub);
   const uint64_t key = a.d.mode == 1 ? *a.d.seed : 0;
   const float inv_c = 1.f / (float)a.C;
-  float acc[NG][NCH][V] = {};
-  for (int64_t r0 = (int64_t)blockIdx.x * slots; r0 < a.R; r0 += (int64_t)gridDim.x * slots) {
-    const int64_t ru = r0 + first, r = ru + sub;
-    const int C = r < a.R ? a.C : 0;
-    u32x4 ud[NCH], uh[NCH], ux[NCH], uy[NCH];
+  // chunk c of the parameters: weight's, gate's, post_weight's
+  const int chunks = (a.C + V - 1) / V;
+  u32x4* par = (u32x4*)sums;
+  for (int c = threadIdx.x; c < chunks; c += threads) {
+    if (a.dh) par[c] = load_chunk<T>(a.w, c * 16, a.C - c * V);
+    if (a.g) par[chunks + c] = load_chunk<T>(a.g, c * 16, a.C - c * V);
+    if constexpr (POST) par[2 * chunks + c] = load_chunk<T>(a.wp, c * 16, a.C - c * V);
+  }
+  __syncthreads();
+  uint32_t where[NCH];                             // of chunk i behind chunk 0
+  int pc[NCH];                                     // its parameters; a lane without a chunk reads the last one's
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      const int at = (l + (i << lg)) * V;
-      if (a.dh) {
-        uh[i] = load_chunk<T>(wh.at(ru, i << lg), wh.off, C - at);
-        ux[i] = load_chunk<T>(wx.at(ru, i << lg), wx.off, C - at);
+  for (int i = 0; i < NCH; ++i) {
+    const int c = l + (i << lg);
+    where[i] = c < chunks ? (uint32_t)(16 * (i << lg)) : NOWHERE;
+    pc[i] = min(c, chunks - 1);
+  }
+  struct Raw { u32x4 d[NCH], h[NCH], x[NCH], y[NCH]; };
+  const auto fetch = [&](int64_t r0, Raw& u) {
+    const int64_t ru = r0 + first;
+    const bool live = ru + sub < a.R;
+    if constexpr (WHOLE) {
+      const uint32_t dead = live ? 0u : NOWHERE;
+      const auto rd = wd.rows(ru), rh = wh.rows(ru), rx = wx.rows(ru), ry = wy.rows(ru);
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        const uint32_t at = where[i] | dead;
+        u.h[i] = wh.load(rh, at);
+        u.x[i] = wx.load(rx, at);
+        u.d[i] = wd.load(rd, at);
+        u.y[i] = wy.load(ry, at);
       }
-      if (a.dxo) ud[i] = load_chunk<T>(wd.at(ru, i << lg), wd.off, C - at);
-      if (a.y) uy[i] = load_chunk<T>(wy.at(ru, i << lg), wy.off, C - at);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        const int left = live ? a.C - (l + (i << lg)) * V : 0;
+        u.h[i] = u.x[i] = u.d[i] = u.y[i] = u32x4{0, 0, 0, 0};
+        if (a.dh) {
+          u.h[i] = load_chunk<T>(wh.at(ru, i << lg), wh.off, left);
+          u.x[i] = load_chunk<T>(wx.at(ru, i << lg), wx.off, left);
+        }
+        if (a.dxo) u.d[i] = load_chunk<T>(wd.at(ru, i << lg), wd.off, left);
+        if (a.y) u.y[i] = load_chunk<T>(wy.at(ru, i << lg), wy.off, left);
+      }
     }
+  };
+  float acc[NG][NCH][V] = {};
+  const int64_t step = (int64_t)gridDim.x * slots;
+  int64_t r0 = (int64_t)blockIdx.x * slots;
+  Raw next;
+  if (r0 < a.R) fetch(r0, next);
+  for (; r0 < a.R; r0 += step) {
+    const int64_t ru = r0 + first, r = ru + sub;
+    const Raw u = next;
+    fetch(r0 + step, next);
+    const auto put = [&](const Rows& w, int i, const float (&v)[V]) {
+      if constexpr (WHOLE) w.store(w.rows(ru), where[i] | (r < a.R ? 0u : NOWHERE), pack<T>(v));
+      else store_chunk<T>(w.at(ru, i << lg), w.off, r < a.R ? a.C - (l + (i << lg)) * V : 0, pack<T>(v));
+    };
     float s[3] = {0.f, 0.f, 0.f};            // of dh w x', x'^2, y^2
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int at = (l + (i << lg)) * V;
       if (a.dh) {
         float h[V], x[V], p[V];
-        unpack<T>(uh[i], h);
-        unpack<T>(ux[i], x);
-        unpack<T>(load_chunk<T>(vw.at(0, i << lg), vw.off, C - at), p);
+        unpack<T>(u.h[i], h);
+        unpack<T>(u.x[i], x);
+        unpack<T>(par[pc[i]], p);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           s[0] = fmaf(h[e] * p[e], x[e], s[0]);
@@ -173,26 +217,26 @@ __global__ __launch_bounds__(1 << MAX_LG) void boundary_back_kernel(BoundaryBack
       }
       if constexpr (POST) {
         float y[V];
-        unpack<T>(uy[i], y);
+        unpack<T>(u.y[i], y);
 #pragma unroll
         for (int e = 0; e < V; ++e) s[2] = fmaf(y[e], y[e], s[2]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
     if (a.dh || POST) row_sums<3>(s, lg, red, turn);
-    const float rx = rsqrtf(s[1] * inv_c + a.eps), mean = s[0] * rx * inv_c;
-    const float rp = POST ? rsqrtf(s[2] * inv_c + a.eps) : 1.f;
-    float dz[NCH][V], t[1] = {0.f};
+    // (a row past the last one has no part in the sums over rows, whatever eps is)
+    const float rx = r < a.R ? rsqrtf(s[1] * inv_c + a.eps) : 0.f, mean = s[0] * rx * inv_c;
+    const float rp = !POST ? 1.f : r < a.R ? rsqrtf(s[2] * inv_c + a.eps) : 0.f;
+    float dz[POST ? NCH : 1][V], t[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int at = (l + (i << lg)) * V;
-      float d[V] = {};
-      if (a.dxo) unpack<T>(ud[i], d);
+      float d[V];
+      unpack<T>(u.d[i], d);
       if (a.dh) {
         float h[V], x[V], p[V];
-        unpack<T>(uh[i], h);
-        unpack<T>(ux[i], x);
-        unpack<T>(load_chunk<T>(vw.at(0, i << lg), vw.off, C - at), p);
+        unpack<T>(u.h[i], h);
+        unpack<T>(u.x[i], x);
+        unpack<T>(par[pc[i]], p);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const float xh = x[e] * rx;
@@ -200,39 +244,40 @@ __global__ __launch_bounds__(1 << MAX_LG) void boundary_back_kernel(BoundaryBack
           acc[0][i][e] = fmaf(h[e], xh, acc[0][i][e]);
         }
       }
-      if (a.dx) store_chunk<T>(wdx.at(ru, i << lg), wdx.off, C - at, pack<T>(d));
-      if (!a.dy && !(a.grads & (GRAD_GATE | GRAD_POST))) continue;
-      // dropout(z) = m z with m in {0, 1 / (1 - p)}: both products with m follow from m dX
-      drop_chunk<V>(d, a.d, key, r, at);
-      float p[V], y[V];
-      if (a.y) unpack<T>(uy[i], y);
-      if constexpr (POST) {
+      if (a.dx) put(wdx, i, d);
+      if (a.dy || (a.grads & (GRAD_GATE | GRAD_POST))) {
+        // dropout(z) = m z with m in {0, 1 / (1 - p)}: both products with m follow from m dX
+        drop_chunk<V>(d, a.d, key, r, (l + (i << lg)) * V);
+        float p[V], y[V];
+        unpack<T>(u.y[i], y);
+        if constexpr (POST) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) y[e] *= rp;
-        unpack<T>(load_chunk<T>(vp.at(0, i << lg), vp.off, C - at), p);
-      }
-      if (a.grads & GRAD_GATE)
-#pragma unroll
-        for (int e = 0; e < V; ++e) acc[1][i][e] = fmaf(d[e], POST ? y[e] * p[e] : y[e], acc[1][i][e]);
-#pragma unroll
-      for (int e = 0; e < V; ++e) dz[i][e] = a.scale * d[e];
-      if (a.g) {
-        float q[V];
-        unpack<T>(load_chunk<T>(vg.at(0, i << lg), vg.off, C - at), q);
-#pragma unroll
-        for (int e = 0; e < V; ++e) dz[i][e] *= q[e];
-      }
-      if constexpr (POST) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          acc[NG - 1][i][e] = fmaf(dz[i][e], y[e], acc[NG - 1][i][e]);
-          dz[i][e] *= p[e];
-          t[0] = fmaf(dz[i][e], y[e], t[0]);
+          for (int e = 0; e < V; ++e) y[e] *= rp;
+          unpack<T>(par[2 * chunks + pc[i]], p);
         }
-      } else if (a.dy) {
-        store_chunk<T>(wdy.at(ru, i << lg), wdy.off, C - at, pack<T>(dz[i]));
+        if (a.grads & GRAD_GATE)
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[1][i][e] = fmaf(d[e], POST ? y[e] * p[e] : y[e], acc[1][i][e]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) d[e] *= a.scale;
+        if (a.g) {
+          float q[V];
+          unpack<T>(par[chunks + pc[i]], q);
+#pragma unroll
+          for (int e = 0; e < V; ++e) d[e] *= q[e];
+        }
+        if constexpr (POST) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            acc[NG - 1][i][e] = fmaf(d[e], y[e], acc[NG - 1][i][e]);
+            dz[i][e] = d[e] * p[e];
+            t[0] = fmaf(dz[i][e], y[e], t[0]);
+          }
+        } else if (a.dy) {
+          put(wdy, i, d);
+        }
       }
-      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_sched_barrier(0);           // chunk after chunk: side by side their masks cost 50 registers more
     }
     if constexpr (POST) {
       if (a.dy) {
@@ -240,17 +285,17 @@ __global__ __launch_bounds__(1 << MAX_LG) void boundary_back_kernel(BoundaryBack
         const float m = t[0] * inv_c * rp;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-          const int at = (l + (i << lg)) * V;
           float y[V];
-          unpack<T>(uy[i], y);
+          unpack<T>(u.y[i], y);
 #pragma unroll
           for (int e = 0; e < V; ++e) dz[i][e] = rp * fmaf(-y[e], m, dz[i][e]);
-          store_chunk<T>(wdy.at(ru, i << lg), wdy.off, C - at, pack<T>(dz[i]));
+          put(wdy, i, dz[i]);
         }
       }
     }
   }
   if (!a.grads) return;
+  __syncthreads();                                 // the parameters are read no more
   // rows that share a wave first, then those of the workgroup's waves
   const int lanes = 1 << lg, wave = threadIdx.x >> 6;
   const int units = lg < 6 ? threads / 64 : slots;
@@ -375,9 +420,18 @@ static bool far_rows(std::initializer_list<const maba_tensor*> all) {
     if (t && t->shape[0] > 1 && t->stride[0] > (int64_t)1 << 27) return true;
   return false;
 }
+// Whether the rows of all of them are whole 16-byte chunks.
+static bool whole_rows(std::initializer_list<const maba_tensor*> all) {
+  for (const maba_tensor* t : all)
+    if (t) {
+      const int64_t size = t->dtype == MABA_F32 ? 4 : 2;
+      if (t->shape[1] * size % 16 || (uintptr_t)t->data % 16 || (t->shape[0] > 1 && t->stride[0] * size % 16)) return false;
+    }
+  return true;
+}
 // Elements of a row a lane has: what is kept of them fits the registers of two waves a SIMD.
 constexpr int FORWARD_ELEMS = 24;
-static constexpr int back_elems(bool post) { return post ? 16 : 24; }
+static constexpr int back_elems(bool post, bool f32) { return post || f32 ? 16 : 24; }
 static int row_threads(int lg) { return std::max(256, 1 << lg); }
 // The workgroups of a backward pass: two waves a SIMD, which its registers allow.
 static int back_groups(int64_t R, int lg) {
@@ -478,7 +532,7 @@ extern "C" size_t maba_hip_residual_norm_backward_workspace_size(const maba_tens
   int groups = 0;                                  // the most that any call on these rows has
   for (bool post : {false, true})
     groups = std::max(groups, back_groups(x_out->shape[0],
-                                          row_geometry(x_out->shape[1], chunk_elems(x_out->dtype), back_elems(post), true).lg));
+                                          row_geometry(x_out->shape[1], chunk_elems(x_out->dtype), back_elems(post, x_out->dtype == MABA_F32), true).lg));
   return (size_t)groups * __builtin_popcount(grads & 7) * x_out->shape[1] * sizeof(float);
 }
 
@@ -518,7 +572,7 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
       if (overlap(outs[i], outs[j])) return fail(MABA_ERR_INVALID, "%s: outputs overlap", who);
   }
   if (C > MAX_WIDTH) return fail(MABA_ERR_UNSUPPORTED, "%s: at most %d channels", who, MAX_WIDTH);
-  const Geometry geo = row_geometry(C, chunk_elems(dt), back_elems(post_weight), far_rows({dx_out, dh, x_out, y, dx, dy}));
+  const Geometry geo = row_geometry(C, chunk_elems(dt), back_elems(post_weight, dt == MABA_F32), far_rows({dx_out, dh, x_out, y, dx, dy}));
   const int grads = (dweight ? GRAD_W : 0) | (dgate ? GRAD_GATE : 0) | (dpost_weight ? GRAD_POST : 0);
   if (!grads && !dx && !dy) return MABA_OK;
   const int groups = back_groups(R, geo.lg), n = __builtin_popcount(grads);
@@ -533,14 +587,24 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
                         make_drop(p, seed, stream_id)};
   if (R > 0) {
     const int threads = row_threads(geo.lg);
-    const size_t lds = grads ? (size_t)(post_weight ? 3 : 2) * threads * chunk_elems(dt) * sizeof(float) : 0;
+    const size_t params = (size_t)(post_weight ? 3 : 2) * ceil_div(C, chunk_elems(dt)) * 16;
+    const size_t lds = std::max(params, grads ? (size_t)(post_weight ? 3 : 2) * threads * chunk_elems(dt) * sizeof(float) : 0);
+    const bool whole = whole_rows({dx_out, dh, x_out, y, dx, dy});
     with_type(dt, [&](auto type) {
       typedef decltype(type) T;
       auto run = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(groups), dim3(threads), lds, (hipStream_t)stream, a);
       };
-      if (post_weight) with_chunks<T, back_elems(true)>(geo.nch, [&](auto n) { run(boundary_back_kernel<T, decltype(n)::value, true>); });
-      else with_chunks<T, back_elems(false)>(geo.nch, [&](auto n) { run(boundary_back_kernel<T, decltype(n)::value, false>); });
+      if (post_weight)
+        with_chunks<T, back_elems(true, T::CODE == MABA_F32)>(geo.nch, [&](auto n) {
+          constexpr int N = decltype(n)::value;
+          run(whole ? boundary_back_kernel<T, N, true, true> : boundary_back_kernel<T, N, true, false>);
+        });
+      else
+        with_chunks<T, back_elems(false, T::CODE == MABA_F32)>(geo.nch, [&](auto n) {
+          constexpr int N = decltype(n)::value;
+          run(whole ? boundary_back_kernel<T, N, false, true> : boundary_back_kernel<T, N, false, false>);
+        });
     });
     rc = check_launch(who);
     if (rc) return rc;

@@ -94,6 +94,22 @@ struct Walk {
 };
 
 // A row's lanes: 2^lg of them, lane l of which holds the chunks l, l + 2^lg, ...  Rows narrower than a wave share it.
+// The same rows where every row is whole chunks, 16-byte aligned: accesses through a buffer descriptor, which drops those of
+// lanes without a chunk or a row, and all of a missing tensor's (whose chunks are zeros), without a branch.
+constexpr uint32_t NOWHERE = 0x80000000u;          // past every descriptor's end
+template <class T>
+struct WholeWalk : Walk<T> {
+  uint32_t bytes;
+  __device__ __forceinline__ WholeWalk(const void* q, int64_t ld, int l, int sub) : Walk<T>(q, ld, l, sub), bytes(q ? 0x7fffffffu : 0u) {}
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows(int64_t row) const { return ffn::rsrc(this->p + row * this->stride, bytes); }
+  __device__ __forceinline__ u32x4 load(__amdgpu_buffer_rsrc_t r, uint32_t chunk) const {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(this->off + chunk), 0, 0));
+  }
+  __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t r, uint32_t chunk, u32x4 u) const {
+    __builtin_amdgcn_raw_buffer_store_b128(u, r, (int)(this->off + chunk), 0, 0);
+  }
+};
+
 // `most` is how many elements a lane may have; far: the rows that share a wave would be further apart than 32 bits of bytes tell.
 constexpr int MAX_LG = 9, MAX_WIDTH = 16 << MAX_LG;
 struct Geometry {

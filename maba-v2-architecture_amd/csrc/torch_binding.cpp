@@ -1,5 +1,5 @@
-// The feed-forward operators as native autograd functions for torch: what the Python path does (maba_sparse/kernels/
-// feed_forward.py over hip_backend.py), without Python in the call or in the autograd engine's thread.
+// The feed-forward operators, the block boundary, dropout and token log probabilities as native autograd functions for
+// torch: what the Python path does (maba_sparse/kernels/feed_forward.py and block_ends.py over hip_backend.py), without Python in the call or in the autograd engine's thread.
 //
 // Bound by the host: a training step of 1,777 x 555 to 1,001, whose kernels take 74 us, takes 95 us here and took 177 by the
 // Python path (an empty autograd function in Python: 78); a forward call 9 and 19.
@@ -29,7 +29,8 @@ typedef std::optional<Tensor> Maybe;
 #define MABA_ENTRIES(X)                                                                                                 \
   X(gated_ffn_workspace_size) X(gated_ffn) X(gated_ffn_backward_workspace_size) X(gated_ffn_backward)                   \
   X(linear_epilogue_workspace_size) X(linear_epilogue) X(linear_epilogue_backward_workspace_size)                       \
-  X(linear_epilogue_backward) X(checkpoint_pack) X(checkpoint_unpack) X(last_error)
+  X(linear_epilogue_backward) X(checkpoint_pack) X(checkpoint_unpack) X(dropout) X(residual_norm)                        \
+  X(residual_norm_backward_workspace_size) X(residual_norm_backward) X(token_logprobs) X(token_logprobs_backward) X(last_error)
 
 // The entry points of the library that the Python side has loaded.
 #define X(name) decltype(&maba_hip_##name) name = nullptr;
@@ -55,6 +56,7 @@ int code_of(const Tensor& t) {
     case at::kBFloat16: return MABA_BF16;
     case at::kFloat8_e4m3fn: return MABA_E4M3;
     case at::kByte: return MABA_U8;
+    case at::kLong: return MABA_I64;
     default: throw Declined();
   }
 }
@@ -105,8 +107,9 @@ bool plain(const Tensor& t) {
              c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
                                   c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize}));
 }
-bool alike(const Tensor& first, std::initializer_list<const Tensor*> others) {
-  if (!plain(first) || (first.scalar_type() != at::kHalf && first.scalar_type() != at::kBFloat16)) return false;
+bool alike(const Tensor& first, std::initializer_list<const Tensor*> others, bool wide = false) {
+  if (!plain(first) || (first.scalar_type() != at::kHalf && first.scalar_type() != at::kBFloat16 &&
+                        !(wide && first.scalar_type() == at::kFloat))) return false;
   for (const Tensor* t : others)
     if (t->defined() && (!plain(*t) || t->scalar_type() != first.scalar_type() || t->device() != first.device())) return false;
   return true;
@@ -277,6 +280,188 @@ struct LinearEpilogue : public torch::autograd::Function<LinearEpilogue> {
   }
 };
 
+// ---------------------------------------------------------------- dropout and the block boundary
+
+// What a call drops by.
+struct Drop {
+  double p;
+  Tensor seed;
+  uint32_t stream;
+  const int64_t* ptr() const { return p > 0 && p < 1 ? (const int64_t*)seed.data_ptr() : nullptr; }
+};
+bool drop_fits(const Tensor& x, double p, const Tensor& seed, int64_t stream) {
+  if (!(p >= 0 && p <= 1) || stream < 0 || stream > 0xffffffffll) return false;
+  if (p == 0 || p == 1) return true;
+  return plain(seed) && seed.scalar_type() == at::kLong && seed.numel() == 1 && seed.device() == x.device();
+}
+
+Tensor dropout_call(const Tensor& x, const Drop& d) {
+  Scope scope(x);
+  Tensor out = at::empty(x.sizes(), x.options());
+  Desc dx(x), dout(out);
+  take(lib.dropout(&dx, d.p, d.ptr(), d.stream, &dout, stream_of(x)));
+  return out;
+}
+
+struct Dropout : public torch::autograd::Function<Dropout> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, double p, const Tensor& seed, int64_t stream) {
+    ctx->save_for_backward({seed});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["stream"] = stream;
+    return dropout_call(x, {p, seed, (uint32_t)stream});
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const Drop d = {ctx->saved_data["p"].toDouble(), ctx->get_saved_variables()[0], (uint32_t)ctx->saved_data["stream"].toInt()};
+    Tensor dx;
+    {
+      Scope scope(grads[0]);
+      dx = at::empty(grads[0].sizes(), grads[0].options());
+      Desc in(grads[0]), out(dx);
+      check_backward(lib.dropout(&in, d.p, d.ptr(), d.stream, &out, stream_of(dx)), "dropout");
+    }
+    once({&dx});
+    return {dx, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+struct Boundary {
+  double scale, eps;
+  Drop d;
+};
+
+// (x_out, h); x_out is undefined without y, h without weight.
+std::pair<Tensor, Tensor> boundary_call(const Tensor& x, const Tensor& y, const Tensor& w, const Tensor& wp, const Tensor& g,
+                                        const Boundary& b) {
+  Scope scope(x);
+  Tensor xo, h;
+  if (y.defined()) xo = at::empty(x.sizes(), x.options());
+  if (w.defined()) h = at::empty(x.sizes(), x.options());
+  Desc dx(x), dy(y), dw(w, true), dp(wp, true), dg(g, true), dxo(xo), dh(h);
+  take(lib.residual_norm(&dx, &dy, &dw, &dp, &dg, (float)b.scale, b.d.p, b.d.ptr(), b.d.stream, (float)b.eps, &dxo, &dh,
+                         stream_of(x)));
+  return {xo, h};
+}
+
+struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
+  // the results that there are
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& y_, const Maybe& w_, const Maybe& wp_,
+                               const Maybe& g_, double scale, double p, const Maybe& seed_, int64_t stream, double eps) {
+    const Tensor y = y_.value_or(Tensor()), w = w_.value_or(Tensor()), wp = wp_.value_or(Tensor()), g = g_.value_or(Tensor());
+    const Tensor seed = seed_.value_or(Tensor());
+    auto out = boundary_call(x, y, w, wp, g, {scale, eps, {p, seed, (uint32_t)stream}});
+    // y is read for its own norm's gradient and for the gate's, x_out for its norm's
+    const bool keeps_y = y.defined() && (wp.defined() || needs(g));
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({w.defined() ? y.defined() ? out.first : x : Tensor(), keeps_y ? y : Tensor(), w, wp, g, seed});
+    ctx->saved_data["need"] = (int64_t)(needs(x) | needs(y) << 1 | needs(w) << 2 | needs(wp) << 3 | needs(g) << 4 | y.defined() << 5);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["stream"] = stream;
+    ctx->saved_data["eps"] = eps;
+    variable_list made;
+    if (out.first.defined()) made.push_back(out.first);
+    if (out.second.defined()) made.push_back(out.second);
+    return made;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const auto kept = ctx->get_saved_variables();
+    const int64_t need = ctx->saved_data["need"].toInt();
+    const Tensor &y = kept[1], &w = kept[2], &wp = kept[3], &g = kept[4];
+    const Tensor dxo = need >> 5 & 1 ? grads[0] : Tensor(), dh = w.defined() ? grads.back() : Tensor();
+    Tensor dx, dy, dw, dwp, dg;
+    if (dxo.defined() || dh.defined()) {
+      const Tensor like = dxo.defined() ? dxo : dh, xo = kept[0].defined() ? kept[0] : like;
+      const Drop d = {ctx->saved_data["p"].toDouble(), kept[5], (uint32_t)ctx->saved_data["stream"].toInt()};
+      Scope scope(like);
+      if (need & 1) dx = at::empty(like.sizes(), like.options());
+      if (need & 2) dy = at::empty(like.sizes(), like.options());
+      if (need & 4) dw = at::empty(w.sizes(), like.options());
+      if (need & 8) dwp = at::empty(wp.sizes(), like.options());
+      if (need & 16) dg = at::empty(g.sizes(), like.options());
+      Desc ddxo(dxo), ddh(dh), dxo_(xo), iy(y), iw(w, true), ip(wp, true), ig(g, true);
+      Desc odx(dx), ody(dy), odw(dw, true), odp(dwp, true), odg(dg, true);
+      const int which = (need >> 2 & 1) | (need >> 4 & 1) << 1 | (need >> 3 & 1) << 2;
+      Tensor ws;
+      if (which) ws = workspace(lib.residual_norm_backward_workspace_size(&dxo_, which), like);
+      check_backward(lib.residual_norm_backward(&ddxo, &ddh, &dxo_, &iy, &iw, &ip, &ig, (float)ctx->saved_data["scale"].toDouble(),
+                                                d.p, d.ptr(), d.stream, (float)ctx->saved_data["eps"].toDouble(), &odx, &ody, &odw,
+                                                &odp, &odg, ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0,
+                                                stream_of(like)),
+                     "residual_norm_backward");
+    }
+    once({&dx, &dy, &dw, &dwp, &dg});
+    return {dx, dy, dw, dwp, dg, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// ---------------------------------------------------------------- token log probabilities
+
+// Logits as [M, V] or [B, L, V] with unit column stride.
+Tensor logit_rows(const Tensor& t) {
+  Tensor r = t.dim() == 2 || t.dim() == 3 ? t : t.reshape({-1, t.size(-1)});
+  return r.stride(-1) != 1 && r.size(-1) != 1 ? r.contiguous() : r;
+}
+maba_tensor desc3(const Tensor& t) {
+  maba_tensor d = {t.data_ptr(), code_of(t), (int)t.dim(), {1, 1, 1, 1}, {0, 0, 0, 0}};
+  for (int i = 0; i < d.ndim; ++i) {
+    d.shape[i] = t.size(i);
+    d.stride[i] = t.stride(i);
+  }
+  return d;
+}
+Tensor flat(const Tensor& t) { return t.defined() ? t.reshape({-1}) : t; }
+
+// logp, entropy, lse and, for top > 0, the alternatives' log probabilities and indexes.
+variable_list logprobs_call(const Tensor& logits, const Tensor& targets, double temperature, int64_t top) {
+  Scope scope(logits);
+  const Tensor x = logit_rows(logits), t = flat(targets);
+  const auto lead = targets.sizes();
+  const auto f32 = logits.options().dtype(at::kFloat);
+  variable_list out = {at::empty(lead, f32), at::empty(lead, f32), at::empty(lead, f32)};
+  Tensor top_logp, top_ids;
+  if (top) {
+    auto shape = lead.vec();
+    shape.push_back(top);
+    out.push_back(at::empty(shape, f32));
+    out.push_back(at::empty(shape, f32.dtype(at::kLong)));
+    top_logp = out[3].view({-1, top});
+    top_ids = out[4].view({-1, top});
+  }
+  maba_tensor dx = desc3(x);
+  Desc dt(t, true), dl(flat(out[0]), true), de(flat(out[1]), true), dz(flat(out[2]), true), dtl(top_logp), dti(top_ids);
+  take(lib.token_logprobs(&dx, &dt, temperature, &dl, &de, &dz, &dtl, &dti, stream_of(x)));
+  return out;
+}
+
+struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& targets, double temperature, int64_t top) {
+    auto out = logprobs_call(logits, targets, temperature, top);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({logits, targets, out[2], out[1]});
+    ctx->saved_data["temperature"] = temperature;
+    if (top) ctx->mark_non_differentiable({out[3], out[4]});
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    Tensor dl;
+    if (grads[0].defined() || grads[1].defined() || grads[2].defined()) {
+      const auto kept = ctx->get_saved_variables();
+      Scope scope(kept[0]);
+      const Tensor x = logit_rows(kept[0]);
+      Tensor d = at::empty(x.sizes(), x.options());
+      maba_tensor dx = desc3(x), out = desc3(d);
+      Desc g0(flat(grads[0]), true), g1(flat(grads[1]), true), g2(flat(grads[2]), true);
+      Desc t(flat(kept[1]), true), z(flat(kept[2]), true), h(flat(kept[3]), true);
+      check_backward(lib.token_logprobs_backward(&g0, &g1, &g2, &dx, &t, &z, &h, ctx->saved_data["temperature"].toDouble(), &out,
+                                                 stream_of(x)),
+                     "token_logprobs_backward");
+      dl = d.sizes() == kept[0].sizes() ? d : d.view(kept[0].sizes());
+    }
+    once({&dl});
+    return {dl, Tensor(), Tensor(), Tensor()};
+  }
+};
+
 // ---------------------------------------------------------------- the module's functions
 
 // Whether the dispatcher's backend for GPU tensors is this library: MABA_BACKEND as its get_backend reads it, without the
@@ -344,6 +529,56 @@ Maybe checkpoint_unpack(const Tensor& codes, const Tensor& scales, at::ScalarTyp
   }
 }
 
+Maybe dropout(const Tensor& x, double p, const Maybe& seed_, int64_t stream) {
+  const Tensor seed = seed_.value_or(Tensor());
+  if (!alike(x, {}, true) || x.dim() < 1 || x.size(-1) == 0 || !drop_fits(x, p, seed, stream)) return std::nullopt;
+  try {
+    if (needs_grad({&x})) return Dropout::apply(x, p, seed, stream);
+    return dropout_call(x, {p, seed, (uint32_t)stream});
+  } catch (const Declined&) {
+    return std::nullopt;
+  }
+}
+
+std::optional<std::pair<Tensor, Maybe>> residual_norm(const Tensor& x, const Maybe& y_, const Maybe& w_, const Maybe& wp_,
+                                                      const Maybe& g_, double scale, double p, const Maybe& seed_, int64_t stream,
+                                                      double eps) {
+  const Tensor y = y_.value_or(Tensor()), w = w_.value_or(Tensor()), wp = wp_.value_or(Tensor()), g = g_.value_or(Tensor());
+  const Tensor seed = seed_.value_or(Tensor());
+  if (!alike(x, {&y, &w, &wp, &g}, true) || x.dim() < 1 || x.size(-1) == 0 || !drop_fits(x, p, seed, stream)) return std::nullopt;
+  if (y.defined() ? y.sizes() != x.sizes() : wp.defined() || g.defined() || !w.defined()) return std::nullopt;
+  for (const Tensor* v : {&w, &wp, &g})
+    if (v->defined() && (v->dim() != 1 || v->size(0) != x.size(-1))) return std::nullopt;
+  try {
+    Tensor xo, h;
+    if (needs_grad({&x, &y, &w, &wp, &g})) {
+      auto out = ResidualNorm::apply(x, y_, w_, wp_, g_, scale, p, seed_, stream, eps);
+      if (y.defined()) xo = out[0];
+      if (w.defined()) h = out.back();
+    } else {
+      std::tie(xo, h) = boundary_call(x, y, w, wp, g, {scale, eps, {p, seed, (uint32_t)stream}});
+    }
+    return std::make_pair(y.defined() ? xo : x, h.defined() ? Maybe(h) : std::nullopt);
+  } catch (const Declined&) {
+    return std::nullopt;
+  }
+}
+
+typedef std::tuple<Tensor, Tensor, Tensor, Maybe, Maybe> Logprobs;
+std::optional<Logprobs> token_logprobs(const Tensor& logits, const Tensor& targets, double temperature, int64_t top) {
+  if (!alike(logits, {}, true) || !plain(targets) || targets.scalar_type() != at::kLong || targets.device() != logits.device() ||
+      logits.dim() < 1 || logits.size(-1) == 0 || targets.sizes() != logits.sizes().slice(0, logits.dim() - 1) || top < 0 ||
+      top > logits.size(-1))
+    return std::nullopt;
+  try {
+    const auto out = needs_grad({&logits}) ? TokenLogprobs::apply(logits, targets, temperature, top)
+                                           : logprobs_call(logits, targets, temperature, top);
+    return Logprobs(out[0], out[1], out[2], top ? Maybe(out[3]) : std::nullopt, top ? Maybe(out[4]) : std::nullopt);
+  } catch (const Declined&) {
+    return std::nullopt;
+  }
+}
+
 // Whether a leaf that `out` was made from, by itself or cast to another type, keeps its autograd node from another stream
 // than the current one: the stream that was current when the eager graph it belongs to was made, by whatever op.
 bool leaf_of_another_stream(const Tensor& out) {
@@ -377,6 +612,9 @@ PYBIND11_MODULE(maba_torch, m) {
   m.def("leaf_of_another_stream", &leaf_of_another_stream);
   m.def("gated_ffn", unlocked(&gated_ffn));
   m.def("linear_epilogue", unlocked(&linear_epilogue));
+  m.def("dropout", unlocked(&dropout));
+  m.def("residual_norm", unlocked(&residual_norm));
+  m.def("token_logprobs", unlocked(&token_logprobs));
   m.def("checkpoint_pack", unlocked(&checkpoint_pack));
   m.def("checkpoint_unpack", unlocked(&checkpoint_unpack));
 }

@@ -270,7 +270,8 @@ def on_device(device: torch.device):
 _binding = None
 _BOUND = ("gated_ffn_workspace_size", "gated_ffn", "gated_ffn_backward_workspace_size", "gated_ffn_backward",
           "linear_epilogue_workspace_size", "linear_epilogue", "linear_epilogue_backward_workspace_size",
-          "linear_epilogue_backward", "checkpoint_pack", "checkpoint_unpack", "last_error")
+          "linear_epilogue_backward", "checkpoint_pack", "checkpoint_unpack", "dropout", "residual_norm",
+          "residual_norm_backward_workspace_size", "residual_norm_backward", "token_logprobs", "token_logprobs_backward", "last_error")
 
 
 def binding():

@@ -495,7 +495,9 @@ def _load_native() -> None:
     binding, ops = _native.binding(), {}
     for op, names in (("gated_ffn", ("gated_ffn", "gated_ffn_backward")), ("checkpoint_pack", ("checkpoint_pack",)),
                       ("linear_epilogue", ("linear_epilogue", "linear_epilogue_backward")),
-                      ("checkpoint_unpack", ("checkpoint_unpack",))):
+                      ("checkpoint_unpack", ("checkpoint_unpack",)), ("dropout", ("dropout",)),
+                      ("residual_norm", ("residual_norm", "residual_norm_backward")),
+                      ("token_logprobs", ("token_logprobs", "token_logprobs_backward"))):
         ops[op] = (getattr(binding, op), tuple((n, getattr(hb, "hip_" + n)) for n in names))
     _NATIVE.update(ops)
 
@@ -694,6 +696,11 @@ def dispatch_dropout(x, p: float, seed=None, stream: int = 0) -> torch.Tensor:
     (counted over the leading dimensions) and the column; see ``common.philox_words``.  A dropped element is 0 whatever it
     was.  A seed that is advanced in place after the backward pass, also inside a captured graph, gives every step
     masks of its own.  Differentiable on every backend."""
+    native = _bound("dropout", x)
+    if native is not None:
+        out = native(x, p, seed, stream)
+        if out is not None:
+            return _ff.guard_capture(out)
     _channels(x)
     _ffn_same(x)
     _drop_args(x, p, seed, stream)
@@ -734,6 +741,12 @@ def dispatch_residual_norm(x, y=None, weight=None, post_weight=None, gate=None, 
     dtype = _autocast_dtype(x)
     if dtype is not None:
         x, y, weight, post_weight, gate = _widest(x, y, weight, post_weight, gate)
+    native = _bound("residual_norm", x)
+    if native is not None:
+        out = native(x, y, weight, post_weight, gate, scale, p, seed, stream, eps)
+        if out is not None:
+            _ff.guard_capture(out[0] if y is not None else out[1])
+            return out
     _boundary_check(x, y, weight, post_weight, gate)
     _drop_args(x, p, seed, stream)
     if y is None:
@@ -804,6 +817,12 @@ def dispatch_token_logprobs(logits, targets, temperature: float = 1.0, top: int 
     stands for none: its logp is 0 and has no gradient; one of V or more gives NaN, since a GPU call cannot refuse it.  Logits
     of -inf have probability zero; a row of nothing else has lse and log probabilities -inf, entropy 0 and no gradient.
     logp, entropy and lse are differentiable on every backend (the logits are kept for it), the alternatives are not."""
+    native = _bound("token_logprobs", logits)
+    if native is not None:
+        out = native(logits, targets, temperature, top)
+        if out is not None:
+            _ff.guard_capture(out[0])
+            return out
     _logprobs_check(logits, targets, temperature)
     if not 0 <= top <= logits.shape[-1]:
         raise ValueError(f"top must be in [0, {logits.shape[-1]}], got {top}")

@@ -516,8 +516,7 @@ def hip_token_logprobs(logits, targets, temperature: float = 1.0, top: int = 0, 
     with N.on_device(dev):
         x, t = _logit_rows(logits), targets.reshape(-1).contiguous()
         M = t.numel()
-        out = torch.empty(3, M, dtype=torch.float32, device=dev)
-        logp, entropy, lse = out.unbind(0)
+        logp, entropy, lse = (torch.empty(M, dtype=torch.float32, device=dev) for _ in range(3))
         top_logp = torch.empty(M, top, dtype=torch.float32, device=dev) if top else None
         top_ids = torch.empty(M, top, dtype=torch.long, device=dev) if top else None
         rc = N.load().maba_hip_token_logprobs(N.desc(x), N.rows_desc(t), float(temperature),
