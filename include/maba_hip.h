@@ -506,7 +506,8 @@ int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const maba_tensor
  * min(64, V), or both NULL.  With u = logits / temperature: lse = log sum exp(u), logp = u[target] - lse (0 where the
  * target is negative, NaN where it is V or more), entropy of exp(u - lse), and the k largest with their log
  * probabilities: by logit (NaN above all, -0 as +0), then the lower index.  A row of nothing but -inf has lse and log
- * probabilities -inf and entropy 0; a row with NaN or +inf has NaN.  fp32 arithmetic.
+ * probabilities -inf and entropy 0 (an lse past f32's range is its largest finite value otherwise); a row with NaN or +inf
+ * has NaN.  fp32 arithmetic.
  *
  * Backward: dlogp, dentropy, dlse f32 [M], any of which may be NULL (zeros); lse and entropy as the forward returned
  * them; dlogits like logits (it may be logits itself).  A row of nothing but -inf has no gradient, and dlogp counts only

@@ -3,13 +3,14 @@
 //   lse = log sum exp(u),  logp = u[t] - lse,  H = lse - sum p u,  p = exp(u - lse)
 //   dl  = 1/T (dlogp (delta_t - p) + dlse p - dH p (log p + H))
 //
-// Forward is one pass with a running maximum: a thread holds (m, S, D) = (max l, sum e, sum (l - m) e), e = exp((l - m) / T),
-// and two such triples over different elements join by rescaling the one with the smaller m.  Then lse = m / T + log S and
-// H = log S - D / (T S): differences from the maximum, so that nothing large cancels.
+// Forward is one pass with a running reference: a thread holds (R, S, D) = (R, sum 2^x, sum x 2^x), x = l c - R, c = log2(e) / T,
+// with R the largest l c so far rounded up to a whole number, so that l c - R is one fused operation without a rounding of R
+// of its own, and two such triples over different elements join by a shift.  Then lse = ln 2 (R + log2 S), logp =
+// ln 2 (l c - R - log2 S) and H = ln 2 (log2 S - D / S): differences from the reference, so that nothing large cancels.
 //
-// Alternatives: a second pass over the row, which the caches still hold, collects the elements that are at least a bound
-// with no fewer than k of them above it, some tens in all, and one wave sorts those.  The order is by value and then the
-// lower index, so ties have one answer.
+// Alternatives: the k-th largest, or so, of the threads' own largest elements is a bound with no fewer than k elements at or
+// above it.  The threads that have any collect theirs, some tens in all, and one wave sorts them.  The order is by
+// value and then the lower index, so ties have one answer.
 //
 // Bound: HBM; forward reads the logits once, backward reads them and writes their gradient.
 #include "row_vec.h"
@@ -20,7 +21,7 @@ namespace logprobs {
 
 using namespace rowvec;
 
-constexpr float LOWEST = -3.40282347e38f, LOG2E = 1.4426950408889634f;
+constexpr float LOWEST = -3.40282347e38f, LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct Logits {
   const char* p;
@@ -44,50 +45,73 @@ __device__ __forceinline__ key64 order_key(float v, uint32_t idx) {
   return ((key64)o << 32) | (key64)(~idx);
 }
 
-struct Triple { float m, s, d; };
-// D of a state whose maximum rises by -dm, f = exp2(dm c).  dm may be past fp32's range, and f is zero then.
-__device__ __forceinline__ float moved(float d, float s, float dm, float f) { return d * f + fmaxf(dm, LOWEST) * f * s; }
-// Joined; a triple of no mass takes no part, whatever its maximum.
-__device__ __forceinline__ Triple join(Triple a, Triple b, float c) {
-  const float m = fmaxf(a.m, b.m), da = a.m - m, db = b.m - m;
-  const float fa = __builtin_amdgcn_exp2f(da * c), fb = __builtin_amdgcn_exp2f(db * c);
-  Triple r = {m, 0.f, 0.f};
-  if (a.s != 0.f) { r.s += a.s * fa; r.d += moved(a.d, a.s, da, fa); }
-  if (b.s != 0.f) { r.s += b.s * fb; r.d += moved(b.d, b.s, db, fb); }
-  return r;
+// R is a whole number or LOWEST (no element yet, or none above it).
+struct Triple { float r, s, d; };
+// (s, d) with the reference raised by -by, f = 2^by.  by may be past fp32's range, and f is zero then.
+__device__ __forceinline__ void raise(float& s, float& d, float by) {
+  const float f = __builtin_amdgcn_exp2f(by);
+  d = fmaf(d, f, fmaxf(by, LOWEST) * f * s);
+  s *= f;
+}
+__device__ __forceinline__ Triple join(Triple a, Triple b) {
+  const float r = fmaxf(a.r, b.r);
+  raise(a.s, a.d, a.r - r);
+  raise(b.s, b.d, b.r - r);
+  return {r, a.s + b.s, a.d + b.d};
 }
 
 // The running state of a thread over its elements, and the largest of them.
-template <bool TOP>
 struct Running {
   Triple t = {LOWEST, 0.f, 0.f};
   float best = -INFINITY;
-  uint32_t best_idx = 0;
-  bool any = false;
-  // N elements, in the order of their indexes: element e has index idx(e)
-  template <int N, class Idx>
-  __device__ __forceinline__ void take(const float (&v)[N], float c, Idx idx) {
-    float b = v[0];
+  template <int N>
+  __device__ __forceinline__ void take(const float (&v)[N], float c) {
+    float b = best;
 #pragma unroll
-    for (int e = 1; e < N; ++e) b = fmaxf(b, v[e]);
-    const float m = fmaxf(t.m, b), dm = t.m - m, f = __builtin_amdgcn_exp2f(dm * c);
-    float s = t.s * f, d = moved(t.d, t.s, dm, f);
+    for (int e = 0; e < N; ++e) b = fmaxf(b, v[e]);
+    best = b;
+    const float r = fmaxf(t.r, ceilf(b * c));
+    raise(t.s, t.d, t.r - r);
+    t.r = r;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const float x = v[e] - m, p = __builtin_amdgcn_exp2f(x * c);
-      s += p;
-      d = fmaf(fmaxf(x, LOWEST), p, d);          // -inf times a p of zero is zero here
-    }
-    t = {m, s, d};
-    if (TOP && b > best) {
-      best = b;
-      any = true;
-#pragma unroll
-      for (int e = N - 1; e >= 0; --e)
-        if (v[e] == b) best_idx = idx(e);
+      const float x = fmaf(v[e], c, -r), p = __builtin_amdgcn_exp2f(x);
+      t.s += p;
+      t.d = fmaf(fmaxf(x, LOWEST), p, t.d);          // -inf times a p of zero is zero here
     }
   }
 };
+
+// The n-th largest (from 1) of a wave's values.
+__device__ __forceinline__ float nth_of_wave(float v, int n) {
+  const int lane = threadIdx.x & 63;
+  if (n <= 8) {                                        // take the largest out n times; beyond that sorting is shorter
+    float m = v;
+    for (int i = 0;; ++i) {
+      m = v;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
+      if (i == n - 1) return m;
+      const uint64_t at = __ballot(v == m);
+      if (lane == __builtin_ctzll(at)) v = -INFINITY;
+    }
+  }
+#pragma unroll
+  for (int k = 2; k <= 64; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      const float o = __shfl_xor(v, j);
+      v = ((lane & j) == 0) == ((lane & k) == 0) ? fmaxf(v, o) : fminf(v, o);
+    }
+  return __shfl(v, n - 1);
+}
+
+template <class T>
+__device__ __forceinline__ float element(const char* row, uint32_t i) {
+  float w[Traits<T>::VEC];
+  unpack<T>(load_chunk<T>(row, i * (16 / Traits<T>::VEC), 1), w);
+  return w[0];
+}
 
 // f(chunk values, first index) over the row's chunks of a group of `lanes` threads, NB at a time while all are whole
 template <class T, int NB, class F>
@@ -119,13 +143,30 @@ __device__ __forceinline__ void for_chunks(const char* row, int V, int lane, int
   }
 }
 
+// v of all W waves' lanes joined.
+template <int W, class F>
+__device__ __forceinline__ float across(float v, float* shared, F f) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) v = f(v, __shfl_xor(v, off));
+  if constexpr (W > 1) {
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = shared[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) v = f(v, shared[w]);
+  }
+  return v;
+}
+
 // W waves a row.  One wave for short rows, four of them in a workgroup; otherwise the workgroup is one row's.
 template <class T, int W, bool TOP>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void logprobs_kernel(ForwardArgs a) {
-  constexpr int E = Traits<T>::VEC, NB = 32 / E, LANES = 64 * W, GROUPS = W == 1 ? 4 : 1, CAP = W == 1 ? 512 : 2048;
-  __shared__ Triple s_t[GROUPS * W];
-  __shared__ key64 s_max[W], s_min[W], s_found[TOP ? GROUPS * CAP : 1];
-  __shared__ int s_count[GROUPS];
+  constexpr int E = Traits<T>::VEC, NB = 32 / E, LANES = 64 * W, GROUPS = W == 1 ? 4 : 1, CAP = W == 1 ? 256 : 1024;
+  __shared__ Triple s_t[W];
+  __shared__ float s_nth[W];
+  __shared__ key64 s_above[TOP ? GROUPS * CAP : 1], s_equal[TOP ? GROUPS * CAP : 1];
+  __shared__ int s_count[GROUPS][2];
+  __shared__ float s_far[3][W];
   const int group = W == 1 ? threadIdx.x >> 6 : 0, lane = threadIdx.x & (LANES - 1), wave = W == 1 ? 0 : threadIdx.x >> 6;
   const int64_t r = (int64_t)blockIdx.x * GROUPS + __builtin_amdgcn_readfirstlane(group);
   if (W == 1 && r >= a.R) return;               // nothing below waits for another wave where W is 1
@@ -133,107 +174,110 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void logprobs_kernel(Forward
   const float c = a.inv * LOG2E;
   const int64_t target = a.targets[r];
   float lt = 0.f;
-  if (target >= 0 && target < a.V) {
-    float w[E];
-    unpack<T>(load_chunk<T>(row + target * (16 / E), 0, 1), w);
-    lt = w[0];
-  }
-  Running<TOP> run;
-  for_chunks<T, NB>(row, a.V, lane, LANES, [&](auto& v, int first) {
-    run.take(v, c, [&](int e) { return (uint32_t)(first + (e / E) * LANES * E + e % E); });
-  });
+  if (target >= 0 && target < a.V) lt = element<T>(row, (uint32_t)target);
+  Running run;
+  for_chunks<T, NB>(row, a.V, lane, LANES, [&](auto& v, int) { run.take(v, c); });
   Triple t = run.t;
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1)
-    t = join(t, {__shfl_xor(t.m, off), __shfl_xor(t.s, off), __shfl_xor(t.d, off)}, c);
-  key64 bound = KEY_NONE;
+  for (int off = 1; off < 64; off <<= 1) t = join(t, {__shfl_xor(t.r, off), __shfl_xor(t.s, off), __shfl_xor(t.d, off)});
+  float bound = 0.f;
   if constexpr (TOP) {
-    // Of a wave's lanes' maxima, sorted: the k-th of any wave has k elements above it, and so has the smallest of all
-    // waves' (k / W)-th.
-    const key64 sorted = wave_sort_desc(run.any ? order_key(run.best, run.best_idx) : KEY_NONE);
-    const key64 kth = __shfl(sorted, a.k - 1), part = __shfl(sorted, (a.k + W - 1) / W - 1);
-    if constexpr (W == 1) {
-      bound = kth;
-    } else if ((threadIdx.x & 63) == 0) {
-      s_max[wave] = kth;
-      s_min[wave] = part;
-    }
-    if (lane == 0) s_count[group] = 0;
+    // each of W waves has k / W elements at or above its own k / W-th largest, and so all have k at or above the least of those
+    bound = nth_of_wave(run.best, (a.k + W - 1) / W);
+    if (lane < 2) s_count[group][lane] = 0;
   }
   if constexpr (W > 1) {
-    if ((threadIdx.x & 63) == 0) s_t[wave] = t;
+    if ((threadIdx.x & 63) == 0) {
+      s_t[wave] = t;
+      s_nth[wave] = bound;
+    }
     __syncthreads();
     t = s_t[0];
+    bound = s_nth[0];
 #pragma unroll
-    for (int w = 1; w < W; ++w) t = join(t, s_t[w], c);
-    if constexpr (TOP) {
-      key64 lo = s_min[0];
-      bound = s_max[0];
-#pragma unroll
-      for (int w = 1; w < W; ++w) {
-        bound = kmax(bound, s_max[w]);
-        lo = kmin(lo, s_min[w]);
-      }
-      bound = kmax(bound, lo);
+    for (int w = 1; w < W; ++w) {
+      t = join(t, s_t[w]);
+      bound = fminf(bound, s_nth[w]);
     }
   }
-  const float log_s = logf(t.s), lse = fmaf(t.m, a.inv, log_s);
-  const bool none = lse == -INFINITY;            // every logit is -inf: so are the log probabilities, and the entropy is 0
-  if (lane == 0) {
-    a.lse[r] = lse;
-    a.entropy[r] = none ? 0.f : log_s - a.inv * (t.d / t.s);
-    a.logp[r] = target < 0 ? 0.f : target >= a.V ? NAN : none ? -INFINITY : (lt - t.m) * a.inv - log_s;
-  }
-  if constexpr (TOP) {
-    const float at_least = bound == KEY_NONE ? -INFINITY : key_score(bound);
-    key64* found = s_found + group * CAP;
-    const auto collect = [&](auto put) {
-      for_chunks<T, NB>(row, a.V, lane, LANES, [&](auto& v, int first) {
-        constexpr int N = sizeof(v) / sizeof(v[0]);
-        bool any = false;
+  // No sum, or none that is a number: every logit is -inf, or one is NaN or +inf, or the largest times c leaves fp32's
+  // range, as where a mask of the type's lowest value leaves nothing else.  Again, then, from the largest itself.
+  const bool far = !(t.s > 0.f);
+  float m = 0.f;
+  if (far) {
+    m = -INFINITY;
+    for_chunks<T, 1>(row, a.V, lane, LANES, [&](auto& v, int) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) any |= !(v[e] < at_least);
-        if (!__any(any)) return;
+      for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
+    });
+    m = across<W>(m, s_far[0], [](float x, float y) { return fmaxf(x, y); });
+    m = m == -INFINITY ? 0.f : m;
+    t = {0.f, 0.f, 0.f};
+    for_chunks<T, 1>(row, a.V, lane, LANES, [&](auto& v, int) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const int idx = first + (e / E) * LANES * E + e % E;
-          const key64 key = order_key(v[e], (uint32_t)idx);
-          const bool in = idx < a.V && key >= bound;
-          if (__any(in)) put(in ? key : KEY_NONE);
-        }
-      });
-    };
-    collect([&](key64 key) {
-      if (key != KEY_NONE) {
-        const int at = atomicAdd(&s_count[group], 1);
-        if (at < CAP) found[at] = key;
+      for (int e = 0; e < E; ++e) {
+        const float x = (v[e] - m) * c, p = __builtin_amdgcn_exp2f(x);
+        t.s += p;
+        t.d = fmaf(fmaxf(x, LOWEST), p, t.d);
       }
     });
+    t.s = across<W>(t.s, s_far[1], [](float x, float y) { return x + y; });
+    t.d = across<W>(t.d, s_far[2], [](float x, float y) { return x + y; });
+  }
+  const float log_s = __builtin_amdgcn_logf(t.s);
+  const bool none = t.s == 0.f;                  // every logit is -inf: so are the log probabilities, and the entropy is 0
+  float lse = far ? fmaf(m, a.inv, log_s * LN2) : (t.r + log_s) * LN2;
+  if (!none) lse = lse < LOWEST ? LOWEST : lse > -LOWEST ? -LOWEST : lse;       // -inf says that there is no mass
+  const auto logp_of = [&](float l) { return none ? -INFINITY : ((far ? (l - m) * c : fmaf(l, c, -t.r)) - log_s) * LN2; };
+  if (lane == 0) {
+    a.lse[r] = lse;
+    a.entropy[r] = none ? 0.f : (log_s - t.d / t.s) * LN2;
+    a.logp[r] = target < 0 ? 0.f : target >= a.V ? NAN : logp_of(lt);
+  }
+  if constexpr (TOP) {
+    key64 *above = s_above + group * CAP, *equal = s_equal + group * CAP;
+    int* count = s_count[group];
+    // a thread whose sum is NaN may have NaN among its elements, which its largest does not tell
+    if (run.best >= bound || run.t.s != run.t.s)
+      for_chunks<T, NB>(row, a.V, lane, LANES, [&](auto& v, int first) {
+        constexpr int N = sizeof(v) / sizeof(v[0]);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          if (v[e] < bound) continue;
+          const int idx = first + (e / E) * LANES * E + e % E;
+          if (idx >= a.V) continue;
+          const bool eq = v[e] == bound;
+          if (eq && *(volatile int*)&count[1] >= CAP) continue;        // more than will be read are not counted on
+          const int at = atomicAdd(&count[eq], 1);
+          if (at < CAP) (eq ? equal : above)[at] = order_key(v[e], (uint32_t)idx);
+        }
+      });
     if constexpr (W > 1) __syncthreads();
     else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (wave != 0) return;
-    const int l = threadIdx.x & 63, n = *(volatile int*)&s_count[group];
+    const int l = threadIdx.x & 63, n = *(volatile int*)&count[0], ties = *(volatile int*)&count[1];
     key64 list = KEY_NONE;
     if (n <= CAP) {
-      for (int i = 0; i < n; i += 64) list = wave_merge_topk(list, i + l < n ? found[i + l] : KEY_NONE, 64);
-    } else {
-      // More than the buffer holds (thousands of the same lanes' elements above the rest): wave 0 goes over the row alone.
-      for (int i = 0; i < a.V; i += 64) {
-        float w[E];
-        key64 key = KEY_NONE;
-        if (i + l < a.V) {
-          unpack<T>(load_chunk<T>(row + (int64_t)(i + l) * (16 / E), 0, 1), w);
-          key = order_key(w[0], (uint32_t)(i + l));
+      for (int i = 0; i < n; i += 64) list = wave_merge_topk(list, i + l < n ? above[i + l] : KEY_NONE, 64);
+      if (n < a.k && ties < CAP) {
+        for (int i = 0; i < ties; i += 64) list = wave_merge_topk(list, i + l < ties ? equal[i + l] : KEY_NONE, 64);
+      } else if (n < a.k) {
+        // many of one value: the first ones of the row, in order
+        for (int i = 0, found = n; i < a.V && found < a.k; i += 64) {
+          const float v = i + l < a.V ? element<T>(row, (uint32_t)(i + l)) : NAN;
+          found += __popcll(__ballot(v == bound));
+          list = wave_merge_topk(list, v == bound ? order_key(v, (uint32_t)(i + l)) : KEY_NONE, 64);
         }
-        list = wave_merge_topk(list, key, a.k);
       }
+    } else {
+      // more above the bound than there is room for: a row whose largest elements are a few threads' own
+      for (int i = 0; i < a.V; i += 64)
+        list = wave_merge_topk(list, i + l < a.V ? order_key(element<T>(row, (uint32_t)(i + l)), (uint32_t)(i + l)) : KEY_NONE, a.k);
     }
     if (l < a.k) {
       const uint32_t idx = key_index(list);
-      float w[E];
-      unpack<T>(load_chunk<T>(row + (int64_t)idx * (16 / E), 0, 1), w);
       a.top_ids[r * a.k + l] = (int64_t)idx;
-      a.top_logp[r * a.k + l] = none ? -INFINITY : (w[0] - t.m) * a.inv - log_s;
+      a.top_logp[r * a.k + l] = logp_of(element<T>(row, idx));
     }
   }
 }
@@ -258,9 +302,26 @@ __global__ __launch_bounds__(256) void logprobs_back_kernel(BackwardArgs a) {
   float lse = a.lse[r];
   const float h = a.entropy[r], gh = a.dentropy ? a.dentropy[r] : 0.f;
   float gl = target < 0 || !a.dlogp ? 0.f : target >= a.V ? NAN : a.dlogp[r], gz = a.dlse ? a.dlse[r] : 0.f;
+  // log p = l / T - lse is as exact as lse, which far from zero is not enough: there the row is summed again, by each wave
+  // for itself, and log p counted from its largest element.
+  float m = 0.f;
   if (lse == -INFINITY) {            // no mass: no element has a gradient
     lse = -LOWEST;
     gl = 0.f;
+  } else if (fabsf(lse) > 256.f) {
+    m = -INFINITY;
+    const int l = threadIdx.x & 63;
+    for_chunks<T, 1>(row, a.V, l, 64, [&](auto& v, int) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
+    });
+    m = across<1>(m, nullptr, [](float x, float y) { return fmaxf(x, y); });
+    float s = 0.f;
+    for_chunks<T, 1>(row, a.V, l, 64, [&](auto& v, int) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((v[e] - m) * a.inv * LOG2E);
+    });
+    lse = __builtin_amdgcn_logf(across<1>(s, nullptr, [](float x, float y) { return x + y; })) * LN2;
   }
   const float base = gz - gl - (gh != 0.f ? gh * h : 0.f), at_target = gl * a.inv;
   const int lanes = a.parts << a.lg, lane = ((int)(blockIdx.x % a.parts) << a.lg) + (threadIdx.x & ((1 << a.lg) - 1));
@@ -276,7 +337,7 @@ __global__ __launch_bounds__(256) void logprobs_back_kernel(BackwardArgs a) {
       unpack<T>(u[b], v);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float lp = fmaf(v[e], a.inv, -lse), p = __builtin_amdgcn_exp2f(lp * LOG2E);
+        const float lp = fmaf(v[e] - m, a.inv, -lse), p = __builtin_amdgcn_exp2f(lp * LOG2E);
         // where p is zero log p may be -inf: bounded, its product with p is zero
         v[e] = a.inv * p * fmaf(-gh, fmaxf(lp, -1e4f), base);
       }

@@ -661,7 +661,7 @@ def ref_token_logprobs(logits, targets, temperature: float = 1.0, top: int = 0, 
     lp = torch.where(none, ninf, d * inv - log_s)
     mean = (torch.where(e == 0, zero, d) * e).sum(-1, keepdim=True) / e.sum(-1, keepdim=True)
     entropy = torch.where(none, zero, log_s - inv * mean)
-    lse = torch.where(none, ninf, m * inv + log_s)
+    lse = torch.where(none, ninf, (m * inv + log_s).clamp(torch.finfo(x.dtype).min, torch.finfo(x.dtype).max))
     t = targets.unsqueeze(-1)
     logp = torch.where(t < 0, zero, torch.where(t >= V, zero / zero, lp.gather(-1, t.clamp(0, V - 1))))
     top_logp = top_ids = None
@@ -678,7 +678,9 @@ def ref_token_logprobs_backward(dlogp, dentropy, dlse, logits, targets, lse, ent
     none, t = (lse == -math.inf).unsqueeze(-1), targets.unsqueeze(-1)
     gl, gh, gz = (zero if g is None else g.to(x.dtype).unsqueeze(-1) for g in (dlogp, dentropy, dlse))
     gl = torch.where((t < 0) | none, zero, torch.where(t >= x.shape[-1], zero / zero, gl))
-    lp = torch.where(none, torch.full((), -math.inf, dtype=x.dtype, device=x.device), x * inv - lse.unsqueeze(-1))
+    # counted from the row's largest, which lse is not exact enough for far from zero
+    z = (x - torch.where(none, zero, x.amax(-1, keepdim=True))) * inv
+    lp = torch.where(none, torch.full((), -math.inf, dtype=x.dtype, device=x.device), z - torch.log(torch.exp(z).sum(-1, keepdim=True)))
     p = torch.exp(lp)
     plogp = torch.where(p == 0, p, p * lp)
     d = (gz - gl) * p - gh * (plogp + p * entropy.unsqueeze(-1))
