@@ -122,9 +122,31 @@ inline Geometry row_geometry(int64_t C, int vec, int most, bool far) {      // C
   return {lg, (int)ceil_div(chunks, (int64_t)1 << lg)};
 }
 
-template <int CTRL>
-__device__ __forceinline__ float dpp_add(float v) {
-  return v + __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(v), CTRL, 0xf, 0xf, true));
+// v of other lanes for a butterfly whose lanes hold equal values below the step: step 0 and 1 exchange with lane ^ 1 and ^ 2,
+// 2 with the other four of eight, 3 with the other eight of sixteen.
+template <int STEP>
+__device__ __forceinline__ float peer(float v) {
+  constexpr int ctrl = STEP == 0 ? 0xb1 : STEP == 1 ? 0x4e : STEP == 2 ? 0x141 : 0x140;
+  return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(v), ctrl, 0xf, 0xf, true));
+}
+// The values of the two 16-lane rows of a half, or of the two halves: (first, second) in all their lanes.
+struct Pair { float a, b; };
+template <bool HALVES>
+__device__ __forceinline__ Pair both(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = HALVES ? __builtin_amdgcn_permlane32_swap(u, u, false, false) : __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return {__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+// v of all 64 lanes joined by f, which takes its arguments in any order.
+template <class F>
+__device__ __forceinline__ float wave_joined(float v, F f) {
+  v = f(v, peer<0>(v));
+  v = f(v, peer<1>(v));
+  v = f(v, peer<2>(v));
+  v = f(v, peer<3>(v));
+  Pair p = both<false>(v);
+  p = both<true>(f(p.a, p.b));
+  return f(p.a, p.b);
 }
 // The sums of v over the 2^lg lanes of a row (lg >= 4), the same bits in each of them.  Rows of more than one wave meet in
 // `red` [2][N][waves]; every thread of the workgroup takes part, and the two halves take turns, so that one barrier a
@@ -133,17 +155,23 @@ template <int N>
 __device__ __forceinline__ void row_sums(float (&v)[N], int lg, float* red, int& turn) {
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    v[n] = dpp_add<0xb1>(v[n]);       // lane ^ 1
-    v[n] = dpp_add<0x4e>(v[n]);       // lane ^ 2
-    v[n] = dpp_add<0x141>(v[n]);      // the other four of eight
-    v[n] = dpp_add<0x140>(v[n]);      // the other eight of sixteen
+    v[n] += peer<0>(v[n]);
+    v[n] += peer<1>(v[n]);
+    v[n] += peer<2>(v[n]);
+    v[n] += peer<3>(v[n]);
   }
   if (lg > 4)
 #pragma unroll
-    for (int n = 0; n < N; ++n) v[n] += __shfl_xor(v[n], 16);
+    for (int n = 0; n < N; ++n) {
+      const Pair p = both<false>(v[n]);
+      v[n] = p.a + p.b;
+    }
   if (lg > 5)
 #pragma unroll
-    for (int n = 0; n < N; ++n) v[n] += __shfl_xor(v[n], 32);
+    for (int n = 0; n < N; ++n) {
+      const Pair p = both<true>(v[n]);
+      v[n] = p.a + p.b;
+    }
   if (lg > 6) {
     const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, per = 1 << (lg - 6);
     float* r = red + turn * N * waves;

@@ -60,6 +60,20 @@ __device__ __forceinline__ Triple join(Triple a, Triple b) {
   return {r, a.s + b.s, a.d + b.d};
 }
 
+// Of all lanes of a wave.
+__device__ __forceinline__ Triple wave_join(Triple t) {
+  t = join(t, {peer<0>(t.r), peer<0>(t.s), peer<0>(t.d)});
+  t = join(t, {peer<1>(t.r), peer<1>(t.s), peer<1>(t.d)});
+  t = join(t, {peer<2>(t.r), peer<2>(t.s), peer<2>(t.d)});
+  t = join(t, {peer<3>(t.r), peer<3>(t.s), peer<3>(t.d)});
+  Pair r = both<false>(t.r), s = both<false>(t.s), d = both<false>(t.d);
+  t = join({r.a, s.a, d.a}, {r.b, s.b, d.b});
+  r = both<true>(t.r), s = both<true>(t.s), d = both<true>(t.d);
+  return join({r.a, s.a, d.a}, {r.b, s.b, d.b});
+}
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float sum_of(float a, float b) { return a + b; }
+
 // The running state of a thread over its elements, and the largest of them.
 struct Running {
   Triple t = {LOWEST, 0.f, 0.f};
@@ -88,9 +102,7 @@ __device__ __forceinline__ float nth_of_wave(float v, int n) {
   if (n <= 8) {                                        // take the largest out n times; beyond that sorting is shorter
     float m = v;
     for (int i = 0;; ++i) {
-      m = v;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
+      m = wave_joined(v, larger);
       if (i == n - 1) return m;
       const uint64_t at = __ballot(v == m);
       if (lane == __builtin_ctzll(at)) v = -INFINITY;
@@ -146,8 +158,7 @@ __device__ __forceinline__ void for_chunks(const char* row, int V, int lane, int
 // v of all W waves' lanes joined.
 template <int W, class F>
 __device__ __forceinline__ float across(float v, float* shared, F f) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) v = f(v, __shfl_xor(v, off));
+  v = wave_joined(v, f);
   if constexpr (W > 1) {
     if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -177,9 +188,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void logprobs_kernel(Forward
   if (target >= 0 && target < a.V) lt = element<T>(row, (uint32_t)target);
   Running run;
   for_chunks<T, NB>(row, a.V, lane, LANES, [&](auto& v, int) { run.take(v, c); });
-  Triple t = run.t;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) t = join(t, {__shfl_xor(t.r, off), __shfl_xor(t.s, off), __shfl_xor(t.d, off)});
+  Triple t = wave_join(run.t);
   float bound = 0.f;
   if constexpr (TOP) {
     // each of W waves has k / W elements at or above its own k / W-th largest, and so all have k at or above the least of those
@@ -210,7 +219,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void logprobs_kernel(Forward
 #pragma unroll
       for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
     });
-    m = across<W>(m, s_far[0], [](float x, float y) { return fmaxf(x, y); });
+    m = across<W>(m, s_far[0], larger);
     m = m == -INFINITY ? 0.f : m;
     t = {0.f, 0.f, 0.f};
     for_chunks<T, 1>(row, a.V, lane, LANES, [&](auto& v, int) {
@@ -221,8 +230,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void logprobs_kernel(Forward
         t.d = fmaf(fmaxf(x, LOWEST), p, t.d);
       }
     });
-    t.s = across<W>(t.s, s_far[1], [](float x, float y) { return x + y; });
-    t.d = across<W>(t.d, s_far[2], [](float x, float y) { return x + y; });
+    t.s = across<W>(t.s, s_far[1], sum_of);
+    t.d = across<W>(t.d, s_far[2], sum_of);
   }
   const float log_s = __builtin_amdgcn_logf(t.s);
   const bool none = t.s == 0.f;                  // every logit is -inf: so are the log probabilities, and the entropy is 0
@@ -241,44 +250,61 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void logprobs_kernel(Forward
     if (run.best >= bound || run.t.s != run.t.s)
       for_chunks<T, NB>(row, a.V, lane, LANES, [&](auto& v, int first) {
         constexpr int N = sizeof(v) / sizeof(v[0]);
+        uint32_t hits = 0;
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          if (v[e] < bound) continue;
-          const int idx = first + (e / E) * LANES * E + e % E;
+        for (int e = 0; e < N; ++e) hits |= v[e] < bound ? 0u : 1u << e;
+        while (hits) {
+          const int e = __builtin_ctz(hits), idx = first + (e / E) * LANES * E + e % E;
+          hits &= hits - 1;
           if (idx >= a.V) continue;
-          const bool eq = v[e] == bound;
+          const float x = element<T>(row, (uint32_t)idx);
+          const bool eq = x == bound;
           if (eq && *(volatile int*)&count[1] >= CAP) continue;        // more than will be read are not counted on
           const int at = atomicAdd(&count[eq], 1);
-          if (at < CAP) (eq ? equal : above)[at] = order_key(v[e], (uint32_t)idx);
+          if (at < CAP) (eq ? equal : above)[at] = order_key(x, (uint32_t)idx);
         }
       });
     if constexpr (W > 1) __syncthreads();
     else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int n = *(volatile int*)&count[0], ties = *(volatile int*)&count[1];
+    const auto put = [&](int rank, key64 key) {
+      a.top_ids[r * a.k + rank] = (int64_t)key_index(key);
+      a.top_logp[r * a.k + rank] = logp_of(key_score(key));
+    };
+    if (n <= CAP && (n >= a.k || ties < CAP)) {
+      // an element's place is the number of those ahead of it; equal ones come behind those above the bound
+      for (int j = lane; j < n; j += LANES) {
+        const key64 key = above[j];
+        int rank = 0;
+        for (int i = 0; i < n; ++i) rank += above[i] > key;
+        if (rank < a.k) put(rank, key);
+      }
+      if (n < a.k)
+        for (int j = lane; j < ties; j += LANES) {
+          const key64 key = equal[j];
+          int rank = n;
+          for (int i = 0; i < ties; ++i) rank += equal[i] > key;
+          if (rank < a.k) put(rank, key);
+        }
+      return;
+    }
     if (wave != 0) return;
-    const int l = threadIdx.x & 63, n = *(volatile int*)&count[0], ties = *(volatile int*)&count[1];
+    const int l = threadIdx.x & 63;
     key64 list = KEY_NONE;
     if (n <= CAP) {
+      // many of one value: the first ones of the row, in order
       for (int i = 0; i < n; i += 64) list = wave_merge_topk(list, i + l < n ? above[i + l] : KEY_NONE, 64);
-      if (n < a.k && ties < CAP) {
-        for (int i = 0; i < ties; i += 64) list = wave_merge_topk(list, i + l < ties ? equal[i + l] : KEY_NONE, 64);
-      } else if (n < a.k) {
-        // many of one value: the first ones of the row, in order
-        for (int i = 0, found = n; i < a.V && found < a.k; i += 64) {
-          const float v = i + l < a.V ? element<T>(row, (uint32_t)(i + l)) : NAN;
-          found += __popcll(__ballot(v == bound));
-          list = wave_merge_topk(list, v == bound ? order_key(v, (uint32_t)(i + l)) : KEY_NONE, 64);
-        }
+      for (int i = 0, found = n; i < a.V && found < a.k; i += 64) {
+        const float v = i + l < a.V ? element<T>(row, (uint32_t)(i + l)) : NAN;
+        found += __popcll(__ballot(v == bound));
+        list = wave_merge_topk(list, v == bound ? order_key(v, (uint32_t)(i + l)) : KEY_NONE, 64);
       }
     } else {
       // more above the bound than there is room for: a row whose largest elements are a few threads' own
       for (int i = 0; i < a.V; i += 64)
         list = wave_merge_topk(list, i + l < a.V ? order_key(element<T>(row, (uint32_t)(i + l)), (uint32_t)(i + l)) : KEY_NONE, a.k);
     }
-    if (l < a.k) {
-      const uint32_t idx = key_index(list);
-      a.top_ids[r * a.k + l] = (int64_t)idx;
-      a.top_logp[r * a.k + l] = logp_of(element<T>(row, idx));
-    }
+    if (l < a.k) put(l, list);
   }
 }
 
@@ -315,13 +341,13 @@ __global__ __launch_bounds__(256) void logprobs_back_kernel(BackwardArgs a) {
 #pragma unroll
       for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
     });
-    m = across<1>(m, nullptr, [](float x, float y) { return fmaxf(x, y); });
+    m = across<1>(m, nullptr, larger);
     float s = 0.f;
     for_chunks<T, 1>(row, a.V, l, 64, [&](auto& v, int) {
 #pragma unroll
       for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((v[e] - m) * a.inv * LOG2E);
     });
-    lse = __builtin_amdgcn_logf(across<1>(s, nullptr, [](float x, float y) { return x + y; })) * LN2;
+    lse = __builtin_amdgcn_logf(across<1>(s, nullptr, sum_of)) * LN2;
   }
   const float base = gz - gl - (gh != 0.f ? gh * h : 0.f), at_target = gl * a.inv;
   const int lanes = a.parts << a.lg, lane = ((int)(blockIdx.x % a.parts) << a.lg) + (threadIdx.x & ((1 << a.lg) - 1));
