@@ -169,7 +169,7 @@ __device__ __forceinline__ float across(float v, float* shared, F f) {
   return v;
 }
 
-// W waves a row.  One wave for short rows, four of them in a workgroup; otherwise the workgroup is one row's.
+// W waves a row (row_waves says how many).  With one, a workgroup has four rows; otherwise it is one row's.
 template <class T, int W, bool TOP>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void logprobs_kernel(ForwardArgs a) {
   constexpr int E = Traits<T>::VEC, NB = 32 / E, LANES = 64 * W, GROUPS = W == 1 ? 4 : 1, CAP = W == 1 ? 256 : 1024;
@@ -400,6 +400,17 @@ static int check_row_vec(const maba_tensor* t, const char* who, const char* name
   if (rows > 0 && !t->data) return fail(MABA_ERR_INVALID, "%s: %s has no data", who, name);
   return MABA_OK;
 }
+// Waves a row, of 1, 2, 4 and 8.  Many rows: as few as leave a thread 16 chunks, since what a row costs besides its elements
+// (its waves' sums joined, the barriers) grows with them.  Few rows: as many as leave each thread a chunk, while all
+// rows' waves are at most eight a compute unit.  In us for bf16 with five alternatives, 1 / 2 / 4 / 8 waves:
+//   4,096 x 8,000   25 / 29 / 31 / 41      4,096 x 32,768   79 / 75 / 64 / 71      4,096 x 65,536   156 / 143 / 121 / 115
+//   16 x 2,000      8.3 / 5.8 / 5.1 / 34 (waves without a chunk bound nothing)     16 x 32,768      28 / 14 / 11 / 8.7
+static int row_waves(int64_t rows, int64_t chunks) {
+  int w = 1;
+  while (w < 8 && chunks > 16 * 64 * w) w *= 2;
+  while (w < 8 && chunks >= 2 * 64 * w && rows * 2 * w <= 8 * (int64_t)device_cu_count()) w *= 2;
+  return w;
+}
 static Logits logits_of(const maba_tensor* t) {
   const int64_t size = t->dtype == MABA_F32 ? 4 : 2;
   if (t->ndim == 2) return {(const char*)t->data, 0, t->stride[0] * size, std::max<int64_t>(t->shape[0], 1)};
@@ -444,13 +455,15 @@ extern "C" int maba_hip_token_logprobs(const maba_tensor* logits, const maba_ten
   const ForwardArgs a = {logits_of(logits), (const int64_t*)targets->data, (float*)logp->data, (float*)entropy->data, (float*)lse->data,
                          k ? (float*)top_logp->data : nullptr, k ? (int64_t*)top_ids->data : nullptr, R, (int)V, (int)k,
                          (float)(1.0 / temperature)};
-  const bool small = V <= 4096;
-  const dim3 grid((unsigned)(small ? ceil_div(R, 4) : R)), block(small ? 256 : 512);
+  const int waves = row_waves(R, ceil_div(V, logits->dtype == MABA_F32 ? 4 : 8));
+  const dim3 grid((unsigned)(waves == 1 ? ceil_div(R, 4) : R)), block(waves == 1 ? 256 : 64 * waves);
   auto run = [&](auto type) {
     typedef decltype(type) T;
-    auto kernel = small ? (k ? logprobs_kernel<T, 1, true> : logprobs_kernel<T, 1, false>)
-                        : (k ? logprobs_kernel<T, 8, true> : logprobs_kernel<T, 8, false>);
-    hipLaunchKernelGGL(kernel, grid, block, 0, (hipStream_t)stream, a);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, (hipStream_t)stream, a); };
+    if (waves == 1) go(k ? logprobs_kernel<T, 1, true> : logprobs_kernel<T, 1, false>);
+    else if (waves == 2) go(k ? logprobs_kernel<T, 2, true> : logprobs_kernel<T, 2, false>);
+    else if (waves == 4) go(k ? logprobs_kernel<T, 4, true> : logprobs_kernel<T, 4, false>);
+    else go(k ? logprobs_kernel<T, 8, true> : logprobs_kernel<T, 8, false>);
   };
   if (logits->dtype == MABA_F32) run(F32());
   else if (logits->dtype == MABA_BF16) run(Bf16());
