@@ -330,7 +330,7 @@ __global__ __launch_bounds__(1 << MAX_LG) void boundary_back_kernel(BoundaryBack
   }
 }
 
-// out[c] = factor * the sum over g of p[g][n][c], in the order of g within each of sixteen runs and of the runs.
+// out[c] = factor * the sum over g of p[g][n][c]: 32 runs of g side by side, each in its order, then the runs in theirs.
 struct ColumnsArgs {
   const float* p;
   void* out[3];
@@ -339,20 +339,21 @@ struct ColumnsArgs {
 };
 template <class T>
 __global__ __launch_bounds__(1024) void columns_kernel(ColumnsArgs a) {
-  __shared__ float part[16][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), run = threadIdx.x >> 6, n = blockIdx.y;
+  constexpr int RUNS = 32;
+  __shared__ float part[RUNS][32];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), run = threadIdx.x >> 5, n = blockIdx.y;
   float s = 0.f;
   if (c < a.C) {
     const float* p = a.p + (int64_t)n * a.C + c;
 #pragma unroll 8
-    for (int g = run; g < a.groups; g += 16) s += p[(int64_t)g * a.n * a.C];
+    for (int g = run; g < a.groups; g += RUNS) s += p[(int64_t)g * a.n * a.C];
   }
-  part[run][threadIdx.x & 63] = s;
+  part[run][threadIdx.x & 31] = s;
   __syncthreads();
   if (run == 0 && c < a.C) {
     float v = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v += part[i][threadIdx.x];
+    for (int i = 0; i < RUNS; ++i) v += part[i][threadIdx.x];
     v *= a.factor[n];
     if constexpr (T::CODE == MABA_F32) ((float*)a.out[n])[c] = v;
     else ((uint16_t*)a.out[n])[c] = (uint16_t)T::down(v);
@@ -429,14 +430,20 @@ static bool whole_rows(std::initializer_list<const maba_tensor*> all) {
     }
   return true;
 }
-// Elements of a row a lane has: what is kept of them fits the registers of two waves a SIMD.
-constexpr int FORWARD_ELEMS = 24;
-static constexpr int back_elems(bool post, bool f32) { return post || f32 ? 16 : 24; }
+// Elements of a row a lane has.  Few give every row more lanes and the chip more waves; more leave fewer lanes without work
+// (80 chunks of 640 16-bit elements fill 62 % of 128 lanes and 83 % of 32 with three each) and share out what a row costs
+// besides its elements.  Forward, in us, 8 / 24 elements: 1 x 640 bf16 3.1 / 4.1, 2,048 x 640 5.5 / 5.8, 32,768 x 640
+// 42.8 / 32.8, 8,192 x 4,096 50.5 / 47.3; fp32 8,192 x 1,000 22.9 / 24.6.  Backward, 8 / 16: 64 x 640 8.6 / 10.4, 16,384 x 640
+// 39.6 / 39.4, 2,048 x 4,096 37 / 43, 8,192 x 4,096 98 / 103.
+constexpr int MOST_ELEMS = 24, MOST_BACK = 16;
+static int forward_elems(int64_t R, int64_t C, int dtype) { return C > 8 << MAX_LG ? 16 : dtype != MABA_F32 && R > 4096 ? MOST_ELEMS : 8; }
+static int back_elems(int64_t C) { return C > 8 << MAX_LG ? MOST_BACK : 8; }
 static int row_threads(int lg) { return std::max(256, 1 << lg); }
-// The workgroups of a backward pass: two waves a SIMD, which its registers allow.
-static int back_groups(int64_t R, int lg) {
-  const int threads = row_threads(lg);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(R, threads >> lg), (int64_t)device_cu_count() * (512 / threads)));
+// The workgroups of a backward pass: as many as are resident at once (three of 256 threads a compute unit, two of 512, one
+// with 16 elements a lane) write the fewest partials.
+static int back_groups(int64_t R, int64_t C, int lg) {
+  const int threads = row_threads(lg), each = threads == 256 ? 3 : back_elems(C) == 8 ? 2 : 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(R, threads >> lg), (int64_t)device_cu_count() * each));
 }
 template <int N>
 struct Num { static constexpr int value = N; };
@@ -509,7 +516,7 @@ extern "C" int maba_hip_residual_norm(const maba_tensor* x, const maba_tensor* y
   if (overlap(h, x) || overlap(h, y) || overlap(h, x_out) || overlap(x_out, y) || (overlap(x_out, x) && !same_place(x_out, x)))
     return fail(MABA_ERR_INVALID, "%s: tensors overlap", who);
   if (C > MAX_WIDTH) return fail(MABA_ERR_UNSUPPORTED, "%s: at most %d channels", who, MAX_WIDTH);
-  const Geometry geo = row_geometry(C, chunk_elems(dt), FORWARD_ELEMS, far_rows({x, y, x_out, h}));
+  const Geometry geo = row_geometry(C, chunk_elems(dt), forward_elems(R, C, dt), far_rows({x, y, x_out, h}));
   BoundaryArgs a = {x->data, y ? y->data : nullptr, weight ? weight->data : nullptr, post_weight ? post_weight->data : nullptr,
                     gate ? gate->data : nullptr, x_out ? x_out->data : nullptr, h ? h->data : nullptr,
                     x->stride[0], y ? y->stride[0] : 0, x_out ? x_out->stride[0] : 0, h ? h->stride[0] : 0, R, (int)C, geo.lg,
@@ -519,7 +526,7 @@ extern "C" int maba_hip_residual_norm(const maba_tensor* x, const maba_tensor* y
   const dim3 grid((unsigned)std::min<int64_t>(ceil_div(R, threads >> geo.lg), (int64_t)device_cu_count() * 8));
   with_type(dt, [&](auto type) {
     typedef decltype(type) T;
-    with_chunks<T, FORWARD_ELEMS>(geo.nch, [&](auto n) {
+    with_chunks<T, T::CODE == MABA_F32 ? MOST_BACK : MOST_ELEMS>(geo.nch, [&](auto n) {
       hipLaunchKernelGGL((boundary_kernel<T, decltype(n)::value>), grid, dim3(threads), 0, (hipStream_t)stream, a);
     });
   });
@@ -529,11 +536,10 @@ extern "C" int maba_hip_residual_norm(const maba_tensor* x, const maba_tensor* y
 extern "C" size_t maba_hip_residual_norm_backward_workspace_size(const maba_tensor* x_out, int grads) {
   if (!x_out || x_out->ndim != 2 || x_out->shape[1] < 1 || !is_float_dt(x_out->dtype) || !(grads & 7)) return 0;
   if (x_out->shape[1] > MAX_WIDTH) return 0;
-  int groups = 0;                                  // the most that any call on these rows has
-  for (bool post : {false, true})
-    groups = std::max(groups, back_groups(x_out->shape[0],
-                                          row_geometry(x_out->shape[1], chunk_elems(x_out->dtype), back_elems(post, x_out->dtype == MABA_F32), true).lg));
-  return (size_t)groups * __builtin_popcount(grads & 7) * x_out->shape[1] * sizeof(float);
+  const int64_t R = x_out->shape[0], C = x_out->shape[1];
+  // (rows far apart have the most lanes, and so the most workgroups)
+  return (size_t)back_groups(R, C, row_geometry(C, chunk_elems(x_out->dtype), back_elems(C), true).lg) * __builtin_popcount(grads & 7) *
+         C * sizeof(float);
 }
 
 extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const maba_tensor* dh, const maba_tensor* x_out,
@@ -572,10 +578,10 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
       if (overlap(outs[i], outs[j])) return fail(MABA_ERR_INVALID, "%s: outputs overlap", who);
   }
   if (C > MAX_WIDTH) return fail(MABA_ERR_UNSUPPORTED, "%s: at most %d channels", who, MAX_WIDTH);
-  const Geometry geo = row_geometry(C, chunk_elems(dt), back_elems(post_weight, dt == MABA_F32), far_rows({dx_out, dh, x_out, y, dx, dy}));
+  const Geometry geo = row_geometry(C, chunk_elems(dt), back_elems(C), far_rows({dx_out, dh, x_out, y, dx, dy}));
   const int grads = (dweight ? GRAD_W : 0) | (dgate ? GRAD_GATE : 0) | (dpost_weight ? GRAD_POST : 0);
   if (!grads && !dx && !dy) return MABA_OK;
-  const int groups = back_groups(R, geo.lg), n = __builtin_popcount(grads);
+  const int groups = back_groups(R, C, geo.lg), n = __builtin_popcount(grads);
   rc = ffn::check_workspace(who, workspace, workspace_bytes, (size_t)groups * n * C * sizeof(float));
   if (rc) return rc;
   const bool need_y = post_weight || dgate;
@@ -596,12 +602,12 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
         hipLaunchKernelGGL(kernel, dim3(groups), dim3(threads), lds, (hipStream_t)stream, a);
       };
       if (post_weight)
-        with_chunks<T, back_elems(true, T::CODE == MABA_F32)>(geo.nch, [&](auto n) {
+        with_chunks<T, MOST_BACK>(geo.nch, [&](auto n) {
           constexpr int N = decltype(n)::value;
           run(whole ? boundary_back_kernel<T, N, true, true> : boundary_back_kernel<T, N, true, false>);
         });
       else
-        with_chunks<T, back_elems(false, T::CODE == MABA_F32)>(geo.nch, [&](auto n) {
+        with_chunks<T, MOST_BACK>(geo.nch, [&](auto n) {
           constexpr int N = decltype(n)::value;
           run(whole ? boundary_back_kernel<T, N, false, true> : boundary_back_kernel<T, N, false, false>);
         });
@@ -616,7 +622,7 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
     if (dgate) { c.out[k] = dgate->data; c.factor[k++] = scale; }
     if (dpost_weight) { c.out[k] = dpost_weight->data; c.factor[k++] = 1.f; }
     auto f = dt == MABA_F32 ? columns_kernel<F32> : dt == MABA_BF16 ? columns_kernel<Bf16> : columns_kernel<Fp16>;
-    hipLaunchKernelGGL(f, dim3((unsigned)ceil_div(C, 64), n), dim3(1024), 0, (hipStream_t)stream, c);
+    hipLaunchKernelGGL(f, dim3((unsigned)ceil_div(C, 32), n), dim3(1024), 0, (hipStream_t)stream, c);
     return check_launch(who);
   }
   return MABA_OK;

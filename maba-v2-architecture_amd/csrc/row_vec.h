@@ -115,7 +115,7 @@ constexpr int MAX_LG = 9, MAX_WIDTH = 16 << MAX_LG;
 struct Geometry {
   int lg, nch;
 };
-inline Geometry row_geometry(int64_t C, int vec, int most, bool far) {      // C <= MAX_WIDTH, most >= 16
+inline Geometry row_geometry(int64_t C, int vec, int most, bool far) {      // C <= most << MAX_LG
   const int64_t chunks = ceil_div(C, vec);
   int lg = far ? 6 : 4;
   while (chunks > (int64_t)(most / vec) << lg) ++lg;
