@@ -45,7 +45,9 @@ __device__ __forceinline__ key64 order_key(float v, uint32_t idx) {
   return ((key64)o << 32) | (key64)(~idx);
 }
 
-// R is a whole number or LOWEST (no element yet, or none above it).
+// R is a whole number of at least FLOOR.  Up to -FLOOR the product that it is rounded up from is off by 64 at most, and 2^x
+// stays in range; elements far below FLOOR have no part in S.
+constexpr float FLOOR = -1073741824.f;
 struct Triple { float r, s, d; };
 // (s, d) with the reference raised by -by, f = 2^by.  by may be past fp32's range, and f is zero then.
 __device__ __forceinline__ void raise(float& s, float& d, float by) {
@@ -76,7 +78,7 @@ __device__ __forceinline__ float sum_of(float a, float b) { return a + b; }
 
 // The running state of a thread over its elements, and the largest of them.
 struct Running {
-  Triple t = {LOWEST, 0.f, 0.f};
+  Triple t = {FLOOR, 0.f, 0.f};
   float best = -INFINITY;
   template <int N>
   __device__ __forceinline__ void take(const float (&v)[N], float c) {
@@ -209,9 +211,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void logprobs_kernel(Forward
       bound = fminf(bound, s_nth[w]);
     }
   }
-  // No sum, or none that is a number: every logit is -inf, or one is NaN or +inf, or the largest times c leaves fp32's
-  // range, as where a mask of the type's lowest value leaves nothing else.  Again, then, from the largest itself.
-  const bool far = !(t.s > 0.f);
+  // No sum, or none that is a number, or a reference out of range: every logit is -inf, or one is NaN or +inf, or the
+  // largest is far from zero, as where a mask of the type's lowest value leaves nothing else.  Again, then, from the largest itself.
+  const bool far = !(t.s > 0.f) || t.r > -FLOOR;
   float m = 0.f;
   if (far) {
     m = -INFINITY;
@@ -237,7 +239,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void logprobs_kernel(Forward
   const bool none = t.s == 0.f;                  // every logit is -inf: so are the log probabilities, and the entropy is 0
   float lse = far ? fmaf(m, a.inv, log_s * LN2) : (t.r + log_s) * LN2;
   if (!none) lse = lse < LOWEST ? LOWEST : lse > -LOWEST ? -LOWEST : lse;       // -inf says that there is no mass
-  const auto logp_of = [&](float l) { return none ? -INFINITY : ((far ? (l - m) * c : fmaf(l, c, -t.r)) - log_s) * LN2; };
+  const auto logp_of = [&](float l) {
+    const float v = ((far ? (l - m) * c : fmaf(l, c, -t.r)) - log_s) * LN2;
+    // c is above 1 / T: a masked token's lowest value can leave fp32's range in base 2 alone
+    return none ? -INFINITY : v == -INFINITY && l != -INFINITY ? fmaf(l, a.inv, -lse) : v;
+  };
   if (lane == 0) {
     a.lse[r] = lse;
     a.entropy[r] = none ? 0.f : (log_s - t.d / t.s) * LN2;

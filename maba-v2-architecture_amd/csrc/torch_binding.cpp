@@ -74,7 +74,8 @@ struct Desc {
       if (!keep.is_contiguous()) keep = keep.contiguous();
     } else {
       if (keep.dim() != 2) keep = keep.reshape({-1, keep.size(-1)});
-      if (keep.size(1) != 1 && keep.stride(1) != 1) keep = keep.contiguous();
+      if (keep.size(1) != 1 && keep.stride(1) != 1)       // (without rows contiguous() may leave any strides as they are)
+        keep = keep.size(0) ? keep.contiguous() : at::empty(keep.sizes(), keep.options());
     }
     d.data = keep.data_ptr();
     d.dtype = code_of(keep);
@@ -399,7 +400,8 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
 // Logits as [M, V] or [B, L, V] with unit column stride.
 Tensor logit_rows(const Tensor& t) {
   Tensor r = t.dim() == 2 || t.dim() == 3 ? t : t.reshape({-1, t.size(-1)});
-  return r.stride(-1) != 1 && r.size(-1) != 1 ? r.contiguous() : r;
+  if (r.stride(-1) == 1 || r.size(-1) == 1) return r;
+  return r.numel() ? r.contiguous() : at::empty(r.sizes(), r.options());
 }
 maba_tensor desc3(const Tensor& t) {
   maba_tensor d = {t.data_ptr(), code_of(t), (int)t.dim(), {1, 1, 1, 1}, {0, 0, 0, 0}};

@@ -240,8 +240,8 @@ def rows_of(t: Optional[torch.Tensor]):
     n, st = t.shape, t.stride()
     if len(n) != 2 or (st[1] != 1 and n[1] != 1):
         t = t.reshape(-1, n[-1])
-        if t.stride(1) != 1 and n[-1] != 1:
-            t = t.contiguous()
+        if t.stride(1) != 1 and n[-1] != 1:         # (without rows contiguous() may leave any strides as they are)
+            t = t.contiguous() if t.shape[0] else t.new_empty(t.shape)
         return t, rows_desc(t)
     code = _DTYPE_CODES.get(t.dtype)
     if code is None:

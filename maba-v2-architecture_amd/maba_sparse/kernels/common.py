@@ -566,7 +566,7 @@ def philox_words(rows: int, cols: int, seed, stream: int = 0) -> torch.Tensor:
         a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57          # modulo 2^64: the shift's sign bits are masked off
         c = [((b >> 32) & low) ^ c[1] ^ k0, b & low, ((a >> 32) & low) ^ c[3] ^ k1, a & low]
         k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
-    return torch.stack(torch.broadcast_tensors(*c), dim=-1).reshape(rows, -1)[:, :cols]
+    return torch.stack(torch.broadcast_tensors(*c), dim=-1).flatten(-2)[:, :cols]
 
 
 def _dropped(v, p, seed, stream):

@@ -505,7 +505,9 @@ def _logit_rows(t):
     """``t [..., V]`` as [M, V] or [B, L, V] with unit column stride, a view where the strides allow it."""
     if t.dim() not in (2, 3):
         t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    if t.stride(-1) == 1 or t.shape[-1] == 1:
+        return t
+    return t.contiguous() if t.numel() else t.new_empty(t.shape)
 
 
 @register_kernel("hip", "token_logprobs")
