@@ -8,8 +8,9 @@ prefill, then single-token steps in which the DGDA blocks carry their recurrent 
 states and the MABA-SA blocks decode over a preallocated ``LatentCache`` (incremental
 latent rows, HCA means and indexer centroids) instead of the reference's per-step
 ``torch.cat`` of the whole cache (``model.py:280-313`` with ``sparse_attention.py:241-261``).
-The multi-token-prediction head and the loss are training-side and are not built here; the
-feed-forward half of a block trains on the GPU with ``MabaConfig.fused_ffn``.
+The multi-token-prediction head is training-side and is not built here.  ``score`` gives the log
+probabilities that a loss is made from; the feed-forward half of a block trains on the GPU with
+``MabaConfig.fused_ffn`` and the boundaries between the halves with ``fused_boundary``.
 """
 from __future__ import annotations
 
@@ -21,7 +22,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from maba_sparse.layers._wcache import WeightCacheMixin, cached
-from maba_sparse.kernels.dispatcher import gated_ffn, get_backend, linear_epilogue
+from maba_sparse.kernels.dispatcher import (dropout, gated_ffn, get_backend, linear_epilogue, residual_norm,
+                                            token_logprobs)
 from maba_sparse.layers.dgda import DGDALayer
 from maba_sparse.layers.sparse_attention import DeviceCache, LatentCache, MabaSparseAttention
 
@@ -54,6 +56,14 @@ class MabaConfig:
     fused_ffn: bool = False
     # With fused_ffn: what those operators keep for the backward pass, None (16 bits) or "e4m3" (8 bits).
     ffn_checkpoint: Optional[str] = None
+    # The boundaries between a block's halves (gated residual and the norm that follows it) through the dispatcher's
+    # residual_norm, forward and backward.  So are they with any of the next three, which the reference does not have:
+    # a norm on each half's output (post_norm1 and post_norm2 of a block), a constant factor on what a half
+    # adds to the residual stream, and dropout on it and on the embeddings while training.
+    fused_boundary: bool = False
+    post_norm: bool = False
+    residual_scale: float = 1.0
+    dropout: float = 0.0
 
 
 def get_101m_config(**overrides: Any) -> MabaConfig:
@@ -127,6 +137,9 @@ class FactorizedEmbeddings(nn.Module):
 
 
 class MabaBlock(WeightCacheMixin, nn.Module):
+    # of a module that was saved without them
+    boundary, residual_scale, dropout = False, 1.0, 0.0
+
     def __init__(self, config: MabaConfig, layer_idx: int) -> None:
         super().__init__()
         self.layer_idx = layer_idx
@@ -138,8 +151,32 @@ class MabaBlock(WeightCacheMixin, nn.Module):
                              getattr(config, "ffn_checkpoint", None))
         self.res_gate1 = nn.Parameter(torch.full((config.dim,), config.residual_gate_bias))
         self.res_gate2 = nn.Parameter(torch.full((config.dim,), config.residual_gate_bias))
+        self.residual_scale = getattr(config, "residual_scale", 1.0)
+        self.dropout = getattr(config, "dropout", 0.0)
+        if getattr(config, "post_norm", False):
+            self.post_norm1 = RMSNorm(config.dim, eps=config.rms_norm_eps)
+            self.post_norm2 = RMSNorm(config.dim, eps=config.rms_norm_eps)
+        self.boundary = getattr(config, "fused_boundary", False) or self.extended or self.dropout > 0
+
+    @property
+    def extended(self) -> bool:
+        """Whether the boundaries are more than a gated residual and a norm outside training."""
+        return "post_norm1" in self._modules or self.residual_scale != 1.0
+
+    def boundary_args(self, half: int, seed: Optional[torch.Tensor] = None) -> dict:
+        """What ``residual_norm`` takes at the end of the block's first or second half besides the stream, the half's
+        output and the next norm; with a ``seed`` (training) dropout."""
+        post = self._modules.get(f"post_norm{half}")
+        gate = _frozen(self, f"g{half}", torch.sigmoid, self.res_gate1 if half == 1 else self.res_gate2)
+        args = dict(post_weight=None if post is None else post.weight, gate=gate, scale=self.residual_scale)
+        if seed is not None:
+            args.update(p=self.dropout, seed=seed, stream=2 * self.layer_idx + half)
+        return args
 
     def _residual(self, x: torch.Tensor, mo: torch.Tensor) -> torch.Tensor:
+        if self.boundary:
+            x, h = residual_norm(x, mo, weight=self.norm2.weight, eps=self.norm2.eps, **self.boundary_args(1))
+            return residual_norm(x, self.ffn(h), eps=self.norm2.eps, **self.boundary_args(2))[0]
         g1 = _frozen(self, "g1", torch.sigmoid, self.res_gate1)
         g2 = _frozen(self, "g2", torch.sigmoid, self.res_gate2)
         x = torch.addcmul(x, g1, mo)
@@ -224,18 +261,21 @@ class ServingStep:
         x = m.embeddings(self.tok)
         n1 = layers[0].norm1
         h = hb.hip_rmsnorm(x, n1.weight, n1.eps)
+
+        def end(layer, half, mo, norm):          # of a block's half: the stream in place, and its norm
+            if layer.extended:
+                return hb.hip_residual_norm(x, mo, weight=norm.weight, eps=norm.eps, x_out=x, **layer.boundary_args(half))[1]
+            g = _frozen(layer, f"g{half}", torch.sigmoid, layer.res_gate1 if half == 1 else layer.res_gate2)
+            return hb.hip_rmsnorm(x, norm.weight, norm.eps, mo=mo, gate=g, x_out=x)
+
         for i, layer in enumerate(layers):
             if layer.is_attention:
                 mo = layer.mixer.decode_step_device(h, self.caches[i], self.counters)
             else:
                 st, hs = self.dgda[i]
                 mo = layer.mixer.step_device(h, st, hs)
-            g1 = _frozen(layer, "g1", torch.sigmoid, layer.res_gate1)
-            g2 = _frozen(layer, "g2", torch.sigmoid, layer.res_gate2)
-            h2 = hb.hip_rmsnorm(x, layer.norm2.weight, layer.norm2.eps, mo=mo, gate=g1, x_out=x)
-            f = layer.ffn.forward_hip(h2)
-            nxt = layers[i + 1].norm1 if i + 1 < len(layers) else m.final_norm
-            h = hb.hip_rmsnorm(x, nxt.weight, nxt.eps, mo=f, gate=g2, x_out=x)
+            f = layer.ffn.forward_hip(end(layer, 1, mo, layer.norm2))
+            h = end(layer, 2, f, layers[i + 1].norm1 if i + 1 < len(layers) else m.final_norm)
         self.last = m.lm_head(m.head_proj(h))[:, -1]
         self.tok.copy_(self.last.argmax(dim=-1, keepdim=True))
         self.counters += 1
@@ -317,6 +357,9 @@ class MabaSparseForCausalLM(WeightCacheMixin, nn.Module):
         self.lm_head = nn.Linear(c.d_emb, c.vocab_size, bias=False)
         self.lm_head.weight = self.embeddings.in_emb.weight      # tied (model.py:205)
         self._install_weight_cache_hooks()
+        if getattr(c, "dropout", 0.0) > 0:
+            # the next training step's masks; not part of the state dict
+            self.register_buffer("dropout_seed", torch.randint(0, 2 ** 62, (1,)), persistent=False)
 
     def init_normal(self, std: float = 0.02) -> "MabaSparseForCausalLM":
         """Every weight matrix and embedding ~ N(0, std) (the BASELINE's random init); norms,
@@ -337,6 +380,8 @@ class MabaSparseForCausalLM(WeightCacheMixin, nn.Module):
         x = self.embeddings(input_ids)
         if self._fused_norms_ok(x):
             return self._forward_fused_norms(x, past_states, last_only)
+        if self.layers[0].boundary:
+            return self._forward_boundary(x, past_states, last_only)
         nps = []
         for i, layer in enumerate(self.layers):
             st, cv, pk = past_states[i] if past_states is not None else (None, None, None)
@@ -351,6 +396,8 @@ class MabaSparseForCausalLM(WeightCacheMixin, nn.Module):
         if x.device.type != "cuda" or get_backend(x.device) != "hip" or x.dtype != torch.bfloat16:
             return False
         if c.dim % 2 or c.dim > 2048 or c.intermediate_size % 2:
+            return False
+        if any(layer.extended or (layer.training and layer.dropout > 0) for layer in self.layers):
             return False
         return not (torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters()))
 
@@ -379,6 +426,49 @@ class MabaSparseForCausalLM(WeightCacheMixin, nn.Module):
             h = hb.hip_rmsnorm(x, nxt.weight, nxt.eps, mo=f, gate=g2, x_out=x)
             nps.append((nst, ncv, nck))
         return self.lm_head(self.head_proj(h[:, -1:] if last_only else h)), nps
+
+    def next_dropout_seed(self) -> Optional[torch.Tensor]:
+        """The seed of this training step's masks, on which ``dropout_seed`` moves on (also where the step is replayed
+        from a captured graph); None where nothing is dropped.  Ranks of a data-parallel job start it from different values."""
+        if not self.training or getattr(self, "dropout_seed", None) is None:
+            return None
+        with torch.no_grad():
+            seed = self.dropout_seed.clone()
+            self.dropout_seed += 1
+        return seed
+
+    def _forward_boundary(self, x: torch.Tensor, past_states, last_only: bool = False):
+        """``forward`` with every boundary, the final norm's among them, as one ``residual_norm``: the end of each half of
+        a block together with the norm that comes next."""
+        seed = self.next_dropout_seed()
+        if seed is not None:
+            x = dropout(x, self.config.dropout, seed)
+        layers = self.layers
+        x, h = residual_norm(x, weight=layers[0].norm1.weight, eps=layers[0].norm1.eps)
+        nps = []
+        for i, layer in enumerate(layers):
+            st, cv, pk = past_states[i] if past_states is not None else (None, None, None)
+            nst = ncv = nck = None
+            if layer.is_attention:
+                mo, nck = layer.mixer(h, past_c_kv=pk)
+            else:
+                mo, nst, ncv = layer.mixer(h, state=st, conv_state=cv)
+            x, h = residual_norm(x, mo, weight=layer.norm2.weight, eps=layer.norm2.eps, **layer.boundary_args(1, seed))
+            nxt = layers[i + 1].norm1 if i + 1 < len(layers) else self.final_norm
+            x, h = residual_norm(x, layer.ffn(h), weight=nxt.weight, eps=nxt.eps, **layer.boundary_args(2, seed))
+            nps.append((nst, ncv, nck))
+        return self.lm_head(self.head_proj(h[:, -1:] if last_only else h)), nps
+
+    def score(self, input_ids: torch.Tensor, temperature: float = 1.0, top: int = 0):
+        """What the model says of each token of ``input_ids [B, L]`` given those before it: ``token_logprobs``'
+        ``(logp, entropy, lse, top_logp, top_ids)``, ``[B, L - 1]`` and ``[B, L - 1, top]``.  Under autograd
+        ``-logp.mean()`` is the language-model loss."""
+        if input_ids.shape[1] < 2:
+            raise ValueError(f"score() needs at least two tokens, got L={input_ids.shape[1]}")
+        logits, _ = self(input_ids)
+        # the last position has no target; taken along, it costs a row where slicing the logits would copy their gradient
+        targets = torch.cat([input_ids[:, 1:], torch.full_like(input_ids[:, :1], -100)], dim=1)
+        return tuple(t if t is None else t[:, :-1] for t in token_logprobs(logits, targets, temperature=temperature, top=top))
 
     def step(self, input_ids: torch.Tensor, past_states: Optional[List[Any]] = None):
         """One token with the reference's state passing (model.py:251-270)."""
