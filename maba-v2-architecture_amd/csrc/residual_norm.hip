@@ -128,8 +128,9 @@ struct BoundaryBackArgs {
 };
 
 // WHOLE: rows of whole 16-byte chunks (WholeWalk).  The next rows' chunks are loaded ahead of the present ones' arithmetic.
+// One chunk a lane: four waves a SIMD, two workgroups of 512 threads a compute unit (97 us at 8,192 x 4,096; one takes 109).
 template <class T, int NCH, bool POST, bool WHOLE>
-__global__ __launch_bounds__(1 << MAX_LG) void boundary_back_kernel(BoundaryBackArgs a) {
+__global__ __launch_bounds__(1 << MAX_LG, NCH == 1 ? 4 : 2) void boundary_back_kernel(BoundaryBackArgs a) {
   constexpr int V = Traits<T>::VEC, NG = POST ? 3 : 2;
   __shared__ float red[2 * 3 * (1 << MAX_LG) / 64];
   extern __shared__ float sums[];                  // [NG][threads * V]; before that, the parameters' chunks
@@ -439,10 +440,11 @@ constexpr int MOST_ELEMS = 24, MOST_BACK = 16;
 static int forward_elems(int64_t R, int64_t C, int dtype) { return C > 8 << MAX_LG ? 16 : dtype != MABA_F32 && R > 4096 ? MOST_ELEMS : 8; }
 static int back_elems(int64_t C) { return C > 8 << MAX_LG ? MOST_BACK : 8; }
 static int row_threads(int lg) { return std::max(256, 1 << lg); }
-// The workgroups of a backward pass: as many as are resident at once (three of 256 threads a compute unit, two of 512, one
-// with 16 elements a lane) write the fewest partials.
-static int back_groups(int64_t R, int64_t C, int lg) {
-  const int threads = row_threads(lg), each = threads == 256 ? 3 : back_elems(C) == 8 ? 2 : 1;
+// The workgroups of a backward pass: as many as are resident at once write the fewest partials.  Three of 256 threads a compute
+// unit or two of 512, one less of each with two chunks a lane (fp32, 8,192 x 2,048: 92, 96 and 108 us with one, two and
+// three), one of 512 beyond.
+static int back_groups(int64_t R, int64_t C, int dtype, int lg) {
+  const int threads = row_threads(lg), each = std::max(1, (threads == 256 ? 3 : 2) - (dtype == MABA_F32) - (back_elems(C) == MOST_BACK));
   return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(R, threads >> lg), (int64_t)device_cu_count() * each));
 }
 template <int N>
@@ -538,7 +540,7 @@ extern "C" size_t maba_hip_residual_norm_backward_workspace_size(const maba_tens
   if (x_out->shape[1] > MAX_WIDTH) return 0;
   const int64_t R = x_out->shape[0], C = x_out->shape[1];
   // (rows far apart have the most lanes, and so the most workgroups)
-  return (size_t)back_groups(R, C, row_geometry(C, chunk_elems(x_out->dtype), back_elems(C), true).lg) * __builtin_popcount(grads & 7) *
+  return (size_t)back_groups(R, C, x_out->dtype, row_geometry(C, chunk_elems(x_out->dtype), back_elems(C), true).lg) * __builtin_popcount(grads & 7) *
          C * sizeof(float);
 }
 
@@ -581,7 +583,7 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
   const Geometry geo = row_geometry(C, chunk_elems(dt), back_elems(C), far_rows({dx_out, dh, x_out, y, dx, dy}));
   const int grads = (dweight ? GRAD_W : 0) | (dgate ? GRAD_GATE : 0) | (dpost_weight ? GRAD_POST : 0);
   if (!grads && !dx && !dy) return MABA_OK;
-  const int groups = back_groups(R, C, geo.lg), n = __builtin_popcount(grads);
+  const int groups = back_groups(R, C, dt, geo.lg), n = __builtin_popcount(grads);
   rc = ffn::check_workspace(who, workspace, workspace_bytes, (size_t)groups * n * C * sizeof(float));
   if (rc) return rc;
   const bool need_y = post_weight || dgate;

@@ -12,6 +12,8 @@ using ffn::u32x4_any;
 using ffn::Bf16;
 using ffn::Fp16;
 typedef u32x4 u32x4_any4 __attribute__((aligned(4)));
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 
 struct F32 { static constexpr int CODE = MABA_F32; };
 template <class T> struct Traits { typedef uint16_t elem; static constexpr int VEC = 8; };
@@ -39,7 +41,10 @@ __device__ __forceinline__ u32x4 pack(const float (&v)[Traits<T>::VEC]) {
     for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(v[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = T::down(v[2 * i]) | (T::down(v[2 * i + 1]) << 16);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (T::CODE == MABA_BF16) u[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[2 * i], v[2 * i + 1]}, bf16x2));
+      else u[i] = T::down(v[2 * i]) | (T::down(v[2 * i + 1]) << 16);
+    }
   }
   return u;
 }
@@ -196,7 +201,7 @@ __device__ __forceinline__ void row_sums(float (&v)[N], int lg, float* red, int&
 // Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011): a block cipher of the counter
 // (column / 4, row, stream) under the seed, whose four output words serve four neighbouring columns.  So any part of the
 // mask can be made anywhere, in any order, and it is never stored.  Seven rounds, the fewest that pass the statistical
-// tests in that paper: ten cost half as much again of what bounds a pass over 16-bit elements next to its traffic.
+// tests in that paper: with ten dropout of 32,768 x 1,024 bf16 takes 31.8 us instead of 28.5 (without the generator 22.0).
 struct Drop {
   const uint64_t* seed;
   uint32_t below, stream;
@@ -210,13 +215,14 @@ inline Drop make_drop(double p, const void* seed, uint32_t stream) {
   return {(const uint64_t*)seed, (uint32_t)(t < 4294967295.0 ? t : 4294967295.0), stream, (float)(1.0 / (1.0 - p)), 1};
 }
 
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
 __device__ __forceinline__ u32x4 philox(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1) {
 #pragma unroll
   for (int i = 0; i < 7; ++i) {
     const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c0 = xor3((uint32_t)(b >> 32), c1, k0);
     c1 = (uint32_t)b;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c2 = xor3((uint32_t)(a >> 32), c3, k1);
     c3 = (uint32_t)a;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
@@ -234,6 +240,7 @@ __device__ __forceinline__ void drop_chunk(float (&v)[V], const Drop& d, uint64_
       w = philox((uint32_t)(at / 4 + q), (uint32_t)row, (uint32_t)(row >> 32), d.stream, (uint32_t)key, (uint32_t)(key >> 32));
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[4 * q + e] = d.mode == 1 && w[e] >= d.below ? v[4 * q + e] * d.keep : 0.f;
+    __builtin_amdgcn_sched_barrier(0);             // one block of the generator after another: fewer registers
   }
 }
 
