@@ -26,7 +26,8 @@ struct BoundaryArgs {
   Drop d;
 };
 
-template <class T, int NCH>
+// CUT: rows end inside a chunk (CutRows).
+template <class T, int NCH, bool CUT>
 __global__ __launch_bounds__(1 << MAX_LG) void boundary_kernel(BoundaryArgs a) {
   constexpr int V = Traits<T>::VEC;
   __shared__ float red[2 * (1 << MAX_LG) / 64];
@@ -38,6 +39,7 @@ __global__ __launch_bounds__(1 << MAX_LG) void boundary_kernel(BoundaryArgs a) {
   const Walk<T> vw(a.w, 0, l, 0), vp(a.wp, 0, l, 0), vg(a.g, 0, l, 0);
   const uint64_t key = a.d.mode == 1 ? *a.d.seed : 0;
   const float inv_c = 1.f / (float)a.C;
+  const CutRows<T, CUT ? NCH : 1> rows(a.R, a.C, l, lg);
   u32x4 w[NCH] = {}, wp[NCH] = {}, g[NCH] = {};
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
@@ -52,11 +54,25 @@ __global__ __launch_bounds__(1 << MAX_LG) void boundary_kernel(BoundaryArgs a) {
     const int64_t ru = r0 + first, r = ru + sub;
     const int C = r < a.R ? a.C : 0;               // a row past the last one has no elements
     u32x4 x[NCH], y[NCH];
+    if constexpr (CUT) {
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      const int at = (l + (i << lg)) * V;
-      x[i] = load_chunk<T>(wx.at(ru, i << lg), wx.off, C - at);
-      if (a.y) y[i] = load_chunk<T>(wy.at(ru, i << lg), wy.off, C - at);
+      for (int i = 0; i < NCH; ++i) {
+        x[i] = rows.load(wx, ru, r < a.R, i);
+        if (a.y) y[i] = rows.load(wy, ru, r < a.R, i);
+      }
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        const int left = C - (l + (i << lg)) * V;
+        x[i] = ended<T>(x[i], left);
+        if (a.y) y[i] = ended<T>(y[i], left);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        const int at = (l + (i << lg)) * V;
+        x[i] = load_chunk<T>(wx.at(ru, i << lg), wx.off, C - at);
+        if (a.y) y[i] = load_chunk<T>(wy.at(ru, i << lg), wy.off, C - at);
+      }
     }
     float rp = 1.f;
     if (a.wp) {
@@ -123,6 +139,7 @@ struct BoundaryBackArgs {
   float* partial;
   int64_t dxos, dhs, xos, ys, dxs, dys, R;
   int C, lg, grads;
+  bool cut;
   float scale, eps;
   Drop d;
 };
@@ -160,6 +177,7 @@ __global__ __launch_bounds__(1 << MAX_LG, NCH == 1 ? 4 : 2) void boundary_back_k
     where[i] = c < chunks ? (uint32_t)(16 * (i << lg)) : NOWHERE;
     pc[i] = min(c, chunks - 1);
   }
+  const CutRows<T, WHOLE ? 1 : NCH> cut(a.R, a.C, l, lg);
   struct Raw { u32x4 d[NCH], h[NCH], x[NCH], y[NCH]; };
   const auto fetch = [&](int64_t r0, Raw& u) {
     const int64_t ru = r0 + first;
@@ -176,16 +194,19 @@ __global__ __launch_bounds__(1 << MAX_LG, NCH == 1 ? 4 : 2) void boundary_back_k
         u.y[i] = wy.load(ry, at);
       }
     } else {
+      const auto one = [&](const Rows& w, int i) {
+        if (a.cut) return cut.load(w, ru, live, i);
+        return load_chunk<T>(w.at(ru, i << lg), w.off, live ? a.C - (l + (i << lg)) * V : 0);
+      };
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
-        const int left = live ? a.C - (l + (i << lg)) * V : 0;
         u.h[i] = u.x[i] = u.d[i] = u.y[i] = u32x4{0, 0, 0, 0};
         if (a.dh) {
-          u.h[i] = load_chunk<T>(wh.at(ru, i << lg), wh.off, left);
-          u.x[i] = load_chunk<T>(wx.at(ru, i << lg), wx.off, left);
+          u.h[i] = one(wh, i);
+          u.x[i] = one(wx, i);
         }
-        if (a.dxo) u.d[i] = load_chunk<T>(wd.at(ru, i << lg), wd.off, left);
-        if (a.y) u.y[i] = load_chunk<T>(wy.at(ru, i << lg), wy.off, left);
+        if (a.dxo) u.d[i] = one(wd, i);
+        if (a.y) u.y[i] = one(wy, i);
       }
     }
   };
@@ -196,8 +217,19 @@ __global__ __launch_bounds__(1 << MAX_LG, NCH == 1 ? 4 : 2) void boundary_back_k
   if (r0 < a.R) fetch(r0, next);
   for (; r0 < a.R; r0 += step) {
     const int64_t ru = r0 + first, r = ru + sub;
-    const Raw u = next;
+    Raw u = next;
     fetch(r0 + step, next);
+    if constexpr (!WHOLE) {
+      if (a.cut)
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+          const int left = r < a.R ? a.C - (l + (i << lg)) * V : 0;
+          u.h[i] = ended<T>(u.h[i], left);
+          u.x[i] = ended<T>(u.x[i], left);
+          u.d[i] = ended<T>(u.d[i], left);
+          u.y[i] = ended<T>(u.y[i], left);
+        }
+    }
     const auto put = [&](const Rows& w, int i, const float (&v)[V]) {
       if constexpr (WHOLE) w.store(w.rows(ru), where[i] | (r < a.R ? 0u : NOWHERE), pack<T>(v));
       else store_chunk<T>(w.at(ru, i << lg), w.off, r < a.R ? a.C - (l + (i << lg)) * V : 0, pack<T>(v));
@@ -412,6 +444,8 @@ static int check_drop(const char* who, double p, const int64_t* seed) {
   return MABA_OK;
 }
 static int chunk_elems(int dtype) { return dtype == MABA_F32 ? 4 : 8; }
+// Whether rows end inside a chunk that is not their first.
+static bool cut_rows(int64_t C, int dtype) { return C > chunk_elems(dtype) && C % chunk_elems(dtype); }
 static bool same_place(const maba_tensor* a, const maba_tensor* b) {
   return a->data == b->data && (a->shape[0] <= 1 || a->stride[0] == b->stride[0]);
 }
@@ -529,7 +563,9 @@ extern "C" int maba_hip_residual_norm(const maba_tensor* x, const maba_tensor* y
   with_type(dt, [&](auto type) {
     typedef decltype(type) T;
     with_chunks<T, T::CODE == MABA_F32 ? MOST_BACK : MOST_ELEMS>(geo.nch, [&](auto n) {
-      hipLaunchKernelGGL((boundary_kernel<T, decltype(n)::value>), grid, dim3(threads), 0, (hipStream_t)stream, a);
+      constexpr int N = decltype(n)::value;
+      hipLaunchKernelGGL((cut_rows(C, dt) ? boundary_kernel<T, N, true> : boundary_kernel<T, N, false>), grid, dim3(threads), 0,
+                         (hipStream_t)stream, a);
     });
   });
   return check_launch(who);
@@ -591,7 +627,7 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
                         weight ? weight->data : nullptr, post_weight ? post_weight->data : nullptr, gate ? gate->data : nullptr,
                         dx ? dx->data : nullptr, dy ? dy->data : nullptr, (float*)workspace,
                         dx_out ? dx_out->stride[0] : 0, dh ? dh->stride[0] : 0, x_out->stride[0], y ? y->stride[0] : 0,
-                        dx ? dx->stride[0] : 0, dy ? dy->stride[0] : 0, R, (int)C, geo.lg, grads, scale, eps,
+                        dx ? dx->stride[0] : 0, dy ? dy->stride[0] : 0, R, (int)C, geo.lg, grads, cut_rows(C, dt), scale, eps,
                         make_drop(p, seed, stream_id)};
   if (R > 0) {
     const int threads = row_threads(geo.lg);
