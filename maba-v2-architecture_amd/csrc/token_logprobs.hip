@@ -174,7 +174,7 @@ __device__ __forceinline__ float across(float v, float* shared, F f) {
 // W waves a row (row_waves says how many).  With one, a workgroup has four rows; otherwise it is one row's.
 template <class T, int W, bool TOP>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void logprobs_kernel(ForwardArgs a) {
-  constexpr int E = Traits<T>::VEC, NB = 32 / E, LANES = 64 * W, GROUPS = W == 1 ? 4 : 1, CAP = W == 1 ? 256 : 1024;
+  constexpr int E = Traits<T>::VEC, NB = 32 / E, LANES = 64 * W, GROUPS = W == 1 ? 4 : 1, CAP = W > 4 ? 1024 : 256 * W;
   __shared__ Triple s_t[W];
   __shared__ float s_nth[W];
   __shared__ key64 s_above[TOP ? GROUPS * CAP : 1], s_equal[TOP ? GROUPS * CAP : 1];
