@@ -314,7 +314,7 @@ __global__ __launch_bounds__(1 << MAX_LG, NCH == 1 ? 4 : 2) void boundary_back_k
     }
     if constexpr (POST) {
       if (a.dy) {
-        row_sums<1>(t, lg, red, turn);
+        row_sums<1, 3>(t, lg, red, turn);
         const float m = t[0] * inv_c * rp;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {

@@ -192,9 +192,9 @@ __device__ __forceinline__ float wave_joined(float v, F f) {
   return f(p.a, p.b);
 }
 // The sums of v over the 2^lg lanes of a row (lg >= 4), the same bits in each of them.  Rows of more than one wave meet in
-// `red` [2][N][waves]; every thread of the workgroup takes part, and the two halves take turns, so that one barrier a
-// sum is enough.
-template <int N>
+// `red` [2][M][waves], M being the kernel's largest N; every thread of the workgroup takes part, and the two halves take
+// turns, so that one barrier a sum is enough.
+template <int N, int M = N>
 __device__ __forceinline__ void row_sums(float (&v)[N], int lg, float* red, int& turn) {
 #pragma unroll
   for (int n = 0; n < N; ++n) {
@@ -217,7 +217,7 @@ __device__ __forceinline__ void row_sums(float (&v)[N], int lg, float* red, int&
     }
   if (lg > 6) {
     const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, per = 1 << (lg - 6);
-    float* r = red + turn * N * waves;
+    float* r = red + turn * M * waves;
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
       for (int n = 0; n < N; ++n) r[n * waves + wave] = v[n];

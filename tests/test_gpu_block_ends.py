@@ -288,6 +288,19 @@ def test_offsets_past_32_bits():
     assert all(torch.equal(a[0], b) for a, b in zip(got, flat))
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("Cw", [1000, 4096, 4095])
+def test_post_norm_backward_has_the_same_bits_on_every_call(dt, Cw):
+    """Rows of several waves sum three values over the row, then one: sums of different rows or calls share nothing."""
+    M, f = 3000, _gen(60)
+    d, dh, xo, y = (f(M, Cw).to(dt) for _ in range(4))
+    w, wp, g = (1 + 0.1 * f(Cw).to(dt) for _ in range(3))
+    call = lambda: D.residual_norm_backward(d, dh, xo, y, w, wp, g, 0.5, 0.1, _seed(), 1)
+    want = call()
+    for _ in range(20):
+        assert all(torch.equal(a, b) for a, b in zip(call(), want))
+
+
 # ----------------------------------------------------------------------------- log probabilities
 
 
