@@ -513,6 +513,8 @@ extern "C" int maba_hip_token_logprobs_backward(const maba_tensor* dlogp, const 
                     (float)(1.0 / temperature)};
   while (a.lg < 8 && chunks > (int64_t)4 << a.lg) ++a.lg;
   a.parts = (int)std::min<int64_t>(ceil_div(chunks, 256 * 8), 0x7fffffff / R);
+  // in place a row is one wave's: it may be summed again, and then nothing of it may have been written yet
+  if (logits->data == dlogits->data) a.lg = 6, a.parts = 1;
   const dim3 grid((unsigned)(ceil_div(R, 256 >> a.lg) * a.parts));
   auto kernel = logits->dtype == MABA_F32 ? logprobs_back_kernel<F32> : logits->dtype == MABA_BF16 ? logprobs_back_kernel<Bf16>
                                                                                                   : logprobs_back_kernel<Fp16>;

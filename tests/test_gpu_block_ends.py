@@ -457,6 +457,19 @@ def test_logits_gradient_in_place():
     _around_is_nan(v, 1, 2)
 
 
+@pytest.mark.parametrize("M,V", [(3, 40000), (300, 9001)])
+def test_logits_gradient_in_place_of_rows_far_from_zero(M, V):
+    """Such rows are summed again by the backward: all of it before any of the row is written."""
+    x, t = _logits(M, V, BF, seed=8)
+    x += 600
+    g = torch.ones(M, device=DEV)
+    _, ent, lse, _, _ = D.token_logprobs(x, t)
+    want = D.token_logprobs_backward(g, g, None, x, t, lse, ent)
+    N.check(N.load().maba_hip_token_logprobs_backward(N.rows_desc(g), N.rows_desc(g), None, N.desc(x), N.rows_desc(t), N.rows_desc(lse),
+                                                      N.rows_desc(ent), 1.0, N.desc(x), N.stream_ptr(x.device)), "token_logprobs_backward")
+    assert torch.equal(x, want)
+
+
 @pytest.mark.parametrize("use", [(0,), (1,), (2,), (0, 1), (0, 1, 2)])
 def test_logprob_autograd_of_some_outputs(use):
     x, t = _logits(40, 300, FL, seed=8)
