@@ -332,14 +332,15 @@ __global__ __launch_bounds__(256) void logprobs_back_kernel(BackwardArgs a) {
   char* out = (char*)a.dx.row(r);
   const int64_t target = a.targets[r];
   float lse = a.lse[r];
-  const float h = a.entropy[r], gh = a.dentropy ? a.dentropy[r] : 0.f;
+  const float h = a.entropy[r];
+  float gh = a.dentropy ? a.dentropy[r] : 0.f;
   float gl = target < 0 || !a.dlogp ? 0.f : target >= a.V ? NAN : a.dlogp[r], gz = a.dlse ? a.dlse[r] : 0.f;
   // log p = l / T - lse is as exact as lse, which far from zero is not enough: there the row is summed again, by each wave
   // for itself, and log p counted from its largest element.
   float m = 0.f;
   if (lse == -INFINITY) {            // no mass: no element has a gradient
     lse = -LOWEST;
-    gl = 0.f;
+    gl = gh = gz = 0.f;              // whatever comes from a loss of lse = -inf
   } else if (fabsf(lse) > 256.f) {
     m = -INFINITY;
     const int l = threadIdx.x & 63;

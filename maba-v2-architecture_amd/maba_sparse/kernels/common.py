@@ -678,6 +678,7 @@ def ref_token_logprobs_backward(dlogp, dentropy, dlse, logits, targets, lse, ent
     none, t = (lse == -math.inf).unsqueeze(-1), targets.unsqueeze(-1)
     gl, gh, gz = (zero if g is None else g.to(x.dtype).unsqueeze(-1) for g in (dlogp, dentropy, dlse))
     gl = torch.where((t < 0) | none, zero, torch.where(t >= x.shape[-1], zero / zero, gl))
+    gh, gz = (torch.where(none, zero, g) for g in (gh, gz))   # NaN, say, from a loss of lse = -inf
     # counted from the row's largest, which lse is not exact enough for far from zero
     z = (x - torch.where(none, zero, x.amax(-1, keepdim=True))) * inv
     lp = torch.where(none, torch.full((), -math.inf, dtype=x.dtype, device=x.device), z - torch.log(torch.exp(z).sum(-1, keepdim=True)))

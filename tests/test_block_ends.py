@@ -192,6 +192,20 @@ def test_logprobs_and_their_backward_op(V, dtype):
     B.check(D.token_logprobs_backward(*g, x, t, lse, H, 0.8), B.logprobs_backward(*g, x, t, 0.8), "dlogits")
 
 
+def test_rows_without_mass_have_no_gradient_whatever_comes_in():
+    """A loss of lse^2 under torch.where sends NaN into such a row."""
+    x, t = _logits(12, 300, torch.float32, seed=9)
+    x[::3] = -math.inf
+    x.requires_grad_()
+    logp, ent, lse, _, _ = D.token_logprobs(x, t)
+    z = torch.where(lse > -math.inf, lse ** 2, torch.zeros_like(lse))
+    (z.sum() + ent.sum() - torch.where(lse > -math.inf, logp, torch.zeros_like(logp)).sum()).backward()
+    assert (x.grad[::3] == 0).all() and x.grad.isfinite().all() and (x.grad[1] != 0).any()
+    nan = torch.full_like(lse, math.nan)
+    d = D.token_logprobs_backward(nan, nan, nan, x.detach(), t, lse.detach(), ent.detach())
+    assert (d[::3] == 0).all() and d[1].isnan().all()
+
+
 def test_rows_of_nan_and_targets_past_the_vocabulary():
     x, t = _logits(4, 10, torch.float32)
     x[1, 4], x[2, 4] = math.nan, math.inf

@@ -470,6 +470,20 @@ def test_logits_gradient_in_place_of_rows_far_from_zero(M, V):
     assert torch.equal(x, want)
 
 
+def test_rows_without_mass_have_no_gradient_whatever_comes_in():
+    """A loss of lse^2 under torch.where sends NaN into such a row."""
+    x, t = _logits(12, 300, FL, seed=9)
+    x[::3] = -math.inf
+    x.requires_grad_()
+    logp, ent, lse, _, _ = D.token_logprobs(x, t)
+    z = torch.where(lse > -math.inf, lse ** 2, torch.zeros_like(lse))
+    (z.sum() + ent.sum() - torch.where(lse > -math.inf, logp, torch.zeros_like(logp)).sum()).backward()
+    assert (x.grad[::3] == 0).all() and x.grad.isfinite().all() and (x.grad[1] != 0).any()
+    nan = torch.full_like(lse, math.nan)
+    d = D.token_logprobs_backward(nan, nan, nan, x.detach(), t, lse.detach(), ent.detach())
+    assert (d[::3] == 0).all() and d[1].isnan().all()
+
+
 @pytest.mark.parametrize("use", [(0,), (1,), (2,), (0, 1), (0, 1, 2)])
 def test_logprob_autograd_of_some_outputs(use):
     x, t = _logits(40, 300, FL, seed=8)
