@@ -427,7 +427,11 @@ def hip_checkpoint_unpack(codes, scales, dtype: torch.dtype = torch.bfloat16, **
 
 
 def _seed_ptr(p: float, seed: Optional[torch.Tensor]) -> Optional[int]:
-    return seed.data_ptr() if 0 < p < 1 else None
+    if not 0 < p < 1:
+        return None
+    if seed is None or seed.dtype != torch.int64 or seed.numel() != 1:
+        raise ValueError("dropout needs a seed: an int64 tensor of one element")
+    return seed.data_ptr()
 
 
 @register_kernel("hip", "dropout")

@@ -484,6 +484,29 @@ def test_rows_without_mass_have_no_gradient_whatever_comes_in():
     assert (d[::3] == 0).all() and d[1].isnan().all()
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("M,V,k", [(3, 4000, 7), (5000, 2500, 20), (1100, 12000, 64), (2100, 17000, 3), (4, 40000, 20)])
+def test_rows_in_order(M, V, k, dt):
+    """All of a row's largest elements are those of a few threads."""
+    x = torch.arange(V, device=DEV).expand(M, V) * (20 / V)
+    t = torch.full((M,), V // 2, device=DEV)
+    for rows in (x.to(dt), x.flip(1).to(dt)):
+        _check_logprobs(rows.contiguous(), t, 1.0, k)
+
+
+def test_more_rows_than_a_launch_takes():
+    M, V = (1 << 22) + 5, 3
+    x, t = _gen(10)(M, V), torch.arange(M, device=DEV) % V
+    x.requires_grad_()
+    out = D.token_logprobs(x, t, top=2)
+    lp = torch.log_softmax(x.detach().double(), -1)
+    assert (out[0].detach().double() - lp.gather(1, t[:, None])[:, 0]).abs().max() < 2e-6
+    assert torch.equal(out[4], torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[:, :2])
+    out[0].sum().backward()
+    d = torch.nn.functional.one_hot(t, V).double() - lp.exp()
+    assert (x.grad.double() - d).abs().max() < 2e-6
+
+
 @pytest.mark.parametrize("use", [(0,), (1,), (2,), (0, 1), (0, 1, 2)])
 def test_logprob_autograd_of_some_outputs(use):
     x, t = _logits(40, 300, FL, seed=8)
