@@ -172,6 +172,12 @@ __device__ __forceinline__ float across(float v, float* shared, F f) {
 }
 
 // W waves a row (row_waves says how many).  With one, a workgroup has four rows; otherwise it is one row's.
+// Without alternatives 8,192 x 32,768 bf16 take 98 us, 5.5 TB/s: HBM; 777 x 50,257 fp32, whose rows start at any 4 bytes, 34 us,
+// 4.6 TB/s.  With them the threads that hold one read their elements again, which the L2 serves, and the other waves of the row
+// wait: 4,096 x 32,768 bf16 54 us without, 65 with 5 and 71 with 20 (4.1 and 3.8 TB/s).  16 x 32,768 take 5.3 and with
+// 20 alternatives 9.4 us, the latency of one row.
+// CAP: room for what is above the bound.  Two lists of 1,024 a row of two waves held the compute unit to ten rows: 4,096 x
+// 16,000 with five alternatives 46 us, with 512 44.
 template <class T, int W, bool TOP>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void logprobs_kernel(ForwardArgs a) {
   constexpr int E = Traits<T>::VEC, NB = 32 / E, LANES = 64 * W, GROUPS = W == 1 ? 4 : 1, CAP = W > 4 ? 1024 : 256 * W;
@@ -342,6 +348,8 @@ struct BackwardArgs {
   float inv;
 };
 
+// One read and one write of the logits: 8,192 x 32,768 bf16 194 us, 777 x 50,257 fp32 57 us, both 5.5 TB/s: HBM.  Long rows go
+// to several workgroups, eight chunks a thread, so that few of them fill the chip too: 16 x 32,768 5.6 us.
 template <class T>
 __global__ __launch_bounds__(256) void logprobs_back_kernel(BackwardArgs a) {
   constexpr int E = Traits<T>::VEC, NB = 2;
@@ -429,8 +437,8 @@ static int check_row_vec(const maba_tensor* t, const char* who, const char* name
 // Waves a row, of 1, 2, 4 and 8.  Many rows: as few as leave a thread 16 chunks, since what a row costs besides its elements
 // (its waves' sums joined, the barriers) grows with them.  Few rows: as many as leave each thread a chunk, while all
 // rows' waves are at most eight a compute unit.  In us for bf16 with five alternatives, 1 / 2 / 4 / 8 waves:
-//   4,096 x 8,000   25 / 29 / 31 / 41      4,096 x 32,768   79 / 75 / 64 / 71      4,096 x 65,536   156 / 143 / 121 / 115
-//   16 x 2,000      8.3 / 5.8 / 5.1 / 34 (waves without a chunk bound nothing)     16 x 32,768      28 / 14 / 11 / 8.7
+//   4,096 x 8,000   25 / 28 / 32 / 43      4,096 x 32,768   78 / 75 / 65 / 74      4,096 x 65,536   155 / 147 / 123 / 118
+//   16 x 2,000      8.2 / 5.7 / 5.1 / 25 (waves without a chunk bound nothing)     16 x 32,768      27 / 14 / 11 / 8.8
 static int row_waves(int64_t rows, int64_t chunks) {
   int w = 1;
   while (w < 8 && chunks > 16 * 64 * w) w *= 2;
