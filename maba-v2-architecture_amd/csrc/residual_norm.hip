@@ -29,8 +29,8 @@ struct BoundaryArgs {
 };
 
 // A row stays in the registers of its lanes from the load to both stores: the sums of y^2 and of x'^2 cost two exchanges, no
-// second read.  16,384 x 640 bf16 with dropout 18.4 us, 4.6 TB/s, and 16.6 without (5.0); 32,768 x 640 30 us, 5.5 TB/s; 8,192 x 4,096 with both norms and dropout 45 us, 5.9 TB/s.  A single row of 640 takes
-// 3.1 us, most of it the launch.
+// second read.  16,384 x 640 bf16 with dropout 18.4 us, 4.6 TB/s, and 16.6 without (5.0); 32,768 x 640 30 us, 5.5 TB/s; 8,192 x
+// 4,096 with both norms and dropout 45 us, 5.9 TB/s.  A single row of 640 takes 3.1 us, most of it the launch.
 // CUT: rows end inside a chunk (CutRows): their accesses are 2- or 4-byte aligned, and the memory path splits most of them in
 // two (8,191 x 4,095 bf16 65 us, 4.1 TB/s).
 template <class T, int NCH, bool CUT>
