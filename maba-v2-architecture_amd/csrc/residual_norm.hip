@@ -481,16 +481,23 @@ static bool whole_rows(std::initializer_list<const maba_tensor*> all) {
 // (80 chunks of 640 16-bit elements fill 62 % of 128 lanes and 83 % of 32 with three each) and share out what a row costs
 // besides its elements.  Forward, in us, 8 / 24 elements: 1 x 640 bf16 3.1 / 4.1, 2,048 x 640 5.5 / 5.8, 32,768 x 640
 // 42.8 / 32.8, 8,192 x 4,096 50.5 / 47.3; fp32 8,192 x 1,000 22.9 / 24.6.  Backward, 8 / 16: 64 x 640 8.6 / 10.4, 16,384 x 640
-// 39.6 / 39.4, 2,048 x 4,096 37 / 43, 8,192 x 4,096 98 / 103.
+// 39.1 / 38.1, 65,536 x 640 118 / 109, with post_weight 24,576 x 640 57 / 49, x 767 87 / 71 (without 72 / 71), x 1,536 107 / 100 and
+// x 2,600 172 / 187; where all lanes of 8 have work 24,576 x 512 36 / 38, 2,048 x 4,096 37 / 43, 8,192 x 4,096 98 / 103.
 constexpr int MOST_ELEMS = 24, MOST_BACK = 16;
 static int forward_elems(int64_t R, int64_t C, int dtype) { return C > 8 << MAX_LG ? 16 : dtype != MABA_F32 && R > 4096 ? MOST_ELEMS : 8; }
-static int back_elems(int64_t C) { return C > 8 << MAX_LG ? MOST_BACK : 8; }
+static int back_elems(int64_t R, int64_t C, int dtype) {
+  if (C > 8 << MAX_LG) return MOST_BACK;
+  const int64_t chunks = ceil_div(C, 8);
+  int64_t lanes = 64;
+  while (lanes < chunks) lanes *= 2;
+  return dtype != MABA_F32 && R >= 16384 && lanes > 64 && lanes <= 256 && chunks * 4 <= lanes * 3 ? MOST_BACK : 8;
+}
 static int row_threads(int lg) { return std::max(256, 1 << lg); }
 // The workgroups of a backward pass: as many as are resident at once write the fewest partials.  Three of 256 threads a compute
 // unit or two of 512, one less of each with two chunks a lane (fp32, 8,192 x 2,048: 92, 96 and 108 us with one, two and
 // three), one of 512 beyond.
 static int back_groups(int64_t R, int64_t C, int dtype, int lg) {
-  const int threads = row_threads(lg), each = std::max(1, (threads == 256 ? 3 : 2) - (dtype == MABA_F32) - (back_elems(C) == MOST_BACK));
+  const int threads = row_threads(lg), each = std::max(1, (threads == 256 ? 3 : 2) - (dtype == MABA_F32) - (back_elems(R, C, dtype) == MOST_BACK));
   return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(R, threads >> lg), (int64_t)device_cu_count() * each));
 }
 template <int N>
@@ -588,7 +595,7 @@ extern "C" size_t maba_hip_residual_norm_backward_workspace_size(const maba_tens
   if (x_out->shape[1] > MAX_WIDTH) return 0;
   const int64_t R = x_out->shape[0], C = x_out->shape[1];
   // (rows far apart have the most lanes, and so the most workgroups)
-  return (size_t)back_groups(R, C, x_out->dtype, row_geometry(C, chunk_elems(x_out->dtype), back_elems(C), true).lg) * __builtin_popcount(grads & 7) *
+  return (size_t)back_groups(R, C, x_out->dtype, row_geometry(C, chunk_elems(x_out->dtype), back_elems(R, C, x_out->dtype), true).lg) * __builtin_popcount(grads & 7) *
          C * sizeof(float);
 }
 
@@ -628,7 +635,7 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
       if (overlap(outs[i], outs[j])) return fail(MABA_ERR_INVALID, "%s: outputs overlap", who);
   }
   if (C > MAX_WIDTH) return fail(MABA_ERR_UNSUPPORTED, "%s: at most %d channels", who, MAX_WIDTH);
-  const Geometry geo = row_geometry(C, chunk_elems(dt), back_elems(C), far_rows({dx_out, dh, x_out, y, dx, dy}));
+  const Geometry geo = row_geometry(C, chunk_elems(dt), back_elems(R, C, dt), far_rows({dx_out, dh, x_out, y, dx, dy}));
   const int grads = (dweight ? GRAD_W : 0) | (dgate ? GRAD_GATE : 0) | (dpost_weight ? GRAD_POST : 0);
   if (!grads && !dx && !dy) return MABA_OK;
   const int groups = back_groups(R, C, dt, geo.lg), n = __builtin_popcount(grads);
