@@ -76,15 +76,23 @@ __device__ __forceinline__ Triple wave_join(Triple t) {
 __device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ float sum_of(float a, float b) { return a + b; }
 
-// The running state of a thread over its elements, and the largest of them.
+// The running state of a thread over its elements, and the largest of them; with TOP also where the round of elements is that
+// has it, and the largest of the other rounds.
+template <bool TOP>
 struct Running {
   Triple t = {FLOOR, 0.f, 0.f};
-  float best = -INFINITY;
+  float best = -INFINITY, other = -INFINITY;
+  int where = 0;
   template <int N>
-  __device__ __forceinline__ void take(const float (&v)[N], float c) {
-    float b = best;
+  __device__ __forceinline__ void take(const float (&v)[N], int first, float c) {
+    float b = TOP ? -INFINITY : best;
 #pragma unroll
     for (int e = 0; e < N; ++e) b = fmaxf(b, v[e]);
+    if constexpr (TOP) {
+      other = fmaxf(other, fminf(best, b));
+      where = b > best ? first : where;
+      b = fmaxf(best, b);
+    }
     best = b;
     const float r = fmaxf(t.r, ceilf(b * c));
     raise(t.s, t.d, t.r - r);
@@ -173,11 +181,11 @@ __device__ __forceinline__ float across(float v, float* shared, F f) {
 
 // W waves a row (row_waves says how many).  With one, a workgroup has four rows; otherwise it is one row's.
 // Without alternatives 8,192 x 32,768 bf16 take 98 us, 5.5 TB/s: HBM; 777 x 50,257 fp32, whose rows start at any 4 bytes, 34 us,
-// 4.6 TB/s.  With them the threads that hold one read their elements again, which the L2 serves, and the other waves of the row
-// wait: 4,096 x 32,768 bf16 54 us without, 65 with 5 and 71 with 20 (4.1 and 3.8 TB/s).  16 x 32,768 take 5.3 and with
-// 20 alternatives 9.4 us, the latency of one row.
+// 4.7 TB/s.  With them the threads that hold one read elements again, and the other waves of the row wait: 4,096 x 32,768 bf16 51 us
+// without, 60 with 5 and 65 with 20 (4.5 and 4.2 TB/s; 65 and 71 where a thread read all of its elements again, a line of 128
+// bytes for 16).  16 x 32,768 take 5.3 and with 20 alternatives 9.4 us, the latency of one row; 17 where all but five logits are -inf.
 // CAP: room for what is above the bound.  Two lists of 1,024 a row of two waves held the compute unit to ten rows: 4,096 x
-// 16,000 with five alternatives 46 us, with 512 44.
+// 16,000 with five alternatives 46 us, with 512 43.
 template <class T, int W, bool TOP>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void logprobs_kernel(ForwardArgs a) {
   constexpr int E = Traits<T>::VEC, NB = 32 / E, LANES = 64 * W, GROUPS = W == 1 ? 4 : 1, CAP = W > 4 ? 1024 : 256 * W;
@@ -194,8 +202,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void logprobs_kernel(Forward
   const int64_t target = a.targets[r];
   float lt = 0.f;
   if (target >= 0 && target < a.V) lt = element<T>(row, (uint32_t)target);
-  Running run;
-  for_chunks<T, NB>(row, a.V, lane, LANES, [&](auto& v, int) { run.take(v, c); });
+  Running<TOP> run;
+  for_chunks<T, NB>(row, a.V, lane, LANES, [&](auto& v, int first) { run.take(v, first, c); });
   Triple t = wave_join(run.t);
   float bound = 0.f;
   if constexpr (TOP) {
@@ -258,24 +266,39 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void logprobs_kernel(Forward
   if constexpr (TOP) {
     key64 *above = s_above + group * CAP, *equal = s_equal + group * CAP;
     int* count = s_count[group];
-    // a thread whose sum is NaN may have NaN among its elements, which its largest does not tell
-    if (run.best >= bound || run.t.s != run.t.s)
-      for_chunks<T, NB>(row, a.V, lane, LANES, [&](auto& v, int first) {
-        constexpr int N = sizeof(v) / sizeof(v[0]);
+    // which of a chunk's elements are at or above the bound, or above it
+    const auto at_least = [&](int at, bool strictly) {
+      float v[E];
+      unpack<T>(load_chunk<T>(row, (uint32_t)at * (16 / E), a.V - at), v);
+      uint32_t hits = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) hits |= v[e] < bound || (strictly && v[e] == bound) ? 0u : 1u << e;
+      return hits;
+    };
+    // Most often one round of a thread's elements is enough.  (A thread whose sum is NaN may have NaN among its elements, which
+    // its largest does not tell.)
+    if (const bool all = run.other >= bound || run.t.s != run.t.s; all || run.best >= bound)
+      for (int first = all ? lane * E : run.where, end = all ? a.V : first + 1; first < end; first += LANES * NB * E) {
         uint32_t hits = 0;
 #pragma unroll
-        for (int e = 0; e < N; ++e) hits |= v[e] < bound ? 0u : 1u << e;
+        for (int b = 0; b < NB; ++b) hits |= at_least(first + b * LANES * E, false) << (b * E);
         while (hits) {
           const int e = __builtin_ctz(hits), idx = first + (e / E) * LANES * E + e % E;
           hits &= hits - 1;
           if (idx >= a.V) continue;
           const float x = element<T>(row, (uint32_t)idx);
           const bool eq = x == bound;
-          if (eq && *(volatile int*)&count[1] >= CAP) continue;        // more than will be read are not counted on
+          if (eq && *(volatile int*)&count[1] >= CAP) {        // more than will be read are not counted on
+            uint32_t over = 0;
+#pragma unroll 1
+            for (int b = 0; b < NB; ++b) over |= at_least(first + b * LANES * E, true) << (b * E);
+            hits &= over;
+            continue;
+          }
           const int at = atomicAdd(&count[eq], 1);
           if (at < CAP) (eq ? equal : above)[at] = order_key(x, (uint32_t)idx);
         }
-      });
+      }
     if constexpr (W > 1) __syncthreads();
     else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const int n = *(volatile int*)&count[0], ties = *(volatile int*)&count[1];
@@ -437,8 +460,8 @@ static int check_row_vec(const maba_tensor* t, const char* who, const char* name
 // Waves a row, of 1, 2, 4 and 8.  Many rows: as few as leave a thread 16 chunks, since what a row costs besides its elements
 // (its waves' sums joined, the barriers) grows with them.  Few rows: as many as leave each thread a chunk, while all
 // rows' waves are at most eight a compute unit.  In us for bf16 with five alternatives, 1 / 2 / 4 / 8 waves:
-//   4,096 x 8,000   25 / 28 / 32 / 43      4,096 x 32,768   78 / 75 / 65 / 74      4,096 x 65,536   155 / 147 / 123 / 118
-//   16 x 2,000      8.2 / 5.7 / 5.1 / 25 (waves without a chunk bound nothing)     16 x 32,768      27 / 14 / 11 / 8.8
+//   4,096 x 8,000   23 / 24 / 29 / 46    4,096 x 32,768   75 / 64 / 60 / 67    4,096 x 65,536   145 / 119 / 112 / 106
+//   16 x 2,000      7.4 / 5.7 / 5.9 / 27 (waves without a chunk bound nothing)     16 x 32,768      20 / 12 / 9.7 / 8.3
 static int row_waves(int64_t rows, int64_t chunks) {
   int w = 1;
   while (w < 8 && chunks > 16 * 64 * w) w *= 2;
