@@ -152,14 +152,16 @@ struct BoundaryBackArgs {
 
 // The row's sums are three at once, of dh w x', x'^2 and y^2 (the mean of dh w x^ is r times that of dh w x'), and with POST a
 // fourth; the chunks stay packed in registers between their two uses.  16,384 x 640 bf16 with dropout 35 us, 3.6 TB/s, where
-// a fifth of the threads has no chunk and partials are written and read; 8,192 x 4,096 with both norms and dropout 90 us, 4.5
-// TB/s; 8,191 x 4,095 130 us, 3.1 TB/s.
+// every second lane has one chunk of two; 8,192 x 4,096 with both norms and dropout 87 us, 4.6 TB/s; 8,191 x 4,095 125 us, 3.2 TB/s.
 // WHOLE: rows of whole 16-byte chunks (WholeWalk).  The next rows' chunks are loaded ahead of the present ones' arithmetic.
-// One chunk a lane: four waves a SIMD, two workgroups of 512 threads a compute unit (97 us at 8,192 x 4,096; one takes 109).
+// One workgroup a compute unit, as large as registers allow: of four waves a SIMD with one chunk a lane, of two beyond.  So
+// the fewest partials are written: 8,192 x 4,096 bf16 with post_weight 92 us and without 86, as two workgroups of half the threads
+// 97 and 92; 2,048 x 640 15.6 and, as three of 256 threads, 17.4; fp32 8,192 x 2,048 82 and 88.
+constexpr int back_threads(int nch) { return nch == 1 ? 1024 : 512; }
 template <class T, int NCH, bool POST, bool WHOLE>
-__global__ __launch_bounds__(1 << MAX_LG, NCH == 1 ? 4 : 2) void boundary_back_kernel(BoundaryBackArgs a) {
+__global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(BoundaryBackArgs a) {
   constexpr int V = Traits<T>::VEC, NG = POST ? 3 : 2;
-  __shared__ float red[2 * 3 * (1 << MAX_LG) / 64];
+  __shared__ float red[2 * 3 * back_threads(NCH) / 64];
   extern __shared__ float sums[];                  // [NG][threads * V]; before that, the parameters' chunks
   const int threads = blockDim.x;
   int turn = 0;
@@ -481,8 +483,9 @@ static bool whole_rows(std::initializer_list<const maba_tensor*> all) {
 // (80 chunks of 640 16-bit elements fill 62 % of 128 lanes and 83 % of 32 with three each) and share out what a row costs
 // besides its elements.  Forward, in us, 8 / 24 elements: 1 x 640 bf16 3.1 / 4.1, 2,048 x 640 5.5 / 5.8, 32,768 x 640
 // 42.8 / 32.8, 8,192 x 4,096 50.5 / 47.3; fp32 8,192 x 1,000 22.9 / 24.6.  Backward, 8 / 16: 64 x 640 8.6 / 10.4, 16,384 x 640
-// 39.1 / 38.1, 65,536 x 640 118 / 109, with post_weight 24,576 x 640 57 / 49, x 767 87 / 71 (without 72 / 71), x 1,536 107 / 100 and
-// x 2,600 172 / 187; where all lanes of 8 have work 24,576 x 512 36 / 38, 2,048 x 4,096 37 / 43, 8,192 x 4,096 98 / 103.
+// 36.7 / 35.5, 65,536 x 640 118 / 109, with post_weight 24,576 x 640 57 / 49, x 767 87 / 71 (without 72 / 71); rows of more than
+// a wave either way 24,576 x 1,345 165 / 173 and without post_weight 16,384 x 1,536 66 / 76; where all lanes of 8 have work
+// 24,576 x 512 36 / 38, 2,048 x 4,096 37 / 43, 8,192 x 4,096 98 / 103.
 constexpr int MOST_ELEMS = 24, MOST_BACK = 16;
 static int forward_elems(int64_t R, int64_t C, int dtype) { return C > 8 << MAX_LG ? 16 : dtype != MABA_F32 && R > 4096 ? MOST_ELEMS : 8; }
 static int back_elems(int64_t R, int64_t C, int dtype) {
@@ -490,15 +493,17 @@ static int back_elems(int64_t R, int64_t C, int dtype) {
   const int64_t chunks = ceil_div(C, 8);
   int64_t lanes = 64;
   while (lanes < chunks) lanes *= 2;
-  return dtype != MABA_F32 && R >= 16384 && lanes > 64 && lanes <= 256 && chunks * 4 <= lanes * 3 ? MOST_BACK : 8;
+  return dtype != MABA_F32 && R >= 16384 && lanes == 128 && chunks * 4 <= lanes * 3 ? MOST_BACK : 8;
 }
-static int row_threads(int lg) { return std::max(256, 1 << lg); }
-// The workgroups of a backward pass: as many as are resident at once write the fewest partials.  Three of 256 threads a compute
-// unit or two of 512, one less of each with two chunks a lane (fp32, 8,192 x 2,048: 92, 96 and 108 us with one, two and
-// three), one of 512 beyond.
-static int back_groups(int64_t R, int64_t C, int dtype, int lg) {
-  const int threads = row_threads(lg), each = std::max(1, (threads == 256 ? 3 : 2) - (dtype == MABA_F32) - (back_elems(R, C, dtype) == MOST_BACK));
-  return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(R, threads >> lg), (int64_t)device_cu_count() * each));
+// A backward pass's threads a workgroup: the fewest until rows fill the chip (64 x 640 bf16 8.4 us, with 1,024 threads 10.6), then
+// as many as fill a compute unit by themselves.
+static int back_size(int64_t R, const Geometry& geo) {
+  const int most = back_threads(geo.nch);
+  return R >= (int64_t)device_cu_count() * (most >> geo.lg) ? most : std::max(256, 1 << geo.lg);
+}
+static int back_groups(int64_t R, const Geometry& geo) {
+  const int threads = back_size(R, geo);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(R, threads >> geo.lg), (int64_t)device_cu_count() * (back_threads(geo.nch) / threads)));
 }
 template <int N>
 struct Num { static constexpr int value = N; };
@@ -577,7 +582,7 @@ extern "C" int maba_hip_residual_norm(const maba_tensor* x, const maba_tensor* y
                     x->stride[0], y ? y->stride[0] : 0, x_out ? x_out->stride[0] : 0, h ? h->stride[0] : 0, R, (int)C, geo.lg,
                     scale, eps, make_drop(p, seed, stream_id)};
   if (R == 0) return MABA_OK;
-  const int threads = row_threads(geo.lg);
+  const int threads = std::max(256, 1 << geo.lg);
   const dim3 grid((unsigned)std::min<int64_t>(ceil_div(R, threads >> geo.lg), (int64_t)device_cu_count() * 8));
   with_type(dt, [&](auto type) {
     typedef decltype(type) T;
@@ -594,9 +599,10 @@ extern "C" size_t maba_hip_residual_norm_backward_workspace_size(const maba_tens
   if (!x_out || x_out->ndim != 2 || x_out->shape[1] < 1 || !is_float_dt(x_out->dtype) || !(grads & 7)) return 0;
   if (x_out->shape[1] > MAX_WIDTH) return 0;
   const int64_t R = x_out->shape[0], C = x_out->shape[1];
-  // (rows far apart have the most lanes, and so the most workgroups)
-  return (size_t)back_groups(R, C, x_out->dtype, row_geometry(C, chunk_elems(x_out->dtype), back_elems(R, C, x_out->dtype), true).lg) * __builtin_popcount(grads & 7) *
-         C * sizeof(float);
+  int groups = 0;
+  for (const bool far : {false, true})               // which of them the call takes depends on all its tensors' strides
+    groups = std::max(groups, back_groups(R, row_geometry(C, chunk_elems(x_out->dtype), back_elems(R, C, x_out->dtype), far)));
+  return (size_t)groups * __builtin_popcount(grads & 7) * C * sizeof(float);
 }
 
 extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const maba_tensor* dh, const maba_tensor* x_out,
@@ -638,7 +644,7 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
   const Geometry geo = row_geometry(C, chunk_elems(dt), back_elems(R, C, dt), far_rows({dx_out, dh, x_out, y, dx, dy}));
   const int grads = (dweight ? GRAD_W : 0) | (dgate ? GRAD_GATE : 0) | (dpost_weight ? GRAD_POST : 0);
   if (!grads && !dx && !dy) return MABA_OK;
-  const int groups = back_groups(R, C, dt, geo.lg), n = __builtin_popcount(grads);
+  const int groups = back_groups(R, geo), n = __builtin_popcount(grads);
   rc = ffn::check_workspace(who, workspace, workspace_bytes, (size_t)groups * n * C * sizeof(float));
   if (rc) return rc;
   const bool need_y = post_weight || dgate;
@@ -649,7 +655,7 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
                         dx ? dx->stride[0] : 0, dy ? dy->stride[0] : 0, R, (int)C, geo.lg, grads, cut_rows(C, dt), scale, eps,
                         make_drop(p, seed, stream_id)};
   if (R > 0) {
-    const int threads = row_threads(geo.lg);
+    const int threads = back_size(R, geo);
     const size_t params = (size_t)(post_weight ? 3 : 2) * ceil_div(C, chunk_elems(dt)) * 16;
     const size_t lds = std::max(params, grads ? (size_t)(post_weight ? 3 : 2) * threads * chunk_elems(dt) * sizeof(float) : 0);
     const bool whole = whole_rows({dx_out, dh, x_out, y, dx, dy});

@@ -107,7 +107,7 @@ PARTS = [("weight",), ("y",), ("y", "weight", "gate"), ("y", "post_weight"), ("y
 # One size for each number of lanes a row and of chunks a lane, and a few for their edges.
 SIZES = [(1, 1), (3, 7), (5, 16), (70, 33), (1, 640), (130, 640), (33, 129), (64, 250), (40, 1024), (21, 1030), (9, 2048), (17, 3333),
          (6, 4096), (5, 4100), (3, 8191), (4, 8192)]
-MANY = [(5000, 24), (4500, 640), (9001, 136), (4200, 1001), (16400, 640), (16389, 651)]
+MANY = [(5000, 24), (4500, 640), (9001, 136), (4200, 1001), (16400, 640), (16389, 651), (8200, 33), (3000, 2049)]
 
 
 def _tensors(M, Cw, dt, parts, seed=0):
