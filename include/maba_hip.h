@@ -482,8 +482,9 @@ int maba_hip_dropout(const maba_tensor* x, double p, const int64_t* seed, uint32
  * alignment; y (then h is x's norm), weight with h, post_weight, gate and x_out may be NULL, and x_out may be x.
  * fp32 arithmetic; x_out is rounded once, and h once from the unrounded x_out.  Dropout as in maba_hip_dropout.
  *
- * Backward: dx_out, dh [M,C], either of which may be NULL (zeros); x_out as the forward returned it, read only with dh;
- * y is read only with post_weight or for dgate; any of dx, dy [M,C], dweight, dpost_weight, dgate [C] may be NULL.
+ * Backward: dx_out, dh [M,C], either of which may be NULL (zeros); x, y as the forward had them, from which it makes the
+ * unrounded x_out again: x is read only with dh, y (NULL where the forward had none) with dh, with post_weight and for
+ * dgate, and may be NULL otherwise; any of dx, dy [M,C], dweight, dpost_weight, dgate [C] may be NULL.
  * Parameters' gradients are summed in fp32 through the workspace (16-byte aligned, of one call at a time; the query
  * depends on the current device's compute-unit count; grads: 1 dweight, 2 dgate, 4 dpost_weight), in a fixed order:
  * results are the same bits on every call.
@@ -492,8 +493,8 @@ int maba_hip_residual_norm(const maba_tensor* x, const maba_tensor* y, const mab
                            const maba_tensor* post_weight, const maba_tensor* gate, float scale, double p,
                            const int64_t* seed, uint32_t stream_id, float eps, maba_tensor* x_out, maba_tensor* h,
                            void* stream);
-size_t maba_hip_residual_norm_backward_workspace_size(const maba_tensor* x_out, int grads);
-int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const maba_tensor* dh, const maba_tensor* x_out,
+size_t maba_hip_residual_norm_backward_workspace_size(const maba_tensor* x, int grads);
+int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const maba_tensor* dh, const maba_tensor* x,
                                     const maba_tensor* y, const maba_tensor* weight, const maba_tensor* post_weight,
                                     const maba_tensor* gate, float scale, double p, const int64_t* seed,
                                     uint32_t stream_id, float eps, maba_tensor* dx, maba_tensor* dy,

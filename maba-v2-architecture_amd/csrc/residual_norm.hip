@@ -4,14 +4,16 @@
 //   h  = RMSNorm(x') * w                         the norm before the next sub-layer
 // (reference model.py:11-22, 92-128 has the gated residual and the norm before, composed of torch modules.)
 //
-// Backward, for the gradients d' of x' and dh of h, with x^ = x' r, y^ = y rp the normalised rows:
+// Backward, for the gradients d' of x' and dh of h, with x^ = x' r, y^ = y rp the normalised rows and x' as the forward had it
+// before it was rounded, made again from x and y:
 //   dX = d' + r (dh w - x^ mean(dh w x^))        the gradient of x, and of x' behind its norm
 //   dz = scale gate dropout(dX)                  the same mask, made again
 //   dy = rp (dz w_post - y^ mean(dz w_post y^))
 //   dw = sum dh x^,  dgate = sum scale dX dropout(z),  dw_post = sum dz y^     over the rows
-// r and rp are made again from the rows that are read anyway; nothing but x' and y is kept from the forward pass.
+// Nothing but x and y is kept from the forward pass.  (From the rounded x' instead, h would be another function's by a rounding of
+// its argument: a gradient of weight over a few rows 1.4 times as far off as its own rounding leaves it.)
 //
-// Bound: HBM.  Forward reads x and y and writes x' and h; backward reads d', dh, x', y and writes dx and dy, once each.
+// Bound: HBM.  Forward reads x and y and writes x' and h; backward reads d', dh, x, y and writes dx and dy, once each.
 // Times below are of single kernels on cold tensors; a copy of 1 GiB reaches 5.1 TB/s, and tensors that the 256 MB cache in
 // front of HBM holds in part go faster.
 #include "row_vec.h"
@@ -140,18 +142,18 @@ __global__ __launch_bounds__(1 << MAX_LG) void boundary_kernel(BoundaryArgs a) {
 // columns_kernel the workgroups' partials [groups][n][C] in their order.
 enum { GRAD_W = 1, GRAD_GATE = 2, GRAD_POST = 4 };
 struct BoundaryBackArgs {
-  const void *dxo, *dh, *xo, *y, *w, *wp, *g;
+  const void *dxo, *dh, *x, *y, *w, *wp, *g;
   void *dx, *dy;
   float* partial;
-  int64_t dxos, dhs, xos, ys, dxs, dys, R;
+  int64_t dxos, dhs, xs, ys, dxs, dys, R;
   int C, lg, grads;
   bool cut;
   float scale, eps;
   Drop d;
 };
 
-// The row's sums are three at once, of dh w x', x'^2 and y^2 (the mean of dh w x^ is r times that of dh w x'), and with POST a
-// fourth; the chunks stay packed in registers between their two uses.  16,384 x 640 bf16 with dropout 35 us, 3.6 TB/s, where
+// A row's sums are exchanged twice: those of dh w x' and x'^2 (the mean of dh w x^ is r times that of dh w x'), and with POST that
+// for dy together with the next row's of y^2.  The chunks stay packed in registers between their uses, the mask as bits.  16,384 x 640 bf16 with dropout 35 us, 3.6 TB/s, where
 // every second lane has one chunk of two; 8,192 x 4,096 with both norms and dropout 87 us, 4.6 TB/s; 8,191 x 4,095 125 us, 3.2 TB/s.
 // WHOLE: rows of whole 16-byte chunks (WholeWalk).  The next rows' chunks are loaded ahead of the present ones' arithmetic.
 // One workgroup a compute unit, as large as registers allow: of four waves a SIMD with one chunk a lane, of two beyond.  So
@@ -161,14 +163,14 @@ constexpr int back_threads(int nch) { return nch == 1 ? 1024 : 512; }
 template <class T, int NCH, bool POST, bool WHOLE>
 __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(BoundaryBackArgs a) {
   constexpr int V = Traits<T>::VEC, NG = POST ? 3 : 2;
-  __shared__ float red[2 * 3 * back_threads(NCH) / 64];
+  __shared__ float red[2 * 2 * back_threads(NCH) / 64];
   extern __shared__ float sums[];                  // [NG][threads * V]; before that, the parameters' chunks
   const int threads = blockDim.x;
   int turn = 0;
   const int lg = a.lg, l = threadIdx.x & ((1 << lg) - 1), slots = threads >> lg;
   const int first = __builtin_amdgcn_readfirstlane(threadIdx.x >> lg), sub = lg < 6 ? (threadIdx.x & 63) >> lg : 0;
   typedef std::conditional_t<WHOLE, WholeWalk<T>, Walk<T>> Rows;
-  const Rows wd(a.dxo, a.dxos, l, sub), wh(a.dh, a.dhs, l, sub), wx(a.xo, a.xos, l, sub), wy(a.y, a.ys, l, sub);
+  const Rows wd(a.dxo, a.dxos, l, sub), wh(a.dh, a.dhs, l, sub), wx(a.x, a.xs, l, sub), wy(a.y, a.ys, l, sub);
   const Rows wdx(a.dx, a.dxs, l, sub), wdy(a.dy, a.dys, l, sub);
   const uint64_t key = a.d.mode == 1 ? *a.d.seed : 0;
   const float inv_c = 1.f / (float)a.C;
@@ -225,8 +227,29 @@ __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(Bounda
   float acc[NG][NCH][V] = {};
   const int64_t step = (int64_t)gridDim.x * slots;
   int64_t r0 = (int64_t)blockIdx.x * slots;
+  // the row's own part of sum y^2, of chunks as they are then used
+  const auto squares = [&](int64_t row, Raw& u) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      if constexpr (!WHOLE)
+        if (a.cut) u.y[i] = ended<T>(u.y[i], row < a.R ? a.C - (l + (i << lg)) * V : 0);
+      float y[V];
+      unpack<T>(u.y[i], y);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s = fmaf(y[e], y[e], s);
+    }
+    return s;
+  };
   Raw next;
-  if (r0 < a.R) fetch(r0, next);
+  float yy[1] = {0.f};
+  if (r0 < a.R) {
+    fetch(r0, next);
+    if constexpr (POST) {
+      yy[0] = squares(r0 + first + sub, next);
+      row_sums<1, 2>(yy, lg, red, turn);
+    }
+  }
   for (; r0 < a.R; r0 += step) {
     const int64_t ru = r0 + first, r = ru + sub;
     Raw u = next;
@@ -239,52 +262,64 @@ __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(Bounda
           u.h[i] = ended<T>(u.h[i], left);
           u.x[i] = ended<T>(u.x[i], left);
           u.d[i] = ended<T>(u.d[i], left);
-          u.y[i] = ended<T>(u.y[i], left);
+          if constexpr (!POST) u.y[i] = ended<T>(u.y[i], left);
         }
     }
     const auto put = [&](const Rows& w, int i, const float (&v)[V]) {
       if constexpr (WHOLE) w.store(w.rows(ru), where[i] | (r < a.R ? 0u : NOWHERE), pack<T>(v));
       else store_chunk<T>(w.at(ru, i << lg), w.off, r < a.R ? a.C - (l + (i << lg)) * V : 0, pack<T>(v));
     };
-    float s[3] = {0.f, 0.f, 0.f};            // of dh w x', x'^2, y^2
+    // (a row past the last one has no part in the sums over rows, whatever eps is)
+    const float rp = !POST ? 1.f : r < a.R ? rsqrtf(yy[0] * inv_c + a.eps) : 0.f;
+    uint32_t bits[NCH];
+    float xn[NCH][V], s[2] = {0.f, 0.f};     // x', and the sums of dh w x' and x'^2
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
+      bits[i] = kept_bits<V>(a.d, key, r, (l + (i << lg)) * V);
       if (a.dh) {
-        float h[V], x[V], p[V];
+        float h[V], p[V];
+        unpack<T>(u.x[i], xn[i]);
+        if (a.y) {                           // as the forward does
+          float z[V];
+          unpack<T>(u.y[i], z);
+          if constexpr (POST) {
+            unpack<T>(par[2 * chunks + pc[i]], p);
+#pragma unroll
+            for (int e = 0; e < V; ++e) z[e] *= rp * p[e];
+          }
+          drop_by<V>(z, a.d, bits[i]);
+          if (a.g) {
+            unpack<T>(par[chunks + pc[i]], p);
+#pragma unroll
+            for (int e = 0; e < V; ++e) z[e] *= p[e];
+          }
+#pragma unroll
+          for (int e = 0; e < V; ++e) xn[i][e] = fmaf(a.scale, z[e], xn[i][e]);
+        }
         unpack<T>(u.h[i], h);
-        unpack<T>(u.x[i], x);
         unpack<T>(par[pc[i]], p);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          s[0] = fmaf(h[e] * p[e], x[e], s[0]);
-          s[1] = fmaf(x[e], x[e], s[1]);
+          s[0] = fmaf(h[e] * p[e], xn[i][e], s[0]);
+          s[1] = fmaf(xn[i][e], xn[i][e], s[1]);
         }
       }
-      if constexpr (POST) {
-        float y[V];
-        unpack<T>(u.y[i], y);
-#pragma unroll
-        for (int e = 0; e < V; ++e) s[2] = fmaf(y[e], y[e], s[2]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_sched_barrier(0);           // chunk after chunk: side by side their masks cost 50 registers more
     }
-    if (a.dh || POST) row_sums<3>(s, lg, red, turn);
-    // (a row past the last one has no part in the sums over rows, whatever eps is)
+    if (a.dh) row_sums<2>(s, lg, red, turn);
     const float rx = r < a.R ? rsqrtf(s[1] * inv_c + a.eps) : 0.f, mean = s[0] * rx * inv_c;
-    const float rp = !POST ? 1.f : r < a.R ? rsqrtf(s[2] * inv_c + a.eps) : 0.f;
-    float dz[POST ? NCH : 1][V], t[1] = {0.f};
+    float dz[POST ? NCH : 1][V], t[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       float d[V];
       unpack<T>(u.d[i], d);
       if (a.dh) {
-        float h[V], x[V], p[V];
+        float h[V], p[V];
         unpack<T>(u.h[i], h);
-        unpack<T>(u.x[i], x);
         unpack<T>(par[pc[i]], p);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float xh = x[e] * rx;
+          const float xh = xn[i][e] * rx;
           d[e] = fmaf(rx, fmaf(h[e], p[e], -xh * mean), d[e]);
           acc[0][i][e] = fmaf(h[e], xh, acc[0][i][e]);
         }
@@ -292,7 +327,7 @@ __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(Bounda
       if (a.dx) put(wdx, i, d);
       if (a.dy || (a.grads & (GRAD_GATE | GRAD_POST))) {
         // dropout(z) = m z with m in {0, 1 / (1 - p)}: both products with m follow from m dX
-        drop_chunk<V>(d, a.d, key, r, (l + (i << lg)) * V);
+        drop_by<V>(d, a.d, bits[i]);
         float p[V], y[V];
         unpack<T>(u.y[i], y);
         if constexpr (POST) {
@@ -322,11 +357,12 @@ __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(Bounda
           put(wdy, i, d);
         }
       }
-      __builtin_amdgcn_sched_barrier(0);           // chunk after chunk: side by side their masks cost 50 registers more
+      __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (POST) {
+      t[1] = squares(r + step, next);
+      row_sums<2>(t, lg, red, turn);
       if (a.dy) {
-        row_sums<1, 3>(t, lg, red, turn);
         const float m = t[0] * inv_c * rp;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
@@ -337,6 +373,7 @@ __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(Bounda
           put(wdy, i, dz[i]);
         }
       }
+      yy[0] = t[1];
     }
   }
   if (!a.grads) return;
@@ -595,32 +632,33 @@ extern "C" int maba_hip_residual_norm(const maba_tensor* x, const maba_tensor* y
   return check_launch(who);
 }
 
-extern "C" size_t maba_hip_residual_norm_backward_workspace_size(const maba_tensor* x_out, int grads) {
-  if (!x_out || x_out->ndim != 2 || x_out->shape[1] < 1 || !is_float_dt(x_out->dtype) || !(grads & 7)) return 0;
-  if (x_out->shape[1] > MAX_WIDTH) return 0;
-  const int64_t R = x_out->shape[0], C = x_out->shape[1];
+extern "C" size_t maba_hip_residual_norm_backward_workspace_size(const maba_tensor* x, int grads) {
+  if (!x || x->ndim != 2 || x->shape[1] < 1 || !is_float_dt(x->dtype) || !(grads & 7)) return 0;
+  if (x->shape[1] > MAX_WIDTH) return 0;
+  const int64_t R = x->shape[0], C = x->shape[1];
   int groups = 0;
   for (const bool far : {false, true})               // which of them the call takes depends on all its tensors' strides
-    groups = std::max(groups, back_groups(R, row_geometry(C, chunk_elems(x_out->dtype), back_elems(R, C, x_out->dtype), far)));
+    groups = std::max(groups, back_groups(R, row_geometry(C, chunk_elems(x->dtype), back_elems(R, C, x->dtype), far)));
   return (size_t)groups * __builtin_popcount(grads & 7) * C * sizeof(float);
 }
 
-extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const maba_tensor* dh, const maba_tensor* x_out,
+extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const maba_tensor* dh, const maba_tensor* x,
                                                const maba_tensor* y, const maba_tensor* weight, const maba_tensor* post_weight,
                                                const maba_tensor* gate, float scale, double p, const int64_t* seed,
                                                uint32_t stream_id, float eps, maba_tensor* dx, maba_tensor* dy,
                                                maba_tensor* dweight, maba_tensor* dpost_weight, maba_tensor* dgate,
                                                void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "residual_norm_backward";
-  int rc = check_float_rows(x_out, who);
+  int rc = check_float_rows(x, who);
   if (!rc) rc = check_drop(who, p, seed);
-  if (!rc) rc = check_rows(x_out, who, "x_out", x_out->dtype, -1, -1);
+  if (!rc) rc = check_rows(x, who, "x", x->dtype, -1, -1);
   if (rc) return rc;
-  const int64_t R = x_out->shape[0], C = x_out->shape[1];
-  const int dt = x_out->dtype;
+  const int64_t R = x->shape[0], C = x->shape[1];
+  const int dt = x->dtype;
   if (!dx_out && !dh) return fail(MABA_ERR_INVALID, "%s: dx_out or dh is required", who);
   if (dh && !weight) return fail(MABA_ERR_INVALID, "%s: dh goes with weight", who);
   if (!y && (post_weight || dpost_weight || dgate)) return fail(MABA_ERR_INVALID, "%s: post_weight and its and gate's gradients go with y", who);
+  if (dh && dy && !y) return fail(MABA_ERR_INVALID, "%s: with dh, dy goes with y", who);
   if ((dpost_weight && !post_weight) || (dgate && !gate) || (dweight && !weight))
     return fail(MABA_ERR_INVALID, "%s: a gradient of a missing parameter", who);
   for (const auto& t : {std::make_pair(dx_out, "dx_out"), std::make_pair(dh, "dh"), std::make_pair(y, "y")})
@@ -635,30 +673,30 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
   if (rc) return rc;
   maba_tensor* outs[] = {dx, dy, dweight, dpost_weight, dgate};
   for (int i = 0; i < 5; ++i) {
-    for (const maba_tensor* in : {dx_out, dh, x_out, y, weight, post_weight, gate})
+    for (const maba_tensor* in : {dx_out, dh, x, y, weight, post_weight, gate})
       if (overlap(outs[i], in)) return fail(MABA_ERR_INVALID, "%s: an output overlaps an input", who);
     for (int j = 0; j < i; ++j)
       if (overlap(outs[i], outs[j])) return fail(MABA_ERR_INVALID, "%s: outputs overlap", who);
   }
   if (C > MAX_WIDTH) return fail(MABA_ERR_UNSUPPORTED, "%s: at most %d channels", who, MAX_WIDTH);
-  const Geometry geo = row_geometry(C, chunk_elems(dt), back_elems(R, C, dt), far_rows({dx_out, dh, x_out, y, dx, dy}));
+  const Geometry geo = row_geometry(C, chunk_elems(dt), back_elems(R, C, dt), far_rows({dx_out, dh, x, y, dx, dy}));
   const int grads = (dweight ? GRAD_W : 0) | (dgate ? GRAD_GATE : 0) | (dpost_weight ? GRAD_POST : 0);
   if (!grads && !dx && !dy) return MABA_OK;
   const int groups = back_groups(R, geo), n = __builtin_popcount(grads);
   rc = ffn::check_workspace(who, workspace, workspace_bytes, (size_t)groups * n * C * sizeof(float));
   if (rc) return rc;
-  const bool need_y = post_weight || dgate;
-  BoundaryBackArgs a = {dx_out ? dx_out->data : nullptr, dh ? dh->data : nullptr, x_out->data, need_y ? y->data : nullptr,
+  const bool need_y = y && (dh || post_weight || dgate);
+  BoundaryBackArgs a = {dx_out ? dx_out->data : nullptr, dh ? dh->data : nullptr, x->data, need_y ? y->data : nullptr,
                         weight ? weight->data : nullptr, post_weight ? post_weight->data : nullptr, gate ? gate->data : nullptr,
                         dx ? dx->data : nullptr, dy ? dy->data : nullptr, (float*)workspace,
-                        dx_out ? dx_out->stride[0] : 0, dh ? dh->stride[0] : 0, x_out->stride[0], y ? y->stride[0] : 0,
+                        dx_out ? dx_out->stride[0] : 0, dh ? dh->stride[0] : 0, x->stride[0], y ? y->stride[0] : 0,
                         dx ? dx->stride[0] : 0, dy ? dy->stride[0] : 0, R, (int)C, geo.lg, grads, cut_rows(C, dt), scale, eps,
                         make_drop(p, seed, stream_id)};
   if (R > 0) {
     const int threads = back_size(R, geo);
     const size_t params = (size_t)(post_weight ? 3 : 2) * ceil_div(C, chunk_elems(dt)) * 16;
     const size_t lds = std::max(params, grads ? (size_t)(post_weight ? 3 : 2) * threads * chunk_elems(dt) * sizeof(float) : 0);
-    const bool whole = whole_rows({dx_out, dh, x_out, y, dx, dy});
+    const bool whole = whole_rows({dx_out, dh, x, y, dx, dy});
     with_type(dt, [&](auto type) {
       typedef decltype(type) T;
       auto run = [&](auto kernel) {

@@ -267,6 +267,27 @@ __device__ __forceinline__ u32x4 philox(uint32_t c0, uint32_t c1, uint32_t c2, u
   }
   return u32x4{c0, c1, c2, c3};
 }
+// Bit e of the answer: whether element e of a chunk is kept.
+template <int V>
+__device__ __forceinline__ uint32_t kept_bits(const Drop& d, uint64_t key, int64_t row, int at) {
+  if (d.mode != 1) return d.mode == 0 ? 0xffu : 0u;
+  uint32_t bits = 0;
+#pragma unroll
+  for (int q = 0; q < V / 4; ++q) {
+    const u32x4 w = philox((uint32_t)(at / 4 + q), (uint32_t)row, (uint32_t)(row >> 32), d.stream, (uint32_t)key, (uint32_t)(key >> 32));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bits |= w[e] >= d.below ? 1u << (4 * q + e) : 0u;
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  return bits;
+}
+// drop_chunk() by such bits.
+template <int V>
+__device__ __forceinline__ void drop_by(float (&v)[V], const Drop& d, uint32_t bits) {
+  if (d.mode == 0) return;
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = bits >> e & 1 ? v[e] * d.keep : 0.f;
+}
 // v where it is kept, times 1 / (1 - p); zero, whatever v is, where it is dropped.  `at` is a multiple of four.
 template <int V>
 __device__ __forceinline__ void drop_chunk(float (&v)[V], const Drop& d, uint64_t key, int64_t row, int at) {

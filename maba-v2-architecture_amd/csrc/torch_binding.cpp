@@ -351,10 +351,10 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
     const Tensor y = y_.value_or(Tensor()), w = w_.value_or(Tensor()), wp = wp_.value_or(Tensor()), g = g_.value_or(Tensor());
     const Tensor seed = seed_.value_or(Tensor());
     auto out = boundary_call(x, y, w, wp, g, {scale, eps, {p, seed, (uint32_t)stream}});
-    // y is read for its own norm's gradient and for the gate's, x_out for its norm's
-    const bool keeps_y = y.defined() && (wp.defined() || needs(g));
+    // x_out is made again for its norm's gradient; y is read for its own norm's and for the gate's too
+    const bool keeps_y = y.defined() && (w.defined() || wp.defined() || needs(g));
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({w.defined() ? y.defined() ? out.first : x : Tensor(), keeps_y ? y : Tensor(), w, wp, g, seed});
+    ctx->save_for_backward({w.defined() ? x : Tensor(), keeps_y ? y : Tensor(), w, wp, g, seed});
     ctx->saved_data["need"] = (int64_t)(needs(x) | needs(y) << 1 | needs(w) << 2 | needs(wp) << 3 | needs(g) << 4 | y.defined() << 5);
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["p"] = p;
@@ -372,7 +372,7 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
     const Tensor dxo = need >> 5 & 1 ? grads[0] : Tensor(), dh = w.defined() ? grads.back() : Tensor();
     Tensor dx, dy, dw, dwp, dg;
     if (dxo.defined() || dh.defined()) {
-      const Tensor like = dxo.defined() ? dxo : dh, xo = kept[0].defined() ? kept[0] : like;
+      const Tensor like = dxo.defined() ? dxo : dh, x = kept[0].defined() ? kept[0] : like;
       const Drop d = {ctx->saved_data["p"].toDouble(), kept[5], (uint32_t)ctx->saved_data["stream"].toInt()};
       Scope scope(like);
       if (need & 1) dx = at::empty(like.sizes(), like.options());
@@ -380,12 +380,12 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
       if (need & 4) dw = at::empty(w.sizes(), like.options());
       if (need & 8) dwp = at::empty(wp.sizes(), like.options());
       if (need & 16) dg = at::empty(g.sizes(), like.options());
-      Desc ddxo(dxo), ddh(dh), dxo_(xo), iy(y), iw(w, true), ip(wp, true), ig(g, true);
+      Desc ddxo(dxo), ddh(dh), ix(x), iy(y), iw(w, true), ip(wp, true), ig(g, true);
       Desc odx(dx), ody(dy), odw(dw, true), odp(dwp, true), odg(dg, true);
       const int which = (need >> 2 & 1) | (need >> 4 & 1) << 1 | (need >> 3 & 1) << 2;
       Tensor ws;
-      if (which) ws = workspace(lib.residual_norm_backward_workspace_size(&dxo_, which), like);
-      check_backward(lib.residual_norm_backward(&ddxo, &ddh, &dxo_, &iy, &iw, &ip, &ig, (float)ctx->saved_data["scale"].toDouble(),
+      if (which) ws = workspace(lib.residual_norm_backward_workspace_size(&ix, which), like);
+      check_backward(lib.residual_norm_backward(&ddxo, &ddh, &ix, &iy, &iw, &ip, &ig, (float)ctx->saved_data["scale"].toDouble(),
                                                 d.p, d.ptr(), d.stream, (float)ctx->saved_data["eps"].toDouble(), &odx, &ody, &odw,
                                                 &odp, &odg, ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0,
                                                 stream_of(like)),

@@ -1,7 +1,7 @@
 """Gradients of the operators around a model's blocks: autograd functions over the dispatcher's forward and backward ops,
 the same on every backend.
 
-The boundary keeps its output and the sub-layer's output for the backward pass, dropout its seed alone: the mask is made
+The boundary keeps its inputs for the backward pass, dropout its seed alone: the mask is made
 again from it, so a seed must not change in between (autograd says so if it does).
 
 Calls that go to this package's own HIP kernels take the same functions natively (``csrc/torch_binding.cpp``); these here
@@ -45,9 +45,9 @@ class ResidualNorm(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         x_out, h = ops.run("residual_norm", x=x, y=y, weight=weight, post_weight=post_weight, gate=gate, seed=seed, **ctx.args)
         needs = ctx.needs_input_grad[5:10]
-        # y is read for its own norm's gradient and for the gate's, x_out for its norm's
-        kept_y = y if post_weight is not None or needs[4] else None
-        ctx.save_for_backward(x_out if weight is not None else None, kept_y, weight, post_weight, gate, seed)
+        # x_out is made again for its norm's gradient; y is read for its own norm's and for the gate's too
+        kept_y = y if weight is not None or post_weight is not None or needs[4] else None
+        ctx.save_for_backward(x if weight is not None else None, kept_y, weight, post_weight, gate, seed)
         ctx.alone = y is None
         if ctx.alone:
             return h
@@ -56,11 +56,11 @@ class ResidualNorm(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, *grads):
-        x_out, y, weight, post_weight, gate, seed = ctx.saved_tensors
+        x, y, weight, post_weight, gate, seed = ctx.saved_tensors
         dx_out, dh = (None, grads[0]) if ctx.alone else (*grads, None)[:2]
         if dx_out is None and dh is None:
             return (None,) * 11
-        out = ctx.ops.run("residual_norm_backward", dx_out=dx_out, dh=dh, x_out=x_out if x_out is not None else dx_out, y=y,
+        out = ctx.ops.run("residual_norm_backward", dx_out=dx_out, dh=dh, x=x if x is not None else dx_out, y=y,
                           weight=weight, post_weight=post_weight, gate=gate, seed=seed, needs=tuple(ctx.needs_input_grad[5:10]),
                           **ctx.args)
         return (None,) * 5 + tuple(out) + (None,)

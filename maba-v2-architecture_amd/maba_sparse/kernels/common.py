@@ -613,17 +613,21 @@ def ref_residual_norm(x, y=None, weight=None, post_weight=None, gate=None, scale
     return out, h.to(x.dtype).reshape(x.shape)
 
 
-def ref_residual_norm_backward(dx_out, dh, x_out, y=None, weight=None, post_weight=None, gate=None, scale: float = 1.0,
+def ref_residual_norm_backward(dx_out, dh, x, y=None, weight=None, post_weight=None, gate=None, scale: float = 1.0,
                                p: float = 0.0, seed=None, stream: int = 0, eps: float = 1e-6,
                                needs=(True, True, True, True, True), **kwargs: Any):
     """``(dx, dy, dweight, dpost_weight, dgate)`` of ``ref_residual_norm`` (None where ``needs`` says so, or where there is
-    no such input) for the gradients of ``x_out`` and ``h``, either of which may be None."""
-    dt, shape = x_out.dtype, x_out.shape
-    d = _rows32(dx_out) if dx_out is not None else torch.zeros_like(_rows32(x_out))
-    yf, one = _rows32(y), _one(None, d)
+    no such input) for the gradients of ``x_out`` and ``h``, either of which may be None.  x_out is made again, unrounded."""
+    dt, shape = x.dtype, x.shape
+    xf, yf = _rows32(x), _rows32(y)
+    d = _rows32(dx_out) if dx_out is not None else torch.zeros_like(xf)
+    one = _one(None, d)
+    rp = torch.rsqrt((yf * yf).mean(-1, keepdim=True) + eps) if post_weight is not None else one
     dw = dpw = dg = None
     if dh is not None:
-        g, xf = _rows32(dh), _rows32(x_out)
+        g = _rows32(dh)
+        if y is not None:
+            xf = xf + scale * (_one(gate, yf) * _dropped(yf * rp * _one(post_weight, yf), p, seed, stream))
         r = torch.rsqrt((xf * xf).mean(-1, keepdim=True) + eps)
         xh, gw = xf * r, g * weight.to(g.dtype)
         dw = (g * xh).sum(0)
@@ -631,7 +635,6 @@ def ref_residual_norm_backward(dx_out, dh, x_out, y=None, weight=None, post_weig
     elif weight is not None:
         dw = torch.zeros(shape[-1], dtype=d.dtype, device=d.device)
     m = _dropped(d, p, seed, stream)                          # the product of the mask and either side
-    rp = torch.rsqrt((yf * yf).mean(-1, keepdim=True) + eps) if post_weight is not None else one
     if gate is not None and needs[4]:
         dg = scale * (m * (yf * rp * _one(post_weight, d))).sum(0)
     dz = scale * (_one(gate, d) * m)
@@ -639,7 +642,7 @@ def ref_residual_norm_backward(dx_out, dh, x_out, y=None, weight=None, post_weig
         yh, wp = yf * rp, post_weight.to(d.dtype)
         dpw = (dz * yh).sum(0)
         dz = rp * (dz * wp - yh * (dz * wp * yh).mean(-1, keepdim=True))
-    grads = (d.reshape(shape), dz.reshape(shape), dw, dpw, dg)
+    grads = (d.reshape(shape), dz.reshape(shape) if dh is None or y is not None else None, dw, dpw, dg)
     return tuple(g.to(dt) if n and g is not None else None for g, n in zip(grads, needs))
 
 

@@ -735,8 +735,8 @@ def dispatch_residual_norm(x, y=None, weight=None, post_weight=None, gate=None, 
 
     x and y ``[..., C]``, weight, post_weight and gate ``[C]`` of one dtype and device; all but x are optional, and without
     y x_out is x itself.  ``p``, ``seed`` and ``stream`` as for ``dropout``.  Computed in fp32 and each result rounded once
-    (h from the unrounded x_out).  Differentiable on every backend, with x_out and (for post_weight or the gate's gradient)
-    y kept for it.  Under autocast the tensors are first cast to the widest of their types.  The HIP backend takes up to
+    (h from the unrounded x_out).  Differentiable on every backend: x and y are kept for it (x for h's gradient, y also for
+    post_weight's and the gate's).  Under autocast the tensors are first cast to the widest of their types.  The HIP backend takes up to
     8,192 channels."""
     dtype = _autocast_dtype(x)
     if dtype is not None:
@@ -766,21 +766,21 @@ def dispatch_residual_norm(x, y=None, weight=None, post_weight=None, gate=None, 
     return (x, out[1]) if y is None else out
 
 
-def dispatch_residual_norm_backward(dx_out, dh, x_out, y=None, weight=None, post_weight=None, gate=None, scale: float = 1.0,
+def dispatch_residual_norm_backward(dx_out, dh, x, y=None, weight=None, post_weight=None, gate=None, scale: float = 1.0,
                                     p: float = 0.0, seed=None, stream: int = 0, eps: float = 1e-6,
                                     needs=(True, True, True, True, True)):
     """``(dx, dy, dweight, dpost_weight, dgate)`` of ``residual_norm`` for the gradients of its results, either of which
-    may be None, each None where ``needs`` is false or there is no such input.  ``x_out`` is the forward's result (only its
-    shape and type count without ``dh``), ``y`` its input (not read without post_weight and without the gate's gradient).
-    No autograd takes part."""
+    may be None, each None where ``needs`` is false or there is no such input.  ``x`` (only its shape and type count without
+    ``dh``) and ``y`` are the forward's inputs; without ``dh``, post_weight and the gate's gradient y is not read and may be
+    left out.  No autograd takes part."""
     first = dx_out if dx_out is not None else dh
     if first is None:
         raise ValueError("dx_out or dh is required")
-    _boundary_check(x_out, y, weight, post_weight, gate)
-    _ffn_same(x_out, dx_out=dx_out, dh=dh)
-    _ffn_shape("dx_out", dx_out, x_out.shape)
-    _ffn_shape("dh", dh, x_out.shape)
-    _drop_args(x_out, p, seed, stream)
+    _boundary_check(x, y, weight, post_weight, gate)
+    _ffn_same(x, dx_out=dx_out, dh=dh)
+    _ffn_shape("dx_out", dx_out, x.shape)
+    _ffn_shape("dh", dh, x.shape)
+    _drop_args(x, p, seed, stream)
     if dh is not None and weight is None:
         raise ValueError("dh goes with weight")
     if len(needs) != 5:
@@ -788,7 +788,7 @@ def dispatch_residual_norm_backward(dx_out, dh, x_out, y=None, weight=None, post
     if y is None and (post_weight is not None or (gate is not None and needs[4])):
         raise ValueError("post_weight and the gate's gradient need y")
     with torch.no_grad():
-        return _FFNOps(x_out.device).run("residual_norm_backward", dx_out=dx_out, dh=dh, x_out=x_out, y=y, weight=weight,
+        return _FFNOps(x.device).run("residual_norm_backward", dx_out=dx_out, dh=dh, x=x, y=y, weight=weight,
                                          post_weight=post_weight, gate=gate, scale=scale, p=p, seed=seed, stream=stream, eps=eps,
                                          needs=tuple(needs))
 

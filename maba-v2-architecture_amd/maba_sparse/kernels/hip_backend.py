@@ -475,30 +475,30 @@ def hip_residual_norm(x, y=None, weight=None, post_weight=None, gate=None, scale
 
 
 @register_kernel("hip", "residual_norm_backward")
-def hip_residual_norm_backward(dx_out, dh, x_out, y=None, weight=None, post_weight=None, gate=None, scale: float = 1.0,
+def hip_residual_norm_backward(dx_out, dh, x, y=None, weight=None, post_weight=None, gate=None, scale: float = 1.0,
                                p: float = 0.0, seed=None, stream: int = 0, eps: float = 1e-6,
                                needs=(True, True, True, True, True), **kwargs: Any):
     """``(dx, dy, dweight, dpost_weight, dgate)`` (contract: ``dispatcher.dispatch_residual_norm_backward``)."""
-    _no_grad_needed("residual_norm_backward", dx_out, dh, x_out, y, weight, post_weight, gate)
-    dev = N.require_device((dx_out, dh, x_out, y, weight, post_weight, gate, seed), "residual_norm_backward")
+    _no_grad_needed("residual_norm_backward", dx_out, dh, x, y, weight, post_weight, gate)
+    dev = N.require_device((dx_out, dh, x, y, weight, post_weight, gate, seed), "residual_norm_backward")
     with N.on_device(dev):
         lib = N.load()
-        (_d, dd), (_h, ddh), (xo, dxo), (_y, dy_) = map(N.rows_of, (dx_out, dh, x_out, y))
+        (_d, dd), (_h, ddh), (x2, dx), (_y, dy) = map(N.rows_of, (dx_out, dh, x, y))
         weight, post_weight, gate = _vec(weight), _vec(post_weight), _vec(gate)
-        there = (True, True, weight is not None, post_weight is not None, gate is not None)
+        there = (True, dh is None or y is not None, weight is not None, post_weight is not None, gate is not None)
         needs = tuple(bool(n) and t for n, t in zip(needs, there))
-        C = x_out.shape[-1]
-        outs = [torch.empty(s, dtype=x_out.dtype, device=dev) if n else None
-                for n, s in zip(needs, (xo.shape, xo.shape, (C,), (C,), (C,)))]
+        C = x.shape[-1]
+        outs = [torch.empty(s, dtype=x.dtype, device=dev) if n else None
+                for n, s in zip(needs, (x2.shape, x2.shape, (C,), (C,), (C,)))]
         grads = needs[2] + 2 * needs[4] + 4 * needs[3]
-        ws = _workspace(lib.maba_hip_residual_norm_backward_workspace_size(dxo, grads), dev) if grads else None
-        rc = lib.maba_hip_residual_norm_backward(dd, ddh, dxo, dy_, N.rows_desc(weight), N.rows_desc(post_weight), N.rows_desc(gate),
+        ws = _workspace(lib.maba_hip_residual_norm_backward_workspace_size(dx, grads), dev) if grads else None
+        rc = lib.maba_hip_residual_norm_backward(dd, ddh, dx, dy, N.rows_desc(weight), N.rows_desc(post_weight), N.rows_desc(gate),
                                                  float(scale), float(p), _seed_ptr(p, seed), stream, float(eps),
                                                  *map(N.rows_desc, outs), ws.data_ptr() if grads else None,
                                                  ws.numel() if grads else 0, N.stream_ptr(dev))
         N.check(rc, "residual_norm_backward")
-    if x_out.dim() != 2:
-        outs[:2] = [o if o is None else o.view(x_out.shape) for o in outs[:2]]
+    if x.dim() != 2:
+        outs[:2] = [o if o is None else o.view(x.shape) for o in outs[:2]]
     return tuple(outs)
 
 

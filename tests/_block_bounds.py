@@ -80,6 +80,19 @@ def _norm(x, eps):
     return torch.rsqrt((x * x).mean(-1, keepdim=True) + eps), ((C + 4) / 2 + 6) * U
 
 
+def added(x, y, wp, g, scale, keep, p, eps):
+    """x_out of x and y in 64 bits, and its error in fp32 before it is rounded."""
+    z, rel = y, 0.0
+    if wp is not None:
+        rp, rel = _norm(y, eps)
+        z = y * rp * wp.double()
+    if keep is not None:
+        z = torch.where(keep, z / (1 - p) if p < 1 else 0.0, 0.0)
+    add = scale * z * (1.0 if g is None else g.double())
+    x = x + add
+    return x, (rel + 7 * U) * add.abs() + U * x.abs()
+
+
 def boundary(x, y, w=None, wp=None, g=None, scale=1.0, keep=None, p=0.0, eps=1e-6):
     """{name: (value, bound)} of x_out and, with a weight, of h."""
     dt = x.dtype
@@ -87,15 +100,7 @@ def boundary(x, y, w=None, wp=None, g=None, scale=1.0, keep=None, p=0.0, eps=1e-
     e = torch.zeros_like(x)
     out = {}
     if y is not None:
-        z, rel = y, 0.0
-        if wp is not None:
-            rp, rel = _norm(y, eps)
-            z = y * rp * wp.double()
-        if keep is not None:
-            z = torch.where(keep, z / (1 - p) if p < 1 else 0.0, 0.0)
-        add = scale * z * (1.0 if g is None else g.double())
-        x = x + add
-        e = (rel + 7 * U) * add.abs() + U * x.abs()
+        x, e = added(x, y, wp, g, scale, keep, p, eps)
         out["x_out"] = (x, rounded(x, e, dt))
     if w is not None:
         r, rel = _norm(x, eps)
@@ -105,26 +110,30 @@ def boundary(x, y, w=None, wp=None, g=None, scale=1.0, keep=None, p=0.0, eps=1e-
     return out
 
 
-def boundary_backward(dxo, dh, xo, y=None, w=None, wp=None, g=None, scale=1.0, keep=None, p=0.0, eps=1e-6):
-    """{name: (value, bound)} of dx, dy, dweight, dpost_weight and dgate."""
-    dt, (R, C) = xo.dtype, xo.shape
-    xo = xo.double()
+def boundary_backward(dxo, dh, x, y=None, w=None, wp=None, g=None, scale=1.0, keep=None, p=0.0, eps=1e-6):
+    """{name: (value, bound)} of dx, dy, dweight, dpost_weight and dgate, for the forward's x and y."""
+    dt, (R, C) = x.dtype, x.shape
+    xo, ex = x.double(), torch.zeros_like(x, dtype=torch.float64)
+    if y is not None and dh is not None:                    # x_out and its error in fp32
+        xo, ex = added(x.double(), y.double(), wp, g, scale, keep, p, eps)
     d = torch.zeros_like(xo) if dxo is None else dxo.double()
     e = torch.zeros_like(d)
     out, rows, cols = {}, (R + 64) * U, (C + 4) * U
     if dh is not None:
         h, w = dh.double(), w.double()
         r, rel = _norm(xo, eps)
-        xh, hw = xo * r, h * w
+        rel = rel + (xo.abs() * ex).sum(-1, keepdim=True) / ((xo * xo).sum(-1, keepdim=True) + C * eps)
+        xh, hw, exh = xo * r, h * w, ex * r
         mean = (hw * xh).mean(-1, keepdim=True)
         em = (hw * xh).abs().mean(-1, keepdim=True) * (cols + rel + 4 * U) + (rel + 3 * U) * mean.abs()
+        em = em + (hw.abs() * exh).mean(-1, keepdim=True)
         inner = hw - xh * mean
-        ei = 2 * U * hw.abs() + xh.abs() * em + (rel + 3 * U) * (xh * mean).abs()
+        ei = 2 * U * hw.abs() + xh.abs() * em + (rel + 3 * U) * (xh * mean).abs() + exh * mean.abs()
         d = d + r * inner
         e = r * ei + (rel + 2 * U) * (r * inner).abs() + 2 * U * d.abs()
         t = h * xh
         dw = t.sum(0)
-        out["dweight"] = (dw, rounded(dw, ((rel + 3 * U + rows) * t.abs()).sum(0), dt))
+        out["dweight"] = (dw, rounded(dw, ((rel + 3 * U + rows) * t.abs() + h.abs() * exh).sum(0), dt))
     elif w is not None:
         out["dweight"] = (torch.zeros(C, dtype=d.dtype, device=d.device),) * 2
     out["dx"] = (d, rounded(d, e, dt))

@@ -116,24 +116,23 @@ def test_boundary_values_and_backward_op(parts, dtype):
     if h is not None:
         B.check(h, want["h"], "h")
     dxo = _rand(9, 33, dtype=dtype, grad=False, seed=9)
-    got = D.residual_norm_backward(dxo, dh, xo, t["y"], **{v: t[v] for v in names.values()}, seed=SEED, stream=2, **kw)
-    want = B.boundary_backward(dxo, dh, xo, t["y"], **{k: t[v] for k, v in names.items()}, keep=keep, **kw)
+    got = D.residual_norm_backward(dxo, dh, t["x"], t["y"], **{v: t[v] for v in names.values()}, seed=SEED, stream=2, **kw)
+    want = B.boundary_backward(dxo, dh, t["x"], t["y"], **{k: t[v] for k, v in names.items()}, keep=keep, **kw)
     for name, v in zip(("dx", "dy", "dweight", "dpost_weight", "dgate"), got):
         if v is not None:
             B.check(v, want[name], name)
         else:
-            assert name != "dx" and name != "dy"
+            assert name != "dx" and (name != "dy" or t["y"] is None)
 
 
 def test_boundary_needs_and_missing_gradients():
     t = {k: v.detach() for k, v in _tensors().items()}
     kw = dict(weight=t["weight"], post_weight=t["post_weight"], gate=t["gate"])
-    xo, h = D.residual_norm(t["x"], t["y"], **kw)
     g = _rand(7, 12, grad=False, seed=9)
-    full = D.residual_norm_backward(g, None, xo, t["y"], **kw)
+    full = D.residual_norm_backward(g, None, t["x"], t["y"], **kw)
     assert torch.equal(full[0], g) and (full[2] == 0).all()
     for needs in ((1, 0, 0, 0, 0), (0, 1, 0, 1, 0), (0, 0, 0, 0, 1)):
-        for a, b, n in zip(D.residual_norm_backward(g, None, xo, t["y"], **kw, needs=needs), full, needs):
+        for a, b, n in zip(D.residual_norm_backward(g, None, t["x"], t["y"], **kw, needs=needs), full, needs):
             assert (a is None) if not n else torch.equal(a, b)
 
 
@@ -445,7 +444,7 @@ def test_c_boundary_backward_refusals(lib):
         return lib.maba_hip_residual_norm_backward(dxo, dh, x, y, weight, wp, g, 1.0, p, seed, 0, 1e-6, dx, dy, dw, dwp, dg, ws, size, None)
 
     for kw, rc, text in ((dict(dxo=None, dh=None), 1, b"required"), (dict(weight=None), 1, b"goes with weight"),
-                         (dict(y=None, wp=w), 1, b"go with y"), (dict(dg=_t([8], data=far)), 1, b"missing parameter"),
+                         (dict(y=None, wp=w), 1, b"go with y"), (dict(y=None, dy=_t([8, 8], data=far)), 1, b"dy"), (dict(y=None, dx=None, dy=t["o"]), 1, b"dy goes with y"), (dict(dg=_t([8], data=far)), 1, b"missing parameter"),
                          (dict(dwp=_t([8], data=far)), 1, b"missing parameter"), (dict(dx=t["d"]), 1, b"overlaps an input"),
                          (dict(dy=t["o"]), 1, b"outputs overlap"), (dict(dw=_t([8], data=far)), 5, b"workspace"),
                          (dict(dw=_t([8], data=far), ws=(8 << 24) + 8, size=1 << 20), 1, b"16-byte aligned"),

@@ -132,9 +132,8 @@ def _check_boundary(t, dt, p, seed=0, wrap=lambda v: v):
         B.check(h, want["h"], "h")
     r = _gen(seed + 1)
     dxo, dh = (0.3 * r(M, Cw)).to(dt), (0.3 * r(M, Cw)).to(dt) if t["weight"] is not None else None
-    xo = x if y is None else xo
-    got = D.residual_norm_backward(wrap(dxo), None if dh is None else wrap(dh), wrap(xo), None if y is None else wrap(y), **kw, **args)
-    want = B.boundary_backward(dxo, dh, xo, y, **ref, scale=0.7, keep=keep, p=p)
+    got = D.residual_norm_backward(wrap(dxo), None if dh is None else wrap(dh), wrap(x), None if y is None else wrap(y), **kw, **args)
+    want = B.boundary_backward(dxo, dh, x, y, **ref, scale=0.7, keep=keep, p=p)
     for name, v in zip(("dx", "dy", "dweight", "dpost_weight", "dgate"), got):
         if v is not None and (name != "dy" or y is not None):
             B.check(v, want[name], name)
@@ -179,7 +178,7 @@ def test_boundary_p_of_one_and_scale_of_zero():
         xo, h = D.residual_norm(t["x"], t["y"], **kw, **args)
         assert torch.equal(xo, t["x"])
         B.check(h, B.boundary(t["x"], None, t["weight"])["h"], "h")
-        dx, dy, dw, dpw, dg = D.residual_norm_backward(t["x"], h, xo, t["y"], **kw, **args)
+        dx, dy, dw, dpw, dg = D.residual_norm_backward(t["x"], h, t["x"], t["y"], **kw, **args)
         assert not dy.any() and not dpw.any() and not dg.any() and dx.any() and dw.any()
 
 
@@ -197,8 +196,8 @@ def test_rows_of_zeros_and_an_eps_of_zero(dt):
     want = B.boundary(x, y, t["weight"], t["post_weight"], t["gate"], eps=0.0)
     B.check(xo, want["x_out"], "x_out")
     B.check(h, want["h"], "h")
-    got = D.residual_norm_backward(x, y, xo, y, **kw, eps=0.0)
-    want = B.boundary_backward(x, y, xo, y, t["weight"], t["post_weight"], t["gate"], eps=0.0)
+    got = D.residual_norm_backward(x, y, x, y, **kw, eps=0.0)
+    want = B.boundary_backward(x, y, x, y, t["weight"], t["post_weight"], t["gate"], eps=0.0)
     for name, v in zip(("dx", "dy", "dweight", "dpost_weight", "dgate"), got):
         B.check(v, want[name], name)
 
@@ -250,8 +249,8 @@ def test_boundary_bad_rows_stay_in_their_rows():
         want = B.boundary(t["x"][rows], t["y"][rows], t["weight"], t["post_weight"], t["gate"])
         B.check(xo[rows], want["x_out"], "x_out")
         B.check(h[rows], want["h"], "h")
-        dx, dy, *_ = D.residual_norm_backward(t["x"], t["y"], xo, t["y"], **kw)
-        want = B.boundary_backward(t["x"][rows], t["y"][rows], xo[rows], t["y"][rows], t["weight"], t["post_weight"], t["gate"])
+        dx, dy, *_ = D.residual_norm_backward(t["x"], t["y"], t["x"], t["y"], **kw)
+        want = B.boundary_backward(t["x"][rows], t["y"][rows], t["x"][rows], t["y"][rows], t["weight"], t["post_weight"], t["gate"])
         B.check(dx[rows], want["dx"], "dx")
         B.check(dy[rows], want["dy"], "dy")
 
@@ -293,9 +292,9 @@ def test_offsets_past_32_bits():
 def test_post_norm_backward_has_the_same_bits_on_every_call(dt, Cw):
     """Rows of several waves sum three values over the row, then one: sums of different rows or calls share nothing."""
     M, f = 3000, _gen(60)
-    d, dh, xo, y = (f(M, Cw).to(dt) for _ in range(4))
+    d, dh, x, y = (f(M, Cw).to(dt) for _ in range(4))
     w, wp, g = (1 + 0.1 * f(Cw).to(dt) for _ in range(3))
-    call = lambda: D.residual_norm_backward(d, dh, xo, y, w, wp, g, 0.5, 0.1, _seed(), 1)
+    call = lambda: D.residual_norm_backward(d, dh, x, y, w, wp, g, 0.5, 0.1, _seed(), 1)
     want = call()
     for _ in range(20):
         assert all(torch.equal(a, b) for a, b in zip(call(), want))
@@ -553,7 +552,7 @@ def test_a_training_step_of_all_of_them():
         B.check(x2, want["x_out"], "x_out")
         B.check(h2, want["h"], "h")
         dxo = (x2.float() * (2e-3 / x2.numel())).to(BF)
-        want = B.boundary_backward(dxo, h2.grad, x2, f, w2, wp, gate, 0.5, keep, 0.2)
+        want = B.boundary_backward(dxo, h2.grad, x, f, w2, wp, gate, 0.5, keep, 0.2)
         for name, v in (("dy", f.grad), ("dweight", w2.grad), ("dpost_weight", wp.grad), ("dgate", gate.grad)):
             B.check(v, want[name], name)
         # x has two gradients, its norm's and the boundary's, each rounded once and their sum again
@@ -676,14 +675,15 @@ def test_saved_tensors_follow_their_versions():
     seed += 1
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
-    xo, h = D.residual_norm(x, x * 2, x.detach()[0].clone())
-    xo.mul_(2)                                                              # the backward pass reads it
+    y = x * 2
+    xo, h = D.residual_norm(x, y, x.detach()[0].clone())
+    y.mul_(2)                                                               # the backward pass reads it
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         h.sum().backward()
     seen = []
     with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t.shape) or t.cpu(), lambda t: t.to(DEV)):
         out = D.residual_norm(x, x.detach(), x.detach()[0].clone(), p=0.5, seed=seed)
-    assert len(seen) == 3                                                   # x_out, the weight and the seed; y is not read
+    assert len(seen) == 4                                                   # x, y, the weight and the seed
     assert torch.isfinite(torch.autograd.grad(out, x, [x.detach(), x.detach()])[0].float()).all()
 
 
