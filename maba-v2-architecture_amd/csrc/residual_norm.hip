@@ -173,7 +173,7 @@ __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(Bounda
   const Rows wd(a.dxo, a.dxos, l, sub), wh(a.dh, a.dhs, l, sub), wx(a.x, a.xs, l, sub), wy(a.y, a.ys, l, sub);
   const Rows wdx(a.dx, a.dxs, l, sub), wdy(a.dy, a.dys, l, sub);
   const uint64_t key = a.d.mode == 1 ? *a.d.seed : 0;
-  const float inv_c = 1.f / (float)a.C;
+  const float inv_c = 1.f / (float)a.C, scale = a.scale * a.d.keep;      // of what is kept
   // chunk c of the parameters: weight's, gate's, post_weight's
   const int chunks = (a.C + V - 1) / V;
   u32x4* par = (u32x4*)sums;
@@ -279,7 +279,7 @@ __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(Bounda
       if (a.dh) {
         float h[V], p[V];
         unpack<T>(u.x[i], xn[i]);
-        if (a.y) {                           // as the forward does
+        if (a.y) {                           // as the forward does, but for the order of its factors
           float z[V];
           unpack<T>(u.y[i], z);
           if constexpr (POST) {
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(Bounda
             for (int e = 0; e < V; ++e) z[e] *= p[e];
           }
 #pragma unroll
-          for (int e = 0; e < V; ++e) xn[i][e] = fmaf(a.scale, z[e], xn[i][e]);
+          for (int e = 0; e < V; ++e) xn[i][e] = fmaf(scale, z[e], xn[i][e]);
         }
         unpack<T>(u.h[i], h);
         unpack<T>(par[pc[i]], p);
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(Bounda
       }
       if (a.dx) put(wdx, i, d);
       if (a.dy || (a.grads & (GRAD_GATE | GRAD_POST))) {
-        // dropout(z) = m z with m in {0, 1 / (1 - p)}: both products with m follow from m dX
+        // dropout(z) = m z with m in {0, 1 / (1 - p)}: both products with m follow from m dX (the factor is in scale)
         drop_by<V>(d, a.d, bits[i]);
         float p[V], y[V];
         unpack<T>(u.y[i], y);
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(Bounda
 #pragma unroll
           for (int e = 0; e < V; ++e) acc[1][i][e] = fmaf(d[e], POST ? y[e] * p[e] : y[e], acc[1][i][e]);
 #pragma unroll
-        for (int e = 0; e < V; ++e) d[e] *= a.scale;
+        for (int e = 0; e < V; ++e) d[e] *= scale;
         if (a.g) {
           float q[V];
           unpack<T>(par[chunks + pc[i]], q);
@@ -720,7 +720,7 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
     ColumnsArgs c = {(const float*)workspace, {}, {}, R > 0 ? groups : 0, n, (int)C};
     int k = 0;
     if (dweight) { c.out[k] = dweight->data; c.factor[k++] = 1.f; }
-    if (dgate) { c.out[k] = dgate->data; c.factor[k++] = scale; }
+    if (dgate) { c.out[k] = dgate->data; c.factor[k++] = scale * a.d.keep; }
     if (dpost_weight) { c.out[k] = dpost_weight->data; c.factor[k++] = 1.f; }
     auto f = dt == MABA_F32 ? columns_kernel<F32> : dt == MABA_BF16 ? columns_kernel<Bf16> : columns_kernel<Fp16>;
     hipLaunchKernelGGL(f, dim3((unsigned)ceil_div(C, 32), n), dim3(1024), 0, (hipStream_t)stream, c);

@@ -281,12 +281,12 @@ __device__ __forceinline__ uint32_t kept_bits(const Drop& d, uint64_t key, int64
   }
   return bits;
 }
-// drop_chunk() by such bits.
+// drop_chunk() by such bits, without the factor.
 template <int V>
 __device__ __forceinline__ void drop_by(float (&v)[V], const Drop& d, uint32_t bits) {
   if (d.mode == 0) return;
 #pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = bits >> e & 1 ? v[e] * d.keep : 0.f;
+  for (int e = 0; e < V; ++e) v[e] = __uint_as_float(__float_as_uint(v[e]) & (uint32_t)__builtin_amdgcn_sbfe((int)bits, e, 1));
 }
 // v where it is kept, times 1 / (1 - p); zero, whatever v is, where it is dropped.  `at` is a multiple of four.
 template <int V>
