@@ -153,12 +153,13 @@ struct BoundaryBackArgs {
 };
 
 // A row's sums are exchanged twice: those of dh w x' and x'^2 (the mean of dh w x^ is r times that of dh w x'), and with POST that
-// for dy together with the next row's of y^2.  The chunks stay packed in registers between their uses, the mask as bits.  16,384 x 640 bf16 with dropout 35 us, 3.6 TB/s, where
-// every second lane has one chunk of two; 8,192 x 4,096 with both norms and dropout 87 us, 4.6 TB/s; 8,191 x 4,095 125 us, 3.2 TB/s.
+// for dy together with the next row's of y^2.  The chunks stay packed in registers between their uses, the mask as bits.  HBM, and
+// arithmetic that its waits do not hide: 16,384 x 640 bf16 with dropout 36 us, 3.5 TB/s (every second lane has one chunk of two),
+// 8,192 x 4,096 86 us, 4.7 TB/s, and with both norms 101, 4.0 TB/s, the vector units 67 % busy; 8,191 x 4,095 132 us, 3.1 TB/s.
 // WHOLE: rows of whole 16-byte chunks (WholeWalk).  The next rows' chunks are loaded ahead of the present ones' arithmetic.
 // One workgroup a compute unit, as large as registers allow: of four waves a SIMD with one chunk a lane, of two beyond.  So
-// the fewest partials are written: 8,192 x 4,096 bf16 with post_weight 92 us and without 86, as two workgroups of half the threads
-// 97 and 92; 2,048 x 640 15.6 and, as three of 256 threads, 17.4; fp32 8,192 x 2,048 82 and 88.
+// the fewest partials are written: 8,192 x 4,096 bf16 87 us, as two workgroups of half the threads 91; 2,048 x 640 13.1, of 512
+// threads 14.3 and of 256 16.2; fp32 8,192 x 2,048 83, of 256 89.
 constexpr int back_threads(int nch) { return nch == 1 ? 1024 : 512; }
 template <class T, int NCH, bool POST, bool WHOLE>
 __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(BoundaryBackArgs a) {
@@ -413,7 +414,7 @@ __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(Bounda
 }
 
 // out[c] = factor * the sum over g of p[g][n][c]: 32 runs of g side by side, each in its order, then the runs in theirs.
-// Bound by the latency of a run's loads: 768 partials of 2 x 640 columns 4 us, 512 of 3 x 4,096 6 us.
+// Bound by the latency of a run's loads: 256 partials of 2 x 640 columns 4.0 us, of 3 x 4,096 5.0 us.
 struct ColumnsArgs {
   const float* p;
   void* out[3];
@@ -520,9 +521,9 @@ static bool whole_rows(std::initializer_list<const maba_tensor*> all) {
 // (80 chunks of 640 16-bit elements fill 62 % of 128 lanes and 83 % of 32 with three each) and share out what a row costs
 // besides its elements.  Forward, in us, 8 / 24 elements: 1 x 640 bf16 3.1 / 4.1, 2,048 x 640 5.5 / 5.8, 32,768 x 640
 // 42.8 / 32.8, 8,192 x 4,096 50.5 / 47.3; fp32 8,192 x 1,000 22.9 / 24.6.  Backward, 8 / 16: 64 x 640 8.6 / 10.4, 16,384 x 640
-// 36.7 / 35.5, 65,536 x 640 118 / 109, with post_weight 24,576 x 640 57 / 49, x 767 87 / 71 (without 72 / 71); rows of more than
-// a wave either way 24,576 x 1,345 165 / 173 and without post_weight 16,384 x 1,536 66 / 76; where all lanes of 8 have work
-// 24,576 x 512 36 / 38, 2,048 x 4,096 37 / 43, 8,192 x 4,096 98 / 103.
+// 38.1 / 37.7, 65,536 x 640 118 / 110 and with post_weight 150 / 131, 24,576 x 767 75 / 72 and with post_weight 101 / 79; where all
+// lanes of 8 have work 24,576 x 512 34 / 37, and rows of more than a wave either way 24,576 x 1,345 128 / 149, 8,192 x 4,096 87 / 87
+// and 2,048 x 4,096 29 / 32.
 constexpr int MOST_ELEMS = 24, MOST_BACK = 16;
 static int forward_elems(int64_t R, int64_t C, int dtype) { return C > 8 << MAX_LG ? 16 : dtype != MABA_F32 && R > 4096 ? MOST_ELEMS : 8; }
 static int back_elems(int64_t R, int64_t C, int dtype) {
