@@ -25,6 +25,8 @@ Differences, all deliberate:
 * The feed-forward operators ``gated_ffn`` and ``linear_epilogue`` (model.py:25-38, 92-128, where
   the reference composes torch modules) carry their own gradients on every backend, through their
   ``*_backward`` ops; ``checkpoint_pack`` and ``checkpoint_unpack`` hold activations in 8 bits.
+* So do ``residual_norm`` (the block boundary of model.py:11-22, 92-128, with a norm on the
+  sub-layer's output, a scale and dropout), ``dropout`` and ``token_logprobs``.
 * ``allow_mixed_dtypes=True`` (keyword) lets ``dgda_prefill``/``dgda_step``
   accept bf16 q/k/v with fp32 gates and state; without it the reference's
   "dtypes must match" ``TypeError`` is kept.

@@ -3,10 +3,12 @@
 Each wrapper keeps the reference op's keyword signature and return
 convention, allocates outputs (and any workspace) with torch on the inputs'
 device, and enqueues the HIP kernels on torch's current stream; the library
-itself never allocates.  The kernels are forward-only: when autograd needs
-gradients a wrapper raises ``NotImplementedError`` so that the dispatcher falls
+itself never allocates.  The wrappers are forward-only: when autograd needs
+gradients one raises ``NotImplementedError`` so that the dispatcher falls
 back to the differentiable reference path (reference tests check gradients
-through the dispatcher, tests/test_dispatcher.py:324-443).
+through the dispatcher, tests/test_dispatcher.py:324-443).  The ops with a
+``*_backward`` wrapper of their own, and dropout, are differentiable through
+the autograd functions of ``feed_forward.py`` and ``block_ends.py``.
 
 Reference wrappers mirrored (paths relative to the reference checkout):
 ``triton_dgda_prefill``/``triton_dgda_step`` (kernels/triton_dgda.py:647-685),
