@@ -367,7 +367,7 @@ struct BackwardArgs {
   const int64_t* targets;
   const float *dlogp, *dentropy, *dlse, *lse, *entropy;
   int64_t first, R;                  // rows first to R - 1
-  int V, lg, parts;                  // 2^lg threads a row and `parts` workgroups side by side on it
+  int V, lg, parts;                  // 2^lg threads a row, 64 or 256, and `parts` workgroups side by side on it
   float inv;
 };
 
@@ -385,26 +385,30 @@ __global__ __launch_bounds__(256) void logprobs_back_kernel(BackwardArgs a) {
   const float h = a.entropy[r];
   float gh = a.dentropy ? a.dentropy[r] : 0.f;
   float gl = target < 0 || !a.dlogp ? 0.f : target >= a.V ? NAN : a.dlogp[r], gz = a.dlse ? a.dlse[r] : 0.f;
-  // log p = l / T - lse is as exact as lse, which far from zero is not enough: there the row is summed again, by each wave
-  // for itself, and log p counted from its largest element.
+  // log p = l / T - lse is as exact as lse, whose rounding far from zero is more than those of p and of the result: there the
+  // row is summed again and log p counted from its largest element.  All of that ends before anything of the row is
+  // written, which may be the logits' own.  (1,024 x 32,768 bf16 24 us without such rows, 63 with nothing else.)
+  constexpr float EXACT = T::CODE == MABA_F32 ? 32.f : 256.f;
+  __shared__ float part[2][4];
   float m = 0.f;
   if (lse == -INFINITY) {            // no mass: no element has a gradient
     lse = -LOWEST;
     gl = gh = gz = 0.f;              // whatever comes from a loss of lse = -inf
-  } else if (fabsf(lse) > 256.f) {
+  } else if (fabsf(lse) > EXACT) {
     m = -INFINITY;
-    const int l = threadIdx.x & 63;
-    for_chunks<T, 1>(row, a.V, l, 64, [&](auto& v, int) {
+    const int l = threadIdx.x & ((1 << a.lg) - 1);
+    const auto of_row = [&](float v, float* shared, auto f) { return a.lg == 8 ? across<4>(v, shared, f) : wave_joined(v, f); };
+    for_chunks<T, 2>(row, a.V, l, 1 << a.lg, [&](auto& v, int) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
+      for (float x : v) m = fmaxf(m, x);
     });
-    m = across<1>(m, nullptr, larger);
+    m = of_row(m, part[0], larger);
     float s = 0.f;
-    for_chunks<T, 1>(row, a.V, l, 64, [&](auto& v, int) {
+    for_chunks<T, 2>(row, a.V, l, 1 << a.lg, [&](auto& v, int) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((v[e] - m) * a.inv * LOG2E);
+      for (float x : v) s += __builtin_amdgcn_exp2f((x - m) * a.inv * LOG2E);
     });
-    lse = __builtin_amdgcn_logf(across<1>(s, nullptr, sum_of)) * LN2;
+    lse = __builtin_amdgcn_logf(of_row(s, part[1], sum_of)) * LN2;
   }
   const float base = gz - gl - (gh != 0.f ? gh * h : 0.f), at_target = gl * a.inv;
   const int lanes = a.parts << a.lg, lane = ((int)(blockIdx.x % a.parts) << a.lg) + (threadIdx.x & ((1 << a.lg) - 1));
@@ -575,10 +579,10 @@ extern "C" int maba_hip_token_logprobs_backward(const maba_tensor* dlogp, const 
                     dlogp ? (const float*)dlogp->data : nullptr, dentropy ? (const float*)dentropy->data : nullptr,
                     dlse ? (const float*)dlse->data : nullptr, (const float*)lse->data, (const float*)entropy->data, 0, R, (int)V, 6, 1,
                     (float)(1.0 / temperature)};
-  while (a.lg < 8 && chunks > (int64_t)4 << a.lg) ++a.lg;
+  // four waves a row, or one (us, one / four: 8,192 x 2,100 bf16 17.9 / 23.3, x 4,000 24.4 / 24.1, 300 x 4,000 6.4 / 5.0)
+  if (chunks > (R > 4 * (int64_t)device_cu_count() ? 512 : 256)) a.lg = 8;
   a.parts = (int)std::min<int64_t>(ceil_div(chunks, 256 * 8), std::max<int64_t>(MOST_ROWS / R, 1));
-  // in place a row is one wave's: it may be summed again, and then nothing of it may have been written yet
-  if (logits->data == dlogits->data) a.lg = 6, a.parts = 1;
+  if (logits->data == dlogits->data) a.parts = 1;
   auto kernel = logits->dtype == MABA_F32 ? logprobs_back_kernel<F32> : logits->dtype == MABA_BF16 ? logprobs_back_kernel<Bf16>
                                                                                                   : logprobs_back_kernel<Fp16>;
   in_launches(R, [&](int64_t first, int64_t end) {
