@@ -346,6 +346,8 @@ def _decode_linear_fits(model: "MabaSparseForCausalLM") -> bool:
 
 
 class MabaSparseForCausalLM(WeightCacheMixin, nn.Module):
+    _generating = False
+
     def __init__(self, config: Optional[MabaConfig] = None) -> None:
         super().__init__()
         self.config = config or get_101m_config()
@@ -430,7 +432,7 @@ class MabaSparseForCausalLM(WeightCacheMixin, nn.Module):
     def next_dropout_seed(self) -> Optional[torch.Tensor]:
         """The seed of this training step's masks, on which ``dropout_seed`` moves on (also where the step is replayed
         from a captured graph); None where nothing is dropped.  Ranks of a data-parallel job start it from different values."""
-        if not self.training or getattr(self, "dropout_seed", None) is None:
+        if not self.training or self._generating or getattr(self, "dropout_seed", None) is None:
             return None
         with torch.no_grad():
             seed = self.dropout_seed.clone()
@@ -520,13 +522,19 @@ class MabaSparseForCausalLM(WeightCacheMixin, nn.Module):
         one HIP graph of a step, captured once and replayed for every further token.
         Otherwise each step runs eagerly over ``LatentCache``s.
 
+        Nothing is dropped out, also of a model that is training.
+
         The stacked and converted weights the decode path keeps are dropped on entry, so a
         weight written through ``.data`` since the last call takes effect."""
         self.clear_weight_caches()
         B, L = input_ids.shape
         if graph is None:
             graph = self.serving_graph_ok(input_ids)
-        logits, states = self(input_ids, last_only=True)
+        self._generating = True
+        try:
+            logits, states = self(input_ids, last_only=True)
+        finally:
+            self._generating = False
         if graph:
             return self._generate_graph(logits, states, L, max_new_tokens, on_prefill_done, return_logits,
                                         on_graph_ready)

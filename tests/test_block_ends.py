@@ -597,6 +597,14 @@ def test_generation_with_post_norms_equals_state_passing():
     assert torch.equal(got, torch.cat(ref, dim=1))
 
 
+def test_generation_drops_nothing():
+    m, ids = _model(dropout=0.5), _ids(100)
+    seed, got = m.dropout_seed.clone(), m.train().generate_greedy(ids, 4)
+    assert torch.equal(got, m.eval().generate_greedy(ids, 4)) and torch.equal(m.dropout_seed, seed)
+    m.train()
+    assert not torch.equal(m(ids)[0], m(ids)[0])
+
+
 def test_blocks_of_configs_and_modules_from_before_the_fields():
     from types import SimpleNamespace
     cfg = MabaConfig(dim=64, n_heads=1, intermediate_size=40, n_layers=1)
