@@ -599,8 +599,10 @@ def test_generation_with_post_norms_equals_state_passing():
 
 def test_generation_drops_nothing():
     m, ids = _model(dropout=0.5), _ids(100)
-    seed, got = m.dropout_seed.clone(), m.train().generate_greedy(ids, 4)
-    assert torch.equal(got, m.eval().generate_greedy(ids, 4)) and torch.equal(m.dropout_seed, seed)
+    seed = m.dropout_seed.clone()
+    # the prompt's logits (the layers keep no decode caches while training, so later ones differ for that)
+    got, want = (v.generate_greedy(ids, 2, return_logits=True)[1][:, 0] for v in (m.train(), m.eval()))
+    assert torch.equal(got, want) and torch.equal(m.dropout_seed, seed)
     m.train()
     assert not torch.equal(m(ids)[0], m(ids)[0])
 
