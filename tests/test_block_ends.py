@@ -601,7 +601,7 @@ def test_generation_drops_nothing():
     m, ids = _model(dropout=0.5), _ids(100)
     seed = m.dropout_seed.clone()
     # the prompt's logits (the layers keep no decode caches while training, so later ones differ for that)
-    got, want = (v.generate_greedy(ids, 2, return_logits=True)[1][:, 0] for v in (m.train(), m.eval()))
+    got, want = (m.train(mode).generate_greedy(ids, 2, return_logits=True)[1][:, 0] for mode in (True, False))
     assert torch.equal(got, want) and torch.equal(m.dropout_seed, seed)
     m.train()
     assert not torch.equal(m(ids)[0], m(ids)[0])
