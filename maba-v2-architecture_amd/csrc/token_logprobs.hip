@@ -446,6 +446,10 @@ static int check_logits(const maba_tensor* t, const char* who, const char* name,
   if (t->shape[n - 1] < 1) return fail(MABA_ERR_INVALID, "%s: the vocabulary must not be empty", who);
   if (t->shape[n - 1] > (1 << 28)) return fail(MABA_ERR_UNSUPPORTED, "%s: at most %d tokens", who, 1 << 28);
   if (t->shape[n - 1] > 1 && t->stride[n - 1] != 1) return fail(MABA_ERR_INVALID, "%s: %s needs unit column stride", who, name);
+  for (int i = 0; i + 1 < n; ++i) {
+    if (t->shape[i] < 0) return fail(MABA_ERR_INVALID, "%s: %s has a negative size", who, name);
+    if (t->shape[i] > 0x7fffffff) return fail(MABA_ERR_UNSUPPORTED, "%s: too many rows", who);
+  }
   rows = t->shape[0] * (n == 3 ? t->shape[1] : 1);
   for (int i = 0; i < n; ++i)
     if (t->stride[i] < 0) return fail(MABA_ERR_INVALID, "%s: %s has a negative stride", who, name);

@@ -478,6 +478,9 @@ def _logprobs(lib, x=None, t=None, T=1.0, outs=None, tl=None, ti=None):
     (dict(tl=_t([4, 9], dtype=F32, data=6 << 24), ti=_t([4, 9], dtype=N.MABA_I64, data=7 << 24)), 1, b"between 1 and V"),
     (dict(tl=_t([4, 2], dtype=F32, data=6 << 24), ti=_t([4, 2], dtype=N.MABA_I32, data=7 << 24)), 2, b"i64"),
     (dict(tl=_t([4, 3], dtype=F32, data=6 << 24), ti=_t([4, 2], dtype=N.MABA_I64, data=7 << 24)), 1, b"contiguous"),
+    (dict(x=_t([1 << 40, 1 << 40, 8], strides=[0, 0, 1], data=A)), 3, b"too many rows"),
+    (dict(x=_t([1 << 32, 1 << 32, 8], strides=[0, 0, 1], data=A)), 3, b"too many rows"),
+    (dict(x=_t([-1, 8], data=A)), 1, b"negative size"),
     (dict(x=_t([4, 100], data=A), tl=_t([4, 65], dtype=F32, data=6 << 24), ti=_t([4, 65], dtype=N.MABA_I64, data=7 << 24)), 3, b"64"),
 ])
 def test_c_logprob_refusals(lib, kw, rc, text):
