@@ -487,6 +487,7 @@ static int check_float_rows(const maba_tensor* t, const char* who) {
   if (!is_float_dt(t->dtype)) return fail(MABA_ERR_DTYPE, "%s: f32, f16 or bf16 only, got dtype code %d", who, t->dtype);
   if (t->ndim != 2) return fail(MABA_ERR_INVALID, "%s: x must be 2D, got %dD", who, t->ndim);
   if (t->shape[1] < 1) return fail(MABA_ERR_INVALID, "%s: the width must be positive", who);
+  if (t->shape[0] < 0) return fail(MABA_ERR_INVALID, "%s: x has a negative size", who);
   if (t->shape[1] > (1 << 30) || t->shape[0] > (int64_t)1 << 40) return fail(MABA_ERR_UNSUPPORTED, "%s: sizes out of range", who);
   return MABA_OK;
 }

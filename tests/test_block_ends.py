@@ -382,6 +382,7 @@ F32 = N.MABA_F32
 @pytest.mark.parametrize("x,p,seed,out,rc,text", [
     (None, 0.1, 64, _t([4, 8], data=Bt), 1, b"missing"),
     (_t([4, 8, 1], data=A), 0.1, 64, _t([4, 8], data=Bt), 1, b"2D"),
+    (_t([-1, 8], data=A), 0.1, 64, _t([-1, 8], data=Bt), 1, b"negative size"),
     (_t([4, 8], dtype=N.MABA_F64, data=A), 0.1, 64, _t([4, 8], data=Bt), 2, b"f32, f16 or bf16"),
     (_t([4, 8], data=A), 1.1, 64, _t([4, 8], data=Bt), 1, b"[0, 1]"),
     (_t([4, 8], data=A), float("nan"), 64, _t([4, 8], data=Bt), 1, b"[0, 1]"),
@@ -417,7 +418,7 @@ def _boundary(lib, x=None, y="y", w="w", wp=None, g=None, p=0.0, seed=None, xo="
 @pytest.mark.parametrize("kw,rc,text", [
     (dict(y=_t([4, 7], data=Bt)), 1, b"y is"), (dict(y=_t([4, 8], dtype=F32, data=Bt)), 2, b"dtype"),
     (dict(y=None), 1, b"go with y"), (dict(y=None, xo=None, g=_t([8], data=Ct)), 1, b"go with y"),
-    (dict(h=None), 1, b"go together"), (dict(w=None), 1, b"go together"), (dict(w=None, h=None, xo=None), 1, b"nothing to compute"),
+    (dict(x=_t([-1, 8], data=A)), 1, b"negative size"), (dict(h=None), 1, b"go together"), (dict(w=None), 1, b"go together"), (dict(w=None, h=None, xo=None), 1, b"nothing to compute"),
     (dict(w=_t([7], data=Ct)), 1, b"weight must be"), (dict(wp=_t([8], strides=[2], data=Ct)), 1, b"unit stride"),
     (dict(g=_t([8], dtype=F32, data=Ct)), 2, b"gate"), (dict(p=0.5), 1, b"seed"),
     (dict(xo=_t([4, 8], data=A + 2)), 1, b"overlap"), (dict(xo=_t([4, 8], data=Bt)), 1, b"overlap"), (dict(h=_t([4, 8], data=A)), 1, b"overlap"),
