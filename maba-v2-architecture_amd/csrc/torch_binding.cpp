@@ -62,16 +62,37 @@ int code_of(const Tensor& t) {
   }
 }
 
-// A tensor [..., C] as [rows, C] with unit column stride (a view where the strides allow it), or a vector.
+// A contiguous tensor as [rows, cols], or for cols = 0 as [rows].
+maba_tensor packed(const Tensor& t, int64_t rows, int64_t cols) {
+  maba_tensor d = {t.data_ptr(), code_of(t), cols ? 2 : 1, {rows, 1, 1, 1}, {cols ? cols : 1, 0, 0, 0}};
+  if (cols) {
+    d.shape[1] = cols;
+    d.stride[1] = 1;
+  }
+  return d;
+}
+
+// A tensor [..., C] as [rows, C] with unit column stride (a view where the strides allow it), a vector, or any as one (FLAT).
+enum Form { ROWS, VECTOR, FLAT };
 struct Desc {
   Tensor keep;
   maba_tensor d = {};
   bool there = false;
   Desc() = default;
-  explicit Desc(const Tensor& t, bool vector = false) {
+  explicit Desc(const Tensor& t, Form form = ROWS) {
     if (!t.defined()) return;
     keep = t;
-    if (vector) {
+    there = true;
+    if (form == FLAT) {
+      if (!keep.is_contiguous()) keep = keep.contiguous();
+      d = packed(keep, keep.numel(), 0);
+      return;
+    }
+    if (form == ROWS && t.dim() != 2 && t.dim() > 0 && t.is_contiguous() && t.size(-1) > 0) {        // the same rows without a view
+      d = packed(t, t.numel() / t.size(-1), t.size(-1));
+      return;
+    }
+    if (form == VECTOR) {
       if (!keep.is_contiguous()) keep = keep.contiguous();
     } else {
       if (keep.dim() != 2) keep = keep.reshape({-1, keep.size(-1)});
@@ -85,7 +106,6 @@ struct Desc {
       d.shape[i] = i < d.ndim ? keep.size(i) : 1;
       d.stride[i] = i < d.ndim ? keep.stride(i) : 0;
     }
-    there = true;
   }
   maba_tensor* operator&() { return there ? &d : nullptr; }
 };
@@ -148,7 +168,7 @@ Tensor gated_call(const Tensor& x, const Tensor& wg, const Tensor& wu) {
 
 Tensor linear_call(const Tensor& x, const Tensor& w, const Tensor& bias, int act, const Tensor& res, const Tensor& gate) {
   Scope scope(x);
-  Desc dx(x), dw(w), db(bias, true), dr(res), dg(gate, true);
+  Desc dx(x), dw(w), db(bias, VECTOR), dr(res), dg(gate, VECTOR);
   Tensor out = at::empty(outer(x, w.size(0)), x.options());
   Desc dout(out);
   void* s = stream_of(x);
@@ -266,12 +286,12 @@ struct LinearEpilogue : public torch::autograd::Function<LinearEpilogue> {
       Scope scope(w);
       // where x is not read, a view of its shape over one weight row takes its place
       const Tensor x = f >> 7 & 1 ? kept[at_++] : w.select(0, 0).expand(shape);
-      Desc ddy(dy), ix(x), is(f >> 8 & 1 ? kept[at_++] : Tensor()), iw(w), ib(bias, true), ig(gate, true);
+      Desc ddy(dy), ix(x), is(f >> 8 & 1 ? kept[at_++] : Tensor()), iw(w), ib(bias, VECTOR), ig(gate, VECTOR);
       if (need & 1) dx = at::empty(shape, w.options());
       if (need & 2) dw = at::empty(w.sizes(), w.options());
       if (need & 4) dbias = at::empty({w.size(0)}, w.options());
       if (need & 8) dgate = at::empty({w.size(0)}, w.options());
-      Desc odx(dx), odw(dw), odb(dbias, true), odg(dgate, true);
+      Desc odx(dx), odw(dw), odb(dbias, VECTOR), odg(dgate, VECTOR);
       Tensor ws = workspace(lib.linear_epilogue_backward_workspace_size(&ddy, &ix, &is, &iw, act, bias.defined(), gate.defined(),
                                                                         need), w);
       check_backward(lib.linear_epilogue_backward(&ddy, &ix, &is, &iw, &ib, act, &ig, &odx, &odw, &odb, &odg, ws.data_ptr(),
@@ -338,7 +358,7 @@ std::pair<Tensor, Tensor> boundary_call(const Tensor& x, const Tensor& y, const 
   Tensor xo, h;
   if (y.defined()) xo = at::empty(x.sizes(), x.options());
   if (w.defined()) h = at::empty(x.sizes(), x.options());
-  Desc dx(x), dy(y), dw(w, true), dp(wp, true), dg(g, true), dxo(xo), dh(h);
+  Desc dx(x), dy(y), dw(w, VECTOR), dp(wp, VECTOR), dg(g, VECTOR), dxo(xo), dh(h);
   take(lib.residual_norm(&dx, &dy, &dw, &dp, &dg, (float)b.scale, b.d.p, b.d.ptr(), b.d.stream, (float)b.eps, &dxo, &dh,
                          stream_of(x)));
   return {xo, h};
@@ -380,8 +400,8 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
       if (need & 4) dw = at::empty(w.sizes(), like.options());
       if (need & 8) dwp = at::empty(wp.sizes(), like.options());
       if (need & 16) dg = at::empty(g.sizes(), like.options());
-      Desc ddxo(dxo), ddh(dh), ix(x), iy(y), iw(w, true), ip(wp, true), ig(g, true);
-      Desc odx(dx), ody(dy), odw(dw, true), odp(dwp, true), odg(dg, true);
+      Desc ddxo(dxo), ddh(dh), ix(x), iy(y), iw(w, VECTOR), ip(wp, VECTOR), ig(g, VECTOR);
+      Desc odx(dx), ody(dy), odw(dw, VECTOR), odp(dwp, VECTOR), odg(dg, VECTOR);
       const int which = (need >> 2 & 1) | (need >> 4 & 1) << 1 | (need >> 3 & 1) << 2;
       Tensor ws;
       if (which) ws = workspace(lib.residual_norm_backward_workspace_size(&ix, which), like);
@@ -412,26 +432,26 @@ maba_tensor desc3(const Tensor& t) {
   }
   return d;
 }
-Tensor flat(const Tensor& t) { return t.defined() ? t.reshape({-1}) : t; }
 
 // logp, entropy, lse and, for top > 0, the alternatives' log probabilities and indexes.
 variable_list logprobs_call(const Tensor& logits, const Tensor& targets, double temperature, int64_t top) {
   Scope scope(logits);
-  const Tensor x = logit_rows(logits), t = flat(targets);
+  const Tensor x = logit_rows(logits);
   const auto lead = targets.sizes();
   const auto f32 = logits.options().dtype(at::kFloat);
   variable_list out = {at::empty(lead, f32), at::empty(lead, f32), at::empty(lead, f32)};
-  Tensor top_logp, top_ids;
   if (top) {
     auto shape = lead.vec();
     shape.push_back(top);
     out.push_back(at::empty(shape, f32));
     out.push_back(at::empty(shape, f32.dtype(at::kLong)));
-    top_logp = out[3].view({-1, top});
-    top_ids = out[4].view({-1, top});
   }
   maba_tensor dx = desc3(x);
-  Desc dt(t, true), dl(flat(out[0]), true), de(flat(out[1]), true), dz(flat(out[2]), true), dtl(top_logp), dti(top_ids);
+  Desc dt(targets, FLAT), dl(out[0], FLAT), de(out[1], FLAT), dz(out[2], FLAT), dtl, dti;
+  if (top) {
+    dtl = Desc(out[3]);
+    dti = Desc(out[4]);
+  }
   take(lib.token_logprobs(&dx, &dt, temperature, &dl, &de, &dz, &dtl, &dti, stream_of(x)));
   return out;
 }
@@ -453,8 +473,8 @@ struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
       const Tensor x = logit_rows(kept[0]);
       Tensor d = at::empty(x.sizes(), x.options());
       maba_tensor dx = desc3(x), out = desc3(d);
-      Desc g0(flat(grads[0]), true), g1(flat(grads[1]), true), g2(flat(grads[2]), true);
-      Desc t(flat(kept[1]), true), z(flat(kept[2]), true), h(flat(kept[3]), true);
+      Desc g0(grads[0], FLAT), g1(grads[1], FLAT), g2(grads[2], FLAT);
+      Desc t(kept[1], FLAT), z(kept[2], FLAT), h(kept[3], FLAT);
       check_backward(lib.token_logprobs_backward(&g0, &g1, &g2, &dx, &t, &z, &h, ctx->saved_data["temperature"].toDouble(), &out,
                                                  stream_of(x)),
                      "token_logprobs_backward");
