@@ -535,13 +535,14 @@ static int back_elems(int64_t R, int64_t C, int dtype) {
   return dtype != MABA_F32 && R >= 16384 && lanes == 128 && chunks * 4 <= lanes * 3 ? MOST_BACK : 8;
 }
 // A backward pass's threads a workgroup: the fewest until rows fill the chip (64 x 640 bf16 8.4 us, with 1,024 threads 10.6), then
-// as many as fill a compute unit by themselves.
-static int back_size(int64_t R, const Geometry& geo) {
-  const int most = back_threads(geo.nch);
+// as many as fill a compute unit by themselves; half of them where rows end inside a chunk, whose accesses keep the waves
+// apart, and a row does not need them all (24,576 x 1,345 bf16 117 us and 128, 24,576 x 1,001 71 and 76; 8,191 x 4,095 113 and 106).
+static int back_size(int64_t R, const Geometry& geo, bool cut) {
+  const int most = cut && geo.lg < MAX_LG ? std::min(back_threads(geo.nch), 512) : back_threads(geo.nch);
   return R >= (int64_t)device_cu_count() * (most >> geo.lg) ? most : std::max(256, 1 << geo.lg);
 }
-static int back_groups(int64_t R, const Geometry& geo) {
-  const int threads = back_size(R, geo);
+static int back_groups(int64_t R, const Geometry& geo, bool cut) {
+  const int threads = back_size(R, geo, cut);
   return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(R, threads >> geo.lg), (int64_t)device_cu_count() * (back_threads(geo.nch) / threads)));
 }
 template <int N>
@@ -640,7 +641,7 @@ extern "C" size_t maba_hip_residual_norm_backward_workspace_size(const maba_tens
   const int64_t R = x->shape[0], C = x->shape[1];
   int groups = 0;
   for (const bool far : {false, true})               // which of them the call takes depends on all its tensors' strides
-    groups = std::max(groups, back_groups(R, row_geometry(C, chunk_elems(x->dtype), back_elems(R, C, x->dtype), far)));
+    groups = std::max(groups, back_groups(R, row_geometry(C, chunk_elems(x->dtype), back_elems(R, C, x->dtype), far), cut_rows(C, x->dtype)));
   return (size_t)groups * __builtin_popcount(grads & 7) * C * sizeof(float);
 }
 
@@ -684,7 +685,7 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
   const Geometry geo = row_geometry(C, chunk_elems(dt), back_elems(R, C, dt), far_rows({dx_out, dh, x, y, dx, dy}));
   const int grads = (dweight ? GRAD_W : 0) | (dgate ? GRAD_GATE : 0) | (dpost_weight ? GRAD_POST : 0);
   if (!grads && !dx && !dy) return MABA_OK;
-  const int groups = back_groups(R, geo), n = __builtin_popcount(grads);
+  const int groups = back_groups(R, geo, cut_rows(C, dt)), n = __builtin_popcount(grads);
   rc = ffn::check_workspace(who, workspace, workspace_bytes, (size_t)groups * n * C * sizeof(float));
   if (rc) return rc;
   const bool need_y = y && (dh || post_weight || dgate);
@@ -695,7 +696,7 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
                         dx ? dx->stride[0] : 0, dy ? dy->stride[0] : 0, R, (int)C, geo.lg, grads, cut_rows(C, dt), scale, eps,
                         make_drop(p, seed, stream_id)};
   if (R > 0) {
-    const int threads = back_size(R, geo);
+    const int threads = back_size(R, geo, cut_rows(C, dt));
     const size_t params = (size_t)(post_weight ? 3 : 2) * ceil_div(C, chunk_elems(dt)) * 16;
     const size_t lds = std::max(params, grads ? (size_t)(post_weight ? 3 : 2) * threads * chunk_elems(dt) * sizeof(float) : 0);
     const bool whole = whole_rows({dx_out, dh, x, y, dx, dy});
