@@ -319,11 +319,14 @@ def _decode_linear_fits(model: "MabaSparseForCausalLM") -> bool:
     """Whether every linear layer of a serving step fits the HIP decode linear: bf16 weights
     (and embedding table), no bias (the MABA-SA stream gate's is added after the stacked
     projection), input widths a multiple of 32, at most 2048 where the input is normalised and
-    4096 elsewhere; bf16 norm weights and residual gates; a vocabulary of whole 8-wide vectors
-    for the argmax."""
+    4096 elsewhere; bf16 norm weights and residual gates; boundaries without a norm on a half's
+    output and without a residual scale, which its input stage does not have; a vocabulary of
+    whole 8-wide vectors for the argmax."""
     normed, plain = [model.head_proj], [model.embeddings.in_emb, model.embeddings.proj, model.lm_head]
     if model.config.vocab_size % 8:
         return False                                       # the argmax kernel's row vectors
+    if any(layer.extended for layer in model.layers):
+        return False
     for layer in model.layers:
         mx = layer.mixer
         normed += [layer.ffn.w_gate, layer.ffn.w_up]

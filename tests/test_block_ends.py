@@ -601,6 +601,15 @@ def test_generation_with_post_norms_equals_state_passing():
     assert torch.equal(got, torch.cat(ref, dim=1))
 
 
+@pytest.mark.parametrize("kw,fits", [({}, True), (dict(fused_boundary=True), True), (dict(dropout=0.1), True), (dict(post_norm=True), False),
+                                     (dict(residual_scale=0.5), False)])
+def test_the_decode_linears_of_a_serving_step_take_plain_boundaries_only(kw, fits):
+    """Their input stage has no norm on a half's output and no scale: a step over them would leave both out."""
+    from maba_sparse.model import _decode_linear_fits
+    m = MabaSparseForCausalLM(get_101m_config(n_layers=4, vocab_size=1024, top_k=4, **kw)).bfloat16()
+    assert _decode_linear_fits(m) == fits
+
+
 def test_generation_drops_nothing():
     m, ids = _model(dropout=0.5), _ids(100)
     seed = m.dropout_seed.clone()

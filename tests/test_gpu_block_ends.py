@@ -595,6 +595,23 @@ def test_the_models_boundaries_and_score(post):
         assert (seen[:, :1] - seen2[:, :1]).abs().max() == 0
 
 
+@pytest.mark.parametrize("kw", [dict(post_norm=True), dict(residual_scale=0.5), dict(post_norm=True, residual_scale=0.7)])
+def test_captured_decoding_of_extended_blocks_equals_state_passing(kw):
+    """Every step's logits, each path given the same tokens.  They differ by bf16 roundings: some ten a block and three of
+    the head, each 2^-9 / sqrt(3) of its values, in four blocks 0.007 of the logits' norm."""
+    from maba_sparse.model import MabaSparseForCausalLM, get_101m_config
+    torch.manual_seed(1)
+    m = MabaSparseForCausalLM(get_101m_config(n_layers=4, vocab_size=1024, top_k=4, **kw)).init_normal(0.05).to(DEV, BF).eval()
+    ids = torch.randint(0, 1024, (2, 300), generator=torch.Generator().manual_seed(2)).to(DEV)
+    with torch.no_grad():
+        toks, seen = m.generate_greedy(ids, 5, return_logits=True, graph=True)
+        states = m(ids)[1]
+        for i in range(4):
+            want, states = m.step(toks[:, i:i + 1], past_states=states)
+            a, b = seen[:, i + 1].float(), want[:, -1].float()
+            assert (a - b).norm() / b.norm() < 0.02, (i, (a - b).norm() / b.norm())
+
+
 # ----------------------------------------------------------------------------- calls
 
 
