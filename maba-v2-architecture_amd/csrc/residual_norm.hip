@@ -503,10 +503,10 @@ static bool same_place(const maba_tensor* a, const maba_tensor* b) {
   return a->data == b->data && (a->shape[0] <= 1 || a->stride[0] == b->stride[0]);
 }
 
-// Whether four rows of one of the tensors are further apart than 32 bits of bytes tell.
+static int64_t row_stride(const maba_tensor* t) { return t ? walked(t->shape[0], t->stride[0]) : 0; }
 static bool far_rows(std::initializer_list<const maba_tensor*> all) {
   for (const maba_tensor* t : all)
-    if (t && t->shape[0] > 1 && t->stride[0] > (int64_t)1 << 27) return true;
+    if (t && far_apart(t->shape[0], t->stride[0])) return true;
   return false;
 }
 // Whether the rows of all of them are whole 16-byte chunks.
@@ -581,7 +581,7 @@ extern "C" int maba_hip_dropout(const maba_tensor* x, double p, const int64_t* s
   if (!rc) rc = check_out(out, who, "out", x->dtype, x->shape[0], x->shape[1]);
   if (rc) return rc;
   if (overlap(x, out) && !same_place(x, out)) return fail(MABA_ERR_INVALID, "%s: x and out overlap", who);
-  DropArgs a = {x->data, out->data, x->stride[0], out->stride[0], x->shape[0], (int)x->shape[1], 0, make_drop(p, seed, stream_id)};
+  DropArgs a = {x->data, out->data, row_stride(x), row_stride(out), x->shape[0], (int)x->shape[1], 0, make_drop(p, seed, stream_id)};
   if (a.R == 0) return MABA_OK;
   const int64_t chunks = ceil_div(a.C, chunk_elems(x->dtype));
   while (a.lg < 8 && chunks > (int64_t)4 << a.lg) ++a.lg;
@@ -619,8 +619,8 @@ extern "C" int maba_hip_residual_norm(const maba_tensor* x, const maba_tensor* y
   const Geometry geo = row_geometry(C, chunk_elems(dt), forward_elems(R, C, dt), far_rows({x, y, x_out, h}));
   BoundaryArgs a = {x->data, y ? y->data : nullptr, weight ? weight->data : nullptr, post_weight ? post_weight->data : nullptr,
                     gate ? gate->data : nullptr, x_out ? x_out->data : nullptr, h ? h->data : nullptr,
-                    x->stride[0], y ? y->stride[0] : 0, x_out ? x_out->stride[0] : 0, h ? h->stride[0] : 0, R, (int)C, geo.lg,
-                    scale, eps, make_drop(p, seed, stream_id)};
+                    row_stride(x), row_stride(y), row_stride(x_out), row_stride(h), R, (int)C, geo.lg, scale, eps,
+                    make_drop(p, seed, stream_id)};
   if (R == 0) return MABA_OK;
   const int threads = std::max(256, 1 << geo.lg);
   const dim3 grid((unsigned)std::min<int64_t>(ceil_div(R, threads >> geo.lg), (int64_t)device_cu_count() * 8));
@@ -692,9 +692,8 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
   BoundaryBackArgs a = {dx_out ? dx_out->data : nullptr, dh ? dh->data : nullptr, x->data, need_y ? y->data : nullptr,
                         weight ? weight->data : nullptr, post_weight ? post_weight->data : nullptr, gate ? gate->data : nullptr,
                         dx ? dx->data : nullptr, dy ? dy->data : nullptr, (float*)workspace,
-                        dx_out ? dx_out->stride[0] : 0, dh ? dh->stride[0] : 0, x->stride[0], y ? y->stride[0] : 0,
-                        dx ? dx->stride[0] : 0, dy ? dy->stride[0] : 0, R, (int)C, geo.lg, grads, cut_rows(C, dt), scale, eps,
-                        make_drop(p, seed, stream_id)};
+                        row_stride(dx_out), row_stride(dh), row_stride(x), row_stride(y), row_stride(dx), row_stride(dy), R, (int)C,
+                        geo.lg, grads, cut_rows(C, dt), scale, eps, make_drop(p, seed, stream_id)};
   if (R > 0) {
     const int threads = back_size(R, geo, cut_rows(C, dt));
     const size_t params = (size_t)(post_weight ? 3 : 2) * ceil_div(C, chunk_elems(dt)) * 16;

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "ffn_common.h"
+#include "row_lanes.h"
 
 namespace maba {
 namespace rowvec {
@@ -115,7 +116,7 @@ struct Walk {
   int64_t stride;          // bytes
   uint32_t row_off, off;
   __device__ __forceinline__ Walk(const void* q, int64_t ld, int l, int sub)
-      : p((char*)q), stride(ld * (int64_t)sizeof(typename Traits<T>::elem)), row_off((uint32_t)(sub * stride)), off(row_off + 16 * l) {}
+      : p((char*)q), stride(ld * (int64_t)sizeof(typename Traits<T>::elem)), row_off(lane_row(sub, stride)), off(row_off + 16 * l) {}
   __device__ __forceinline__ char* at(int64_t row, int chunk) const { return p + row * stride + 16 * (int64_t)chunk; }
 };
 // A lane's chunks l, l + 2^lg, ... of rows that end inside a chunk, for ended().
@@ -138,17 +139,16 @@ struct CutRows {
 
 // The same rows where every row is whole chunks, 16-byte aligned: accesses through a buffer descriptor, which drops those of
 // lanes without a chunk or a row, and all of a missing tensor's (whose chunks are zeros), without a branch.
-constexpr uint32_t NOWHERE = 0x80000000u;          // past every descriptor's end
 template <class T>
 struct WholeWalk : Walk<T> {
   uint32_t bytes;
-  __device__ __forceinline__ WholeWalk(const void* q, int64_t ld, int l, int sub) : Walk<T>(q, ld, l, sub), bytes(q ? 0x7fffffffu : 0u) {}
+  __device__ __forceinline__ WholeWalk(const void* q, int64_t ld, int l, int sub) : Walk<T>(q, ld, l, sub), bytes(q ? DESCRIPTOR_END : 0u) {}
   __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows(int64_t row) const { return ffn::rsrc(this->p + row * this->stride, bytes); }
   __device__ __forceinline__ u32x4 load(__amdgpu_buffer_rsrc_t r, uint32_t chunk) const {
-    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(this->off + chunk), 0, 0));
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)lane_access(this->off, chunk), 0, 0));
   }
   __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t r, uint32_t chunk, u32x4 u) const {
-    __builtin_amdgcn_raw_buffer_store_b128(u, r, (int)(this->off + chunk), 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(u, r, (int)lane_access(this->off, chunk), 0, 0);
   }
 };
 

@@ -287,6 +287,29 @@ def test_offsets_past_32_bits():
     assert all(torch.equal(a[0], b) for a, b in zip(got, flat))
 
 
+@pytest.mark.parametrize("stride", [2 ** 27 + 8, 400_000_000, 2 ** 28, 2 ** 30, 2 ** 31])
+@pytest.mark.parametrize("dt", [BF, FL])
+@pytest.mark.parametrize("Cw", [16, 64, 120, 33, 640])
+def test_a_single_row_has_no_stride(Cw, dt, stride):
+    """What a dimension of one element has for a stride is never walked by."""
+    t = _tensors(1, Cw, dt, PARTS[-1], seed=14)
+    d, dh = t["y"].clone(), t["x"].clone()
+    kw = dict(weight=t["weight"], post_weight=t["post_weight"], gate=t["gate"], p=0.2, seed=_seed())
+    far = lambda v: v.as_strided((1, Cw), (stride, 1))
+    for a, b in zip(D.residual_norm(far(t["x"]), far(t["y"]), **kw), D.residual_norm(t["x"], t["y"], **kw)):
+        assert torch.equal(a, b)
+    want = D.residual_norm_backward(d, dh, t["x"], t["y"], **kw)
+    for a, b in zip(D.residual_norm_backward(far(d), far(dh), far(t["x"]), far(t["y"]), **kw), want):
+        assert torch.equal(a, b)
+    outs = [torch.full_like(v, math.nan) for v in want]
+    ws = torch.empty(N.load().maba_hip_residual_norm_backward_workspace_size(N.rows_desc(t["x"]), 7), dtype=torch.uint8, device=DEV)
+    seed, ins = _seed(), [N.rows_desc(v) for v in (far(d), far(dh), far(t["x"]), far(t["y"]), t["weight"], t["post_weight"], t["gate"])]
+    N.check(N.load().maba_hip_residual_norm_backward(*ins, 1.0, 0.2, seed.data_ptr(), 0, 1e-6, N.rows_desc(far(outs[0])),
+                                                     N.rows_desc(far(outs[1])), *map(N.rows_desc, outs[2:]), ws.data_ptr(), ws.numel(),
+                                                     N.stream_ptr(d.device)), "residual_norm_backward")
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("Cw", [1000, 4096, 4095])
 def test_post_norm_backward_has_the_same_bits_on_every_call(dt, Cw):

@@ -61,3 +61,40 @@ def test_layer_rows(rows, L, stride):
                     assert got % step == first and got // step <= left
                 else:
                     assert got == min(r, left) * step + first
+
+
+@pytest.fixture(scope="module")
+def lanes(tmp_path_factory):
+    d = tmp_path_factory.mktemp("lanes")
+    src = d / "lanes.cpp"
+    src.write_text('#include "row_lanes.h"\n'
+                   'using namespace maba::rowvec;\n'
+                   'extern "C" bool far(int64_t rows, int64_t stride) { return far_apart(rows, stride); }\n'
+                   'extern "C" uint32_t at(int64_t rows, int64_t stride, int es, int sub, uint32_t chunk, bool live) {\n'
+                   '  return lane_access(lane_row(sub, walked(rows, stride) * es), chunk | (live ? 0u : NOWHERE));\n'
+                   '}\n'
+                   'extern "C" uint32_t end() { return DESCRIPTOR_END; }\n')
+    so = d / "lanes.so"
+    subprocess.run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-I", CSRC, "-o", str(so), str(src)], check=True)
+    lib = ctypes.CDLL(str(so))
+    lib.far.argtypes, lib.far.restype = [ctypes.c_int64] * 2, ctypes.c_bool
+    lib.at.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_uint32, ctypes.c_bool]
+    lib.at.restype = lib.end.restype = ctypes.c_uint32
+    return lib
+
+
+@pytest.mark.parametrize("es", [2, 4])
+@pytest.mark.parametrize("stride", [0, 64, 2 ** 26, 2 ** 27, 2 ** 27 + 1, 2 ** 28, 357913942, 400_000_000, 2 ** 29, 2 ** 30, 2 ** 31, 2 ** 40 + 8,
+                                    2 ** 62 // 4])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 1000])
+def test_rows_that_share_a_wave(lanes, rows, stride, es):
+    """A lane's access behind the row of its wave's first lane: inside the row that the lane has, and past the descriptor's end
+    where it has none, also for the stride that a single row may come with."""
+    if lanes.far(rows, stride):
+        assert rows > 1 and 3 * stride * 4 > lanes.end() // 2   # whatever the type
+        return                                    # such rows have a wave each
+    for sub in range(4):
+        for chunk in (0, 16, 1008, 16 * 512 * 3):
+            if sub < rows:
+                assert lanes.at(rows, stride, es, sub, chunk, True) == sub * stride * es + chunk < lanes.end()
+            assert lanes.at(rows, stride, es, sub, chunk, False) >= lanes.end()
