@@ -1,7 +1,7 @@
 // Log probabilities of given tokens, the entropy of their distributions and the likeliest alternatives, from logits
 // [rows, V], and the gradient of the first two and of the normaliser.  With u = l / T:
 //   lse = log sum exp(u),  logp = u[t] - lse,  H = lse - sum p u,  p = exp(u - lse)
-//   dl  = 1/T (dlogp (delta_t - p) + dlse p - dH p (log p + H))
+//   dl  = 1/T (dlogp (delta_t - p) + dlse p - dH p (log p + H)),  and for the target 1 - p = the sum of the others' p
 //
 // Forward is one pass with a running reference: a thread holds (R, S, D) = (R, sum 2^x, sum x 2^x), x = l c - R, c = log2(e) / T,
 // with R the largest l c so far rounded up to a whole number, so that l c - R is one fused operation without a rounding of R
@@ -389,15 +389,15 @@ __global__ __launch_bounds__(256) void logprobs_back_kernel(BackwardArgs a) {
   // row is summed again and log p counted from its largest element.  All of that ends before anything of the row is
   // written, which may be the logits' own.  (1,024 x 32,768 bf16 24 us without such rows, 63 with nothing else.)
   constexpr float EXACT = T::CODE == MABA_F32 ? 32.f : 256.f;
-  __shared__ float part[2][4];
+  __shared__ float part[3][4];
+  const int l = threadIdx.x & ((1 << a.lg) - 1);
+  const auto of_row = [&](float v, float* shared, auto f) { return a.lg == 8 ? across<4>(v, shared, f) : wave_joined(v, f); };
   float m = 0.f;
   if (lse == -INFINITY) {            // no mass: no element has a gradient
     lse = -LOWEST;
     gl = gh = gz = 0.f;              // whatever comes from a loss of lse = -inf
   } else if (fabsf(lse) > EXACT) {
     m = -INFINITY;
-    const int l = threadIdx.x & ((1 << a.lg) - 1);
-    const auto of_row = [&](float v, float* shared, auto f) { return a.lg == 8 ? across<4>(v, shared, f) : wave_joined(v, f); };
     for_chunks<T, 2>(row, a.V, l, 1 << a.lg, [&](auto& v, int) {
 #pragma unroll
       for (float x : v) m = fmaxf(m, x);
@@ -410,9 +410,31 @@ __global__ __launch_bounds__(256) void logprobs_back_kernel(BackwardArgs a) {
     });
     lse = __builtin_amdgcn_logf(of_row(s, part[1], sum_of)) * LN2;
   }
-  const float base = gz - gl - (gh != 0.f ? gh * h : 0.f), at_target = gl * a.inv;
-  const int lanes = a.parts << a.lg, lane = ((int)(blockIdx.x % a.parts) << a.lg) + (threadIdx.x & ((1 << a.lg) - 1));
+  const int lanes = a.parts << a.lg, lane = ((int)(blockIdx.x % a.parts) << a.lg) + l;
   const int mine = target >= 0 && target < a.V ? (int)(target / E) : -1, chunks = (a.V + E - 1) / E;
+  // The target's element has dlogp (1 - p).  Of a likely target 1 - p is little more than lse's rounding: below `sure`, where
+  // that is more than an eighth of a 16-bit result's half step (32 of an fp32 one's), it is the sum of the others' p
+  // instead, made by the workgroup that has the element, before the row is written.  Only a row of little entropy can hold
+  // such a target.  (8,192 x 32,768 bf16 194 us without such targets, 231 with nothing else.)
+  constexpr float SHARE = T::CODE == MABA_F32 ? 32.f : T::CODE == MABA_BF16 ? 2048.f : 256.f;
+  const float sure = fminf((fabsf(lse) + 4.f) / SHARE, 0.5f);
+  float rest = -1.f;
+  if (mine >= 0 && gl != 0.f && h < sure * (2.f + __logf((float)a.V / sure))) {
+    const float at = element<T>(row, (uint32_t)target);
+    if (a.lg == 8) __syncthreads();  // all waves have it before one of them writes the row
+    if (-expm1f(fmaf(at - m, a.inv, -lse)) < sure && mine % lanes >> a.lg == (int)(blockIdx.x % a.parts)) {
+      float s = 0.f;
+      for_chunks<T, 2>(row, a.V, l, 1 << a.lg, [&](auto& v, int first) {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(v) / sizeof(float)); ++i) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(v[i] - m, a.inv, -lse) * LOG2E);
+          s += first + (i / E << a.lg) * E + i % E == (int)target ? 0.f : p;
+        }
+      });
+      rest = of_row(s, part[2], sum_of);
+    }
+  }
+  const float base = gz - gl - (gh != 0.f ? gh * h : 0.f), at_target = gl * a.inv;
   for (int c0 = lane; c0 < chunks; c0 += lanes * NB) {
     u32x4 u[NB];
 #pragma unroll
@@ -428,9 +450,11 @@ __global__ __launch_bounds__(256) void logprobs_back_kernel(BackwardArgs a) {
         // where p is zero log p may be -inf: bounded, its product with p is zero
         v[e] = a.inv * p * fmaf(-gh, fmaxf(lp, -1e4f), base);
       }
-      if (ch == mine)
+      if (ch == mine) {
+        const float own = a.inv * fmaf(gl, rest, (1.f - rest) * (gz - (gh != 0.f ? gh * (log1pf(-rest) + h) : 0.f)));
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] += e == (int)(target % E) ? at_target : 0.f;
+        for (int e = 0; e < E; ++e) v[e] = e != (int)(target % E) ? v[e] : rest < 0.f ? v[e] + at_target : own;
+      }
       store_chunk<T>(out, (uint32_t)ch * 16u, a.V - ch * E, pack<T>(v));
     }
   }

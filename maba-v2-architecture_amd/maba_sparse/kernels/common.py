@@ -687,6 +687,8 @@ def ref_token_logprobs_backward(dlogp, dentropy, dlse, logits, targets, lse, ent
     lp = torch.where(none, torch.full((), -math.inf, dtype=x.dtype, device=x.device), z - torch.log(torch.exp(z).sum(-1, keepdim=True)))
     p = torch.exp(lp)
     plogp = torch.where(p == 0, p, p * lp)
-    d = (gz - gl) * p - gh * (plogp + p * entropy.unsqueeze(-1))
-    d = d + torch.where(torch.arange(x.shape[-1], device=x.device) == t, gl, zero)
+    hit = torch.arange(x.shape[-1], device=x.device) == t
+    rest = torch.where(hit, zero, p).sum(-1, keepdim=True)    # 1 - p of a likely target, which the difference would lose
+    d = gz * p - gh * (plogp + p * entropy.unsqueeze(-1))
+    d = d + torch.where(hit, gl * torch.where(p > 0.5, rest, 1 - p), -gl * p)
     return (inv * d).to(logits.dtype)

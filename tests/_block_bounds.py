@@ -237,3 +237,23 @@ def logprobs_backward(gl, gh, gz, x, t, T=1.0):
     # beside it, log p of no more than 88 among them, by that many times
     e = e + 2.0 ** -126 * (gz.abs() + gl.abs() + gh.abs() * (H.abs() + 88)) / T
     return d, rounded(d, e, x.dtype)
+
+
+def likely_rows(V, lse, below, dtype, seed=0):
+    """Rows of one likely token, the target, of logit ``lse``, the others ``below`` to ``below + 8`` below it: whole numbers, exact in
+    every type; and the gradients of -logp at the targets in 64 bits with their bounds.
+
+    They are the targets' 1 - p, which is the sum of the others' p: relative to itself it is off by what each p is, and that
+    by the forward's lse (its sum's terms, (V / 64 + 74 + 30 + 4 |u|) u, and 4 u |lse|), by log p's three roundings, and by
+    4 u for the exponential, then by its own sum and the products behind it."""
+    g = torch.Generator().manual_seed(seed + V)
+    x = lse - below - torch.randint(0, 9, (5, V), generator=g).double()
+    t = torch.tensor([0, V - 1, V // 2, 1, V // 3])
+    x[torch.arange(5), t] = lse
+    assert torch.equal(x.to(dtype).double(), x)
+    p = torch.softmax(x, -1)
+    p[torch.arange(5), t] = 0
+    want = p.sum(-1)
+    rel = half_step(dtype) + 1.05 * U * (2 * (V / 64 + 74) + 40 + 8 * abs(lse) + 3 * (below + 8))
+    f = torch.finfo(dtype)
+    return x.to(dtype), t, want, rel * want + f.tiny * f.eps / 2

@@ -191,6 +191,18 @@ def test_logprobs_and_their_backward_op(V, dtype):
     B.check(D.token_logprobs_backward(*g, x, t, lse, H, 0.8), B.logprobs_backward(*g, x, t, 0.8), "dlogits")
 
 
+@pytest.mark.parametrize("dt", [torch.float32, BF, HF])
+@pytest.mark.parametrize("V,below", [(3, 9), (700, 12), (700, 17)])
+@pytest.mark.parametrize("lse", [-200, 0, 30, 120, 240])
+def test_gradient_of_a_likely_target_is_the_others_sum(V, below, lse, dt):
+    """1 - p from a p near 1, or from an lse far from zero, would keep few of its bits or none."""
+    x, t, want, bound = B.likely_rows(V, lse, below, dt)
+    x.requires_grad_()
+    d, = torch.autograd.grad(-D.token_logprobs(x, t)[0].sum(), x)
+    got = -d.double().gather(1, t[:, None])[:, 0]
+    assert ((got - want).abs() <= bound).all(), (got, want)
+
+
 def test_rows_without_mass_have_no_gradient_whatever_comes_in():
     """A loss of lse^2 under torch.where sends NaN into such a row."""
     x, t = _logits(12, 300, torch.float32, seed=9)

@@ -492,6 +492,24 @@ def test_logits_gradient_in_place_of_rows_far_from_zero(M, V):
     assert torch.equal(x, want)
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("V,below", [(3, 9), (64, 10), (700, 12), (700, 17), (9001, 14), (40000, 15), (40000, 19)])
+@pytest.mark.parametrize("lse", [-200, 0, 30, 120, 240])
+def test_gradient_of_a_likely_target_is_the_others_sum(V, below, lse, dt):
+    """1 - p from a p near 1, or from an lse far from zero, would keep few of its bits or none."""
+    x, t, want, bound = B.likely_rows(V, lse, below, dt)
+    x, t = x.to(DEV).requires_grad_(), t.to(DEV)
+    logp, ent, z, _, _ = D.token_logprobs(x, t)
+    d, = torch.autograd.grad(-logp.sum(), x)
+    got = -d.double().gather(1, t[:, None])[:, 0].cpu()
+    assert ((got - want).abs() <= bound).all(), (got, want)
+    x, g = x.detach(), torch.full_like(logp, -1)
+    _check_logprobs(x, t, 1.0, 2)
+    N.check(N.load().maba_hip_token_logprobs_backward(N.rows_desc(g), None, None, N.desc(x), N.rows_desc(t), N.rows_desc(z.detach()),
+                                                      N.rows_desc(ent.detach()), 1.0, N.desc(x), N.stream_ptr(x.device)), "token_logprobs_backward")
+    assert torch.equal(x, d)                                                   # over the logits
+
+
 def test_rows_without_mass_have_no_gradient_whatever_comes_in():
     """A loss of lse^2 under torch.where sends NaN into such a row."""
     x, t = _logits(12, 300, FL, seed=9)
