@@ -412,14 +412,14 @@ __global__ __launch_bounds__(256) void logprobs_back_kernel(BackwardArgs a) {
   }
   const int lanes = a.parts << a.lg, lane = ((int)(blockIdx.x % a.parts) << a.lg) + l;
   const int mine = target >= 0 && target < a.V ? (int)(target / E) : -1, chunks = (a.V + E - 1) / E;
-  // The target's element has dlogp (1 - p).  Of a likely target 1 - p is little more than lse's rounding: below `sure`, where
-  // that is more than an eighth of a 16-bit result's half step (32 of an fp32 one's), it is the sum of the others' p
-  // instead, made by the workgroup that has the element, before the row is written.  Only a row of little entropy can hold
-  // such a target.  (8,192 x 32,768 bf16 194 us without such targets, 231 with nothing else.)
+  // The target's element has dlogp (1 - p) and dH p (log p + H).  Of a likely target 1 - p and log p are little more than lse's
+  // rounding: below `sure`, where that is more than an eighth of a 16-bit result's half step (32 of an fp32 one's), 1 - p is
+  // the sum of the others' p instead, made by the workgroup that has the element, before the row is written.  Only a row of
+  // little entropy can hold such a target.  (8,192 x 32,768 bf16 194 us without such targets, 231 with nothing else.)
   constexpr float SHARE = T::CODE == MABA_F32 ? 32.f : T::CODE == MABA_BF16 ? 2048.f : 256.f;
   const float sure = fminf((fabsf(lse) + 4.f) / SHARE, 0.5f);
   float rest = -1.f;
-  if (mine >= 0 && gl != 0.f && h < sure * (2.f + __logf((float)a.V / sure))) {
+  if (mine >= 0 && (gl != 0.f || gh != 0.f) && h < sure * (2.f + __logf((float)a.V / sure))) {
     const float at = element<T>(row, (uint32_t)target);
     if (a.lg == 8) __syncthreads();  // all waves have it before one of them writes the row
     if (-expm1f(fmaf(at - m, a.inv, -lse)) < sure && mine % lanes >> a.lg == (int)(blockIdx.x % a.parts)) {

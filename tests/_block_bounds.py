@@ -241,19 +241,22 @@ def logprobs_backward(gl, gh, gz, x, t, T=1.0):
 
 def likely_rows(V, lse, below, dtype, seed=0):
     """Rows of one likely token, the target, of logit ``lse``, the others ``below`` to ``below + 8`` below it: whole numbers, exact in
-    every type; and the gradients of -logp at the targets in 64 bits with their bounds.
+    every type; and the gradients of -logp and of the entropy at the targets in 64 bits with their bounds.
 
     They are the targets' 1 - p, which is the sum of the others' p: relative to itself it is off by what each p is, and that
     by the forward's lse (its sum's terms, (V / 64 + 74 + 30 + 4 |u|) u, and 4 u |lse|), by log p's three roundings, and by
-    4 u for the exponential, then by its own sum and the products behind it."""
+    4 u for the exponential, then by its own sum and the products behind it.  The entropy's are -p (log p + H), log p being
+    log(1 - (1 - p)): as far off as 1 - p for log p, u for H, 3 u for their sum and its product."""
     g = torch.Generator().manual_seed(seed + V)
     x = lse - below - torch.randint(0, 9, (5, V), generator=g).double()
     t = torch.tensor([0, V - 1, V // 2, 1, V // 3])
     x[torch.arange(5), t] = lse
     assert torch.equal(x.to(dtype).double(), x)
     p = torch.softmax(x, -1)
+    H = -(p * torch.log(p)).sum(-1)
     p[torch.arange(5), t] = 0
-    want = p.sum(-1)
-    rel = half_step(dtype) + 1.05 * U * (2 * (V / 64 + 74) + 40 + 8 * abs(lse) + 3 * (below + 8))
-    f = torch.finfo(dtype)
-    return x.to(dtype), t, want, rel * want + f.tiny * f.eps / 2
+    rest = p.sum(-1)
+    rel = 1.05 * U * (2 * (V / 64 + 74) + 40 + 8 * abs(lse) + 3 * (below + 8))
+    lp = torch.log1p(-rest)
+    dH = -(1 - rest) * (lp + H)
+    return x.to(dtype), t, H, (rest, rounded(rest, rel * rest, dtype)), (dH, rounded(dH, rel * lp.abs() + U * H + 3 * U * dH.abs(), dtype))

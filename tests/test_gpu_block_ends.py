@@ -497,12 +497,13 @@ def test_logits_gradient_in_place_of_rows_far_from_zero(M, V):
 @pytest.mark.parametrize("lse", [-200, 0, 30, 120, 240])
 def test_gradient_of_a_likely_target_is_the_others_sum(V, below, lse, dt):
     """1 - p from a p near 1, or from an lse far from zero, would keep few of its bits or none."""
-    x, t, want, bound = B.likely_rows(V, lse, below, dt)
+    x, t, H, want, wantH = B.likely_rows(V, lse, below, dt)
     x, t = x.to(DEV).requires_grad_(), t.to(DEV)
     logp, ent, z, _, _ = D.token_logprobs(x, t)
     d, = torch.autograd.grad(-logp.sum(), x)
-    got = -d.double().gather(1, t[:, None])[:, 0].cpu()
-    assert ((got - want).abs() <= bound).all(), (got, want)
+    B.check(-d.gather(1, t[:, None])[:, 0].cpu(), want, "at the target")
+    dH = D.token_logprobs_backward(None, torch.ones_like(logp), None, x.detach(), t, z.detach(), H.float().to(DEV))
+    B.check(dH.gather(1, t[:, None])[:, 0].cpu(), wantH, "the entropy's")
     x, g = x.detach(), torch.full_like(logp, -1)
     _check_logprobs(x, t, 1.0, 2)
     N.check(N.load().maba_hip_token_logprobs_backward(N.rows_desc(g), None, None, N.desc(x), N.rows_desc(t), N.rows_desc(z.detach()),
