@@ -277,6 +277,7 @@ __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(Bounda
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       bits[i] = kept_bits<V>(a.d, key, r, (l + (i << lg)) * V);
+      if constexpr (!POST) u.y[i] = drop_packed<T>(u.y[i], a.d, bits[i]);      // all that y is used for is dropped with it
       if (a.dh) {
         float h[V], p[V];
         unpack<T>(u.x[i], xn[i]);
@@ -287,8 +288,8 @@ __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(Bounda
             unpack<T>(par[2 * chunks + pc[i]], p);
 #pragma unroll
             for (int e = 0; e < V; ++e) z[e] *= rp * p[e];
+            drop_by<V>(z, a.d, bits[i]);
           }
-          drop_by<V>(z, a.d, bits[i]);
           if (a.g) {
             unpack<T>(par[chunks + pc[i]], p);
 #pragma unroll
@@ -327,8 +328,7 @@ __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(Bounda
       }
       if (a.dx) put(wdx, i, d);
       if (a.dy || (a.grads & (GRAD_GATE | GRAD_POST))) {
-        // dropout(z) = m z with m in {0, 1 / (1 - p)}: both products with m follow from m dX (the factor is in scale)
-        drop_by<V>(d, a.d, bits[i]);
+        // dropout(z) = m z with m in {0, 1 / (1 - p)}, the factor being in scale; a dropped z is zero whatever it was, also for dgate
         float p[V], y[V];
         unpack<T>(u.y[i], y);
         if constexpr (POST) {
@@ -336,9 +336,15 @@ __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(Bounda
           for (int e = 0; e < V; ++e) y[e] *= rp;
           unpack<T>(par[2 * chunks + pc[i]], p);
         }
-        if (a.grads & GRAD_GATE)
+        if (a.grads & GRAD_GATE) {
+          float z[V];
 #pragma unroll
-          for (int e = 0; e < V; ++e) acc[1][i][e] = fmaf(d[e], POST ? y[e] * p[e] : y[e], acc[1][i][e]);
+          for (int e = 0; e < V; ++e) z[e] = POST ? y[e] * p[e] : y[e];
+          if constexpr (POST) drop_by<V>(z, a.d, bits[i]);
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[1][i][e] = fmaf(d[e], z[e], acc[1][i][e]);
+        }
+        drop_by<V>(d, a.d, bits[i]);
 #pragma unroll
         for (int e = 0; e < V; ++e) d[e] *= scale;
         if (a.g) {

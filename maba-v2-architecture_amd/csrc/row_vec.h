@@ -288,6 +288,21 @@ __device__ __forceinline__ void drop_by(float (&v)[V], const Drop& d, uint32_t b
 #pragma unroll
   for (int e = 0; e < V; ++e) v[e] = __uint_as_float(__float_as_uint(v[e]) & (uint32_t)__builtin_amdgcn_sbfe((int)bits, e, 1));
 }
+// A packed chunk by such bits.
+template <class T>
+__device__ __forceinline__ u32x4 drop_packed(u32x4 u, const Drop& d, uint32_t bits) {
+  if (d.mode == 0) return u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (Traits<T>::VEC == 4) {
+      u[i] &= (uint32_t)__builtin_amdgcn_sbfe((int)bits, i, 1);
+    } else {
+      const uint32_t lo = (uint32_t)__builtin_amdgcn_sbfe((int)bits, 2 * i, 1), hi = (uint32_t)__builtin_amdgcn_sbfe((int)bits, 2 * i + 1, 1);
+      u[i] &= (lo & 0xffffu) | (hi & 0xffff0000u);
+    }
+  }
+  return u;
+}
 // v where it is kept, times 1 / (1 - p); zero, whatever v is, where it is dropped.  `at` is a multiple of four.
 template <int V>
 __device__ __forceinline__ void drop_chunk(float (&v)[V], const Drop& d, uint64_t key, int64_t row, int at) {

@@ -634,10 +634,9 @@ def ref_residual_norm_backward(dx_out, dh, x, y=None, weight=None, post_weight=N
         d = d + r * (gw - xh * (gw * xh).mean(-1, keepdim=True))
     elif weight is not None:
         dw = torch.zeros(shape[-1], dtype=d.dtype, device=d.device)
-    m = _dropped(d, p, seed, stream)                          # the product of the mask and either side
-    if gate is not None and needs[4]:
-        dg = scale * (m * (yf * rp * _one(post_weight, d))).sum(0)
-    dz = scale * (_one(gate, d) * m)
+    if gate is not None and needs[4]:                         # a dropped z is zero whatever it was
+        dg = scale * (d * _dropped(yf * rp * _one(post_weight, d), p, seed, stream)).sum(0)
+    dz = scale * (_one(gate, d) * _dropped(d, p, seed, stream))
     if post_weight is not None:
         yh, wp = yf * rp, post_weight.to(d.dtype)
         dpw = (dz * yh).sum(0)

@@ -136,6 +136,26 @@ def test_boundary_needs_and_missing_gradients():
             assert (a is None) if not n else torch.equal(a, b)
 
 
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_dropped_elements_have_no_part_in_the_gates_gradient(bad, post):
+    """As in the forward's own derivative, where a dropped element is zero whatever it was.  (Its own norm makes a row of one
+    infinite element zero elsewhere, and a row of one NaN nothing but NaN.)"""
+    if post and math.isnan(bad):
+        return
+    t = {k: v.detach() for k, v in _tensors().items()}
+    kw = dict(post_weight=t["post_weight"] if post else None, scale=0.7, p=0.4, seed=SEED)
+    keep, y = B.kept(t["x"], 0.4, SEED), t["y"].clone()
+    for r in (1, 4):
+        y[r, int((~keep[r]).nonzero()[0])] = bad
+    gate = t["gate"].requires_grad_()
+    xo, h = C.ref_residual_norm(t["x"], y, t["weight"], gate=gate, **kw)
+    want, = torch.autograd.grad((xo * t["x"]).sum() + (h * t["y"]).sum(), gate)
+    got = D.residual_norm_backward(t["x"], t["y"], t["x"], y, t["weight"], gate=gate.detach(), **kw)[4]
+    assert want.isfinite().all()
+    torch.testing.assert_close(got, want)
+
+
 def test_boundary_is_torchs_modules():
     import torch.nn.functional as F
     t = {k: v.detach() for k, v in _tensors(5, 16).items()}

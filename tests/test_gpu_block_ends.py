@@ -88,6 +88,23 @@ def test_dropped_elements_are_zero_whatever_they_were():
     assert (dy[~keep] == 0).all() and not torch.isfinite(dy[keep]).any()
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("M,Cw", [(40, 72), (40, 37), (9, 2056)])
+def test_dropped_elements_have_no_part_in_the_gates_gradient(M, Cw, post, dt):
+    """(Its own norm makes a row of one infinite element zero elsewhere, and a row of one NaN nothing but NaN.)"""
+    t = _tensors(M, Cw, dt, PARTS[-1] if post else PARTS[2], seed=12)
+    kw = dict(weight=t["weight"], post_weight=t["post_weight"], gate=t["gate"], p=0.5, seed=_seed())
+    drop, x, y = ~B.kept(t["y"], 0.5, _seed()), t["x"], t["y"]
+    y[1] = y[2] = y[3] = 0 if post else 1
+    clean = y.clone()
+    for r, bad in ((1, math.inf), (2, -math.inf), (3, math.inf if post else math.nan)):
+        y[r, int(drop[r].nonzero()[-1])] = bad
+    got, want = (D.residual_norm_backward(x, y.flip(0).nan_to_num(0, 1, -1), x, v, **kw) for v in (y, clean))
+    assert want[4].isfinite().all() and torch.equal(got[4], want[4])
+    assert torch.equal(got[0], want[0]) and (post or torch.equal(got[1], want[1]))
+
+
 def test_dropout_in_place_and_inside_other_rows():
     x = _gen(2)(50, 37).to(BF)
     want = D.dropout(x, 0.4, _seed())
