@@ -483,8 +483,9 @@ int maba_hip_dropout(const maba_tensor* x, double p, const int64_t* seed, uint32
  * fp32 arithmetic; x_out is rounded once, and h once from the unrounded x_out.  Dropout as in maba_hip_dropout.
  *
  * Backward: dx_out, dh [M,C], either of which may be NULL (zeros); x, y as the forward had them, from which it makes the
- * unrounded x_out again: x is read only with dh, y (NULL where the forward had none) with dh, with post_weight and for
- * dgate, and may be NULL otherwise; any of dx, dy [M,C], dweight, dpost_weight, dgate [C] may be NULL.
+ * unrounded x_out again.  x's elements are read only with dh; without it x tells the shape and type, and its data may be
+ * NULL.  y (NULL where the forward had none) is read with dh, with post_weight and for dgate, and may be NULL otherwise.
+ * Any of dx, dy [M,C], dweight, dpost_weight, dgate [C] may be NULL.
  * Parameters' gradients are summed in fp32 through the workspace (16-byte aligned, of one call at a time; the query
  * depends on the current device's compute-unit count; grads: 1 dweight, 2 dgate, 4 dpost_weight), in a fixed order:
  * results are the same bits on every call.

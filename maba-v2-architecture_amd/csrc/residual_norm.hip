@@ -660,7 +660,7 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
   const char* who = "residual_norm_backward";
   int rc = check_float_rows(x, who);
   if (!rc) rc = check_drop(who, p, seed);
-  if (!rc) rc = check_rows(x, who, "x", x->dtype, -1, -1);
+  if (!rc && (dh || x->data)) rc = check_rows(x, who, "x", x->dtype, -1, -1);
   if (rc) return rc;
   const int64_t R = x->shape[0], C = x->shape[1];
   const int dt = x->dtype;
@@ -681,30 +681,31 @@ extern "C" int maba_hip_residual_norm_backward(const maba_tensor* dx_out, const 
   if (!rc && dy) rc = check_out(dy, who, "dy", dt, R, C);
   if (rc) return rc;
   maba_tensor* outs[] = {dx, dy, dweight, dpost_weight, dgate};
+  const maba_tensor* rx = dh ? x : nullptr;                // x as it is read
   for (int i = 0; i < 5; ++i) {
-    for (const maba_tensor* in : {dx_out, dh, x, y, weight, post_weight, gate})
+    for (const maba_tensor* in : {dx_out, dh, rx, y, weight, post_weight, gate})
       if (overlap(outs[i], in)) return fail(MABA_ERR_INVALID, "%s: an output overlaps an input", who);
     for (int j = 0; j < i; ++j)
       if (overlap(outs[i], outs[j])) return fail(MABA_ERR_INVALID, "%s: outputs overlap", who);
   }
   if (C > MAX_WIDTH) return fail(MABA_ERR_UNSUPPORTED, "%s: at most %d channels", who, MAX_WIDTH);
-  const Geometry geo = row_geometry(C, chunk_elems(dt), back_elems(R, C, dt), far_rows({dx_out, dh, x, y, dx, dy}));
+  const Geometry geo = row_geometry(C, chunk_elems(dt), back_elems(R, C, dt), far_rows({dx_out, dh, rx, y, dx, dy}));
   const int grads = (dweight ? GRAD_W : 0) | (dgate ? GRAD_GATE : 0) | (dpost_weight ? GRAD_POST : 0);
   if (!grads && !dx && !dy) return MABA_OK;
   const int groups = back_groups(R, geo, cut_rows(C, dt)), n = __builtin_popcount(grads);
   rc = ffn::check_workspace(who, workspace, workspace_bytes, (size_t)groups * n * C * sizeof(float));
   if (rc) return rc;
   const bool need_y = y && (dh || post_weight || dgate);
-  BoundaryBackArgs a = {dx_out ? dx_out->data : nullptr, dh ? dh->data : nullptr, x->data, need_y ? y->data : nullptr,
+  BoundaryBackArgs a = {dx_out ? dx_out->data : nullptr, dh ? dh->data : nullptr, rx ? rx->data : nullptr, need_y ? y->data : nullptr,
                         weight ? weight->data : nullptr, post_weight ? post_weight->data : nullptr, gate ? gate->data : nullptr,
                         dx ? dx->data : nullptr, dy ? dy->data : nullptr, (float*)workspace,
-                        row_stride(dx_out), row_stride(dh), row_stride(x), row_stride(y), row_stride(dx), row_stride(dy), R, (int)C,
+                        row_stride(dx_out), row_stride(dh), row_stride(rx), row_stride(y), row_stride(dx), row_stride(dy), R, (int)C,
                         geo.lg, grads, cut_rows(C, dt), scale, eps, make_drop(p, seed, stream_id)};
   if (R > 0) {
     const int threads = back_size(R, geo, cut_rows(C, dt));
     const size_t params = (size_t)(post_weight ? 3 : 2) * ceil_div(C, chunk_elems(dt)) * 16;
     const size_t lds = std::max(params, grads ? (size_t)(post_weight ? 3 : 2) * threads * chunk_elems(dt) * sizeof(float) : 0);
-    const bool whole = whole_rows({dx_out, dh, x, y, dx, dy});
+    const bool whole = whole_rows({dx_out, dh, rx, y, dx, dy});
     with_type(dt, [&](auto type) {
       typedef decltype(type) T;
       auto run = [&](auto kernel) {

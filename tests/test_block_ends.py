@@ -486,6 +486,18 @@ def test_c_boundary_backward_refusals(lib):
         assert text in lib.maba_hip_last_error(), (kw, lib.maba_hip_last_error())
 
 
+def test_c_boundary_backward_takes_x_without_data_where_h_has_no_gradient(lib):
+    """The calls stop at the workspace, behind all checks of tensors."""
+    d, h, x, y, out = (_t([4, 8], data=p) for p in (A, Bt, 0, Ct, Et))
+    w, dg = _t([8], data=6 << 24), _t([8], data=7 << 24)
+    call = lambda dh, x, dx: lib.maba_hip_residual_norm_backward(d, dh, x, y, w, None, w, 1.0, 0.0, None, 0, 1e-6, dx, None, None, None, dg,
+                                                                 None, 0, None)
+    for dh, xx, dx, rc, text in ((None, x, out, 5, b"workspace"), (h, x, out, 1, b"x has no data"),
+                                 (None, _t([4, 8], data=Et), out, 5, b"workspace"), (h, _t([4, 8], data=Et), out, 1, b"overlaps an input"),
+                                 (None, _t([4, 7], data=0), out, 1, b"expected")):
+        assert call(dh, xx, dx) == rc and text in lib.maba_hip_last_error(), lib.maba_hip_last_error()
+
+
 def test_c_workspace_sizes(lib):
     size = lib.maba_hip_residual_norm_backward_workspace_size
     x = _t([1000, 640], data=A)

@@ -235,6 +235,22 @@ def test_boundary_gradients_of_some_inputs(needs, Cw):
     assert all(torch.equal(a, b) for a, b in zip(xo, zero))
 
 
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("M,Cw", [(1, 40), (90, 64), (90, 50), (20, 2056), (300, 640)])
+def test_x_is_not_read_where_h_has_no_gradient(M, Cw, post):
+    t = _tensors(M, Cw, BF, PARTS[-1] if post else ("y", "gate"), seed=15)
+    seed, d = _seed(), t["y"].flip(0).contiguous()
+    want = D.residual_norm_backward(d, None, t["x"], t["y"], post_weight=t["post_weight"], gate=t["gate"], p=0.2, seed=seed)
+    outs = [torch.full_like(v, math.nan) if v is not None else None for v in want]
+    size = N.load().maba_hip_residual_norm_backward_workspace_size(N.rows_desc(d), 7)
+    ws = torch.empty(size, dtype=torch.uint8, device=DEV)
+    none = bytes(8) + N.rows_desc(t["x"])[8:]                                  # the shape and type alone
+    N.check(N.load().maba_hip_residual_norm_backward(N.rows_desc(d), None, none, N.rows_desc(t["y"]), None, N.rows_desc(t["post_weight"]),
+                                                     N.rows_desc(t["gate"]), 1.0, 0.2, seed.data_ptr(), 0, 1e-6, *map(N.rows_desc, outs),
+                                                     ws.data_ptr(), ws.numel(), N.stream_ptr(d.device)), "residual_norm_backward")
+    assert all(torch.equal(a, b) for a, b in zip(outs, want) if b is not None)
+
+
 @pytest.mark.parametrize("which", [(0,), (1,), (2,), (3,), (4,), (0, 2), (1, 4), (2, 3, 4)])
 @pytest.mark.parametrize("post", [False, True])
 def test_boundary_autograd_of_some_inputs(post, which):
