@@ -363,8 +363,15 @@ class MabaSparseForCausalLM(WeightCacheMixin, nn.Module):
         self.lm_head.weight = self.embeddings.in_emb.weight      # tied (model.py:205)
         self._install_weight_cache_hooks()
         if getattr(c, "dropout", 0.0) > 0:
-            # the next training step's masks; not part of the state dict
-            self.register_buffer("dropout_seed", torch.randint(0, 2 ** 62, (1,)), persistent=False)
+            # the next training step's masks; no part of the state dict, and no buffer: a data-parallel wrapper sends rank 0's
+            # buffers to all ranks, which would then drop by one mask
+            self.dropout_seed = torch.randint(0, 2 ** 62, (1,))
+
+    def _apply(self, fn, *args, **kwargs):
+        out = super()._apply(fn, *args, **kwargs)
+        if "dropout_seed" in self.__dict__:
+            self.dropout_seed = fn(self.dropout_seed)
+        return out
 
     def init_normal(self, std: float = 0.02) -> "MabaSparseForCausalLM":
         """Every weight matrix and embedding ~ N(0, std) (the BASELINE's random init); norms,

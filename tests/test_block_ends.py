@@ -1,8 +1,11 @@
 """Dropout, the block boundary and token log probabilities on the CPU: the definitions, gradients against differences,
 refusals of the dispatcher and of the C entry points, and the model's paths over them."""
+import copy
 import ctypes
 import math
 import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -629,6 +632,60 @@ def test_dropout_of_the_model():
     with torch.no_grad():
         seed = m.dropout_seed.clone()
         assert torch.equal(m(ids)[0], m(ids)[0]) and torch.equal(m.dropout_seed, seed)
+
+
+def test_the_models_seed_moves_with_it():
+    m = _model(dropout=0.2)
+    assert "dropout_seed" not in dict(m.named_buffers()) and not any("dropout_seed" in k for k in m.state_dict())
+    c = copy.deepcopy(m)
+    c.dropout_seed += 1
+    assert not torch.equal(c.dropout_seed, m.dropout_seed)
+    assert m.to("meta").dropout_seed.device.type == "meta" and c.bfloat16().dropout_seed.dtype == torch.int64
+    assert "dropout_seed" not in _model().__dict__
+
+
+DATA_PARALLEL = """
+import sys
+import torch
+import torch.distributed as dist
+from maba_sparse.model import MabaSparseForCausalLM, get_101m_config
+
+rank, store = int(sys.argv[1]), sys.argv[2]
+dist.init_process_group("gloo", init_method="file://" + store, rank=rank, world_size=2)
+torch.manual_seed(0)
+m = MabaSparseForCausalLM(get_101m_config(dim=64, n_layers=2, n_heads=1, d_head=64, vocab_size=32, d_emb=16, intermediate_size=48,
+                                          dropout=0.5))
+m.dropout_seed.fill_(100 + rank)
+ddp = torch.nn.parallel.DistributedDataParallel(m, find_unused_parameters=True)
+ids = torch.arange(24).view(2, 12)
+outs = [ddp(ids)[0] for _ in range(2)]
+outs[-1].sum().backward()
+assert m.dropout_seed.tolist() == [102 + rank], m.dropout_seed
+both = [torch.empty_like(outs[0]) for _ in range(2)]
+dist.all_gather(both, outs[0].detach())
+assert not torch.equal(*both)                   # each rank by its own masks
+g = m.final_norm.weight.grad
+grads = [torch.empty_like(g) for _ in range(2)]
+dist.all_gather(grads, g)
+assert torch.equal(*grads) and g.any()          # and one gradient
+dist.destroy_process_group()
+"""
+
+
+def test_ranks_of_a_data_parallel_job_drop_by_their_own_seeds(tmp_path):
+    script = tmp_path / "rank.py"
+    script.write_text(DATA_PARALLEL)
+    package = os.path.dirname(os.path.dirname(os.path.abspath(N.__file__)))
+    env = dict(os.environ, PYTHONPATH=package, GLOO_SOCKET_IFNAME="lo", OMP_NUM_THREADS="2")
+    ranks = [subprocess.Popen([sys.executable, str(script), str(r), str(tmp_path / "store")], env=env, stdout=subprocess.PIPE,
+                              stderr=subprocess.STDOUT, text=True) for r in range(2)]
+    try:
+        for r in ranks:
+            out, _ = r.communicate(timeout=240)
+            assert r.returncode == 0, out
+    finally:
+        for r in ranks:
+            r.kill()
 
 
 def test_generation_with_post_norms_equals_state_passing():

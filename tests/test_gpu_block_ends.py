@@ -687,6 +687,33 @@ def test_captured_decoding_of_extended_blocks_equals_state_passing(kw):
             assert (a - b).norm() / b.norm() < 0.02, (i, (a - b).norm() / b.norm())
 
 
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+def test_a_model_trains_with_dropout_as_on_the_cpu(monkeypatch):
+    """The same masks from the same seed: fp32 against 64 bits, gradients among them (its mixers' come from torch).  Of relative
+    roundings of 6e-8 some thousands lie on a way through the model, and another mask changes it by tenths."""
+    from maba_sparse.model import MabaSparseForCausalLM, get_101m_config
+    monkeypatch.setenv("MABA_STRICT_BACKEND", "0")
+    torch.manual_seed(3)
+    cfg = get_101m_config(dim=128, n_layers=4, n_heads=2, d_head=64, vocab_size=97, d_emb=16, d_c=32, d_idx=16, intermediate_size=96,
+                          top_k=4, post_norm=True, residual_scale=0.7, dropout=0.3)
+    ref = MabaSparseForCausalLM(cfg).init_normal(0.1).double()
+    m = MabaSparseForCausalLM(cfg)
+    m.load_state_dict(ref.state_dict())
+    m.to(DEV)
+    assert m.dropout_seed.device.type == "cuda"
+    m.dropout_seed.copy_(ref.dropout_seed)
+    ids = torch.randint(0, 97, (2, 70), generator=torch.Generator().manual_seed(4))
+    for i in range(2):
+        assert int(m.dropout_seed) == int(ref.dropout_seed)
+        a, b = (-n.score(ids.to(n.dropout_seed.device))[0].mean() for n in (m, ref))
+        assert abs(a.item() - b.item()) < 1e-4 * abs(b.item())
+        a.backward()
+        b.backward()
+        for (name, p), q in zip(m.named_parameters(), ref.parameters()):
+            if q.grad is not None:
+                assert (p.grad.cpu().double() - q.grad).norm() <= 1e-3 * q.grad.norm() + 1e-9, (name, i)
+
+
 # ----------------------------------------------------------------------------- calls
 
 
