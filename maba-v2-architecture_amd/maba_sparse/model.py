@@ -349,8 +349,6 @@ def _decode_linear_fits(model: "MabaSparseForCausalLM") -> bool:
 
 
 class MabaSparseForCausalLM(WeightCacheMixin, nn.Module):
-    _generating = False
-
     def __init__(self, config: Optional[MabaConfig] = None) -> None:
         super().__init__()
         self.config = config or get_101m_config()
@@ -385,15 +383,17 @@ class MabaSparseForCausalLM(WeightCacheMixin, nn.Module):
     def _logits(self, x: torch.Tensor) -> torch.Tensor:
         return self.lm_head(self.head_proj(self.final_norm(x)))
 
-    def forward(self, input_ids: torch.Tensor, past_states: Optional[List[Any]] = None, last_only: bool = False):
+    def forward(self, input_ids: torch.Tensor, past_states: Optional[List[Any]] = None, last_only: bool = False,
+                drop: bool = True):
         """Prefill: ``(logits, past_states)`` with ``(state, conv_state, c_kv)`` per block
         (reference model.py:207-234; the loss and MTP head are left out).  ``last_only`` returns
-        the logits of the last position only, ``[B, 1, vocab]`` (what generation reads)."""
+        the logits of the last position only, ``[B, 1, vocab]`` (what generation reads); without ``drop`` nothing is dropped
+        out, also of a model that is training."""
         x = self.embeddings(input_ids)
         if self._fused_norms_ok(x):
             return self._forward_fused_norms(x, past_states, last_only)
         if self.layers[0].boundary:
-            return self._forward_boundary(x, past_states, last_only)
+            return self._forward_boundary(x, past_states, last_only, drop)
         nps = []
         for i, layer in enumerate(self.layers):
             st, cv, pk = past_states[i] if past_states is not None else (None, None, None)
@@ -442,17 +442,17 @@ class MabaSparseForCausalLM(WeightCacheMixin, nn.Module):
     def next_dropout_seed(self) -> Optional[torch.Tensor]:
         """The seed of this training step's masks, on which ``dropout_seed`` moves on (also where the step is replayed
         from a captured graph); None where nothing is dropped.  Ranks of a data-parallel job start it from different values."""
-        if not self.training or self._generating or getattr(self, "dropout_seed", None) is None:
+        if not self.training or getattr(self, "dropout_seed", None) is None:
             return None
         with torch.no_grad():
             seed = self.dropout_seed.clone()
             self.dropout_seed += 1
         return seed
 
-    def _forward_boundary(self, x: torch.Tensor, past_states, last_only: bool = False):
+    def _forward_boundary(self, x: torch.Tensor, past_states, last_only: bool = False, drop: bool = True):
         """``forward`` with every boundary, the final norm's among them, as one ``residual_norm``: the end of each half of
         a block together with the norm that comes next."""
-        seed = self.next_dropout_seed()
+        seed = self.next_dropout_seed() if drop else None
         if seed is not None:
             x = dropout(x, self.config.dropout, seed)
         layers = self.layers
@@ -540,11 +540,7 @@ class MabaSparseForCausalLM(WeightCacheMixin, nn.Module):
         B, L = input_ids.shape
         if graph is None:
             graph = self.serving_graph_ok(input_ids)
-        self._generating = True
-        try:
-            logits, states = self(input_ids, last_only=True)
-        finally:
-            self._generating = False
+        logits, states = self(input_ids, last_only=True, drop=False)
         if graph:
             return self._generate_graph(logits, states, L, max_new_tokens, on_prefill_done, return_logits,
                                         on_graph_ready)

@@ -6,6 +6,7 @@ import math
 import os
 import subprocess
 import sys
+import threading
 
 import pytest
 import torch
@@ -718,6 +719,22 @@ def test_generation_drops_nothing():
     assert torch.equal(got, want) and torch.equal(m.dropout_seed, seed)
     m.train()
     assert not torch.equal(m(ids)[0], m(ids)[0])
+
+
+def test_generation_leaves_a_training_step_in_another_thread_its_dropout():
+    m, ids = _model(dropout=0.5), _ids(80)
+    seeds = []
+
+    def meanwhile(*_):
+        t = threading.Thread(target=lambda: seeds.append(m.next_dropout_seed()))
+        t.start()
+        t.join()
+
+    start = m.dropout_seed.clone()
+    hook = m.embeddings.register_forward_hook(meanwhile)             # within the prompt's pass
+    m.generate_greedy(ids, 1)
+    hook.remove()
+    assert len(seeds) == 1 and torch.equal(seeds[0], start)
 
 
 def test_blocks_of_configs_and_modules_from_before_the_fields():
