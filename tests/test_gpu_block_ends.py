@@ -320,6 +320,32 @@ def test_offsets_past_32_bits():
     assert all(torch.equal(a[0], b) for a, b in zip(got, flat))
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("M,Cw", [(1, 64), (129, 640), (2049, 640), (4097, 128), (16385, 640), (16400, 640), (65537, 96), (8193, 24), (5001, 33),
+                                  (1025, 2048), (4099, 1001), (3001, 2049), (513, 4096), (2051, 4095), (770, 8192)])
+def test_parameters_sums_have_every_row_once(M, Cw, post, dt):
+    """Whole numbers all the way: normalised rows of +-1, gradients without a part along them.  What a row adds to a sum is 1 at
+    least or nothing, so that a row lost or taken twice shows against the sums' own magnitude times some 2^-24."""
+    r = _gen(M + Cw)
+    sign = lambda: torch.where(r(M, Cw) > 0, 1.0, -1.0)
+    ints = lambda k: (r(M, Cw) * 1.5).round().clamp(-k, k)
+    keep = B.kept(torch.empty(M, Cw, device=DEV), 0.5, _seed(), 4)
+    y, xo, dxo, e = sign(), sign(), ints(3), ints(2)
+    e = torch.cat([e[:, :Cw // 2], -e[:, :Cw // 2], torch.zeros(M, Cw % 2, device=DEV)], 1)      # rows of sum zero
+    z = torch.where(keep, 2 * y, 0.0)
+    x, dh, one = xo - z, e * xo, torch.ones(Cw, device=DEV)
+    got = D.residual_norm_backward(dxo.to(dt), dh.to(dt), x.to(dt), y.to(dt), one.to(dt), one.to(dt) if post else None, one.to(dt), p=0.5,
+                                   seed=_seed(), stream=4, eps=0.0)
+    dx = (dxo + dh).double()
+    for name, v, t in (("dx", got[0], None), ("dweight", got[2], dh * xo), ("dgate", got[4], dx * z), ("dpost_weight", got[3], dx * z)):
+        if t is not None and v is not None:
+            t = t.double()
+            B.check(v, (t.sum(0), 16 * B.U * t.abs().sum(0) + B.half_step(dt) * t.sum(0).abs()), name)
+        elif v is not None:
+            B.check(v, (dx, 16 * B.U * (dx.abs() + 1)), name)
+
+
 @pytest.mark.parametrize("stride", [2 ** 27 + 8, 400_000_000, 2 ** 28, 2 ** 30, 2 ** 31])
 @pytest.mark.parametrize("dt", [BF, FL])
 @pytest.mark.parametrize("Cw", [16, 64, 120, 33, 640])
