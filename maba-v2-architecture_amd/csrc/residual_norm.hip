@@ -154,12 +154,13 @@ struct BoundaryBackArgs {
 
 // A row's sums are exchanged twice: those of dh w x' and x'^2 (the mean of dh w x^ is r times that of dh w x'), and with POST that
 // for dy together with the next row's of y^2.  The chunks stay packed in registers between their uses, the mask as bits.  HBM, and
-// arithmetic that its waits do not hide: 16,384 x 640 bf16 with dropout 36 us, 3.5 TB/s (every second lane has one chunk of two),
-// 8,192 x 4,096 86 us, 4.7 TB/s, and with both norms 101, 4.0 TB/s, the vector units 67 % busy; 8,191 x 4,095 132 us, 3.1 TB/s.
+// arithmetic that its waits do not hide: 16,384 x 640 bf16 with dropout 36 us with the sums over the partials, 3.5 TB/s (three
+// lanes of four have one chunk of two), 8,192 x 4,096 85 us, 4.7 TB/s, and with both norms 98, 4.1 TB/s, the vector units 65 %
+// busy; 8,191 x 4,095 106 us, 3.8 TB/s, and 123.
 // WHOLE: rows of whole 16-byte chunks (WholeWalk).  The next rows' chunks are loaded ahead of the present ones' arithmetic.
-// One workgroup a compute unit, as large as registers allow: of four waves a SIMD with one chunk a lane, of two beyond.  So
-// the fewest partials are written: 8,192 x 4,096 bf16 87 us, as two workgroups of half the threads 91; 2,048 x 640 13.1, of 512
-// threads 14.3 and of 256 16.2; fp32 8,192 x 2,048 83, of 256 89.
+// back_size() says how many threads a workgroup has.  Registers: of fp32 rows of more than 6,144 a lane has four chunks, which
+// with POST or without WHOLE spill 52 to 212 bytes a lane (4,096 x 8,192 169 us, 4.8 TB/s, and with both norms 239; x 6,144, whose
+// three chunks fit, 127 and 133), and 16-bit rows of one chunk with POST and without WHOLE 16.
 constexpr int back_threads(int nch) { return nch == 1 ? 1024 : 512; }
 template <class T, int NCH, bool POST, bool WHOLE>
 __global__ __launch_bounds__(back_threads(NCH)) void boundary_back_kernel(BoundaryBackArgs a) {
@@ -459,7 +460,8 @@ struct DropArgs {
   Drop d;
 };
 // 2^lg lanes a row, four chunks a lane in flight.  Bound by the generator's 32-bit multiplications and HBM about alike: 32,768 x
-// 1,024 bf16 26.6 us, 5.0 TB/s; 16,384 x 640 12.1 us.
+// 1,024 bf16 26.6 us, 5.0 TB/s; 16,384 x 640 12.1 us.  A row is one workgroup's at most: few long ones leave the chip idle (16.8M
+// elements as 16,384 rows 17 us, as 256 24, as 16 264, as one 4.0 ms).
 template <class T>
 __global__ __launch_bounds__(256) void dropout_kernel(DropArgs a) {
   constexpr int V = Traits<T>::VEC, N = 4;
@@ -527,10 +529,12 @@ static bool whole_rows(std::initializer_list<const maba_tensor*> all) {
 // Elements of a row a lane has.  Few give every row more lanes and the chip more waves; more leave fewer lanes without work
 // (80 chunks of 640 16-bit elements fill 62 % of 128 lanes and 83 % of 32 with three each) and share out what a row costs
 // besides its elements.  Forward, in us, 8 / 24 elements: 1 x 640 bf16 3.1 / 4.1, 2,048 x 640 5.5 / 5.8, 32,768 x 640
-// 42.8 / 32.8, 8,192 x 4,096 50.5 / 47.3; fp32 8,192 x 1,000 22.9 / 24.6.  Backward, 8 / 16: 64 x 640 8.6 / 10.4, 16,384 x 640
-// 38.1 / 37.7, 65,536 x 640 118 / 110 and with post_weight 150 / 131, 24,576 x 767 75 / 72 and with post_weight 101 / 79; where all
-// lanes of 8 have work 24,576 x 512 34 / 37, and rows of more than a wave either way 24,576 x 1,345 128 / 149, 8,192 x 4,096 87 / 87
-// and 2,048 x 4,096 29 / 32.
+// 42.8 / 32.8, 8,192 x 4,096 50.5 / 47.3; fp32 8,192 x 1,000 22.9 / 24.6.
+// Backward: two chunks a lane make one wave's of a row that would be two waves', so that its sums need no LDS and no barrier.
+// That pays for many rows, and where all 128 lanes would have had work it costs more than it saves.  In us, 8 / 16 elements:
+// 64 x 640 8.3 / 10.5, 2,048 x 640 12.3 / 13.0, 16,384 x 640 37.7 / 36.4, 65,536 x 640 113 / 107 and with post_weight 152 / 129,
+// 24,576 x 767 69 / 71 and with post_weight 85 / 78, x 1,001 72 / 74; rows of one wave 24,576 x 512 37 / 40, and of more than a wave either
+// way 24,576 x 1,345 117 / 148, 8,192 x 4,096 85 / 86, 2,048 x 4,096 33 / 35.
 constexpr int MOST_ELEMS = 24, MOST_BACK = 16;
 static int forward_elems(int64_t R, int64_t C, int dtype) { return C > 8 << MAX_LG ? 16 : dtype != MABA_F32 && R > 4096 ? MOST_ELEMS : 8; }
 static int back_elems(int64_t R, int64_t C, int dtype) {
@@ -540,9 +544,12 @@ static int back_elems(int64_t R, int64_t C, int dtype) {
   while (lanes < chunks) lanes *= 2;
   return dtype != MABA_F32 && R >= 16384 && lanes == 128 && chunks * 4 <= lanes * 3 ? MOST_BACK : 8;
 }
-// A backward pass's threads a workgroup: the fewest until rows fill the chip (64 x 640 bf16 8.4 us, with 1,024 threads 10.6), then
-// as many as fill a compute unit by themselves; half of them where rows end inside a chunk, whose accesses keep the waves
-// apart, and a row does not need them all (24,576 x 1,345 bf16 117 us and 128, 24,576 x 1,001 71 and 76; 8,191 x 4,095 113 and 106).
+// A backward pass's threads a workgroup, and so how many workgroups a compute unit has: together four waves a SIMD with one
+// chunk a lane, two beyond, as registers allow.  Many rows: one workgroup, since the fewest partials are then written (in us, one /
+// as many as there are of 256 threads or a row's: 2,048 x 640 bf16 12.3 / 14.4, 8,192 x 4,096 85 / 91, 8,191 x 4,095 106 / 115,
+// fp32 8,192 x 2,048 83 / 86.5).  Two where rows end inside a chunk, whose accesses keep the waves apart, and a row does not need all
+// threads (one / two: 24,576 x 1,345 128 / 117, x 1,001 78 / 72).  Until rows fill the chip the smallest (64 x 640 8.4, of 1,024
+// threads 10.6).
 static int back_size(int64_t R, const Geometry& geo, bool cut) {
   const int most = cut && geo.lg < MAX_LG ? std::min(back_threads(geo.nch), 512) : back_threads(geo.nch);
   return R >= (int64_t)device_cu_count() * (most >> geo.lg) ? most : std::max(256, 1 << geo.lg);

@@ -180,10 +180,12 @@ __device__ __forceinline__ float across(float v, float* shared, F f) {
 }
 
 // W waves a row (row_waves says how many).  With one, a workgroup has four rows; otherwise it is one row's.
-// Without alternatives 8,192 x 32,768 bf16 take 98 us, 5.5 TB/s: HBM; 777 x 50,257 fp32, whose rows start at any 4 bytes, 34 us,
-// 4.7 TB/s.  With them the threads that hold one read elements again, and the other waves of the row wait: 4,096 x 32,768 bf16 51 us
-// without, 60 with 5 and 65 with 20 (4.5 and 4.2 TB/s; 65 and 71 where a thread read all of its elements again, a line of 128
-// bytes for 16).  16 x 32,768 take 5.3 and with 20 alternatives 9.4 us, the latency of one row; 17 where all but five logits are -inf.
+// By itself and without alternatives 8,192 x 32,768 bf16 take 98 us, 5.5 TB/s: HBM; 777 x 50,257 fp32, whose rows start at any 4
+// bytes, 34 us, 4.7 TB/s, and with eight alternatives 37.  (Behind a kernel that has just written as much, as a training step's
+// gradient, the cache in front of HBM writes back meanwhile: 130 and, with the alternatives, 53.)  With them the threads that hold one
+// read elements again, and the other waves of the row wait: 4,096 x 32,768 bf16 51 us without, 60 with 5 and 65 with 20 (4.5 and
+// 4.2 TB/s; 65 and 71 where a thread read all of its elements again, a line of 128 bytes for 16).  16 x 32,768 take 5.3 and with 20
+// alternatives 9.4 us, the latency of one row; 17 where all but five logits are -inf.
 // CAP: room for what is above the bound.  Two lists of 1,024 a row of two waves held the compute unit to ten rows: 4,096 x
 // 16,000 with five alternatives 46 us, with 512 43.
 template <class T, int W, bool TOP>
@@ -387,7 +389,8 @@ __global__ __launch_bounds__(256) void logprobs_back_kernel(BackwardArgs a) {
   float gl = target < 0 || !a.dlogp ? 0.f : target >= a.V ? NAN : a.dlogp[r], gz = a.dlse ? a.dlse[r] : 0.f;
   // log p = l / T - lse is as exact as lse, whose rounding far from zero is more than those of p and of the result: there the
   // row is summed again and log p counted from its largest element.  All of that ends before anything of the row is
-  // written, which may be the logits' own.  (1,024 x 32,768 bf16 24 us without such rows, 63 with nothing else.)
+  // written, which may be the logits' own.  Each of a row's workgroups does so for itself.  (1,024 x 32,768 bf16, two of them, 23 us
+  // without such rows and 61 with nothing else; 777 x 50,257 fp32, seven, 53 and 359.)
   constexpr float EXACT = T::CODE == MABA_F32 ? 32.f : 256.f;
   __shared__ float part[3][4];
   const int l = threadIdx.x & ((1 << a.lg) - 1);
