@@ -454,6 +454,7 @@ class MabaSparseForCausalLM(WeightCacheMixin, nn.Module):
         a block together with the norm that comes next."""
         seed = self.next_dropout_seed() if drop else None
         if seed is not None:
+            seed = seed.to(x.device)           # of a replica that shares it with a model on another device
             x = dropout(x, self.config.dropout, seed)
         layers = self.layers
         x, h = residual_norm(x, weight=layers[0].norm1.weight, eps=layers[0].norm1.eps)

@@ -740,6 +740,21 @@ def test_a_model_trains_with_dropout_as_on_the_cpu(monkeypatch):
                 assert (p.grad.cpu().double() - q.grad).norm() <= 1e-3 * q.grad.norm() + 1e-9, (name, i)
 
 
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+def test_a_seed_on_another_device_than_the_model(monkeypatch):
+    """As a replica has it whose model keeps its seed elsewhere."""
+    from maba_sparse.model import MabaSparseForCausalLM, get_101m_config
+    monkeypatch.setenv("MABA_STRICT_BACKEND", "0")
+    torch.manual_seed(5)
+    m = MabaSparseForCausalLM(get_101m_config(dim=64, n_layers=1, n_heads=1, d_head=64, vocab_size=32, d_emb=16, intermediate_size=48,
+                                              dropout=0.5)).to(DEV)
+    ids = torch.randint(0, 32, (2, 20), device=DEV)
+    seed = m.dropout_seed.clone()
+    want = m(ids)[0]
+    m.dropout_seed = seed.cpu()
+    assert torch.equal(m(ids)[0], want) and int(m.dropout_seed) == int(seed) + 1
+
+
 # ----------------------------------------------------------------------------- calls
 
 
