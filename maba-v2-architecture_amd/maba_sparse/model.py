@@ -15,7 +15,7 @@ probabilities that a loss is made from; the feed-forward half of a block trains 
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Any, List, Optional, Tuple
+from typing import Any, List, Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
@@ -384,11 +384,12 @@ class MabaSparseForCausalLM(WeightCacheMixin, nn.Module):
         return self.lm_head(self.head_proj(self.final_norm(x)))
 
     def forward(self, input_ids: torch.Tensor, past_states: Optional[List[Any]] = None, last_only: bool = False,
-                drop: bool = True):
+                drop: Union[bool, torch.Tensor] = True):
         """Prefill: ``(logits, past_states)`` with ``(state, conv_state, c_kv)`` per block
         (reference model.py:207-234; the loss and MTP head are left out).  ``last_only`` returns
-        the logits of the last position only, ``[B, 1, vocab]`` (what generation reads); without ``drop`` nothing is dropped
-        out, also of a model that is training."""
+        the logits of the last position only, ``[B, 1, vocab]`` (what generation reads); with ``drop=False`` nothing is dropped
+        out, also of a model that is training, and with a seed as ``drop`` that one's masks are taken: a pass that is run
+        again, as activation checkpointing does, takes other masks unless it is given ``next_dropout_seed()`` from outside."""
         x = self.embeddings(input_ids)
         if self._fused_norms_ok(x):
             return self._forward_fused_norms(x, past_states, last_only)
@@ -449,10 +450,14 @@ class MabaSparseForCausalLM(WeightCacheMixin, nn.Module):
             self.dropout_seed += 1
         return seed
 
-    def _forward_boundary(self, x: torch.Tensor, past_states, last_only: bool = False, drop: bool = True):
+    def _forward_boundary(self, x: torch.Tensor, past_states, last_only: bool = False,
+                          drop: Union[bool, torch.Tensor] = True):
         """``forward`` with every boundary, the final norm's among them, as one ``residual_norm``: the end of each half of
         a block together with the norm that comes next."""
-        seed = self.next_dropout_seed() if drop else None
+        if isinstance(drop, torch.Tensor):
+            seed = drop if self.training and self.config.dropout > 0 else None
+        else:
+            seed = self.next_dropout_seed() if drop else None
         if seed is not None:
             seed = seed.to(x.device)           # of a replica that shares it with a model on another device
             x = dropout(x, self.config.dropout, seed)

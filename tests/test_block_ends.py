@@ -645,6 +645,21 @@ def test_the_models_seed_moves_with_it():
     assert "dropout_seed" not in _model().__dict__
 
 
+def test_a_pass_that_is_run_again_takes_the_seed_it_is_given():
+    from torch.utils.checkpoint import checkpoint
+    m, ids = _model(dropout=0.4).double(), _ids(40)
+    p, grads = m.final_norm.weight, []
+    seed = m.next_dropout_seed()
+    for run in (lambda: m(ids, drop=seed)[0], lambda: checkpoint(lambda i: m(i, drop=seed)[0], ids, use_reentrant=False)):
+        before = m.dropout_seed.clone()
+        grads.append(torch.autograd.grad((run() ** 2).sum(), [p, m.layers[0].res_gate1]))
+        assert torch.equal(m.dropout_seed, before)
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    m.eval()
+    with torch.no_grad():
+        assert torch.equal(m(ids, drop=seed)[0], m(ids)[0])
+
+
 DATA_PARALLEL = """
 import sys
 import torch
